@@ -13,6 +13,9 @@ package is its host-side mirror of the reference interface:
                      KV-split flash decoding (no reference counterpart)
   DecodeBatcher      continuous batching of decode steps, the batched form
                      of crates/api/src/main.rs:266-354's one-request loop
+  page_plan / paged_append / tree_attention / paged_commit, PagedBatcher
+                     the paged KV cache and the attention of drafted tokens
+                     over it (no reference counterpart)
   read_tensor_f32 / WeightTensor.matmul_f64
                      gguf_compiler.rs:351-470 and :1239-1255 on the device
 """
@@ -21,4 +24,6 @@ from .attention import (SeqBatch, Workspace, decode_batched, decode_partial,  # 
                         merge_lse, merge_lse_packed, prefill, softmax_f32)
 from .kv_cache import HashConsedKV  # noqa: F401
 from .batching import AtCapacity, DecodeBatcher, MAX_PENDING_REQUESTS  # noqa: F401
+from .paged import (OutOfPages, PagedBatcher, PagePlan, page_plan, paged_append, paged_commit,  # noqa: F401
+                    tree_attention, tree_workspace_size)
 from .weights import WeightTensor, matmul_f64, read_tensor_f32  # noqa: F401

@@ -99,6 +99,15 @@ SIGNATURES = {
     "bml_attn_merge_lse_packed": (_st, [_vp, _u32, _u32, _u32, _vp, _vp]),
     "bml_attn_prefill": (_st, [_vp, _vp, _vp, _u32, _u32, _u32, _u32, _u32, C.c_int, C.c_float,
                                C.c_int, _vp, C.c_int, _vp]),
+    "bml_paged_plan": (_st, [_vp, _vp, _vp, _u32, _vp, _u32, _vp, _u32, _u32, _vp, _vp, _u32, _u32, _vp, _vp, _vp,
+                             _vp, _vp, _vp, _vp, _vp, _vp]),
+    "bml_paged_append": (_st, [_vp, _vp, _vp, C.c_int, _vp, _vp, _u32, _u32, _u32, _u32, C.c_double, _vp, _vp, _vp,
+                               C.c_int, C.c_uint64, _vp]),
+    "bml_attn_tree_workspace_size": (_st, [_u32, _i32, C.POINTER(_sz)]),
+    "bml_attn_tree": (_st, [_vp, C.c_int, _u32, _u32, _u32, _u32, _vp, _vp, C.c_int, _u32, _u32, _vp, _u32, _vp, _vp,
+                            _u32, _vp, _u32, C.c_float, _vp, _vp, _sz, _vp]),
+    "bml_paged_commit": (_st, [_vp, _vp, _u32, _u32, _u32, _u32, _u32, C.c_int, _vp, _u32, _vp, _vp, _vp, _u32, _vp,
+                               _u32, _vp, _vp, _vp]),
     "bml_softmax_f32": (_st, [_vp, _u32, _u32, _vp, _vp]),
     # include/bml_weights.h
     "bml_read_tensor_f32": (_st, [_vp, C.c_uint64, _i32, C.c_uint64, _vp, C.POINTER(C.c_uint64), _vp]),

@@ -1,0 +1,508 @@
+// tree.cu -- attention of drafted tokens over a paged cache, 32-bit form,
+// and the merge of divided units.
+//
+//   o[t,h] = sum_p softmax_p(scale * q[t,h] . k[p]) v[p]
+//
+// over the positions p < P = kv_len - T and the drafted nodes p = P + j that
+// node t's mask names (its ancestors and itself): the attention block of
+// forward_layer_cached (crates/compiler/src/gguf_compiler.rs:1008-1050 in
+// SugarFreeDoNoSo/bml) for every node of a draft at once.  A row that sees
+// nothing is zero.
+//
+// tree_f32_kernel serves 32-bit queries (and 32-bit pages): results to about
+// f32 precision from TF32 matrix instructions.  Every f32 operand is split
+// x = hi + lo, hi = tf32(x), lo = tf32(x - hi) (22 bits together), and
+// products are hi*hi + lo*hi + hi*lo; f16 and bf16 values are tf32 values
+// already, so 16-bit pages need no lo.  A warp keeps 16 rows' output in
+// registers, its positions' K and V arrive by cp.async in a private ring.
+#include <math.h>
+
+#include "tree.cuh"
+
+namespace bml {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
+
+__device__ __forceinline__ uint32_t tf32_hi(float x) {
+    uint32_t r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ void tf32_split(float x, uint32_t &hi, uint32_t &lo) {
+    hi = tf32_hi(x);
+    lo = tf32_hi(x - __uint_as_float(hi));
+}
+__device__ __forceinline__ void mma_tf32(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 16 bytes global -> shared; bytes = 0 writes zeros and reads nothing.
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ float load_q(const void *q, int type, size_t i) {
+    if (type == BML_F32) return static_cast<const float *>(q)[i];
+    if (type == BML_F16) return __half2float(static_cast<const __half *>(q)[i]);
+    return __bfloat162float(static_cast<const __nv_bfloat16 *>(q)[i]);
+}
+__device__ __forceinline__ void store_out(void *out, int type, size_t i, float x) {
+    if (type == BML_F32) static_cast<float *>(out)[i] = x;
+    else if (type == BML_F16) static_cast<__half *>(out)[i] = __float2half_rn(x);
+    else static_cast<__nv_bfloat16 *>(out)[i] = __float2bfloat16_rn(x);
+}
+
+// RW warps cover RW * 16 rows; the 8 / RW groups of RW warps take turns at
+// stages of SP = 8 * RW positions.
+template <int D, typename KT, int RW>
+struct FCfg {
+    static constexpr int ES = sizeof(KT);
+    static constexpr int GROUPS = kWarps / RW;
+    static constexpr int SP = 8 * RW;
+    static constexpr int STEPS = kTreeTile / (GROUPS * SP);  // stages of a group per tile
+    // Row strides in bytes.  K: lane (g, c) reads 16-byte pieces at row g,
+    // 16-byte column 2c (f32) or c (16-bit); V: at rows 2c, 2c+1, column g.
+    // With these paddings the 8 lanes of a quarter-warp meet 8 bank groups.
+    static constexpr int KS = D * ES + (ES == 4 ? 16 : 64);
+    static constexpr int VS = D * ES + 16;
+    static constexpr int STAGE = SP * (KS + VS);
+    static constexpr int Q_BYTES = RW * 16 * D * 8;  // hi and lo fragments
+    static constexpr int NST = 3 * GROUPS * STAGE + Q_BYTES <= 224 * 1024 ? 3 : 2;
+    static constexpr int RING = GROUPS * NST * STAGE;
+    static constexpr int OUT_BYTES = kWarps * 16 * (D + 4) * 4;  // combine area, over the ring
+    static constexpr int MAIN = RING > OUT_BYTES ? RING : OUT_BYTES;
+    static constexpr int FLAGS = GROUPS * NST * RW;  // one word per 8 positions of a stage
+    static constexpr int SMEM = Q_BYTES + MAIN + FLAGS * 4;
+};
+
+template <int RW>
+__device__ __forceinline__ void group_sync(int group) {
+    if (RW == 1) __syncwarp();
+    else named_bar_sync(1 + group, RW * 32);
+}
+
+template <int D, typename KT, int RW>
+__global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_constant__ TreeParams p) {
+    using C = FCfg<D, KT, RW>;
+    constexpr bool kF32 = C::ES == 4;
+    constexpr int NT = D / 8;          // output column tiles of a warp
+    constexpr int VE = 16 / C::ES;     // V elements of one 16-byte piece
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint32_t *sQ = reinterpret_cast<uint32_t *>(smem);
+    uint8_t *ring = smem + C::Q_BYTES;
+    uint32_t *flags = reinterpret_cast<uint32_t *>(ring + C::MAIN);
+    __shared__ TreeShared sh;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+    const int rw = warp % RW, grp = warp / RW, tig = rw * 32 + lane;  // thread in its group
+    uint8_t *my_ring = ring + grp * C::NST * C::STAGE;
+    uint32_t *my_flags = flags + grp * C::NST * RW;
+    const size_t prow = (size_t)p.n_kv * D;  // elements of a pool row
+    const uint32_t pmask = (1u << p.page_shift) - 1;
+
+    const TreeRange range = tree_range(p, &sh, blockIdx.x, gridDim.x);
+    TreeWalk walk(p, range);
+    TreeSeg sg;
+    while (walk.next(p, sg)) {
+        // Q fragments, split: [row warp][k-step][hi | lo][lane][4]
+        for (int i = threadIdx.x; i < RW * (D / 8) * 32; i += kThreads) {
+            const int l = i & 31, ks = (i >> 5) % (D / 8), w = i / (32 * (D / 8));
+            const int dim = (ks >> 2) * 32 + (l & 3) * 8 + (ks & 3) * 2;
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int h8 = 0; h8 < 2; ++h8) {
+                const uint32_t r = w * 16 + (l >> 2) + h8 * 8;
+                float x0 = 0.f, x1 = 0.f;
+                if (r < sg.rows) {
+                    const size_t at = tree_row(p, sg, sg.row0 + r, D) + dim;
+                    x0 = load_q(p.q, p.q_type, at);
+                    x1 = load_q(p.q, p.q_type, at + 1);
+                }
+                tf32_split(x0, hi[h8], lo[h8]);
+                tf32_split(x1, hi[h8 + 2], lo[h8 + 2]);
+            }
+            uint4 *dst = reinterpret_cast<uint4 *>(sQ) + ((size_t)(w * (D / 8) + ks) * 2) * 32 + l;
+            dst[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            dst[32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        __syncthreads();
+
+        const uint32_t P = sg.s.L - min(sg.s.T, sg.s.L);  // committed positions
+        const uint32_t pos0 = sg.t0 * kTreeTile;
+        const uint32_t n_steps = (sg.t1 - sg.t0) * C::STEPS;
+        const int32_t *table = p.table + (size_t)sg.seq * p.max_pages;
+        auto step_pos = [&](uint32_t k) { return pos0 + (k * C::GROUPS + grp) * C::SP; };
+        // the group's copies of step k into stage k % NST
+        auto fetch = [&](uint32_t k) {
+            if (k < n_steps) {
+                const uint32_t base = step_pos(k), st = k % C::NST;
+                uint8_t *dk = my_ring + st * C::STAGE, *dv = dk + C::SP * C::KS;
+                constexpr int PER = D * C::ES / 16;  // pieces of a row
+#pragma unroll
+                for (int i = 0; i < C::SP * PER / (RW * 32); ++i) {
+                    const int piece = i * RW * 32 + tig, r = piece / PER, x = piece % PER;
+                    const uint32_t pos = base + r;
+                    uint32_t page = 0xffffffffu;
+                    if (pos < sg.s.L) page = (uint32_t)table[pos >> p.page_shift];
+                    const bool ok = page < p.n_pages;
+                    const size_t at = ok ? ((((size_t)page << p.page_shift) + (pos & pmask)) * prow + (size_t)sg.head * D) * C::ES + x * 16 : 0;
+                    cp16(smem_u32(dk + r * C::KS + x * 16), static_cast<const char *>(p.k) + at, ok ? 16 : 0);
+                    cp16(smem_u32(dv + r * C::VS + x * 16), static_cast<const char *>(p.v) + at, ok ? 16 : 0);
+                    if (x == 0 && (r & 7) == 0) my_flags[st * RW + (r >> 3)] = ok;  // 8 positions share a page
+                }
+            }
+            cp_commit();
+        };
+
+        float o[NT][4];
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // rows g and g + 8; l: this lane's share
+        const uint32_t r0 = sg.row0 + rw * 16 + g, r1 = r0 + 8;
+        const uint32_t t0 = r0 / p.group, t1 = r1 / p.group;
+        const bool v0 = r0 < sg.row0 + sg.rows, v1 = r1 < sg.row0 + sg.rows;
+        const uint4 *qf = reinterpret_cast<const uint4 *>(sQ) + (size_t)(rw * (D / 8) * 2) * 32 + lane;
+
+#pragma unroll
+        for (int i = 0; i < C::NST - 1; ++i) fetch(i);
+        for (uint32_t k = 0; k < n_steps; ++k) {
+            cp_wait<C::NST - 2>();
+            group_sync<RW>(grp);
+            fetch(k + C::NST - 1);  // into the stage that step k - 1 has left (the barrier above)
+            const uint32_t st = k % C::NST;
+            const uint8_t *sk = my_ring + st * C::STAGE, *sv = sk + C::SP * C::KS;
+            const bool row_live = sg.rows > (uint32_t)rw * 16;
+            if (!row_live) continue;
+#pragma unroll 1
+            for (int nt = 0; nt < RW; ++nt) {
+                const uint32_t base = step_pos(k) + nt * 8;
+                if (base >= sg.s.L || !my_flags[st * RW + nt]) continue;  // nothing to see here
+                // S = Q K^T for 8 positions, in three sums of their own
+                float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
+                const uint8_t *krow = sk + (nt * 8 + g) * C::KS;
+#pragma unroll
+                for (int s = 0; s < D / 32; ++s) {
+                    float x[8];
+                    if (kF32) {
+                        Elem<float>::widen(lds128(krow + s * 128 + c * 32), x);
+                        Elem<float>::widen(lds128(krow + s * 128 + c * 32 + 16), x + 4);
+                    } else {
+                        Elem<KT>::widen(lds128(krow + s * 64 + c * 16), x);
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk) {
+                        const uint4 qh = qf[((s * 4 + kk) * 2) * 32], ql = qf[((s * 4 + kk) * 2 + 1) * 32];
+                        uint32_t b0, b1, e0 = 0, e1 = 0;
+                        if (kF32) {
+                            tf32_split(x[2 * kk], b0, e0);
+                            tf32_split(x[2 * kk + 1], b1, e1);
+                        } else {
+                            b0 = __float_as_uint(x[2 * kk]);
+                            b1 = __float_as_uint(x[2 * kk + 1]);
+                        }
+                        mma_tf32(s0, &qh.x, b0, b1);
+                        mma_tf32(s1, &ql.x, b0, b1);
+                        if (kF32) mma_tf32(s2, &qh.x, e0, e1);
+                    }
+                }
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = (s0[e] + (s1[e] + s2[e])) * p.scale_log2;
+                const bool edge = base + 8 > P;
+                if (edge) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t pos = base + 2 * c + e;
+                        if (pos >= P) {
+                            if (!(v0 && tree_sees(p, sg.s, t0, pos - P))) x[e] = -INFINITY;
+                            if (!(v1 && tree_sees(p, sg.s, t1, pos - P))) x[2 + e] = -INFINITY;
+                        }
+                    }
+                }
+                float a = fmaxf(x[0], x[1]), b = fmaxf(x[2], x[3]);
+                a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
+                b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, 1));
+                a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
+                b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, 2));
+                if (__any_sync(0xffffffffu, a > m0 || b > m1)) {
+                    const float n0 = fmaxf(m0, a), n1 = fmaxf(m1, b);
+                    const float f0 = n0 == -INFINITY ? 1.f : exp2f(m0 - n0), f1 = n1 == -INFINITY ? 1.f : exp2f(m1 - n1);
+                    m0 = n0;
+                    m1 = n1;
+                    l0 *= f0;
+                    l1 *= f1;
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        o[j][0] *= f0;
+                        o[j][1] *= f0;
+                        o[j][2] *= f1;
+                        o[j][3] *= f1;
+                    }
+                }
+                const float u0 = m0 == -INFINITY ? 0.f : m0, u1 = m1 == -INFINITY ? 0.f : m1;
+                x[0] = exp2f(x[0] - u0);
+                x[1] = exp2f(x[1] - u0);
+                x[2] = exp2f(x[2] - u1);
+                x[3] = exp2f(x[3] - u1);
+                l0 += x[0] + x[1];
+                l1 += x[2] + x[3];
+                // P as the A operand: k index c is position 2c, c + 4 is 2c + 1
+                uint32_t ph[4], pl[4];
+                tf32_split(x[0], ph[0], pl[0]);
+                tf32_split(x[2], ph[1], pl[1]);
+                tf32_split(x[1], ph[2], pl[2]);
+                tf32_split(x[3], ph[3], pl[3]);
+                const uint8_t *va = sv + (nt * 8 + 2 * c) * C::VS + g * 16, *vb = va + C::VS;
+                bool odd = false;  // a V value that is not finite: 0 * it must not reach rows that do not see it
+#pragma unroll
+                for (int s = 0; s < NT / VE; ++s) {
+                    float y0[VE], y1[VE];
+                    Elem<KT>::widen(lds128(va + s * 128), y0);
+                    Elem<KT>::widen(lds128(vb + s * 128), y1);
+                    if (edge) {
+#pragma unroll
+                        for (int e = 0; e < VE; ++e) {
+                            if (!(fabsf(y0[e]) < INFINITY)) { y0[e] = 0.f; odd = true; }
+                            if (!(fabsf(y1[e]) < INFINITY)) { y1[e] = 0.f; odd = true; }
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) {
+                        uint32_t b0, b1, e0 = 0, e1 = 0;
+                        if (kF32) {
+                            tf32_split(y0[e], b0, e0);
+                            tf32_split(y1[e], b1, e1);
+                        } else {
+                            b0 = __float_as_uint(y0[e]);
+                            b1 = __float_as_uint(y1[e]);
+                        }
+                        float *oj = o[s * VE + e];
+                        mma_tf32(oj, pl, b0, b1);
+                        if (kF32) mma_tf32(oj, ph, e0, e1);
+                        mma_tf32(oj, ph, b0, b1);
+                    }
+                }
+                if (edge && __any_sync(0xffffffffu, odd)) {
+                    // rare: the values that were taken as zero above, added for the rows that see them
+#pragma unroll 1
+                    for (int q8 = 0; q8 < 8; ++q8) {
+                        const int src = (lane & ~3) | (q8 >> 1);
+                        const float w0 = __shfl_sync(0xffffffffu, (q8 & 1) ? x[1] : x[0], src);
+                        const float w1 = __shfl_sync(0xffffffffu, (q8 & 1) ? x[3] : x[2], src);
+                        const uint8_t *vr = sv + (nt * 8 + q8) * C::VS;
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int dim = (j / VE) * 8 * VE + VE * (2 * c + e) + j % VE;
+                                const float y = load_q(vr, Elem<KT>::kCode, dim);
+                                if (!(fabsf(y) < INFINITY)) {
+                                    if (w0 > 0.f) o[j][e] += w0 * y;
+                                    if (w1 > 0.f) o[j][2 + e] += w1 * y;
+                                }
+                            }
+                    }
+                }
+            }
+        }
+        cp_wait<0>();
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+        __syncthreads();  // the ring is free: [warp][16 rows][D + m + l], in groups' order
+        constexpr int OS = D + 4;
+        float *mine = reinterpret_cast<float *>(ring) + (size_t)warp * 16 * OS;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int dim = (j / VE) * 8 * VE + VE * (2 * c + e) + j % VE;
+                mine[g * OS + dim] = o[j][e];
+                mine[(g + 8) * OS + dim] = o[j][2 + e];
+            }
+        if (c == 0) {
+            mine[g * OS + D] = m0;
+            mine[g * OS + D + 1] = l0;
+            mine[(g + 8) * OS + D] = m1;
+            mine[(g + 8) * OS + D + 1] = l1;
+        }
+        __syncthreads();
+        // joined over the groups: thread (row, 4 dims)
+        float *part = sg.slot < 2 ? tree_part(p, D, blockIdx.x, sg.slot) : nullptr;
+        for (int i = threadIdx.x; i < RW * 16 * (D / 4); i += kThreads) {
+            const uint32_t r = i / (D / 4);
+            const int x4 = i % (D / 4);
+            if (r >= sg.rows) break;
+            const float *src = reinterpret_cast<float *>(ring) + ((size_t)(r / 16) * 16 + r % 16) * OS;
+            constexpr size_t GS = (size_t)RW * 16 * OS;
+            float m = -INFINITY;
+#pragma unroll
+            for (int q8 = 0; q8 < C::GROUPS; ++q8) m = fmaxf(m, src[q8 * GS + D]);
+            const float mu = m == -INFINITY ? 0.f : m;
+            float l = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int q8 = 0; q8 < C::GROUPS; ++q8) {
+                const float f = exp2f(src[q8 * GS + D] - mu);
+                const float4 y = *reinterpret_cast<const float4 *>(src + q8 * GS + x4 * 4);
+                l += f * src[q8 * GS + D + 1];
+                // a group that saw nothing (f = 0) holds zeros
+                acc.x += f * y.x;
+                acc.y += f * y.y;
+                acc.z += f * y.z;
+                acc.w += f * y.w;
+            }
+            if (part) {
+                *reinterpret_cast<float4 *>(part + (size_t)r * D + x4 * 4) = acc;
+                if (x4 == 0) {
+                    part[(size_t)p.rpg * D + r] = m;
+                    part[(size_t)p.rpg * (D + 1) + r] = l;
+                }
+            } else {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                const size_t at = tree_row(p, sg, sg.row0 + r, D) + x4 * 4;
+                store_out(p.out, p.q_type, at, acc.x * inv);
+                store_out(p.out, p.q_type, at + 1, acc.y * inv);
+                store_out(p.out, p.q_type, at + 2, acc.z * inv);
+                store_out(p.out, p.q_type, at + 3, acc.w * inv);
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Merge of the units that a cut divides.  CTA (x, y): cut x + 1 of the line;
+// it serves the unit that the cut divides, if it is the first cut in it, and
+// the rows y, y + gridDim.y, ... in blocks of 8 (a warp each).  Segments are
+// added in tile order, so a unit's result does not depend on timing.
+// ---------------------------------------------------------------------------
+template <int D>
+__global__ void __launch_bounds__(kThreads) tree_merge_kernel(const __grid_constant__ TreeParams p, uint32_t grid) {
+    __shared__ TreeShared sh;
+    const uint32_t b = blockIdx.x + 1;
+    const TreeRange range = tree_range(p, &sh, b, grid);
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the segments' partials are written
+    if (range.w0 >= range.w1) return;
+    TreeWalk walk(p, range);
+    TreeSeg sg;
+    walk.next(p, sg);
+    if (sg.t0 == 0) return;  // the cut lies between two units
+    // the unit's place on the line, and the cuts inside it
+    const unsigned long long u0 = range.w0 - sg.t0, u1 = u0 + sg.s.tiles;
+    const unsigned long long total = range.total;      // cut x is at total * x / active
+    if (total * (b - 1) / range.active > u0) return;  // an earlier cut is inside the unit
+    uint32_t last = b;  // last CTA with a segment of the unit
+    while (last + 1 < range.active && total * (last + 1) / range.active < u1) ++last;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int V = D / 32;  // values of a lane
+    for (uint32_t r = blockIdx.y * kWarps + warp; r < sg.rows; r += gridDim.y * kWarps) {
+        float m = -INFINITY;
+        for (uint32_t s = b - 1 + lane; s <= last; s += 32)
+            m = fmaxf(m, tree_part(p, D, s, s == b - 1 ? 1u : 0u)[(size_t)p.rpg * D + r]);
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+        const float mu = m == -INFINITY ? 0.f : m;
+        float acc[V], l = 0.f;
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = 0.f;
+#pragma unroll 4
+        for (uint32_t s = b - 1; s <= last; ++s) {
+            const float *part = tree_part(p, D, s, s == b - 1 ? 1u : 0u);
+            const float f = exp2f(part[(size_t)p.rpg * D + r] - mu);
+            l += f * part[(size_t)p.rpg * (D + 1) + r];
+            if (V == 4) {
+                const float4 y = *reinterpret_cast<const float4 *>(part + (size_t)r * D + lane * 4);
+                acc[0] += f * y.x;
+                acc[1] += f * y.y;
+                acc[V > 2 ? 2 : 0] += f * y.z;
+                acc[V > 2 ? 3 : 1] += f * y.w;
+            } else {
+                const float2 y = *reinterpret_cast<const float2 *>(part + (size_t)r * D + lane * 2);
+                acc[0] += f * y.x;
+                acc[1] += f * y.y;
+            }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const size_t at = tree_row(p, sg, sg.row0 + r, D) + lane * V;
+#pragma unroll
+        for (int i = 0; i < V; ++i) store_out(p.out, p.q_type, at + i, acc[i] * inv);
+    }
+}
+
+template <typename F>
+cudaError_t allow_smem(F *f, int bytes) {
+    return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+template <int D, typename KT, int RW>
+cudaError_t launch_f32(TreeParams p, int num_sms, cudaStream_t st) {
+    using C = FCfg<D, KT, RW>;
+    static_assert(C::SMEM <= 227 * 1024 - 512, "shared memory");
+    auto kern = tree_f32_kernel<D, KT, RW>;
+    cudaError_t e = allow_smem(kern, C::SMEM);
+    if (e != cudaSuccess) return e;
+    p.rpg = RW * 16;
+    p.min_tiles = 1;
+    kern<<<num_sms, kThreads, C::SMEM, st>>>(p);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    return launch_tree_merge(p, D, num_sms, st);
+}
+
+template <int D, typename KT>
+cudaError_t launch_rows(const TreeParams &p, int num_sms, cudaStream_t st) {
+    // rows of a request and kv head on average: above 16, one CTA covers 64
+    const uint64_t rows = (uint64_t)p.n_tokens * p.group / p.n_seqs;
+    return rows > 16 ? launch_f32<D, KT, 4>(p, num_sms, st) : launch_f32<D, KT, 1>(p, num_sms, st);
+}
+
+template <int D>
+cudaError_t launch_kv(const TreeArgs &a, cudaStream_t st) {
+    switch (a.kv_type) {
+        case BML_F32: return launch_rows<D, float>(a.p, a.num_sms, st);
+        case BML_F16: return launch_rows<D, __half>(a.p, a.num_sms, st);
+        case BML_BF16: return launch_rows<D, __nv_bfloat16>(a.p, a.num_sms, st);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+cudaError_t launch_tree_merge(const TreeParams &p, uint32_t D, int grid, cudaStream_t st) {
+    if (grid < 2) return cudaSuccess;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid - 1, p.rpg > 64 ? 8 : 2);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return D == 128 ? cudaLaunchKernelEx(&cfg, tree_merge_kernel<128>, p, (uint32_t)grid)
+                    : cudaLaunchKernelEx(&cfg, tree_merge_kernel<64>, p, (uint32_t)grid);
+}
+
+size_t tree_workspace_bytes(uint32_t D, int num_sms) {
+    return (size_t)2 * num_sms * kTreeMaxRows * (D + 2) * sizeof(float);
+}
+
+cudaError_t launch_tree(const TreeArgs &a, cudaStream_t st) {
+    return a.D == 128 ? launch_kv<128>(a, st) : launch_kv<64>(a, st);
+}
+
+}  // namespace bml

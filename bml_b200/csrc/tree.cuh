@@ -1,0 +1,198 @@
+// tree.cuh -- attention of drafted tokens over a paged cache: parameters,
+// the tile schedule shared by the kernels, and the launch interface.
+#pragma once
+
+#include "paged.cuh"
+
+namespace bml {
+
+constexpr int kTreeTile = 128;         // positions of one schedule tile
+constexpr uint32_t kTreeMaxSeqs = 1024;  // requests of one launch
+
+struct TreeParams {
+    const void *q;  // [n_tokens][n_heads][D]
+    void *out;      // same shape and type
+    const void *k, *v;  // pools [n_pages][page][n_kv][D]
+    const int32_t *table;  // [n_seqs][max_pages]
+    const int32_t *kv_lens, *node_start;
+    const uint64_t *mask;  // [n_tokens][n_words] or null: node t sees nodes 0..t
+    uint32_t n_seqs, n_tokens, n_heads, n_kv, group, max_pages, n_pages, page_shift, n_words;
+    float scale_log2;
+    int q_type;  // bml_dtype of q and out
+    // partials: slots of rpg rows, o [rpg][D] un-normalised, then m [rpg], l [rpg]
+    float *part;
+    uint32_t rpg;        // rows of a row group
+    uint32_t min_tiles;  // tiles a CTA takes at least
+    uint32_t *err;       // sticky error word of the tensor-core kernel
+};
+
+struct TreeArgs {
+    TreeParams p;
+    uint32_t D;
+    bml_dtype kv_type;
+    int num_sms;
+};
+
+constexpr uint32_t kTreeMaxRows = 256;  // rows of the largest row group
+cudaError_t launch_tree_merge(const TreeParams &p, uint32_t D, int grid, cudaStream_t st);
+size_t tree_workspace_bytes(uint32_t D, int num_sms);
+cudaError_t launch_tree(const TreeArgs &a, cudaStream_t st);
+
+#ifdef __CUDACC__
+// ---------------------------------------------------------------------------
+// Schedule.  A unit is one (request, kv head, row group): the query rows
+// (node t, q head g of the kv head) of up to rpg consecutive t * group + g,
+// over all positions of the request.  Units are laid out request by request,
+// kv head by kv head, row group by row group, each as its number of
+// 128-position tiles, and the line of all tiles is cut evenly over the CTAs,
+// so the lengths stay on the GPU and no CTA works longer than another by more
+// than a tile.  A unit that a cut divides leaves partial results (max, sum,
+// un-normalised output) which tree_merge_kernel joins in tile order.
+// ---------------------------------------------------------------------------
+struct TreeSeq {
+    uint32_t first;  // first token row
+    uint32_t T, L;   // drafted tokens; positions (0: refused, its rows are zero)
+    uint32_t rows, groups, tiles;
+};
+
+__device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, uint32_t i) {
+    TreeSeq s;
+    const int32_t a = p.node_start[i], b = p.node_start[i + 1], L = p.kv_lens[i];
+    const bool rows_ok = a >= 0 && b > a && (uint32_t)b <= p.n_tokens;
+    s.first = rows_ok ? (uint32_t)a : 0u;
+    s.T = rows_ok ? (uint32_t)(b - a) : 0u;
+    const uint32_t most = p.mask ? p.n_words * 64 : kTreeMaxNodes;
+    const bool ok = s.T <= most && L >= (int32_t)s.T && (uint64_t)L <= ((uint64_t)p.max_pages << p.page_shift);
+    s.L = ok ? (uint32_t)L : 0u;
+    s.rows = s.T * p.group;
+    s.groups = (s.rows + p.rpg - 1) / p.rpg;
+    s.tiles = s.L ? (s.L + kTreeTile - 1) / kTreeTile : 1u;
+    return s;
+}
+
+struct TreeShared {
+    unsigned long long warp_sums[32];
+    unsigned long long base;  // place of seq's first tile on the line
+    uint32_t seq;
+};
+
+// CTA b's range of the line, and where it starts.
+struct TreeRange {
+    unsigned long long w0, w1, base, total;
+    uint32_t seq, active;  // CTAs that share the line
+};
+
+// Every thread of the CTA calls it (blockDim a multiple of 32); three
+// barriers.  w0 == w1: nothing for this CTA.
+__device__ __forceinline__ TreeRange tree_range(const TreeParams &p, TreeShared *sh, uint32_t b, uint32_t grid) {
+    const uint32_t nt = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t per = (p.n_seqs + nt - 1) / nt;
+    const uint32_t i0 = min(threadIdx.x * per, p.n_seqs), i1 = min(i0 + per, p.n_seqs);
+    auto cost = [&](uint32_t i) {
+        const TreeSeq s = tree_seq(p, i);
+        return (unsigned long long)s.tiles * s.groups * p.n_kv;
+    };
+    unsigned long long sum = 0;
+    for (uint32_t i = i0; i < i1; ++i) sum += cost(i);
+    unsigned long long inc = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= (uint32_t)o) inc += u;
+    }
+    if (lane == 31) sh->warp_sums[warp] = inc;
+    __syncthreads();
+    unsigned long long first = inc - sum, total = 0;
+    for (uint32_t w = 0; w < nt / 32; ++w) {
+        const unsigned long long s = sh->warp_sums[w];
+        if (w < warp) first += s;
+        total += s;
+    }
+    TreeRange r;
+    r.total = total;
+    const unsigned long long most = (total + p.min_tiles - 1) / p.min_tiles;
+    r.active = most < grid ? (uint32_t)most : grid;
+    r.w0 = r.w1 = 0;
+    if (b < r.active) {
+        r.w0 = total * b / r.active;
+        r.w1 = total * (b + 1) / r.active;
+    }
+    if (r.w0 < r.w1 && r.w0 >= first && r.w0 < first + sum) {
+        unsigned long long at = first;
+        uint32_t i = i0;
+        while (true) {
+            const unsigned long long c = cost(i);
+            if (r.w0 < at + c) break;
+            at += c;
+            ++i;
+        }
+        sh->seq = i;
+        sh->base = at;
+    }
+    __syncthreads();
+    r.seq = sh->seq;
+    r.base = sh->base;
+    __syncthreads();
+    return r;
+}
+
+// The segments of a range in order: consecutive tiles of one unit.
+struct TreeSeg {
+    uint32_t seq, head, rg;
+    uint32_t t0, t1;     // tiles of the unit, [t0, t1)
+    uint32_t row0, rows; // first row (t * group + g) and row count of the group
+    uint32_t slot;       // partial slot of the CTA: 0 the unit began before this range, 1 it ends after it, 2 whole
+    TreeSeq s;
+};
+
+struct TreeWalk {
+    unsigned long long pos, end, base;
+    uint32_t seq;
+    TreeSeq s;
+    __device__ __forceinline__ TreeWalk(const TreeParams &p, const TreeRange &r) : pos(r.w0), end(r.w1), base(r.base), seq(r.seq) {
+        if (pos < end) s = tree_seq(p, seq);
+    }
+    __device__ __forceinline__ bool next(const TreeParams &p, TreeSeg &g) {
+        if (pos >= end) return false;
+        unsigned long long units;
+        while (pos >= base + (units = (unsigned long long)s.groups * p.n_kv) * s.tiles) {
+            base += units * s.tiles;
+            s = tree_seq(p, ++seq);
+        }
+        const unsigned long long off = pos - base;
+        const uint32_t u = (uint32_t)(off / s.tiles);
+        const unsigned long long left = end - pos;
+        g.seq = seq;
+        g.s = s;
+        g.head = u / s.groups;
+        g.rg = u - g.head * s.groups;
+        g.t0 = (uint32_t)(off - (unsigned long long)u * s.tiles);
+        g.t1 = left < s.tiles - g.t0 ? g.t0 + (uint32_t)left : s.tiles;
+        g.row0 = g.rg * p.rpg;
+        g.rows = min(p.rpg, s.rows - g.row0);
+        g.slot = g.t0 > 0 ? 0u : (g.t1 < s.tiles ? 1u : 2u);
+        pos += g.t1 - g.t0;
+        return true;
+    }
+};
+
+// Partial slot `which` (0 or 1) of CTA b.
+__device__ __forceinline__ float *tree_part(const TreeParams &p, uint32_t D, uint32_t b, uint32_t which) {
+    return p.part + (size_t)(2 * b + which) * p.rpg * (D + 2);
+}
+
+// Element index of row r (t * group + g) of kv head h of a request in q and out.
+__device__ __forceinline__ size_t tree_row(const TreeParams &p, const TreeSeg &g, uint32_t r, uint32_t D) {
+    const uint32_t t = r / p.group, qg = r - t * p.group;
+    return ((size_t)(g.s.first + t) * p.n_heads + (size_t)g.head * p.group + qg) * D;
+}
+
+// Whether node t of a request sees position pos >= P (= node pos - P).
+__device__ __forceinline__ bool tree_sees(const TreeParams &p, const TreeSeq &s, uint32_t t, uint32_t node) {
+    if (node >= s.T) return false;
+    if (!p.mask) return node <= t;
+    return (p.mask[(size_t)(s.first + t) * p.n_words + (node >> 6)] >> (node & 63)) & 1;
+}
+#endif
+
+}  // namespace bml

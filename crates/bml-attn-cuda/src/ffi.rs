@@ -86,6 +86,27 @@ extern "C" {
                             seq_len: u32, n_heads: u32, n_kv: u32, head_dim: u32, input: bml_dtype,
                             scale: f32, causal: c_int, out: *mut c_void, out_dtype: bml_dtype,
                             stream: *mut c_void) -> bml_status;
+    pub fn bml_paged_plan(lens: *const i32, n_new: *const i32, owned: *const i32, n: u32, free_pages: *const i32,
+                          n_free: u32, free_used: *const i32, page_size: u32, max_pages: u32,
+                          block_table: *mut i32, parents: *const i32, n_tokens: u32, n_words: u32,
+                          node_start: *mut i32, kv_lens: *mut i32, owned_out: *mut i32, free_used_out: *mut i32,
+                          slots: *mut i64, positions: *mut i32, mask: *mut u64, status: *mut i32,
+                          stream: *mut c_void) -> bml_status;
+    pub fn bml_paged_append(q: *const c_void, k: *const c_void, v: *const c_void, src: bml_dtype, slots: *const i64,
+                            positions: *const i32, n_tokens: u32, n_heads: u32, n_kv: u32, head_dim: u32,
+                            theta: f64, q_out: *mut c_void, k_pool: *mut c_void, v_pool: *mut c_void,
+                            kv: bml_dtype, n_rows: u64, stream: *mut c_void) -> bml_status;
+    pub fn bml_attn_tree_workspace_size(head_dim: u32, device: i32, bytes: *mut usize) -> bml_status;
+    pub fn bml_attn_tree(q: *const c_void, q_dtype: bml_dtype, n_tokens: u32, n_heads: u32, n_kv: u32,
+                         head_dim: u32, k_pool: *const c_void, v_pool: *const c_void, kv: bml_dtype, n_pages: u32,
+                         page_size: u32, block_table: *const i32, max_pages: u32, kv_lens: *const i32,
+                         node_start: *const i32, n_seqs: u32, mask: *const u64, n_words: u32, scale: f32,
+                         out: *mut c_void, ws: *mut c_void, ws_bytes: usize, stream: *mut c_void) -> bml_status;
+    pub fn bml_paged_commit(k_pool: *mut c_void, v_pool: *mut c_void, n_layers: u32, n_pages: u32, page_size: u32,
+                            n_kv: u32, head_dim: u32, kv: bml_dtype, block_table: *const i32, max_pages: u32,
+                            lens: *const i32, kv_lens: *const i32, node_start: *const i32, n: u32,
+                            path: *const i32, max_path: u32, n_accept: *const i32, lens_out: *mut i32,
+                            stream: *mut c_void) -> bml_status;
     pub fn bml_softmax_f32(x: *const f32, n_rows: u32, n: u32, out: *mut f32,
                            stream: *mut c_void) -> bml_status;
     pub fn bml_attn_workspace_check(ws: *mut c_void, bytes: usize, stream: *mut c_void) -> bml_status;

@@ -386,6 +386,142 @@ bml_status bml_attn_decode_kvsplit(bml_kvsplit *h, const bml_seq_desc *slice_hos
 bml_status bml_kvsplit_destroy(bml_kvsplit *h);
 
 /* ------------------------------------------------------------------------ */
+/* Paged KV cache and drafted tokens                                        */
+/* ------------------------------------------------------------------------ */
+
+/* A paged cache keeps every request's K and V in pages of page_size
+ * positions out of one pool per layer, [n_pages][page_size][n_kv_heads]
+ * [head_dim] (a row of the pool is one position of all kv heads, the
+ * reference's layout, kv_cache.rs:17), and a block table [n][max_pages] of
+ * page indices per request.  All sizes of a step -- lengths, new tokens,
+ * page counts -- stay on the device, so a step needs no host
+ * synchronisation and can be captured in a CUDA graph.  No reference
+ * counterpart: the reference keeps one flat buffer per layer and decodes
+ * one token at a time.
+ *
+ * A step of a batch of n requests:
+ *   bml_paged_plan      pages for the new tokens, their slots, positions and
+ *                       (for drafts) ancestor masks -- once a step
+ *   bml_paged_append    RoPE of q and k, K and V rows stored -- every layer
+ *   bml_attn_tree       attention of the new tokens -- every layer
+ *   bml_paged_commit    the rows of the accepted path moved to the front,
+ *                       all layers, new lengths -- once a step
+ * page_size is a power of two from 16 to 1024 and max_pages * page_size
+ * below 2^31 in every call. */
+
+/* Plans one step.  Request i has lens[i] committed positions, owned[i] pages
+ * in its row of block_table, and n_new[i] new tokens (0 for none); token rows
+ * are the requests' new tokens in request order.
+ *   free_pages [n_free]: the pool's pages; the first *free_used are taken,
+ *       and pages are taken from there on, in request order;
+ *   node_start [n+1]: first token row of each request, and the end;
+ *   kv_lens [n]: lens + n_new, or 0 for a refused request;
+ *   owned_out [n], free_used_out [1]: the counts after this plan (their own
+ *       buffers: not owned, not free_used);
+ *   block_table [n][max_pages]: new entries written, others left;
+ *   slots [n_tokens] int64: row of the pool for each token, -1 for a token of
+ *       a refused request and for rows behind the last token;
+ *   positions [n_tokens]: RoPE position: lens + j for the j-th token, with
+ *       parents lens + depth; 0 where the slot is -1;
+ *   parents [n_tokens] or NULL: a drafted token's parent among its request's
+ *       tokens, -1 (or anything not before the token) for a child of the last
+ *       committed token;
+ *   mask [n_tokens][n_words] (with parents; n_words 1 to 4): bits of the
+ *       token's ancestors and of itself; zero where the slot is -1;
+ *   status [n]: 0, or why the request is refused: 1 not enough free pages
+ *       (for it and the requests before it), 2 more positions than its table
+ *       row holds, more than 64 * n_words drafted tokens, or a negative
+ *       count, 4 its tokens lie beyond n_tokens.  A refused request takes no
+ *       pages.
+ * All arrays are int32 on the device unless noted.  n <= 4096.
+ * Asynchronous. */
+bml_status bml_paged_plan(const int32_t *lens, const int32_t *n_new,
+                          const int32_t *owned, uint32_t n,
+                          const int32_t *free_pages, uint32_t n_free,
+                          const int32_t *free_used, uint32_t page_size,
+                          uint32_t max_pages, int32_t *block_table,
+                          const int32_t *parents, uint32_t n_tokens,
+                          uint32_t n_words, int32_t *node_start,
+                          int32_t *kv_lens, int32_t *owned_out,
+                          int32_t *free_used_out, int64_t *slots,
+                          int32_t *positions, uint64_t *mask, int32_t *status,
+                          void *stream);
+
+/* RoPE and store of n_tokens tokens of one layer: q [n_tokens][n_heads]
+ * [head_dim] turned by positions (interleaved pairs, angle position *
+ * theta^(-2i/head_dim), gguf_compiler.rs:1290-1317 with theta 10000) into
+ * q_out (q itself, or a buffer that does not overlap it), k turned and v as
+ * is ([n_tokens][n_kv_heads][head_dim]) into row slots[t] of the pools.
+ * positions NULL: no rotation.  q and q_out NULL: no queries.  A token whose
+ * slot is outside [0, n_rows) is skipped: nothing of it is written.  Angles
+ * are f64, the rotation f32; results are rounded once to the destination's
+ * type.  Slots of one call must differ (of two tokens with the same slot,
+ * either's values may be stored).  head_dim even; pointers aligned to two
+ * elements.  Asynchronous. */
+bml_status bml_paged_append(const void *q_dev, const void *k_dev,
+                            const void *v_dev, bml_dtype src_dtype,
+                            const int64_t *slots, const int32_t *positions,
+                            uint32_t n_tokens, uint32_t n_heads,
+                            uint32_t n_kv_heads, uint32_t head_dim,
+                            double theta, void *q_out_dev, void *k_pool,
+                            void *v_pool, bml_dtype kv_dtype, uint64_t n_rows,
+                            void *stream);
+
+/* Scratch bytes of bml_attn_tree on `device` (whatever the batch). */
+bml_status bml_attn_tree_workspace_size(uint32_t head_dim, int32_t device,
+                                        size_t *bytes);
+
+/* Attention of every request's new tokens over its pages: token row t of
+ * request i (node j = t - node_start[i] of T) attends over the committed
+ * positions [0, kv_lens[i] - T) and over those nodes whose bits are set in
+ * mask[t]; mask NULL: over nodes 0..j (a chain; T = 1 is plain decode).
+ *   q_dev, out_dev: [n_tokens][n_heads][head_dim] in q_dtype: BML_F32 with
+ *       pages of any type, or the pages' own 16-bit type;
+ *   workspace: bml_attn_tree_workspace_size bytes, 16-byte aligned, no
+ *       contents needed; calls that share one must not overlap in time.
+ * At most 256 nodes a request (64 * n_words with a mask).  Rows that see
+ * nothing are zero; so are all rows of a request with kv_lens[i] < T (one
+ * that bml_paged_plan refused), with more nodes than that, or with more
+ * positions than its table holds.  Positions on a page outside [0, n_pages)
+ * count as masked.  What lies in masked places -- cache rows past kv_lens,
+ * nodes that a row does not see, infinities and NaN among them -- does not
+ * reach the row.  Token rows outside the requests' are left as they were.
+ * 16-bit queries: scores and sums in f32, the softmax weights rounded to the
+ * 16-bit type before P.V, one rounding of the output; 32-bit queries: about
+ * f32 precision throughout.  Results are the same from run to run on one
+ * device.  head_dim 64 or 128.  Asynchronous. */
+bml_status bml_attn_tree(const void *q_dev, bml_dtype q_dtype,
+                         uint32_t n_tokens, uint32_t n_heads,
+                         uint32_t n_kv_heads, uint32_t head_dim,
+                         const void *k_pool, const void *v_pool,
+                         bml_dtype kv_dtype, uint32_t n_pages,
+                         uint32_t page_size, const int32_t *block_table,
+                         uint32_t max_pages, const int32_t *kv_lens,
+                         const int32_t *node_start, uint32_t n_seqs,
+                         const uint64_t *mask, uint32_t n_words, float scale,
+                         void *out_dev, void *workspace,
+                         size_t workspace_bytes, void *stream);
+
+/* Commits the accepted path of every request's draft: in the K and V pools of
+ * all n_layers layers (layer l at pool + l * n_pages * page_size * row), row
+ * lens[i] + path[i][k] moves to row lens[i] + k for k < n_accept[i], and
+ * lens_out[i] = lens[i] + the accepted count.  path [n][max_path] int32 holds
+ * strictly increasing node indices; an entry that is not larger than the one
+ * before, or not below the request's node count, ends the path there, and the
+ * count with it.  A request with kv_lens[i] != lens[i] + its node count (one
+ * that the plan refused) commits nothing.  lens_out is its own buffer, not
+ * lens.  Asynchronous. */
+bml_status bml_paged_commit(void *k_pool, void *v_pool, uint32_t n_layers,
+                            uint32_t n_pages, uint32_t page_size,
+                            uint32_t n_kv_heads, uint32_t head_dim,
+                            bml_dtype kv_dtype, const int32_t *block_table,
+                            uint32_t max_pages, const int32_t *lens,
+                            const int32_t *kv_lens, const int32_t *node_start,
+                            uint32_t n, const int32_t *path, uint32_t max_path,
+                            const int32_t *n_accept, int32_t *lens_out,
+                            void *stream);
+
+/* ------------------------------------------------------------------------ */
 /* Device-side error word                                                   */
 /* ------------------------------------------------------------------------ */
 
