@@ -502,6 +502,7 @@ size_t tree_workspace_bytes(uint32_t D, int num_sms) {
 }
 
 cudaError_t launch_tree(const TreeArgs &a, cudaStream_t st) {
+    if (tree_umma_fits(a)) return launch_tree_umma(a, st);
     return a.D == 128 ? launch_kv<128>(a, st) : launch_kv<64>(a, st);
 }
 

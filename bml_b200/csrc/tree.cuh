@@ -23,7 +23,6 @@ struct TreeParams {
     float *part;
     uint32_t rpg;        // rows of a row group
     uint32_t min_tiles;  // tiles a CTA takes at least
-    uint32_t *err;       // sticky error word of the tensor-core kernel
 };
 
 struct TreeArgs {
@@ -37,6 +36,8 @@ constexpr uint32_t kTreeMaxRows = 256;  // rows of the largest row group
 cudaError_t launch_tree_merge(const TreeParams &p, uint32_t D, int grid, cudaStream_t st);
 size_t tree_workspace_bytes(uint32_t D, int num_sms);
 cudaError_t launch_tree(const TreeArgs &a, cudaStream_t st);
+bool tree_umma_fits(const TreeArgs &a);
+cudaError_t launch_tree_umma(const TreeArgs &a, cudaStream_t st);
 
 #ifdef __CUDACC__
 // ---------------------------------------------------------------------------
