@@ -402,44 +402,65 @@ __global__ void __launch_bounds__(kThreads) tree_merge_kernel(const __grid_const
     walk.next(p, sg);
     if (sg.t0 == 0) return;  // the cut lies between two units
     // the unit's place on the line, and the cuts inside it
-    const unsigned long long u0 = range.w0 - sg.t0, u1 = u0 + sg.s.tiles;
-    const unsigned long long total = range.total;      // cut x is at total * x / active
-    if (total * (b - 1) / range.active > u0) return;  // an earlier cut is inside the unit
+    const uint32_t u0 = range.w0 - sg.t0, u1 = u0 + sg.s.tiles;
+    if (tree_cut(range.total, b - 1, range.active) > u0) return;  // an earlier cut is inside the unit
     uint32_t last = b;  // last CTA with a segment of the unit
-    while (last + 1 < range.active && total * (last + 1) / range.active < u1) ++last;
+    while (last + 1 < range.active && tree_cut(range.total, last + 1, range.active) < u1) ++last;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr int V = D / 32;  // values of a lane
-    for (uint32_t r = blockIdx.y * kWarps + warp; r < sg.rows; r += gridDim.y * kWarps) {
-        float m = -INFINITY;
-        for (uint32_t s = b - 1 + lane; s <= last; s += 32)
-            m = fmaxf(m, tree_part(p, D, s, s == b - 1 ? 1u : 0u)[(size_t)p.rpg * D + r]);
+    // A lane holds V values of kRows rows at a time; the loads of up to 8
+    // segments are in flight together.
+    constexpr int kRows = 2;
+    for (uint32_t r0 = (blockIdx.y * kWarps + warp) * kRows; r0 < sg.rows; r0 += gridDim.y * kWarps * kRows) {
+        float m[kRows], acc[kRows][V], l[kRows];
 #pragma unroll
-        for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-        const float mu = m == -INFINITY ? 0.f : m;
-        float acc[V], l = 0.f;
+        for (int i = 0; i < kRows; ++i) {
+            m[i] = -INFINITY;
+            l[i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = 0.f;
-#pragma unroll 4
+            for (int v = 0; v < V; ++v) acc[i][v] = 0.f;
+        }
+        for (uint32_t s = b - 1 + lane; s <= last; s += 32) {
+            const float *part = tree_part(p, D, s, s == b - 1 ? 1u : 0u) + (size_t)p.rpg * D;
+#pragma unroll
+            for (int i = 0; i < kRows; ++i)
+                if (r0 + i < sg.rows) m[i] = fmaxf(m[i], part[r0 + i]);
+        }
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+#pragma unroll
+            for (int x = 16; x > 0; x >>= 1) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], x));
+            if (m[i] == -INFINITY) m[i] = 0.f;
+        }
+#pragma unroll 8
         for (uint32_t s = b - 1; s <= last; ++s) {
             const float *part = tree_part(p, D, s, s == b - 1 ? 1u : 0u);
-            const float f = exp2f(part[(size_t)p.rpg * D + r] - mu);
-            l += f * part[(size_t)p.rpg * (D + 1) + r];
-            if (V == 4) {
-                const float4 y = *reinterpret_cast<const float4 *>(part + (size_t)r * D + lane * 4);
-                acc[0] += f * y.x;
-                acc[1] += f * y.y;
-                acc[V > 2 ? 2 : 0] += f * y.z;
-                acc[V > 2 ? 3 : 1] += f * y.w;
-            } else {
-                const float2 y = *reinterpret_cast<const float2 *>(part + (size_t)r * D + lane * 2);
-                acc[0] += f * y.x;
-                acc[1] += f * y.y;
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                const uint32_t r = min(r0 + i, sg.rows - 1);
+                const float f = exp2f(part[(size_t)p.rpg * D + r] - m[i]);
+                l[i] += f * part[(size_t)p.rpg * (D + 1) + r];
+                if (V == 4) {
+                    const float4 y = *reinterpret_cast<const float4 *>(part + (size_t)r * D + lane * 4);
+                    acc[i][0] += f * y.x;
+                    acc[i][1] += f * y.y;
+                    acc[i][V > 2 ? 2 : 0] += f * y.z;
+                    acc[i][V > 2 ? 3 : 1] += f * y.w;
+                } else {
+                    const float2 y = *reinterpret_cast<const float2 *>(part + (size_t)r * D + lane * 2);
+                    acc[i][0] += f * y.x;
+                    acc[i][1] += f * y.y;
+                }
             }
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        const size_t at = tree_row(p, sg, sg.row0 + r, D) + lane * V;
 #pragma unroll
-        for (int i = 0; i < V; ++i) store_out(p.out, p.q_type, at + i, acc[i] * inv);
+        for (int i = 0; i < kRows; ++i) {
+            if (r0 + i >= sg.rows) break;
+            const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
+            const size_t at = tree_row(p, sg, sg.row0 + r0 + i, D) + lane * V;
+#pragma unroll
+            for (int v = 0; v < V; ++v) store_out(p.out, p.q_type, at + v, acc[i][v] * inv);
+        }
     }
 }
 
@@ -485,7 +506,7 @@ cudaError_t launch_kv(const TreeArgs &a, cudaStream_t st) {
 cudaError_t launch_tree_merge(const TreeParams &p, uint32_t D, int grid, cudaStream_t st) {
     if (grid < 2) return cudaSuccess;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid - 1, p.rpg > 64 ? 8 : 2);
+    cfg.gridDim = dim3(grid - 1, p.rpg > 64 ? 16 : (p.rpg + 15) / 16);
     cfg.blockDim = dim3(kThreads);
     cfg.stream = st;
     cudaLaunchAttribute at[1];

@@ -72,14 +72,21 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, uint32_t i) {
 }
 
 struct TreeShared {
-    unsigned long long warp_sums[32];
-    unsigned long long base;  // place of seq's first tile on the line
+    uint32_t warp_sums[32];
+    uint32_t base;  // place of seq's first tile on the line
     uint32_t seq;
 };
 
+// Where cut b of n falls on a line of `total` tiles: total * b / n, without
+// its 64-bit division.
+__device__ __forceinline__ uint32_t tree_cut(uint32_t total, uint32_t b, uint32_t n) {
+    const uint32_t q = total / n;
+    return q * b + (total - q * n) * b / n;
+}
+
 // CTA b's range of the line, and where it starts.
 struct TreeRange {
-    unsigned long long w0, w1, base, total;
+    uint32_t w0, w1, base, total;
     uint32_t seq, active;  // CTAs that share the line
 };
 
@@ -91,38 +98,38 @@ __device__ __forceinline__ TreeRange tree_range(const TreeParams &p, TreeShared 
     const uint32_t i0 = min(threadIdx.x * per, p.n_seqs), i1 = min(i0 + per, p.n_seqs);
     auto cost = [&](uint32_t i) {
         const TreeSeq s = tree_seq(p, i);
-        return (unsigned long long)s.tiles * s.groups * p.n_kv;
+        return s.tiles * s.groups * p.n_kv;
     };
-    unsigned long long sum = 0;
+    uint32_t sum = 0;
     for (uint32_t i = i0; i < i1; ++i) sum += cost(i);
-    unsigned long long inc = sum;
+    uint32_t inc = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const unsigned long long u = __shfl_up_sync(0xffffffffu, inc, o);
+        const uint32_t u = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= (uint32_t)o) inc += u;
     }
     if (lane == 31) sh->warp_sums[warp] = inc;
     __syncthreads();
-    unsigned long long first = inc - sum, total = 0;
+    uint32_t first = inc - sum, total = 0;
     for (uint32_t w = 0; w < nt / 32; ++w) {
-        const unsigned long long s = sh->warp_sums[w];
+        const uint32_t s = sh->warp_sums[w];
         if (w < warp) first += s;
         total += s;
     }
     TreeRange r;
     r.total = total;
-    const unsigned long long most = (total + p.min_tiles - 1) / p.min_tiles;
+    const uint32_t most = (total + p.min_tiles - 1) / p.min_tiles;
     r.active = most < grid ? (uint32_t)most : grid;
     r.w0 = r.w1 = 0;
     if (b < r.active) {
-        r.w0 = total * b / r.active;
-        r.w1 = total * (b + 1) / r.active;
+        r.w0 = tree_cut(total, b, r.active);
+        r.w1 = tree_cut(total, b + 1, r.active);
     }
     if (r.w0 < r.w1 && r.w0 >= first && r.w0 < first + sum) {
-        unsigned long long at = first;
+        uint32_t at = first;
         uint32_t i = i0;
         while (true) {
-            const unsigned long long c = cost(i);
+            const uint32_t c = cost(i);
             if (r.w0 < at + c) break;
             at += c;
             ++i;
@@ -147,7 +154,7 @@ struct TreeSeg {
 };
 
 struct TreeWalk {
-    unsigned long long pos, end, base;
+    uint32_t pos, end, base;
     uint32_t seq;
     TreeSeq s;
     __device__ __forceinline__ TreeWalk(const TreeParams &p, const TreeRange &r) : pos(r.w0), end(r.w1), base(r.base), seq(r.seq) {
@@ -155,20 +162,20 @@ struct TreeWalk {
     }
     __device__ __forceinline__ bool next(const TreeParams &p, TreeSeg &g) {
         if (pos >= end) return false;
-        unsigned long long units;
-        while (pos >= base + (units = (unsigned long long)s.groups * p.n_kv) * s.tiles) {
+        uint32_t units;
+        while (pos - base >= (units = s.groups * p.n_kv) * s.tiles) {
             base += units * s.tiles;
             s = tree_seq(p, ++seq);
         }
-        const unsigned long long off = pos - base;
-        const uint32_t u = (uint32_t)(off / s.tiles);
-        const unsigned long long left = end - pos;
+        const uint32_t off = pos - base;
+        const uint32_t u = off / s.tiles;
+        const uint32_t left = end - pos;
         g.seq = seq;
         g.s = s;
         g.head = u / s.groups;
         g.rg = u - g.head * s.groups;
-        g.t0 = (uint32_t)(off - (unsigned long long)u * s.tiles);
-        g.t1 = left < s.tiles - g.t0 ? g.t0 + (uint32_t)left : s.tiles;
+        g.t0 = off - u * s.tiles;
+        g.t1 = left < s.tiles - g.t0 ? g.t0 + left : s.tiles;
         g.row0 = g.rg * p.rpg;
         g.rows = min(p.rpg, s.rows - g.row0);
         g.slot = g.t0 > 0 ? 0u : (g.t1 < s.tiles ? 1u : 2u);

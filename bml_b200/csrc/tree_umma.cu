@@ -29,6 +29,8 @@
 // is not 0); the epilogue adds those nodes for the rows that see them.
 #include <math.h>
 
+#include <type_traits>
+
 #include "tree.cuh"
 #include "umma.cuh"
 
@@ -38,7 +40,7 @@ namespace {
 
 constexpr int BM = 128;  // rows of a row tile (TMEM lanes)
 constexpr int BN = kTreeTile;
-constexpr int kThreads = 320;
+constexpr int kThreads = 352;  // K and Q producer, MMA issuer, 4 + 4 softmax warps, V producer
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
 constexpr int kBadRing = 16;               // tiles whose page flags are kept; more than the ring holds
 
@@ -63,6 +65,34 @@ struct UmmaParams {
     uint32_t box_rows;  // min(page, 128)
 };
 
+// mbar_wait that looks at the clock only once in 256 tries: reading
+// %globaltimer takes longer than most of these waits.
+__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag) {
+    if (mbar_test_wait(bar, parity)) return true;
+    uint64_t t0 = 0;
+    while (true) {
+#pragma unroll 1
+        for (int i = 0; i < 256; ++i)
+            if (mbar_try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+        const uint64_t t = globaltimer_ns();
+        if (t0 == 0) t0 = t;
+        if (t - t0 > kWaitNs) {
+            *abort_flag = 1u;
+            return false;
+        }
+    }
+}
+
+// One segment, as the softmax warps read it.
+struct Board {
+    uint32_t seq, first, T, L, head, row0, t0;
+    uint32_t packed;  // tiles | slot << 28 | whether there is another segment << 31
+};
+// Entries of the ring of segments: the V producer is at most (slots / 2 + 2)
+// segments ahead of the softmax.
+constexpr uint32_t kBoard = 8;
+
 // Small shared arrays behind the ring.
 struct alignas(16) UmmaShared {
     uint64_t full[11], empty[11];
@@ -76,6 +106,8 @@ struct alignas(16) UmmaShared {
     uint32_t odd[8];         // drafted nodes whose V has a value that is not finite
     float2 ml[256];          // (m, l) of both chains' rows
     TreeShared sched;
+    uint64_t seg_full[kBoard];
+    Board board[kBoard];  // the segments, published by the V producer, which runs ahead
 };
 static_assert(sizeof(UmmaShared) <= 3072, "small arrays");
 
@@ -87,44 +119,66 @@ __device__ __forceinline__ uint32_t v_index(bool pair, uint32_t j, uint32_t n) {
     return pair ? 2 * j + 1 : min(2 * j + 2, 2 * n - 1);
 }
 
-// Mask bits of nodes n0 .. n0 + 31 for node t of the request (n0 < 0: the
-// committed positions before the nodes, seen by all).
-__device__ __forceinline__ uint32_t see32(const TreeParams &p, const TreeSeq &s, uint32_t t, int32_t n0) {
-    if (n0 >= (int32_t)s.T || s.L == 0) return 0u;
-    if (n0 <= -32) return 0xffffffffu;
-    const uint32_t first = n0 < 0 ? 0u : (uint32_t)n0;
-    uint64_t w;  // bit i: node first + i
-    if (p.mask) {
-        const uint64_t *m = p.mask + (size_t)(s.first + t) * p.n_words;
-        const uint32_t i = first >> 6, sh = first & 63;
-        w = m[i] >> sh;
-        if (sh > 32 && i + 1 < p.n_words) w |= m[i + 1] << (64 - sh);
-    } else {
-        const int32_t k = (int32_t)t - (int32_t)first;  // nodes up to t
-        w = k < 0 ? 0ull : k >= 63 ? ~0ull : (2ull << k) - 1;
+// Which of a tile's 128 positions the row sees, as four words; node0: node of
+// the tile's first position (negative: committed positions, seen by all).
+// bad: 16-position blocks on pages outside the pool.  Out of line: few tiles
+// need it, and the softmax's registers are dear.
+__device__ __noinline__ void see_tile(const TreeParams &p, const volatile Board *b, uint32_t row, int32_t node0, bool edge,
+                                      uint32_t bad, uint32_t *see) {
+    const uint32_t T = b->T, L = b->L, t = min((b->row0 + row) / p.group, T - 1);
+    const uint64_t *m = p.mask ? p.mask + (size_t)(b->first + t) * p.n_words : nullptr;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int32_t n0 = node0 + 32 * q;
+        uint32_t s = 0xffffffffu;
+        if (edge && (n0 >= (int32_t)T || L == 0)) s = 0u;
+        else if (edge && n0 > -32) {
+            const uint32_t first = n0 < 0 ? 0u : (uint32_t)n0;
+            uint64_t w;  // bit i: node first + i
+            if (m) {
+                const uint32_t i = first >> 6, sh = first & 63;
+                w = m[i] >> sh;
+                if (sh > 32 && i + 1 < p.n_words) w |= m[i + 1] << (64 - sh);
+            } else {
+                const int32_t k = (int32_t)t - (int32_t)first;  // nodes up to t
+                w = k < 0 ? 0ull : k >= 63 ? ~0ull : (2ull << k) - 1;
+            }
+            const uint32_t left = T - first;
+            if (left < 32) w &= (1ull << left) - 1;
+            s = n0 < 0 ? (uint32_t)(w << -n0) | ((1u << -n0) - 1) : (uint32_t)w;
+        }
+        if (bad >> (2 * q) & 1) s &= 0xffff0000u;
+        if (bad >> (2 * q + 1) & 1) s &= 0x0000ffffu;
+        see[q] = s;
     }
-    const uint32_t left = s.T - first;
-    if (left < 32) w &= (1ull << left) - 1;
-    if (n0 < 0) return (uint32_t)(w << -n0) | ((1u << -n0) - 1);
-    return (uint32_t)w;
-}
-
-// 2^(scale q.k) of one row and one position, from global memory; for the rare
-// nodes that the epilogue adds.
-template <int D, bool kF16>
-__device__ __noinline__ float rare_score(const uint16_t *q, const uint16_t *k) {
-    float s = 0.f;
-    for (int i = 0; i < D; ++i) {
-        const float a = kF16 ? __half2float(reinterpret_cast<const __half *>(q)[i]) : __uint_as_float((uint32_t)q[i] << 16);
-        const float b = kF16 ? __half2float(reinterpret_cast<const __half *>(k)[i]) : __uint_as_float((uint32_t)k[i] << 16);
-        s = fmaf(a, b, s);
-    }
-    return s;
 }
 
 template <bool kF16>
 __device__ __forceinline__ float one16(uint16_t x) {
     return kF16 ? __half2float(*reinterpret_cast<const __half *>(&x)) : __uint_as_float((uint32_t)x << 16);
+}
+
+// Adds to o (32 columns of a row of node t from `col` on, relative to maximum
+// m) the drafted nodes whose V rows were zeroed because a value is not finite,
+// where the row sees them.  Rare: everything is recomputed from global memory.
+template <int D, bool kF16>
+__device__ __noinline__ void add_odd(const TreeParams &p, const volatile Board *b, const uint32_t *odd, uint32_t P, uint32_t t,
+                                     size_t q_at, uint32_t col, float m, float *o) {
+    const uint32_t lo = b->t0 * BN, hi = lo + (b->packed & 0xfffffffu) * BN;
+    TreeSeq s;
+    s.first = b->first;
+    s.T = b->T;
+    for (uint32_t node = 0; node < s.T; ++node) {
+        const uint32_t pos = P + node;
+        if (!(odd[node >> 5] >> (node & 31) & 1) || pos < lo || pos >= hi || !tree_sees(p, s, t, node)) continue;
+        const uint32_t page = (uint32_t)p.table[(size_t)b->seq * p.max_pages + (pos >> p.page_shift)];
+        const size_t at = ((((size_t)page << p.page_shift) + (pos & ((1u << p.page_shift) - 1))) * p.n_kv + b->head) * D;
+        const uint16_t *q = static_cast<const uint16_t *>(p.q) + q_at, *k = static_cast<const uint16_t *>(p.k) + at;
+        float sc = 0.f;
+        for (int i = 0; i < D; ++i) sc = fmaf(one16<kF16>(q[i]), one16<kF16>(k[i]), sc);
+        const float w = fast_exp2(sc * p.scale_log2 - m);
+        for (int u = 0; u < 32; ++u) o[u] = fmaf(w, one16<kF16>(static_cast<const uint16_t *>(p.v)[at + col + u]), o[u]);
+    }
 }
 
 template <int D, bool kF16>
@@ -152,6 +206,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
             mbar_init(&sh.p_full[2 * x + 1], 4);
             mbar_init(&sh.o_final[x], 1);
         }
+        for (uint32_t i = 0; i < kBoard; ++i) mbar_init(&sh.seg_full[i], 1);
         mbar_init(&sh.drain, 1);
         sh.abort = 0u;
         fence_mbar_init();
@@ -172,92 +227,109 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
     const TreeRange range = tree_range(p, &sh.sched, blockIdx.x, gridDim.x);  // has the barriers for the set-up above
     tc_fence_after();
     const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may take its place; it waits for this grid
     TreeWalk walk(p, range);
-    TreeSeg sg;
+    TreeSeg sg = {};
 
-    if (warp == 0) {
-        // ------------------------------------------------------------- producer
-        uint32_t cnt = 0, tiles = 0, segs = 0;  // slots, tiles, segments so far
+    if (warp == 0 || warp == 10) {
+        // ------------------------------------------------------------- producers
+        // Warp 0 copies Q and K, warp 10 V.  A lane issues one box: 128-byte
+        // column block kb of part `part` of a tile.
+        const bool is_k = warp == 0;
+        const CUtensorMap *map = is_k ? &up.tk : &up.tv;
+        uint32_t tiles = 0, segs = 0;  // tiles, segments so far
+        uint32_t slot = 0, use = 0;    // ring position of the segment's next tile of either kind, and its use of the slot
         const uint32_t per_tile = BN / up.box_rows, part = lane / C::KB, kb = lane % C::KB;
         const uint32_t ps_mask = (1u << p.page_shift) - 1;
         const bool mine = part < per_tile;
-        auto wait_all = [&](uint64_t *bar, uint32_t parity) {
-            bool ok = mbar_wait(bar, parity, abort_flag, nullptr);
-            return __all_sync(0xffffffffu, ok);
-        };
         bool live = true;
+        auto wait_all = [&](uint64_t *bar, uint32_t parity) {
+            live = live && __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag));
+        };
+        auto index = [&](bool pair, uint32_t j, uint32_t n) { return is_k ? k_index(pair, j) : v_index(pair, j, n); };
+        auto advance = [&](uint32_t by) {  // at most 3
+            slot += by;
+            if (slot >= (uint32_t)C::SLOTS) {
+                slot -= C::SLOTS;
+                ++use;
+            }
+        };
+        auto publish = [&](uint32_t more) {
+            if (lane == 0) {
+                Board &b = sh.board[segs % kBoard];
+                if (more) b = Board{sg.seq, sg.s.first, sg.s.T, sg.s.L, sg.head, sg.row0, sg.t0, (sg.t1 - sg.t0) | sg.slot << 28 | 1u << 31};
+                else b.packed = 0u;
+                mbar_arrive(&sh.seg_full[segs % kBoard]);
+            }
+            __syncwarp();
+        };
         while (live && walk.next(p, sg)) {
             const bool pair = sg.rows > up.rt;
             const uint32_t n = sg.t1 - sg.t0;
-            if (segs > 0) live = wait_all(&sh.q_empty, (segs - 1) & 1u);
-            if (!live) break;
-            if (lane == 0) {
-                const uint32_t tile_rows = up.rt;
-                const uint32_t bytes = tile_rows * 128 * C::KB;
-                mbar_arrive_expect_tx(&sh.q_full, bytes * (pair ? 2 : 1));
-                const int tok = (int)(sg.s.first + sg.row0 / p.group);
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    if (x && !pair) break;
-#pragma unroll
-                    for (int b = 0; b < C::KB; ++b)
-                        tma_load_3d(smem + x * C::TILE + b * BM * 128, &up.tq, b * 64, (int)(sg.head * p.group),
-                                    tok + x * (int)(tile_rows / p.group), &sh.q_full);
-                }
-            }
             const int32_t *table = p.table + (size_t)sg.seq * p.max_pages;
-            // row of the pools where this lane's box of tile j starts; -1: past the length, -2: not in the pool
-            auto box_row = [&](uint32_t j) -> int {
-                const uint32_t pos = (sg.t0 + j) * BN + part * up.box_rows;
-                if (!mine || j >= n || pos >= sg.s.L) return -1;
+            // Table entries come 32 boxes at a time, one window ahead: lane l
+            // holds the first row of box 32 w + l of the segment (-1: past the
+            // length, -2: a page outside the pool).
+            auto window = [&](uint32_t w) -> int {
+                const uint32_t box = w * 32 + lane, pos = sg.t0 * BN + box * up.box_rows;
+                if (box >= n * per_tile || pos >= sg.s.L) return -1;
                 const uint32_t page = (uint32_t)table[pos >> p.page_shift];
                 return page < p.n_pages ? (int)((page << p.page_shift) + (pos & ps_mask)) : -2;
             };
-            auto issue = [&](bool is_k, int row) {
-                const uint32_t slot = cnt % C::SLOTS;
-                if (cnt >= (uint32_t)C::SLOTS && !wait_all(&sh.empty[slot], ((cnt / C::SLOTS) & 1u) ^ 1u)) return false;
+            int win = window(0), win_next = window(1);
+            if (!is_k) publish(1u);
+            if (is_k) {
+                if (segs > 0) wait_all(&sh.q_empty, (segs - 1) & 1u);
+                if (!live) break;
+                // Q: a box per row tile and column block
+                const uint32_t boxes = pair ? 2 * C::KB : C::KB;
+                if (lane == 0) mbar_arrive_expect_tx(&sh.q_full, boxes * up.rt * 128);
+                __syncwarp();
+                if (lane < boxes) {
+                    const uint32_t x = lane / C::KB, b = lane % C::KB;
+                    tma_load_3d(smem + x * C::TILE + b * BM * 128, &up.tq, (int)b * 64, (int)(sg.head * p.group),
+                                (int)(sg.s.first + (sg.row0 + x * up.rt) / p.group), &sh.q_full);
+                }
+                __syncwarp();
+            }
+            advance(index(pair, 0, n));
+            for (uint32_t j = 0; j < n && live; ++j) {
+                const uint32_t box = j * per_tile;
+                if (j > 0 && (box & 31) == 0) {
+                    win = win_next;
+                    win_next = window(box / 32 + 1);
+                }
+                int row = __shfl_sync(0xffffffffu, win, (box + part) & 31);
+                if (!mine) row = -1;
+                if (is_k) {
+                    const uint32_t bits = up.box_rows / 16;  // 16-position blocks of a box
+                    uint32_t flag = 0;
+                    if (__any_sync(0xffffffffu, row == -2))
+                        flag = __reduce_or_sync(0xffffffffu, row == -2 ? ((1u << bits) - 1) << (part * bits) : 0u);
+                    if (lane == 0) *(volatile uint32_t *)&sh.bad[(tiles + j) % kBadRing] = flag;
+                }
+                if (use > 0) wait_all(&sh.empty[slot], (use & 1u) ^ 1u);
+                if (!live) break;
                 const uint32_t boxes = __popc(__ballot_sync(0xffffffffu, row != -1));
                 if (lane == 0) mbar_arrive_expect_tx(&sh.full[slot], boxes * up.box_rows * 128);
                 __syncwarp();
                 // a page outside the pool is read past the map's end: zeros
                 if (row != -1)
-                    tma_load_3d(ring + slot * C::TILE + kb * BN * 128 + part * up.box_rows * 128, is_k ? &up.tk : &up.tv,
-                                (int)kb * 64, (int)sg.head, row == -2 ? (int)(p.n_pages << p.page_shift) : row, &sh.full[slot]);
-                ++cnt;
-                return true;
-            };
-            // rows of the tiles whose K, V come next; V trails K by one (two row tiles: none)
-            int row_k = box_row(0), row_v = row_k;
-            auto step_k = [&](uint32_t j) {
-                const uint32_t bits = up.box_rows / 16;  // 16-position blocks of a box
-                uint32_t flag = row_k == -2 ? ((1u << bits) - 1) << (part * bits) : 0u;
-                flag = __reduce_or_sync(0xffffffffu, flag);
-                if (lane == 0) *(volatile uint32_t *)&sh.bad[(tiles + j) % kBadRing] = flag;
+                    tma_load_3d(ring + slot * C::TILE + kb * BN * 128 + part * up.box_rows * 128, map, (int)kb * 64,
+                                (int)sg.head, row == -2 ? (int)(p.n_pages << p.page_shift) : row, &sh.full[slot]);
                 __syncwarp();
-                return issue(true, row_k);
-            };
-            if (pair) {
-                for (uint32_t j = 0; j < n && live; ++j) {
-                    live = step_k(j);
-                    row_v = row_k;
-                    row_k = box_row(j + 1);
-                    live = live && issue(false, row_v);
-                }
-            } else {
-                live = step_k(0);
-                for (uint32_t j = 0; j < n && live; ++j) {
-                    row_v = row_k;
-                    row_k = box_row(j + 1);
-                    if (j + 1 < n) live = step_k(j + 1);
-                    live = live && issue(false, row_v);
-                }
+                advance(j + 1 < n ? index(pair, j + 1, n) - index(pair, j, n) : 2 * n - index(pair, j, n));
             }
             tiles += n;
             ++segs;
         }
-        // no copy may outlive the CTA (all have landed unless a wait gave up)
-        for (uint32_t i = cnt > (uint32_t)C::SLOTS ? cnt - C::SLOTS : 0; i < cnt; ++i)
-            mbar_drain(&sh.full[i % C::SLOTS], (i / C::SLOTS) & 1u, kWaitNs);
+        if (!is_k) publish(0u);
+        // No copy may outlive the CTA: all have landed unless a wait gave up,
+        // and then none is issued any more, so those that have not will soon.
+        if (!live) {
+            const uint64_t t0 = globaltimer_ns();
+            while (globaltimer_ns() - t0 < 1000000ull) {}
+        }
         __syncwarp();
     } else if (warp == 1) {
         // ------------------------------------------------------------- MMA issuer
@@ -267,84 +339,174 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
         const uint64_t dq = smem_desc(smem_u32(smem), 16, 1024);
         const uint64_t dk = smem_desc(smem_u32(ring), 16, 1024);
         const uint64_t dv = smem_desc(smem_u32(ring), BN * 128, 1024);
-        uint32_t cnt = 0, segs = 0;
-        uint32_t done[2] = {0, 0};  // tiles of each chain so far
+        // Slots are read in ring order; cur is the next one.
+        struct Cursor {
+            uint32_t slot, phase;
+            __device__ __forceinline__ Cursor next() {
+                const Cursor c = *this;
+                if (++slot == (uint32_t)C::SLOTS) {
+                    slot = 0;
+                    phase ^= 1u;
+                }
+                return c;
+            }
+        };
+        Cursor cur = {0, 0};
+        uint32_t segs = 0, par = 0;  // par bit x: phase parity of chain x's P barriers
         bool live = true;
-        auto gate = [&](uint64_t *bar, uint32_t parity) {
-            live = live && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, nullptr));
+        // Before the last MMA of a block the barriers of the next block are
+        // tested, so that a block whose operands are there follows without a gap.
+        struct Gate {  // one or two barrier phases; b0 null: none
+            uint64_t *b0;
+            uint32_t p0;
+            uint64_t *b1;
+            uint32_t p1;
+        };
+        const Gate none = {nullptr, 0u, nullptr, 0u};
+        auto full = [&](const Cursor &c) { return Gate{&sh.full[c.slot], c.phase, nullptr, 0u}; };
+        auto p_half = [&](uint32_t x, uint32_t h) { return Gate{&sh.p_full[2 * x + h], par >> x & 1u, nullptr, 0u}; };
+        auto gate_test = [&](const Gate &g) {
+            bool ok = g.b0 == nullptr || mbar_test_wait(g.b0, g.p0);
+            if (g.b1) ok = ok & mbar_test_wait(g.b1, g.p1);
+            return ok;
+        };
+        auto gate_wait = [&](const Gate &g, bool ready) {
+            if (!ready) {
+                bool ok = true;
+                if (g.b0) ok = wait_bar(g.b0, g.p0, abort_flag);
+                if (g.b1) ok = wait_bar(g.b1, g.p1, abort_flag) && ok;
+                live = live && __all_sync(0xffffffffu, ok);
+            }
             __syncwarp();
             tc_fence_after();
         };
-        while (live && walk.next(p, sg)) {
-            const bool pair = sg.rows > up.rt;
-            const uint32_t n = sg.t1 - sg.t0;
-            const uint32_t nt[2] = {pair ? n : (n + 1) / 2, pair ? n : n / 2};
-            auto tile = [&](uint32_t x, uint32_t i) { return pair ? i : 2 * i + x; };
-            auto qk = [&](uint32_t x, uint32_t i) {
-                const uint32_t c = cnt + k_index(pair, tile(x, i)), slot = c % C::SLOTS;
-                gate(&sh.full[slot], (c / C::SLOTS) & 1u);
-                if (!live) return;
-                const uint64_t a0 = dq + ((pair ? x * C::TILE : 0) >> 4), b0 = dk + ((slot * C::TILE) >> 4);
-                const uint32_t d = tmem + x * 128;
+        // S of chain x from Q tile qt and the K tile in slot k
+        auto qk = [&](uint32_t x, uint32_t qt, uint32_t k, bool release, bool last, const Gate &next) {
+            const uint64_t a0 = dq + ((qt * C::TILE) >> 4), b0 = dk + ((k * C::TILE) >> 4);
+            const uint32_t d = tmem + x * 128;
+            bool ready = true;
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t off = ((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4;
-                    if (elect_one()) tc_mma_ss(d, a0 + off, b0 + off, idesc_qk, kk > 0);
-                    __syncwarp();
-                }
-                if (elect_one()) {
-                    tc_commit(&sh.s_full[x]);
-                    if (!pair || x == 1) tc_commit(&sh.empty[slot]);
-                }
+            for (int kk = 0; kk < D / 16; ++kk) {
+                if (kk == D / 16 - 1) ready = gate_test(next);
+                const uint32_t off = ((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4;
+                if (elect_one()) tc_mma_ss(d, a0 + off, b0 + off, idesc_qk, kk > 0);
                 __syncwarp();
-            };
-            auto pv = [&](uint32_t x, uint32_t i) {
-                const uint32_t c = cnt + v_index(pair, tile(x, i), n), slot = c % C::SLOTS;
-                const uint64_t b0 = dv + ((slot * C::TILE) >> 4);
-                const uint32_t d = tmem + C::O_COL0 + x * D, a = tmem + x * 128;
-                const uint32_t par = (done[x] + i) & 1u;
-                gate(&sh.full[slot], (c / C::SLOTS) & 1u);
+            }
+            if (elect_one()) {
+                tc_commit(&sh.s_full[x]);
+                if (release) tc_commit(&sh.empty[k]);
+                if (last) tc_commit(&sh.q_empty);  // the segment's Q has been read
+            }
+            __syncwarp();
+            return ready;
+        };
+        // O of chain x += P V over positions 64 h .. 64 h + 63 of the V tile in slot v
+        auto pv = [&](uint32_t x, uint32_t v, int h, uint32_t acc, const Gate &next) {
+            const uint64_t b0 = dv + ((v * C::TILE) >> 4);
+            const uint32_t d = tmem + C::O_COL0 + x * D, a = tmem + x * 128;
+            bool ready = true;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    gate(&sh.p_full[2 * x + h], par);
-                    if (!live) return;
-#pragma unroll
-                    for (int k4 = 0; k4 < BN / 32; ++k4) {
-                        const int kk = h * (BN / 32) + k4;
-                        if (elect_one())
-                            tc_mma_ts(d, a + kk * 8, b0 + ((kk * 16 * 128) >> 4), idesc_pv, (kk > 0 || i > 0) ? 1u : 0u);
-                        __syncwarp();
+            for (int k4 = 0; k4 < BN / 32; ++k4) {
+                const int kk = h * (BN / 32) + k4;
+                if (k4 == BN / 32 - 1) ready = gate_test(next);
+                if (elect_one()) tc_mma_ts(d, a + kk * 8, b0 + ((kk * 16 * 128) >> 4), idesc_pv, kk > 0 ? 1u : acc);
+                __syncwarp();
+            }
+            return ready;
+        };
+        auto pv_done = [&](uint32_t x, uint32_t v, bool release, bool last) {
+            if (elect_one()) {
+                if (release) tc_commit(&sh.empty[v]);
+                if (last) tc_commit(&sh.o_final[x]);
+            }
+            __syncwarp();
+        };
+        while (live && walk.next(p, sg)) {
+            const uint32_t n = sg.t1 - sg.t0;
+            Cursor k = cur.next();
+            gate_wait(Gate{&sh.q_full, segs & 1u, &sh.full[k.slot], k.phase}, false);
+            if (!live) break;
+            if (sg.rows > up.rt) {
+                // two row tiles: per K/V tile PV_A, S_A of the next, PV_B, S_B of the next
+                qk(0, 0, k.slot, false, false, none);
+                Cursor v = cur.next();
+                Gate gv = {&sh.full[v.slot], v.phase, &sh.p_full[0], par & 1u};
+                bool ready = qk(1, 1, k.slot, true, n == 1, gv);
+                for (uint32_t i = 0; i < n; ++i) {
+                    const bool more = i + 1 < n;
+                    const uint32_t acc = i > 0;
+                    gate_wait(gv, ready);
+                    if (!live) break;
+                    Gate g = p_half(0, 1);
+                    gate_wait(g, pv(0, v.slot, 0, acc, g));
+                    if (!live) break;
+                    Gate gb = p_half(1, 0);
+                    if (more) {
+                        k = cur.next();
+                        g = full(k);
+                        ready = pv(0, v.slot, 1, acc, g);
+                        gate_wait(g, ready);
+                        if (!live) break;
+                        ready = qk(0, 0, k.slot, false, false, gb);
+                    } else {
+                        ready = pv(0, v.slot, 1, acc, gb);
+                        pv_done(0, v.slot, false, true);
+                    }
+                    gate_wait(gb, ready);
+                    if (!live) break;
+                    g = p_half(1, 1);
+                    gate_wait(g, pv(1, v.slot, 0, acc, g));
+                    if (!live) break;
+                    pv(1, v.slot, 1, acc, none);
+                    pv_done(1, v.slot, true, !more);
+                    par ^= 3u;
+                    if (more) {
+                        v = cur.next();
+                        gv = {&sh.full[v.slot], v.phase, &sh.p_full[0], par & 1u};
+                        ready = qk(1, 1, k.slot, true, i + 2 == n, gv);
                     }
                 }
-                if (elect_one()) {
-                    if (!pair || x == 1) tc_commit(&sh.empty[slot]);
-                    if (i + 1 == nt[x]) tc_commit(&sh.o_final[x]);
+            } else {
+                // one row tile: chain j & 1 takes tile j; PV(j), then S(j + 2)
+                bool ready;
+                if (n > 1) {
+                    const Cursor k1 = cur.next();
+                    const Gate g = full(k1);
+                    gate_wait(g, qk(0, 0, k.slot, true, false, g));
+                    if (!live) break;
+                    k = k1;
                 }
-                __syncwarp();
-            };
-            gate(&sh.q_full, segs & 1u);
-            uint32_t left = nt[0] + nt[1];  // S still to issue
-            auto qk_last = [&](uint32_t x, uint32_t i) {
-                qk(x, i);
-                if (--left == 0) {  // the segment's Q has been read once this commit's MMAs are done
-                    if (elect_one()) tc_commit(&sh.q_empty);
-                    __syncwarp();
-                }
-            };
-            if (live) qk_last(0, 0);
-            if (live && nt[1]) qk_last(1, 0);
-            for (uint32_t i = 0; i < nt[0] && live; ++i) {
-#pragma unroll
-                for (uint32_t x = 0; x < 2; ++x) {
-                    if (i < nt[x] && live) {
-                        pv(x, i);
-                        if (i + 1 < nt[x] && live) qk_last(x, i + 1);
+                Cursor v = cur.next();
+                Gate gv = {&sh.full[v.slot], v.phase, &sh.p_full[0], par & 1u};
+                ready = qk(n > 1 ? 1 : 0, 0, k.slot, true, n < 3, gv);
+                for (uint32_t j = 0; j < n; ++j) {
+                    const uint32_t x = j & 1u, acc = j > 1;
+                    gate_wait(gv, ready);
+                    if (!live) break;
+                    const Gate g = p_half(x, 1);
+                    gate_wait(g, pv(x, v.slot, 0, acc, g));
+                    if (!live) break;
+                    const bool more = j + 2 < n;
+                    const uint32_t vs = v.slot;
+                    Gate gk = none;
+                    if (more) {
+                        k = cur.next();
+                        gk = full(k);
+                    }
+                    ready = pv(x, vs, 1, acc, gk);
+                    pv_done(x, vs, true, !more);
+                    par ^= 1u << x;
+                    if (more) {
+                        gate_wait(gk, ready);
+                        if (!live) break;
+                    }
+                    if (j + 1 < n) {
+                        v = cur.next();
+                        gv = {&sh.full[v.slot], v.phase, &sh.p_full[2 * (x ^ 1u)], par >> (x ^ 1u) & 1u};
+                        ready = more ? qk(x, 0, k.slot, true, j + 3 == n, gv) : gate_test(gv);
                     }
                 }
             }
-            cnt += 2 * n;
-            done[0] += nt[0];
-            done[1] += nt[1];
             ++segs;
         }
         if (elect_one()) tc_commit(&sh.drain);  // no MMA outlives the CTA
@@ -360,22 +522,26 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
         const uint32_t o_base = tmem + lane_addr + C::O_COL0;
         const uint32_t o_col = o_base + x * D;
         const float c = p.scale_log2;
-        uint32_t cnt = 0, tiles = 0, done = 0, finals = 0, finals_other = 0;
-        while (walk.next(p, sg)) {
-            const bool pair = sg.rows > up.rt;
-            const uint32_t n = sg.t1 - sg.t0;
+        uint32_t cnt = 0, tiles = 0, done = 0, segs = 0;
+        uint32_t finals = 0;  // bit x: phase parity of o_final[x]
+        while (true) {
+            if (!wait_bar(&sh.seg_full[segs % kBoard], (segs / kBoard) & 1u, abort_flag)) break;
+            const volatile Board *b = &sh.board[segs % kBoard];
+            const uint32_t packed = b->packed, n = packed & 0xfffffffu, slot_of = packed >> 28 & 7u;
+            if (packed == 0u) break;
+            const uint32_t rows = min(b->T * p.group - b->row0, p.rpg);
+            const bool pair = rows > up.rt;
             const uint32_t nt = pair ? n : (x ? n / 2 : (n + 1) / 2);
-            const uint32_t row = (pair ? x * up.rt : 0) + r;      // row of the group
-            const bool valid = r < up.rt && row < sg.rows;
+            const uint32_t row = (pair ? x * up.rt : 0) + r;  // row of the group
+            const bool valid = r < up.rt && row < rows;
             const bool warp_live = __any_sync(0xffffffffu, valid);
-            const uint32_t t = min((sg.row0 + row) / p.group, sg.s.T - 1);
-            const uint32_t P = sg.s.L - min(sg.s.T, sg.s.L);
+            const uint32_t P = b->L - min(b->T, b->L), kv_first = b->t0 * BN;
             float m_run = -INFINITY, l_run = 0.f;
 
             for (uint32_t i = 0; i < nt; ++i) {
                 const uint32_t j = pair ? i : 2 * i + x;
-                const uint32_t kv0 = (sg.t0 + j) * BN;
-                mbar_wait(&sh.s_full[x], (done + i) & 1u, abort_flag, nullptr);
+                const uint32_t kv0 = kv_first + j * BN;
+                wait_bar(&sh.s_full[x], (done + i) & 1u, abort_flag);
                 __syncwarp();
                 tc_fence_after();
                 const uint32_t bad = *(volatile uint32_t *)&sh.bad[(tiles + j) % kBadRing];
@@ -385,13 +551,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
                     // V rows that must not be read as they are: this thread's row is kv0 + r
                     const uint32_t pos = kv0 + r, cv = cnt + v_index(pair, j, n), slot = cv % C::SLOTS;
                     if (__any_sync(0xffffffffu, pos >= P)) {
-                        mbar_wait(&sh.full[slot], (cv / C::SLOTS) & 1u, abort_flag, nullptr);
+                        wait_bar(&sh.full[slot], (cv / C::SLOTS) & 1u, abort_flag);
                         uint8_t *vrow = ring + slot * C::TILE + r * 128;
-                        bool zero = pos >= sg.s.L;
+                        bool zero = pos >= b->L;
                         if (pos >= P && !zero) {
                             constexpr uint32_t em = kF16 ? 0x7c00u : 0x7f80u;
                             bool odd = false;
-#pragma unroll
+#pragma unroll 4
                             for (int u = 0; u < C::KB * 8; ++u) {
                                 const uint4 w = lds128(vrow + (u >> 3) * BN * 128 + ((u + lane) & 7) * 16);
                                 const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
@@ -405,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
                             }
                         }
                         if (zero) {
-#pragma unroll
+#pragma unroll 4
                             for (int u = 0; u < C::KB * 8; ++u)
                                 *reinterpret_cast<uint4 *>(vrow + (u >> 3) * BN * 128 + ((u + lane) & 7) * 16) =
                                     make_uint4(0, 0, 0, 0);
@@ -428,15 +594,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
                 for (int cc = 0; cc < BN / 32; ++cc) tmem_ld32(s_col + cc * 32, sv + cc * 32);
                 tmem_wait_ld();
                 if (edge || bad) {
+                    uint32_t see[4];
+                    see_tile(p, b, row, (int32_t)(kv0 - P), edge, bad, see);
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        uint32_t see = edge ? see32(p, sg.s, t, (int32_t)(kv0 + 32 * w) - (int32_t)P) : 0xffffffffu;
-                        if (bad >> (2 * w) & 1) see &= 0xffff0000u;
-                        if (bad >> (2 * w + 1) & 1) see &= 0x0000ffffu;
+                    for (int w = 0; w < 4; ++w)
 #pragma unroll
-                        for (int b = 0; b < 32; ++b)
-                            if (!(see >> b & 1)) sv[w * 32 + b] = -INFINITY;
-                    }
+                        for (int k = 0; k < 32; ++k)
+                            if (!(see[w] >> k & 1)) sv[w * 32 + k] = -INFINITY;
                 }
                 float mx8[8];
 #pragma unroll
@@ -447,8 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
                     mx8[k] = fmaxf(a, sv[k + BN - 8]);
                 }
                 const float mh = fmax3(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
-                // scale >= 0; with scale 0 a row that sees something has maximum 0
-                const float m_tile = mh == -INFINITY ? -INFINITY : mh * c;
+                const float m_tile = mh * c;  // c > 0
                 float m_new = m_run;
                 if (m_run == -INFINITY || m_tile > m_run + kRescaleThreshold) m_new = fmaxf(m_run, m_tile);
                 const float m_use = (m_new == -INFINITY) ? 0.f : m_new;
@@ -456,6 +619,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
                 const bool rescale = (i > 0) && (m_new != m_run);
                 m_run = m_new;
 
+                // P = 2^(s c - m) over S as packed 16-bit pairs, in two halves,
+                // each released to the MMA warp as soon as it is written
                 const float2 c2 = make_float2(c, c), nm2 = make_float2(-m_use, -m_use);
                 float2 sum4[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
@@ -480,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
                     }
                     if (hv == 0 && __any_sync(0xffffffffu, rescale)) {
                         const float a = rescale ? alpha : 1.f;
-#pragma unroll
+#pragma unroll 1
                         for (int cc = 0; cc < D / 32; ++cc) {
                             float o[32];
                             tmem_ld32(o_col + cc * 32, o);
@@ -501,94 +666,72 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
             if (m_run == -INFINITY && l_run == l_run) l_run = 0.f;  // saw nothing (a NaN stays)
 
             // --------------------------------------------------------- epilogue
-            // One row tile: both chains' (m, l) meet in shared memory; chain x
+            // Row = wa * O_A + wb * O_B, un-normalised, with maximum m and sum l.
+            // One row tile: both chains' (m, l) meet in shared memory, and chain x
             // writes columns x * D / 2 .. of the joined row.
-            float wa, wb, m, l;  // row = wa * O_A + wb * O_B, un-normalised
+            float wa, wb, m = m_run, l = l_run;
             if (pair) {
-                mbar_wait(&sh.o_final[x], finals & 1u, abort_flag, nullptr);
-                wa = x == 0 && m_run > -INFINITY ? 1.f : 0.f;
-                wb = x == 1 && m_run > -INFINITY ? 1.f : 0.f;
-                m = m_run;
-                l = l_run;
+                wait_bar(&sh.o_final[x], (finals >> x) & 1u, abort_flag);
+                wa = m_run == -INFINITY ? 0.f : 1.f;
+                wb = 0.f;
             } else {
                 sh.ml[x * 128 + r] = make_float2(m_run, l_run);
-                mbar_wait(&sh.o_final[0], (x == 0 ? finals : finals_other) & 1u, abort_flag, nullptr);
-                if (n > 1) mbar_wait(&sh.o_final[1], (x == 1 ? finals : finals_other) & 1u, abort_flag, nullptr);
+                wait_bar(&sh.o_final[0], finals & 1u, abort_flag);
+                if (n > 1) wait_bar(&sh.o_final[1], finals >> 1 & 1u, abort_flag);
                 __syncwarp();
                 named_bar_sync(1, 256);
-                const float2 a = sh.ml[r], b = sh.ml[128 + r];
-                m = fmaxf(a.x, b.x);
-                wa = a.x == -INFINITY ? 0.f : fast_exp2(a.x - m);
-                wb = n < 2 || b.x == -INFINITY ? 0.f : fast_exp2(b.x - m);
-                l = wa * a.y + wb * b.y;
+                const float2 ma = sh.ml[r], mb = sh.ml[128 + r];
+                m = fmaxf(ma.x, mb.x);
+                wa = ma.x == -INFINITY ? 0.f : fast_exp2(ma.x - m);
+                wb = mb.x == -INFINITY ? 0.f : fast_exp2(mb.x - m);  // no tiles: -inf
+                l = wa * ma.y + wb * mb.y;
             }
             __syncwarp();
             tc_fence_after();
             const bool gave_up = *abort_flag != 0u;
-            const float inv = gave_up ? __int_as_float(0x7fffffff) : l == 0.f ? 0.f : 1.f / l;
-            const uint32_t tt = (sg.row0 + row) / p.group;
-            const size_t at = valid ? tree_row(p, sg, sg.row0 + row, D) : 0;
-            float *part = sg.slot < 2 ? tree_part(p, D, blockIdx.x, sg.slot) : nullptr;
-            const uint32_t first_cc = pair ? 0u : x * (D / 64), n_cc = pair ? D / 32 : D / 64;
+            if (gave_up) l = __int_as_float(0x7fffffff);
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const uint32_t gr = b->row0 + row, t = gr / p.group;  // node; q head gr - t * group of the kv head
+            const size_t at = valid ? ((size_t)(b->first + t) * p.n_heads + (size_t)b->head * p.group + (gr - t * p.group)) * D : 0;
+            float *part = slot_of < 2 ? tree_part(p, D, blockIdx.x, slot_of) : nullptr;
+            uint32_t any_odd = 0;
+            if (kv_first + n * BN > P)
+#pragma unroll
+                for (int w = 0; w < 8; ++w) any_odd |= *(volatile uint32_t *)&sh.odd[w];
             if (warp_live) {
+                const uint32_t first = pair ? 0u : x * (D / 2), n_cols = pair ? D : D / 2;
+                const uint32_t src0 = pair ? o_col : o_base;
 #pragma unroll 1
-                for (uint32_t k = 0; k < n_cc; ++k) {
-                    const uint32_t cc = first_cc + k;
+                for (uint32_t col = first; col < first + n_cols; col += 32) {
                     float o[32];
                     __syncwarp();
-                    if (pair) {
-                        tmem_ld32(o_col + cc * 32, o);
-                        tmem_wait_ld();
-                        const float w = wa + wb;
+                    tmem_ld32(src0 + col, o);
+                    tmem_wait_ld();
 #pragma unroll
-                        for (int u = 0; u < 32; ++u) o[u] = w == 0.f ? 0.f : o[u];
-                    } else {
+                    for (int u = 0; u < 32; ++u) o[u] = wa == 0.f ? 0.f : o[u] * wa;
+                    if (__any_sync(0xffffffffu, wb != 0.f)) {
                         float o2[32];
-                        tmem_ld32(o_base + cc * 32, o);
-                        tmem_ld32(o_base + D + cc * 32, o2);
+                        tmem_ld32(o_base + D + col, o2);
                         tmem_wait_ld();
+                        if (wb != 0.f)
 #pragma unroll
-                        for (int u = 0; u < 32; ++u) {
-                            o[u] = wa == 0.f ? 0.f : o[u] * wa;
-                            if (wb != 0.f) o[u] = fmaf(o2[u], wb, o[u]);
-                        }
+                            for (int u = 0; u < 32; ++u) o[u] = fmaf(o2[u], wb, o[u]);
                     }
-                    // nodes whose V was zeroed because a value is not finite
-                    for (uint32_t node = 0; node < sg.s.T; ++node) {
-                        if ((node & 31) == 0 && sh.odd[node >> 5] == 0u) {
-                            node += 31;
-                            continue;
+                    if (valid) {
+                        if (any_odd) add_odd<D, kF16>(p, b, sh.odd, P, t, at, col, m, o);
+                        if (part) {
+                            float4 *dst = reinterpret_cast<float4 *>(part + (size_t)row * D + col);
+#pragma unroll
+                            for (int u = 0; u < 8; ++u) dst[u] = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                        } else {
+                            uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + at + col);
+#pragma unroll
+                            for (int u = 0; u < 4; ++u)
+                                dst[u] = make_uint4(pack2<kF16>(o[8 * u] * inv, o[8 * u + 1] * inv),
+                                                    pack2<kF16>(o[8 * u + 2] * inv, o[8 * u + 3] * inv),
+                                                    pack2<kF16>(o[8 * u + 4] * inv, o[8 * u + 5] * inv),
+                                                    pack2<kF16>(o[8 * u + 6] * inv, o[8 * u + 7] * inv));
                         }
-                        const uint32_t pos = P + node;
-                        if (!(sh.odd[node >> 5] >> (node & 31) & 1) || pos < sg.t0 * BN || pos >= sg.t1 * BN) continue;
-                        if (!valid || !tree_sees(p, sg.s, tt, node)) continue;
-                        const uint32_t page = (uint32_t)p.table[(size_t)sg.seq * p.max_pages + (pos >> p.page_shift)];
-                        const size_t kvrow = ((((size_t)page << p.page_shift) + (pos & ((1u << p.page_shift) - 1))) * p.n_kv + sg.head) * D;
-                        const float s = rare_score<D, kF16>(static_cast<const uint16_t *>(p.q) + at, static_cast<const uint16_t *>(p.k) + kvrow);
-                        const float w = fast_exp2(s * c - m);
-#pragma unroll 1
-                        for (int u = 0; u < 32; ++u) {
-                            const float v = one16<kF16>(static_cast<const uint16_t *>(p.v)[kvrow + cc * 32 + u]);
-                            const float y = w * v;
-#pragma unroll
-                            for (int z = 0; z < 32; ++z)
-                                if (z == u) o[z] += y;
-                        }
-                    }
-                    if (valid && part) {
-                        float4 *dst = reinterpret_cast<float4 *>(part + (size_t)row * D + cc * 32);
-                        const float poison = gave_up ? inv : 1.f;
-#pragma unroll
-                        for (int u = 0; u < 8; ++u)
-                            dst[u] = make_float4(o[4 * u] * poison, o[4 * u + 1] * poison, o[4 * u + 2] * poison, o[4 * u + 3] * poison);
-                    } else if (valid) {
-                        uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + at + cc * 32);
-#pragma unroll
-                        for (int u = 0; u < 4; ++u)
-                            dst[u] = make_uint4(pack2<kF16>(o[8 * u] * inv, o[8 * u + 1] * inv),
-                                                pack2<kF16>(o[8 * u + 2] * inv, o[8 * u + 3] * inv),
-                                                pack2<kF16>(o[8 * u + 4] * inv, o[8 * u + 5] * inv),
-                                                pack2<kF16>(o[8 * u + 6] * inv, o[8 * u + 7] * inv));
                     }
                 }
                 if (valid && part && (pair || x == 0)) {
@@ -600,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
             __syncwarp();
             // The next segment's first P.V may overwrite O, its ml and odd words
             // be set, once both chains are here.
-            const bool had_edge = sg.t1 * BN > P;
+            const bool had_edge = kv_first + n * BN > P;
             if (!pair || had_edge) named_bar_sync(1, 256);
             if (had_edge) {
                 if (threadIdx.x >= 64 && threadIdx.x < 72) sh.odd[threadIdx.x - 64] = 0u;
@@ -610,8 +753,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
             cnt += 2 * n;
             tiles += n;
             done += nt;
-            if (nt) ++finals;
-            if (pair || (x == 0 ? n / 2 : (n + 1) / 2)) ++finals_other;
+            finals ^= pair || n > 1 ? 3u : 1u;  // chains that had tiles
+            ++segs;
         }
     }
 
