@@ -208,6 +208,7 @@ BML_API bml_status bml_attn_tree(const void *q_dev, bml_dtype q_dtype, uint32_t 
     a.D = head_dim;
     a.kv_type = kv_dtype;
     a.num_sms = sms;
+    a.rows = (uint32_t)((uint64_t)n_tokens * (n_heads / n_kv_heads) / n_seqs);
     bml::TreeParams &p = a.p;
     p.q = q_dev;
     p.out = out_dev;

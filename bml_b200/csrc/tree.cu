@@ -41,25 +41,23 @@ __device__ __forceinline__ void mma_tf32(float *d, const uint32_t *a, uint32_t b
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// 16 bytes global -> shared; bytes = 0 writes zeros and reads nothing.
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src, uint32_t bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 __device__ __forceinline__ float load_q(const void *q, int type, size_t i) {
     if (type == BML_F32) return static_cast<const float *>(q)[i];
     if (type == BML_F16) return __half2float(static_cast<const __half *>(q)[i]);
     return __bfloat162float(static_cast<const __nv_bfloat16 *>(q)[i]);
 }
-__device__ __forceinline__ void store_out(void *out, int type, size_t i, float x) {
-    if (type == BML_F32) static_cast<float *>(out)[i] = x;
-    else if (type == BML_F16) static_cast<__half *>(out)[i] = __float2half_rn(x);
-    else static_cast<__nv_bfloat16 *>(out)[i] = __float2bfloat16_rn(x);
+__device__ __forceinline__ void store_out4(void *out, int type, size_t i, float4 x) {
+    if (type == BML_F32) {
+        *reinterpret_cast<float4 *>(static_cast<float *>(out) + i) = x;
+    } else if (type == BML_F16) {
+        const __half2 a = __floats2half2_rn(x.x, x.y), b = __floats2half2_rn(x.z, x.w);
+        *reinterpret_cast<uint2 *>(static_cast<__half *>(out) + i) =
+            make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    } else {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(x.x, x.y), b = __floats2bfloat162_rn(x.z, x.w);
+        *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(out) + i) =
+            make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
+    }
 }
 
 // RW warps cover RW * 16 rows; the 8 / RW groups of RW warps take turns at
@@ -343,9 +341,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
         // joined over the groups: thread (row, 4 dims)
         float *part = sg.slot < 2 ? tree_part(p, D, blockIdx.x, sg.slot) : nullptr;
         for (int i = threadIdx.x; i < RW * 16 * (D / 4); i += kThreads) {
-            const uint32_t r = i / (D / 4);
-            const int x4 = i % (D / 4);
-            if (r >= sg.rows) break;
+            const uint32_t r = i % (RW * 16);
+            const int x4 = i / (RW * 16);
+            if (r >= sg.rows) continue;
             const float *src = reinterpret_cast<float *>(ring) + ((size_t)(r / 16) * 16 + r % 16) * OS;
             constexpr size_t GS = (size_t)RW * 16 * OS;
             float m = -INFINITY;
@@ -366,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
                 acc.w += f * y.w;
             }
             if (part) {
-                *reinterpret_cast<float4 *>(part + (size_t)r * D + x4 * 4) = acc;
+                reinterpret_cast<float4 *>(part)[x4 * p.rpg + r] = acc;
                 if (x4 == 0) {
                     part[(size_t)p.rpg * D + r] = m;
                     part[(size_t)p.rpg * (D + 1) + r] = l;
@@ -374,10 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
             } else {
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 const size_t at = tree_row(p, sg, sg.row0 + r, D) + x4 * 4;
-                store_out(p.out, p.q_type, at, acc.x * inv);
-                store_out(p.out, p.q_type, at + 1, acc.y * inv);
-                store_out(p.out, p.q_type, at + 2, acc.z * inv);
-                store_out(p.out, p.q_type, at + 3, acc.w * inv);
+                store_out4(p.out, p.q_type, at, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
             }
         }
         __syncthreads();
@@ -406,61 +401,34 @@ __global__ void __launch_bounds__(kThreads) tree_merge_kernel(const __grid_const
     if (tree_cut(range.total, b - 1, range.active) > u0) return;  // an earlier cut is inside the unit
     uint32_t last = b;  // last CTA with a segment of the unit
     while (last + 1 < range.active && tree_cut(range.total, last + 1, range.active) < u1) ++last;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr int V = D / 32;  // values of a lane
-    // A lane holds V values of kRows rows at a time; the loads of up to 8
-    // segments are in flight together.
-    constexpr int kRows = 2;
-    for (uint32_t r0 = (blockIdx.y * kWarps + warp) * kRows; r0 < sg.rows; r0 += gridDim.y * kWarps * kRows) {
-        float m[kRows], acc[kRows][V], l[kRows];
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            m[i] = -INFINITY;
-            l[i] = 0.f;
-#pragma unroll
-            for (int v = 0; v < V; ++v) acc[i][v] = 0.f;
-        }
-        for (uint32_t s = b - 1 + lane; s <= last; s += 32) {
-            const float *part = tree_part(p, D, s, s == b - 1 ? 1u : 0u) + (size_t)p.rpg * D;
-#pragma unroll
-            for (int i = 0; i < kRows; ++i)
-                if (r0 + i < sg.rows) m[i] = fmaxf(m[i], part[r0 + i]);
-        }
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-#pragma unroll
-            for (int x = 16; x > 0; x >>= 1) m[i] = fmaxf(m[i], __shfl_xor_sync(0xffffffffu, m[i], x));
-            if (m[i] == -INFINITY) m[i] = 0.f;
-        }
+    // A warp takes 8 rows x 16 columns at a time (lane: row, 4 columns); the
+    // loads of up to 8 segments are in flight together.
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t tasks = (sg.rows + 7) / 8 * (D / 16);
+    for (uint32_t task = blockIdx.y * kWarps + warp; task < tasks; task += gridDim.y * kWarps) {
+        const uint32_t r = task / (D / 16) * 8 + (lane & 7), x4 = task % (D / 16) * 4 + (lane >> 3);
+        if (r >= sg.rows) continue;
+        float m = -INFINITY;
+#pragma unroll 8
+        for (uint32_t s = b - 1; s <= last; ++s)
+            m = fmaxf(m, tree_part(p, D, s, s == b - 1 ? 1u : 0u)[(size_t)p.rpg * D + r]);
+        if (m == -INFINITY) m = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.f;
 #pragma unroll 8
         for (uint32_t s = b - 1; s <= last; ++s) {
             const float *part = tree_part(p, D, s, s == b - 1 ? 1u : 0u);
-#pragma unroll
-            for (int i = 0; i < kRows; ++i) {
-                const uint32_t r = min(r0 + i, sg.rows - 1);
-                const float f = exp2f(part[(size_t)p.rpg * D + r] - m[i]);
-                l[i] += f * part[(size_t)p.rpg * (D + 1) + r];
-                if (V == 4) {
-                    const float4 y = *reinterpret_cast<const float4 *>(part + (size_t)r * D + lane * 4);
-                    acc[i][0] += f * y.x;
-                    acc[i][1] += f * y.y;
-                    acc[i][V > 2 ? 2 : 0] += f * y.z;
-                    acc[i][V > 2 ? 3 : 1] += f * y.w;
-                } else {
-                    const float2 y = *reinterpret_cast<const float2 *>(part + (size_t)r * D + lane * 2);
-                    acc[i][0] += f * y.x;
-                    acc[i][1] += f * y.y;
-                }
-            }
+            const float f = exp2f(part[(size_t)p.rpg * D + r] - m);
+            const float4 y = reinterpret_cast<const float4 *>(part)[x4 * p.rpg + r];
+            l += f * part[(size_t)p.rpg * (D + 1) + r];
+            acc.x += f * y.x;
+            acc.y += f * y.y;
+            acc.z += f * y.z;
+            acc.w += f * y.w;
         }
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            if (r0 + i >= sg.rows) break;
-            const float inv = l[i] == 0.f ? 0.f : 1.f / l[i];
-            const size_t at = tree_row(p, sg, sg.row0 + r0 + i, D) + lane * V;
-#pragma unroll
-            for (int v = 0; v < V; ++v) store_out(p.out, p.q_type, at + v, acc[i][v] * inv);
-        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const size_t at = tree_row(p, sg, sg.row0 + r, D) + x4 * 4;
+        store_out4(p.out, p.q_type, at, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
     }
 }
 
@@ -485,18 +453,17 @@ cudaError_t launch_f32(TreeParams p, int num_sms, cudaStream_t st) {
 }
 
 template <int D, typename KT>
-cudaError_t launch_rows(const TreeParams &p, int num_sms, cudaStream_t st) {
-    // rows of a request and kv head on average: above 16, one CTA covers 64
-    const uint64_t rows = (uint64_t)p.n_tokens * p.group / p.n_seqs;
+cudaError_t launch_rows(const TreeParams &p, uint32_t rows, int num_sms, cudaStream_t st) {
+    // above 16 rows one CTA covers 64
     return rows > 16 ? launch_f32<D, KT, 4>(p, num_sms, st) : launch_f32<D, KT, 1>(p, num_sms, st);
 }
 
 template <int D>
 cudaError_t launch_kv(const TreeArgs &a, cudaStream_t st) {
     switch (a.kv_type) {
-        case BML_F32: return launch_rows<D, float>(a.p, a.num_sms, st);
-        case BML_F16: return launch_rows<D, __half>(a.p, a.num_sms, st);
-        case BML_BF16: return launch_rows<D, __nv_bfloat16>(a.p, a.num_sms, st);
+        case BML_F32: return launch_rows<D, float>(a.p, a.rows, a.num_sms, st);
+        case BML_F16: return launch_rows<D, __half>(a.p, a.rows, a.num_sms, st);
+        case BML_BF16: return launch_rows<D, __nv_bfloat16>(a.p, a.rows, a.num_sms, st);
     }
     return cudaErrorInvalidValue;
 }
@@ -506,7 +473,8 @@ cudaError_t launch_kv(const TreeArgs &a, cudaStream_t st) {
 cudaError_t launch_tree_merge(const TreeParams &p, uint32_t D, int grid, cudaStream_t st) {
     if (grid < 2) return cudaSuccess;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid - 1, p.rpg > 64 ? 16 : (p.rpg + 15) / 16);
+    // 16 CTAs for 256 rows; a CTA has 8 tasks of 8 rows x 16 columns at a time
+    cfg.gridDim = dim3(grid - 1, p.rpg > 64 ? 16 : (p.rpg + 7) / 8 * (D / 16) / kWarps);
     cfg.blockDim = dim3(kThreads);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
@@ -523,7 +491,12 @@ size_t tree_workspace_bytes(uint32_t D, int num_sms) {
 }
 
 cudaError_t launch_tree(const TreeArgs &a, cudaStream_t st) {
-    if (tree_umma_fits(a)) return launch_tree_umma(a, st);
+    if (a.kv_type != BML_F32 && a.p.q_type == a.kv_type && a.p.scale_log2 > 0.f) {
+        // (their masked scores are scaled after they were set to -inf, so a scale
+        // of 0 is left to the 32-bit form)
+        if (a.rows <= 64) return launch_tree_warp(a, st);
+        if (tree_umma_fits(a)) return launch_tree_umma(a, st);
+    }
     return a.D == 128 ? launch_kv<128>(a, st) : launch_kv<64>(a, st);
 }
 

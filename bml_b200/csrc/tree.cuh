@@ -19,7 +19,8 @@ struct TreeParams {
     uint32_t n_seqs, n_tokens, n_heads, n_kv, group, max_pages, n_pages, page_shift, n_words;
     float scale_log2;
     int q_type;  // bml_dtype of q and out
-    // partials: slots of rpg rows, o [rpg][D] un-normalised, then m [rpg], l [rpg]
+    // partials: slots of rpg rows, o [D / 4][rpg][4] un-normalised (a warp whose
+    // lanes hold rows writes whole lines), then m [rpg], l [rpg]
     float *part;
     uint32_t rpg;        // rows of a row group
     uint32_t min_tiles;  // tiles a CTA takes at least
@@ -29,6 +30,7 @@ struct TreeArgs {
     TreeParams p;
     uint32_t D;
     bml_dtype kv_type;
+    uint32_t rows;  // rows of a request and kv head, on average
     int num_sms;
 };
 
@@ -37,6 +39,7 @@ cudaError_t launch_tree_merge(const TreeParams &p, uint32_t D, int grid, cudaStr
 size_t tree_workspace_bytes(uint32_t D, int num_sms);
 cudaError_t launch_tree(const TreeArgs &a, cudaStream_t st);
 bool tree_umma_fits(const TreeArgs &a);
+cudaError_t launch_tree_warp(const TreeArgs &a, cudaStream_t st);
 cudaError_t launch_tree_umma(const TreeArgs &a, cudaStream_t st);
 
 #ifdef __CUDACC__
@@ -200,6 +203,49 @@ __device__ __forceinline__ bool tree_sees(const TreeParams &p, const TreeSeq &s,
     if (node >= s.T) return false;
     if (!p.mask) return node <= t;
     return (p.mask[(size_t)(s.first + t) * p.n_words + (node >> 6)] >> (node & 63)) & 1;
+}
+
+// Which of the nodes n0 .. n0 + 15 (n0 > -16; below 0: committed positions,
+// seen by all) node t of a request sees.
+__device__ __forceinline__ uint32_t tree_see16(const TreeParams &p, const TreeSeq &s, uint32_t t, int32_t n0) {
+    if (n0 >= (int32_t)s.T) return 0u;
+    const uint32_t first = n0 < 0 ? 0u : (uint32_t)n0, left = s.T - first;
+    uint64_t w;  // bit i: node first + i
+    if (p.mask) {
+        const uint64_t *m = p.mask + (size_t)(s.first + t) * p.n_words;
+        const uint32_t i = first >> 6, b = first & 63;
+        w = m[i] >> b;
+        if (b > 48 && i + 1 < p.n_words) w |= m[i + 1] << (64 - b);
+    } else {
+        const int32_t k = (int32_t)t - (int32_t)first;  // nodes up to t
+        w = k < 0 ? 0ull : k >= 63 ? ~0ull : (2ull << k) - 1;
+    }
+    if (left < 16) w &= (1ull << left) - 1;
+    return n0 < 0 ? (uint32_t)(w << -n0) | ((1u << -n0) - 1) : (uint32_t)w;
+}
+
+// 16 bytes global -> shared; bytes = 0 writes zeros and reads nothing.
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Barrier over `threads` threads that also says whether any of them has x.
+__device__ __forceinline__ bool group_any(uint32_t id, uint32_t threads, bool x) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred a, b;\n\t"
+        "setp.ne.u32 a, %1, 0;\n\t"
+        "bar.red.or.pred b, %2, %3, a;\n\t"
+        "selp.u32 %0, 1, 0, b;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)x), "r"(id), "r"(threads)
+        : "memory");
+    return r != 0;
 }
 #endif
 

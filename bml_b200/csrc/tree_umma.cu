@@ -720,9 +720,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
                     if (valid) {
                         if (any_odd) add_odd<D, kF16>(p, b, sh.odd, P, t, at, col, m, o);
                         if (part) {
-                            float4 *dst = reinterpret_cast<float4 *>(part + (size_t)row * D + col);
+                            float4 *dst = reinterpret_cast<float4 *>(part) + (size_t)(col / 4) * p.rpg + row;
 #pragma unroll
-                            for (int u = 0; u < 8; ++u) dst[u] = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                            for (int u = 0; u < 8; ++u) dst[u * p.rpg] = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
                         } else {
                             uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + at + col);
 #pragma unroll
@@ -795,8 +795,7 @@ cudaError_t launch_u(const UmmaParams &up, int num_sms, cudaStream_t st) {
 
 }  // namespace
 
-// A scale of 0 goes to the 32-bit form: here masked scores are scaled after they were set to -inf.
-bool tree_umma_fits(const TreeArgs &a) { return a.kv_type != BML_F32 && a.p.q_type == a.kv_type && a.p.group <= (uint32_t)BM && a.p.scale_log2 > 0.f; }
+bool tree_umma_fits(const TreeArgs &a) { return a.p.group <= (uint32_t)BM; }
 
 cudaError_t launch_tree_umma(const TreeArgs &a, cudaStream_t st) {
     static thread_local UmmaParams up;
