@@ -4,6 +4,7 @@
 // the kernels themselves.
 #include <math.h>
 
+#include <atomic>
 #include <initializer_list>
 
 #include "tree.cuh"
@@ -21,11 +22,15 @@ namespace {
 using bml::api_fail;
 
 int sm_count(int device) {
+    static std::atomic<int> known[64];
+    const bool keep = device >= 0 && device < 64;
+    if (keep && known[device].load(std::memory_order_relaxed) > 0) return known[device].load(std::memory_order_relaxed);
     int n = 0;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) {
         (void)cudaGetLastError();
-        n = 148;
+        return 148;
     }
+    if (keep) known[device].store(n, std::memory_order_relaxed);
     return n;
 }
 

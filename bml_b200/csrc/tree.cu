@@ -432,17 +432,13 @@ __global__ void __launch_bounds__(kThreads) tree_merge_kernel(const __grid_const
     }
 }
 
-template <typename F>
-cudaError_t allow_smem(F *f, int bytes) {
-    return cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
-
 template <int D, typename KT, int RW>
 cudaError_t launch_f32(TreeParams p, int num_sms, cudaStream_t st) {
     using C = FCfg<D, KT, RW>;
     static_assert(C::SMEM <= 227 * 1024 - 512, "shared memory");
     auto kern = tree_f32_kernel<D, KT, RW>;
-    cudaError_t e = allow_smem(kern, C::SMEM);
+    static SmemSet set;  // one for each instantiation
+    cudaError_t e = set.allow(kern, C::SMEM);
     if (e != cudaSuccess) return e;
     p.rpg = RW * 16;
     p.min_tiles = 1;

@@ -2,6 +2,8 @@
 // the tile schedule shared by the kernels, and the launch interface.
 #pragma once
 
+#include <atomic>
+
 #include "paged.cuh"
 
 namespace bml {
@@ -37,6 +39,22 @@ struct TreeArgs {
 constexpr uint32_t kTreeMaxRows = 256;  // rows of the largest row group
 cudaError_t launch_tree_merge(const TreeParams &p, uint32_t D, int grid, cudaStream_t st);
 size_t tree_workspace_bytes(uint32_t D, int num_sms);
+
+// Allows a kernel its dynamic shared memory, once for each device.
+struct SmemSet {
+    std::atomic<bool> done[64] = {};
+    template <typename F>
+    cudaError_t allow(F *kernel, int bytes) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        const bool keep = dev >= 0 && dev < 64;
+        if (keep && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess && keep) done[dev].store(true, std::memory_order_release);
+        return e;
+    }
+};
 cudaError_t launch_tree(const TreeArgs &a, cudaStream_t st);
 bool tree_umma_fits(const TreeArgs &a);
 cudaError_t launch_tree_warp(const TreeArgs &a, cudaStream_t st);

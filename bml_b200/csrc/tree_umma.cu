@@ -785,7 +785,8 @@ template <int D, bool kF16>
 cudaError_t launch_u(const UmmaParams &up, int num_sms, cudaStream_t st) {
     using C = UCfg<D>;
     auto kern = tree_umma_kernel<D, kF16>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    static SmemSet set;  // one for each instantiation
+    cudaError_t e = set.allow(kern, C::SMEM);
     if (e != cudaSuccess) return e;
     kern<<<num_sms, kThreads, C::SMEM, st>>>(up);
     e = cudaGetLastError();

@@ -344,7 +344,8 @@ cudaError_t launch_w(TreeParams p, int num_sms, cudaStream_t st) {
     using C = WCfg<D, RW>;
     static_assert(C::SMEM <= 227 * 1024 - 512, "shared memory");
     auto kern = tree_warp_kernel<D, kF16, RW>;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    static SmemSet set;  // one for each instantiation
+    cudaError_t e = set.allow(kern, C::SMEM);
     if (e != cudaSuccess) return e;
     p.rpg = RW * 16;
     p.min_tiles = 1;

@@ -20,12 +20,11 @@ one; `stream` defaults to that device's current stream.
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass
 
 import torch
 
 from . import _lib as L
-from .attention import _need, _ptr, _stream, dtype_code
+from .attention import _need, dtype_code
 from .batching import MAX_PENDING_REQUESTS, AtCapacity
 
 MAX_NODES = 256  # drafted tokens of one request in tree_attention
@@ -36,42 +35,92 @@ class OutOfPages(RuntimeError):
     """A plan that refused a request (its status says why)."""
 
 
-def _arg(t, name: str, dtype, shape=None, device=None) -> None:
-    _need(t, name, dtype)
+# A call costs the host several microseconds and the GPU often less, so the
+# wrappers take care: one test per tensor on the way that is right (_bad says
+# what is wrong on the other), raw stream handles and addresses, few
+# allocations.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _bad(t, name: str, dtype=None, ndim=None, shape=None, device=None):
+    """Raises the error that says what is wrong with an argument."""
+    _need(t, name, dtype, ndim)
     if shape is not None and tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
+    raise ValueError(f"{name} is not a valid argument")
+
+
+def _ints(t, name: str, device, shape=None, ndim: int = 1, dtype=torch.int32) -> int:
+    """The address of a contiguous integer tensor on `device`."""
+    if (not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device or not t.is_contiguous()
+            or (t.shape != shape if shape is not None else t.dim() != ndim)):
+        _bad(t, name, dtype, None if shape is not None else ndim, shape, device)
+    return t.data_ptr()
+
+
+def _data(t, name: str, ndim: int, dtype=None, device=None) -> int:
+    """The address of a contiguous CUDA tensor."""
+    if (not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != ndim or not t.is_contiguous()
+            or (dtype is not None and t.dtype is not dtype) or (device is not None and t.device != device)):
+        _bad(t, name, dtype, ndim, None, device)
+    return t.data_ptr()
 
 
 class _On:
     """Makes a call's device current, and its stream where one is given, so
-    that the buffers it allocates belong to the stream that uses them."""
+    that the buffers it allocates belong to the stream that uses them; the
+    stream's handle on entry."""
 
-    def __init__(self, device: torch.device, stream=None):
+    def __init__(self, device: torch.device, stream):
         if stream is not None and stream.device != device:
             raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
+        self._index = device.index
         self._ctx = torch.cuda.stream(stream) if stream is not None else torch.cuda.device(device)
 
     def __enter__(self):
         self._ctx.__enter__()
-        return _stream()
+        return _raw_stream(self._index)
 
     def __exit__(self, *exc):
         return self._ctx.__exit__(*exc)
 
 
-@dataclass
+class _Here:
+    """_On for the usual case: the device is current, no stream is given."""
+
+    def __init__(self, index: int):
+        self._index = index
+
+    def __enter__(self):
+        return _raw_stream(self._index)
+
+    def __exit__(self, *exc):
+        return False
+
+
+_here: dict = {}
+
+
+def _on(device: torch.device, stream):
+    i = device.index
+    if stream is None and i == torch.cuda.current_device():
+        h = _here.get(i)
+        if h is None:
+            h = _here[i] = _Here(i)
+        return h
+    return _On(device, stream)
+
+
 class PagePlan:
-    """One step's plan; all tensors on the device (see bml_paged_plan)."""
-    node_start: torch.Tensor  # int32 [n + 1]
-    kv_lens: torch.Tensor     # int32 [n]
-    owned: torch.Tensor       # int32 [n]
-    free_used: torch.Tensor   # int32 [1]
-    slots: torch.Tensor       # int64 [n_tokens]
-    positions: torch.Tensor   # int32 [n_tokens]
-    status: torch.Tensor      # int32 [n]
-    mask: torch.Tensor | None  # int64 [n_tokens, n_words], with parents
+    """One step's plan; all tensors on the device (see bml_paged_plan).
+
+    node_start int32 [n + 1], kv_lens, owned, status int32 [n], free_used
+    int32 [1], slots int64 [n_tokens], positions int32 [n_tokens], mask int64
+    [n_tokens, n_words] (None without parents)."""
+
+    __slots__ = ("node_start", "kv_lens", "owned", "free_used", "status", "positions", "slots", "mask")
 
     def check(self) -> None:
         """Raises OutOfPages if a request was refused.  Waits for the GPU."""
@@ -90,46 +139,52 @@ def page_plan(lens: torch.Tensor, n_new: torch.Tensor, owned: torch.Tensor, bloc
     [n], free_pages, free_used [1] are int32; n_tokens is the row count of
     the step's token arrays, at least the sum of n_new.  lens, owned and
     free_used are not changed: the plan carries their next values."""
-    _arg(lens, "lens", torch.int32)
-    if lens.dim() != 1:
-        raise ValueError("lens must have 1 dim")
-    n, dev = lens.shape[0], lens.device
-    _arg(n_new, "n_new", torch.int32, (n,), dev)
-    _arg(owned, "owned", torch.int32, (n,), dev)
-    _arg(block_table, "block_table", torch.int32, None, dev)
-    if block_table.dim() != 2 or block_table.shape[0] != n:
+    dev = lens.device if isinstance(lens, torch.Tensor) else None
+    if dev is None or dev.type != "cuda":
+        _bad(lens, "lens", torch.int32, 1)
+    a_lens = _ints(lens, "lens", dev)
+    one = lens.shape
+    n = one[0]
+    a_new, a_owned = _ints(n_new, "n_new", dev, one), _ints(owned, "owned", dev, one)
+    a_table = _ints(block_table, "block_table", dev, ndim=2)
+    rows, max_pages = block_table.shape
+    if rows != n:
         raise ValueError(f"block_table must be [{n}, max_pages], got {tuple(block_table.shape)}")
-    _arg(free_pages, "free_pages", torch.int32, None, dev)
-    if free_pages.dim() != 1:
-        raise ValueError("free_pages must have 1 dim")
-    _arg(free_used, "free_used", torch.int32, (1,), dev)
+    a_free, a_used = _ints(free_pages, "free_pages", dev), _ints(free_used, "free_used", dev, (1,))
     if n_tokens < 0:
         raise ValueError("n_tokens must not be negative")
+    a_parents = None
     if parents is not None:
-        _arg(parents, "parents", torch.int32, (n_tokens,), dev)
+        a_parents = _ints(parents, "parents", dev, (n_tokens,))
         if not 1 <= n_words <= MAX_NODES // 64:
             raise ValueError(f"n_words must be 1 to {MAX_NODES // 64}, got {n_words}")
-    with _On(dev, stream) as st:
-        i32 = dict(dtype=torch.int32, device=dev)
-        p = PagePlan(torch.empty(n + 1, **i32), torch.empty(n, **i32), torch.empty(n, **i32), torch.empty(1, **i32),
-                     torch.empty(n_tokens, dtype=torch.int64, device=dev), torch.empty(n_tokens, **i32),
-                     torch.empty(n, **i32),
-                     None if parents is None else torch.empty(n_tokens, n_words, dtype=torch.int64, device=dev))
-        L.call("bml_paged_plan", _ptr(lens), _ptr(n_new), _ptr(owned), n, _ptr(free_pages), free_pages.numel(),
-               _ptr(free_used), page_size, block_table.shape[1], _ptr(block_table),
-               None if parents is None else _ptr(parents), n_tokens, n_words, _ptr(p.node_start), _ptr(p.kv_lens),
-               _ptr(p.owned), _ptr(p.free_used), _ptr(p.slots), _ptr(p.positions),
-               None if p.mask is None else _ptr(p.mask), _ptr(p.status), st)
+    p = PagePlan()
+    with _on(dev, stream) as st:
+        # two buffers: the int64 arrays, the int32 ones
+        wide = torch.empty(n_tokens * (1 if parents is None else 1 + n_words), dtype=torch.int64, device=dev)
+        small = torch.empty(4 * n + 2 + n_tokens, dtype=torch.int32, device=dev)
+        a, w = small.data_ptr(), wide.data_ptr()
+        L.call("bml_paged_plan", a_lens, a_new, a_owned, n, a_free, free_pages.shape[0], a_used, page_size, max_pages,
+               a_table, a_parents, n_tokens, n_words, a, a + 4 * (n + 1), a + 4 * (2 * n + 1), a + 4 * (4 * n + 1), w,
+               a + 4 * (4 * n + 2), None if parents is None else w + 8 * n_tokens, a + 4 * (3 * n + 1), st)
+    p.node_start, p.kv_lens, p.owned, p.status, p.free_used, p.positions = small.split(
+        (n + 1, n, n, n, 1, n_tokens))
+    if parents is None:
+        p.slots, p.mask = wide, None
+    else:
+        p.slots, mask = wide.split((n_tokens, n_tokens * n_words))
+        p.mask = mask.view(n_tokens, n_words)
     return p
 
 
 def _pools(k_pool, v_pool, ndim: int, device=None):
-    _need(k_pool, "k_pool", None, ndim)
-    _need(v_pool, "v_pool", k_pool.dtype, ndim)
-    if k_pool.shape != v_pool.shape or k_pool.device != v_pool.device:
-        raise ValueError(f"k_pool {tuple(k_pool.shape)} and v_pool {tuple(v_pool.shape)} do not match")
-    if device is not None and k_pool.device != device:
-        raise ValueError(f"the pools are on {k_pool.device}, expected {device}")
+    """The pools' addresses and shape."""
+    a = _data(k_pool, "k_pool", ndim, None, device)
+    b = _data(v_pool, "v_pool", ndim, k_pool.dtype, k_pool.device)
+    shape = k_pool.shape
+    if shape != v_pool.shape:
+        raise ValueError(f"k_pool {tuple(shape)} and v_pool {tuple(v_pool.shape)} do not match")
+    return a, b, shape
 
 
 def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor,
@@ -141,35 +196,36 @@ def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, slots
     [n_pages, page_size, n_kv, d].  q, k, v in one type (f32, f16, bf16), the
     pools in any.  positions None: no rotation; q None: no queries.  A token
     whose slot is -1 (or outside the pool) is skipped.  Returns the turned q."""
-    _need(k, "k", None, 3)
-    _need(v, "v", k.dtype, 3)
-    n, n_kv, d = k.shape
-    dev = k.device
-    if k.shape != v.shape or v.device != dev:
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not match")
-    _pools(k_pool, v_pool, 4, dev)
-    if tuple(k_pool.shape[2:]) != (n_kv, d):
-        raise ValueError(f"pool rows {tuple(k_pool.shape[2:])} do not match k {tuple(k.shape)}")
-    _arg(slots, "slots", torch.int64, (n,), dev)
-    if positions is not None:
-        _arg(positions, "positions", torch.int32, (n,), dev)
-    n_heads = 0
+    a_k = _data(k, "k", 3)
+    dev, dtype = k.device, k.dtype
+    a_v = _data(v, "v", 3, dtype, dev)
+    shape = k.shape
+    n, n_kv, d = shape
+    if shape != v.shape:
+        raise ValueError(f"k {tuple(shape)} and v {tuple(v.shape)} do not match")
+    a_kp, a_vp, pool = _pools(k_pool, v_pool, 4, dev)
+    if pool[2] != n_kv or pool[3] != d:
+        raise ValueError(f"pool rows {tuple(pool[2:])} do not match k {tuple(shape)}")
+    a_slots = _ints(slots, "slots", dev, (n,), dtype=torch.int64)
+    a_pos = None if positions is None else _ints(positions, "positions", dev, (n,))
+    n_heads, a_q, a_out = 0, None, None
     if q is not None:
-        _arg(q, "q", k.dtype, None, dev)
-        if q.dim() != 3 or q.shape[0] != n or q.shape[2] != d:
-            raise ValueError(f"q {tuple(q.shape)} does not match k {tuple(k.shape)}")
-        n_heads = q.shape[1]
+        a_q = a_out = _data(q, "q", 3, dtype, dev)
+        q_shape = q.shape
+        n_heads = q_shape[1]
+        if q_shape[0] != n or q_shape[2] != d:
+            raise ValueError(f"q {tuple(q_shape)} does not match k {tuple(shape)}")
         if q_out is None:
             q_out = q
         else:
-            _arg(q_out, "q_out", q.dtype, q.shape, dev)
+            a_out = _data(q_out, "q_out", 3, dtype, dev)
+            if q_out.shape != q_shape:
+                raise ValueError(f"q_out {tuple(q_out.shape)} does not match q {tuple(q_shape)}")
     elif q_out is not None:
         raise ValueError("q_out without q")
-    with _On(dev, stream) as st:
-        L.call("bml_paged_append", None if q is None else _ptr(q), _ptr(k), _ptr(v), dtype_code(k.dtype), _ptr(slots),
-               None if positions is None else _ptr(positions), n, n_heads, n_kv, d, float(theta),
-               None if q is None else _ptr(q_out), _ptr(k_pool), _ptr(v_pool), dtype_code(k_pool.dtype),
-               k_pool.shape[0] * k_pool.shape[1], st)
+    with _on(dev, stream) as st:
+        L.call("bml_paged_append", a_q, a_k, a_v, dtype_code(dtype), a_slots, a_pos, n, n_heads, n_kv, d, theta, a_out,
+               a_kp, a_vp, dtype_code(k_pool.dtype), pool[0] * pool[1], st)
     return q_out
 
 
@@ -205,37 +261,39 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     workspace: an uint8 tensor of tree_workspace_size bytes for calls that
     must not allocate; calls that share one must not overlap.  By default
     scratch comes from torch's allocator, on the call's stream."""
-    _need(q, "q", None, 3)
-    n_tokens, n_heads, d = q.shape
-    dev = q.device
-    _pools(k_pool, v_pool, 4, dev)
-    if k_pool.shape[3] != d:
-        raise ValueError(f"q {tuple(q.shape)} does not match the pools {tuple(k_pool.shape)}")
-    n = kv_lens.shape[0] if isinstance(kv_lens, torch.Tensor) and kv_lens.dim() == 1 else -1
-    _arg(kv_lens, "kv_lens", torch.int32, (n,), dev)
-    _arg(node_start, "node_start", torch.int32, (n + 1,), dev)
-    _arg(block_table, "block_table", torch.int32, None, dev)
-    if block_table.dim() != 2 or block_table.shape[0] != n:
+    a_q = _data(q, "q", 3)
+    shape, dev, dtype = q.shape, q.device, q.dtype
+    n_tokens, n_heads, d = shape
+    a_k, a_v, pool = _pools(k_pool, v_pool, 4, dev)
+    n_pages, page_size, n_kv, pd = pool
+    if pd != d:
+        raise ValueError(f"q {tuple(shape)} does not match the pools {tuple(pool)}")
+    a_len = _ints(kv_lens, "kv_lens", dev)
+    n = kv_lens.shape[0]
+    a_start = _ints(node_start, "node_start", dev, (n + 1,))
+    a_table = _ints(block_table, "block_table", dev, ndim=2)
+    rows, max_pages = block_table.shape
+    if rows != n:
         raise ValueError(f"block_table must be [{n}, max_pages], got {tuple(block_table.shape)}")
-    n_words = 0
+    a_mask, n_words = None, 0
     if mask is not None:
-        _arg(mask, "mask", torch.int64, None, dev)
-        if mask.dim() != 2 or mask.shape[0] != n_tokens or not 1 <= mask.shape[1] <= MAX_NODES // 64:
+        a_mask = _ints(mask, "mask", dev, ndim=2, dtype=torch.int64)
+        rows, n_words = mask.shape
+        if rows != n_tokens or not 1 <= n_words <= MAX_NODES // 64:
             raise ValueError(f"mask must be [{n_tokens}, 1 to {MAX_NODES // 64}], got {tuple(mask.shape)}")
-        n_words = mask.shape[1]
-    with _On(dev, stream) as st:
+    with _on(dev, stream) as st:
         if out is None:
             out = torch.empty_like(q)
-        else:
-            _arg(out, "out", q.dtype, q.shape, dev)
+        elif _data(out, "out", 3, dtype, dev) and out.shape != shape:
+            raise ValueError(f"out {tuple(out.shape)} does not match q {tuple(shape)}")
         if workspace is None:
-            workspace = torch.empty(tree_workspace_size(d, dev), dtype=torch.uint8, device=dev)
+            need = _ws_bytes.get((dev.index, d)) or tree_workspace_size(d, dev)
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
         else:
-            _arg(workspace, "workspace", torch.uint8, None, dev)
-        L.call("bml_attn_tree", _ptr(q), dtype_code(q.dtype), n_tokens, n_heads, k_pool.shape[2], d, _ptr(k_pool),
-               _ptr(v_pool), dtype_code(k_pool.dtype), k_pool.shape[0], k_pool.shape[1], _ptr(block_table),
-               block_table.shape[1], _ptr(kv_lens), _ptr(node_start), n, None if mask is None else _ptr(mask), n_words,
-               float(scale), _ptr(out), _ptr(workspace), workspace.numel(), st)
+            _ints(workspace, "workspace", dev, dtype=torch.uint8)
+        L.call("bml_attn_tree", a_q, dtype_code(dtype), n_tokens, n_heads, n_kv, d, a_k, a_v, dtype_code(k_pool.dtype),
+               n_pages, page_size, a_table, max_pages, a_len, a_start, n, a_mask, n_words, scale, out.data_ptr(),
+               workspace.data_ptr(), workspace.shape[0], st)
     return out
 
 
@@ -248,25 +306,25 @@ def paged_commit(k_pools: torch.Tensor, v_pools: torch.Tensor, block_table: torc
     path [n, max_path] int32 holds strictly increasing node indices; an entry
     that is not ends the path.  Returns the new lengths int32 [n]; a request
     that page_plan refused keeps its own."""
-    _pools(k_pools, v_pools, 5)
+    a_k, a_v, pool = _pools(k_pools, v_pools, 5)
+    layers, n_pages, page_size, n_kv, d = pool
     dev = k_pools.device
-    n = lens.shape[0] if isinstance(lens, torch.Tensor) and lens.dim() == 1 else -1
-    _arg(lens, "lens", torch.int32, (n,), dev)
-    _arg(kv_lens, "kv_lens", torch.int32, (n,), dev)
-    _arg(node_start, "node_start", torch.int32, (n + 1,), dev)
-    _arg(n_accept, "n_accept", torch.int32, (n,), dev)
-    _arg(block_table, "block_table", torch.int32, None, dev)
-    _arg(path, "path", torch.int32, None, dev)
-    if block_table.dim() != 2 or block_table.shape[0] != n:
+    a_lens = _ints(lens, "lens", dev)
+    one = lens.shape
+    n = one[0]
+    a_len, a_start = _ints(kv_lens, "kv_lens", dev, one), _ints(node_start, "node_start", dev, (n + 1,))
+    a_accept, a_table = _ints(n_accept, "n_accept", dev, one), _ints(block_table, "block_table", dev, ndim=2)
+    a_path = _ints(path, "path", dev, ndim=2)
+    rows, max_pages = block_table.shape
+    path_rows, max_path = path.shape
+    if rows != n:
         raise ValueError(f"block_table must be [{n}, max_pages], got {tuple(block_table.shape)}")
-    if path.dim() != 2 or path.shape[0] != n:
+    if path_rows != n:
         raise ValueError(f"path must be [{n}, max_path], got {tuple(path.shape)}")
-    layers, n_pages, page_size, n_kv, d = k_pools.shape
-    with _On(dev, stream) as st:
+    with _on(dev, stream) as st:
         new = torch.empty_like(lens)
-        L.call("bml_paged_commit", _ptr(k_pools), _ptr(v_pools), layers, n_pages, page_size, n_kv, d,
-               dtype_code(k_pools.dtype), _ptr(block_table), block_table.shape[1], _ptr(lens), _ptr(kv_lens),
-               _ptr(node_start), n, _ptr(path), path.shape[1], _ptr(n_accept), _ptr(new), st)
+        L.call("bml_paged_commit", a_k, a_v, layers, n_pages, page_size, n_kv, d, dtype_code(k_pools.dtype), a_table,
+               max_pages, a_lens, a_len, a_start, n, a_path, max_path, a_accept, new.data_ptr(), st)
     return new
 
 
