@@ -487,11 +487,11 @@ size_t tree_workspace_bytes(uint32_t D, int num_sms) {
 }
 
 cudaError_t launch_tree(const TreeArgs &a, cudaStream_t st) {
-    if (a.kv_type != BML_F32 && a.p.q_type == a.kv_type && a.p.scale_log2 > 0.f) {
-        // (their masked scores are scaled after they were set to -inf, so a scale
-        // of 0 is left to the 32-bit form)
-        if (a.rows <= 64) return launch_tree_warp(a, st);
-        if (tree_umma_fits(a)) return launch_tree_umma(a, st);
+    // 16-bit pages, except for a scale of 0 (those kernels scale masked scores
+    // after they were set to -inf)
+    if (a.kv_type != BML_F32 && a.p.scale_log2 > 0.f) {
+        if (a.p.q_type == BML_F32 || a.rows <= 64 || !tree_umma_fits(a)) return launch_tree_warp(a, st);
+        return launch_tree_umma(a, st);
     }
     return a.D == 128 ? launch_kv<128>(a, st) : launch_kv<64>(a, st);
 }

@@ -1,5 +1,6 @@
 // tree_warp.cu -- attention of drafted tokens over a paged cache for few rows
-// (up to 64 a kv head): 16-bit queries over pages of their type.
+// (up to 64 a kv head) over 16-bit pages: 16-bit queries of the pages' type, or
+// 32-bit queries.
 //
 // The mathematics and the schedule are those of tree.cu / tree.cuh.  With few
 // rows the work is to stream K and V: 4 * rows FLOP per 2-byte K/V element
@@ -17,6 +18,13 @@
 // own ring, some steps ahead and across the ends of segments; RW == 1 needs no
 // barrier at all inside a segment.  At a segment's end the groups' (m, l, o)
 // meet in shared memory, 32 columns at a time.
+//
+// 32-bit queries (kQ32) are split into 16-bit terms of the pages' type, so
+// that products are exact in the f32 sums: three bf16 terms hold all 24 bits;
+// two f16 terms hold 22 of a row that is first scaled by a power of two to a
+// largest value in [2^10, 2^11) (f16's range is small).  The softmax weights
+// are split the same way, and each block's P.V is summed apart and added to O
+// with a rounding, since the matrix unit's own accumulation truncates.
 #include <math.h>
 
 #include "mma_frag.cuh"
@@ -30,19 +38,22 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr float kGrow = 8.0f;  // log2 units a row's maximum may grow before O is rescaled
 
-template <int D, int RW>
+template <int D, bool kF16, int RW, bool kQ32>
 struct WCfg {
+    static constexpr int TERMS = kQ32 ? (kF16 ? 2 : 3) : 1;  // 16-bit terms of a query or a weight
     static constexpr int GROUPS = kWarps / RW;
     static constexpr int SP = 16 * RW;             // positions of a group's step
     static constexpr int RS = D * 2 + 16;          // row stride: 8 rows of an ldmatrix in 8 bank groups
     static constexpr int STAGE = 2 * SP * RS;      // K then V
-    static constexpr int NST = D == 128 ? 3 : 5;   // about 209 / 184 KB of ring
+    // stages of a group's ring: 209 KB (139 beside the terms' 12 to 48 KB) or 184 KB
+    static constexpr int NST = D == 128 ? (kQ32 ? 2 : 3) : (kQ32 ? 4 : 5);
     static constexpr int CH = 32;                  // columns that meet at once
     static constexpr int CS = CH + 4;
     static constexpr int OFF_MEET = GROUPS * NST * STAGE;
     static constexpr int OFF_ML = OFF_MEET + kWarps * 16 * CS * 4;
     static constexpr int OFF_FLAGS = OFF_ML + kWarps * 16 * 8;
-    static constexpr int SMEM = OFF_FLAGS + GROUPS * NST * 4 * 4;
+    static constexpr int OFF_Q = OFF_FLAGS + GROUPS * NST * 4 * 4;  // kQ32: fragments [row warp][k-step][term][lane]
+    static constexpr int SMEM = OFF_Q + (kQ32 ? RW * 16 * D * 2 * TERMS : 0);
 };
 
 template <bool kF16>
@@ -65,9 +76,24 @@ __device__ __forceinline__ float wide16(uint16_t x) {
     return kF16 ? __half2float(*reinterpret_cast<const __half *>(&x)) : __uint_as_float((uint32_t)x << 16);
 }
 
-template <int D, bool kF16, int RW>
+// x as TERMS 16-bit terms, the largest first: x is their sum to 24 (three
+// bf16) or 22 bits (two f16).
+template <bool kF16, int TERMS>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&t)[TERMS]) {
+#pragma unroll
+    for (int i = 0; i < TERMS; ++i) {
+        t[i] = pack16<kF16>(x, y);
+        if (i + 1 < TERMS) {
+            x -= wide16<kF16>((uint16_t)t[i]);
+            y -= wide16<kF16>((uint16_t)(t[i] >> 16));
+        }
+    }
+}
+
+template <int D, bool kF16, int RW, bool kQ32>
 __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_constant__ TreeParams p) {
-    using C = WCfg<D, RW>;
+    using C = WCfg<D, kF16, RW, kQ32>;
+    constexpr int TERMS = C::TERMS;
     constexpr int NT = D / 8;       // output column tiles of a warp
     constexpr int PER = D * 2 / 16; // 16-byte pieces of a row
     extern __shared__ __align__(16) uint8_t smem[];
@@ -120,6 +146,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
         cp_commit();
         f_stage = f_stage + 1 == (uint32_t)C::NST ? 0 : f_stage + 1;
     };
+    auto weight = [](float x) { return kQ32 ? exp2f(x) : fast_exp2(x); };
     auto group_sync = [&]() {
         if (RW == 1) __syncwarp();
         else named_bar_sync(1 + grp, RW * 32);
@@ -135,13 +162,55 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
         const uint32_t r0 = rw * 16 + g, r1 = r0 + 8;  // this lane's rows of the group
         const bool v0 = r0 < sg.rows, v1 = r1 < sg.rows;
         const uint32_t t0 = (sg.row0 + r0) / p.group, t1 = (sg.row0 + r1) / p.group;
-        uint32_t q[D / 16][4];
-        {
+        uint32_t q[kQ32 ? 1 : D / 16][4];
+        float c0 = p.scale_log2, c1 = p.scale_log2;  // score scales of rows g and g + 8
+        uint4 *qf = reinterpret_cast<uint4 *>(smem + C::OFF_Q) + rw * (D / 16) * TERMS * 32 + lane;
+        if (kQ32) {
+            const float *qp = static_cast<const float *>(p.q);
+            const float *q0 = qp + (v0 ? tree_row(p, sg, sg.row0 + r0, D) : 0) + 2 * c;
+            const float *q1 = qp + (v1 ? tree_row(p, sg, sg.row0 + r1, D) : 0) + 2 * c;
+            float e0 = 1.f, e1 = 1.f;
+            if (kF16) {
+                float a = 0.f, b = 0.f;
+#pragma unroll 4
+                for (int s = 0; s < D / 8; ++s) {
+                    const float2 x = v0 ? *reinterpret_cast<const float2 *>(q0 + s * 8) : make_float2(0.f, 0.f);
+                    const float2 y = v1 ? *reinterpret_cast<const float2 *>(q1 + s * 8) : make_float2(0.f, 0.f);
+                    a = fmaxf(a, fmaxf(fabsf(x.x), fabsf(x.y)));
+                    b = fmaxf(b, fmaxf(fabsf(y.x), fabsf(y.y)));
+                }
+                a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
+                b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, 1));
+                a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
+                b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, 2));
+                // exponents: 2^(10 - floor(log2 a)), kept where both it and its inverse are normal
+                const int ea = min(max((int)(__float_as_uint(a) >> 23), 30), 240), eb = min(max((int)(__float_as_uint(b) >> 23), 30), 240);
+                e0 = __uint_as_float((uint32_t)(254 + 10 - ea) << 23);
+                e1 = __uint_as_float((uint32_t)(254 + 10 - eb) << 23);
+                c0 *= __uint_as_float((uint32_t)(ea - 10) << 23);
+                c1 *= __uint_as_float((uint32_t)(eb - 10) << 23);
+            }
+#pragma unroll 2
+            for (int s = 0; s < D / 16; ++s) {
+                uint32_t t[4][TERMS];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float2 x = v0 ? *reinterpret_cast<const float2 *>(q0 + s * 16 + h * 8) : make_float2(0.f, 0.f);
+                    const float2 y = v1 ? *reinterpret_cast<const float2 *>(q1 + s * 16 + h * 8) : make_float2(0.f, 0.f);
+                    split_pair<kF16>(x.x * e0, x.y * e0, t[2 * h]);
+                    split_pair<kF16>(y.x * e1, y.y * e1, t[2 * h + 1]);
+                }
+                if (grp == 0)
+#pragma unroll
+                    for (int z = 0; z < TERMS; ++z) qf[(s * TERMS + z) * 32] = make_uint4(t[0][z], t[1][z], t[2][z], t[3][z]);
+            }
+            __syncthreads();
+        } else {
             const uint16_t *qp = static_cast<const uint16_t *>(p.q);
             const uint16_t *q0 = qp + (v0 ? tree_row(p, sg, sg.row0 + r0, D) : 0) + 2 * c;
             const uint16_t *q1 = qp + (v1 ? tree_row(p, sg, sg.row0 + r1, D) : 0) + 2 * c;
 #pragma unroll
-            for (int s = 0; s < D / 16; ++s) {
+            for (int s = 0; s < (kQ32 ? 1 : D / 16); ++s) {
                 q[s][0] = v0 ? *reinterpret_cast<const uint32_t *>(q0 + s * 16) : 0u;
                 q[s][1] = v1 ? *reinterpret_cast<const uint32_t *>(q1 + s * 16) : 0u;
                 q[s][2] = v0 ? *reinterpret_cast<const uint32_t *>(q0 + s * 16 + 8) : 0u;
@@ -190,14 +259,30 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
                 const uint32_t base = pos + b * 16;
                 if (base >= sg.s.L || !flags[st * 4 + b]) continue;
                 float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+                float lo[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};  // kQ32: the smaller terms' sums
                 const uint8_t *ka = sk + (b * 16 + (lane & 7) + ((lane >> 4) << 3)) * C::RS + ((lane >> 3) & 1) * 16;
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) {
                     uint32_t r[4];
                     ldsm_x4(smem_u32(ka + ks * 32), r);
-                    mma16816<kF16>(s[0], q[ks], r[0], r[1]);
-                    mma16816<kF16>(s[1], q[ks], r[2], r[3]);
+                    if (kQ32) {
+#pragma unroll
+                        for (int z = 0; z < TERMS; ++z) {
+                            const uint4 x = qf[(ks * TERMS + z) * 32];
+                            const uint32_t a4[4] = {x.x, x.y, x.z, x.w};
+                            mma16816<kF16>(z ? lo[0] : s[0], a4, r[0], r[1]);
+                            mma16816<kF16>(z ? lo[1] : s[1], a4, r[2], r[3]);
+                        }
+                    } else {
+                        mma16816<kF16>(s[0], q[kQ32 ? 0 : ks], r[0], r[1]);
+                        mma16816<kF16>(s[1], q[kQ32 ? 0 : ks], r[2], r[3]);
+                    }
                 }
+                if (kQ32)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[h][e] += lo[h][e];
                 if (base + 16 > P) {
                     const uint32_t w0 = v0 ? tree_see16(p, sg.s, t0, (int32_t)(base - P)) : 0u;
                     const uint32_t w1 = v1 ? tree_see16(p, sg.s, t1, (int32_t)(base - P)) : 0u;
@@ -215,11 +300,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
                 d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, 1));
                 a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
                 d = fmaxf(d, __shfl_xor_sync(0xffffffffu, d, 2));
-                a *= p.scale_log2;  // > 0
-                d *= p.scale_log2;
+                a *= c0;  // > 0
+                d *= c1;
                 if (__any_sync(0xffffffffu, a > m0 + kGrow || d > m1 + kGrow)) {
                     const float n0 = a > m0 + kGrow ? a : m0, n1 = d > m1 + kGrow ? d : m1;
-                    const float f0 = n0 == -INFINITY ? 1.f : fast_exp2(m0 - n0), f1 = n1 == -INFINITY ? 1.f : fast_exp2(m1 - n1);
+                    const float f0 = n0 == -INFINITY ? 1.f : weight(m0 - n0), f1 = n1 == -INFINITY ? 1.f : weight(m1 - n1);
                     m0 = n0;
                     m1 = n1;
                     l0 *= f0;
@@ -237,21 +322,43 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        s[h][e] = fast_exp2(fmaf(s[h][e], p.scale_log2, -u0));
-                        s[h][2 + e] = fast_exp2(fmaf(s[h][2 + e], p.scale_log2, -u1));
+                        s[h][e] = weight(fmaf(s[h][e], c0, -u0));
+                        s[h][2 + e] = weight(fmaf(s[h][2 + e], c1, -u1));
                     }
                 l0 += (s[0][0] + s[0][1]) + (s[1][0] + s[1][1]);
                 l1 += (s[0][2] + s[0][3]) + (s[1][2] + s[1][3]);
-                // P as the A operand of P.V, rounded to the pages' type
-                const uint32_t pa[4] = {pack16<kF16>(s[0][0], s[0][1]), pack16<kF16>(s[0][2], s[0][3]),
-                                        pack16<kF16>(s[1][0], s[1][1]), pack16<kF16>(s[1][2], s[1][3])};
+                // P as the A operand of P.V, rounded to the pages' type (kQ32: split)
+                uint32_t pa[TERMS][4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        uint32_t t[TERMS];
+                        split_pair<kF16>(s[h][2 * e], s[h][2 * e + 1], t);
+#pragma unroll
+                        for (int z = 0; z < TERMS; ++z) pa[z][2 * h + e] = t[z];
+                    }
                 const uint8_t *va = sv + (b * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * C::RS + (lane >> 4) * 16;
 #pragma unroll
                 for (int j = 0; j < NT; j += 2) {
                     uint32_t r[4];
                     ldsm_x4_t(smem_u32(va + j * 16), r);
-                    mma16816<kF16>(o[j], pa, r[0], r[1]);
-                    mma16816<kF16>(o[j + 1], pa, r[2], r[3]);
+                    if (kQ32) {
+                        float x[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                        for (int z = TERMS - 1; z >= 0; --z) {
+                            mma16816<kF16>(x[0], pa[z], r[0], r[1]);
+                            mma16816<kF16>(x[1], pa[z], r[2], r[3]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            o[j][e] += x[0][e];
+                            o[j + 1][e] += x[1][e];
+                        }
+                    } else {
+                        mma16816<kF16>(o[j], pa[0], r[0], r[1]);
+                        mma16816<kF16>(o[j + 1], pa[0], r[2], r[3]);
+                    }
                 }
                 if (odd) {
                     // rare: the values that became zeros, from global memory
@@ -312,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
 #pragma unroll
                 for (int q8 = 0; q8 < C::GROUPS; ++q8) {
                     const float2 a = ml[q8 * RW * 16 + r];
-                    const float f = fast_exp2(a.x - mu);
+                    const float f = weight(a.x - mu);
                     const float4 y = *reinterpret_cast<const float4 *>(meet + (q8 * RW * 16 + r) * C::CS + x4 * 4);
                     l += f * a.y;
                     acc.x += f * y.x;
@@ -329,8 +436,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
                     }
                 } else {
                     const float inv = l == 0.f ? 0.f : 1.f / l;
-                    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + tree_row(p, sg, sg.row0 + r, D) + col4 * 4) =
-                        make_uint2(pack16<kF16>(acc.x * inv, acc.y * inv), pack16<kF16>(acc.z * inv, acc.w * inv));
+                    const size_t at = tree_row(p, sg, sg.row0 + r, D) + col4 * 4;
+                    if (kQ32)
+                        *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) =
+                            make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+                    else
+                        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at) =
+                            make_uint2(pack16<kF16>(acc.x * inv, acc.y * inv), pack16<kF16>(acc.z * inv, acc.w * inv));
                 }
             }
             __syncthreads();
@@ -339,11 +451,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
     cp_wait<0>();
 }
 
-template <int D, bool kF16, int RW>
+template <int D, bool kF16, int RW, bool kQ32>
 cudaError_t launch_w(TreeParams p, int num_sms, cudaStream_t st) {
-    using C = WCfg<D, RW>;
+    using C = WCfg<D, kF16, RW, kQ32>;
     static_assert(C::SMEM <= 227 * 1024 - 512, "shared memory");
-    auto kern = tree_warp_kernel<D, kF16, RW>;
+    auto kern = tree_warp_kernel<D, kF16, RW, kQ32>;
     static SmemSet set;  // one for each instantiation
     cudaError_t e = set.allow(kern, C::SMEM);
     if (e != cudaSuccess) return e;
@@ -355,20 +467,24 @@ cudaError_t launch_w(TreeParams p, int num_sms, cudaStream_t st) {
     return launch_tree_merge(p, D, num_sms, st);
 }
 
-template <int D, bool kF16>
-cudaError_t launch_rows(const TreeParams &p, uint32_t rows, int num_sms, cudaStream_t st) {
-    if (rows > 32) return launch_w<D, kF16, 4>(p, num_sms, st);
-    if (rows > 16) return launch_w<D, kF16, 2>(p, num_sms, st);
-    return launch_w<D, kF16, 1>(p, num_sms, st);
+template <int D, bool kF16, bool kQ32>
+cudaError_t launch_rows(const TreeArgs &a, cudaStream_t st) {
+    if (a.rows > 32) return launch_w<D, kF16, 4, kQ32>(a.p, a.num_sms, st);
+    if (a.rows > 16) return launch_w<D, kF16, 2, kQ32>(a.p, a.num_sms, st);
+    return launch_w<D, kF16, 1, kQ32>(a.p, a.num_sms, st);
+}
+
+template <int D>
+cudaError_t launch_types(const TreeArgs &a, cudaStream_t st) {
+    const bool f16 = a.kv_type == BML_F16;
+    if (a.p.q_type == BML_F32) return f16 ? launch_rows<D, true, true>(a, st) : launch_rows<D, false, true>(a, st);
+    return f16 ? launch_rows<D, true, false>(a, st) : launch_rows<D, false, false>(a, st);
 }
 
 }  // namespace
 
 cudaError_t launch_tree_warp(const TreeArgs &a, cudaStream_t st) {
-    const uint32_t rows = a.rows;
-    const bool f16 = a.kv_type == BML_F16;
-    if (a.D == 128) return f16 ? launch_rows<128, true>(a.p, rows, a.num_sms, st) : launch_rows<128, false>(a.p, rows, a.num_sms, st);
-    return f16 ? launch_rows<64, true>(a.p, rows, a.num_sms, st) : launch_rows<64, false>(a.p, rows, a.num_sms, st);
+    return a.D == 128 ? launch_types<128>(a, st) : launch_types<64>(a, st);
 }
 
 }  // namespace bml
