@@ -200,11 +200,6 @@ BML_API bml_status bml_attn_tree(const void *q_dev, bml_dtype q_dtype, uint32_t 
     const int sms = sm_count(this_device());
     if (workspace_bytes < bml::tree_workspace_bytes(head_dim, sms))
         return api_fail(BML_E_INVALID, "%s: workspace of %zu bytes, need %zu", fn, workspace_bytes, bml::tree_workspace_bytes(head_dim, sms));
-    // the schedule counts a launch's tiles (128 positions of up to 16 rows or more) in 32 bits
-    const uint64_t tiles = ((uint64_t)max_pages * page_size + bml::kTreeTile - 1) / bml::kTreeTile;
-    const uint64_t groups = (uint64_t)n_tokens * (n_heads / n_kv_heads) / 16 + bml::kTreeMaxSeqs;
-    if (groups * n_kv_heads > 0xffffffffull / tiles)
-        return api_fail(BML_E_UNSUPPORTED, "%s: %u tokens over tables of %u pages", fn, n_tokens, max_pages);
     const size_t es = bml::dtype_size(q_dtype);
     const uintptr_t qa = reinterpret_cast<uintptr_t>(q_dev), oa = reinterpret_cast<uintptr_t>(out_dev);
     if ((qa < oa ? oa - qa : qa - oa) < (uint64_t)n_tokens * n_heads * head_dim * es)

@@ -108,7 +108,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
     const size_t prow = (size_t)p.n_kv * D;  // elements of a pool row
     const uint32_t pmask = (1u << p.page_shift) - 1;
 
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const TreeRange range = tree_range(p, &sh, blockIdx.x, gridDim.x);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge, which waits for this grid
     TreeWalk walk(p, range);
     TreeSeg sg;
     while (walk.next(p, sg)) {
@@ -380,55 +382,140 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
 }
 
 // ---------------------------------------------------------------------------
-// Merge of the units that a cut divides.  CTA (x, y): cut x + 1 of the line;
-// it serves the unit that the cut divides, if it is the first cut in it, and
-// the rows y, y + gridDim.y, ... in blocks of 8 (a warp each).  Segments are
-// added in tile order, so a unit's result does not depend on timing.
+// Merge of the units that a cut divides.  With fewer units than cuts (by_unit)
+// CTA (x, y) serves unit x, else the unit that cut x + 1 divides, if that is
+// the first cut in it; it takes the unit's tasks y, y + gridDim.y, ... .
+// Segments are added in a fixed order, so a result does not depend on timing.
 // ---------------------------------------------------------------------------
 template <int D>
-__global__ void __launch_bounds__(kThreads) tree_merge_kernel(const __grid_constant__ TreeParams p, uint32_t grid) {
+__global__ void __launch_bounds__(kThreads) tree_merge_kernel(const __grid_constant__ TreeParams p, uint32_t grid, uint32_t by_unit) {
     __shared__ TreeShared sh;
-    const uint32_t b = blockIdx.x + 1;
-    const TreeRange range = tree_range(p, &sh, b, grid);
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // the segments' partials are written
-    if (range.w0 >= range.w1) return;
-    TreeWalk walk(p, range);
-    TreeSeg sg;
-    walk.next(p, sg);
-    if (sg.t0 == 0) return;  // the cut lies between two units
-    // the unit's place on the line, and the cuts inside it
-    const uint32_t u0 = range.w0 - sg.t0, u1 = u0 + sg.s.tiles;
-    if (tree_cut(range.total, b - 1, range.active) > u0) return;  // an earlier cut is inside the unit
-    uint32_t last = b;  // last CTA with a segment of the unit
-    while (last + 1 < range.active && tree_cut(range.total, last + 1, range.active) < u1) ++last;
-    // A warp takes 8 rows x 16 columns at a time (lane: row, 4 columns); the
-    // loads of up to 8 segments are in flight together.
+    __shared__ float4 s_acc[2][kWarps][32];
+    __shared__ float2 s_ml[kWarps][32];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t tasks = (sg.rows + 7) / 8 * (D / 16);
-    for (uint32_t task = blockIdx.y * kWarps + warp; task < tasks; task += gridDim.y * kWarps) {
-        const uint32_t r = task / (D / 16) * 8 + (lane & 7), x4 = task % (D / 16) * 4 + (lane >> 3);
-        if (r >= sg.rows) continue;
-        float m = -INFINITY;
-#pragma unroll 8
-        for (uint32_t s = b - 1; s <= last; ++s)
-            m = fmaxf(m, tree_part(p, D, s, s == b - 1 ? 1u : 0u)[(size_t)p.rpg * D + r]);
-        if (m == -INFINITY) m = 0.f;
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        float l = 0.f;
-#pragma unroll 8
-        for (uint32_t s = b - 1; s <= last; ++s) {
-            const float *part = tree_part(p, D, s, s == b - 1 ? 1u : 0u);
-            const float f = exp2f(part[(size_t)p.rpg * D + r] - m);
-            const float4 y = reinterpret_cast<const float4 *>(part)[x4 * p.rpg + r];
-            l += f * part[(size_t)p.rpg * (D + 1) + r];
-            acc.x += f * y.x;
-            acc.y += f * y.y;
-            acc.z += f * y.z;
-            acc.w += f * y.w;
+    TreeSeg sg;
+    uint32_t u0, total, b;
+    // (the lengths are inputs of the call, not results of the kernel before;
+    // that kernel has waited for their writer)
+    if (by_unit) {
+        const TreeUnit u = tree_unit(p, &sh, blockIdx.x);
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // the segments' partials are written
+        if (!u.found) return;
+        total = u.total;
+        u0 = u.u0;
+        sg.seq = u.seq;
+        sg.head = u.head;
+        sg.s = u.s;
+        sg.row0 = u.rg * p.rpg;
+        b = TreeCuts(total, grid).owner(u0) + 1;  // the first cut behind u0
+    } else {
+        b = blockIdx.x + 1;
+        const TreeRange range = tree_range(p, &sh, b, grid);
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (range.w0 >= range.w1) return;
+        TreeWalk walk(p, range);
+        walk.next(p, sg);
+        if (sg.t0 == 0) return;  // the cut lies between two units
+        total = range.total;
+        u0 = range.w0 - sg.t0;
+    }
+    const TreeCuts cuts(total, grid);
+    // the CTAs with a segment of the unit: b - 1 to last
+    const uint32_t last = cuts.owner(u0 + sg.s.tiles - 1);
+    if (last < b || cuts.at(b - 1) > u0) return;  // not divided, or an earlier cut is inside the unit
+    sg.rows = min(p.rpg, sg.s.rows - sg.row0);
+    // A task is 8 rows x 32 columns (lane: row, twice 4 columns).  Up to 32
+    // segments: a warp a task, the loads of 6 segments in flight together; more
+    // (one long request): a CTA a task, the warps taking the segments in turns
+    // and meeting in shared memory.
+    constexpr uint32_t kBatch = 6;
+    const uint32_t R = p.rpg * p.hpu, tasks = (R + 7) / 8 * (D / 32);
+    const bool many = last - b > 30;
+    const uint32_t step = many ? kWarps : 1;
+    for (uint32_t task = many ? blockIdx.y : blockIdx.y * kWarps + warp; task < tasks; task += gridDim.y * (many ? 1 : kWarps)) {
+        const uint32_t row = task / (D / 32) * 8 + (lane & 7), x4 = task % (D / 32) * 8 + (lane >> 3);
+        const uint32_t h = row / p.rpg, r = row - h * p.rpg;
+        const bool valid = row < R && r < sg.rows;
+        if (!many && !valid) continue;
+        float m = -INFINITY, l = 0.f;
+        float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+        if (valid) {
+            const uint32_t first = b - 1 + (many ? warp : 0);
+            const size_t slot = (size_t)R * (D + 2);
+            auto seg_part = [&](uint32_t s) { return p.part + (2 * (size_t)s + (s == b - 1 ? 1 : 0)) * slot; };
+            // batches of explicit loads: a loop over segments is not unrolled so
+            // that its loads overlap
+            for (uint32_t s0 = first; s0 <= last; s0 += kBatch * step) {
+                float y[kBatch];
+#pragma unroll
+                for (uint32_t u = 0; u < kBatch; ++u) {
+                    const uint32_t s = s0 + u * step;
+                    y[u] = s <= last ? seg_part(s)[(size_t)R * D + row] : -INFINITY;
+                }
+#pragma unroll
+                for (uint32_t u = 0; u < kBatch; ++u) m = fmaxf(m, y[u]);
+            }
+            const float mu = m == -INFINITY ? 0.f : m;
+            for (uint32_t s0 = first; s0 <= last; s0 += kBatch * step) {
+                float f[kBatch], ls[kBatch];
+                float4 y[kBatch][2];
+#pragma unroll
+                for (uint32_t u = 0; u < kBatch; ++u) {
+                    const uint32_t s = s0 + u * step;
+                    const float *part = seg_part(s <= last ? s : last);
+                    f[u] = part[(size_t)R * D + row];
+                    ls[u] = part[(size_t)R * (D + 1) + row];
+                    y[u][0] = reinterpret_cast<const float4 *>(part)[x4 * R + row];
+                    y[u][1] = reinterpret_cast<const float4 *>(part)[(x4 + 4) * R + row];
+                }
+#pragma unroll
+                for (uint32_t u = 0; u < kBatch; ++u) {
+                    if (s0 + u * step > last) break;
+                    const float w = exp2f(f[u] - mu);
+                    l += w * ls[u];
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        acc[z].x += w * y[u][z].x;
+                        acc[z].y += w * y[u][z].y;
+                        acc[z].z += w * y[u][z].z;
+                        acc[z].w += w * y[u][z].w;
+                    }
+                }
+            }
+        }
+        if (many) {
+            __syncthreads();
+            s_acc[0][warp][lane] = acc[0];
+            s_acc[1][warp][lane] = acc[1];
+            s_ml[warp][lane] = make_float2(m, l);
+            __syncthreads();
+            if (warp != 0 || !valid) continue;
+            m = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_ml[w][lane].x);
+            const float mu = m == -INFINITY ? 0.f : m;
+            l = 0.f;
+            acc[0] = acc[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float2 a = s_ml[w][lane];
+                const float f = exp2f(a.x - mu);
+                l += f * a.y;
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                    const float4 y = s_acc[z][w][lane];
+                    acc[z].x += f * y.x;
+                    acc[z].y += f * y.y;
+                    acc[z].z += f * y.z;
+                    acc[z].w += f * y.w;
+                }
+            }
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        const size_t at = tree_row(p, sg, sg.row0 + r, D) + x4 * 4;
-        store_out4(p.out, p.q_type, at, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        const size_t at = tree_row(p, sg, sg.row0 + r, D, h) + x4 * 4;
+#pragma unroll
+        for (int z = 0; z < 2; ++z)
+            store_out4(p.out, p.q_type, at + 16 * z, make_float4(acc[z].x * inv, acc[z].y * inv, acc[z].z * inv, acc[z].w * inv));
     }
 }
 
@@ -441,9 +528,10 @@ cudaError_t launch_f32(TreeParams p, int num_sms, cudaStream_t st) {
     cudaError_t e = set.allow(kern, C::SMEM);
     if (e != cudaSuccess) return e;
     p.rpg = RW * 16;
-    p.min_tiles = 1;
-    kern<<<num_sms, kThreads, C::SMEM, st>>>(p);
-    e = cudaGetLastError();
+    p.hpu = 1;
+    p.tile = kTreeTile;
+    if (!tree_line_fits(p)) return cudaErrorNotSupported;
+    e = launch_after(kern, dim3(num_sms), kThreads, C::SMEM, st, p);
     if (e != cudaSuccess) return e;
     return launch_tree_merge(p, D, num_sms, st);
 }
@@ -468,18 +556,15 @@ cudaError_t launch_kv(const TreeArgs &a, cudaStream_t st) {
 
 cudaError_t launch_tree_merge(const TreeParams &p, uint32_t D, int grid, cudaStream_t st) {
     if (grid < 2) return cudaSuccess;
-    cudaLaunchConfig_t cfg = {};
-    // 16 CTAs for 256 rows; a CTA has 8 tasks of 8 rows x 16 columns at a time
-    cfg.gridDim = dim3(grid - 1, p.rpg > 64 ? 16 : (p.rpg + 7) / 8 * (D / 16) / kWarps);
-    cfg.blockDim = dim3(kThreads);
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return D == 128 ? cudaLaunchKernelEx(&cfg, tree_merge_kernel<128>, p, (uint32_t)grid)
-                    : cudaLaunchKernelEx(&cfg, tree_merge_kernel<64>, p, (uint32_t)grid);
+    const uint64_t units = tree_most_units(p);
+    const bool by_unit = units < (uint64_t)(grid - 1);
+    const uint32_t x = by_unit ? (uint32_t)units : (uint32_t)(grid - 1);
+    // about 8 CTAs an SM, no more than the tasks
+    const uint32_t tasks = (p.rpg * p.hpu + 7) / 8 * (D / 32);
+    uint32_t y = (uint32_t)grid * 8 / x;
+    y = y < 1 ? 1 : y > tasks ? tasks : y;
+    return D == 128 ? launch_after(tree_merge_kernel<128>, dim3(x, y), kThreads, 0, st, p, (uint32_t)grid, (uint32_t)by_unit)
+                    : launch_after(tree_merge_kernel<64>, dim3(x, y), kThreads, 0, st, p, (uint32_t)grid, (uint32_t)by_unit);
 }
 
 size_t tree_workspace_bytes(uint32_t D, int num_sms) {
@@ -490,6 +575,7 @@ cudaError_t launch_tree(const TreeArgs &a, cudaStream_t st) {
     // 16-bit pages, except for a scale of 0 (those kernels scale masked scores
     // after they were set to -inf)
     if (a.kv_type != BML_F32 && a.p.scale_log2 > 0.f) {
+        if (a.rows <= 8) return launch_tree_few(a, st);
         if (a.p.q_type == BML_F32 || a.rows <= 64 || !tree_umma_fits(a)) return launch_tree_warp(a, st);
         return launch_tree_umma(a, st);
     }

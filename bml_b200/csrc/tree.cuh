@@ -8,7 +8,7 @@
 
 namespace bml {
 
-constexpr int kTreeTile = 128;         // positions of one schedule tile
+constexpr int kTreeTile = 128;         // positions of one schedule tile, but for tree_few_kernel
 constexpr uint32_t kTreeMaxSeqs = 1024;  // requests of one launch
 
 struct TreeParams {
@@ -21,11 +21,12 @@ struct TreeParams {
     uint32_t n_seqs, n_tokens, n_heads, n_kv, group, max_pages, n_pages, page_shift, n_words;
     float scale_log2;
     int q_type;  // bml_dtype of q and out
-    // partials: slots of rpg rows, o [D / 4][rpg][4] un-normalised (a warp whose
-    // lanes hold rows writes whole lines), then m [rpg], l [rpg]
+    // partials: slots of R = hpu * rpg rows, o [D / 4][R][4] un-normalised (a warp
+    // whose lanes hold rows writes whole lines), then m [R], l [R]
     float *part;
     uint32_t rpg;        // rows of a row group
-    uint32_t min_tiles;  // tiles a CTA takes at least
+    uint32_t hpu;        // kv heads of a unit
+    uint32_t tile;       // positions of a schedule tile
 };
 
 struct TreeArgs {
@@ -36,7 +37,7 @@ struct TreeArgs {
     int num_sms;
 };
 
-constexpr uint32_t kTreeMaxRows = 256;  // rows of the largest row group
+constexpr uint32_t kTreeMaxRows = 256;  // rows of the largest partial slot
 cudaError_t launch_tree_merge(const TreeParams &p, uint32_t D, int grid, cudaStream_t st);
 size_t tree_workspace_bytes(uint32_t D, int num_sms);
 
@@ -58,15 +59,44 @@ struct SmemSet {
 cudaError_t launch_tree(const TreeArgs &a, cudaStream_t st);
 bool tree_umma_fits(const TreeArgs &a);
 cudaError_t launch_tree_warp(const TreeArgs &a, cudaStream_t st);
+cudaError_t launch_tree_few(const TreeArgs &a, cudaStream_t st);
 cudaError_t launch_tree_umma(const TreeArgs &a, cudaStream_t st);
+
+// Whether the schedule can count the launch's tiles in 32 bits, whatever the
+// lengths on the device are.
+inline uint64_t tree_most_units(const TreeParams &p) {
+    return ((uint64_t)p.n_tokens * p.group / p.rpg + p.n_seqs) * (p.n_kv / p.hpu);
+}
+inline bool tree_line_fits(const TreeParams &p) {
+    const uint64_t tiles = (((uint64_t)p.max_pages << p.page_shift) + p.tile - 1) / p.tile;
+    return tree_most_units(p) <= 0xffffffffull / tiles;
+}
+
+// A launch that may begin while the kernel before it on the stream ends; the
+// tree kernels wait for that kernel (griddepcontrol.wait) before they read or
+// write global memory.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, int threads, int smem, cudaStream_t st, const Args &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
 
 #ifdef __CUDACC__
 // ---------------------------------------------------------------------------
-// Schedule.  A unit is one (request, kv head, row group): the query rows
-// (node t, q head g of the kv head) of up to rpg consecutive t * group + g,
-// over all positions of the request.  Units are laid out request by request,
-// kv head by kv head, row group by row group, each as its number of
-// 128-position tiles, and the line of all tiles is cut evenly over the CTAs,
+// Schedule.  A unit is one (request, hpu kv heads, row group): for each of the
+// heads the query rows (node t, q head g of the kv head) of up to rpg
+// consecutive t * group + g, over all positions of the request.  Units are laid
+// out request by request, heads by heads, row group by row group, each as its
+// number of tiles of positions, and the line of all tiles is cut evenly over the CTAs,
 // so the lengths stay on the GPU and no CTA works longer than another by more
 // than a tile.  A unit that a cut divides leaves partial results (max, sum,
 // un-normalised output) which tree_merge_kernel joins in tile order.
@@ -88,27 +118,37 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, uint32_t i) {
     s.L = ok ? (uint32_t)L : 0u;
     s.rows = s.T * p.group;
     s.groups = (s.rows + p.rpg - 1) / p.rpg;
-    s.tiles = s.L ? (s.L + kTreeTile - 1) / kTreeTile : 1u;
+    s.tiles = s.L ? (s.L + p.tile - 1) / p.tile : 1u;
     return s;
 }
 
 struct TreeShared {
-    uint32_t warp_sums[32];
+    uint32_t warp_sums[32], warp_units[32];
     uint32_t base;  // place of seq's first tile on the line
-    uint32_t seq;
+    uint32_t seq, unit;
 };
 
-// Where cut b of n falls on a line of `total` tiles: total * b / n, without
-// its 64-bit division.
-__device__ __forceinline__ uint32_t tree_cut(uint32_t total, uint32_t b, uint32_t n) {
-    const uint32_t q = total / n;
-    return q * b + (total - q * n) * b / n;
-}
+// How a line of `total` tiles is cut for `active` CTAs: the first `more` take
+// one tile more than the others.
+struct TreeCuts {
+    uint32_t each, more, active;
+    __device__ __forceinline__ TreeCuts(uint32_t total, uint32_t grid) {
+        active = total < grid ? total : grid;
+        each = active ? total / active : 0u;
+        more = total - each * active;
+    }
+    __device__ __forceinline__ uint32_t at(uint32_t b) const { return each * b + min(b, more); }
+    // the CTA that takes tile w
+    __device__ __forceinline__ uint32_t owner(uint32_t w) const {
+        const uint32_t wide = more * (each + 1);
+        return w < wide ? w / (each + 1) : more + (w - wide) / each;
+    }
+};
 
 // CTA b's range of the line, and where it starts.
 struct TreeRange {
     uint32_t w0, w1, base, total;
-    uint32_t seq, active;  // CTAs that share the line
+    uint32_t seq;
 };
 
 // Every thread of the CTA calls it (blockDim a multiple of 32); three
@@ -119,7 +159,7 @@ __device__ __forceinline__ TreeRange tree_range(const TreeParams &p, TreeShared 
     const uint32_t i0 = min(threadIdx.x * per, p.n_seqs), i1 = min(i0 + per, p.n_seqs);
     auto cost = [&](uint32_t i) {
         const TreeSeq s = tree_seq(p, i);
-        return s.tiles * s.groups * p.n_kv;
+        return s.tiles * s.groups * (p.n_kv / p.hpu);
     };
     uint32_t sum = 0;
     for (uint32_t i = i0; i < i1; ++i) sum += cost(i);
@@ -138,13 +178,12 @@ __device__ __forceinline__ TreeRange tree_range(const TreeParams &p, TreeShared 
         total += s;
     }
     TreeRange r;
+    const TreeCuts cuts(total, grid);
     r.total = total;
-    const uint32_t most = (total + p.min_tiles - 1) / p.min_tiles;
-    r.active = most < grid ? (uint32_t)most : grid;
     r.w0 = r.w1 = 0;
-    if (b < r.active) {
-        r.w0 = tree_cut(total, b, r.active);
-        r.w1 = tree_cut(total, b + 1, r.active);
+    if (b < cuts.active) {
+        r.w0 = cuts.at(b);
+        r.w1 = cuts.at(b + 1);
     }
     if (r.w0 < r.w1 && r.w0 >= first && r.w0 < first + sum) {
         uint32_t at = first;
@@ -165,9 +204,81 @@ __device__ __forceinline__ TreeRange tree_range(const TreeParams &p, TreeShared 
     return r;
 }
 
+// A unit's place on the line: tiles [u0, u0 + s.tiles).
+struct TreeUnit {
+    uint32_t u0, total;
+    uint32_t seq, head, rg;
+    TreeSeq s;
+    bool found;
+};
+
+// The unit with index u in line order.  As tree_range: every thread calls it.
+__device__ __forceinline__ TreeUnit tree_unit(const TreeParams &p, TreeShared *sh, uint32_t u) {
+    const uint32_t nt = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t per = (p.n_seqs + nt - 1) / nt;
+    const uint32_t i0 = min(threadIdx.x * per, p.n_seqs), i1 = min(i0 + per, p.n_seqs);
+    uint32_t tiles = 0, units = 0;
+    for (uint32_t i = i0; i < i1; ++i) {
+        const TreeSeq s = tree_seq(p, i);
+        const uint32_t n = s.groups * (p.n_kv / p.hpu);
+        units += n;
+        tiles += n * s.tiles;
+    }
+    uint32_t inc_t = tiles, inc_u = units;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t a = __shfl_up_sync(0xffffffffu, inc_t, o), b = __shfl_up_sync(0xffffffffu, inc_u, o);
+        if (lane >= (uint32_t)o) {
+            inc_t += a;
+            inc_u += b;
+        }
+    }
+    if (lane == 31) {
+        sh->warp_sums[warp] = inc_t;
+        sh->warp_units[warp] = inc_u;
+    }
+    __syncthreads();
+    uint32_t ft = inc_t - tiles, fu = inc_u - units, all_t = 0, all_u = 0;
+    for (uint32_t w = 0; w < nt / 32; ++w) {
+        if (w < warp) {
+            ft += sh->warp_sums[w];
+            fu += sh->warp_units[w];
+        }
+        all_t += sh->warp_sums[w];
+        all_u += sh->warp_units[w];
+    }
+    if (u >= fu && u < fu + units) {
+        uint32_t i = i0;
+        while (true) {
+            const TreeSeq s = tree_seq(p, i);
+            const uint32_t n = s.groups * (p.n_kv / p.hpu);
+            if (u < fu + n) break;
+            fu += n;
+            ft += n * s.tiles;
+            ++i;
+        }
+        sh->seq = i;
+        sh->base = ft;
+        sh->unit = u - fu;
+    }
+    __syncthreads();
+    TreeUnit r;
+    r.found = u < all_u;
+    r.total = all_t;
+    if (r.found) {
+        r.seq = sh->seq;
+        r.s = tree_seq(p, r.seq);
+        r.head = sh->unit / r.s.groups;
+        r.rg = sh->unit - r.head * r.s.groups;
+        r.head *= p.hpu;
+        r.u0 = sh->base + sh->unit * r.s.tiles;
+    }
+    return r;
+}
+
 // The segments of a range in order: consecutive tiles of one unit.
 struct TreeSeg {
-    uint32_t seq, head, rg;
+    uint32_t seq, head, rg;  // head: the first of the unit's
     uint32_t t0, t1;     // tiles of the unit, [t0, t1)
     uint32_t row0, rows; // first row (t * group + g) and row count of the group
     uint32_t slot;       // partial slot of the CTA: 0 the unit began before this range, 1 it ends after it, 2 whole
@@ -184,7 +295,7 @@ struct TreeWalk {
     __device__ __forceinline__ bool next(const TreeParams &p, TreeSeg &g) {
         if (pos >= end) return false;
         uint32_t units;
-        while (pos - base >= (units = s.groups * p.n_kv) * s.tiles) {
+        while (pos - base >= (units = s.groups * (p.n_kv / p.hpu)) * s.tiles) {
             base += units * s.tiles;
             s = tree_seq(p, ++seq);
         }
@@ -195,6 +306,7 @@ struct TreeWalk {
         g.s = s;
         g.head = u / s.groups;
         g.rg = u - g.head * s.groups;
+        g.head *= p.hpu;
         g.t0 = off - u * s.tiles;
         g.t1 = left < s.tiles - g.t0 ? g.t0 + left : s.tiles;
         g.row0 = g.rg * p.rpg;
@@ -207,13 +319,13 @@ struct TreeWalk {
 
 // Partial slot `which` (0 or 1) of CTA b.
 __device__ __forceinline__ float *tree_part(const TreeParams &p, uint32_t D, uint32_t b, uint32_t which) {
-    return p.part + (size_t)(2 * b + which) * p.rpg * (D + 2);
+    return p.part + (size_t)(2 * b + which) * p.rpg * p.hpu * (D + 2);
 }
 
-// Element index of row r (t * group + g) of kv head h of a request in q and out.
-__device__ __forceinline__ size_t tree_row(const TreeParams &p, const TreeSeg &g, uint32_t r, uint32_t D) {
+// Element index of row r (t * group + g) of the unit's kv head `h` in q and out.
+__device__ __forceinline__ size_t tree_row(const TreeParams &p, const TreeSeg &g, uint32_t r, uint32_t D, uint32_t h = 0) {
     const uint32_t t = r / p.group, qg = r - t * p.group;
-    return ((size_t)(g.s.first + t) * p.n_heads + (size_t)g.head * p.group + qg) * D;
+    return ((size_t)(g.s.first + t) * p.n_heads + (size_t)(g.head + h) * p.group + qg) * D;
 }
 
 // Whether node t of a request sees position pos >= P (= node pos - P).

@@ -224,6 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     tc_fence_before();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const TreeRange range = tree_range(p, &sh.sched, blockIdx.x, gridDim.x);  // has the barriers for the set-up above
     tc_fence_after();
     const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
@@ -788,8 +789,7 @@ cudaError_t launch_u(const UmmaParams &up, int num_sms, cudaStream_t st) {
     static SmemSet set;  // one for each instantiation
     cudaError_t e = set.allow(kern, C::SMEM);
     if (e != cudaSuccess) return e;
-    kern<<<num_sms, kThreads, C::SMEM, st>>>(up);
-    e = cudaGetLastError();
+    e = launch_after(kern, dim3(num_sms), kThreads, C::SMEM, st, up);
     if (e != cudaSuccess) return e;
     return launch_tree_merge(up.t, D, num_sms, st);
 }
@@ -806,7 +806,9 @@ cudaError_t launch_tree_umma(const TreeArgs &a, cudaStream_t st) {
     up.rt = BM / group * group;
     up.box_rows = page < (uint32_t)BN ? page : (uint32_t)BN;
     up.t.rpg = 2 * up.rt;
-    up.t.min_tiles = 1;
+    up.t.hpu = 1;
+    up.t.tile = kTreeTile;
+    if (!tree_line_fits(up.t)) return cudaErrorNotSupported;
     const uint64_t rows = (uint64_t)a.p.n_pages << a.p.page_shift;
     if (!tree_map(&up.tq, a.p.q, f16, a.D, a.p.n_heads, a.p.n_tokens, group, BM / group) ||
         !tree_map(&up.tk, a.p.k, f16, a.D, a.p.n_kv, rows, 1, up.box_rows) ||

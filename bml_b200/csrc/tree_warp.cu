@@ -107,6 +107,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
     const size_t prow = (size_t)p.n_kv * D * 2;  // bytes of a pool row
     const uint32_t pmask = (1u << p.page_shift) - 1;
 
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const TreeRange range = tree_range(p, &sh, blockIdx.x, gridDim.x);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
@@ -460,9 +461,10 @@ cudaError_t launch_w(TreeParams p, int num_sms, cudaStream_t st) {
     cudaError_t e = set.allow(kern, C::SMEM);
     if (e != cudaSuccess) return e;
     p.rpg = RW * 16;
-    p.min_tiles = 1;
-    kern<<<num_sms, kThreads, C::SMEM, st>>>(p);
-    e = cudaGetLastError();
+    p.hpu = 1;
+    p.tile = kTreeTile;
+    if (!tree_line_fits(p)) return cudaErrorNotSupported;
+    e = launch_after(kern, dim3(num_sms), kThreads, C::SMEM, st, p);
     if (e != cudaSuccess) return e;
     return launch_tree_merge(p, D, num_sms, st);
 }
