@@ -388,47 +388,54 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
 // Segments are added in a fixed order, so a result does not depend on timing.
 // ---------------------------------------------------------------------------
 template <int D>
-__global__ void __launch_bounds__(kThreads) tree_merge_kernel(const __grid_constant__ TreeParams p, uint32_t grid, uint32_t by_unit) {
+__global__ void __launch_bounds__(kThreads, 2) tree_merge_kernel(const __grid_constant__ TreeParams p, uint32_t grid, uint32_t by_unit) {
     __shared__ TreeShared sh;
     __shared__ float4 s_acc[2][kWarps][32];
     __shared__ float2 s_ml[kWarps][32];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    TreeSeg sg;
-    uint32_t u0, total, b;
-    // (the lengths are inputs of the call, not results of the kernel before;
-    // that kernel has waited for their writer)
+    TreeSeg sg = {};
+    uint32_t u0 = 0, total = 0, b = 0;
+    // (the lengths are inputs of the call, not results of the kernel before,
+    // and that kernel has waited for their writer)
+    bool mine;
     if (by_unit) {
         const TreeUnit u = tree_unit(p, &sh, blockIdx.x);
-        asm volatile("griddepcontrol.wait;" ::: "memory");  // the segments' partials are written
-        if (!u.found) return;
-        total = u.total;
-        u0 = u.u0;
-        sg.seq = u.seq;
-        sg.head = u.head;
-        sg.s = u.s;
-        sg.row0 = u.rg * p.rpg;
-        b = TreeCuts(total, grid).owner(u0) + 1;  // the first cut behind u0
+        mine = u.found;
+        if (mine) {
+            total = u.total;
+            u0 = u.u0;
+            sg.seq = u.seq;
+            sg.head = u.head;
+            sg.s = u.s;
+            sg.row0 = u.rg * p.rpg;
+            b = TreeCuts(total, grid).owner(u0) + 1;  // the first cut behind u0
+        }
     } else {
         b = blockIdx.x + 1;
         const TreeRange range = tree_range(p, &sh, b, grid);
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-        if (range.w0 >= range.w1) return;
-        TreeWalk walk(p, range);
-        walk.next(p, sg);
-        if (sg.t0 == 0) return;  // the cut lies between two units
-        total = range.total;
-        u0 = range.w0 - sg.t0;
+        mine = range.w0 < range.w1;
+        if (mine) {
+            TreeWalk walk(p, range);
+            walk.next(p, sg);
+            mine = sg.t0 > 0;  // else the cut lies between two units
+            total = range.total;
+            u0 = range.w0 - sg.t0;
+        }
     }
-    const TreeCuts cuts(total, grid);
-    // the CTAs with a segment of the unit: b - 1 to last
-    const uint32_t last = cuts.owner(u0 + sg.s.tiles - 1);
-    if (last < b || cuts.at(b - 1) > u0) return;  // not divided, or an earlier cut is inside the unit
-    sg.rows = min(p.rpg, sg.s.rows - sg.row0);
+    uint32_t last = 0;  // the CTAs with a segment of the unit: b - 1 to last
+    if (mine) {
+        const TreeCuts cuts(total, grid);
+        last = cuts.owner(u0 + sg.s.tiles - 1);
+        mine = last >= b && cuts.at(b - 1) <= u0;  // divided, and no earlier cut inside the unit
+        sg.rows = min(p.rpg, sg.s.rows - sg.row0);
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the segments' partials are written
+    if (!mine) return;
     // A task is 8 rows x 32 columns (lane: row, twice 4 columns).  Up to 32
-    // segments: a warp a task, the loads of 6 segments in flight together; more
+    // segments: a warp a task, the loads of 8 segments in flight together; more
     // (one long request): a CTA a task, the warps taking the segments in turns
     // and meeting in shared memory.
-    constexpr uint32_t kBatch = 6;
+    constexpr uint32_t kBatch = 8;
     const uint32_t R = p.rpg * p.hpu, tasks = (R + 7) / 8 * (D / 32);
     const bool many = last - b > 30;
     const uint32_t step = many ? kWarps : 1;
@@ -443,34 +450,38 @@ __global__ void __launch_bounds__(kThreads) tree_merge_kernel(const __grid_const
             const uint32_t first = b - 1 + (many ? warp : 0);
             const size_t slot = (size_t)R * (D + 2);
             auto seg_part = [&](uint32_t s) { return p.part + (2 * (size_t)s + (s == b - 1 ? 1 : 0)) * slot; };
-            // batches of explicit loads: a loop over segments is not unrolled so
-            // that its loads overlap
-            for (uint32_t s0 = first; s0 <= last; s0 += kBatch * step) {
-                float y[kBatch];
-#pragma unroll
-                for (uint32_t u = 0; u < kBatch; ++u) {
-                    const uint32_t s = s0 + u * step;
-                    y[u] = s <= last ? seg_part(s)[(size_t)R * D + row] : -INFINITY;
-                }
-#pragma unroll
-                for (uint32_t u = 0; u < kBatch; ++u) m = fmaxf(m, y[u]);
-            }
-            const float mu = m == -INFINITY ? 0.f : m;
+            // Batches of explicit loads: a loop over segments is not unrolled so
+            // that its loads overlap.  The running maximum is kept per batch.
             for (uint32_t s0 = first; s0 <= last; s0 += kBatch * step) {
                 float f[kBatch], ls[kBatch];
                 float4 y[kBatch][2];
 #pragma unroll
                 for (uint32_t u = 0; u < kBatch; ++u) {
                     const uint32_t s = s0 + u * step;
-                    const float *part = seg_part(s <= last ? s : last);
+                    const float *part = seg_part(min(s, last));
                     f[u] = part[(size_t)R * D + row];
                     ls[u] = part[(size_t)R * (D + 1) + row];
                     y[u][0] = reinterpret_cast<const float4 *>(part)[x4 * R + row];
                     y[u][1] = reinterpret_cast<const float4 *>(part)[(x4 + 4) * R + row];
                 }
+                float mn = m;
 #pragma unroll
                 for (uint32_t u = 0; u < kBatch; ++u) {
-                    if (s0 + u * step > last) break;
+                    if (s0 + u * step > last) f[u] = -INFINITY;
+                    mn = fmaxf(mn, f[u]);
+                }
+                const float mu = mn == -INFINITY ? 0.f : mn, old = exp2f(m - mu);  // m -inf: 0
+                l *= old;
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                    acc[z].x *= old;
+                    acc[z].y *= old;
+                    acc[z].z *= old;
+                    acc[z].w *= old;
+                }
+#pragma unroll
+                for (uint32_t u = 0; u < kBatch; ++u) {
+                    if (s0 + u * step > last) continue;
                     const float w = exp2f(f[u] - mu);
                     l += w * ls[u];
 #pragma unroll
@@ -481,6 +492,7 @@ __global__ void __launch_bounds__(kThreads) tree_merge_kernel(const __grid_const
                         acc[z].w += w * y[u][z].w;
                     }
                 }
+                m = mn;
             }
         }
         if (many) {

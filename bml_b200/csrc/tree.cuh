@@ -151,56 +151,122 @@ struct TreeRange {
     uint32_t seq;
 };
 
-// Every thread of the CTA calls it (blockDim a multiple of 32); three
-// barriers.  w0 == w1: nothing for this CTA.
-__device__ __forceinline__ TreeRange tree_range(const TreeParams &p, TreeShared *sh, uint32_t b, uint32_t grid) {
-    const uint32_t nt = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t per = (p.n_seqs + nt - 1) / nt;
-    const uint32_t i0 = min(threadIdx.x * per, p.n_seqs), i1 = min(i0 + per, p.n_seqs);
-    auto cost = [&](uint32_t i) {
-        const TreeSeq s = tree_seq(p, i);
-        return s.tiles * s.groups * (p.n_kv / p.hpu);
-    };
-    uint32_t sum = 0;
-    for (uint32_t i = i0; i < i1; ++i) sum += cost(i);
-    uint32_t inc = sum;
+// The request that holds tile w (by_unit: unit w) of the line.  Up to 128
+// requests every warp finds it by itself (four requests a lane, no barrier);
+// with more the CTA's threads share them.  Every thread of the CTA calls it.
+struct TreePlace {
+    uint32_t total, units;  // of the line
+    uint32_t seq, base, unit0;  // the request, its first tile, its first unit
+};
+
+template <typename Target>
+__device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *sh, bool by_unit, Target target) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, upr = p.n_kv / p.hpu;
+    const bool alone = p.n_seqs <= 128;
+    const uint32_t members = alone ? 32u : blockDim.x, me = alone ? lane : threadIdx.x;
+    const uint32_t per = (p.n_seqs + members - 1) / members;
+    const uint32_t i0 = min(me * per, p.n_seqs), i1 = min(i0 + per, p.n_seqs);
+    uint32_t tiles = 0, units = 0;
+    uint32_t n4[4] = {0, 0, 0, 0}, t4[4] = {0, 0, 0, 0};  // alone: units and tiles of the lane's requests
+    if (alone) {
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k)
+            if (i0 + k < i1) {
+                const TreeSeq s = tree_seq(p, i0 + k);
+                n4[k] = s.groups * upr;
+                t4[k] = n4[k] * s.tiles;
+                units += n4[k];
+                tiles += t4[k];
+            }
+    } else {
+        for (uint32_t i = i0; i < i1; ++i) {
+            const TreeSeq s = tree_seq(p, i);
+            units += s.groups * upr;
+            tiles += s.groups * upr * s.tiles;
+        }
+    }
+    uint32_t inc_t = tiles, inc_u = units;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t u = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= (uint32_t)o) inc += u;
-    }
-    if (lane == 31) sh->warp_sums[warp] = inc;
-    __syncthreads();
-    uint32_t first = inc - sum, total = 0;
-    for (uint32_t w = 0; w < nt / 32; ++w) {
-        const uint32_t s = sh->warp_sums[w];
-        if (w < warp) first += s;
-        total += s;
-    }
-    TreeRange r;
-    const TreeCuts cuts(total, grid);
-    r.total = total;
-    r.w0 = r.w1 = 0;
-    if (b < cuts.active) {
-        r.w0 = cuts.at(b);
-        r.w1 = cuts.at(b + 1);
-    }
-    if (r.w0 < r.w1 && r.w0 >= first && r.w0 < first + sum) {
-        uint32_t at = first;
-        uint32_t i = i0;
-        while (true) {
-            const uint32_t c = cost(i);
-            if (r.w0 < at + c) break;
-            at += c;
-            ++i;
+        const uint32_t a = __shfl_up_sync(0xffffffffu, inc_t, o), b = __shfl_up_sync(0xffffffffu, inc_u, o);
+        if (lane >= (uint32_t)o) {
+            inc_t += a;
+            inc_u += b;
         }
-        sh->seq = i;
-        sh->base = at;
     }
-    __syncthreads();
-    r.seq = sh->seq;
-    r.base = sh->base;
-    __syncthreads();
+    TreePlace r;
+    uint32_t ft = inc_t - tiles, fu = inc_u - units;
+    if (alone) {
+        r.total = __shfl_sync(0xffffffffu, inc_t, 31);
+        r.units = __shfl_sync(0xffffffffu, inc_u, 31);
+    } else {
+        if (lane == 31) {
+            sh->warp_sums[warp] = inc_t;
+            sh->warp_units[warp] = inc_u;
+        }
+        __syncthreads();
+        r.total = r.units = 0;
+        for (uint32_t w = 0; w < blockDim.x / 32; ++w) {
+            if (w < warp) {
+                ft += sh->warp_sums[w];
+                fu += sh->warp_units[w];
+            }
+            r.total += sh->warp_sums[w];
+            r.units += sh->warp_units[w];
+        }
+    }
+    const uint32_t w = target(r.total);
+    const bool mine = by_unit ? w >= fu && w < fu + units : w >= ft && w < ft + tiles;
+    uint32_t seq = i0;
+    if (alone) {
+#pragma unroll
+        for (uint32_t k = 0; k < 3; ++k)
+            if (mine && seq == i0 + k && (by_unit ? w >= fu + n4[k] : w >= ft + t4[k])) {
+                fu += n4[k];
+                ft += t4[k];
+                ++seq;
+            }
+        const uint32_t who = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;  // none: lane 31's, unused
+        r.seq = __shfl_sync(0xffffffffu, seq, who & 31);
+        r.base = __shfl_sync(0xffffffffu, ft, who & 31);
+        r.unit0 = __shfl_sync(0xffffffffu, fu, who & 31);
+    } else {
+        if (mine) {
+            while (true) {
+                const TreeSeq s = tree_seq(p, seq);
+                const uint32_t n = s.groups * upr;
+                if (by_unit ? w < fu + n : w < ft + n * s.tiles) break;
+                fu += n;
+                ft += n * s.tiles;
+                ++seq;
+            }
+            sh->seq = seq;
+            sh->base = ft;
+            sh->unit = fu;
+        }
+        __syncthreads();
+        r.seq = sh->seq;
+        r.base = sh->base;
+        r.unit0 = sh->unit;
+    }
+    return r;
+}
+
+// CTA b's range.  w0 == w1: nothing for this CTA.
+__device__ __forceinline__ TreeRange tree_range(const TreeParams &p, TreeShared *sh, uint32_t b, uint32_t grid) {
+    TreeRange r;
+    r.w0 = r.w1 = 0;
+    const TreePlace at = tree_find(p, sh, false, [&](uint32_t total) {
+        const TreeCuts cuts(total, grid);
+        if (b < cuts.active) {
+            r.w0 = cuts.at(b);
+            r.w1 = cuts.at(b + 1);
+        }
+        return r.w0;
+    });
+    r.total = at.total;
+    r.base = at.base;
+    r.seq = at.seq;
     return r;
 }
 
@@ -212,66 +278,20 @@ struct TreeUnit {
     bool found;
 };
 
-// The unit with index u in line order.  As tree_range: every thread calls it.
+// The unit with index u in line order.
 __device__ __forceinline__ TreeUnit tree_unit(const TreeParams &p, TreeShared *sh, uint32_t u) {
-    const uint32_t nt = blockDim.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t per = (p.n_seqs + nt - 1) / nt;
-    const uint32_t i0 = min(threadIdx.x * per, p.n_seqs), i1 = min(i0 + per, p.n_seqs);
-    uint32_t tiles = 0, units = 0;
-    for (uint32_t i = i0; i < i1; ++i) {
-        const TreeSeq s = tree_seq(p, i);
-        const uint32_t n = s.groups * (p.n_kv / p.hpu);
-        units += n;
-        tiles += n * s.tiles;
-    }
-    uint32_t inc_t = tiles, inc_u = units;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t a = __shfl_up_sync(0xffffffffu, inc_t, o), b = __shfl_up_sync(0xffffffffu, inc_u, o);
-        if (lane >= (uint32_t)o) {
-            inc_t += a;
-            inc_u += b;
-        }
-    }
-    if (lane == 31) {
-        sh->warp_sums[warp] = inc_t;
-        sh->warp_units[warp] = inc_u;
-    }
-    __syncthreads();
-    uint32_t ft = inc_t - tiles, fu = inc_u - units, all_t = 0, all_u = 0;
-    for (uint32_t w = 0; w < nt / 32; ++w) {
-        if (w < warp) {
-            ft += sh->warp_sums[w];
-            fu += sh->warp_units[w];
-        }
-        all_t += sh->warp_sums[w];
-        all_u += sh->warp_units[w];
-    }
-    if (u >= fu && u < fu + units) {
-        uint32_t i = i0;
-        while (true) {
-            const TreeSeq s = tree_seq(p, i);
-            const uint32_t n = s.groups * (p.n_kv / p.hpu);
-            if (u < fu + n) break;
-            fu += n;
-            ft += n * s.tiles;
-            ++i;
-        }
-        sh->seq = i;
-        sh->base = ft;
-        sh->unit = u - fu;
-    }
-    __syncthreads();
-    TreeUnit r;
-    r.found = u < all_u;
-    r.total = all_t;
+    const TreePlace at = tree_find(p, sh, true, [&](uint32_t) { return u; });
+    TreeUnit r = {};
+    r.found = u < at.units;
+    r.total = at.total;
     if (r.found) {
-        r.seq = sh->seq;
+        r.seq = at.seq;
         r.s = tree_seq(p, r.seq);
-        r.head = sh->unit / r.s.groups;
-        r.rg = sh->unit - r.head * r.s.groups;
+        const uint32_t in = u - at.unit0;
+        r.head = in / r.s.groups;
+        r.rg = in - r.head * r.s.groups;
         r.head *= p.hpu;
-        r.u0 = sh->base + sh->unit * r.s.tiles;
+        r.u0 = at.base + in * r.s.tiles;
     }
     return r;
 }

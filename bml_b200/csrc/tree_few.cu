@@ -121,7 +121,8 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
         prefetch_tmap(&fp.tv);
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const TreeRange range = tree_range(p, &sh, blockIdx.x, gridDim.x);  // has the barriers for the set-up above
+    const TreeRange range = tree_range(p, &sh, blockIdx.x, gridDim.x);
+    __syncthreads();  // the set-up above
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     // ------------------------------------------------------------ copies, ahead
@@ -159,13 +160,11 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
         if (--f_left) f_page = page_at(f_pos);  // there when the next step needs it
         f_stage = f_stage + 1 == (uint32_t)C::NST ? 0 : f_stage + 1;
     };
-#pragma unroll 1
-    for (int i = 0; i < C::NST - 1; ++i) fetch();
-
     auto weight = [](float x) { return kQ32 ? exp2f(x) : fast_exp2(x); };
     TreeWalk walk(p, range);
-    TreeSeg sg;
+    TreeSeg sg = {};
     uint32_t stage = 0, phase = 0;
+    bool first = true;
     // ldmatrix addresses inside a box: row and swizzled 16-byte column
     // K as the A operand (positions x d), V^T as the A operand (d x positions)
     const uint32_t k_row = (lane & 7) + ((lane >> 3) & 1) * 8, k_col = lane >> 4;
@@ -210,6 +209,11 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
 #pragma unroll
                     for (int h = 0; h < 2; ++h) q[s][h][0] = v ? *reinterpret_cast<const uint32_t *>(qp + s * 16 + h * 8) : 0u;
             }
+        }
+        if (first) {  // the queries' loads are on their way with the table's
+            first = false;
+#pragma unroll 1
+            for (int i = 0; i < C::NST - 1; ++i) fetch();
         }
         float o[NJ][4];  // O^T: d = 16 j + g (+ 8), rows 2c and 2c + 1
 #pragma unroll
@@ -370,8 +374,11 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
             ml[warp * kRows + 2 * c] = make_float2(m0, l0);
             ml[warp * kRows + 2 * c + 1] = make_float2(m1, l1);
         }
-        const uint32_t R = kRows * p.hpu;
+        const uint32_t R = kRows * p.hpu;  // a power of two that divides the thread count
         float *part = sg.slot < 2 ? tree_part(p, D, blockIdx.x, sg.slot) : nullptr;
+        const uint32_t row = threadIdx.x & (R - 1), h = row / kRows, r = row % kRows;  // this thread's in what follows
+        float m = -INFINITY, mu = 0.f, l = 0.f, inv = 0.f;
+        size_t at = 0;
 #pragma unroll
         for (int ch = 0; ch < 2; ++ch) {
             float *mine = meet + warp * kRows * C::CS;
@@ -384,41 +391,41 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
                 mine[(2 * c + 1) * C::CS + j * 16 + g + 8] = oj[3];
             }
             __syncthreads();
-            for (uint32_t i = threadIdx.x; i < R * (C::CH / 4); i += THREADS) {
-                const uint32_t x4 = i / R, row = i - x4 * R, h = row / kRows, r = row % kRows;
-                if (r >= sg.rows) continue;
-                float m = -INFINITY;
-                for (uint32_t s = 0; s < fp.splits; ++s) m = fmaxf(m, ml[(s * p.hpu + h) * kRows + r].x);
-                const float mu = m == -INFINITY ? 0.f : m;
-                float l = 0.f;
-                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (uint32_t s = 0; s < fp.splits; ++s) {
-                    const uint32_t w = (s * p.hpu + h) * kRows + r;
-                    const float2 a = ml[w];
-                    const float f = weight(a.x - mu);
-                    const float4 y = *reinterpret_cast<const float4 *>(meet + w * C::CS + x4 * 4);
-                    l += f * a.y;
-                    acc.x += f * y.x;
-                    acc.y += f * y.y;
-                    acc.z += f * y.z;
-                    acc.w += f * y.w;
-                }
-                if (*abort_flag) l = __int_as_float(0x7fffffff);  // a copy did not arrive: NaN
-                const uint32_t col4 = ch * (C::CH / 4) + x4;
-                if (part) {
-                    reinterpret_cast<float4 *>(part)[col4 * R + row] = acc;
-                    if (col4 == 0) {
+            if (r < sg.rows) {
+                if (ch == 0) {
+                    for (uint32_t s = 0; s < fp.splits; ++s) m = fmaxf(m, ml[(s * p.hpu + h) * kRows + r].x);
+                    mu = m == -INFINITY ? 0.f : m;
+                    for (uint32_t s = 0; s < fp.splits; ++s) {
+                        const float2 a = ml[(s * p.hpu + h) * kRows + r];
+                        l += weight(a.x - mu) * a.y;
+                    }
+                    if (*abort_flag) l = __int_as_float(0x7fffffff);  // a copy did not arrive: NaN
+                    inv = l == 0.f ? 0.f : 1.f / l;
+                    at = tree_row(p, sg, sg.row0 + r, D, h);
+                    if (part && threadIdx.x < R) {
                         part[(size_t)R * D + row] = m;
                         part[(size_t)R * (D + 1) + row] = l;
                     }
-                } else {
-                    const float inv = l == 0.f ? 0.f : 1.f / l;
-                    const size_t at = tree_row(p, sg, sg.row0 + r, D, h) + col4 * 4;
-                    if (kQ32)
-                        *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at) =
+                }
+                for (uint32_t x4 = threadIdx.x / R; x4 < C::CH / 4; x4 += THREADS / R) {
+                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (uint32_t s = 0; s < fp.splits; ++s) {
+                        const uint32_t w = (s * p.hpu + h) * kRows + r;
+                        const float f = weight(ml[w].x - mu);
+                        const float4 y = *reinterpret_cast<const float4 *>(meet + w * C::CS + x4 * 4);
+                        acc.x += f * y.x;
+                        acc.y += f * y.y;
+                        acc.z += f * y.z;
+                        acc.w += f * y.w;
+                    }
+                    const uint32_t col4 = ch * (C::CH / 4) + x4;
+                    if (part)
+                        reinterpret_cast<float4 *>(part)[col4 * R + row] = acc;
+                    else if (kQ32)
+                        *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at + col4 * 4) =
                             make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
                     else
-                        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at) =
+                        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at + col4 * 4) =
                             make_uint2(pack2<kF16>(acc.x * inv, acc.y * inv), pack2<kF16>(acc.z * inv, acc.w * inv));
                 }
             }

@@ -123,8 +123,9 @@ __device__ __forceinline__ uint32_t v_index(bool pair, uint32_t j, uint32_t n) {
 // the tile's first position (negative: committed positions, seen by all).
 // bad: 16-position blocks on pages outside the pool.  Out of line: few tiles
 // need it, and the softmax's registers are dear.
-__device__ __noinline__ void see_tile(const TreeParams &p, const volatile Board *b, uint32_t row, int32_t node0, bool edge,
-                                      uint32_t bad, uint32_t *see) {
+__device__ __noinline__ uint4 see_tile(const TreeParams &p, const volatile Board *b, uint32_t row, int32_t node0, bool edge,
+                                       uint32_t bad) {
+    uint32_t see[4];
     const uint32_t T = b->T, L = b->L, t = min((b->row0 + row) / p.group, T - 1);
     const uint64_t *m = p.mask ? p.mask + (size_t)(b->first + t) * p.n_words : nullptr;
 #pragma unroll
@@ -151,6 +152,36 @@ __device__ __noinline__ void see_tile(const TreeParams &p, const volatile Board 
         if (bad >> (2 * q + 1) & 1) s &= 0x0000ffffu;
         see[q] = s;
     }
+    return make_uint4(see[0], see[1], see[2], see[3]);
+}
+
+// One V row of a tile before its first P.V: zeros past the length, and where a
+// drafted node's row has a value that is not finite (noted in odd).  row: its
+// first 128 bytes; the lanes start at different 16-byte pieces, against bank
+// conflicts.
+template <int KB, bool kF16>
+__device__ __noinline__ void fix_v(uint8_t *row, bool node_row, bool past, uint32_t node, uint32_t *odd) {
+    const uint32_t lane = threadIdx.x & 31;
+    bool zero = past;
+    if (node_row && !past) {
+        constexpr uint32_t em = kF16 ? 0x7c00u : 0x7f80u;
+        bool bad = false;
+#pragma unroll 4
+        for (int u = 0; u < KB * 8; ++u) {
+            const uint4 w = lds128(row + (u >> 3) * BN * 128 + ((u + lane) & 7) * 16);
+            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bad |= (ws[e] & em) == em || ((ws[e] >> 16) & em) == em;
+        }
+        if (bad) {
+            atomicOr(&odd[node >> 5], 1u << (node & 31));
+            zero = true;
+        }
+    }
+    if (zero)
+#pragma unroll 4
+        for (int u = 0; u < KB * 8; ++u)
+            *reinterpret_cast<uint4 *>(row + (u >> 3) * BN * 128 + ((u + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
 }
 
 template <bool kF16>
@@ -225,7 +256,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
     }
     tc_fence_before();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const TreeRange range = tree_range(p, &sh.sched, blockIdx.x, gridDim.x);  // has the barriers for the set-up above
+    const TreeRange range = tree_range(p, &sh.sched, blockIdx.x, gridDim.x);
+    __syncthreads();  // the set-up above
     tc_fence_after();
     const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may take its place; it waits for this grid
@@ -553,30 +585,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
                     const uint32_t pos = kv0 + r, cv = cnt + v_index(pair, j, n), slot = cv % C::SLOTS;
                     if (__any_sync(0xffffffffu, pos >= P)) {
                         wait_bar(&sh.full[slot], (cv / C::SLOTS) & 1u, abort_flag);
-                        uint8_t *vrow = ring + slot * C::TILE + r * 128;
-                        bool zero = pos >= b->L;
-                        if (pos >= P && !zero) {
-                            constexpr uint32_t em = kF16 ? 0x7c00u : 0x7f80u;
-                            bool odd = false;
-#pragma unroll 4
-                            for (int u = 0; u < C::KB * 8; ++u) {
-                                const uint4 w = lds128(vrow + (u >> 3) * BN * 128 + ((u + lane) & 7) * 16);
-                                const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    odd |= (ws[e] & em) == em || ((ws[e] >> 16) & em) == em;
-                            }
-                            if (odd) {
-                                atomicOr(&sh.odd[(pos - P) >> 5], 1u << ((pos - P) & 31));
-                                zero = true;
-                            }
-                        }
-                        if (zero) {
-#pragma unroll 4
-                            for (int u = 0; u < C::KB * 8; ++u)
-                                *reinterpret_cast<uint4 *>(vrow + (u >> 3) * BN * 128 + ((u + lane) & 7) * 16) =
-                                    make_uint4(0, 0, 0, 0);
-                        }
+                        fix_v<C::KB, kF16>(ring + slot * C::TILE + r * 128, pos >= P, pos >= b->L, pos - P, sh.odd);
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     }
                 }
@@ -590,18 +599,19 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
                     }
                     continue;
                 }
+                uint4 see;  // before the scores are loaded: the call would spill them
+                if (edge || bad) see = see_tile(p, b, row, (int32_t)(kv0 - P), edge, bad);
                 float sv[BN];
 #pragma unroll
                 for (int cc = 0; cc < BN / 32; ++cc) tmem_ld32(s_col + cc * 32, sv + cc * 32);
                 tmem_wait_ld();
                 if (edge || bad) {
-                    uint32_t see[4];
-                    see_tile(p, b, row, (int32_t)(kv0 - P), edge, bad, see);
+                    const uint32_t sees[4] = {see.x, see.y, see.z, see.w};
 #pragma unroll
                     for (int w = 0; w < 4; ++w)
 #pragma unroll
                         for (int k = 0; k < 32; ++k)
-                            if (!(see[w] >> k & 1)) sv[w * 32 + k] = -INFINITY;
+                            if (!(sees[w] >> k & 1)) sv[w * 32 + k] = -INFINITY;
                 }
                 float mx8[8];
 #pragma unroll
@@ -719,7 +729,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
                             for (int u = 0; u < 32; ++u) o[u] = fmaf(o2[u], wb, o[u]);
                     }
                     if (valid) {
-                        if (any_odd) add_odd<D, kF16>(p, b, sh.odd, P, t, at, col, m, o);
+                        if (any_odd) {
+                            float tmp[32];  // its address is taken, o's is not
+#pragma unroll
+                            for (int u = 0; u < 32; ++u) tmp[u] = o[u];
+                            add_odd<D, kF16>(p, b, sh.odd, P, t, at, col, m, tmp);
+#pragma unroll
+                            for (int u = 0; u < 32; ++u) o[u] = tmp[u];
+                        }
                         if (part) {
                             float4 *dst = reinterpret_cast<float4 *>(part) + (size_t)(col / 4) * p.rpg + row;
 #pragma unroll
