@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_merge_kernel(const __grid_co
     __shared__ float2 s_ml[kWarps][32];
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     TreeSeg sg = {};
-    uint32_t u0 = 0, total = 0, b = 0;
+    uint32_t u0 = 0, w = 1, total = 0, b = 0;
     // (the lengths are inputs of the call, not results of the kernel before,
     // and that kernel has waited for their writer)
     bool mine;
@@ -404,11 +404,12 @@ __global__ void __launch_bounds__(kThreads, 2) tree_merge_kernel(const __grid_co
         if (mine) {
             total = u.total;
             u0 = u.u0;
+            w = u.w;
             sg.seq = u.seq;
             sg.head = u.head;
             sg.s = u.s;
             sg.row0 = u.rg * p.rpg;
-            b = TreeCuts(total, grid).owner(u0) + 1;  // the first cut behind u0
+            b = TreeCuts(p, total, grid).owner(u0) + 1;  // the first cut behind u0
         }
     } else {
         b = blockIdx.x + 1;
@@ -416,16 +417,16 @@ __global__ void __launch_bounds__(kThreads, 2) tree_merge_kernel(const __grid_co
         mine = range.w0 < range.w1;
         if (mine) {
             TreeWalk walk(p, range);
-            walk.next(p, sg);
-            mine = sg.t0 > 0;  // else the cut lies between two units
+            mine = walk.next(p, sg) && sg.t0 > 0;  // else the cut lies between two units
             total = range.total;
-            u0 = range.w0 - sg.t0;
+            u0 = sg.u0;
+            w = sg.w;
         }
     }
     uint32_t last = 0;  // the CTAs with a segment of the unit: b - 1 to last
     if (mine) {
-        const TreeCuts cuts(total, grid);
-        last = cuts.owner(u0 + sg.s.tiles - 1);
+        const TreeCuts cuts(p, total, grid);
+        last = cuts.owner(u0 + (sg.s.tiles - 1) * w);
         mine = last >= b && cuts.at(b - 1) <= u0;  // divided, and no earlier cut inside the unit
         sg.rows = min(p.rpg, sg.s.rows - sg.row0);
     }
@@ -542,6 +543,8 @@ cudaError_t launch_f32(TreeParams p, int num_sms, cudaStream_t st) {
     p.rpg = RW * 16;
     p.hpu = 1;
     p.tile = kTreeTile;
+    p.heavy_rows = 0xffffffffu;
+    p.heavy = p.light = 1;
     if (!tree_line_fits(p)) return cudaErrorNotSupported;
     e = launch_after(kern, dim3(num_sms), kThreads, C::SMEM, st, p);
     if (e != cudaSuccess) return e;
@@ -571,10 +574,11 @@ cudaError_t launch_tree_merge(const TreeParams &p, uint32_t D, int grid, cudaStr
     const uint64_t units = tree_most_units(p);
     const bool by_unit = units < (uint64_t)(grid - 1);
     const uint32_t x = by_unit ? (uint32_t)units : (uint32_t)(grid - 1);
-    // about 8 CTAs an SM, no more than the tasks
+    // One wave of two CTAs an SM; few units (long requests) take a CTA a task.
     const uint32_t tasks = (p.rpg * p.hpu + 7) / 8 * (D / 32);
-    uint32_t y = (uint32_t)grid * 8 / x;
-    y = y < 1 ? 1 : y > tasks ? tasks : y;
+    const uint32_t most = x < 32 ? tasks : (tasks + kWarps - 1) / kWarps;
+    uint32_t y = (uint32_t)grid * 2 / x;
+    y = y < 1 ? 1 : y > most ? most : y;
     return D == 128 ? launch_after(tree_merge_kernel<128>, dim3(x, y), kThreads, 0, st, p, (uint32_t)grid, (uint32_t)by_unit)
                     : launch_after(tree_merge_kernel<64>, dim3(x, y), kThreads, 0, st, p, (uint32_t)grid, (uint32_t)by_unit);
 }

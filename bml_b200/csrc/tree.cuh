@@ -27,6 +27,8 @@ struct TreeParams {
     uint32_t rpg;        // rows of a row group
     uint32_t hpu;        // kv heads of a unit
     uint32_t tile;       // positions of a schedule tile
+    // a tile's weight: heavy with more rows than heavy_rows, else light
+    uint32_t heavy_rows, heavy, light;
 };
 
 struct TreeArgs {
@@ -69,7 +71,7 @@ inline uint64_t tree_most_units(const TreeParams &p) {
 }
 inline bool tree_line_fits(const TreeParams &p) {
     const uint64_t tiles = (((uint64_t)p.max_pages << p.page_shift) + p.tile - 1) / p.tile;
-    return tree_most_units(p) <= 0xffffffffull / tiles;
+    return tree_most_units(p) * p.heavy <= 0xffffffffull / tiles;
 }
 
 // A launch that may begin while the kernel before it on the stream ends; the
@@ -96,7 +98,7 @@ cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, int threads, int s
 // heads the query rows (node t, q head g of the kv head) of up to rpg
 // consecutive t * group + g, over all positions of the request.  Units are laid
 // out request by request, heads by heads, row group by row group, each as its
-// number of tiles of positions, and the line of all tiles is cut evenly over the CTAs,
+// number of tiles of positions times a tile's weight, and the line of all tiles is cut evenly over the CTAs,
 // so the lengths stay on the GPU and no CTA works longer than another by more
 // than a tile.  A unit that a cut divides leaves partial results (max, sum,
 // un-normalised output) which tree_merge_kernel joins in tile order.
@@ -105,7 +107,11 @@ struct TreeSeq {
     uint32_t first;  // first token row
     uint32_t T, L;   // drafted tokens; positions (0: refused, its rows are zero)
     uint32_t rows, groups, tiles;
+    uint32_t w_last, weight;  // a tile's weight in the last row group; in all groups of a head
 };
+
+// A tile's weight in a full row group.
+__device__ __forceinline__ uint32_t tree_full_weight(const TreeParams &p) { return p.rpg > p.heavy_rows ? p.heavy : p.light; }
 
 __device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, uint32_t i) {
     TreeSeq s;
@@ -119,6 +125,8 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, uint32_t i) {
     s.rows = s.T * p.group;
     s.groups = (s.rows + p.rpg - 1) / p.rpg;
     s.tiles = s.L ? (s.L + p.tile - 1) / p.tile : 1u;
+    s.w_last = s.rows - (s.groups - 1) * p.rpg > p.heavy_rows ? p.heavy : p.light;
+    s.weight = s.groups ? (s.groups - 1) * tree_full_weight(p) + s.w_last : 0u;
     return s;
 }
 
@@ -128,17 +136,20 @@ struct TreeShared {
     uint32_t seq, unit;
 };
 
-// How a line of `total` tiles is cut for `active` CTAs: the first `more` take
-// one tile more than the others.
+// How a line of weight `total` is cut for up to `grid` CTAs, at least a heavy
+// tile's weight each: the first `more` take one more than the others.  A tile
+// belongs to the CTA in whose part it begins; a part inside one unit holds at
+// least one beginning.
 struct TreeCuts {
     uint32_t each, more, active;
-    __device__ __forceinline__ TreeCuts(uint32_t total, uint32_t grid) {
-        active = total < grid ? total : grid;
+    __device__ __forceinline__ TreeCuts(const TreeParams &p, uint32_t total, uint32_t grid) {
+        const uint32_t most = total / p.heavy;
+        active = most < 1 ? (total ? 1u : 0u) : most < grid ? most : grid;
         each = active ? total / active : 0u;
         more = total - each * active;
     }
     __device__ __forceinline__ uint32_t at(uint32_t b) const { return each * b + min(b, more); }
-    // the CTA that takes tile w
+    // the CTA that holds place w
     __device__ __forceinline__ uint32_t owner(uint32_t w) const {
         const uint32_t wide = more * (each + 1);
         return w < wide ? w / (each + 1) : more + (w - wide) / each;
@@ -174,7 +185,7 @@ __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *
             if (i0 + k < i1) {
                 const TreeSeq s = tree_seq(p, i0 + k);
                 n4[k] = s.groups * upr;
-                t4[k] = n4[k] * s.tiles;
+                t4[k] = s.weight * upr * s.tiles;
                 units += n4[k];
                 tiles += t4[k];
             }
@@ -182,7 +193,7 @@ __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *
         for (uint32_t i = i0; i < i1; ++i) {
             const TreeSeq s = tree_seq(p, i);
             units += s.groups * upr;
-            tiles += s.groups * upr * s.tiles;
+            tiles += s.weight * upr * s.tiles;
         }
     }
     uint32_t inc_t = tiles, inc_u = units;
@@ -234,10 +245,10 @@ __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *
         if (mine) {
             while (true) {
                 const TreeSeq s = tree_seq(p, seq);
-                const uint32_t n = s.groups * upr;
-                if (by_unit ? w < fu + n : w < ft + n * s.tiles) break;
+                const uint32_t n = s.groups * upr, t = s.weight * upr * s.tiles;
+                if (by_unit ? w < fu + n : w < ft + t) break;
                 fu += n;
-                ft += n * s.tiles;
+                ft += t;
                 ++seq;
             }
             sh->seq = seq;
@@ -257,7 +268,7 @@ __device__ __forceinline__ TreeRange tree_range(const TreeParams &p, TreeShared 
     TreeRange r;
     r.w0 = r.w1 = 0;
     const TreePlace at = tree_find(p, sh, false, [&](uint32_t total) {
-        const TreeCuts cuts(total, grid);
+        const TreeCuts cuts(p, total, grid);
         if (b < cuts.active) {
             r.w0 = cuts.at(b);
             r.w1 = cuts.at(b + 1);
@@ -270,9 +281,9 @@ __device__ __forceinline__ TreeRange tree_range(const TreeParams &p, TreeShared 
     return r;
 }
 
-// A unit's place on the line: tiles [u0, u0 + s.tiles).
+// A unit's place on the line: [u0, u0 + w * s.tiles).
 struct TreeUnit {
-    uint32_t u0, total;
+    uint32_t u0, w, total;
     uint32_t seq, head, rg;
     TreeSeq s;
     bool found;
@@ -290,8 +301,9 @@ __device__ __forceinline__ TreeUnit tree_unit(const TreeParams &p, TreeShared *s
         const uint32_t in = u - at.unit0;
         r.head = in / r.s.groups;
         r.rg = in - r.head * r.s.groups;
+        r.u0 = at.base + (r.head * r.s.weight + r.rg * tree_full_weight(p)) * r.s.tiles;
+        r.w = r.rg + 1 == r.s.groups ? r.s.w_last : tree_full_weight(p);
         r.head *= p.hpu;
-        r.u0 = at.base + in * r.s.tiles;
     }
     return r;
 }
@@ -300,6 +312,7 @@ __device__ __forceinline__ TreeUnit tree_unit(const TreeParams &p, TreeShared *s
 struct TreeSeg {
     uint32_t seq, head, rg;  // head: the first of the unit's
     uint32_t t0, t1;     // tiles of the unit, [t0, t1)
+    uint32_t u0, w;      // the unit's place on the line, a tile's weight
     uint32_t row0, rows; // first row (t * group + g) and row count of the group
     uint32_t slot;       // partial slot of the CTA: 0 the unit began before this range, 1 it ends after it, 2 whole
     TreeSeq s;
@@ -313,27 +326,32 @@ struct TreeWalk {
         if (pos < end) s = tree_seq(p, seq);
     }
     __device__ __forceinline__ bool next(const TreeParams &p, TreeSeg &g) {
-        if (pos >= end) return false;
-        uint32_t units;
-        while (pos - base >= (units = s.groups * (p.n_kv / p.hpu)) * s.tiles) {
-            base += units * s.tiles;
-            s = tree_seq(p, ++seq);
+        while (pos < end) {
+            uint32_t per_head;
+            while (pos - base >= (per_head = s.weight * s.tiles) * (p.n_kv / p.hpu)) {
+                base += per_head * (p.n_kv / p.hpu);
+                s = tree_seq(p, ++seq);
+            }
+            const uint32_t off = pos - base, wf = tree_full_weight(p);
+            const uint32_t head = off / per_head, in_head = off - head * per_head;
+            g.rg = s.groups > 1 ? min(in_head / (wf * s.tiles), s.groups - 1) : 0u;
+            g.w = g.rg + 1 == s.groups ? s.w_last : wf;
+            const uint32_t in = in_head - g.rg * wf * s.tiles, left = end - pos;
+            const uint32_t out = min(in + left, g.w * s.tiles);  // where the range ends in the unit
+            g.t0 = g.w == 1 ? in : (in + g.w - 1) / g.w;
+            g.t1 = g.w == 1 ? out : (out + g.w - 1) / g.w;
+            g.u0 = pos - in;
+            pos += out - in;
+            if (g.t0 == g.t1) continue;  // no tile begins here
+            g.seq = seq;
+            g.s = s;
+            g.head = head * p.hpu;
+            g.row0 = g.rg * p.rpg;
+            g.rows = min(p.rpg, s.rows - g.row0);
+            g.slot = g.t0 > 0 ? 0u : (g.t1 < s.tiles ? 1u : 2u);
+            return true;
         }
-        const uint32_t off = pos - base;
-        const uint32_t u = off / s.tiles;
-        const uint32_t left = end - pos;
-        g.seq = seq;
-        g.s = s;
-        g.head = u / s.groups;
-        g.rg = u - g.head * s.groups;
-        g.head *= p.hpu;
-        g.t0 = off - u * s.tiles;
-        g.t1 = left < s.tiles - g.t0 ? g.t0 + left : s.tiles;
-        g.row0 = g.rg * p.rpg;
-        g.rows = min(p.rpg, s.rows - g.row0);
-        g.slot = g.t0 > 0 ? 0u : (g.t1 < s.tiles ? 1u : 2u);
-        pos += g.t1 - g.t0;
-        return true;
+        return false;
     }
 };
 

@@ -464,6 +464,8 @@ cudaError_t launch_n(const TreeArgs &a, cudaStream_t st) {
     fp.t.hpu = hpu;
     fp.t.rpg = kRows;
     fp.t.tile = 16 * fp.splits;
+    fp.t.heavy_rows = 0xffffffffu;
+    fp.t.heavy = fp.t.light = 1;
     if (!tree_line_fits(fp.t)) return cudaErrorNotSupported;
     const uint64_t rows = (uint64_t)a.p.n_pages << a.p.page_shift;
     if (!few_map(&fp.tk, a.p.k, kF16, D, a.p.n_kv, rows) || !few_map(&fp.tv, a.p.v, kF16, D, a.p.n_kv, rows))

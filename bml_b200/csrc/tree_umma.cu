@@ -825,6 +825,11 @@ cudaError_t launch_tree_umma(const TreeArgs &a, cudaStream_t st) {
     up.t.rpg = 2 * up.rt;
     up.t.hpu = 1;
     up.t.tile = kTreeTile;
+    // A tile of two row tiles against one of one: measured on B200, d = 128, 32
+    // requests of 8000 positions in L2: 2.4 us with 256 rows, 1.4 with 128.
+    up.t.heavy_rows = up.rt;
+    up.t.heavy = 5;
+    up.t.light = 3;
     if (!tree_line_fits(up.t)) return cudaErrorNotSupported;
     const uint64_t rows = (uint64_t)a.p.n_pages << a.p.page_shift;
     if (!tree_map(&up.tq, a.p.q, f16, a.D, a.p.n_heads, a.p.n_tokens, group, BM / group) ||

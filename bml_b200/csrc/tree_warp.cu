@@ -463,6 +463,8 @@ cudaError_t launch_w(TreeParams p, int num_sms, cudaStream_t st) {
     p.rpg = RW * 16;
     p.hpu = 1;
     p.tile = kTreeTile;
+    p.heavy_rows = 0xffffffffu;
+    p.heavy = p.light = 1;
     if (!tree_line_fits(p)) return cudaErrorNotSupported;
     e = launch_after(kern, dim3(num_sms), kThreads, C::SMEM, st, p);
     if (e != cudaSuccess) return e;
