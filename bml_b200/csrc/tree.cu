@@ -24,6 +24,7 @@ namespace bml {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr float kGrow = 8.0f;  // log2 units a row's maximum may grow before O is rescaled
 constexpr int kWarps = kThreads / 32;
 
 __device__ __forceinline__ uint32_t tf32_hi(float x) {
@@ -94,6 +95,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
     using C = FCfg<D, KT, RW>;
     constexpr bool kF32 = C::ES == 4;
     constexpr int NT = D / 8;          // output column tiles of a warp
+    constexpr int NB = RW;             // blocks of 8 positions at a time
     constexpr int VE = 16 / C::ES;     // V elements of one 16-byte piece
     extern __shared__ __align__(16) uint8_t smem[];
     uint32_t *sQ = reinterpret_cast<uint32_t *>(smem);
@@ -186,61 +188,84 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
             const bool row_live = sg.rows > (uint32_t)rw * 16;
             if (!row_live) continue;
 #pragma unroll 1
-            for (int nt = 0; nt < RW; ++nt) {
-                const uint32_t base = step_pos(k) + nt * 8;
-                if (base >= sg.s.L || !my_flags[st * RW + nt]) continue;  // nothing to see here
-                // S = Q K^T for 8 positions, in three sums of their own
-                float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
-                const uint8_t *krow = sk + (nt * 8 + g) * C::KS;
+            for (int n0 = 0; n0 < RW; n0 += NB) {  // NB blocks of 8 positions share the Q fragments
+                const uint32_t base = step_pos(k) + n0 * 8;
+                uint32_t live = 0;  // bit per block: inside the length, on a page of the pool
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+                    if (base + n * 8 < sg.s.L && my_flags[st * RW + n0 + n]) live |= 1u << n;
+                if (live == 0) continue;
+                // S = Q K^T: hi * hi apart from the cross terms
+                float s0[NB][4], s1[NB][4];
+#pragma unroll
+                for (int n = 0; n < NB; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s0[n][e] = s1[n][e] = 0.f;
+                const uint8_t *krow = sk + (n0 * 8 + g) * C::KS;
 #pragma unroll
                 for (int s = 0; s < D / 32; ++s) {
-                    float x[8];
-                    if (kF32) {
-                        Elem<float>::widen(lds128(krow + s * 128 + c * 32), x);
-                        Elem<float>::widen(lds128(krow + s * 128 + c * 32 + 16), x + 4);
-                    } else {
-                        Elem<KT>::widen(lds128(krow + s * 64 + c * 16), x);
-                    }
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk) {
-                        const uint4 qh = qf[((s * 4 + kk) * 2) * 32], ql = qf[((s * 4 + kk) * 2 + 1) * 32];
-                        uint32_t b0, b1, e0 = 0, e1 = 0;
-                        if (kF32) {
-                            tf32_split(x[2 * kk], b0, e0);
-                            tf32_split(x[2 * kk + 1], b1, e1);
-                        } else {
-                            b0 = __float_as_uint(x[2 * kk]);
-                            b1 = __float_as_uint(x[2 * kk + 1]);
+                    for (int h = 0; h < 2; ++h) {  // two k-steps: 16 bytes of f32, half of 16 bytes of 16-bit values
+                        uint4 qh[2], ql[2];
+#pragma unroll
+                        for (int kk = 0; kk < 2; ++kk) {
+                            qh[kk] = qf[((s * 4 + 2 * h + kk) * 2) * 32];
+                            ql[kk] = qf[((s * 4 + 2 * h + kk) * 2 + 1) * 32];
                         }
-                        mma_tf32(s0, &qh.x, b0, b1);
-                        mma_tf32(s1, &ql.x, b0, b1);
-                        if (kF32) mma_tf32(s2, &qh.x, e0, e1);
-                    }
-                }
-                float x[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] = (s0[e] + (s1[e] + s2[e])) * p.scale_log2;
-                const bool edge = base + 8 > P;
-                if (edge) {
+                        for (int n = 0; n < NB; ++n) {
+                            const uint8_t *kr = krow + n * 8 * C::KS;
+                            float x[8];
+                            if (kF32) Elem<float>::widen(lds128(kr + s * 128 + c * 32 + h * 16), x);
+                            else Elem<KT>::widen(lds128(kr + s * 64 + c * 16), x);
+                            const float *y = kF32 ? x : x + 4 * h;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint32_t pos = base + 2 * c + e;
-                        if (pos >= P) {
-                            if (!(v0 && tree_sees(p, sg.s, t0, pos - P))) x[e] = -INFINITY;
-                            if (!(v1 && tree_sees(p, sg.s, t1, pos - P))) x[2 + e] = -INFINITY;
+                            for (int kk = 0; kk < 2; ++kk) {
+                                uint32_t b0, b1, e0 = 0, e1 = 0;
+                                if (kF32) {
+                                    tf32_split(y[2 * kk], b0, e0);
+                                    tf32_split(y[2 * kk + 1], b1, e1);
+                                } else {
+                                    b0 = __float_as_uint(y[2 * kk]);
+                                    b1 = __float_as_uint(y[2 * kk + 1]);
+                                }
+                                mma_tf32(s0[n], &qh[kk].x, b0, b1);
+                                mma_tf32(s1[n], &ql[kk].x, b0, b1);
+                                if (kF32) mma_tf32(s1[n], &qh[kk].x, e0, e1);
+                            }
                         }
                     }
                 }
-                float a = fmaxf(x[0], x[1]), b = fmaxf(x[2], x[3]);
-                a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
-                b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, 1));
-                a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
-                b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, 2));
-                if (__any_sync(0xffffffffu, a > m0 || b > m1)) {
-                    const float n0 = fmaxf(m0, a), n1 = fmaxf(m1, b);
-                    const float f0 = n0 == -INFINITY ? 1.f : exp2f(m0 - n0), f1 = n1 == -INFINITY ? 1.f : exp2f(m1 - n1);
-                    m0 = n0;
-                    m1 = n1;
+                const bool edge = base + NB * 8 > P;
+                float a = -INFINITY, b = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    float *x = s0[n];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = (x[e] + s1[n][e]) * p.scale_log2;
+                    if (!(live >> n & 1)) x[0] = x[1] = x[2] = x[3] = -INFINITY;
+                    else if (edge) {
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t pos = base + n * 8 + 2 * c + e;
+                            if (pos >= P) {
+                                if (!(v0 && tree_sees(p, sg.s, t0, pos - P))) x[e] = -INFINITY;
+                                if (!(v1 && tree_sees(p, sg.s, t1, pos - P))) x[2 + e] = -INFINITY;
+                            }
+                        }
+                    }
+                    a = fmaxf(a, fmaxf(x[0], x[1]));
+                    b = fmaxf(b, fmaxf(x[2], x[3]));
+                }
+                if (__any_sync(0xffffffffu, a > m0 + kGrow || b > m1 + kGrow)) {
+                    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
+                    b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, 1));
+                    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
+                    b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, 2));
+                    const float n0m = a > m0 + kGrow ? a : m0, n1m = b > m1 + kGrow ? b : m1;
+                    const float f0 = n0m == -INFINITY ? 1.f : exp2f(m0 - n0m), f1 = n1m == -INFINITY ? 1.f : exp2f(m1 - n1m);
+                    m0 = n0m;
+                    m1 = n1m;
                     l0 *= f0;
                     l1 *= f1;
 #pragma unroll
@@ -252,56 +277,77 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
                     }
                 }
                 const float u0 = m0 == -INFINITY ? 0.f : m0, u1 = m1 == -INFINITY ? 0.f : m1;
-                x[0] = exp2f(x[0] - u0);
-                x[1] = exp2f(x[1] - u0);
-                x[2] = exp2f(x[2] - u1);
-                x[3] = exp2f(x[3] - u1);
-                l0 += x[0] + x[1];
-                l1 += x[2] + x[3];
-                // P as the A operand: k index c is position 2c, c + 4 is 2c + 1
-                uint32_t ph[4], pl[4];
-                tf32_split(x[0], ph[0], pl[0]);
-                tf32_split(x[2], ph[1], pl[1]);
-                tf32_split(x[1], ph[2], pl[2]);
-                tf32_split(x[3], ph[3], pl[3]);
-                const uint8_t *va = sv + (nt * 8 + 2 * c) * C::VS + g * 16, *vb = va + C::VS;
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    float *x = s0[n];
+                    x[0] = exp2f(x[0] - u0);
+                    x[1] = exp2f(x[1] - u0);
+                    x[2] = exp2f(x[2] - u1);
+                    x[3] = exp2f(x[3] - u1);
+                    l0 += x[0] + x[1];
+                    l1 += x[2] + x[3];
+                }
+                // P as the A operand: k index c is position 2c, c + 4 is 2c + 1.  The
+                // matrix unit's accumulation truncates, so the NB blocks are summed
+                // apart and added to O with a rounding.
                 bool odd = false;  // a V value that is not finite: 0 * it must not reach rows that do not see it
 #pragma unroll
                 for (int s = 0; s < NT / VE; ++s) {
-                    float y0[VE], y1[VE];
-                    Elem<KT>::widen(lds128(va + s * 128), y0);
-                    Elem<KT>::widen(lds128(vb + s * 128), y1);
-                    if (edge) {
+                    float y[VE][4];
+#pragma unroll
+                    for (int e = 0; e < VE; ++e) y[e][0] = y[e][1] = y[e][2] = y[e][3] = 0.f;
+#pragma unroll
+                    for (int n = 0; n < NB; ++n) {
+                        uint32_t ph[4], pl[4];
+                        tf32_split(s0[n][0], ph[0], pl[0]);
+                        tf32_split(s0[n][2], ph[1], pl[1]);
+                        tf32_split(s0[n][1], ph[2], pl[2]);
+                        tf32_split(s0[n][3], ph[3], pl[3]);
+                        const uint8_t *va = sv + ((n0 + n) * 8 + 2 * c) * C::VS + g * 16, *vb = va + C::VS;
+                        float y0[VE], y1[VE];
+                        Elem<KT>::widen(lds128(va + s * 128), y0);
+                        Elem<KT>::widen(lds128(vb + s * 128), y1);
+                        if (edge) {
+#pragma unroll
+                            for (int e = 0; e < VE; ++e) {
+                                if (!(fabsf(y0[e]) < INFINITY)) { y0[e] = 0.f; odd = true; }
+                                if (!(fabsf(y1[e]) < INFINITY)) { y1[e] = 0.f; odd = true; }
+                            }
+                        }
 #pragma unroll
                         for (int e = 0; e < VE; ++e) {
-                            if (!(fabsf(y0[e]) < INFINITY)) { y0[e] = 0.f; odd = true; }
-                            if (!(fabsf(y1[e]) < INFINITY)) { y1[e] = 0.f; odd = true; }
+                            uint32_t b0, b1, e0 = 0, e1 = 0;
+                            if (kF32) {
+                                tf32_split(y0[e], b0, e0);
+                                tf32_split(y1[e], b1, e1);
+                            } else {
+                                b0 = __float_as_uint(y0[e]);
+                                b1 = __float_as_uint(y1[e]);
+                            }
+                            mma_tf32(y[e], pl, b0, b1);
+                            if (kF32) mma_tf32(y[e], ph, e0, e1);
+                            mma_tf32(y[e], ph, b0, b1);
                         }
                     }
 #pragma unroll
-                    for (int e = 0; e < VE; ++e) {
-                        uint32_t b0, b1, e0 = 0, e1 = 0;
-                        if (kF32) {
-                            tf32_split(y0[e], b0, e0);
-                            tf32_split(y1[e], b1, e1);
-                        } else {
-                            b0 = __float_as_uint(y0[e]);
-                            b1 = __float_as_uint(y1[e]);
-                        }
-                        float *oj = o[s * VE + e];
-                        mma_tf32(oj, pl, b0, b1);
-                        if (kF32) mma_tf32(oj, ph, e0, e1);
-                        mma_tf32(oj, ph, b0, b1);
-                    }
+                    for (int e = 0; e < VE; ++e)
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) o[s * VE + e][z] += y[e][z];
                 }
                 if (edge && __any_sync(0xffffffffu, odd)) {
                     // rare: the values that were taken as zero above, added for the rows that see them
 #pragma unroll 1
-                    for (int q8 = 0; q8 < 8; ++q8) {
-                        const int src = (lane & ~3) | (q8 >> 1);
-                        const float w0 = __shfl_sync(0xffffffffu, (q8 & 1) ? x[1] : x[0], src);
-                        const float w1 = __shfl_sync(0xffffffffu, (q8 & 1) ? x[3] : x[2], src);
-                        const uint8_t *vr = sv + (nt * 8 + q8) * C::VS;
+                    for (int q = 0; q < NB * 8; ++q) {
+                        const int src = (lane & ~3) | ((q & 7) >> 1);
+                        float y0 = 0.f, y1 = 0.f;
+#pragma unroll
+                        for (int n = 0; n < NB; ++n)
+                            if (n == q >> 3) {
+                                y0 = (q & 1) ? s0[n][1] : s0[n][0];
+                                y1 = (q & 1) ? s0[n][3] : s0[n][2];
+                            }
+                        const float w0 = __shfl_sync(0xffffffffu, y0, src), w1 = __shfl_sync(0xffffffffu, y1, src);
+                        const uint8_t *vr = sv + (n0 * 8 + q) * C::VS;
 #pragma unroll
                         for (int j = 0; j < NT; ++j)
 #pragma unroll

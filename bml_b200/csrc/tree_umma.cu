@@ -270,6 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
         // column block kb of part `part` of a tile.
         const bool is_k = warp == 0;
         const CUtensorMap *map = is_k ? &up.tk : &up.tv;
+        const uint64_t policy = l2_policy_evict_first();
         uint32_t tiles = 0, segs = 0;  // tiles, segments so far
         uint32_t slot = 0, use = 0;    // ring position of the segment's next tile of either kind, and its use of the slot
         const uint32_t per_tile = BN / up.box_rows, part = lane / C::KB, kb = lane % C::KB;
@@ -347,9 +348,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
                 if (lane == 0) mbar_arrive_expect_tx(&sh.full[slot], boxes * up.box_rows * 128);
                 __syncwarp();
                 // a page outside the pool is read past the map's end: zeros
-                if (row != -1)
-                    tma_load_3d(ring + slot * C::TILE + kb * BN * 128 + part * up.box_rows * 128, map, (int)kb * 64,
-                                (int)sg.head, row == -2 ? (int)(p.n_pages << p.page_shift) : row, &sh.full[slot]);
+                if (row != -1) {
+                    uint8_t *dst = ring + slot * C::TILE + kb * BN * 128 + part * up.box_rows * 128;
+                    const int at = row == -2 ? (int)(p.n_pages << p.page_shift) : row;
+                    // with one row group K and V are read once: 7% faster out of HBM with the hint (32 x 8000, 32 nodes)
+                    if (sg.s.groups == 1) tma_load_3d_hint(dst, map, (int)kb * 64, (int)sg.head, at, &sh.full[slot], policy);
+                    else tma_load_3d(dst, map, (int)kb * 64, (int)sg.head, at, &sh.full[slot]);
+                }
                 __syncwarp();
                 advance(j + 1 < n ? index(pair, j + 1, n) - index(pair, j, n) : 2 * n - index(pair, j, n));
             }
