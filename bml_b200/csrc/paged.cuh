@@ -6,6 +6,24 @@
 
 namespace bml {
 
+// A launch that may begin while the kernel before it on the stream ends; the
+// kernels wait for that kernel (griddepcontrol.wait) before they read or write
+// global memory.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, int threads, int smem, cudaStream_t st, const Args &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 constexpr uint32_t kPlanMaxSeqs = 4096;  // requests of one plan (their prefix sums live in shared memory)
 constexpr uint32_t kTreeMaxNodes = 256;  // drafted tokens of one request (4 mask words)
 
@@ -39,7 +57,7 @@ struct PagedAppendParams {
     const int64_t *slots;
     const int32_t *positions;  // null: no rotation
     uint32_t n_tokens, n_heads, n_kv, d;
-    double theta;
+    double log2_theta;
     void *k_pool, *v_pool;
     uint64_t n_rows;  // rows of a pool
     bml_dtype src, dst;

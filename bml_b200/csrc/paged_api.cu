@@ -153,7 +153,7 @@ BML_API bml_status bml_paged_append(const void *q_dev, const void *k_dev, const 
     p.n_heads = q_dev ? n_heads : 0;
     p.n_kv = n_kv_heads;
     p.d = head_dim;
-    p.theta = theta;
+    p.log2_theta = log2(theta);
     p.k_pool = k_pool;
     p.v_pool = v_pool;
     p.n_rows = n_rows;

@@ -68,7 +68,7 @@ struct FCfg {
     static constexpr int ES = sizeof(KT);
     static constexpr int GROUPS = kWarps / RW;
     static constexpr int SP = 8 * RW;
-    static constexpr int STEPS = kTreeTile / (GROUPS * SP);  // stages of a group per tile
+    static constexpr int TILE = GROUPS * SP;  // positions of a schedule tile: a stage of every group
     // Row strides in bytes.  K: lane (g, c) reads 16-byte pieces at row g,
     // 16-byte column 2c (f32) or c (16-bit); V: at rows 2c, 2c+1, column g.
     // With these paddings the 8 lanes of a quarter-warp meet 8 bank groups.
@@ -140,8 +140,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
         __syncthreads();
 
         const uint32_t P = sg.s.L - min(sg.s.T, sg.s.L);  // committed positions
-        const uint32_t pos0 = sg.t0 * kTreeTile;
-        const uint32_t n_steps = (sg.t1 - sg.t0) * C::STEPS;
+        const uint32_t pos0 = sg.t0 * C::TILE;
+        const uint32_t n_steps = sg.t1 - sg.t0;
         const int32_t *table = p.table + (size_t)sg.seq * p.max_pages;
         auto step_pos = [&](uint32_t k) { return pos0 + (k * C::GROUPS + grp) * C::SP; };
         // the group's copies of step k into stage k % NST
@@ -588,7 +588,7 @@ cudaError_t launch_f32(TreeParams p, int num_sms, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     p.rpg = RW * 16;
     p.hpu = 1;
-    p.tile = kTreeTile;
+    p.tile = C::TILE;
     p.heavy_rows = 0xffffffffu;
     p.heavy = p.light = 1;
     if (!tree_line_fits(p)) return cudaErrorNotSupported;

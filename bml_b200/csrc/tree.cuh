@@ -8,7 +8,7 @@
 
 namespace bml {
 
-constexpr int kTreeTile = 128;         // positions of one schedule tile, but for tree_few_kernel
+constexpr int kTreeTile = 128;         // positions of a schedule tile (tree_umma.cu, tree_warp.cu)
 constexpr uint32_t kTreeMaxSeqs = 1024;  // requests of one launch
 
 struct TreeParams {
@@ -72,24 +72,6 @@ inline uint64_t tree_most_units(const TreeParams &p) {
 inline bool tree_line_fits(const TreeParams &p) {
     const uint64_t tiles = (((uint64_t)p.max_pages << p.page_shift) + p.tile - 1) / p.tile;
     return tree_most_units(p) * p.heavy <= 0xffffffffull / tiles;
-}
-
-// A launch that may begin while the kernel before it on the stream ends; the
-// tree kernels wait for that kernel (griddepcontrol.wait) before they read or
-// write global memory.
-template <typename... KArgs, typename... Args>
-cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, int threads, int smem, cudaStream_t st, const Args &...args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 #ifdef __CUDACC__

@@ -40,6 +40,7 @@ class OutOfPages(RuntimeError):
 # what is wrong on the other), raw stream handles and addresses, few
 # allocations.
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
 def _bad(t, name: str, dtype=None, ndim=None, shape=None, device=None):
@@ -68,49 +69,32 @@ def _data(t, name: str, ndim: int, dtype=None, device=None) -> int:
     return t.data_ptr()
 
 
-class _On:
-    """Makes a call's device current, and its stream where one is given, so
-    that the buffers it allocates belong to the stream that uses them; the
-    stream's handle on entry."""
-
-    def __init__(self, device: torch.device, stream):
-        if stream is not None and stream.device != device:
+def _enter(device: torch.device, stream):
+    """Makes the device current, and the stream where one is given, so that
+    the buffers a call allocates belong to the stream that uses them.  None in
+    the usual case, where both are; else a context that has been entered."""
+    if stream is None:
+        if device.index == _current_device():
+            return None
+        ctx = torch.cuda.device(device)
+    else:
+        if stream.device != device:
             raise ValueError(f"the stream is on {stream.device}, the tensors on {device}")
-        self._index = device.index
-        self._ctx = torch.cuda.stream(stream) if stream is not None else torch.cuda.device(device)
-
-    def __enter__(self):
-        self._ctx.__enter__()
-        return _raw_stream(self._index)
-
-    def __exit__(self, *exc):
-        return self._ctx.__exit__(*exc)
+        ctx = torch.cuda.stream(stream)
+    ctx.__enter__()
+    return ctx
 
 
-class _Here:
-    """_On for the usual case: the device is current, no stream is given."""
-
-    def __init__(self, index: int):
-        self._index = index
-
-    def __enter__(self):
-        return _raw_stream(self._index)
-
-    def __exit__(self, *exc):
-        return False
+_fns: dict = {}
 
 
-_here: dict = {}
-
-
-def _on(device: torch.device, stream):
-    i = device.index
-    if stream is None and i == torch.cuda.current_device():
-        h = _here.get(i)
-        if h is None:
-            h = _here[i] = _Here(i)
-        return h
-    return _On(device, stream)
+def _call(fn: str, *args) -> None:
+    f = _fns.get(fn)
+    if f is None:
+        f = _fns[fn] = getattr(L.lib(), fn)
+    status = f(*args)
+    if status:
+        L.check(status, fn)
 
 
 class PagePlan:
@@ -159,21 +143,24 @@ def page_plan(lens: torch.Tensor, n_new: torch.Tensor, owned: torch.Tensor, bloc
         if not 1 <= n_words <= MAX_NODES // 64:
             raise ValueError(f"n_words must be 1 to {MAX_NODES // 64}, got {n_words}")
     p = PagePlan()
-    with _on(dev, stream) as st:
-        # two buffers: the int64 arrays, the int32 ones
-        wide = torch.empty(n_tokens * (1 if parents is None else 1 + n_words), dtype=torch.int64, device=dev)
-        small = torch.empty(4 * n + 2 + n_tokens, dtype=torch.int32, device=dev)
-        a, w = small.data_ptr(), wide.data_ptr()
-        L.call("bml_paged_plan", a_lens, a_new, a_owned, n, a_free, free_pages.shape[0], a_used, page_size, max_pages,
-               a_table, a_parents, n_tokens, n_words, a, a + 4 * (n + 1), a + 4 * (2 * n + 1), a + 4 * (4 * n + 1), w,
-               a + 4 * (4 * n + 2), None if parents is None else w + 8 * n_tokens, a + 4 * (3 * n + 1), st)
-    p.node_start, p.kv_lens, p.owned, p.status, p.free_used, p.positions = small.split(
-        (n + 1, n, n, n, 1, n_tokens))
-    if parents is None:
-        p.slots, p.mask = wide, None
-    else:
-        p.slots, mask = wide.split((n_tokens, n_tokens * n_words))
-        p.mask = mask.view(n_tokens, n_words)
+    ctx = _enter(dev, stream)
+    try:
+        p.slots = torch.empty(n_tokens, dtype=torch.int64, device=dev)
+        p.mask = a_mask = None
+        if parents is not None:
+            p.mask = torch.empty((n_tokens, n_words), dtype=torch.int64, device=dev)
+            a_mask = p.mask.data_ptr()
+        small = torch.empty(4 * n + 2 + n_tokens, dtype=torch.int32, device=dev)  # the int32 arrays
+        a = small.data_ptr()
+        b = a + 4 * n_tokens
+        _call("bml_paged_plan", a_lens, a_new, a_owned, n, a_free, free_pages.shape[0], a_used, page_size, max_pages,
+              a_table, a_parents, n_tokens, n_words, b, b + 4 * (n + 1), b + 4 * (2 * n + 1), b + 4 * (4 * n + 1),
+              p.slots.data_ptr(), a, a_mask, b + 4 * (3 * n + 1), _raw_stream(dev.index))
+    finally:
+        if ctx is not None:
+            ctx.__exit__(None, None, None)
+    p.positions, p.node_start, p.kv_lens, p.owned, p.status, p.free_used = torch.unsafe_split_with_sizes(
+        small, (n_tokens, n + 1, n, n, n, 1))
     return p
 
 
@@ -223,9 +210,13 @@ def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, slots
                 raise ValueError(f"q_out {tuple(q_out.shape)} does not match q {tuple(q_shape)}")
     elif q_out is not None:
         raise ValueError("q_out without q")
-    with _on(dev, stream) as st:
-        L.call("bml_paged_append", a_q, a_k, a_v, dtype_code(dtype), a_slots, a_pos, n, n_heads, n_kv, d, theta, a_out,
-               a_kp, a_vp, dtype_code(k_pool.dtype), pool[0] * pool[1], st)
+    ctx = _enter(dev, stream)
+    try:
+        _call("bml_paged_append", a_q, a_k, a_v, dtype_code(dtype), a_slots, a_pos, n, n_heads, n_kv, d, theta, a_out,
+              a_kp, a_vp, dtype_code(k_pool.dtype), pool[0] * pool[1], _raw_stream(dev.index))
+    finally:
+        if ctx is not None:
+            ctx.__exit__(None, None, None)
     return q_out
 
 
@@ -281,7 +272,8 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
         rows, n_words = mask.shape
         if rows != n_tokens or not 1 <= n_words <= MAX_NODES // 64:
             raise ValueError(f"mask must be [{n_tokens}, 1 to {MAX_NODES // 64}], got {tuple(mask.shape)}")
-    with _on(dev, stream) as st:
+    ctx = _enter(dev, stream)
+    try:
         if out is None:
             out = torch.empty_like(q)
         elif _data(out, "out", 3, dtype, dev) and out.shape != shape:
@@ -291,9 +283,12 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
         else:
             _ints(workspace, "workspace", dev, dtype=torch.uint8)
-        L.call("bml_attn_tree", a_q, dtype_code(dtype), n_tokens, n_heads, n_kv, d, a_k, a_v, dtype_code(k_pool.dtype),
-               n_pages, page_size, a_table, max_pages, a_len, a_start, n, a_mask, n_words, scale, out.data_ptr(),
-               workspace.data_ptr(), workspace.shape[0], st)
+        _call("bml_attn_tree", a_q, dtype_code(dtype), n_tokens, n_heads, n_kv, d, a_k, a_v, dtype_code(k_pool.dtype),
+              n_pages, page_size, a_table, max_pages, a_len, a_start, n, a_mask, n_words, scale, out.data_ptr(),
+              workspace.data_ptr(), workspace.shape[0], _raw_stream(dev.index))
+    finally:
+        if ctx is not None:
+            ctx.__exit__(None, None, None)
     return out
 
 
@@ -321,10 +316,15 @@ def paged_commit(k_pools: torch.Tensor, v_pools: torch.Tensor, block_table: torc
         raise ValueError(f"block_table must be [{n}, max_pages], got {tuple(block_table.shape)}")
     if path_rows != n:
         raise ValueError(f"path must be [{n}, max_path], got {tuple(path.shape)}")
-    with _on(dev, stream) as st:
+    ctx = _enter(dev, stream)
+    try:
         new = torch.empty_like(lens)
-        L.call("bml_paged_commit", a_k, a_v, layers, n_pages, page_size, n_kv, d, dtype_code(k_pools.dtype), a_table,
-               max_pages, a_lens, a_len, a_start, n, a_path, max_path, a_accept, new.data_ptr(), st)
+        _call("bml_paged_commit", a_k, a_v, layers, n_pages, page_size, n_kv, d, dtype_code(k_pools.dtype), a_table,
+              max_pages, a_lens, a_len, a_start, n, a_path, max_path, a_accept, new.data_ptr(),
+              _raw_stream(dev.index))
+    finally:
+        if ctx is not None:
+            ctx.__exit__(None, None, None)
     return new
 
 
