@@ -1,6 +1,7 @@
 """Builds libbmlattn.so (the CUDA library behind include/bml_attn.h) in-tree
-for sm_100a with nvcc.  No JIT cache is involved: the .so sits next to this
-file and travels with the source tree."""
+for sm_100a with nvcc, and the Python binding of its paged calls with g++.  No
+JIT cache is involved: the .so files sit next to this file and travel with the
+source tree."""
 from __future__ import annotations
 
 import glob
@@ -12,6 +13,8 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libbmlattn.so")
+CALLS = os.path.join(HERE, "_torch_calls.so")
+CALLS_SRC = os.path.join(CSRC, "torch_calls.cpp")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -35,10 +38,34 @@ def headers() -> list[str]:
 
 
 def needs_build() -> bool:
-    if not os.path.exists(LIB):
+    return _older(LIB, sources() + headers()) or _older(CALLS, [CALLS_SRC, *headers()])
+
+
+def _older(target: str, deps: list[str]) -> bool:
+    if not os.path.exists(target):
         return True
-    t = os.path.getmtime(LIB)
-    return any(os.path.getmtime(d) > t for d in sources() + headers())
+    t = os.path.getmtime(target)
+    return any(os.path.getmtime(d) > t for d in deps)
+
+
+def _build_calls(verbose: bool) -> None:
+    """The Python binding of the paged calls (csrc/torch_calls.cpp): host code
+    against the installed torch."""
+    import sysconfig
+
+    import torch
+    root = os.path.join(os.path.dirname(torch.__file__))
+    cuda = os.path.dirname(os.path.dirname(nvcc_path()))
+    inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-I{d}" for d in inc),
+           "-o", CALLS + ".tmp", CALLS_SRC, "-L" + os.path.join(root, "lib"),
+           *(f"-l{x}" for x in ("c10", "c10_cuda", "torch_cpu", "torch_cuda", "torch", "torch_python"))]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    subprocess.run(cmd, check=True)
+    os.replace(CALLS + ".tmp", CALLS)
 
 
 def _object(src: str, newest_header: float, force: bool, verbose: bool) -> str:
@@ -55,17 +82,21 @@ def _object(src: str, newest_header: float, force: bool, verbose: bool) -> str:
 
 def build(force: bool = False, verbose: bool = False) -> str:
     """Compiles every csrc/*.cu to an object (in parallel, each only when it
-    or a header changed) and links libbmlattn.so."""
+    or a header changed) and links libbmlattn.so; then _torch_calls.so."""
     if not force and not needs_build():
         return LIB
     from concurrent.futures import ThreadPoolExecutor
     os.makedirs(BUILD_DIR, exist_ok=True)
     newest = max((os.path.getmtime(h) for h in headers()), default=0.0)
     srcs = sources()
-    with ThreadPoolExecutor(max_workers=min(len(srcs), os.cpu_count() or 4)) as ex:
-        objs = list(ex.map(lambda f: _object(f, newest, force, verbose), srcs))
-    subprocess.run([nvcc_path(), *ARCH, "-shared", "-o", LIB + ".tmp", *objs], check=True)
-    os.replace(LIB + ".tmp", LIB)
+    with ThreadPoolExecutor(max_workers=min(len(srcs), os.cpu_count() or 4) + 1) as ex:
+        calls = ex.submit(_build_calls, verbose) if force or _older(CALLS, [CALLS_SRC, *headers()]) else None
+        if force or _older(LIB, srcs + headers()):
+            objs = list(ex.map(lambda f: _object(f, newest, force, verbose), srcs))
+            subprocess.run([nvcc_path(), *ARCH, "-shared", "-o", LIB + ".tmp", *objs], check=True)
+            os.replace(LIB + ".tmp", LIB)
+        if calls is not None:
+            calls.result()
     return LIB
 
 

@@ -20,6 +20,7 @@ one; `stream` defaults to that device's current stream.
 from __future__ import annotations
 
 import ctypes as C
+import os
 
 import torch
 
@@ -36,9 +37,10 @@ class OutOfPages(RuntimeError):
 
 
 # A call costs the host several microseconds and the GPU often less, so the
-# wrappers take care: one test per tensor on the way that is right (_bad says
-# what is wrong on the other), raw stream handles and addresses, few
-# allocations.
+# usual ones (plain tensors, the current device and stream) are made by a module
+# in C++ (_load); what it leaves alone is checked and called below, with one
+# test per tensor on the way that is right (_bad says what is wrong on the
+# other), raw stream handles and addresses, few allocations.
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 
@@ -85,6 +87,23 @@ def _enter(device: torch.device, stream):
     return ctx
 
 
+_fast = None  # csrc/torch_calls.cpp: the usual calls without Python's share of the time
+
+
+def _load():
+    """Loads that module and gives it the library's entry points."""
+    global _fast
+    path = os.path.join(L.HERE, "_torch_calls.so")
+    if not os.path.exists(path):
+        raise RuntimeError(f"{path} is missing: build it with `python -m bml_b200.build`")
+    from . import _torch_calls
+    lib = L.lib()
+    _torch_calls.set_calls(*(C.cast(getattr(lib, f), C.c_void_p).value for f in (
+        "bml_paged_plan", "bml_paged_append", "bml_attn_tree", "bml_paged_commit", "bml_attn_tree_workspace_size")))
+    _fast = _torch_calls
+    return _fast
+
+
 _fns: dict = {}
 
 
@@ -123,6 +142,13 @@ def page_plan(lens: torch.Tensor, n_new: torch.Tensor, owned: torch.Tensor, bloc
     [n], free_pages, free_used [1] are int32; n_tokens is the row count of
     the step's token arrays, at least the sum of n_new.  lens, owned and
     free_used are not changed: the plan carries their next values."""
+    if stream is None:
+        r = (_fast or _load()).plan(lens, n_new, owned, block_table, free_pages, free_used, page_size, n_tokens, parents,
+                                    n_words)
+        if r is not None:
+            p = PagePlan()
+            p.node_start, p.kv_lens, p.owned, p.free_used, p.status, p.positions, p.slots, p.mask = r
+            return p
     dev = lens.device if isinstance(lens, torch.Tensor) else None
     if dev is None or dev.type != "cuda":
         _bad(lens, "lens", torch.int32, 1)
@@ -183,6 +209,10 @@ def paged_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, slots
     [n_pages, page_size, n_kv, d].  q, k, v in one type (f32, f16, bf16), the
     pools in any.  positions None: no rotation; q None: no queries.  A token
     whose slot is -1 (or outside the pool) is skipped.  Returns the turned q."""
+    if stream is None:
+        r = (_fast or _load()).append(q, k, v, slots, positions, k_pool, v_pool, q_out, theta)
+        if r is not None:
+            return None if r is True else r
     a_k = _data(k, "k", 3)
     dev, dtype = k.device, k.dtype
     a_v = _data(v, "v", 3, dtype, dev)
@@ -252,6 +282,10 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     workspace: an uint8 tensor of tree_workspace_size bytes for calls that
     must not allocate; calls that share one must not overlap.  By default
     scratch comes from torch's allocator, on the call's stream."""
+    if stream is None and out is None and workspace is None:
+        r = (_fast or _load()).tree(q, k_pool, v_pool, block_table, kv_lens, node_start, mask, scale)
+        if r is not None:
+            return r
     a_q = _data(q, "q", 3)
     shape, dev, dtype = q.shape, q.device, q.dtype
     n_tokens, n_heads, d = shape
@@ -301,6 +335,10 @@ def paged_commit(k_pools: torch.Tensor, v_pools: torch.Tensor, block_table: torc
     path [n, max_path] int32 holds strictly increasing node indices; an entry
     that is not ends the path.  Returns the new lengths int32 [n]; a request
     that page_plan refused keeps its own."""
+    if stream is None:
+        r = (_fast or _load()).commit(k_pools, v_pools, block_table, lens, kv_lens, node_start, path, n_accept)
+        if r is not None:
+            return r
     a_k, a_v, pool = _pools(k_pools, v_pools, 5)
     layers, n_pages, page_size, n_kv, d = pool
     dev = k_pools.device

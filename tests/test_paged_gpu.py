@@ -647,3 +647,117 @@ def test_batcher_limits(cuda):
     b.begin({1: 40})
     b.commit()
     assert b.length(1) == 42
+
+
+# ---------------------------------------------------------------------------
+# The two ways of the Python wrappers
+# ---------------------------------------------------------------------------
+class _Leaves:
+    """Stands for the binding in C++ and leaves every call to the wrappers."""
+
+    def __getattr__(self, name):
+        return lambda *a: None
+
+
+def _all_calls():
+    import bml_b200
+    c = Paged([40, 3], [3, 1], 4, 2, 64, 16, "bf16", "bf16", seed=30)
+    free, used = ints(list(range(20))), ints([0])
+    p = bml_b200.page_plan(ints([0, 5]), ints([3, 20]), ints([0, 1]), c.table.clone(), free, used, 16, 25,
+                           parents=ints([-1, 0, 0] + list(range(-1, 19)) + [0, 0]), n_words=2)
+    outs = [p.node_start, p.kv_lens, p.owned, p.free_used, p.status, p.positions, p.slots, p.mask]
+    p = bml_b200.page_plan(ints([0, 5]), ints([3, 20]), ints([0, 1]), c.table.clone(), free, used, 16, 23)
+    outs += [p.positions, p.slots]
+    assert p.mask is None
+    kp, vp = torch.zeros(3, 16, 2, 64, device="cuda"), torch.zeros(3, 16, 2, 64, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(31)
+    q, k, v = (torch.randn(4, h, 64, device="cuda", generator=g) for h in (4, 2, 2))
+    slots, pos = torch.tensor([1, -1, 40, 7], device="cuda"), ints([5, 6, 7, 100000])
+    q2 = torch.empty_like(q).fill_(1)
+    assert bml_b200.paged_append(q, k, v, slots, pos, kp, vp, q_out=q2) is q2
+    assert bml_b200.paged_append(None, k, v, slots, None, vp, kp) is None
+    outs += [q2, kp, vp]
+    outs.append(bml_b200.tree_attention(c.q, c.k, c.v, c.table, c.kv_lens, c.start))
+    outs.append(bml_b200.tree_attention(c.q, c.k, c.v, c.table, c.kv_lens, c.start, scale=0.3, mask=torch.full(
+        (4, 1), 5, dtype=torch.int64, device="cuda")))
+    kc, vc = c.k[None].nan_to_num().contiguous(), c.v[None].nan_to_num().contiguous()
+    outs.append(bml_b200.paged_commit(kc, vc, c.table, ints([40, 3]), c.kv_lens, c.start, ints([[0, 2], [0, 0]]), ints([2, 1])))
+    return outs + [kc, vc]
+
+
+def test_both_ways_agree(cuda, monkeypatch):
+    """The binding in C++ and the wrappers' own way give the same bits."""
+    import bml_b200.paged as P
+    a = _all_calls()
+    assert P._fast is not None
+    monkeypatch.setattr(P, "_fast", _Leaves())
+    b = _all_calls()
+    assert len(a) == len(b)
+    for x, y in zip(a, b):
+        assert x.dtype == y.dtype and x.shape == y.shape and torch.equal(x, y)
+
+
+def test_refusals_of_gpu_tensors(cuda):
+    """What either way must not let through: another type, shape, device or
+    layout, and what the C call refuses."""
+    import bml_b200
+    c = Paged([40, 3], [3, 1], 4, 2, 64, 16, "bf16", "bf16", seed=32)
+    t = bml_b200.tree_attention
+    good = (c.q, c.k, c.v, c.table, c.kv_lens, c.start)
+    assert t(*good).shape == c.q.shape
+
+    def bad(i, x, err=ValueError, **kw):
+        args = list(good)
+        if i is not None:
+            args[i] = x
+        with pytest.raises(err):
+            t(*args, **kw)
+
+    bad(0, c.q.double(), TypeError)
+    bad(0, c.q.half(), bml_b200.BmlUnsupported)
+    bad(0, c.q.transpose(0, 1).contiguous().transpose(0, 1))
+    bad(0, c.q[:, :3].contiguous(), bml_b200.BmlInvalid)          # 3 heads over 2
+    bad(0, torch.cat([c.q, c.q], 2), ValueError)
+    bad(0, c.q.cpu())
+    bad(1, c.k.float(), TypeError)
+    bad(1, c.k[:, :8].contiguous())
+    bad(2, c.v[:1])
+    bad(3, c.table.long(), TypeError)
+    bad(3, c.table[:1])
+    bad(4, c.kv_lens[:1])
+    bad(4, c.kv_lens.long(), TypeError)
+    bad(5, c.start[:2])
+    bad(None, None, mask=torch.zeros(4, 1, dtype=torch.int32, device="cuda"), err=TypeError)
+    bad(None, None, mask=torch.zeros(3, 1, dtype=torch.int64, device="cuda"))
+    bad(None, None, mask=torch.zeros(4, 5, dtype=torch.int64, device="cuda"))
+    bad(None, None, scale=float("nan"), err=bml_b200.BmlInvalid)
+    bad(None, None, out=c.q, err=bml_b200.BmlInvalid)
+    bad(None, None, out=torch.empty_like(c.q[:2]))
+    bad(None, None, workspace=torch.empty(64, dtype=torch.uint8, device="cuda"), err=bml_b200.BmlInvalid)
+    odd = torch.empty(c.k.numel() + 1, dtype=c.k.dtype, device="cuda")[1:].view(c.k.shape)
+    bad(1, odd, bml_b200.BmlInvalid)                               # pool off a 16-byte boundary
+    wide = torch.zeros(4, 4, 96, device="cuda", dtype=torch.bfloat16)
+    pool = torch.zeros(4, 16, 2, 96, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(bml_b200.BmlUnsupported):
+        t(wide, pool, pool, *good[3:])
+    i2 = ints([1, 1])
+    with pytest.raises(ValueError):
+        bml_b200.page_plan(i2, ints([1]), i2, c.table, i2, ints([0]), 16, 2)
+    with pytest.raises(bml_b200.BmlInvalid):
+        bml_b200.page_plan(i2, i2, i2, c.table, i2, ints([0]), 17, 2)
+    with pytest.raises(ValueError):
+        bml_b200.page_plan(i2, i2, i2, c.table, i2, ints([0]), 16, 2, parents=i2, n_words=5)
+    with pytest.raises(ValueError):
+        bml_b200.page_plan(i2, i2, i2, c.table, i2, ints([0]), 16, -1)
+    q, kv = torch.zeros(2, 4, 64, device="cuda"), torch.zeros(2, 2, 64, device="cuda")
+    sl = torch.zeros(2, dtype=torch.int64, device="cuda")
+    with pytest.raises(TypeError):
+        bml_b200.paged_append(q.half(), kv, kv, sl, i2, c.k, c.v)
+    with pytest.raises(ValueError):
+        bml_b200.paged_append(q, kv, kv, sl[:1], i2, c.k, c.v)
+    with pytest.raises(ValueError):
+        bml_b200.paged_append(None, kv, kv, sl, i2, c.k, c.v, q_out=q)
+    with pytest.raises(bml_b200.BmlInvalid):
+        bml_b200.paged_append(q, kv, kv, sl, i2, c.k, c.v, theta=-1.0)
+    with pytest.raises(ValueError):
+        bml_b200.paged_commit(c.k[None], c.v[None], c.table, i2, c.kv_lens, c.start, i2, i2)
