@@ -336,6 +336,89 @@ def test_streams_and_graphs(cuda, qt, ct):
     assert torch.equal(outs[0], bml_b200.tree_attention(c.q, c.k, c.v, c.table, c.kv_lens, c.start))
 
 
+@pytest.mark.parametrize("qt,ct", TYPES)
+def test_uneven_batches(cuda, qt, ct):
+    """Batches whose average picks a kernel for few rows, with requests of many
+    (several row groups a head), and the other way round."""
+    import bml_b200
+    rng = np.random.default_rng(40)
+    for nodes in ([1] * 60 + [100, 9, 33], [8] * 20 + [256, 0, 70], [256, 256, 1, 0, 5, 64, 60]):
+        lens = [int(x) for x in rng.integers(0, 700, len(nodes))]
+        c = Paged(lens, nodes, 8, 2, 64, 32, qt, ct, seed=len(nodes))
+        masks = [mask_of(random_parents(rng, t)) for t in nodes]
+        sees = [np.concatenate([np.ones((t, p), bool), m.reshape(t, t)], 1) for t, p, m in zip(nodes, lens, masks)]
+        got = bml_b200.tree_attention(c.q, c.k, c.v, c.table, c.kv_lens, c.start, mask=pack(masks, 4))
+        check(c, got, sees, qt)
+
+
+@pytest.mark.parametrize("qt,ct", TYPES)
+@pytest.mark.parametrize("heads,kv", [(160, 1), (96, 1), (7, 7), (40, 8), (6, 2), (24, 12)])
+def test_head_groups(cuda, qt, ct, heads, kv):
+    """Groups of 1 to 160 q heads a kv head, kv heads that no power of two divides."""
+    import bml_b200
+    for nodes in ([1, 1, 1], [30, 2, 17]):
+        lens = [200, 0, 513]
+        c = Paged(lens, nodes, heads, kv, 64, 16, qt, ct, seed=heads)
+        got = bml_b200.tree_attention(c.q, c.k, c.v, c.table, c.kv_lens, c.start)
+        check(c, got, [chain(t, p) for t, p in zip(nodes, lens)], qt)
+
+
+@pytest.mark.parametrize("qt,ct", TYPES)
+@pytest.mark.parametrize("nodes", [[1, 1], [4, 4], [40, 40]])
+def test_scales(cuda, qt, ct, nodes):
+    """A scale of 0 (the mean of what a row sees), a tiny and a large one."""
+    import bml_b200
+    lens = [150, 5]
+    c = Paged(lens, nodes, 8, 2, 128, 16, qt, ct, seed=41)
+    for scale in (0.0, 1e-20, 0.7):
+        got = bml_b200.tree_attention(c.q, c.k, c.v, c.table, c.kv_lens, c.start, scale=scale)
+        check(c, got, [chain(t, p) for t, p in zip(nodes, lens)], qt, scale=scale)
+
+
+@pytest.mark.parametrize("qt,ct", TYPES)
+@pytest.mark.parametrize("nodes", [[1, 1, 1], [3, 2, 5], [40, 40, 3]])
+def test_nan_that_is_seen(cuda, qt, ct, nodes):
+    """A NaN in a committed K row makes its head's rows of that request NaN, one
+    in a V row the same dims of them; a NaN query its own row; nothing else."""
+    import bml_b200
+    lens = [300, 300, 300]
+    for where in range(0, 300, 37):
+        c = Paged(lens, nodes, 4, 2, 64, 16, qt, ct, seed=42)
+        page = int(c.table[0, where // 16])
+        c.k[page, where % 16, 1, 5] = float("nan")
+        page = int(c.table[1, where // 16])
+        c.v[page, where % 16, 0, 7] = float("nan")
+        c.q[-1, 2] = float("nan")
+        got = bml_b200.tree_attention(c.q, c.k, c.v, c.table, c.kv_lens, c.start)
+        want = torch.zeros_like(got, dtype=torch.bool)
+        s = c.start.tolist()
+        want[:s[1], 2:] = True            # q heads 2, 3 read kv head 1
+        want[s[1]:s[2], :2, 7] = True
+        want[-1, 2] = True
+        assert torch.equal(torch.isnan(got), want)
+
+
+def test_two_streams_at_once(cuda):
+    """Eager calls of every form on two streams, neither waiting for the other."""
+    import bml_b200
+    cases = [Paged([900, 30, 77], nodes, 8, 2, 128, 64, qt, ct, seed=s)
+             for s, (nodes, qt, ct) in enumerate([([1, 1, 1], "bf16", "bf16"), ([9, 3, 8], "f16", "f16"),
+                                                  ([50, 60, 3], "bf16", "bf16"), ([9, 3, 8], "f32", "f32"),
+                                                  ([1, 1, 1], "f32", "bf16")])]
+    call = lambda c, st=None: bml_b200.tree_attention(c.q, c.k, c.v, c.table, c.kv_lens, c.start, stream=st)  # noqa: E731
+    want = [call(c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for _ in range(10):
+        for st in streams:
+            got.append([call(c, st) for c in cases])
+    torch.cuda.synchronize()
+    for g in got:
+        for x, w in zip(g, want):
+            assert torch.equal(x, w)
+
+
 # ---------------------------------------------------------------------------
 # page_plan
 # ---------------------------------------------------------------------------
