@@ -15,27 +15,37 @@ namespace bml {
 namespace {
 
 // ---------------------------------------------------------------------------
-// Block-wide exclusive scan of one 64-bit value per thread
+// Block-wide exclusive scan of two 64-bit values per thread
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t *warp_sums, int64_t *total) {
+struct Pair64 {
+    int64_t x, y;
+};
+__device__ __forceinline__ Pair64 block_scan(Pair64 v, Pair64 *warp_sums, Pair64 *total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    int64_t inc = v;
+    Pair64 inc = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t u = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += u;
+        const int64_t a = __shfl_up_sync(0xffffffffu, inc.x, o), b = __shfl_up_sync(0xffffffffu, inc.y, o);
+        if (lane >= o) {
+            inc.x += a;
+            inc.y += b;
+        }
     }
     if (lane == 31) warp_sums[warp] = inc;
     __syncthreads();
-    int64_t before = 0, all = 0;
+    Pair64 before = {0, 0}, all = {0, 0};
     for (int w = 0; w < nw; ++w) {
-        const int64_t s = warp_sums[w];
-        before += w < warp ? s : 0;
-        all += s;
+        const Pair64 s = warp_sums[w];
+        if (w < warp) {
+            before.x += s.x;
+            before.y += s.y;
+        }
+        all.x += s.x;
+        all.y += s.y;
     }
     __syncthreads();
     *total = all;
-    return before + inc - v;
+    return {before.x + inc.x - v.x, before.y + inc.y - v.y};
 }
 
 // ---------------------------------------------------------------------------
@@ -62,18 +72,15 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParam
     int32_t *s_start = sh;                 // [n + 1] first token
     int32_t *s_base = sh + p.n + 1;        // [n] first new page's place in the free list
     int32_t *s_own = s_base + p.n;         // [n] pages held before, or -1: refused
-    __shared__ int64_t warp_sums[kPlanThreads / 32];
+    __shared__ Pair64 warp_sums[kPlanThreads / 32];
     const uint32_t per = (p.n + kPlanThreads - 1) / kPlanThreads;
     const uint32_t i0 = min(threadIdx.x * per, p.n), i1 = min(i0 + per, p.n);
     const int64_t ps = 1ll << p.page_shift;
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    int64_t tok = 0;
-    for (uint32_t i = i0; i < i1; ++i) tok += max(p.n_new[i], 0);
-    int64_t all_tok;
-    int64_t at = block_scan(tok, warp_sums, &all_tok);
-    const int64_t first_tok = at;
-    // pages: requests that are bad or whose tokens do not fit take none
+    // A request that is bad takes no pages, and neither does one whose tokens do
+    // not fit: that is known only after the scan of the tokens, so in the rare
+    // case that they do not all fit the pages are summed again.
     auto judge = [&](uint32_t i, int64_t end, int64_t &add) {
         const int64_t len = p.lens[i], nw = p.n_new[i], own = p.owned[i];
         const int64_t need = (len + nw + ps - 1) >> p.page_shift;
@@ -85,15 +92,27 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParam
         add = need > own ? need - own : 0;
         return 0;
     };
-    int64_t pages = 0;
+    Pair64 mine = {0, 0}, all;
     for (uint32_t i = i0; i < i1; ++i) {
         int64_t add;
-        at += max(p.n_new[i], 0);
-        judge(i, at, add);
-        pages += add;
+        judge(i, 0, add);
+        mine.x += max(p.n_new[i], 0);
+        mine.y += add;
     }
-    int64_t all_pages;
-    int64_t cum = block_scan(pages, warp_sums, &all_pages);
+    Pair64 before = block_scan(mine, warp_sums, &all);
+    const int64_t first_tok = before.x, all_tok = all.x;
+    int64_t at = first_tok;
+    if (all_tok > p.n_tokens) {
+        mine.y = 0;
+        for (uint32_t i = i0; i < i1; ++i) {
+            int64_t add;
+            at += max(p.n_new[i], 0);
+            judge(i, at, add);
+            mine.y += add;
+        }
+        before = block_scan(mine, warp_sums, &all);
+    }
+    int64_t cum = before.y;
     const int64_t used = min(max(*p.free_used, 0), (int32_t)p.n_free);
     const int64_t avail = (int64_t)p.n_free - used;
     int64_t granted = 0;  // largest running sum that still fits
@@ -126,13 +145,13 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParam
             const int64_t u = __shfl_xor_sync(0xffffffffu, granted, o);
             granted = granted > u ? granted : u;
         }
-        if ((threadIdx.x & 31) == 0) warp_sums[threadIdx.x >> 5] = granted;
+        if ((threadIdx.x & 31) == 0) warp_sums[threadIdx.x >> 5].x = granted;
     }
     __syncthreads();
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         p.node_start[p.n] = s_start[p.n];
         int64_t g = 0;
-        for (int w = 0; w < kPlanThreads / 32; ++w) g = g > warp_sums[w] ? g : warp_sums[w];
+        for (int w = 0; w < kPlanThreads / 32; ++w) g = g > warp_sums[w].x ? g : warp_sums[w].x;
         *p.free_used_out = (int32_t)(used + g);
     }
 

@@ -27,14 +27,13 @@ constexpr int kThreads = 256;
 constexpr float kGrow = 8.0f;  // log2 units a row's maximum may grow before O is rescaled
 constexpr int kWarps = kThreads / 32;
 
-__device__ __forceinline__ uint32_t tf32_hi(float x) {
-    uint32_t r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-    return r;
-}
+// hi: x rounded to TF32's 10 fraction bits, half away from zero, with integer
+// operations (a conversion instruction runs at a quarter of their rate and set
+// the time: 4 requests of 618 to 2671 positions 85 -> 75 us).  lo: the rest, of
+// which the matrix unit takes the upper bits itself.
 __device__ __forceinline__ void tf32_split(float x, uint32_t &hi, uint32_t &lo) {
-    hi = tf32_hi(x);
-    lo = tf32_hi(x - __uint_as_float(hi));
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
 }
 __device__ __forceinline__ void mma_tf32(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
     asm volatile(
