@@ -478,12 +478,12 @@ __global__ void __launch_bounds__(kThreads, 2) tree_merge_kernel(const __grid_co
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the segments' partials are written
     if (!mine) return;
     // A task is 8 rows x 32 columns (lane: row, twice 4 columns).  Up to 32
-    // segments: a warp a task, the loads of 8 segments in flight together; more
-    // (one long request): a CTA a task, the warps taking the segments in turns
-    // and meeting in shared memory.
+    // segments (8 where there is a CTA for every task): a warp a task, the loads
+    // of 8 segments in flight together; more (one long request): a CTA a task,
+    // the warps taking the segments in turns and meeting in shared memory.
     constexpr uint32_t kBatch = 8;
     const uint32_t R = p.rpg * p.hpu, tasks = (R + 7) / 8 * (D / 32);
-    const bool many = last - b > 30;
+    const bool many = last - b > 30 || (last - b > 6 && gridDim.y >= tasks);
     const uint32_t step = many ? kWarps : 1;
     for (uint32_t task = many ? blockIdx.y : blockIdx.y * kWarps + warp; task < tasks; task += gridDim.y * (many ? 1 : kWarps)) {
         const uint32_t row = task / (D / 32) * 8 + (lane & 7), x4 = task % (D / 32) * 8 + (lane >> 3);
@@ -634,10 +634,19 @@ size_t tree_workspace_bytes(uint32_t D, int num_sms) {
 
 cudaError_t launch_tree(const TreeArgs &a, cudaStream_t st) {
     // 16-bit pages, except for a scale of 0 (those kernels scale masked scores
-    // after they were set to -inf)
+    // after they were set to -inf).  Up to 8 rows a kv head (on average): the
+    // form with positions as MMA rows (64 x 4000, d = 64, 8 rows: 49 us, 73 with
+    // tree_warp.cu).  16-bit queries of more rows: tcgen05 where there is enough
+    // work for its longer start (32 x 8000, d = 128: 24 rows 177 us against 217,
+    // 64 rows 178 against 339; 12 rows 177 against 187; 64 x 4000, d = 64: 24
+    // rows 82 against 93, 48 rows 78 against 144, 16 rows 82 against 74; but one
+    // request of 708 positions, 4 kv heads, 64 rows 15 against 11 us).  How much
+    // work there is the host knows only as a bound, the tables' width.
     if (a.kv_type != BML_F32 && a.p.scale_log2 > 0.f) {
         if (a.rows <= 8) return launch_tree_few(a, st);
-        if (a.p.q_type == BML_F32 || a.rows <= 64 || !tree_umma_fits(a)) return launch_tree_warp(a, st);
+        const uint64_t most = (((uint64_t)a.p.max_pages << a.p.page_shift) + kTreeTile - 1) / kTreeTile * a.p.n_seqs * a.p.n_kv;
+        const bool small = most <= 2ull * a.num_sms || a.rows <= (a.D == 128 ? 8u : 16u);
+        if (a.p.q_type == BML_F32 || !tree_umma_fits(a) || (small && a.rows <= 64)) return launch_tree_warp(a, st);
         return launch_tree_umma(a, st);
     }
     return a.D == 128 ? launch_kv<128>(a, st) : launch_kv<64>(a, st);

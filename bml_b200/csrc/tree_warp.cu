@@ -8,9 +8,8 @@
 // call, of a segment's start and of its end.  So a warp keeps everything of
 // its 16 rows in registers (Q fragments, scores, output) and works through
 // its positions by itself with mma.sync.m16n8k16; a 128-row tcgen05 tile
-// would spend its softmax and its epilogue on empty rows (measured on B200:
-// tree_umma.cu takes 93 us for 64 requests of 4000 positions, d = 64, one
-// token each, this kernel a third of that).
+// would spend its softmax and its epilogue on empty rows.  Its calls and the
+// rule that picks it stand in tree.cu.
 //
 // RW warps (1, 2 or 4) cover RW * 16 rows; the 8 / RW groups of RW warps take
 // turns at blocks of SP = 16 * RW positions, so that a tile of 128 positions
