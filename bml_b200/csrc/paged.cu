@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParam
     // A request that is bad takes no pages, and neither does one whose tokens do
     // not fit: that is known only after the scan of the tokens, so in the rare
     // case that they do not all fit the pages are summed again.
-    auto judge = [&](uint32_t i, int64_t end, int64_t &add) {
+    auto verify = [&](uint32_t i, int64_t end, int64_t &add) {
         const int64_t len = p.lens[i], nw = p.n_new[i], own = p.owned[i];
         const int64_t need = (len + nw + ps - 1) >> p.page_shift;
         add = 0;
@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParam
     Pair64 mine = {0, 0}, all;
     for (uint32_t i = i0; i < i1; ++i) {
         int64_t add;
-        judge(i, 0, add);
+        verify(i, 0, add);
         mine.x += max(p.n_new[i], 0);
         mine.y += add;
     }
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParam
         for (uint32_t i = i0; i < i1; ++i) {
             int64_t add;
             at += max(p.n_new[i], 0);
-            judge(i, at, add);
+            verify(i, at, add);
             mine.y += add;
         }
         before = block_scan(mine, warp_sums, &all);
@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParam
         int64_t add;
         const int64_t begin = at;
         at += max(p.n_new[i], 0);
-        int32_t st = judge(i, at, add);
+        int32_t st = verify(i, at, add);
         const int64_t base = cum;
         cum += add;
         if (st == 0 && add > 0) {

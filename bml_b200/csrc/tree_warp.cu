@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
                 const bool ok = page < p.n_pages;
                 const size_t at = ok ? (((size_t)page << p.page_shift) + (pos & pmask)) * prow + (size_t)fs.head * (D * 2) : 0;
                 if (tig == 0) flags[f_stage * 4 + b] = ok;
-                constexpr int ROWS = RW * 32 / PER;  // rows of one round of pieces
+                constexpr int ROWS = RW * 32 / PER;  // rows of one pass over the pieces
 #pragma unroll
                 for (int i = 0; i < 16 / ROWS; ++i) {
                     const int r = i * ROWS + tig / PER, x = (tig % PER) * 16;

@@ -100,7 +100,7 @@ def test_workspace_size(L):
     assert 0 < n.value < 1 << 27
 
 
-def test_python_refusals():
+def test_python_refusals(L):
     """CPU tensors are refused by name before the library is reached."""
     import bml_b200
     i, x = torch.zeros(2, dtype=torch.int32), torch.zeros(2, 4, 64)

@@ -697,6 +697,33 @@ def test_batcher_run(cuda, qt, ct):
     assert sorted(held + b.free[used:].tolist()) == list(range(40))
 
 
+def test_empty_steps(cuda):
+    """No request at all, requests without new tokens, and a request without a
+    prompt whose first step is a draft."""
+    import bml_b200
+    b = bml_b200.PagedBatcher(1, 4, 2, 64, n_pages=8, page_size=16, max_positions=64, max_requests=3)
+    none = [torch.empty(0, h, 64, device="cuda", dtype=torch.bfloat16) for h in (4, 2, 2)]
+    for _ in range(2):
+        plan = b.begin({})
+        assert plan.slots.numel() == 0 and plan.node_start.tolist() == [0] * 4
+        assert b.step(0, *none).shape == (0, 4, 64)
+        b.commit()
+        if not len(b):
+            b.add("x")
+            b.add("y")
+    plan = b.begin({"y": [-1, -1, 0, 2]})
+    assert plan.node_start.tolist() == [0, 0, 4, 4] and plan.positions.tolist() == [0, 0, 1, 2]
+    q, k, v = (torch.randn(4, h, 64, device="cuda").bfloat16() for h in (4, 2, 2))
+    out = b.step(0, q, k, v)
+    want = v[:2].repeat_interleave(2, 1)      # a root sees itself only
+    assert torch.equal(out[:2], want)
+    b.commit({"y": []})
+    assert b.length("x") == b.length("y") == 0
+    b.remove("y")
+    b.remove("x")
+    assert len(b) == 0 and int(b.used) == 0 and sorted(b.free.tolist()) == list(range(8))
+
+
 def test_batcher_limits(cuda):
     import bml_b200
     b = bml_b200.PagedBatcher(1, 4, 2, 64, n_pages=3, page_size=16, max_positions=64, max_requests=2)
