@@ -66,6 +66,21 @@ bml_status ints(const char *fn, std::initializer_list<const void *> ps) {
     return BML_OK;
 }
 
+// Whether an array that a call writes overlaps one that it reads: its CTAs do
+// not wait for one another.
+struct Span {
+    const void *p;
+    uint64_t bytes;
+};
+bool overlap(std::initializer_list<Span> written, std::initializer_list<Span> read) {
+    for (const Span &w : written)
+        for (const Span &r : read) {
+            const uintptr_t a = reinterpret_cast<uintptr_t>(w.p), b = reinterpret_cast<uintptr_t>(r.p);
+            if (a && b && a < b + r.bytes && b < a + w.bytes) return true;
+        }
+    return false;
+}
+
 }  // namespace
 
 BML_API bml_status bml_paged_plan(const int32_t *lens, const int32_t *n_new, const int32_t *owned, uint32_t n,
@@ -83,13 +98,17 @@ BML_API bml_status bml_paged_plan(const int32_t *lens, const int32_t *n_new, con
     if (n_free && (!free_pages || !aligned(free_pages, 4))) return api_fail(BML_E_INVALID, "%s: null or misaligned free_pages", fn);
     if (n_tokens && (!slots || !aligned(slots, 8) || !positions || !aligned(positions, 4)))
         return api_fail(BML_E_INVALID, "%s: null or misaligned slots or positions", fn);
-    if (owned_out == owned || free_used_out == free_used)
-        return api_fail(BML_E_INVALID, "%s: owned_out and free_used_out need buffers of their own", fn);
     if (n_tokens && parents) {
         if (n_words < 1 || n_words > bml::kTreeMaxNodes / 64) return api_fail(BML_E_INVALID, "%s: %u mask words (1 to 4)", fn, n_words);
         if (!aligned(parents, 4) || !mask || !aligned(mask, 8))
             return api_fail(BML_E_INVALID, "%s: parents need a mask (both aligned)", fn);
     }
+    const uint64_t n4 = 4ull * n, t4 = 4ull * n_tokens;
+    const bool drafts = n_tokens && parents;
+    if (overlap({{node_start, n4 + 4}, {kv_lens, n4}, {owned_out, n4}, {free_used_out, 4}, {status, n4}, {slots, 2 * t4},
+                 {positions, t4}, {drafts ? mask : nullptr, 2 * t4 * n_words}, {block_table, n4 * max_pages}},
+                {{lens, n4}, {n_new, n4}, {owned, n4}, {free_pages, 4ull * n_free}, {free_used, 4}, {drafts ? parents : nullptr, t4}}))
+        return api_fail(BML_E_INVALID, "%s: results need buffers of their own, not those of lens, n_new, owned, parents or the free list", fn);
     bml::PlanParams p = {};
     p.lens = lens;
     p.n_new = n_new;
@@ -130,6 +149,7 @@ BML_API bml_status bml_paged_append(const void *q_dev, const void *k_dev, const 
     if ((q_dev == nullptr) != (q_out_dev == nullptr)) return api_fail(BML_E_INVALID, "%s: q and q_out come together", fn);
     if (q_dev && n_heads == 0) return api_fail(BML_E_INVALID, "%s: zero q heads", fn);
     if (positions && !(theta > 0.0 && isfinite(theta))) return api_fail(BML_E_INVALID, "%s: theta must be positive", fn);
+    if (positions && theta < 1.0 / 65536) return api_fail(BML_E_UNSUPPORTED, "%s: theta %g (at least 2^-16)", fn, theta);
     if (n_tokens == 0) return bml::api_ok();
     if (n_tokens > 0x7fffffffu || n_rows > 0x7fffffffull) return api_fail(BML_E_INVALID, "%s: count above 2^31 - 1", fn);
     if (!k_dev || !v_dev || !k_pool || !v_pool || !slots) return api_fail(BML_E_INVALID, "%s: null pointer", fn);
@@ -189,7 +209,7 @@ BML_API bml_status bml_attn_tree(const void *q_dev, bml_dtype q_dtype, uint32_t 
     if (bml_status st = check_pages(page_size, max_pages, fn)) return st;
     if ((uint64_t)n_pages * page_size >= (1ull << 31)) return api_fail(BML_E_INVALID, "%s: %u pages of %u positions", fn, n_pages, page_size);
     if (mask && (n_words < 1 || n_words > bml::kTreeMaxNodes / 64)) return api_fail(BML_E_INVALID, "%s: %u mask words (1 to 4)", fn, n_words);
-    if (isnan(scale) || isinf(scale)) return api_fail(BML_E_INVALID, "%s: scale is not finite", fn);
+    if (isnan(scale) || isinf(scale * 1.4426950f)) return api_fail(BML_E_INVALID, "%s: scale is not finite", fn);
     if (bml_status st = ints(fn, {block_table, kv_lens, node_start})) return st;
     if (n_tokens == 0) return bml::api_ok();
     if (n_tokens > 0x7fffffffu) return api_fail(BML_E_INVALID, "%s: %u tokens", fn, n_tokens);
@@ -255,7 +275,9 @@ BML_API bml_status bml_paged_commit(void *k_pool, void *v_pool, uint32_t n_layer
     const uint64_t row = (uint64_t)n_kv_heads * head_dim * bml::dtype_size(kv_dtype);
     if (row > 0x7fffffffull) return api_fail(BML_E_INVALID, "%s: a row of %llu bytes", fn, (unsigned long long)row);
     if (!k_pool || !v_pool || !aligned(k_pool, 4) || !aligned(v_pool, 4)) return api_fail(BML_E_INVALID, "%s: null or misaligned pool", fn);
-    if (lens_out == lens) return api_fail(BML_E_INVALID, "%s: lens_out needs a buffer of its own", fn);
+    if (overlap({{lens_out, 4ull * n}}, {{lens, 4ull * n}, {kv_lens, 4ull * n}, {node_start, 4ull * n + 4}, {n_accept, 4ull * n},
+                                          {path, 4ull * n * max_path}, {block_table, 4ull * n * max_pages}}))
+        return api_fail(BML_E_INVALID, "%s: lens_out needs a buffer of its own", fn);
     bml::CommitParams p = {};
     p.k_pool = static_cast<char *>(k_pool);
     p.v_pool = static_cast<char *>(v_pool);

@@ -416,8 +416,7 @@ bml_status bml_kvsplit_destroy(bml_kvsplit *h);
  *       and pages are taken from there on, in request order;
  *   node_start [n+1]: first token row of each request, and the end;
  *   kv_lens [n]: lens + n_new, or 0 for a refused request;
- *   owned_out [n], free_used_out [1]: the counts after this plan (their own
- *       buffers: not owned, not free_used);
+ *   owned_out [n], free_used_out [1]: the counts after this plan;
  *   block_table [n][max_pages]: new entries written, others left;
  *   slots [n_tokens] int64: row of the pool for each token, -1 for a token of
  *       a refused request and for rows behind the last token;
@@ -433,8 +432,8 @@ bml_status bml_kvsplit_destroy(bml_kvsplit *h);
  *       row holds, more than 64 * n_words drafted tokens, or a negative
  *       count, 4 its tokens lie beyond n_tokens.  A refused request takes no
  *       pages.
- * All arrays are int32 on the device unless noted.  n <= 4096.
- * Asynchronous. */
+ * All arrays are int32 on the device unless noted; results have buffers of
+ * their own.  n <= 4096.  Asynchronous. */
 bml_status bml_paged_plan(const int32_t *lens, const int32_t *n_new,
                           const int32_t *owned, uint32_t n,
                           const int32_t *free_pages, uint32_t n_free,
@@ -457,7 +456,8 @@ bml_status bml_paged_plan(const int32_t *lens, const int32_t *n_new,
  * are f64, the rotation f32; results are rounded once to the destination's
  * type.  Slots of one call must differ (of two tokens with the same slot,
  * either's values may be stored).  head_dim even; pointers aligned to two
- * elements.  Asynchronous. */
+ * elements; theta at least 2^-16; negative positions count as 0.
+ * Asynchronous. */
 bml_status bml_paged_append(const void *q_dev, const void *k_dev,
                             const void *v_dev, bml_dtype src_dtype,
                             const int64_t *slots, const int32_t *positions,
@@ -475,6 +475,7 @@ bml_status bml_attn_tree_workspace_size(uint32_t head_dim, int32_t device,
  * request i (node j = t - node_start[i] of T) attends over the committed
  * positions [0, kv_lens[i] - T) and over those nodes whose bits are set in
  * mask[t]; mask NULL: over nodes 0..j (a chain; T = 1 is plain decode).
+ *   node_start: ascending, as bml_paged_plan writes it;
  *   q_dev, out_dev: [n_tokens][n_heads][head_dim] in q_dtype: BML_F32 with
  *       pages of any type, or the pages' own 16-bit type;
  *   workspace: bml_attn_tree_workspace_size bytes, 16-byte aligned, no
@@ -509,8 +510,8 @@ bml_status bml_attn_tree(const void *q_dev, bml_dtype q_dtype,
  * strictly increasing node indices; an entry that is not larger than the one
  * before, or not below the request's node count, ends the path there, and the
  * count with it.  A request with kv_lens[i] != lens[i] + its node count (one
- * that the plan refused) commits nothing.  lens_out is its own buffer, not
- * lens.  Asynchronous. */
+ * that the plan refused) commits nothing.  lens_out is its own buffer.
+ * Asynchronous. */
 bml_status bml_paged_commit(void *k_pool, void *v_pool, uint32_t n_layers,
                             uint32_t n_pages, uint32_t page_size,
                             uint32_t n_kv_heads, uint32_t head_dim,

@@ -77,8 +77,30 @@ def test_invalid_arguments(L, call, bad):
     assert L.last_error()
 
 
+B = 1 << 24
+APART = {  # (call, arrays it reads, arrays it writes)
+    plan: (("lens", "n_new", "owned", "free_pages", "free_used", "parents"),
+           ("node_start", "kv_lens", "owned_out", "free_used_out", "status", "slots", "positions", "mask", "block_table")),
+    commit: (("lens", "kv_lens", "node_start", "n_accept", "path", "table"), ("lens_out",)),
+}
+
+
+@pytest.mark.parametrize("call,read,written", [(c, r, w) for c, (rs, ws) in APART.items() for r in rs for w in ws])
+def test_results_have_buffers_of_their_own(L, call, read, written):
+    """An array that a call both reads and writes, or one that ends inside
+    another, is refused: its CTAs do not wait for one another."""
+    names = APART[call][0] + APART[call][1]
+    apart = {n: B + 4096 * i for i, n in enumerate(names)}
+    before = {"free_used_out": 0, "slots": 8, "mask": 8}.get(written, 4)
+    for same in (apart[read], apart[read] - before):
+        assert call(L.lib(), **{**apart, written: same}) == L.BML_E_INVALID
+        assert "own" in L.last_error()
+
+
 def test_unsupported(L):
     lib = L.lib()
+    assert append(lib, theta=1e-6) == L.BML_E_UNSUPPORTED
+    assert attend(lib, scale=3e38) == L.BML_E_INVALID         # not finite in units of log2
     assert attend(lib, head_dim=96) == L.BML_E_UNSUPPORTED
     assert attend(lib, q_dtype=1) == L.BML_E_UNSUPPORTED      # f16 queries, bf16 pages
     assert attend(lib, q_dtype=2, kv=0) == L.BML_E_UNSUPPORTED
