@@ -97,7 +97,8 @@ __device__ __forceinline__ uint32_t tree_full_weight(const TreeParams &p) { retu
 
 __device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, uint32_t i) {
     TreeSeq s;
-    const int32_t a = p.node_start[i], b = p.node_start[i + 1], L = p.kv_lens[i];
+    // from L2: the merge reads them before its griddepcontrol.wait
+    const int32_t a = __ldcg(p.node_start + i), b = __ldcg(p.node_start + i + 1), L = __ldcg(p.kv_lens + i);
     const bool rows_ok = a >= 0 && b > a && (uint32_t)b <= p.n_tokens;
     s.first = rows_ok ? (uint32_t)a : 0u;
     s.T = rows_ok ? (uint32_t)(b - a) : 0u;
@@ -228,7 +229,7 @@ __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *
             while (true) {
                 const TreeSeq s = tree_seq(p, seq);
                 const uint32_t n = s.groups * upr, t = s.weight * upr * s.tiles;
-                if (by_unit ? w < fu + n : w < ft + t) break;
+                if ((by_unit ? w < fu + n : w < ft + t) || seq + 1 >= i1) break;
                 fu += n;
                 ft += t;
                 ++seq;
@@ -312,7 +313,11 @@ struct TreeWalk {
             uint32_t per_head;
             while (pos - base >= (per_head = s.weight * s.tiles) * (p.n_kv / p.hpu)) {
                 base += per_head * (p.n_kv / p.hpu);
-                s = tree_seq(p, ++seq);
+                if (++seq >= p.n_seqs) {  // only with a node_start that does not ascend
+                    pos = end;
+                    return false;
+                }
+                s = tree_seq(p, seq);
             }
             const uint32_t off = pos - base, wf = tree_full_weight(p);
             const uint32_t head = off / per_head, in_head = off - head * per_head;

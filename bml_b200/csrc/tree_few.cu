@@ -131,6 +131,7 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
     TreeWalk fw(p, range);
     TreeSeg fs = {};
     uint32_t f_left = 0, f_pos = 0, f_stage = 0, f_page = 0;
+    bool live = true;  // no wait has given up: after that nothing is copied any more
     const int32_t *f_table = nullptr;
     auto page_at = [&](uint32_t pos) { return pos < fs.s.L ? (uint32_t)f_table[pos >> p.page_shift] : 0xffffffffu; };
     auto fetch = [&]() {
@@ -141,7 +142,7 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
             f_table = p.table + (size_t)fs.seq * p.max_pages;
             f_page = page_at(f_pos);
         }
-        if (lane == 0) {
+        if (lane == 0 && live) {
             const bool ok = f_page < p.n_pages;
             flags[f_stage] = ok;
             if (f_pos < fs.s.L) {
@@ -191,11 +192,12 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
                     }
                     a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1));
                     a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
-                    const int ea = min(max((int)(__float_as_uint(a) >> 23), 30), 240);
+                    const int ea = min(max((int)(__float_as_uint(a) >> 23), 11), 254);
                     e = __uint_as_float((uint32_t)(254 + 10 - ea) << 23);
                     const float back = __uint_as_float((uint32_t)(ea - 10) << 23);
-                    c0 *= __shfl_sync(0xffffffffu, back, 8 * c);
-                    c1 *= __shfl_sync(0xffffffffu, back, 8 * c + 4);
+                    // never 0 or infinite, as in tree_warp.cu
+                    c0 = fminf(fmaxf(c0 * __shfl_sync(0xffffffffu, back, 8 * c), 1.17549435e-38f), 3.40282347e38f);
+                    c1 = fminf(fmaxf(c1 * __shfl_sync(0xffffffffu, back, 8 * c + 4), 1.17549435e-38f), 3.40282347e38f);
                 }
 #pragma unroll
                 for (int s = 0; s < NJ; ++s)
@@ -226,7 +228,7 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
 
 #pragma unroll 1
         for (uint32_t k = sg.t0; k < sg.t1; ++k) {
-            copy_wait(&full[stage], phase, abort_flag);
+            if (!copy_wait(&full[stage], phase, abort_flag)) live = false;
             __syncwarp();  // and every lane has left the stage that fetch() fills
             fetch();
             const uint32_t base = k * p.tile + split * 16, st = stage;
@@ -349,6 +351,7 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
                     const uint32_t at = base + i;
                     if (at < P || at >= sg.s.L) continue;
                     const uint32_t page = (uint32_t)p.table[(size_t)sg.seq * p.max_pages + (at >> p.page_shift)];
+                    if (page >= p.n_pages) continue;
                     const uint16_t *v = reinterpret_cast<const uint16_t *>(static_cast<const char *>(p.v) +
                                                                            (((size_t)page << p.page_shift) + (at & pmask)) * prow) +
                                         (sg.head + hsub) * D;

@@ -209,6 +209,7 @@ __device__ __noinline__ void add_odd(const TreeParams &p, const volatile Board *
         const uint32_t pos = P + node;
         if (!(odd[node >> 5] >> (node & 31) & 1) || pos < lo || pos >= hi || !tree_sees(p, s, t, node)) continue;
         const uint32_t page = (uint32_t)p.table[(size_t)b->seq * p.max_pages + (pos >> p.page_shift)];
+        if (page >= p.n_pages) continue;
         const size_t at = ((((size_t)page << p.page_shift) + (pos & ((1u << p.page_shift) - 1))) * p.n_kv + b->head) * D;
         const uint16_t *q = static_cast<const uint16_t *>(p.q) + q_at, *k = static_cast<const uint16_t *>(p.k) + at;
         float sc = 0.f;

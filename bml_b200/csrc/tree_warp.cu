@@ -184,11 +184,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
                 a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2));
                 b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, 2));
                 // exponents: 2^(10 - floor(log2 a)), kept where both it and its inverse are normal
-                const int ea = min(max((int)(__float_as_uint(a) >> 23), 30), 240), eb = min(max((int)(__float_as_uint(b) >> 23), 30), 240);
+                const int ea = min(max((int)(__float_as_uint(a) >> 23), 11), 254), eb = min(max((int)(__float_as_uint(b) >> 23), 11), 254);
                 e0 = __uint_as_float((uint32_t)(254 + 10 - ea) << 23);
                 e1 = __uint_as_float((uint32_t)(254 + 10 - eb) << 23);
-                c0 *= __uint_as_float((uint32_t)(ea - 10) << 23);
-                c1 *= __uint_as_float((uint32_t)(eb - 10) << 23);
+                // never 0 or infinite (a masked score is -inf): scores are below 2^11 * 2^16 * D,
+                // so that a scale below the smallest normal number makes all weights 1 either way
+                c0 = fminf(fmaxf(c0 * __uint_as_float((uint32_t)(ea - 10) << 23), 1.17549435e-38f), 3.40282347e38f);
+                c1 = fminf(fmaxf(c1 * __uint_as_float((uint32_t)(eb - 10) << 23), 1.17549435e-38f), 3.40282347e38f);
             }
 #pragma unroll 2
             for (int s = 0; s < D / 16; ++s) {
@@ -371,6 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
                         const uint32_t at = base + i;
                         if (at < P || at >= sg.s.L) continue;
                         const uint32_t page = (uint32_t)p.table[(size_t)sg.seq * p.max_pages + (at >> p.page_shift)];
+                        if (page >= p.n_pages) continue;
                         const uint16_t *v = reinterpret_cast<const uint16_t *>(
                             static_cast<const char *>(p.v) + (((size_t)page << p.page_shift) + (at & pmask)) * prow) + sg.head * D;
 #pragma unroll

@@ -435,12 +435,12 @@ class PagedBatcher:
         try:
             plan = self._planned({rid: n})
             plan.check()
-        except OutOfPages:
-            del self._rows[rid]
+            for layer in range(self.n_layers):
+                paged_append(None, k_prompt[layer].contiguous(), v_prompt[layer].contiguous(), plan.slots, None,
+                             self.k[layer], self.v[layer])
+        except Exception:
+            del self._rows[rid]  # and its pages stay free: owned and used are those before the plan
             raise
-        for layer in range(self.n_layers):
-            paged_append(None, k_prompt[layer].contiguous(), v_prompt[layer].contiguous(), plan.slots, None,
-                         self.k[layer], self.v[layer])
         self.owned, self.used, self.lens = plan.owned, plan.free_used, plan.kv_lens + self._idle(plan)
 
     def _idle(self, plan: PagePlan) -> torch.Tensor:

@@ -375,6 +375,19 @@ def test_scales(cuda, qt, ct, nodes):
         check(c, got, [chain(t, p) for t, p in zip(nodes, lens)], qt, scale=scale)
 
 
+@pytest.mark.parametrize("ct", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("nodes", [[1, 1], [4, 4], [40, 40]])
+@pytest.mark.parametrize("size,scale", [(0.0, 1e-30), (2.0 ** -100, 2.0 ** 97), (2.0 ** 118, 2.0 ** -121)])
+def test_ranges_of_queries(cuda, ct, nodes, size, scale):
+    """32-bit queries of any size, and rows of zeros beside a tiny scale."""
+    import bml_b200
+    lens = [150, 5]
+    c = Paged(lens, nodes, 8, 2, 128, 16, "f32", ct, seed=43)
+    c.q *= size
+    got = bml_b200.tree_attention(c.q, c.k, c.v, c.table, c.kv_lens, c.start, scale=scale)
+    check(c, got, [chain(t, p) for t, p in zip(nodes, lens)], "f32", scale=scale)
+
+
 @pytest.mark.parametrize("qt,ct", TYPES)
 @pytest.mark.parametrize("nodes", [[1, 1, 1], [3, 2, 5], [40, 40, 3]])
 def test_nan_that_is_seen(cuda, qt, ct, nodes):
@@ -757,6 +770,22 @@ def test_batcher_limits(cuda):
     b.begin({1: 40})
     b.commit()
     assert b.length(1) == 42
+
+
+def test_batcher_prompt_that_fails(cuda):
+    """A prompt that cannot be stored leaves no request and takes no pages."""
+    import bml_b200
+    b = bml_b200.PagedBatcher(1, 4, 2, 64, n_pages=3, page_size=16, max_positions=64, max_requests=2)
+    x = torch.zeros(1, 20, 2, 64, device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(TypeError):
+        b.add("a", x.double(), x.double())
+    with pytest.raises(ValueError):
+        b.add("a", x.cpu(), x.cpu())
+    with pytest.raises(bml_b200.OutOfPages):
+        b.add("a", x.repeat(1, 3, 1, 1), x.repeat(1, 3, 1, 1))
+    assert len(b) == 0 and int(b.used) == 0
+    b.add("a", x, x)
+    assert b.length("a") == 20 and int(b.used) == 2
 
 
 # ---------------------------------------------------------------------------
