@@ -27,14 +27,6 @@ constexpr int kThreads = 256;
 constexpr float kGrow = 8.0f;  // log2 units a row's maximum may grow before O is rescaled
 constexpr int kWarps = kThreads / 32;
 
-// hi: x rounded to TF32's 10 fraction bits, half away from zero, with integer
-// operations (a conversion instruction runs at a quarter of their rate and set
-// the time: 4 requests of 618 to 2671 positions 85 -> 75 us).  lo: the rest, of
-// which the matrix unit takes the upper bits itself.
-__device__ __forceinline__ void tf32_split(float x, uint32_t &hi, uint32_t &lo) {
-    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
-    lo = __float_as_uint(x - __uint_as_float(hi));
-}
 __device__ __forceinline__ void mma_tf32(float *d, const uint32_t *a, uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -112,7 +104,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const TreeRange range = tree_range(p, &sh, blockIdx.x, gridDim.x);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge, which waits for this grid
-    TreeWalk walk(p, range);
+    TreeWalk walk(range);
     TreeSeg sg;
     while (walk.next(p, sg)) {
         // Q fragments, split: [row warp][k-step][hi | lo][lane][4]
@@ -461,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_merge_kernel(const __grid_co
         const TreeRange range = tree_range(p, &sh, b, grid);
         mine = range.w0 < range.w1;
         if (mine) {
-            TreeWalk walk(p, range);
+            TreeWalk walk(range);
             mine = walk.next(p, sg) && sg.t0 > 0;  // else the cut lies between two units
             total = range.total;
             u0 = sg.u0;
@@ -494,8 +486,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_merge_kernel(const __grid_co
         float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
         if (valid) {
             const uint32_t first = b - 1 + (many ? warp : 0);
-            const size_t slot = (size_t)R * (D + 2);
-            auto seg_part = [&](uint32_t s) { return p.part + (2 * (size_t)s + (s == b - 1 ? 1 : 0)) * slot; };
+            auto seg_part = [&](uint32_t s) { return tree_part(p, D, s, s == b - 1 ? 1u : 0u); };
             // Batches of explicit loads: a loop over segments is not unrolled so
             // that its loads overlap.  The running maximum is kept per batch.
             for (uint32_t s0 = first; s0 <= last; s0 += kBatch * step) {
@@ -590,7 +581,7 @@ cudaError_t launch_f32(TreeParams p, int num_sms, cudaStream_t st) {
     p.tile = C::TILE;
     p.heavy_rows = 0xffffffffu;
     p.heavy = p.light = 1;
-    if (!tree_line_fits(p)) return cudaErrorNotSupported;
+    if (!tree_line(p)) return cudaErrorNotSupported;
     e = launch_after(kern, dim3(num_sms), kThreads, C::SMEM, st, p);
     if (e != cudaSuccess) return e;
     return launch_tree_merge(p, D, num_sms, st);
@@ -649,6 +640,7 @@ cudaError_t launch_tree(const TreeArgs &a, cudaStream_t st) {
         if (a.p.q_type == BML_F32 || !tree_umma_fits(a) || (small && a.rows <= 64)) return launch_tree_warp(a, st);
         return launch_tree_umma(a, st);
     }
+    if (a.kv_type == BML_F32 && a.p.scale_log2 > 0.f && a.rows > 16 && a.p.group <= 128) return launch_tree_umma32(a, st);
     return a.D == 128 ? launch_kv<128>(a, st) : launch_kv<64>(a, st);
 }
 

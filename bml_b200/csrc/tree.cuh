@@ -26,7 +26,8 @@ struct TreeParams {
     float *part;
     uint32_t rpg;        // rows of a row group
     uint32_t hpu;        // kv heads of a unit
-    uint32_t tile;       // positions of a schedule tile
+    uint32_t tile;       // positions of a schedule tile, a power of two
+    uint32_t tile_shift, upr;  // log2(tile); units of a row group: n_kv / hpu (tree_line)
     // a tile's weight: heavy with more rows than heavy_rows, else light
     uint32_t heavy_rows, heavy, light;
 };
@@ -63,13 +64,17 @@ bool tree_umma_fits(const TreeArgs &a);
 cudaError_t launch_tree_warp(const TreeArgs &a, cudaStream_t st);
 cudaError_t launch_tree_few(const TreeArgs &a, cudaStream_t st);
 cudaError_t launch_tree_umma(const TreeArgs &a, cudaStream_t st);
+cudaError_t launch_tree_umma32(const TreeArgs &a, cudaStream_t st);
 
-// Whether the schedule can count the launch's tiles in 32 bits, whatever the
-// lengths on the device are.
+// Sets what follows from the other fields, and says whether the schedule can
+// count the launch's tiles in 32 bits, whatever the lengths on the device are.
 inline uint64_t tree_most_units(const TreeParams &p) {
-    return ((uint64_t)p.n_tokens * p.group / p.rpg + p.n_seqs) * (p.n_kv / p.hpu);
+    return ((uint64_t)p.n_tokens * p.group / p.rpg + p.n_seqs) * p.upr;
 }
-inline bool tree_line_fits(const TreeParams &p) {
+inline bool tree_line(TreeParams &p) {
+    p.tile_shift = 0;
+    while (1u << p.tile_shift < p.tile) ++p.tile_shift;
+    p.upr = p.n_kv / p.hpu;
     const uint64_t tiles = (((uint64_t)p.max_pages << p.page_shift) + p.tile - 1) / p.tile;
     return tree_most_units(p) * p.heavy <= 0xffffffffull / tiles;
 }
@@ -95,10 +100,17 @@ struct TreeSeq {
 // A tile's weight in a full row group.
 __device__ __forceinline__ uint32_t tree_full_weight(const TreeParams &p) { return p.rpg > p.heavy_rows ? p.heavy : p.light; }
 
-__device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, uint32_t i) {
-    TreeSeq s;
+// What the device holds of a request: rows [a, b), positions.
+struct TreeRaw {
+    int32_t a, b, L;
+};
+__device__ __forceinline__ TreeRaw tree_raw(const TreeParams &p, uint32_t i) {
     // from L2: the merge reads them before its griddepcontrol.wait
-    const int32_t a = __ldcg(p.node_start + i), b = __ldcg(p.node_start + i + 1), L = __ldcg(p.kv_lens + i);
+    return {__ldcg(p.node_start + i), __ldcg(p.node_start + i + 1), __ldcg(p.kv_lens + i)};
+}
+__device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, const TreeRaw &raw) {
+    TreeSeq s;
+    const int32_t a = raw.a, b = raw.b, L = raw.L;
     const bool rows_ok = a >= 0 && b > a && (uint32_t)b <= p.n_tokens;
     s.first = rows_ok ? (uint32_t)a : 0u;
     s.T = rows_ok ? (uint32_t)(b - a) : 0u;
@@ -107,11 +119,13 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, uint32_t i) {
     s.L = ok ? (uint32_t)L : 0u;
     s.rows = s.T * p.group;
     s.groups = (s.rows + p.rpg - 1) / p.rpg;
-    s.tiles = s.L ? (s.L + p.tile - 1) / p.tile : 1u;
+    s.tiles = s.L ? (s.L + p.tile - 1) >> p.tile_shift : 1u;
     s.w_last = s.rows - (s.groups - 1) * p.rpg > p.heavy_rows ? p.heavy : p.light;
     s.weight = s.groups ? (s.groups - 1) * tree_full_weight(p) + s.w_last : 0u;
     return s;
 }
+
+__device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, uint32_t i) { return tree_seq(p, tree_raw(p, i)); }
 
 struct TreeShared {
     uint32_t warp_sums[32], warp_units[32];
@@ -126,7 +140,7 @@ struct TreeShared {
 struct TreeCuts {
     uint32_t each, more, active;
     __device__ __forceinline__ TreeCuts(const TreeParams &p, uint32_t total, uint32_t grid) {
-        const uint32_t most = total / p.heavy;
+        const uint32_t most = p.heavy == 1 ? total : total / p.heavy;
         active = most < 1 ? (total ? 1u : 0u) : most < grid ? most : grid;
         each = active ? total / active : 0u;
         more = total - each * active;
@@ -143,6 +157,7 @@ struct TreeCuts {
 struct TreeRange {
     uint32_t w0, w1, base, total;
     uint32_t seq;
+    TreeSeq s;  // of seq
 };
 
 // The request that holds tile w (by_unit: unit w) of the line.  Up to 128
@@ -151,22 +166,25 @@ struct TreeRange {
 struct TreePlace {
     uint32_t total, units;  // of the line
     uint32_t seq, base, unit0;  // the request, its first tile, its first unit
+    TreeSeq s;
 };
 
 template <typename Target>
 __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *sh, bool by_unit, Target target) {
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, upr = p.n_kv / p.hpu;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, upr = p.upr;
     const bool alone = p.n_seqs <= 128;
     const uint32_t members = alone ? 32u : blockDim.x, me = alone ? lane : threadIdx.x;
     const uint32_t per = (p.n_seqs + members - 1) / members;
     const uint32_t i0 = min(me * per, p.n_seqs), i1 = min(i0 + per, p.n_seqs);
     uint32_t tiles = 0, units = 0;
     uint32_t n4[4] = {0, 0, 0, 0}, t4[4] = {0, 0, 0, 0};  // alone: units and tiles of the lane's requests
+    TreeRaw raw[4] = {};
     if (alone) {
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k)
             if (i0 + k < i1) {
-                const TreeSeq s = tree_seq(p, i0 + k);
+                raw[k] = tree_raw(p, i0 + k);
+                const TreeSeq s = tree_seq(p, raw[k]);
                 n4[k] = s.groups * upr;
                 t4[k] = s.weight * upr * s.tiles;
                 units += n4[k];
@@ -218,12 +236,15 @@ __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *
             if (mine && seq == i0 + k && (by_unit ? w >= fu + n4[k] : w >= ft + t4[k])) {
                 fu += n4[k];
                 ft += t4[k];
+                raw[0] = raw[k + 1];  // of seq
                 ++seq;
             }
         const uint32_t who = __ffs(__ballot_sync(0xffffffffu, mine)) - 1;  // none: lane 31's, unused
         r.seq = __shfl_sync(0xffffffffu, seq, who & 31);
         r.base = __shfl_sync(0xffffffffu, ft, who & 31);
         r.unit0 = __shfl_sync(0xffffffffu, fu, who & 31);
+        r.s = tree_seq(p, TreeRaw{__shfl_sync(0xffffffffu, raw[0].a, who & 31), __shfl_sync(0xffffffffu, raw[0].b, who & 31),
+                                  __shfl_sync(0xffffffffu, raw[0].L, who & 31)});
     } else {
         if (mine) {
             while (true) {
@@ -242,6 +263,7 @@ __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *
         r.seq = sh->seq;
         r.base = sh->base;
         r.unit0 = sh->unit;
+        if (r.seq < p.n_seqs) r.s = tree_seq(p, r.seq);
     }
     return r;
 }
@@ -261,6 +283,7 @@ __device__ __forceinline__ TreeRange tree_range(const TreeParams &p, TreeShared 
     r.total = at.total;
     r.base = at.base;
     r.seq = at.seq;
+    r.s = at.s;
     return r;
 }
 
@@ -280,7 +303,7 @@ __device__ __forceinline__ TreeUnit tree_unit(const TreeParams &p, TreeShared *s
     r.total = at.total;
     if (r.found) {
         r.seq = at.seq;
-        r.s = tree_seq(p, r.seq);
+        r.s = at.s;
         const uint32_t in = u - at.unit0;
         r.head = in / r.s.groups;
         r.rg = in - r.head * r.s.groups;
@@ -305,14 +328,12 @@ struct TreeWalk {
     uint32_t pos, end, base;
     uint32_t seq;
     TreeSeq s;
-    __device__ __forceinline__ TreeWalk(const TreeParams &p, const TreeRange &r) : pos(r.w0), end(r.w1), base(r.base), seq(r.seq) {
-        if (pos < end) s = tree_seq(p, seq);
-    }
+    __device__ __forceinline__ explicit TreeWalk(const TreeRange &r) : pos(r.w0), end(r.w1), base(r.base), seq(r.seq), s(r.s) {}
     __device__ __forceinline__ bool next(const TreeParams &p, TreeSeg &g) {
         while (pos < end) {
             uint32_t per_head;
-            while (pos - base >= (per_head = s.weight * s.tiles) * (p.n_kv / p.hpu)) {
-                base += per_head * (p.n_kv / p.hpu);
+            while (pos - base >= (per_head = s.weight * s.tiles) * p.upr) {
+                base += per_head * p.upr;
                 if (++seq >= p.n_seqs) {  // only with a node_start that does not ascend
                     pos = end;
                     return false;
@@ -342,9 +363,12 @@ struct TreeWalk {
     }
 };
 
+// Floats of a partial slot, a multiple of 4: slots start on 16 bytes also where
+// the rows are odd in number (125 of them for groups of 5).
+__device__ __forceinline__ size_t tree_slot(const TreeParams &p, uint32_t D) { return ((size_t)p.rpg * p.hpu * (D + 2) + 3) & ~(size_t)3; }
 // Partial slot `which` (0 or 1) of CTA b.
 __device__ __forceinline__ float *tree_part(const TreeParams &p, uint32_t D, uint32_t b, uint32_t which) {
-    return p.part + (size_t)(2 * b + which) * p.rpg * p.hpu * (D + 2);
+    return p.part + (2 * (size_t)b + which) * tree_slot(p, D);
 }
 
 // Element index of row r (t * group + g) of the unit's kv head `h` in q and out.
@@ -379,6 +403,14 @@ __device__ __forceinline__ uint32_t tree_see16(const TreeParams &p, const TreeSe
     return n0 < 0 ? (uint32_t)(w << -n0) | ((1u << -n0) - 1) : (uint32_t)w;
 }
 
+// hi: x rounded to TF32's 10 fraction bits, half away from zero, with integer
+// operations (a conversion instruction runs at a quarter of their rate and set
+// the time: 4 requests of 618 to 2671 positions 85 -> 75 us).  lo: the rest, of
+// which the matrix unit takes the upper bits itself.
+__device__ __forceinline__ void tf32_split(float x, uint32_t &hi, uint32_t &lo) {
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi));
+}
 // 16 bytes global -> shared; bytes = 0 writes zeros and reads nothing.
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");

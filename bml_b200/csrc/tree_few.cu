@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     // ------------------------------------------------------------ copies, ahead
-    TreeWalk fw(p, range);
+    TreeWalk fw(range);
     TreeSeg fs = {};
     uint32_t f_left = 0, f_pos = 0, f_stage = 0, f_page = 0;
     bool live = true;  // no wait has given up: after that nothing is copied any more
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
         f_stage = f_stage + 1 == (uint32_t)C::NST ? 0 : f_stage + 1;
     };
     auto weight = [](float x) { return kQ32 ? exp2f(x) : fast_exp2(x); };
-    TreeWalk walk(p, range);
+    TreeWalk walk(range);
     TreeSeg sg = {};
     uint32_t stage = 0, phase = 0;
     bool first = true;
@@ -471,7 +471,7 @@ cudaError_t launch_n(const TreeArgs &a, cudaStream_t st) {
     fp.t.tile = 16 * fp.splits;
     fp.t.heavy_rows = 0xffffffffu;
     fp.t.heavy = fp.t.light = 1;
-    if (!tree_line_fits(fp.t)) return cudaErrorNotSupported;
+    if (!tree_line(fp.t)) return cudaErrorNotSupported;
     const uint64_t rows = (uint64_t)a.p.n_pages << a.p.page_shift;
     if (!few_map(&fp.tk, a.p.k, kF16, D, a.p.n_kv, rows) || !few_map(&fp.tv, a.p.v, kF16, D, a.p.n_kv, rows))
         return cudaErrorInvalidValue;

@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
     tc_fence_after();
     const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may take its place; it waits for this grid
-    TreeWalk walk(p, range);
+    TreeWalk walk(range);
     TreeSeg sg = {};
 
     if (warp == 0 || warp == 10) {
@@ -851,7 +851,7 @@ cudaError_t launch_tree_umma(const TreeArgs &a, cudaStream_t st) {
     up.t.heavy_rows = up.rt;
     up.t.heavy = 5;
     up.t.light = 3;
-    if (!tree_line_fits(up.t)) return cudaErrorNotSupported;
+    if (!tree_line(up.t)) return cudaErrorNotSupported;
     const uint64_t rows = (uint64_t)a.p.n_pages << a.p.page_shift;
     if (!tree_map(&up.tq, a.p.q, f16, a.D, a.p.n_heads, a.p.n_tokens, group, BM / group) ||
         !tree_map(&up.tk, a.p.k, f16, a.D, a.p.n_kv, rows, 1, up.box_rows) ||

@@ -1,0 +1,613 @@
+// tree_umma32.cu -- attention of drafted tokens over a paged cache of 32-bit
+// values on tcgen05 tensor cores (sm_100a): results to about f32 precision
+// from TF32 products.
+//
+// The mathematics and the schedule are those of tree.cu / tree.cuh: a CTA (one
+// per SM) works through its even share of the line of 64-position tiles,
+// segment by segment.  A unit is one request, kv head and group of up to RT
+// query rows, RT = the most whole tokens' rows that fit 128; row r of it is
+// (node r / group, q head r % group) and TMEM lane r.
+//
+// Every f32 operand x is hi + lo with hi = x rounded to TF32 and lo = x - hi,
+// of which the tensor core takes the upper bits (22 together), and a product is
+// hi*hi + (lo*hi + hi*lo).  The tensor core's sums truncate, so S's two parts
+// are summed apart, and a tile's O (its small terms first) is added to the
+// output in registers, with a rounding, and not summed on from tile to tile in
+// tensor memory.
+//
+//   Q hi, lo     tensor memory (D columns each), written once a segment;
+//   K hi, lo     shared memory, K-major as it arrives; hi replaces K, lo is the
+//                next 64 rows of the MMA's B operand;
+//   P hi, lo     tensor memory, hi over S;
+//   V hi, lo     shared memory, transposed on the way (positions are the MMA's
+//                K index).
+//
+//   warp 0       copies K and V tiles (cp.async.bulk.tensor; K two stages)
+//   warp 1       tensor memory, and every tcgen05.mma
+//   warps 2-5    Q, and the softmax: thread = row = TMEM lane
+//   warps 6-13   split K and V; add the tiles' O (a warp: 32 rows, half of the
+//                columns) and write the rows.
+//
+// V is split while S is computed, and the next tile's K after it.
+//
+// What a row does not see must not reach it: scores are replaced by -inf (bad
+// pages, rows past the length, nodes outside the mask), V rows past the length
+// and values of drafted nodes that are not finite are split as zeros, and the
+// latter are added at the end for the rows that see them.
+#include <math.h>
+
+#include "tree.cuh"
+#include "umma.cuh"
+
+namespace bml {
+
+namespace {
+
+constexpr int BM = 128, BN = 64;
+constexpr int kThreads = 448;
+constexpr int kSplitWarps = 8;
+constexpr int kBadRing = 16;  // tiles whose page flags are kept
+
+template <int D>
+struct XCfg {
+    static constexpr int KB = D / 32;          // 128-byte column blocks of a K row
+    static constexpr int TILE = BN * D * 4;    // a K or V tile
+    static constexpr int OFF_K = 0;            // two stages: per column block 64 rows hi (in place), 64 rows lo
+    static constexpr int OFF_V = 4 * TILE;
+    static constexpr int OFF_VHI = 5 * TILE;   // [2 blocks of 32 positions][D][128 B]
+    static constexpr int OFF_VLO = 6 * TILE;
+    static constexpr int OFF_SH = 7 * TILE;
+    static constexpr int SMEM = OFF_SH + 3 * 1024;
+    // tensor memory columns
+    static constexpr uint32_t QHI = 0, QLO = D, OC = 2 * D;
+    static constexpr uint32_t SC = 3 * D, PLO = SC + BN;  // S: Q hi * K hi, and the other two products; then P
+    static constexpr uint32_t TMEM_COLS = 512;
+};
+static_assert(XCfg<128>::SMEM <= 227 * 1024 && XCfg<128>::PLO + BN == 512, "shared and tensor memory");
+
+struct XParams {
+    CUtensorMap tk, tv;  // (d, n_kv, rows); box (32, 1, box_rows) swizzled, (d, 1, box_rows) plain
+    TreeParams t;
+    uint32_t box_rows;  // min(page, 64)
+};
+
+struct alignas(16) XShared {
+    uint64_t k_full[2], k_empty[2], k_ready[2];
+    uint64_t v_full, v_empty, q_ready, v_ready, s_full, p_ready, o_full, o_free, drain;
+    uint32_t tmem, abort;
+    uint32_t bad[kBadRing];  // per tile: 16-position blocks on pages outside the pool
+    uint32_t odd[3][8];      // per segment: drafted nodes with a V value that is not finite
+    float alpha[2][BM];      // per tile: what the rows' output is scaled by before it is added
+    float2 ml[BM];           // the segment's rows' (m, l)
+    TreeShared sched;
+};
+static_assert(sizeof(XShared) <= 3 * 1024, "small arrays");
+
+// Bounded wait that looks at the clock once in 256 tries.
+__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag) {
+    if (mbar_test_wait(bar, parity)) return true;
+    uint64_t t0 = 0;
+    while (true) {
+#pragma unroll 1
+        for (int i = 0; i < 256; ++i)
+            if (mbar_try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+        const uint64_t t = globaltimer_ns();
+        if (t0 == 0) t0 = t;
+        if (t - t0 > kWaitNs) {
+            *abort_flag = 1u;
+            return false;
+        }
+    }
+}
+
+// D[tmem] (+)= A[tmem] * B[smem desc], TF32: A is M x 8, 8 columns.
+__device__ __forceinline__ void mma_tf32_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// 32 values as hi and lo, to tensor memory.
+__device__ __forceinline__ void put_split(uint32_t hi_at, uint32_t lo_at, const float *x) {
+#pragma unroll
+    for (int c = 0; c < 32; c += 16) {
+        uint32_t hi[16], lo[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) tf32_split(x[c + k], hi[k], lo[k]);
+        tmem_st16(hi_at + c, hi);
+        tmem_st16(lo_at + c, lo);
+    }
+}
+
+// Which of the 64 positions from node0 on (negative: committed ones, seen by
+// all) node t sees.
+__device__ __forceinline__ uint64_t see_tile(const TreeParams &p, const TreeSeq &s, uint32_t t, int32_t node0) {
+    if (s.L == 0) return 0ull;
+    uint64_t see = 0;
+#pragma unroll 1
+    for (int b = 0; b < 4; ++b) {
+        const int32_t n0 = node0 + 16 * b;
+        see |= (uint64_t)(n0 <= -16 ? 0xffffu : tree_see16(p, s, t, n0) & 0xffffu) << (16 * b);
+    }
+    return see;
+}
+
+// Adds to o (32 columns from `col` on of a row of node t, relative to maximum m)
+// the values of drafted nodes that are not finite, where the row sees them.
+// Rare: everything is recomputed from global memory.
+template <int D>
+__device__ __noinline__ void add_odd(const TreeParams &p, const TreeSeg &sg, const uint32_t *odd, uint32_t t, size_t q_at,
+                                     uint32_t col, float m, float *o) {
+    const uint32_t lo = sg.t0 * BN, hi = sg.t1 * BN, P = sg.s.L - min(sg.s.T, sg.s.L);
+    for (uint32_t node = 0; node < sg.s.T; ++node) {
+        const uint32_t pos = P + node;
+        if (!(odd[node >> 5] >> (node & 31) & 1) || pos < lo || pos >= hi || !tree_sees(p, sg.s, t, node)) continue;
+        const uint32_t page = (uint32_t)p.table[(size_t)sg.seq * p.max_pages + (pos >> p.page_shift)];
+        if (page >= p.n_pages) continue;
+        const size_t at = ((((size_t)page << p.page_shift) + (pos & ((1u << p.page_shift) - 1))) * p.n_kv + sg.head) * D;
+        const float *q = static_cast<const float *>(p.q) + q_at, *k = static_cast<const float *>(p.k) + at;
+        float sc = 0.f;
+        for (int i = 0; i < D; ++i) sc = fmaf(q[i], k[i], sc);
+        const float w = exp2f(sc * p.scale_log2 - m);
+        for (int u = 0; u < 32; ++u) {
+            const float v = static_cast<const float *>(p.v)[at + col + u];
+            if (!(fabsf(v) < INFINITY) && !(w <= 0.f)) o[u] = fmaf(w, v, o[u]);
+        }
+    }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_constant__ XParams xp) {
+    using C = XCfg<D>;
+    const TreeParams &p = xp.t;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    XShared &sh = *reinterpret_cast<XShared *>(smem + C::OFF_SH);
+    volatile uint32_t *abort_flag = &sh.abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.k_full[i], 1);
+            mbar_init(&sh.k_empty[i], 1);
+            mbar_init(&sh.k_ready[i], kSplitWarps);
+        }
+        mbar_init(&sh.v_full, 1);
+        mbar_init(&sh.v_empty, kSplitWarps);
+        mbar_init(&sh.q_ready, 4);
+        mbar_init(&sh.v_ready, kSplitWarps);
+        mbar_init(&sh.s_full, 1);
+        mbar_init(&sh.p_ready, 4);
+        mbar_init(&sh.o_full, 1);
+        mbar_init(&sh.o_free, kSplitWarps);
+        mbar_init(&sh.drain, 1);
+        sh.abort = 0u;
+        fence_mbar_init();
+    }
+    if (threadIdx.x < 24) sh.odd[threadIdx.x / 8][threadIdx.x % 8] = 0u;
+    if (warp == 0 && lane == 0) {
+        prefetch_tmap(&xp.tk);
+        prefetch_tmap(&xp.tv);
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
+                     "r"(C::TMEM_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const TreeRange range = tree_range(p, &sh.sched, blockIdx.x, gridDim.x);
+    __syncthreads();  // the set-up above
+    tc_fence_after();
+    const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge, which waits for this grid
+    TreeWalk walk(range);
+    TreeSeg sg = {};
+    uint32_t it = 0, segs = 0;  // tiles, segments so far
+
+    if (warp == 0) {
+        // --------------------------------------------------------------- producer
+        // Lanes 0-15 issue K's boxes (column block lane % KB of part lane / KB),
+        // lanes 16-19 V's (part lane - 16).
+        const uint64_t policy = l2_policy_evict_first();
+        const uint32_t parts = BN / xp.box_rows, ps_mask = (1u << p.page_shift) - 1;
+        const bool is_k = lane < 16;
+        const uint32_t part = is_k ? lane / C::KB : lane - 16, kb = is_k ? lane % C::KB : 0u;
+        const bool mine = part < parts && lane < 20;
+        bool live = true;
+        while (live && walk.next(p, sg)) {
+            const int32_t *table = p.table + (size_t)sg.seq * p.max_pages;
+            // a lane's first row in the pool of tile j (-1: past the length, -2: a page outside the pool)
+            auto row_of = [&](uint32_t j) -> int {
+                const uint32_t pos = j * BN + part * xp.box_rows;
+                if (!mine || pos >= sg.s.L) return -1;
+                const uint32_t page = (uint32_t)table[pos >> p.page_shift];
+                return page < p.n_pages ? (int)((page << p.page_shift) + (pos & ps_mask)) : -2;
+            };
+            int next = row_of(sg.t0);
+            for (uint32_t j = sg.t0; j < sg.t1; ++j, ++it) {
+                const int row = next;
+                if (j + 1 < sg.t1) next = row_of(j + 1);
+                const uint32_t st = it & 1u, use = it >> 1;
+                const uint32_t bits = xp.box_rows / 16;
+                uint32_t flag = 0;
+                if (__any_sync(0xffffffffu, row == -2))
+                    flag = __reduce_or_sync(0xffffffffu, row == -2 ? ((1u << bits) - 1) << (part * bits) : 0u);
+                if (lane == 0) *(volatile uint32_t *)&sh.bad[it % kBadRing] = flag;
+                // a page outside the pool is read past the map's end: zeros
+                const int at = row == -2 ? (int)(p.n_pages << p.page_shift) : row;
+                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, row != -1 && !is_k)) * xp.box_rows * D * 4;
+                const bool once = sg.s.groups == 1;  // K and V are read once
+                auto copy = [&](bool k, uint64_t *full, uint8_t *dst) {
+                    if (lane == 0) mbar_arrive_expect_tx(full, bytes);
+                    __syncwarp();
+                    if (row != -1 && is_k == k) {
+                        if (once) tma_load_3d_hint(dst, k ? &xp.tk : &xp.tv, (int)kb * 32, (int)sg.head, at, full, policy);
+                        else tma_load_3d(dst, k ? &xp.tk : &xp.tv, (int)kb * 32, (int)sg.head, at, full);
+                    }
+                    __syncwarp();
+                };
+                if (use > 0) live = __all_sync(0xffffffffu, wait_bar(&sh.k_empty[st], (use & 1u) ^ 1u, abort_flag));
+                if (!live) break;
+                copy(true, &sh.k_full[st], smem + C::OFF_K + st * 2 * C::TILE + kb * 2 * BN * 128 + part * xp.box_rows * 128);
+                if (it > 0) live = __all_sync(0xffffffffu, wait_bar(&sh.v_empty, (it & 1u) ^ 1u, abort_flag));
+                if (!live) break;
+                copy(false, &sh.v_full, smem + C::OFF_V + part * xp.box_rows * D * 4);
+            }
+        }
+        // No copy may outlive the CTA: all have landed unless a wait gave up,
+        // and then none is issued any more, so those that have not will soon.
+        if (!live) {
+            const uint64_t t0 = globaltimer_ns();
+            while (globaltimer_ns() - t0 < 1000000ull) {}
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------------------- MMA issuer
+        // 2: TF32.  Q hi meets K hi and lo in one MMA of 128 columns (an MMA of 64
+        // takes as long), Q lo only K hi.
+        constexpr uint32_t idesc_qk = make_idesc(2u, BM, 2 * BN, 0), idesc_lo = make_idesc(2u, BM, BN, 0), idesc_pv = make_idesc(2u, BM, D, 0);
+        const uint64_t d_k = smem_desc(smem_u32(smem + C::OFF_K), 16, 1024);
+        const uint64_t d_vhi = smem_desc(smem_u32(smem + C::OFF_VHI), 16, 1024), d_vlo = smem_desc(smem_u32(smem + C::OFF_VLO), 16, 1024);
+        bool live = true;
+        auto wait_all = [&](uint64_t *bar, uint32_t parity) {
+            live = live && __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag));
+            __syncwarp();
+            tc_fence_after();
+        };
+        // one term's chain over kK columns of A
+        auto chain = [&](uint32_t d, uint32_t a, uint64_t b, uint32_t block, uint32_t idesc, int n, bool first) {
+            for (int kk = 0; kk < n; ++kk) {
+                const uint32_t off = ((kk >> 2) * block + (kk & 3) * 32) >> 4;
+                if (elect_one()) mma_tf32_ts(d, a + kk * 8, b + off, idesc, first && kk == 0 ? 0u : 1u);
+                __syncwarp();
+            }
+        };
+        while (live && walk.next(p, sg)) {
+            wait_all(&sh.q_ready, segs & 1u);
+            for (uint32_t j = sg.t0; j < sg.t1 && live; ++j, ++it) {
+                const uint32_t st = it & 1u, par = it & 1u;
+                wait_all(&sh.k_ready[st], (it >> 1) & 1u);
+                if (!live) break;
+                const uint64_t k = d_k + ((st * 2 * C::TILE) >> 4);
+                chain(tmem + C::SC, tmem + C::QHI, k, 2 * BN * 128, idesc_qk, D / 8, true);
+                chain(tmem + C::PLO, tmem + C::QLO, k, 2 * BN * 128, idesc_lo, D / 8, false);
+                if (elect_one()) {
+                    tc_commit(&sh.s_full);
+                    tc_commit(&sh.k_empty[st]);
+                }
+                __syncwarp();
+                wait_all(&sh.v_ready, par);
+                if (it > 0) wait_all(&sh.o_free, par ^ 1u);
+                wait_all(&sh.p_ready, par);
+                if (!live) break;
+                chain(tmem + C::OC, tmem + C::PLO, d_vhi, D * 128, idesc_pv, BN / 8, true);
+                chain(tmem + C::OC, tmem + C::SC, d_vlo, D * 128, idesc_pv, BN / 8, false);
+                chain(tmem + C::OC, tmem + C::SC, d_vhi, D * 128, idesc_pv, BN / 8, false);
+                if (elect_one()) tc_commit(&sh.o_full);
+                __syncwarp();
+            }
+            ++segs;
+        }
+        if (elect_one()) tc_commit(&sh.drain);  // no MMA outlives the CTA
+        __syncwarp();
+        mbar_drain(&sh.drain, 0, kWaitNs);
+        __syncwarp();
+    } else if (warp < 6) {
+        // ---------------------------------------------------------- Q and softmax
+        const uint32_t q4 = warp & 3, r = q4 * 32 + lane, lane_addr = (q4 * 32) << 16;
+        const uint32_t at = tmem + lane_addr;
+        while (walk.next(p, sg)) {
+            const bool valid = r < sg.rows;
+            const bool warp_live = q4 * 32 < sg.rows;
+            const uint32_t P = sg.s.L - min(sg.s.T, sg.s.L), t = min((sg.row0 + r) / p.group, sg.s.T - 1);
+            if (warp_live) {
+                const float *q = static_cast<const float *>(p.q) + (valid ? tree_row(p, sg, sg.row0 + r, D) : 0);
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    float x[32];
+#pragma unroll
+                    for (int u = 0; u < 8; ++u) {
+                        const float4 y = valid ? *reinterpret_cast<const float4 *>(q + c + 4 * u) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        x[4 * u] = y.x;
+                        x[4 * u + 1] = y.y;
+                        x[4 * u + 2] = y.z;
+                        x[4 * u + 3] = y.w;
+                    }
+                    __syncwarp();
+                    put_split(at + C::QHI + c, at + C::QLO + c, x);
+                }
+                tmem_wait_st();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.q_ready);
+            float m = -INFINITY, l = 0.f;
+            for (uint32_t j = sg.t0; j < sg.t1; ++j, ++it) {
+                wait_bar(&sh.s_full, it & 1u, abort_flag);
+                __syncwarp();
+                tc_fence_after();
+                if (warp_live) {
+                    const uint32_t bad = *(volatile uint32_t *)&sh.bad[it % kBadRing], kv0 = j * BN;
+                    const bool edge = kv0 + BN > P;
+                    uint64_t see = ~0ull;
+                    if (edge || bad) {
+                        if (edge) see = see_tile(p, sg.s, t, (int32_t)(kv0 - P));
+#pragma unroll
+                        for (int b = 0; b < 4; ++b)
+                            if (bad >> b & 1) see &= ~(0xffffull << (16 * b));
+                    }
+                    float s[BN];
+                    tmem_ld32(at + C::SC, s);
+                    tmem_ld32(at + C::SC + 32, s + 32);
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        float y[16];
+                        tmem_ld16(at + C::PLO + 16 * h, y);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) s[16 * h + k] += y[k];
+                    }
+                    if (edge || bad) {
+                        const uint32_t w[2] = {(uint32_t)see, (uint32_t)(see >> 32)};
+#pragma unroll
+                        for (int k = 0; k < BN; ++k)
+                            if (!(w[k >> 5] >> (k & 31) & 1)) s[k] = -INFINITY;
+                    }
+                    float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                    for (int k = 4; k < BN; ++k) mx[k & 3] = fmaxf(mx[k & 3], s[k]);
+                    const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2);  // > 0
+                    const float mu = m_new == -INFINITY ? 0.f : m_new, alpha = fast_exp2(m - mu);
+                    m = m_new;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            s[32 * h + k] = fast_exp2(fmaf(s[32 * h + k], p.scale_log2, -mu));
+                            sum[k & 3] += s[32 * h + k];
+                        }
+                        put_split(at + C::SC + 32 * h, at + C::PLO + 32 * h, s + 32 * h);
+                    }
+                    l = fmaf(l, alpha, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+                    sh.alpha[it & 1u][r] = alpha;
+                    tmem_wait_st();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.p_ready);
+            }
+            wait_bar(&sh.v_ready, (it - 1) & 1u, abort_flag);  // the split warps have read the last segment's
+            sh.ml[r] = make_float2(m, l);
+            __syncwarp();
+            named_bar_sync(1, 384);
+            ++segs;
+        }
+    } else {
+        // ------------------------------------- K and V split, O added, rows written
+        const uint32_t cw = warp - 6, half = cw >> 2, q4 = warp & 3, r = q4 * 32 + lane, tid = cw * 32 + lane;
+        const uint32_t o_at = tmem + ((q4 * 32) << 16) + C::OC + half * (D / 2);
+        uint32_t total = 0;  // tiles of this CTA
+        {
+            TreeWalk w(range);
+            TreeSeg g;
+            while (w.next(p, g)) total += g.t1 - g.t0;
+        }
+        auto arrive = [&](uint64_t *bar) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
+        auto split_k = [&](uint32_t i) {
+            wait_bar(&sh.k_full[i & 1u], (i >> 1) & 1u, abort_flag);
+            __syncwarp();
+            uint4 *hi = reinterpret_cast<uint4 *>(smem + C::OFF_K + (i & 1u) * 2 * C::TILE);
+#pragma unroll
+            for (int u = 0; u < C::TILE / 16 / (kSplitWarps * 32); ++u) {
+                constexpr uint32_t kBlock = BN * 8;  // 16-byte pieces of a block's hi (or lo) rows
+                const uint32_t x16 = u * kSplitWarps * 32 + tid, e = x16 / kBlock * 2 * kBlock + x16 % kBlock;
+                const uint4 x = hi[e];
+                uint4 h, l;
+                tf32_split(__uint_as_float(x.x), h.x, l.x);
+                tf32_split(__uint_as_float(x.y), h.y, l.y);
+                tf32_split(__uint_as_float(x.z), h.z, l.z);
+                tf32_split(__uint_as_float(x.w), h.w, l.w);
+                hi[e] = h;
+                hi[e + kBlock] = l;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            arrive(&sh.k_ready[i & 1u]);
+        };
+        if (total) split_k(0);
+        while (walk.next(p, sg)) {
+            const uint32_t P = sg.s.L - min(sg.s.T, sg.s.L);
+            const bool valid = r < sg.rows, warp_live = q4 * 32 < sg.rows;
+            uint32_t *odd = sh.odd[segs % 3];
+            if (cw == 0 && lane < 8) sh.odd[(segs + 1) % 3][lane] = 0u;  // read last two segments ago
+            float o[D / 2];
+#pragma unroll
+            for (int k = 0; k < D / 2; ++k) o[k] = 0.f;
+            // the O of tile i, once it is there
+            auto add = [&](uint32_t i) {
+                wait_bar(&sh.o_full, i & 1u, abort_flag);
+                __syncwarp();
+                tc_fence_after();
+                if (warp_live) {
+                    const float alpha = sh.alpha[i & 1u][r];
+#pragma unroll
+                    for (int c = 0; c < D / 2; c += 16) {
+                        float y[16];
+                        tmem_ld16(o_at + c, y);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int u = 0; u < 16; ++u) o[c + u] = fmaf(o[c + u], alpha, y[u]);
+                    }
+                }
+                tc_fence_before();
+                arrive(&sh.o_free);
+            };
+            for (uint32_t j = sg.t0; j < sg.t1; ++j, ++it) {
+                if (j > sg.t0) add(it - 1);
+                // V(it) transposed: thread = 4 positions of one column
+                wait_bar(&sh.v_full, it & 1u, abort_flag);
+                __syncwarp();
+                const float *v = reinterpret_cast<const float *>(smem + C::OFF_V);
+                const uint32_t kv0 = j * BN;
+                const bool edge = kv0 + BN > P;
+#pragma unroll
+                for (int u = 0; u < 2 * D / 32; ++u) {
+                    const uint32_t quad = cw * 2 + (u & 1), d = (u >> 1) * 32 + lane;
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = v[(quad * 4 + e) * D + d];
+                    if (edge) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t pos = kv0 + quad * 4 + e;
+                            if (pos >= sg.s.L) x[e] = 0.f;
+                            else if (pos >= P && !(fabsf(x[e]) < INFINITY)) {
+                                x[e] = 0.f;
+                                atomicOr(&odd[(pos - P) >> 5], 1u << ((pos - P) & 31));
+                            }
+                        }
+                    }
+                    uint4 h, l;
+                    tf32_split(x[0], h.x, l.x);
+                    tf32_split(x[1], h.y, l.y);
+                    tf32_split(x[2], h.z, l.z);
+                    tf32_split(x[3], h.w, l.w);
+                    const uint32_t to = (quad >> 3) * (D * 128) + d * 128 + (((quad & 7) ^ (d & 7)) << 4);
+                    *reinterpret_cast<uint4 *>(smem + C::OFF_VHI + to) = h;
+                    *reinterpret_cast<uint4 *>(smem + C::OFF_VLO + to) = l;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&sh.v_empty);
+                    mbar_arrive(&sh.v_ready);
+                }
+                if (it + 1 < total) split_k(it + 1);
+            }
+            add(it - 1);
+            named_bar_sync(1, 384);  // m and l, and the odd words
+            const float2 ml = sh.ml[r];
+            float l = ml.y;
+            if (*abort_flag) l = __int_as_float(0x7fffffff);  // a wait gave up: NaN
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            float *part = sg.slot < 2 ? tree_part(p, D, blockIdx.x, sg.slot) : nullptr;
+            uint32_t any_odd = 0;
+            if (sg.t1 * BN > P)
+#pragma unroll
+                for (int w = 0; w < 8; ++w) any_odd |= *(volatile uint32_t *)&odd[w];
+            if (valid) {
+                const size_t at = tree_row(p, sg, sg.row0 + r, D);
+                if (any_odd) {
+                    const uint32_t t = (sg.row0 + r) / p.group;
+                    const TreeSeg g = sg;  // as are their copies'
+#pragma unroll
+                    for (int c = 0; c < D / 2; c += 32) {
+                        float tmp[32];  // its address is taken, o's is not
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) tmp[u] = o[c + u];
+                        add_odd<D>(p, g, odd, t, at, half * (D / 2) + c, ml.x, tmp);
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) o[c + u] = tmp[u];
+                    }
+                }
+                if (part) {
+                    float4 *dst = reinterpret_cast<float4 *>(part) + (size_t)half * (D / 8) * p.rpg + r;
+#pragma unroll
+                    for (int u = 0; u < D / 8; ++u) dst[(size_t)u * p.rpg] = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                    if (half == 0) {
+                        part[(size_t)p.rpg * D + r] = ml.x;
+                        part[(size_t)p.rpg * (D + 1) + r] = l;
+                    }
+                } else {
+                    float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at + half * (D / 2));
+#pragma unroll
+                    for (int u = 0; u < D / 8; ++u)
+                        dst[u] = make_float4(o[4 * u] * inv, o[4 * u + 1] * inv, o[4 * u + 2] * inv, o[4 * u + 3] * inv);
+                }
+            }
+            __syncwarp();
+            ++segs;
+        }
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS) : "memory");
+    }
+}
+
+// (d, n_kv, rows) view of a pool.
+bool pool_map(CUtensorMap *map, const void *base, uint32_t d, uint32_t n_kv, uint64_t rows, uint32_t box_d, uint32_t box_rows,
+              CUtensorMapSwizzle swizzle) {
+    auto enc = get_encode();
+    if (!enc) return false;
+    cuuint64_t dims[3] = {d, n_kv, rows};
+    cuuint64_t strides[2] = {(cuuint64_t)d * 4, (cuuint64_t)d * n_kv * 4};
+    cuuint32_t box[3] = {box_d, 1, box_rows};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void *>(base), dims, strides, box, estr,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D>
+cudaError_t launch_x(const TreeArgs &a, cudaStream_t st) {
+    using C = XCfg<D>;
+    static thread_local XParams xp;
+    xp.t = a.p;
+    const uint32_t page = 1u << a.p.page_shift;
+    xp.box_rows = page < (uint32_t)BN ? page : (uint32_t)BN;
+    xp.t.rpg = BM / a.p.group * a.p.group;
+    xp.t.hpu = 1;
+    xp.t.tile = BN;
+    xp.t.heavy_rows = 0xffffffffu;
+    xp.t.heavy = xp.t.light = 1;
+    if (!tree_line(xp.t)) return cudaErrorNotSupported;
+    const uint64_t rows = (uint64_t)a.p.n_pages << a.p.page_shift;
+    if (!pool_map(&xp.tk, a.p.k, D, a.p.n_kv, rows, 32, xp.box_rows, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !pool_map(&xp.tv, a.p.v, D, a.p.n_kv, rows, D, xp.box_rows, CU_TENSOR_MAP_SWIZZLE_NONE))
+        return cudaErrorInvalidValue;
+    auto kern = tree_umma32_kernel<D>;
+    static SmemSet set;  // one for each instantiation
+    cudaError_t e = set.allow(kern, C::SMEM);
+    if (e != cudaSuccess) return e;
+    e = launch_after(kern, dim3(a.num_sms), kThreads, C::SMEM, st, xp);
+    if (e != cudaSuccess) return e;
+    return launch_tree_merge(xp.t, D, a.num_sms, st);
+}
+
+}  // namespace
+
+cudaError_t launch_tree_umma32(const TreeArgs &a, cudaStream_t st) { return a.D == 128 ? launch_x<128>(a, st) : launch_x<64>(a, st); }
+
+}  // namespace bml

@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     // ------------------------------------------------------------ copies, ahead
-    TreeWalk fw(p, range);
+    TreeWalk fw(range);
     TreeSeg fs = {};
     uint32_t f_left = 0, f_pos = 0, f_stage = 0;  // steps left of the segment, the next step's position, its stage
     auto fetch = [&]() {
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
 #pragma unroll 1
     for (int i = 0; i < C::NST - 1; ++i) fetch();
 
-    TreeWalk walk(p, range);
+    TreeWalk walk(range);
     TreeSeg sg;
     uint32_t stage = 0;
     while (walk.next(p, sg)) {
@@ -467,7 +467,7 @@ cudaError_t launch_w(TreeParams p, int num_sms, cudaStream_t st) {
     p.tile = kTreeTile;
     p.heavy_rows = 0xffffffffu;
     p.heavy = p.light = 1;
-    if (!tree_line_fits(p)) return cudaErrorNotSupported;
+    if (!tree_line(p)) return cudaErrorNotSupported;
     e = launch_after(kern, dim3(num_sms), kThreads, C::SMEM, st, p);
     if (e != cudaSuccess) return e;
     return launch_tree_merge(p, D, num_sms, st);
