@@ -450,11 +450,11 @@ __global__ void __launch_bounds__(kThreads, 2) tree_merge_kernel(const __grid_co
         }
     } else {
         b = blockIdx.x + 1;
-        const TreeRange range = tree_range(p, &sh, b, grid);
+        const TreeRange range = tree_range<true>(p, &sh, b, grid);
         mine = range.w0 < range.w1;
         if (mine) {
             TreeWalk walk(range);
-            mine = walk.next(p, sg) && sg.t0 > 0;  // else the cut lies between two units
+            mine = walk.next<true>(p, sg) && sg.t0 > 0;  // else the cut lies between two units
             total = range.total;
             u0 = sg.u0;
             w = sg.w;

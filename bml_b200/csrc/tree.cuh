@@ -104,9 +104,11 @@ __device__ __forceinline__ uint32_t tree_full_weight(const TreeParams &p) { retu
 struct TreeRaw {
     int32_t a, b, L;
 };
+// kEarly: before griddepcontrol.wait (the merge, which reads past L1).
+template <bool kEarly>
 __device__ __forceinline__ TreeRaw tree_raw(const TreeParams &p, uint32_t i) {
-    // from L2: the merge reads them before its griddepcontrol.wait
-    return {__ldcg(p.node_start + i), __ldcg(p.node_start + i + 1), __ldcg(p.kv_lens + i)};
+    if (kEarly) return {__ldcg(p.node_start + i), __ldcg(p.node_start + i + 1), __ldcg(p.kv_lens + i)};
+    return {p.node_start[i], p.node_start[i + 1], p.kv_lens[i]};
 }
 __device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, const TreeRaw &raw) {
     TreeSeq s;
@@ -125,7 +127,10 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, const TreeRaw &
     return s;
 }
 
-__device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, uint32_t i) { return tree_seq(p, tree_raw(p, i)); }
+template <bool kEarly>
+__device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, uint32_t i) {
+    return tree_seq(p, tree_raw<kEarly>(p, i));
+}
 
 struct TreeShared {
     uint32_t warp_sums[32], warp_units[32];
@@ -169,7 +174,7 @@ struct TreePlace {
     TreeSeq s;
 };
 
-template <typename Target>
+template <bool kEarly, typename Target>
 __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *sh, bool by_unit, Target target) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, upr = p.upr;
     const bool alone = p.n_seqs <= 128;
@@ -183,7 +188,7 @@ __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *
 #pragma unroll
         for (uint32_t k = 0; k < 4; ++k)
             if (i0 + k < i1) {
-                raw[k] = tree_raw(p, i0 + k);
+                raw[k] = tree_raw<kEarly>(p, i0 + k);
                 const TreeSeq s = tree_seq(p, raw[k]);
                 n4[k] = s.groups * upr;
                 t4[k] = s.weight * upr * s.tiles;
@@ -192,7 +197,7 @@ __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *
             }
     } else {
         for (uint32_t i = i0; i < i1; ++i) {
-            const TreeSeq s = tree_seq(p, i);
+            const TreeSeq s = tree_seq<kEarly>(p, i);
             units += s.groups * upr;
             tiles += s.weight * upr * s.tiles;
         }
@@ -248,7 +253,7 @@ __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *
     } else {
         if (mine) {
             while (true) {
-                const TreeSeq s = tree_seq(p, seq);
+                const TreeSeq s = tree_seq<kEarly>(p, seq);
                 const uint32_t n = s.groups * upr, t = s.weight * upr * s.tiles;
                 if ((by_unit ? w < fu + n : w < ft + t) || seq + 1 >= i1) break;
                 fu += n;
@@ -263,16 +268,17 @@ __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *
         r.seq = sh->seq;
         r.base = sh->base;
         r.unit0 = sh->unit;
-        if (r.seq < p.n_seqs) r.s = tree_seq(p, r.seq);
+        if (r.seq < p.n_seqs) r.s = tree_seq<kEarly>(p, r.seq);
     }
     return r;
 }
 
 // CTA b's range.  w0 == w1: nothing for this CTA.
+template <bool kEarly = false>
 __device__ __forceinline__ TreeRange tree_range(const TreeParams &p, TreeShared *sh, uint32_t b, uint32_t grid) {
     TreeRange r;
     r.w0 = r.w1 = 0;
-    const TreePlace at = tree_find(p, sh, false, [&](uint32_t total) {
+    const TreePlace at = tree_find<kEarly>(p, sh, false, [&](uint32_t total) {
         const TreeCuts cuts(p, total, grid);
         if (b < cuts.active) {
             r.w0 = cuts.at(b);
@@ -295,9 +301,9 @@ struct TreeUnit {
     bool found;
 };
 
-// The unit with index u in line order.
+// The unit with index u in line order (for the merge).
 __device__ __forceinline__ TreeUnit tree_unit(const TreeParams &p, TreeShared *sh, uint32_t u) {
-    const TreePlace at = tree_find(p, sh, true, [&](uint32_t) { return u; });
+    const TreePlace at = tree_find<true>(p, sh, true, [&](uint32_t) { return u; });
     TreeUnit r = {};
     r.found = u < at.units;
     r.total = at.total;
@@ -329,6 +335,7 @@ struct TreeWalk {
     uint32_t seq;
     TreeSeq s;
     __device__ __forceinline__ explicit TreeWalk(const TreeRange &r) : pos(r.w0), end(r.w1), base(r.base), seq(r.seq), s(r.s) {}
+    template <bool kEarly = false>
     __device__ __forceinline__ bool next(const TreeParams &p, TreeSeg &g) {
         while (pos < end) {
             uint32_t per_head;
@@ -338,7 +345,7 @@ struct TreeWalk {
                     pos = end;
                     return false;
                 }
-                s = tree_seq(p, seq);
+                s = tree_seq<kEarly>(p, seq);
             }
             const uint32_t off = pos - base, wf = tree_full_weight(p);
             const uint32_t head = off / per_head, in_head = off - head * per_head;

@@ -24,9 +24,10 @@
 //
 //   warp 0       copies K and V tiles (cp.async.bulk.tensor; K two stages)
 //   warp 1       tensor memory, and every tcgen05.mma
-//   warps 2-5    Q, and the softmax: thread = row = TMEM lane
-//   warps 6-13   split K and V; add the tiles' O (a warp: 32 rows, half of the
-//                columns) and write the rows.
+//   warps 2-9    thread = row = TMEM lane and half of the columns: Q; the
+//                softmax (the halves' maxima meet in shared memory); O added
+//                in registers; the rows written
+//   warps 10-15  split K and V.
 //
 // V is split while S is computed, and the next tile's K after it.
 //
@@ -44,8 +45,8 @@ namespace bml {
 namespace {
 
 constexpr int BM = 128, BN = 64;
-constexpr int kThreads = 448;
-constexpr int kSplitWarps = 8;
+constexpr int kRowWarps = 8, kSplitWarps = 6;
+constexpr int kThreads = 32 * (2 + kRowWarps + kSplitWarps);  // 512: up to 128 registers a thread
 constexpr int kBadRing = 16;  // tiles whose page flags are kept
 
 template <int D>
@@ -77,8 +78,7 @@ struct alignas(16) XShared {
     uint32_t tmem, abort;
     uint32_t bad[kBadRing];  // per tile: 16-position blocks on pages outside the pool
     uint32_t odd[3][8];      // per segment: drafted nodes with a V value that is not finite
-    float alpha[2][BM];      // per tile: what the rows' output is scaled by before it is added
-    float2 ml[BM];           // the segment's rows' (m, l)
+    float top[2][BM], sum[2][BM];  // [half][row]: maximum of a tile; l of a segment
     TreeShared sched;
 };
 static_assert(sizeof(XShared) <= 3 * 1024, "small arrays");
@@ -123,15 +123,15 @@ __device__ __forceinline__ void put_split(uint32_t hi_at, uint32_t lo_at, const 
     }
 }
 
-// Which of the 64 positions from node0 on (negative: committed ones, seen by
+// Which of the 32 positions from node0 on (negative: committed ones, seen by
 // all) node t sees.
-__device__ __forceinline__ uint64_t see_tile(const TreeParams &p, const TreeSeq &s, uint32_t t, int32_t node0) {
-    if (s.L == 0) return 0ull;
-    uint64_t see = 0;
+__device__ __forceinline__ uint32_t see_half(const TreeParams &p, const TreeSeq &s, uint32_t t, int32_t node0) {
+    if (s.L == 0) return 0u;
+    uint32_t see = 0;
 #pragma unroll 1
-    for (int b = 0; b < 4; ++b) {
+    for (int b = 0; b < 2; ++b) {
         const int32_t n0 = node0 + 16 * b;
-        see |= (uint64_t)(n0 <= -16 ? 0xffffu : tree_see16(p, s, t, n0) & 0xffffu) << (16 * b);
+        see |= (n0 <= -16 ? 0xffffu : tree_see16(p, s, t, n0) & 0xffffu) << (16 * b);
     }
     return see;
 }
@@ -177,12 +177,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
         }
         mbar_init(&sh.v_full, 1);
         mbar_init(&sh.v_empty, kSplitWarps);
-        mbar_init(&sh.q_ready, 4);
+        mbar_init(&sh.q_ready, kRowWarps);
         mbar_init(&sh.v_ready, kSplitWarps);
         mbar_init(&sh.s_full, 1);
-        mbar_init(&sh.p_ready, 4);
+        mbar_init(&sh.p_ready, kRowWarps);
         mbar_init(&sh.o_full, 1);
-        mbar_init(&sh.o_free, kSplitWarps);
+        mbar_init(&sh.o_free, kRowWarps);
         mbar_init(&sh.drain, 1);
         sh.abort = 0u;
         fence_mbar_init();
@@ -317,170 +317,211 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
         __syncwarp();
         mbar_drain(&sh.drain, 0, kWaitNs);
         __syncwarp();
-    } else if (warp < 6) {
+    } else if (warp < 2 + kRowWarps) {
         // ---------------------------------------------------------- Q and softmax
-        const uint32_t q4 = warp & 3, r = q4 * 32 + lane, lane_addr = (q4 * 32) << 16;
-        const uint32_t at = tmem + lane_addr;
+        const uint32_t q4 = warp & 3, half = (warp - 2) >> 2, r = q4 * 32 + lane;
+        const uint32_t at = tmem + ((q4 * 32) << 16), hi_at = at + C::SC + 32 * half, lo_at = at + C::PLO + 32 * half, o_at = at + C::OC + half * (D / 2);
         while (walk.next(p, sg)) {
             const bool valid = r < sg.rows;
             const bool warp_live = q4 * 32 < sg.rows;
             const uint32_t P = sg.s.L - min(sg.s.T, sg.s.L), t = min((sg.row0 + r) / p.group, sg.s.T - 1);
             if (warp_live) {
                 const float *q = static_cast<const float *>(p.q) + (valid ? tree_row(p, sg, sg.row0 + r, D) : 0);
-#pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    float x[32];
+                float x[D / 2];
 #pragma unroll
-                    for (int u = 0; u < 8; ++u) {
-                        const float4 y = valid ? *reinterpret_cast<const float4 *>(q + c + 4 * u) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        x[4 * u] = y.x;
-                        x[4 * u + 1] = y.y;
-                        x[4 * u + 2] = y.z;
-                        x[4 * u + 3] = y.w;
-                    }
-                    __syncwarp();
-                    put_split(at + C::QHI + c, at + C::QLO + c, x);
+                for (int u = 0; u < D / 8; ++u) {
+                    const float4 y = valid ? *reinterpret_cast<const float4 *>(q + half * (D / 2) + 4 * u) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    x[4 * u] = y.x;
+                    x[4 * u + 1] = y.y;
+                    x[4 * u + 2] = y.z;
+                    x[4 * u + 3] = y.w;
                 }
+                __syncwarp();
+#pragma unroll
+                for (int c = 0; c < D / 2; c += 32) put_split(at + C::QHI + half * (D / 2) + c, at + C::QLO + half * (D / 2) + c, x + c);
                 tmem_wait_st();
             }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.q_ready);
-            float m = -INFINITY, l = 0.f;
+            float m = -INFINITY, l = 0.f;  // l: of this half of the positions
+            float o[D / 2];                // this half of the columns
+#pragma unroll
+            for (int k = 0; k < D / 2; ++k) o[k] = 0.f;
             for (uint32_t j = sg.t0; j < sg.t1; ++j, ++it) {
                 wait_bar(&sh.s_full, it & 1u, abort_flag);
                 __syncwarp();
                 tc_fence_after();
+                float alpha = 1.f;
                 if (warp_live) {
-                    const uint32_t bad = *(volatile uint32_t *)&sh.bad[it % kBadRing], kv0 = j * BN;
-                    const bool edge = kv0 + BN > P;
-                    uint64_t see = ~0ull;
+                    const uint32_t bad = *(volatile uint32_t *)&sh.bad[it % kBadRing] >> (2 * half) & 3u, kv0 = j * BN + 32 * half;
+                    const bool edge = kv0 + 32 > P;
+                    uint32_t see = ~0u;
                     if (edge || bad) {
-                        if (edge) see = see_tile(p, sg.s, t, (int32_t)(kv0 - P));
-#pragma unroll
-                        for (int b = 0; b < 4; ++b)
-                            if (bad >> b & 1) see &= ~(0xffffull << (16 * b));
+                        if (edge) see = see_half(p, sg.s, t, (int32_t)(kv0 - P));
+                        if (bad & 1) see &= 0xffff0000u;
+                        if (bad & 2) see &= 0x0000ffffu;
                     }
-                    float s[BN];
-                    tmem_ld32(at + C::SC, s);
-                    tmem_ld32(at + C::SC + 32, s + 32);
+                    float s[32];
+                    tmem_ld32(hi_at, s);
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) {
+                    for (int h = 0; h < 2; ++h) {
                         float y[16];
-                        tmem_ld16(at + C::PLO + 16 * h, y);
+                        tmem_ld16(lo_at + 16 * h, y);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) s[16 * h + k] += y[k];
+                        for (int k = 0; k < 16; k += 2) {
+                            const float2 z = __fadd2_rn(make_float2(s[16 * h + k], s[16 * h + k + 1]), make_float2(y[k], y[k + 1]));
+                            s[16 * h + k] = z.x;
+                            s[16 * h + k + 1] = z.y;
+                        }
                     }
                     if (edge || bad) {
-                        const uint32_t w[2] = {(uint32_t)see, (uint32_t)(see >> 32)};
 #pragma unroll
-                        for (int k = 0; k < BN; ++k)
-                            if (!(w[k >> 5] >> (k & 31) & 1)) s[k] = -INFINITY;
+                        for (int k = 0; k < 32; ++k)
+                            if (!(see >> k & 1)) s[k] = -INFINITY;
                     }
                     float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                    for (int k = 4; k < BN; ++k) mx[k & 3] = fmaxf(mx[k & 3], s[k]);
-                    const float m_new = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2);  // > 0
-                    const float mu = m_new == -INFINITY ? 0.f : m_new, alpha = fast_exp2(m - mu);
+                    for (int k = 4; k < 32; ++k) mx[k & 3] = fmaxf(mx[k & 3], s[k]);
+                    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;  // > 0
+                    sh.top[half][r] = top;
+                    named_bar_sync(2 + q4, 64);
+                    const float m_new = fmaxf(m, fmaxf(top, sh.top[half ^ 1u][r]));
+                    const float mu = m_new == -INFINITY ? 0.f : m_new;
+                    alpha = fast_exp2(m - mu);
                     m = m_new;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    const float2 c2 = make_float2(p.scale_log2, p.scale_log2), nm2 = make_float2(-mu, -mu);
+                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            s[32 * h + k] = fast_exp2(fmaf(s[32 * h + k], p.scale_log2, -mu));
-                            sum[k & 3] += s[32 * h + k];
-                        }
-                        put_split(at + C::SC + 32 * h, at + C::PLO + 32 * h, s + 32 * h);
+                    for (int k = 0; k < 32; k += 2) {
+                        const float2 z = __ffma2_rn(make_float2(s[k], s[k + 1]), c2, nm2);
+                        s[k] = fast_exp2(z.x);
+                        s[k + 1] = fast_exp2(z.y);
+                        sum[k >> 1 & 1] = __fadd2_rn(sum[k >> 1 & 1], make_float2(s[k], s[k + 1]));
                     }
-                    l = fmaf(l, alpha, (sum[0] + sum[1]) + (sum[2] + sum[3]));
-                    sh.alpha[it & 1u][r] = alpha;
+                    put_split(hi_at, lo_at, s);
+                    const float2 both = __fadd2_rn(sum[0], sum[1]);
+                    l = fmaf(l, alpha, both.x + both.y);
                     tmem_wait_st();
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.p_ready);
-            }
-            wait_bar(&sh.v_ready, (it - 1) & 1u, abort_flag);  // the split warps have read the last segment's
-            sh.ml[r] = make_float2(m, l);
-            __syncwarp();
-            named_bar_sync(1, 384);
-            ++segs;
-        }
-    } else {
-        // ------------------------------------- K and V split, O added, rows written
-        const uint32_t cw = warp - 6, half = cw >> 2, q4 = warp & 3, r = q4 * 32 + lane, tid = cw * 32 + lane;
-        const uint32_t o_at = tmem + ((q4 * 32) << 16) + C::OC + half * (D / 2);
-        uint32_t total = 0;  // tiles of this CTA
-        {
-            TreeWalk w(range);
-            TreeSeg g;
-            while (w.next(p, g)) total += g.t1 - g.t0;
-        }
-        auto arrive = [&](uint64_t *bar) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar);
-        };
-        auto split_k = [&](uint32_t i) {
-            wait_bar(&sh.k_full[i & 1u], (i >> 1) & 1u, abort_flag);
-            __syncwarp();
-            uint4 *hi = reinterpret_cast<uint4 *>(smem + C::OFF_K + (i & 1u) * 2 * C::TILE);
-#pragma unroll
-            for (int u = 0; u < C::TILE / 16 / (kSplitWarps * 32); ++u) {
-                constexpr uint32_t kBlock = BN * 8;  // 16-byte pieces of a block's hi (or lo) rows
-                const uint32_t x16 = u * kSplitWarps * 32 + tid, e = x16 / kBlock * 2 * kBlock + x16 % kBlock;
-                const uint4 x = hi[e];
-                uint4 h, l;
-                tf32_split(__uint_as_float(x.x), h.x, l.x);
-                tf32_split(__uint_as_float(x.y), h.y, l.y);
-                tf32_split(__uint_as_float(x.z), h.z, l.z);
-                tf32_split(__uint_as_float(x.w), h.w, l.w);
-                hi[e] = h;
-                hi[e + kBlock] = l;
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            arrive(&sh.k_ready[i & 1u]);
-        };
-        if (total) split_k(0);
-        while (walk.next(p, sg)) {
-            const uint32_t P = sg.s.L - min(sg.s.T, sg.s.L);
-            const bool valid = r < sg.rows, warp_live = q4 * 32 < sg.rows;
-            uint32_t *odd = sh.odd[segs % 3];
-            if (cw == 0 && lane < 8) sh.odd[(segs + 1) % 3][lane] = 0u;  // read last two segments ago
-            float o[D / 2];
-#pragma unroll
-            for (int k = 0; k < D / 2; ++k) o[k] = 0.f;
-            // the O of tile i, once it is there
-            auto add = [&](uint32_t i) {
-                wait_bar(&sh.o_full, i & 1u, abort_flag);
+                wait_bar(&sh.o_full, it & 1u, abort_flag);
                 __syncwarp();
                 tc_fence_after();
-                if (warp_live) {
-                    const float alpha = sh.alpha[i & 1u][r];
+                if (warp_live)
 #pragma unroll
                     for (int c = 0; c < D / 2; c += 16) {
                         float y[16];
                         tmem_ld16(o_at + c, y);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int u = 0; u < 16; ++u) o[c + u] = fmaf(o[c + u], alpha, y[u]);
+                        for (int u = 0; u < 16; u += 2) {
+                            const float2 z = __ffma2_rn(make_float2(o[c + u], o[c + u + 1]), make_float2(alpha, alpha), make_float2(y[u], y[u + 1]));
+                            o[c + u] = z.x;
+                            o[c + u + 1] = z.y;
+                        }
+                    }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.o_free);
+            }
+            if (warp_live) {
+                sh.sum[half][r] = l;
+                named_bar_sync(2 + q4, 64);
+                l += sh.sum[half ^ 1u][r];
+            }
+            if (*abort_flag) l = __int_as_float(0x7fffffff);  // a wait gave up: NaN
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const uint32_t *odd = sh.odd[segs % 3];  // all V of the segment has been split
+            float *part = sg.slot < 2 ? tree_part(p, D, blockIdx.x, sg.slot) : nullptr;
+            uint32_t any_odd = 0;
+            if (sg.t1 * BN > P)
+#pragma unroll
+                for (int w = 0; w < 8; ++w) any_odd |= *(const volatile uint32_t *)&odd[w];
+            if (valid) {
+                const size_t at = tree_row(p, sg, sg.row0 + r, D);
+                if (any_odd) {
+                    const uint32_t t = (sg.row0 + r) / p.group;
+                    const TreeSeg g = sg;  // as are their copies'
+#pragma unroll
+                    for (int c = 0; c < D / 2; c += 32) {
+                        float tmp[32];  // its address is taken, o's is not
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) tmp[u] = o[c + u];
+                        add_odd<D>(p, g, odd, t, at, half * (D / 2) + c, m, tmp);
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) o[c + u] = tmp[u];
                     }
                 }
-                tc_fence_before();
-                arrive(&sh.o_free);
-            };
+                if (part) {
+                    float4 *dst = reinterpret_cast<float4 *>(part) + (size_t)half * (D / 8) * p.rpg + r;
+#pragma unroll
+                    for (int u = 0; u < D / 8; ++u) dst[(size_t)u * p.rpg] = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
+                    if (half == 0) {
+                        part[(size_t)p.rpg * D + r] = m;
+                        part[(size_t)p.rpg * (D + 1) + r] = l;
+                    }
+                } else {
+                    float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at + half * (D / 2));
+#pragma unroll
+                    for (int u = 0; u < D / 8; ++u)
+                        dst[u] = make_float4(o[4 * u] * inv, o[4 * u + 1] * inv, o[4 * u + 2] * inv, o[4 * u + 3] * inv);
+                }
+            }
+            __syncwarp();
+            ++segs;
+        }
+    } else {
+        // --------------------------------------------------------- K and V split
+        const uint32_t cw = warp - 2 - kRowWarps, tid = cw * 32 + lane;
+        constexpr uint32_t kN = kSplitWarps * 32;
+        uint32_t total = 0;  // tiles of this CTA
+        {
+            TreeWalk w(range);
+            TreeSeg g;
+            while (w.next(p, g)) total += g.t1 - g.t0;
+        }
+        auto split_k = [&](uint32_t i) {
+            wait_bar(&sh.k_full[i & 1u], (i >> 1) & 1u, abort_flag);
+            __syncwarp();
+            uint4 *k = reinterpret_cast<uint4 *>(smem + C::OFF_K + (i & 1u) * 2 * C::TILE);
+#pragma unroll 4
+            for (uint32_t x = tid; x < C::TILE / 16; x += kN) {
+                constexpr uint32_t kBlock = BN * 8;  // 16-byte pieces of a block's hi (or lo) rows
+                const uint32_t e = x + x / kBlock * kBlock;
+                const uint4 y = k[e];
+                uint4 h, l;
+                tf32_split(__uint_as_float(y.x), h.x, l.x);
+                tf32_split(__uint_as_float(y.y), h.y, l.y);
+                tf32_split(__uint_as_float(y.z), h.z, l.z);
+                tf32_split(__uint_as_float(y.w), h.w, l.w);
+                k[e] = h;
+                k[e + kBlock] = l;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.k_ready[i & 1u]);
+        };
+        if (total) split_k(0);
+        while (walk.next(p, sg)) {
+            const uint32_t P = sg.s.L - min(sg.s.T, sg.s.L);
+            uint32_t *odd = sh.odd[segs % 3];
             for (uint32_t j = sg.t0; j < sg.t1; ++j, ++it) {
-                if (j > sg.t0) add(it - 1);
                 // V(it) transposed: thread = 4 positions of one column
                 wait_bar(&sh.v_full, it & 1u, abort_flag);
+                if (it > 0) wait_bar(&sh.o_full, (it & 1u) ^ 1u, abort_flag);  // the last tile's V has been read
                 __syncwarp();
+                // read two segments ago: the rows' warps have since been through a tile of the last one
+                if (j == sg.t0 && cw == 0 && lane < 8) sh.odd[(segs + 1) % 3][lane] = 0u;
                 const float *v = reinterpret_cast<const float *>(smem + C::OFF_V);
                 const uint32_t kv0 = j * BN;
                 const bool edge = kv0 + BN > P;
-#pragma unroll
-                for (int u = 0; u < 2 * D / 32; ++u) {
-                    const uint32_t quad = cw * 2 + (u & 1), d = (u >> 1) * 32 + lane;
+#pragma unroll 4
+                for (uint32_t u = cw; u < BN / 4 * (D / 32); u += kSplitWarps) {
+                    const uint32_t quad = u % (BN / 4), d = u / (BN / 4) * 32 + lane;
                     float x[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[e] = v[(quad * 4 + e) * D + d];
@@ -512,48 +553,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
                 }
                 if (it + 1 < total) split_k(it + 1);
             }
-            add(it - 1);
-            named_bar_sync(1, 384);  // m and l, and the odd words
-            const float2 ml = sh.ml[r];
-            float l = ml.y;
-            if (*abort_flag) l = __int_as_float(0x7fffffff);  // a wait gave up: NaN
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            float *part = sg.slot < 2 ? tree_part(p, D, blockIdx.x, sg.slot) : nullptr;
-            uint32_t any_odd = 0;
-            if (sg.t1 * BN > P)
-#pragma unroll
-                for (int w = 0; w < 8; ++w) any_odd |= *(volatile uint32_t *)&odd[w];
-            if (valid) {
-                const size_t at = tree_row(p, sg, sg.row0 + r, D);
-                if (any_odd) {
-                    const uint32_t t = (sg.row0 + r) / p.group;
-                    const TreeSeg g = sg;  // as are their copies'
-#pragma unroll
-                    for (int c = 0; c < D / 2; c += 32) {
-                        float tmp[32];  // its address is taken, o's is not
-#pragma unroll
-                        for (int u = 0; u < 32; ++u) tmp[u] = o[c + u];
-                        add_odd<D>(p, g, odd, t, at, half * (D / 2) + c, ml.x, tmp);
-#pragma unroll
-                        for (int u = 0; u < 32; ++u) o[c + u] = tmp[u];
-                    }
-                }
-                if (part) {
-                    float4 *dst = reinterpret_cast<float4 *>(part) + (size_t)half * (D / 8) * p.rpg + r;
-#pragma unroll
-                    for (int u = 0; u < D / 8; ++u) dst[(size_t)u * p.rpg] = make_float4(o[4 * u], o[4 * u + 1], o[4 * u + 2], o[4 * u + 3]);
-                    if (half == 0) {
-                        part[(size_t)p.rpg * D + r] = ml.x;
-                        part[(size_t)p.rpg * (D + 1) + r] = l;
-                    }
-                } else {
-                    float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(p.out) + at + half * (D / 2));
-#pragma unroll
-                    for (int u = 0; u < D / 8; ++u)
-                        dst[u] = make_float4(o[4 * u] * inv, o[4 * u + 1] * inv, o[4 * u + 2] * inv, o[4 * u + 3] * inv);
-                }
-            }
-            __syncwarp();
             ++segs;
         }
     }
