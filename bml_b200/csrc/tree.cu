@@ -581,6 +581,7 @@ cudaError_t launch_f32(TreeParams p, int num_sms, cudaStream_t st) {
     p.tile = C::TILE;
     p.heavy_rows = 0xffffffffu;
     p.heavy = p.light = 1;
+    p.lead = 2;  // 64 requests of 100 to 2000 positions, d = 64: 44.8 us, 51.7 without, 48.3 with 4
     if (!tree_line(p)) return cudaErrorNotSupported;
     e = launch_after(kern, dim3(num_sms), kThreads, C::SMEM, st, p);
     if (e != cudaSuccess) return e;

@@ -30,6 +30,7 @@ struct TreeParams {
     uint32_t tile_shift, upr;  // log2(tile); units of a row group: n_kv / hpu (tree_line)
     // a tile's weight: heavy with more rows than heavy_rows, else light
     uint32_t heavy_rows, heavy, light;
+    uint32_t lead;  // places ahead of a unit's first tile: what its start and end cost
 };
 
 struct TreeArgs {
@@ -76,7 +77,7 @@ inline bool tree_line(TreeParams &p) {
     while (1u << p.tile_shift < p.tile) ++p.tile_shift;
     p.upr = p.n_kv / p.hpu;
     const uint64_t tiles = (((uint64_t)p.max_pages << p.page_shift) + p.tile - 1) / p.tile;
-    return tree_most_units(p) * p.heavy <= 0xffffffffull / tiles;
+    return tree_most_units(p) * p.heavy <= 0xffffffffull / (tiles + p.lead);
 }
 
 #ifdef __CUDACC__
@@ -85,7 +86,8 @@ inline bool tree_line(TreeParams &p) {
 // heads the query rows (node t, q head g of the kv head) of up to rpg
 // consecutive t * group + g, over all positions of the request.  Units are laid
 // out request by request, heads by heads, row group by row group, each as its
-// number of tiles of positions times a tile's weight, and the line of all tiles is cut evenly over the CTAs,
+// number of tiles of positions times a tile's weight, with `lead` places ahead of
+// the first tile, and the line of all places is cut evenly over the CTAs,
 // so the lengths stay on the GPU and no CTA works longer than another by more
 // than a tile.  A unit that a cut divides leaves partial results (max, sum,
 // un-normalised output) which tree_merge_kernel joins in tile order.
@@ -95,6 +97,7 @@ struct TreeSeq {
     uint32_t T, L;   // drafted tokens; positions (0: refused, its rows are zero)
     uint32_t rows, groups, tiles;
     uint32_t w_last, weight;  // a tile's weight in the last row group; in all groups of a head
+    uint32_t places;          // of a head
 };
 
 // A tile's weight in a full row group.
@@ -124,6 +127,7 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, const TreeRaw &
     s.tiles = s.L ? (s.L + p.tile - 1) >> p.tile_shift : 1u;
     s.w_last = s.rows - (s.groups - 1) * p.rpg > p.heavy_rows ? p.heavy : p.light;
     s.weight = s.groups ? (s.groups - 1) * tree_full_weight(p) + s.w_last : 0u;
+    s.places = s.weight * s.tiles + s.groups * p.lead;
     return s;
 }
 
@@ -191,7 +195,7 @@ __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *
                 raw[k] = tree_raw<kEarly>(p, i0 + k);
                 const TreeSeq s = tree_seq(p, raw[k]);
                 n4[k] = s.groups * upr;
-                t4[k] = s.weight * upr * s.tiles;
+                t4[k] = upr * s.places;
                 units += n4[k];
                 tiles += t4[k];
             }
@@ -199,7 +203,7 @@ __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *
         for (uint32_t i = i0; i < i1; ++i) {
             const TreeSeq s = tree_seq<kEarly>(p, i);
             units += s.groups * upr;
-            tiles += s.weight * upr * s.tiles;
+            tiles += upr * s.places;
         }
     }
     uint32_t inc_t = tiles, inc_u = units;
@@ -254,7 +258,7 @@ __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *
         if (mine) {
             while (true) {
                 const TreeSeq s = tree_seq<kEarly>(p, seq);
-                const uint32_t n = s.groups * upr, t = s.weight * upr * s.tiles;
+                const uint32_t n = s.groups * upr, t = upr * s.places;
                 if ((by_unit ? w < fu + n : w < ft + t) || seq + 1 >= i1) break;
                 fu += n;
                 ft += t;
@@ -293,7 +297,7 @@ __device__ __forceinline__ TreeRange tree_range(const TreeParams &p, TreeShared 
     return r;
 }
 
-// A unit's place on the line: [u0, u0 + w * s.tiles).
+// A unit's place on the line: its tiles lie at [u0, u0 + w * s.tiles).
 struct TreeUnit {
     uint32_t u0, w, total;
     uint32_t seq, head, rg;
@@ -313,7 +317,7 @@ __device__ __forceinline__ TreeUnit tree_unit(const TreeParams &p, TreeShared *s
         const uint32_t in = u - at.unit0;
         r.head = in / r.s.groups;
         r.rg = in - r.head * r.s.groups;
-        r.u0 = at.base + (r.head * r.s.weight + r.rg * tree_full_weight(p)) * r.s.tiles;
+        r.u0 = at.base + r.head * r.s.places + r.rg * (tree_full_weight(p) * r.s.tiles + p.lead) + p.lead;
         r.w = r.rg + 1 == r.s.groups ? r.s.w_last : tree_full_weight(p);
         r.head *= p.hpu;
     }
@@ -339,7 +343,7 @@ struct TreeWalk {
     __device__ __forceinline__ bool next(const TreeParams &p, TreeSeg &g) {
         while (pos < end) {
             uint32_t per_head;
-            while (pos - base >= (per_head = s.weight * s.tiles) * p.upr) {
+            while (pos - base >= (per_head = s.places) * p.upr) {
                 base += per_head * p.upr;
                 if (++seq >= p.n_seqs) {  // only with a node_start that does not ascend
                     pos = end;
@@ -349,13 +353,15 @@ struct TreeWalk {
             }
             const uint32_t off = pos - base, wf = tree_full_weight(p);
             const uint32_t head = off / per_head, in_head = off - head * per_head;
-            g.rg = s.groups > 1 ? min(in_head / (wf * s.tiles), s.groups - 1) : 0u;
+            const uint32_t full = wf * s.tiles + p.lead;
+            g.rg = s.groups > 1 ? min(in_head / full, s.groups - 1) : 0u;
             g.w = g.rg + 1 == s.groups ? s.w_last : wf;
-            const uint32_t in = in_head - g.rg * wf * s.tiles, left = end - pos;
-            const uint32_t out = min(in + left, g.w * s.tiles);  // where the range ends in the unit
-            g.t0 = g.w == 1 ? in : (in + g.w - 1) / g.w;
-            g.t1 = g.w == 1 ? out : (out + g.w - 1) / g.w;
-            g.u0 = pos - in;
+            const uint32_t in = in_head - g.rg * full, left = end - pos;
+            const uint32_t out = min(in + left, g.w * s.tiles + p.lead);  // where the range ends in the unit
+            const uint32_t ti = max(in, p.lead) - p.lead, to = max(out, p.lead) - p.lead;
+            g.t0 = g.w == 1 ? ti : (ti + g.w - 1) / g.w;
+            g.t1 = g.w == 1 ? to : (to + g.w - 1) / g.w;
+            g.u0 = pos - in + p.lead;
             pos += out - in;
             if (g.t0 == g.t1) continue;  // no tile begins here
             g.seq = seq;

@@ -471,6 +471,9 @@ cudaError_t launch_n(const TreeArgs &a, cudaStream_t st) {
     fp.t.tile = 16 * fp.splits;
     fp.t.heavy_rows = 0xffffffffu;
     fp.t.heavy = fp.t.light = 1;
+    // 64 requests of 200 to 4000 positions, d = 64: 25.8 us, 31 without a lead, 26.2 with
+    // 8; 16 of 500 to 8000, d = 128: 45.5, 49.8, 45.7
+    fp.t.lead = 6;
     if (!tree_line(fp.t)) return cudaErrorNotSupported;
     const uint64_t rows = (uint64_t)a.p.n_pages << a.p.page_shift;
     if (!few_map(&fp.tk, a.p.k, kF16, D, a.p.n_kv, rows) || !few_map(&fp.tv, a.p.v, kF16, D, a.p.n_kv, rows))
