@@ -9,8 +9,9 @@
 // SugarFreeDoNoSo/bml) for every node of a draft at once.  A row that sees
 // nothing is zero.
 //
-// tree_f32_kernel serves 32-bit queries (and 32-bit pages): results to about
-// f32 precision from TF32 matrix instructions.  Every f32 operand is split
+// tree_f32_kernel serves 32-bit pages where tree_umma32.cu does not (the rule
+// stands in launch_tree): results to about f32 precision from TF32 matrix
+// instructions.  Every f32 operand is split
 // x = hi + lo, hi = tf32(x), lo = tf32(x - hi) (22 bits together), and
 // products are hi*hi + lo*hi + hi*lo; f16 and bf16 values are tf32 values
 // already, so 16-bit pages need no lo.  A warp keeps 16 rows' output in
@@ -625,8 +626,8 @@ size_t tree_workspace_bytes(uint32_t D, int num_sms) {
 }
 
 cudaError_t launch_tree(const TreeArgs &a, cudaStream_t st) {
-    // 16-bit pages, except for a scale of 0 (those kernels scale masked scores
-    // after they were set to -inf).  Up to 8 rows a kv head (on average): the
+    // All but tree_f32_kernel scale masked scores after they were set to -inf, so a
+    // scale of 0 is its.  16-bit pages:  Up to 8 rows a kv head (on average): the
     // form with positions as MMA rows (64 x 4000, d = 64, 8 rows: 49 us, 73 with
     // tree_warp.cu).  16-bit queries of more rows: tcgen05 where there is enough
     // work for its longer start (32 x 8000, d = 128: 24 rows 177 us against 217,
@@ -634,14 +635,19 @@ cudaError_t launch_tree(const TreeArgs &a, cudaStream_t st) {
     // rows 82 against 93, 48 rows 78 against 144, 16 rows 82 against 74; but one
     // request of 708 positions, 4 kv heads, 64 rows 15 against 11 us).  How much
     // work there is the host knows only as a bound, the tables' width.
-    if (a.kv_type != BML_F32 && a.p.scale_log2 > 0.f) {
+    // 32-bit pages, more than 16 rows: tcgen05, with d = 64 where there is work
+    // (d = 128: 64 requests of 1000 positions, 20 rows 247 us against 391, 1 of 700
+    // 19.5 against 17.4, 64 rows 20.7 against 22.1; with 16 rows 247 against 166.
+    // d = 64: 64 of 1000, 32 rows 180 against 212; 1 of 700 14.5 against 12.6).
+    const uint64_t most = (((uint64_t)a.p.max_pages << a.p.page_shift) + kTreeTile - 1) / kTreeTile * a.p.n_seqs * a.p.n_kv;
+    const bool little = most <= 2ull * a.num_sms;
+    if (a.p.scale_log2 > 0.f && a.kv_type != BML_F32) {
         if (a.rows <= 8) return launch_tree_few(a, st);
-        const uint64_t most = (((uint64_t)a.p.max_pages << a.p.page_shift) + kTreeTile - 1) / kTreeTile * a.p.n_seqs * a.p.n_kv;
-        const bool small = most <= 2ull * a.num_sms || a.rows <= (a.D == 128 ? 8u : 16u);
+        const bool small = little || a.rows <= (a.D == 128 ? 8u : 16u);
         if (a.p.q_type == BML_F32 || !tree_umma_fits(a) || (small && a.rows <= 64)) return launch_tree_warp(a, st);
         return launch_tree_umma(a, st);
     }
-    if (a.kv_type == BML_F32 && a.p.scale_log2 > 0.f && a.rows > 16 && a.p.group <= 128) return launch_tree_umma32(a, st);
+    if (a.p.scale_log2 > 0.f && a.rows > 16 && tree_umma_fits(a) && !(a.D == 64 && little)) return launch_tree_umma32(a, st);
     return a.D == 128 ? launch_kv<128>(a, st) : launch_kv<64>(a, st);
 }
 

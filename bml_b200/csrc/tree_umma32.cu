@@ -31,6 +31,13 @@
 //
 // V is split while S is computed, and the next tile's K after it.
 //
+// Measured on B200, d = 128: 3.55 us a tile and CTA, of which the S products
+// take 1.6 (1.0 while nothing else uses shared memory), the softmax 1.4 and P V
+// 0.9, one after another: Q's two parts, S and O fill the tensor memory, so S
+// has no second buffer; copies, splits and MMA operands pass 3600 cycles' worth
+// of shared memory.  4 requests of 618 to 2671 positions, 32 to 84 rows: 43 us,
+// 75.6 with tree.cu's kernel.
+//
 // What a row does not see must not reach it: scores are replaced by -inf (bad
 // pages, rows past the length, nodes outside the mask), V rows past the length
 // and values of drafted nodes that are not finite are split as zeros, and the

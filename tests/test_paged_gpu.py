@@ -303,6 +303,45 @@ def test_more_requests_than_one_launch(cuda):
     check(c, got, [chain(1, p) for p in lens], "bf16", only=[0, 1, 700, 1023, 1024, 1025, 1499])
 
 
+@pytest.mark.parametrize("qt,ct", TYPES)
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 16), (128, 128)])
+def test_wide_tables(cuda, qt, ct, d, page):
+    """Tables far wider than the requests (the kernels for much work): rows that
+    see nothing, values that are not finite in nodes that a row does not see and
+    in one that it sees, and pages outside the pool."""
+    import bml_b200
+    lens, nodes = [0, 200, 0, 300, 129], [6, 7, 70, 20, 64]
+    c = Paged(lens, nodes, 8, 2, d, page, qt, ct, seed=14)
+    c.table = torch.cat([c.table, torch.full((5, 16384 // page), -1, dtype=torch.int32, device="cuda")], 1).contiguous()
+    rng = np.random.default_rng(2)
+    masks = [np.zeros((6, 6), bool), np.tril(np.ones((7, 7), bool))] + [rng.random((t, t)) < 0.3 for t in nodes[2:]]
+    masks[0][1, 0] = masks[0][2, 5] = masks[0][5, 5] = True   # rows 0, 3, 4 see nothing
+    masks[1][:, 3] = masks[2][:, 3] = False                    # NaN: by nobody
+    masks[2][:, 67:] = False
+    masks[2][69, 68] = True                                    # an infinity: by row 69 only
+    for i, node, k, v in ((1, 3, float("inf"), float("nan")), (2, 3, float("nan"), float("nan")), (2, 68, None, float("inf"))):
+        pos = lens[i] + node
+        at = int(c.table[i, pos // page])
+        if k is not None:
+            c.k[at, pos % page] = k
+        c.v[at, pos % page, :, ::3] = v
+        c.ks[i][pos] = 0 if k is not None else c.ks[i][pos]    # seen by nobody: the formula's 0 * NaN is not the kernel's
+        c.vs[i][pos, :, ::3] = v
+    c.table[3, 1] = c.k.shape[0]                               # positions page .. 2 page - 1
+    call = lambda: bml_b200.tree_attention(c.q, c.k, c.v, c.table, c.kv_lens, c.start, mask=pack(masks, 2))
+    got = call()
+    assert torch.equal(got.view(torch.uint8), call().view(torch.uint8))
+    assert (got[[0, 3, 4]] == 0).all()
+    row = int(c.start[2]) + 69
+    assert torch.isposinf(got[row, :, ::3]).all()
+    assert torch.isfinite(got[row][:, [x for x in range(d) if x % 3]]).all()
+    got[row] = 0
+    masks[2][69] = False
+    sees = [np.concatenate([np.ones((t, p), bool), m], 1) for t, p, m in zip(nodes, lens, masks)]
+    sees[3][:, page:2 * page] = False
+    check(c, got, sees, qt)
+
+
 @pytest.mark.parametrize("qt,ct", [("bf16", "bf16"), ("f32", "f16")])
 def test_streams_and_graphs(cuda, qt, ct):
     """Another stream; two graphs whose replays overlap on two streams."""
