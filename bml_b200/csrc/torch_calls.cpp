@@ -71,11 +71,11 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, c10::Device dev) {
     return at::detail::empty_cuda(sizes, type, dev, std::nullopt);
 }
 
-// `n` elements of a 1-D buffer from `at` on, as a tensor of its own.
-PyObject *piece(const at::Tensor &buf, int64_t at, int64_t n) {
-    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), buf.dtype());
+// Elements of `type` from element `at` of a buffer on, as a tensor of its own.
+PyObject *piece(const at::Tensor &buf, const caffe2::TypeMeta &type, int64_t at, at::IntArrayRef sizes) {
+    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), type);
     impl->set_storage_offset(at);
-    impl->set_sizes_contiguous({n});
+    impl->set_sizes_contiguous(sizes);
     return THPVariable_Wrap(at::Tensor(std::move(impl)));
 }
 
@@ -110,30 +110,32 @@ PyObject *plan_impl(PyObject *const *a) {
         parents = typed(a[8], 1, at::kInt, dev);
         USUAL(parents && parents->size(0) == n_tokens && words >= 1 && words <= 4);
     }
-    at::Tensor slots = fresh({n_tokens}, at::kLong, dev), mask;
-    if (parents) mask = fresh({n_tokens, words}, at::kLong, dev);
-    at::Tensor small = fresh({n_tokens + 4 * n + 2}, at::kInt, dev);
-    int32_t *pos = small.mutable_data_ptr<int32_t>(), *b = pos + n_tokens;
+    // all results in one buffer: slots and mask, then the int32 arrays
+    const int64_t wide = n_tokens * (parents ? 1 + words : 1);
+    at::Tensor all = fresh({wide + (n_tokens + 4 * n + 3) / 2}, at::kLong, dev);
+    int64_t *slots = all.mutable_data_ptr<int64_t>();
+    int32_t *pos = reinterpret_cast<int32_t *>(slots + wide), *b = pos + n_tokens;
     const bml_status st =
         g_plan(lens->const_data_ptr<int32_t>(), n_new->const_data_ptr<int32_t>(), owned->const_data_ptr<int32_t>(), (uint32_t)n,
                free->const_data_ptr<int32_t>(), (uint32_t)free->size(0), used->const_data_ptr<int32_t>(), (uint32_t)page,
                (uint32_t)table->size(1), table->mutable_data_ptr<int32_t>(),
                parents ? parents->const_data_ptr<int32_t>() : nullptr, (uint32_t)n_tokens, (uint32_t)words, b, b + n + 1,
-               b + 2 * n + 1, b + 4 * n + 1, slots.mutable_data_ptr<int64_t>(), pos,
-               parents ? reinterpret_cast<uint64_t *>(mask.mutable_data_ptr<int64_t>()) : nullptr, b + 3 * n + 1, stream_of(dev));
+               b + 2 * n + 1, b + 4 * n + 1, slots, pos, parents ? reinterpret_cast<uint64_t *>(slots + n_tokens) : nullptr,
+               b + 3 * n + 1, stream_of(dev));
     USUAL(st == BML_OK);
     PyObject *out = PyTuple_New(8);
     if (!out) return nullptr;
-    const int64_t o = n_tokens;
-    PyTuple_SET_ITEM(out, 0, piece(small, o, n + 1));              // node_start
-    PyTuple_SET_ITEM(out, 1, piece(small, o + n + 1, n));          // kv_lens
-    PyTuple_SET_ITEM(out, 2, piece(small, o + 2 * n + 1, n));      // owned
-    PyTuple_SET_ITEM(out, 3, piece(small, o + 4 * n + 1, 1));      // free_used
-    PyTuple_SET_ITEM(out, 4, piece(small, o + 3 * n + 1, n));      // status
-    PyTuple_SET_ITEM(out, 5, piece(small, 0, n_tokens));           // positions
-    PyTuple_SET_ITEM(out, 6, THPVariable_Wrap(std::move(slots)));
+    static const caffe2::TypeMeta i32 = caffe2::TypeMeta::Make<int32_t>(), i64 = caffe2::TypeMeta::Make<int64_t>();
+    const int64_t p0 = 2 * wide, o = p0 + n_tokens;
+    PyTuple_SET_ITEM(out, 0, piece(all, i32, o, {n + 1}));              // node_start
+    PyTuple_SET_ITEM(out, 1, piece(all, i32, o + n + 1, {n}));          // kv_lens
+    PyTuple_SET_ITEM(out, 2, piece(all, i32, o + 2 * n + 1, {n}));      // owned
+    PyTuple_SET_ITEM(out, 3, piece(all, i32, o + 4 * n + 1, {1}));      // free_used
+    PyTuple_SET_ITEM(out, 4, piece(all, i32, o + 3 * n + 1, {n}));      // status
+    PyTuple_SET_ITEM(out, 5, piece(all, i32, p0, {n_tokens}));          // positions
+    PyTuple_SET_ITEM(out, 6, piece(all, i64, 0, {n_tokens}));           // slots
     if (parents) {
-        PyTuple_SET_ITEM(out, 7, THPVariable_Wrap(std::move(mask)));
+        PyTuple_SET_ITEM(out, 7, piece(all, i64, n_tokens, {n_tokens, words}));
     } else {
         Py_INCREF(Py_None);
         PyTuple_SET_ITEM(out, 7, Py_None);

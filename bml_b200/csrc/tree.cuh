@@ -418,7 +418,7 @@ __device__ __forceinline__ uint32_t tree_see16(const TreeParams &p, const TreeSe
 
 // hi: x rounded to TF32's 10 fraction bits, half away from zero, with integer
 // operations (a conversion instruction runs at a quarter of their rate and set
-// the time: 4 requests of 618 to 2671 positions 85 -> 75 us).  lo: the rest, of
+// tree_f32_kernel's time: 4 requests of 618 to 2671 positions 85 -> 75 us).  lo: the rest, of
 // which the matrix unit takes the upper bits itself.
 __device__ __forceinline__ void tf32_split(float x, uint32_t &hi, uint32_t &lo) {
     hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
