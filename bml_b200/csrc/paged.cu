@@ -77,6 +77,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParam
     const uint32_t i0 = min(threadIdx.x * per, p.n), i1 = min(i0 + per, p.n);
     const int64_t ps = 1ll << p.page_shift;
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int32_t used_now = *p.free_used;  // on its way with the lengths
 
     // A request that is bad takes no pages, and neither does one whose tokens do
     // not fit: that is known only after the scan of the tokens, so in the rare
@@ -113,7 +114,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParam
         before = block_scan(mine, warp_sums, &all);
     }
     int64_t cum = before.y;
-    const int64_t used = min(max(*p.free_used, 0), (int32_t)p.n_free);
+    const int64_t used = min(max(used_now, 0), (int32_t)p.n_free);
     const int64_t avail = (int64_t)p.n_free - used;
     int64_t granted = 0;  // largest running sum that still fits
     at = first_tok;
