@@ -187,47 +187,64 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParam
         }
         int32_t own = s_own[lo];
         int64_t len = p.lens[lo], held = -1, page = 0;  // page: of index held in the request's table
+        const int32_t j0 = (int32_t)first - s_start[lo];
+        if (kRun == 4 && own >= 0 && j0 >= 0 && (int32_t)first + 4 <= s_start[lo + 1]) {
+            // tokens of one request, on one page or two (1.05 M tokens of 512
+            // requests 11.8 -> 9.1 us)
+            auto page_of = [&](uint32_t pg) -> int64_t {
+                return (int64_t)(pg < (uint32_t)own ? p.table[(size_t)lo * p.max_pages + pg] : p.free_pages[s_base[lo] + (pg - own)])
+                       << p.page_shift;
+            };
+            const uint32_t pos = (uint32_t)len + j0, off = pos & ((uint32_t)ps - 1), pg = pos >> p.page_shift;
+            const int64_t a = page_of(pg) + off, b = off + 3 < (uint32_t)ps ? a : page_of(pg + 1) + off - ps;
 #pragma unroll
-        for (uint32_t u = 0; u < kRun; ++u) {
-            const int32_t t = (int32_t)(first + u);
-            slot[u] = -1;
-            rope[u] = 0;
-            uint64_t m[kTreeMaxNodes / 64] = {0, 0, 0, 0};
-            if (t < total) {
-                if (t >= s_start[lo + 1]) {
-                    do ++lo;
-                    while (t >= s_start[lo + 1]);
-                    own = s_own[lo];
-                    len = p.lens[lo];
-                    held = -1;
-                }
-                if (own >= 0) {
-                    const int32_t j = t - s_start[lo];
-                    const int64_t pos = len + j, pg = pos >> p.page_shift;
-                    if (pg != held) {
-                        page = pg < own ? p.table[(size_t)lo * p.max_pages + pg] : p.free_pages[s_base[lo] + (pg - own)];
-                        held = pg;
-                    }
-                    slot[u] = (page << p.page_shift) + (pos & (ps - 1));
-                    rope[u] = (int32_t)pos;
-                    if (p.parents) {
-                        // up the tree; a parent that is not an earlier node ends the walk (a root)
-                        int32_t a = j, depth = 0;
-                        while (true) {
-                            m[a >> 6] |= 1ull << (a & 63);
-                            const int32_t up = p.parents[s_start[lo] + a];
-                            if (up < 0 || up >= a) break;
-                            a = up;
-                            ++depth;
-                        }
-                        rope[u] = (int32_t)len + depth;
-                    }
-                }
+            for (uint32_t u = 0; u < kRun; ++u) {
+                slot[u] = (off + u < (uint32_t)ps ? a : b) + u;
+                rope[u] = (int32_t)(pos + u);
             }
-            if (p.mask && first + u < p.n_tokens)
+        } else {
 #pragma unroll
-                for (uint32_t w = 0; w < kTreeMaxNodes / 64; ++w)
-                    if (w < p.n_words) p.mask[(size_t)t * p.n_words + w] = m[w];
+            for (uint32_t u = 0; u < kRun; ++u) {
+                const int32_t t = (int32_t)(first + u);
+                slot[u] = -1;
+                rope[u] = 0;
+                uint64_t m[kTreeMaxNodes / 64] = {0, 0, 0, 0};
+                if (t < total) {
+                    if (t >= s_start[lo + 1]) {
+                        do ++lo;
+                        while (t >= s_start[lo + 1]);
+                        own = s_own[lo];
+                        len = p.lens[lo];
+                        held = -1;
+                    }
+                    if (own >= 0) {
+                        const int32_t j = t - s_start[lo];
+                        const int64_t pos = len + j, pg = pos >> p.page_shift;
+                        if (pg != held) {
+                            page = pg < own ? p.table[(size_t)lo * p.max_pages + pg] : p.free_pages[s_base[lo] + (pg - own)];
+                            held = pg;
+                        }
+                        slot[u] = (page << p.page_shift) + (pos & (ps - 1));
+                        rope[u] = (int32_t)pos;
+                        if (p.parents) {
+                            // up the tree; a parent that is not an earlier node ends the walk (a root)
+                            int32_t a = j, depth = 0;
+                            while (true) {
+                                m[a >> 6] |= 1ull << (a & 63);
+                                const int32_t up = p.parents[s_start[lo] + a];
+                                if (up < 0 || up >= a) break;
+                                a = up;
+                                ++depth;
+                            }
+                            rope[u] = (int32_t)len + depth;
+                        }
+                    }
+                }
+                if (p.mask && first + u < p.n_tokens)
+#pragma unroll
+                    for (uint32_t w = 0; w < kTreeMaxNodes / 64; ++w)
+                        if (w < p.n_words) p.mask[(size_t)t * p.n_words + w] = m[w];
+            }
         }
         if (kRun == 4 && wide && first + kRun <= p.n_tokens) {
             longlong2 *s2 = reinterpret_cast<longlong2 *>(p.slots + first);

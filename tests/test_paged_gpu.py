@@ -557,6 +557,35 @@ def test_plan_matches_reference(cuda, seed):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("n,page", [(1, 16), (3, 64), (40, 16), (300, 128), (300, 16)])
+def test_plan_of_prompts(cuda, n, page):
+    """Long runs of tokens without drafts: runs that end inside a page or a
+    request, requests of none to three tokens between long ones."""
+    import bml_b200
+    rng = np.random.default_rng(n + page)
+    lens = rng.integers(0, 300, n)
+    new = np.where(rng.random(n) < 0.5, rng.integers(0, 4, n), rng.integers(0, 700, n))
+    own = -(-lens // page) + rng.choice([0, 0, 1, 5], n)
+    need = -(-(lens + new) // page)
+    width = int(max(own.max(), need.max())) + 1
+    pages = rng.permutation(int(own.sum() + np.maximum(need - own, 0).sum()) + 5)
+    table, at = np.full((n, width), -1, np.int64), 0
+    for i in range(n):
+        table[i, :own[i]] = pages[at:at + own[i]]
+        at += own[i]
+    table = ints(table)
+    total = int(new.sum()) + int(rng.integers(0, 9))
+    plan = bml_b200.page_plan(ints(lens), ints(new), ints(own), table, ints(pages), ints([at]), page, total)
+    plan.check()
+    pos = np.concatenate([np.arange(l, l + w) for l, w in zip(lens, new)])
+    who = np.repeat(np.arange(n), new)
+    slots = table.cpu().numpy().astype(np.int64)[who, pos // page] * page + pos % page
+    assert (slots >= 0).all() and len(set(slots.tolist())) == len(slots)
+    pad = total - len(pos)
+    assert plan.slots.tolist() == slots.tolist() + [-1] * pad
+    assert plan.positions.tolist() == pos.tolist() + [0] * pad
+
+
 # ---------------------------------------------------------------------------
 # paged_append
 # ---------------------------------------------------------------------------
