@@ -103,9 +103,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
     const uint32_t pmask = (1u << p.page_shift) - 1;
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const TreeRange range = tree_range(p, &sh, blockIdx.x, gridDim.x);
+    const TreeRange range = tree_range<false>(p, &sh, blockIdx.x, gridDim.x);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge, which waits for this grid
-    TreeWalk walk(range);
+    TreeWalk<false> walk(range);
     TreeSeg sg;
     while (walk.next(p, sg)) {
         // Q fragments, split: [row warp][k-step][hi | lo][lane][4]
@@ -447,14 +447,14 @@ __global__ void __launch_bounds__(kThreads, 2) tree_merge_kernel(const __grid_co
             sg.head = u.head;
             sg.s = u.s;
             sg.row0 = u.rg * p.rpg;
-            b = TreeCuts(p, total, grid).owner(u0) + 1;  // the first cut behind u0
+            b = TreeCuts<true>(p, total, grid).owner(u0) + 1;  // the first cut behind u0
         }
     } else {
         b = blockIdx.x + 1;
-        const TreeRange range = tree_range<true>(p, &sh, b, grid);
+        const TreeRange range = tree_range<true, true>(p, &sh, b, grid);
         mine = range.w0 < range.w1;
         if (mine) {
-            TreeWalk walk(range);
+            TreeWalk<true> walk(range);
             mine = walk.next<true>(p, sg) && sg.t0 > 0;  // else the cut lies between two units
             total = range.total;
             u0 = sg.u0;
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 2) tree_merge_kernel(const __grid_co
     }
     uint32_t last = 0;  // the CTAs with a segment of the unit: b - 1 to last
     if (mine) {
-        const TreeCuts cuts(p, total, grid);
+        const TreeCuts<true> cuts(p, total, grid);
         last = cuts.owner(u0 + (sg.s.tiles - 1) * w);
         mine = last >= b && cuts.at(b - 1) <= u0;  // divided, and no earlier cut inside the unit
         sg.rows = min(p.rpg, sg.s.rows - sg.row0);

@@ -100,8 +100,12 @@ struct TreeSeq {
     uint32_t places;          // of a head
 };
 
-// A tile's weight in a full row group.
-__device__ __forceinline__ uint32_t tree_full_weight(const TreeParams &p) { return p.rpg > p.heavy_rows ? p.heavy : p.light; }
+// A tile's weight in a row group.  kW false: all are 1 (the kernels without
+// weights leave them out, since a launch meets this code cold).
+template <bool kW>
+__device__ __forceinline__ uint32_t tree_weight(const TreeParams &p, uint32_t rows) {
+    return !kW ? 1u : rows > p.heavy_rows ? p.heavy : p.light;
+}
 
 // What the device holds of a request: rows [a, b), positions.
 struct TreeRaw {
@@ -113,6 +117,7 @@ __device__ __forceinline__ TreeRaw tree_raw(const TreeParams &p, uint32_t i) {
     if (kEarly) return {__ldcg(p.node_start + i), __ldcg(p.node_start + i + 1), __ldcg(p.kv_lens + i)};
     return {p.node_start[i], p.node_start[i + 1], p.kv_lens[i]};
 }
+template <bool kW>
 __device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, const TreeRaw &raw) {
     TreeSeq s;
     const int32_t a = raw.a, b = raw.b, L = raw.L;
@@ -125,15 +130,15 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, const TreeRaw &
     s.rows = s.T * p.group;
     s.groups = (s.rows + p.rpg - 1) / p.rpg;
     s.tiles = s.L ? (s.L + p.tile - 1) >> p.tile_shift : 1u;
-    s.w_last = s.rows - (s.groups - 1) * p.rpg > p.heavy_rows ? p.heavy : p.light;
-    s.weight = s.groups ? (s.groups - 1) * tree_full_weight(p) + s.w_last : 0u;
+    s.w_last = tree_weight<kW>(p, s.rows - (s.groups - 1) * p.rpg);
+    s.weight = s.groups ? (s.groups - 1) * tree_weight<kW>(p, p.rpg) + s.w_last : 0u;
     s.places = s.weight * s.tiles + s.groups * p.lead;
     return s;
 }
 
-template <bool kEarly>
+template <bool kEarly, bool kW>
 __device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, uint32_t i) {
-    return tree_seq(p, tree_raw<kEarly>(p, i));
+    return tree_seq<kW>(p, tree_raw<kEarly>(p, i));
 }
 
 struct TreeShared {
@@ -146,10 +151,11 @@ struct TreeShared {
 // tile's weight each: the first `more` take one more than the others.  A tile
 // belongs to the CTA in whose part it begins; a part inside one unit holds at
 // least one beginning.
+template <bool kW>
 struct TreeCuts {
     uint32_t each, more, active;
     __device__ __forceinline__ TreeCuts(const TreeParams &p, uint32_t total, uint32_t grid) {
-        const uint32_t most = p.heavy == 1 ? total : total / p.heavy;
+        const uint32_t most = kW ? total / p.heavy : total;
         active = most < 1 ? (total ? 1u : 0u) : most < grid ? most : grid;
         each = active ? total / active : 0u;
         more = total - each * active;
@@ -178,7 +184,7 @@ struct TreePlace {
     TreeSeq s;
 };
 
-template <bool kEarly, typename Target>
+template <bool kEarly, bool kW, typename Target>
 __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *sh, bool by_unit, Target target) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, upr = p.upr;
     const bool alone = p.n_seqs <= 128;
@@ -193,7 +199,7 @@ __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *
         for (uint32_t k = 0; k < 4; ++k)
             if (i0 + k < i1) {
                 raw[k] = tree_raw<kEarly>(p, i0 + k);
-                const TreeSeq s = tree_seq(p, raw[k]);
+                const TreeSeq s = tree_seq<kW>(p, raw[k]);
                 n4[k] = s.groups * upr;
                 t4[k] = upr * s.places;
                 units += n4[k];
@@ -201,7 +207,7 @@ __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *
             }
     } else {
         for (uint32_t i = i0; i < i1; ++i) {
-            const TreeSeq s = tree_seq<kEarly>(p, i);
+            const TreeSeq s = tree_seq<kEarly, kW>(p, i);
             units += s.groups * upr;
             tiles += upr * s.places;
         }
@@ -252,12 +258,12 @@ __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *
         r.seq = __shfl_sync(0xffffffffu, seq, who & 31);
         r.base = __shfl_sync(0xffffffffu, ft, who & 31);
         r.unit0 = __shfl_sync(0xffffffffu, fu, who & 31);
-        r.s = tree_seq(p, TreeRaw{__shfl_sync(0xffffffffu, raw[0].a, who & 31), __shfl_sync(0xffffffffu, raw[0].b, who & 31),
+        r.s = tree_seq<kW>(p, TreeRaw{__shfl_sync(0xffffffffu, raw[0].a, who & 31), __shfl_sync(0xffffffffu, raw[0].b, who & 31),
                                   __shfl_sync(0xffffffffu, raw[0].L, who & 31)});
     } else {
         if (mine) {
             while (true) {
-                const TreeSeq s = tree_seq<kEarly>(p, seq);
+                const TreeSeq s = tree_seq<kEarly, kW>(p, seq);
                 const uint32_t n = s.groups * upr, t = upr * s.places;
                 if ((by_unit ? w < fu + n : w < ft + t) || seq + 1 >= i1) break;
                 fu += n;
@@ -272,18 +278,18 @@ __device__ __forceinline__ TreePlace tree_find(const TreeParams &p, TreeShared *
         r.seq = sh->seq;
         r.base = sh->base;
         r.unit0 = sh->unit;
-        if (r.seq < p.n_seqs) r.s = tree_seq<kEarly>(p, r.seq);
+        if (r.seq < p.n_seqs) r.s = tree_seq<kEarly, kW>(p, r.seq);
     }
     return r;
 }
 
 // CTA b's range.  w0 == w1: nothing for this CTA.
-template <bool kEarly = false>
+template <bool kW, bool kEarly = false>
 __device__ __forceinline__ TreeRange tree_range(const TreeParams &p, TreeShared *sh, uint32_t b, uint32_t grid) {
     TreeRange r;
     r.w0 = r.w1 = 0;
-    const TreePlace at = tree_find<kEarly>(p, sh, false, [&](uint32_t total) {
-        const TreeCuts cuts(p, total, grid);
+    const TreePlace at = tree_find<kEarly, kW>(p, sh, false, [&](uint32_t total) {
+        const TreeCuts<kW> cuts(p, total, grid);
         if (b < cuts.active) {
             r.w0 = cuts.at(b);
             r.w1 = cuts.at(b + 1);
@@ -307,7 +313,7 @@ struct TreeUnit {
 
 // The unit with index u in line order (for the merge).
 __device__ __forceinline__ TreeUnit tree_unit(const TreeParams &p, TreeShared *sh, uint32_t u) {
-    const TreePlace at = tree_find<true>(p, sh, true, [&](uint32_t) { return u; });
+    const TreePlace at = tree_find<true, true>(p, sh, true, [&](uint32_t) { return u; });
     TreeUnit r = {};
     r.found = u < at.units;
     r.total = at.total;
@@ -317,8 +323,8 @@ __device__ __forceinline__ TreeUnit tree_unit(const TreeParams &p, TreeShared *s
         const uint32_t in = u - at.unit0;
         r.head = in / r.s.groups;
         r.rg = in - r.head * r.s.groups;
-        r.u0 = at.base + r.head * r.s.places + r.rg * (tree_full_weight(p) * r.s.tiles + p.lead) + p.lead;
-        r.w = r.rg + 1 == r.s.groups ? r.s.w_last : tree_full_weight(p);
+        r.u0 = at.base + r.head * r.s.places + r.rg * (tree_weight<true>(p, p.rpg) * r.s.tiles + p.lead) + p.lead;
+        r.w = r.rg + 1 == r.s.groups ? r.s.w_last : tree_weight<true>(p, p.rpg);
         r.head *= p.hpu;
     }
     return r;
@@ -334,6 +340,7 @@ struct TreeSeg {
     TreeSeq s;
 };
 
+template <bool kW>
 struct TreeWalk {
     uint32_t pos, end, base;
     uint32_t seq;
@@ -349,9 +356,9 @@ struct TreeWalk {
                     pos = end;
                     return false;
                 }
-                s = tree_seq<kEarly>(p, seq);
+                s = tree_seq<kEarly, kW>(p, seq);
             }
-            const uint32_t off = pos - base, wf = tree_full_weight(p);
+            const uint32_t off = pos - base, wf = tree_weight<kW>(p, p.rpg);
             const uint32_t head = off / per_head, in_head = off - head * per_head;
             const uint32_t full = wf * s.tiles + p.lead;
             g.rg = s.groups > 1 ? min(in_head / full, s.groups - 1) : 0u;
@@ -359,8 +366,8 @@ struct TreeWalk {
             const uint32_t in = in_head - g.rg * full, left = end - pos;
             const uint32_t out = min(in + left, g.w * s.tiles + p.lead);  // where the range ends in the unit
             const uint32_t ti = max(in, p.lead) - p.lead, to = max(out, p.lead) - p.lead;
-            g.t0 = g.w == 1 ? ti : (ti + g.w - 1) / g.w;
-            g.t1 = g.w == 1 ? to : (to + g.w - 1) / g.w;
+            g.t0 = kW ? (ti + g.w - 1) / g.w : ti;
+            g.t1 = kW ? (to + g.w - 1) / g.w : to;
             g.u0 = pos - in + p.lead;
             pos += out - in;
             if (g.t0 == g.t1) continue;  // no tile begins here

@@ -123,12 +123,12 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
         prefetch_tmap(&fp.tv);
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const TreeRange range = tree_range(p, &sh, blockIdx.x, gridDim.x);
+    const TreeRange range = tree_range<false>(p, &sh, blockIdx.x, gridDim.x);
     __syncthreads();  // the set-up above
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     // ------------------------------------------------------------ copies, ahead
-    TreeWalk fw(range);
+    TreeWalk<false> fw(range);
     TreeSeg fs = {};
     uint32_t f_left = 0, f_pos = 0, f_stage = 0, f_page = 0;
     bool live = true;  // no wait has given up: after that nothing is copied any more
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
         f_stage = f_stage + 1 == (uint32_t)C::NST ? 0 : f_stage + 1;
     };
     auto weight = [](float x) { return kQ32 ? exp2f(x) : fast_exp2(x); };
-    TreeWalk walk(range);
+    TreeWalk<false> walk(range);
     TreeSeg sg = {};
     uint32_t stage = 0, phase = 0;
     bool first = true;

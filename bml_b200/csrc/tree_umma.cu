@@ -263,12 +263,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
     }
     tc_fence_before();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const TreeRange range = tree_range(p, &sh.sched, blockIdx.x, gridDim.x);
+    const TreeRange range = tree_range<true>(p, &sh.sched, blockIdx.x, gridDim.x);
     __syncthreads();  // the set-up above
     tc_fence_after();
     const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may take its place; it waits for this grid
-    TreeWalk walk(range);
+    TreeWalk<true> walk(range);
     TreeSeg sg = {};
 
     if (warp == 0 || warp == 10) {

@@ -207,12 +207,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
     }
     tc_fence_before();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const TreeRange range = tree_range(p, &sh.sched, blockIdx.x, gridDim.x);
+    const TreeRange range = tree_range<false>(p, &sh.sched, blockIdx.x, gridDim.x);
     __syncthreads();  // the set-up above
     tc_fence_after();
     const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge, which waits for this grid
-    TreeWalk walk(range);
+    TreeWalk<false> walk(range);
     TreeSeg sg = {};
     uint32_t it = 0, segs = 0;  // tiles, segments so far
 
@@ -487,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
         constexpr uint32_t kN = kSplitWarps * 32;
         uint32_t total = 0;  // tiles of this CTA
         {
-            TreeWalk w(range);
+            TreeWalk<false> w(range);
             TreeSeg g;
             while (w.next(p, g)) total += g.t1 - g.t0;
         }

@@ -107,11 +107,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
     const uint32_t pmask = (1u << p.page_shift) - 1;
 
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const TreeRange range = tree_range(p, &sh, blockIdx.x, gridDim.x);
+    const TreeRange range = tree_range<false>(p, &sh, blockIdx.x, gridDim.x);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     // ------------------------------------------------------------ copies, ahead
-    TreeWalk fw(range);
+    TreeWalk<false> fw(range);
     TreeSeg fs = {};
     uint32_t f_left = 0, f_pos = 0, f_stage = 0;  // steps left of the segment, the next step's position, its stage
     auto fetch = [&]() {
@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
 #pragma unroll 1
     for (int i = 0; i < C::NST - 1; ++i) fetch();
 
-    TreeWalk walk(range);
+    TreeWalk<false> walk(range);
     TreeSeg sg;
     uint32_t stage = 0;
     while (walk.next(p, sg)) {
