@@ -64,8 +64,8 @@ __device__ __forceinline__ Pair64 block_scan(Pair64 v, Pair64 *warp_sums, Pair64
 constexpr int kPlanThreads = 256;
 
 // kRun: consecutive tokens of a thread.  4 without drafts, where they mostly
-// share a request and a page; 1 with drafts, whose threads walk a tree each
-// (16 drafts, 500 tokens: 6.5 us, 10.3 with 4).
+// share a request and a page (no parents then); 1 with drafts, whose threads
+// walk a tree each (16 drafts, 500 tokens took 1.6 times as long with 4).
 template <uint32_t kRun>
 __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(const PlanParams p) {
     extern __shared__ int32_t sh[];

@@ -9,7 +9,7 @@
 // again, says what is wrong, or makes the call.  A refused C call has launched
 // nothing.  The entry points of libbmlattn.so are handed over by set_calls().
 //
-// Host time of a call beside a B200, against the way through ctypes: page_plan 7
+// Host time of a call beside a B200, against the way through ctypes: page_plan 5.3
 // and 20 us, paged_append 3.3 and 10, tree_attention (two launches) 7.1 and 16.5,
 // paged_commit 4.2 and 12.
 #include <ATen/ATen.h>
