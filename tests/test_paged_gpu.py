@@ -375,6 +375,35 @@ def test_streams_and_graphs(cuda, qt, ct):
     assert torch.equal(outs[0], bml_b200.tree_attention(c.q, c.k, c.v, c.table, c.kv_lens, c.start))
 
 
+@pytest.mark.parametrize("d", [64, 128])
+def test_wide_f32_on_streams(cuda, d):
+    """32-bit pages with many rows: two graphs replayed on two streams at once,
+    one behind the other's plan-like writes of its lengths."""
+    import bml_b200
+    cs = [Paged([2000, 10, 700] * 5, [20, 8, 30] * 5, 8, 2, d, 16, "f32", "f32", seed=s) for s in (22, 23)]
+    want = [bml_b200.tree_attention(c.q, c.k, c.v, c.table, c.kv_lens, c.start) for c in cs]
+    check(cs[0], want[0], [chain(t, p) for t, p in zip(cs[0].nodes, cs[0].lens)], "f32")
+    full = [c.kv_lens.clone() for c in cs]
+    graphs, outs = [], []
+    for c, f in zip(cs, full):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            c.kv_lens.zero_()
+            bml_b200.tree_attention(c.q, c.k, c.v, c.table, c.kv_lens, c.start)
+            c.kv_lens.copy_(f)
+            outs.append(bml_b200.tree_attention(c.q, c.k, c.v, c.table, c.kv_lens, c.start))
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert torch.equal(o, w)
+
+
 @pytest.mark.parametrize("qt,ct", TYPES)
 def test_uneven_batches(cuda, qt, ct):
     """Batches whose average picks a kernel for few rows, with requests of many
