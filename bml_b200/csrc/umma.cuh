@@ -164,13 +164,12 @@ __host__ __device__ constexpr uint32_t make_idesc(uint32_t in_fmt, uint32_t m, u
 // 2^n added to the exponent field as an integer.  Arguments below -120
 // (masked keys are -inf) give 2^-120 instead of 0: ~1e-36 of a row sum of
 // at least 1.
-// kNan: an argument that is NaN gives NaN (without it, a finite number).
-template <bool kNan = false>
+// kExact: below -120 exactly 0, so that a masked place adds nothing whatever V
+// holds there (2^-120 is a normal number in bf16: times 3e38 it is 226), and an
+// argument that is NaN gives NaN (without it, a finite number).
+template <bool kExact = false>
 __device__ __forceinline__ float2 exp2_poly_pair(float2 e) {
-    if (kNan) {
-        asm("max.NaN.f32 %0, %0, 0fC2F00000;" : "+f"(e.x));  // -120
-        asm("max.NaN.f32 %0, %0, 0fC2F00000;" : "+f"(e.y));
-    } else {
+    if (!kExact) {
         e.x = fmaxf(e.x, -120.f);
         e.y = fmaxf(e.y, -120.f);
     }
@@ -182,7 +181,11 @@ __device__ __forceinline__ float2 exp2_poly_pair(float2 e) {
     q = __ffma2_rn(f, q, make_float2(0.99992895f, 0.99992895f));
     q.x = __int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23));
     q.y = __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23));
-    if (kNan) q = __ffma2_rn(e, make_float2(0.f, 0.f), q);
+    if (kExact) {
+        q = __ffma2_rn(e, make_float2(0.f, 0.f), q);
+        if (e.x < -120.f) q.x = 0.f;
+        if (e.y < -120.f) q.y = 0.f;
+    }
     return q;
 }
 
