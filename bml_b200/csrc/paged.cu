@@ -495,7 +495,8 @@ __global__ void __launch_bounds__(kCommitThreads) paged_commit_kernel(const Comm
 cudaError_t launch_page_plan(const PlanParams &p, cudaStream_t st) {
     const size_t smem = (3 * (size_t)p.n + 1) * sizeof(int32_t);  // at most 49,156 B for kPlanMaxSeqs
     auto kern = p.parents ? page_plan_kernel<1> : page_plan_kernel<4>;
-    if (smem > 48 * 1024) {
+    // without the allowance the dynamic and the static part (warp_sums) together have 48 KB
+    if (smem + kPlanThreads / 32 * sizeof(Pair64) > 48 * 1024) {
         cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 64 * 1024);
         if (e != cudaSuccess) return e;
     }
