@@ -134,6 +134,8 @@ SIGNATURES = {
                                       _vp, _vp, _sz, _vp]),
     "bml_kvsplit_destroy": (_st, [_vp]),
     # include/bml_diag.h (test-only)
+    "bml_diag_attn_tree": (_st, [_vp, C.c_int, _u32, _u32, _u32, _u32, _vp, _vp, C.c_int, _u32, _u32, _vp, _u32, _vp,
+                                 _vp, _u32, _vp, _u32, C.c_float, _vp, _vp, _sz, C.c_uint64, _u32, _vp]),
     "bml_diag_exp2": (_st, [_vp, _u32, _vp, _vp]),
     "bml_diag_decode_batched": (_st, [C.POINTER(bml_seq_desc), _u32, _u32, _u32, _u32, C.c_int,
                                       C.c_float, _vp, _vp, _vp, _sz, C.c_int, C.c_uint64, _u32, _vp]),

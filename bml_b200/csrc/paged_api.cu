@@ -7,6 +7,7 @@
 #include <atomic>
 #include <initializer_list>
 
+#include "../../include/bml_diag.h"
 #include "tree.cuh"
 
 #define BML_API extern "C" __attribute__((visibility("default")))
@@ -192,13 +193,15 @@ BML_API bml_status bml_attn_tree_workspace_size(uint32_t head_dim, int32_t devic
     return bml::api_ok();
 }
 
-BML_API bml_status bml_attn_tree(const void *q_dev, bml_dtype q_dtype, uint32_t n_tokens, uint32_t n_heads,
-                                 uint32_t n_kv_heads, uint32_t head_dim, const void *k_pool, const void *v_pool,
-                                 bml_dtype kv_dtype, uint32_t n_pages, uint32_t page_size, const int32_t *block_table,
-                                 uint32_t max_pages, const int32_t *kv_lens, const int32_t *node_start, uint32_t n_seqs,
-                                 const uint64_t *mask, uint32_t n_words, float scale, void *out_dev, void *workspace,
-                                 size_t workspace_bytes, void *stream) {
-    const char *fn = "bml_attn_tree";
+namespace {
+
+// What bml_attn_tree takes, and what only tests set.
+bml_status attn_tree(const char *fn, const void *q_dev, bml_dtype q_dtype, uint32_t n_tokens, uint32_t n_heads,
+                     uint32_t n_kv_heads, uint32_t head_dim, const void *k_pool, const void *v_pool, bml_dtype kv_dtype,
+                     uint32_t n_pages, uint32_t page_size, const int32_t *block_table, uint32_t max_pages,
+                     const int32_t *kv_lens, const int32_t *node_start, uint32_t n_seqs, const uint64_t *mask,
+                     uint32_t n_words, float scale, void *out_dev, void *workspace, size_t workspace_bytes,
+                     uint64_t wait_ns, uint32_t diag, void *stream) {
     if (!valid_dtype(q_dtype) || !valid_dtype(kv_dtype)) return api_fail(BML_E_INVALID, "%s: unknown dtype", fn);
     if (q_dtype != BML_F32 && q_dtype != kv_dtype)
         return api_fail(BML_E_UNSUPPORTED, "%s: 16-bit queries need pages of their own type", fn);
@@ -248,6 +251,8 @@ BML_API bml_status bml_attn_tree(const void *q_dev, bml_dtype q_dtype, uint32_t 
     p.scale_log2 = (float)(sc * 1.4426950408889634);
     p.q_type = q_dtype;
     p.part = static_cast<float *>(workspace);
+    p.wait_ns = wait_ns;
+    p.diag = diag;
     for (uint32_t base = 0; base < n_seqs; base += bml::kTreeMaxSeqs) {
         p.n_seqs = n_seqs - base < bml::kTreeMaxSeqs ? n_seqs - base : bml::kTreeMaxSeqs;
         p.table = block_table + (size_t)base * max_pages;
@@ -257,6 +262,32 @@ BML_API bml_status bml_attn_tree(const void *q_dev, bml_dtype q_dtype, uint32_t 
         if (e != cudaSuccess) return bml::api_cuda_fail(e, fn);
     }
     return bml::api_ok();
+}
+
+}  // namespace
+
+BML_API bml_status bml_attn_tree(const void *q_dev, bml_dtype q_dtype, uint32_t n_tokens, uint32_t n_heads,
+                                 uint32_t n_kv_heads, uint32_t head_dim, const void *k_pool, const void *v_pool,
+                                 bml_dtype kv_dtype, uint32_t n_pages, uint32_t page_size, const int32_t *block_table,
+                                 uint32_t max_pages, const int32_t *kv_lens, const int32_t *node_start, uint32_t n_seqs,
+                                 const uint64_t *mask, uint32_t n_words, float scale, void *out_dev, void *workspace,
+                                 size_t workspace_bytes, void *stream) {
+    return attn_tree("bml_attn_tree", q_dev, q_dtype, n_tokens, n_heads, n_kv_heads, head_dim, k_pool, v_pool, kv_dtype, n_pages,
+                     page_size, block_table, max_pages, kv_lens, node_start, n_seqs, mask, n_words, scale, out_dev, workspace,
+                     workspace_bytes, bml::kWaitNs, 0u, stream);
+}
+
+BML_API bml_status bml_diag_attn_tree(const void *q_dev, bml_dtype q_dtype, uint32_t n_tokens, uint32_t n_heads,
+                                      uint32_t n_kv_heads, uint32_t head_dim, const void *k_pool, const void *v_pool,
+                                      bml_dtype kv_dtype, uint32_t n_pages, uint32_t page_size, const int32_t *block_table,
+                                      uint32_t max_pages, const int32_t *kv_lens, const int32_t *node_start, uint32_t n_seqs,
+                                      const uint64_t *mask, uint32_t n_words, float scale, void *out_dev, void *workspace,
+                                      size_t workspace_bytes, uint64_t wait_ns, uint32_t flags, void *stream) {
+    const char *fn = "bml_diag_attn_tree";
+    if (flags & ~BML_DIAG_STALL) return api_fail(BML_E_INVALID, "%s: flags 0x%x", fn, flags);
+    return attn_tree(fn, q_dev, q_dtype, n_tokens, n_heads, n_kv_heads, head_dim, k_pool, v_pool, kv_dtype, n_pages, page_size,
+                     block_table, max_pages, kv_lens, node_start, n_seqs, mask, n_words, scale, out_dev, workspace, workspace_bytes,
+                     wait_ns ? wait_ns : bml::kWaitNs, (flags & BML_DIAG_STALL) ? bml::kTreeStall : 0u, stream);
 }
 
 BML_API bml_status bml_paged_commit(void *k_pool, void *v_pool, uint32_t n_layers, uint32_t n_pages, uint32_t page_size,

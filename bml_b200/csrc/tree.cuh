@@ -31,7 +31,13 @@ struct TreeParams {
     // a tile's weight: heavy with more rows than heavy_rows, else light
     uint32_t heavy_rows, heavy, light;
     uint32_t lead;  // places ahead of a unit's first tile: what its start and end cost
+    uint64_t wait_ns;  // limit of every bounded wait
+    uint32_t diag;     // kTreeStall, 0 outside tests
 };
+
+// Test-only behaviour (bml_diag_attn_tree): nothing is copied (tree_umma.cu: no
+// Q and K), so that the waits for it run out.
+constexpr uint32_t kTreeStall = 1u;
 
 struct TreeArgs {
     TreeParams p;
@@ -395,6 +401,30 @@ __device__ __forceinline__ float *tree_part(const TreeParams &p, uint32_t D, uin
 __device__ __forceinline__ size_t tree_row(const TreeParams &p, const TreeSeg &g, uint32_t r, uint32_t D, uint32_t h = 0) {
     const uint32_t t = r / p.group, qg = r - t * p.group;
     return ((size_t)(g.s.first + t) * p.n_heads + (size_t)(g.head + h) * p.group + qg) * D;
+}
+
+// A wait of the CTA gave up: NaN in the rows of all its segments (in the sums of
+// those that the merge joins), which covers segments that nobody has begun.
+// Out of line, for every thread of the CTA; 16-bit results.
+template <bool kW>
+__device__ __noinline__ void tree_give_up(const TreeParams &p, TreeShared *sh, uint32_t D) {
+    const TreeRange range = tree_range<kW>(p, sh, blockIdx.x, gridDim.x);
+    TreeWalk<kW> walk(range);
+    TreeSeg g;
+    while (walk.next(p, g)) {
+        const uint32_t R = p.rpg * p.hpu;
+        float *part = g.slot < 2 ? tree_part(p, D, blockIdx.x, g.slot) : nullptr;
+        for (uint32_t i = threadIdx.x; i < g.rows * p.hpu; i += blockDim.x) {
+            const uint32_t h = i / g.rows, r = i - h * g.rows;
+            if (part) {
+                part[(size_t)R * D + h * p.rpg + r] = 0.f;
+                part[(size_t)R * (D + 1) + h * p.rpg + r] = __int_as_float(0x7fffffff);
+            } else {
+                uint4 *out = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.out) + tree_row(p, g, g.row0 + r, D, h));
+                for (uint32_t u = 0; u < D / 8; ++u) out[u] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+            }
+        }
+    }
 }
 
 // Whether node t of a request sees position pos >= P (= node pos - P).

@@ -74,24 +74,6 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&t)[TERMS
     }
 }
 
-// Waits for a copy, bounded: false (and the CTA's flag set) after kWaitNs.
-__device__ __forceinline__ bool copy_wait(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag) {
-    if (mbar_test_wait(bar, parity)) return true;
-    uint64_t t0 = 0;
-    while (true) {
-#pragma unroll 1
-        for (int i = 0; i < 256; ++i)
-            if (mbar_try_wait(bar, parity)) return true;
-        if (*abort_flag) return false;
-        const uint64_t t = globaltimer_ns();
-        if (t0 == 0) t0 = t;
-        if (t - t0 > kWaitNs) {
-            *abort_flag = 1u;
-            return false;
-        }
-    }
-}
-
 template <int D, bool kF16, bool kQ32>
 __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kernel(const __grid_constant__ FewParams fp) {
     using C = NCfg<D, kF16, kQ32>;
@@ -131,7 +113,7 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
     TreeWalk<false> fw(range);
     TreeSeg fs = {};
     uint32_t f_left = 0, f_pos = 0, f_stage = 0, f_page = 0;
-    bool live = true;  // no wait has given up: after that nothing is copied any more
+    bool live = !(p.diag & kTreeStall);  // no wait has given up: after that nothing is copied any more
     const int32_t *f_table = nullptr;
     auto page_at = [&](uint32_t pos) { return pos < fs.s.L ? (uint32_t)f_table[pos >> p.page_shift] : 0xffffffffu; };
     auto fetch = [&]() {
@@ -228,7 +210,7 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
 
 #pragma unroll 1
         for (uint32_t k = sg.t0; k < sg.t1; ++k) {
-            if (!copy_wait(&full[stage], phase, abort_flag)) live = false;
+            if (!wait_bar(&full[stage], phase, abort_flag, p.wait_ns)) live = false;
             __syncwarp();  // and every lane has left the stage that fetch() fills
             fetch();
             const uint32_t base = k * p.tile + split * 16, st = stage;

@@ -71,25 +71,6 @@ struct UmmaParams {
     uint32_t box_rows;  // min(page, 128)
 };
 
-// mbar_wait that looks at the clock only once in 256 tries: reading
-// %globaltimer takes longer than most of these waits.
-__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag) {
-    if (mbar_test_wait(bar, parity)) return true;
-    uint64_t t0 = 0;
-    while (true) {
-#pragma unroll 1
-        for (int i = 0; i < 256; ++i)
-            if (mbar_try_wait(bar, parity)) return true;
-        if (*abort_flag) return false;
-        const uint64_t t = globaltimer_ns();
-        if (t0 == 0) t0 = t;
-        if (t - t0 > kWaitNs) {
-            *abort_flag = 1u;
-            return false;
-        }
-    }
-}
-
 // One segment, as the softmax warps read it.
 struct Board {
     uint32_t seq, first, T, L, head, row0, t0;
@@ -283,9 +264,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
         const uint32_t per_tile = BN / up.box_rows, part = lane / C::KB, kb = lane % C::KB;
         const uint32_t ps_mask = (1u << p.page_shift) - 1;
         const bool mine = part < per_tile;
-        bool live = true;
+        bool live = !(is_k && (p.diag & kTreeStall));
         auto wait_all = [&](uint64_t *bar, uint32_t parity) {
-            live = live && __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag));
+            live = live && __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag, p.wait_ns));
         };
         auto index = [&](bool pair, uint32_t j, uint32_t n) { return is_k ? k_index(pair, j) : v_index(pair, j, n); };
         auto advance = [&](uint32_t by) {  // at most 3
@@ -422,8 +403,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
         auto gate_wait = [&](const Gate &g, bool ready) {
             if (!ready) {
                 bool ok = true;
-                if (g.b0) ok = wait_bar(g.b0, g.p0, abort_flag);
-                if (g.b1) ok = wait_bar(g.b1, g.p1, abort_flag) && ok;
+                if (g.b0) ok = wait_bar(g.b0, g.p0, abort_flag, p.wait_ns);
+                if (g.b1) ok = wait_bar(g.b1, g.p1, abort_flag, p.wait_ns) && ok;
                 live = live && __all_sync(0xffffffffu, ok);
             }
             __syncwarp();
@@ -560,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
         }
         if (elect_one()) tc_commit(&sh.drain);  // no MMA outlives the CTA
         __syncwarp();
-        mbar_drain(&sh.drain, 0, kWaitNs);
+        mbar_drain(&sh.drain, 0, p.wait_ns);
         __syncwarp();
     } else {
         // ------------------------------------------------------------- softmax
@@ -575,10 +556,14 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
         uint32_t finals = 0;  // bit x: phase parity of o_final[x]
         while (true) {
             // not cut short by the abort flag: the V producer's own waits are
-            // bounded, and it always publishes an end
+            // bounded, and it always publishes an end; segments behind it (a wait
+            // gave up) are tree_give_up's
             uint64_t *seg = &sh.seg_full[segs % kBoard];
             const uint32_t seg_phase = (segs / kBoard) & 1u;
-            if (!mbar_test_wait(seg, seg_phase) && !mbar_drain(seg, seg_phase, 8 * kWaitNs)) break;
+            if (!mbar_test_wait(seg, seg_phase) && !mbar_drain(seg, seg_phase, 8 * p.wait_ns)) {
+                *abort_flag = 1u;
+                break;
+            }
             __syncwarp();
             const volatile Board *b = &sh.board[segs % kBoard];
             const uint32_t packed = b->packed, n = packed & 0xfffffffu, slot_of = packed >> 28 & 7u;
@@ -595,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
             for (uint32_t i = 0; i < nt; ++i) {
                 const uint32_t j = pair ? i : 2 * i + x;
                 const uint32_t kv0 = kv_first + j * BN;
-                wait_bar(&sh.s_full[x], (done + i) & 1u, abort_flag);
+                wait_bar(&sh.s_full[x], (done + i) & 1u, abort_flag, p.wait_ns);
                 __syncwarp();
                 tc_fence_after();
                 const uint32_t bad = *(volatile uint32_t *)&sh.bad[(tiles + j) % kBadRing];
@@ -605,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
                     // V rows that must not be read as they are: this thread's row is kv0 + r
                     const uint32_t pos = kv0 + r, cv = cnt + v_index(pair, j, n), slot = cv % C::SLOTS;
                     if (__any_sync(0xffffffffu, pos >= P)) {
-                        wait_bar(&sh.full[slot], (cv / C::SLOTS) & 1u, abort_flag);
+                        wait_bar(&sh.full[slot], (cv / C::SLOTS) & 1u, abort_flag, p.wait_ns);
                         fix_v<C::KB, kF16>(ring + slot * C::TILE + r * 128, pos >= P, pos >= b->L, pos - P, sh.odd);
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     }
@@ -703,13 +688,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
             // writes columns x * D / 2 .. of the joined row.
             float wa, wb, m = m_run, l = l_run;
             if (pair) {
-                wait_bar(&sh.o_final[x], (finals >> x) & 1u, abort_flag);
+                wait_bar(&sh.o_final[x], (finals >> x) & 1u, abort_flag, p.wait_ns);
                 wa = m_run == -INFINITY ? 0.f : 1.f;
                 wb = 0.f;
             } else {
                 sh.ml[x * 128 + r] = make_float2(m_run, l_run);
-                wait_bar(&sh.o_final[0], finals & 1u, abort_flag);
-                if (n > 1) wait_bar(&sh.o_final[1], finals >> 1 & 1u, abort_flag);
+                wait_bar(&sh.o_final[0], finals & 1u, abort_flag, p.wait_ns);
+                if (n > 1) wait_bar(&sh.o_final[1], finals >> 1 & 1u, abort_flag, p.wait_ns);
                 __syncwarp();
                 named_bar_sync(1, 256);
                 const float2 ma = sh.ml[r], mb = sh.ml[128 + r];
@@ -799,6 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
 
     tc_fence_before();
     __syncthreads();
+    if (*abort_flag) tree_give_up<true>(p, &sh.sched, D);
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS) : "memory");

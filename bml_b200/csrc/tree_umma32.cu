@@ -90,24 +90,6 @@ struct alignas(16) XShared {
 };
 static_assert(sizeof(XShared) <= 3 * 1024, "small arrays");
 
-// Bounded wait that looks at the clock once in 256 tries.
-__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag) {
-    if (mbar_test_wait(bar, parity)) return true;
-    uint64_t t0 = 0;
-    while (true) {
-#pragma unroll 1
-        for (int i = 0; i < 256; ++i)
-            if (mbar_try_wait(bar, parity)) return true;
-        if (*abort_flag) return false;
-        const uint64_t t = globaltimer_ns();
-        if (t0 == 0) t0 = t;
-        if (t - t0 > kWaitNs) {
-            *abort_flag = 1u;
-            return false;
-        }
-    }
-}
-
 // D[tmem] (+)= A[tmem] * B[smem desc], TF32: A is M x 8, 8 columns.
 __device__ __forceinline__ void mma_tf32_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
@@ -225,7 +207,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
         const bool is_k = lane < 16;
         const uint32_t part = is_k ? lane / C::KB : lane - 16, kb = is_k ? lane % C::KB : 0u;
         const bool mine = part < parts && lane < 20;
-        bool live = true;
+        bool live = !(p.diag & kTreeStall);
         while (live && walk.next(p, sg)) {
             const int32_t *table = p.table + (size_t)sg.seq * p.max_pages;
             // a lane's first row in the pool of tile j (-1: past the length, -2: a page outside the pool)
@@ -258,10 +240,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
                     }
                     __syncwarp();
                 };
-                if (use > 0) live = __all_sync(0xffffffffu, wait_bar(&sh.k_empty[st], (use & 1u) ^ 1u, abort_flag));
+                if (use > 0) live = __all_sync(0xffffffffu, wait_bar(&sh.k_empty[st], (use & 1u) ^ 1u, abort_flag, p.wait_ns));
                 if (!live) break;
                 copy(true, &sh.k_full[st], smem + C::OFF_K + st * 2 * C::TILE + kb * 2 * BN * 128 + part * xp.box_rows * 128);
-                if (it > 0) live = __all_sync(0xffffffffu, wait_bar(&sh.v_empty, (it & 1u) ^ 1u, abort_flag));
+                if (it > 0) live = __all_sync(0xffffffffu, wait_bar(&sh.v_empty, (it & 1u) ^ 1u, abort_flag, p.wait_ns));
                 if (!live) break;
                 copy(false, &sh.v_full, smem + C::OFF_V + part * xp.box_rows * D * 4);
             }
@@ -282,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
         const uint64_t d_vhi = smem_desc(smem_u32(smem + C::OFF_VHI), 16, 1024), d_vlo = smem_desc(smem_u32(smem + C::OFF_VLO), 16, 1024);
         bool live = true;
         auto wait_all = [&](uint64_t *bar, uint32_t parity) {
-            live = live && __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag));
+            live = live && __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag, p.wait_ns));
             __syncwarp();
             tc_fence_after();
         };
@@ -322,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
         }
         if (elect_one()) tc_commit(&sh.drain);  // no MMA outlives the CTA
         __syncwarp();
-        mbar_drain(&sh.drain, 0, kWaitNs);
+        mbar_drain(&sh.drain, 0, p.wait_ns);
         __syncwarp();
     } else if (warp < 2 + kRowWarps) {
         // ---------------------------------------------------------- Q and softmax
@@ -356,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
 #pragma unroll
             for (int k = 0; k < D / 2; ++k) o[k] = 0.f;
             for (uint32_t j = sg.t0; j < sg.t1; ++j, ++it) {
-                wait_bar(&sh.s_full, it & 1u, abort_flag);
+                wait_bar(&sh.s_full, it & 1u, abort_flag, p.wait_ns);
                 __syncwarp();
                 tc_fence_after();
                 float alpha = 1.f;
@@ -415,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.p_ready);
-                wait_bar(&sh.o_full, it & 1u, abort_flag);
+                wait_bar(&sh.o_full, it & 1u, abort_flag, p.wait_ns);
                 __syncwarp();
                 tc_fence_after();
                 if (warp_live)
@@ -492,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
             while (w.next(p, g)) total += g.t1 - g.t0;
         }
         auto split_k = [&](uint32_t i) {
-            wait_bar(&sh.k_full[i & 1u], (i >> 1) & 1u, abort_flag);
+            wait_bar(&sh.k_full[i & 1u], (i >> 1) & 1u, abort_flag, p.wait_ns);
             __syncwarp();
             uint4 *k = reinterpret_cast<uint4 *>(smem + C::OFF_K + (i & 1u) * 2 * C::TILE);
 #pragma unroll 4
@@ -518,8 +500,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
             uint32_t *odd = sh.odd[segs % 3];
             for (uint32_t j = sg.t0; j < sg.t1; ++j, ++it) {
                 // V(it) transposed: thread = 4 positions of one column
-                wait_bar(&sh.v_full, it & 1u, abort_flag);
-                if (it > 0) wait_bar(&sh.o_full, (it & 1u) ^ 1u, abort_flag);  // the last tile's V has been read
+                wait_bar(&sh.v_full, it & 1u, abort_flag, p.wait_ns);
+                if (it > 0) wait_bar(&sh.o_full, (it & 1u) ^ 1u, abort_flag, p.wait_ns);  // the last tile's V has been read
                 __syncwarp();
                 // read two segments ago: the rows' warps have since been through a tile of the last one
                 if (j == sg.t0 && cw == 0 && lane < 8) sh.odd[(segs + 1) % 3][lane] = 0u;

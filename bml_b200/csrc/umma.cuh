@@ -1,5 +1,5 @@
 // umma.cuh -- tcgen05, tensor-memory and TMA helpers of the tensor-core
-// attention kernels (prefill.cu, tree_umma.cu).
+// attention kernels (prefill.cu, tree_umma.cu, tree_umma32.cu, tree_few.cu).
 #pragma once
 
 #include <cudaTypedefs.h>
@@ -29,6 +29,26 @@ __device__ __forceinline__ void tma_load_3d_hint(void *dst, const CUtensorMap *m
         " [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(smem_u32(dst)),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar)), "l"(policy)
         : "memory");
+}
+
+// mbar_wait that looks at the clock only once in 256 tries: reading
+// %globaltimer takes longer than most of these waits.  false (and the CTA's
+// flag set) after limit_ns, or once another wait has given up.
+__device__ __forceinline__ bool wait_bar(uint64_t *bar, uint32_t parity, volatile uint32_t *abort_flag, uint64_t limit_ns) {
+    if (mbar_test_wait(bar, parity)) return true;
+    uint64_t t0 = 0;
+    while (true) {
+#pragma unroll 1
+        for (int i = 0; i < 256; ++i)
+            if (mbar_try_wait(bar, parity)) return true;
+        if (*abort_flag) return false;
+        const uint64_t t = globaltimer_ns();
+        if (t0 == 0) t0 = t;
+        if (t - t0 > limit_ns) {
+            *abort_flag = 1u;
+            return false;
+        }
+    }
 }
 
 __device__ __forceinline__ void prefetch_tmap(const CUtensorMap *map) {
