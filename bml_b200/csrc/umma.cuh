@@ -184,7 +184,7 @@ __host__ __device__ constexpr uint32_t make_idesc(uint32_t in_fmt, uint32_t m, u
 // 2^n added to the exponent field as an integer.  Arguments below -120
 // (masked keys are -inf) give 2^-120 instead of 0: ~1e-36 of a row sum of
 // at least 1.
-// kExact: below -120 exactly 0, so that a masked place adds nothing whatever V
+// kExact: below -125 exactly 0, so that a masked place adds nothing whatever V
 // holds there (2^-120 is a normal number in bf16: times 3e38 it is 226), and an
 // argument that is NaN gives NaN (without it, a finite number).
 template <bool kExact = false>
@@ -202,9 +202,10 @@ __device__ __forceinline__ float2 exp2_poly_pair(float2 e) {
     q.x = __int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23));
     q.y = __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23));
     if (kExact) {
-        q = __ffma2_rn(e, make_float2(0.f, 0.f), q);
-        if (e.x < -120.f) q.x = 0.f;
-        if (e.y < -120.f) q.y = 0.f;
+        q.x = e.x < -125.f ? 0.f : q.x;
+        q.y = e.y < -125.f ? 0.f : q.y;
+        q.x = e.x == e.x ? q.x : e.x;
+        q.y = e.y == e.y ? q.y : e.y;
     }
     return q;
 }
