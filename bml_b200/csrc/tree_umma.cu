@@ -657,6 +657,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
                             }
                             sum4[(k >> 1) & 3] = __fadd2_rn(sum4[(k >> 1) & 3], e);
                             w[k >> 1] = pack2<kF16>(e.x, e.y);
+                            if (!kF16 && ((k >> 1) & 7) == 7) w[k >> 1] = drop_tiny(w[k >> 1]);
                         }
                         tmem_st16(s_col + qc * 16, w);
                     }
