@@ -122,8 +122,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
                     x0 = load_q(p.q, p.q_type, at);
                     x1 = load_q(p.q, p.q_type, at + 1);
                 }
-                tf32_split(x0, hi[h8], lo[h8]);
-                tf32_split(x1, hi[h8 + 2], lo[h8 + 2]);
+                tf32_split_any(x0, hi[h8], lo[h8]);
+                tf32_split_any(x1, hi[h8 + 2], lo[h8 + 2]);
             }
             uint4 *dst = reinterpret_cast<uint4 *>(sQ) + ((size_t)(w * (D / 8) + ks) * 2) * 32 + l;
             dst[0] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
@@ -164,6 +164,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // rows g and g + 8; l: this lane's share
+        bool odd = false;  // a node has values taken as zeros
         const uint32_t r0 = sg.row0 + rw * 16 + g, r1 = r0 + 8;
         const uint32_t t0 = r0 / p.group, t1 = r1 / p.group;
         const bool v0 = r0 < sg.row0 + sg.rows, v1 = r1 < sg.row0 + sg.rows;
@@ -215,8 +216,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
                             for (int kk = 0; kk < 2; ++kk) {
                                 uint32_t b0, b1, e0 = 0, e1 = 0;
                                 if (kF32) {
-                                    tf32_split(y[2 * kk], b0, e0);
-                                    tf32_split(y[2 * kk + 1], b1, e1);
+                                    tf32_split_any(y[2 * kk], b0, e0);
+                                    tf32_split_any(y[2 * kk + 1], b1, e1);
                                 } else {
                                     b0 = __float_as_uint(y[2 * kk]);
                                     b1 = __float_as_uint(y[2 * kk + 1]);
@@ -282,7 +283,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
                 // P as the A operand: k index c is position 2c, c + 4 is 2c + 1.  The
                 // matrix unit's accumulation truncates, so the NB blocks are summed
                 // apart and added to O with a rounding.
-                bool odd = false;  // a V value that is not finite: 0 * it must not reach rows that do not see it
+                // A node's V value that is not finite is taken as zero: 0 * it must not
+                // reach rows that do not see it (tree_nonfinite adds it to the others).
 #pragma unroll
                 for (int s = 0; s < NT / VE; ++s) {
                     float y[VE][4];
@@ -310,8 +312,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
                         for (int e = 0; e < VE; ++e) {
                             uint32_t b0, b1, e0 = 0, e1 = 0;
                             if (kF32) {
-                                tf32_split(y0[e], b0, e0);
-                                tf32_split(y1[e], b1, e1);
+                                tf32_split_any(y0[e], b0, e0);
+                                tf32_split_any(y1[e], b1, e1);
                             } else {
                                 b0 = __float_as_uint(y0[e]);
                                 b1 = __float_as_uint(y1[e]);
@@ -326,33 +328,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
 #pragma unroll
                         for (int z = 0; z < 4; ++z) o[s * VE + e][z] += y[e][z];
                 }
-                if (edge && __any_sync(0xffffffffu, odd)) {
-                    // rare: the values that were taken as zero above, added for the rows that see them
-#pragma unroll 1
-                    for (int q = 0; q < NB * 8; ++q) {
-                        const int src = (lane & ~3) | ((q & 7) >> 1);
-                        float y0 = 0.f, y1 = 0.f;
-#pragma unroll
-                        for (int n = 0; n < NB; ++n)
-                            if (n == q >> 3) {
-                                y0 = (q & 1) ? s0[n][1] : s0[n][0];
-                                y1 = (q & 1) ? s0[n][3] : s0[n][2];
-                            }
-                        const float w0 = __shfl_sync(0xffffffffu, y0, src), w1 = __shfl_sync(0xffffffffu, y1, src);
-                        const uint8_t *vr = sv + (n0 * 8 + q) * C::VS;
-#pragma unroll
-                        for (int j = 0; j < NT; ++j)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int dim = (j / VE) * 8 * VE + VE * (2 * c + e) + j % VE;
-                                const float y = load_q(vr, Elem<KT>::kCode, dim);
-                                if (!(fabsf(y) < INFINITY)) {
-                                    if (w0 > 0.f) o[j][e] += w0 * y;
-                                    if (w1 > 0.f) o[j][2 + e] += w1 * y;
-                                }
-                            }
-                    }
-                }
             }
         }
         cp_wait<0>();
@@ -360,6 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
         l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
         l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+        odd = __any_sync(0xffffffffu, odd);
         __syncthreads();  // the ring is free: [warp][16 rows][D + m + l], in groups' order
         constexpr int OS = D + 4;
         float *mine = reinterpret_cast<float *>(ring) + (size_t)warp * 16 * OS;
@@ -373,9 +349,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
             }
         if (c == 0) {
             mine[g * OS + D] = m0;
-            mine[g * OS + D + 1] = l0;
+            mine[g * OS + D + 1] = odd_sign(l0, odd);
             mine[(g + 8) * OS + D] = m1;
-            mine[(g + 8) * OS + D + 1] = l1;
+            mine[(g + 8) * OS + D + 1] = odd_sign(l1, odd);
         }
         __syncthreads();
         // joined over the groups: thread (row, 4 dims)
@@ -391,18 +367,21 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
             for (int q8 = 0; q8 < C::GROUPS; ++q8) m = fmaxf(m, src[q8 * GS + D]);
             const float mu = m == -INFINITY ? 0.f : m;
             float l = 0.f;
+            bool some_odd = false;
             float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int q8 = 0; q8 < C::GROUPS; ++q8) {
                 const float f = exp2f(src[q8 * GS + D] - mu);
                 const float4 y = *reinterpret_cast<const float4 *>(src + q8 * GS + x4 * 4);
-                l += f * src[q8 * GS + D + 1];
+                l += f * fabsf(src[q8 * GS + D + 1]);
+                some_odd |= sign_odd(src[q8 * GS + D + 1]);
                 // a group that saw nothing (f = 0) holds zeros
                 acc.x += f * y.x;
                 acc.y += f * y.y;
                 acc.z += f * y.z;
                 acc.w += f * y.w;
             }
+            tree_nonfinite4<D, KT>(p, sg, sg.head, r, x4 * 4, l, some_odd, acc);
             if (part) {
                 reinterpret_cast<float4 *>(part)[x4 * p.rpg + r] = acc;
                 if (x4 == 0) {
@@ -425,6 +404,24 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
 // the first cut in it; it takes the unit's tasks y, y + gridDim.y, ... .
 // Segments are added in a fixed order, so a result does not depend on timing.
 // ---------------------------------------------------------------------------
+// A joined value that came out NaN: a segment's infinity met a weight that is 0
+// in 32 bits.  Such a column is the sum of the segments' values that are not
+// finite.  at4: its place in a slot.
+__device__ __noinline__ float4 merge_nonfinite(const TreeParams &p, uint32_t D, uint32_t first, uint32_t last, size_t at4, float4 x) {
+    float o[4] = {x.x, x.y, x.z, x.w}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t s = first; s <= last; ++s) {
+        const float4 y = reinterpret_cast<const float4 *>(tree_part(p, D, s, s == first ? 1u : 0u))[at4];
+        const float v[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (!(fabsf(v[e]) < INFINITY)) sum[e] += v[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (sum[e] != 0.f) o[e] = sum[e];
+    return make_float4(o[0], o[1], o[2], o[3]);
+}
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 2) tree_merge_kernel(const __grid_constant__ TreeParams p, uint32_t grid, uint32_t by_unit) {
     __shared__ TreeShared sh;
@@ -563,6 +560,11 @@ __global__ void __launch_bounds__(kThreads, 2) tree_merge_kernel(const __grid_co
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const size_t at = tree_row(p, sg, sg.row0 + r, D, h) + x4 * 4;
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            const float any = (acc[z].x + acc[z].y) + (acc[z].z + acc[z].w);
+            if (__builtin_expect(any != any && l == l, 0)) acc[z] = merge_nonfinite(p, D, b - 1, last, (size_t)(x4 + 4 * z) * R + row, acc[z]);
+        }
 #pragma unroll
         for (int z = 0; z < 2; ++z)
             store_out4(p.out, p.q_type, at + 16 * z, make_float4(acc[z].x * inv, acc[z].y * inv, acc[z].z * inv, acc[z].w * inv));

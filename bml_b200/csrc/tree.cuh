@@ -2,7 +2,10 @@
 // the tile schedule shared by the kernels, and the launch interface.
 #pragma once
 
+#include <math.h>
+
 #include <atomic>
+#include <type_traits>
 
 #include "paged.cuh"
 
@@ -456,10 +459,85 @@ __device__ __forceinline__ uint32_t tree_see16(const TreeParams &p, const TreeSe
 // hi: x rounded to TF32's 10 fraction bits, half away from zero, with integer
 // operations (a conversion instruction runs at a quarter of their rate and set
 // tree_f32_kernel's time: 4 requests of 618 to 2671 positions 85 -> 75 us).  lo: the rest, of
-// which the matrix unit takes the upper bits itself.
+// which the matrix unit takes the upper bits itself.  For softmax weights: x at
+// most 2^8, or NaN (which lo keeps).
 __device__ __forceinline__ void tf32_split(float x, uint32_t &hi, uint32_t &lo) {
     hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
     lo = __float_as_uint(x - __uint_as_float(hi));
+}
+// A value of any size.  hi stays finite: of a value that would round to infinity,
+// of an infinity and of a NaN it is the largest TF32 value of their sign, and lo
+// is the rest (an infinity or NaN as such), so that x * inf is what it should be
+// and not x * inf - x * inf.
+__device__ __forceinline__ void tf32_split_any(float x, uint32_t &hi, uint32_t &lo) {
+    float h = __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u);
+    asm("min.xorsign.abs.f32 %0, %0, 0f7F7FE000;" : "+f"(h));  // the smaller magnitude, the sign of h
+    hi = __float_as_uint(h);
+    lo = __float_as_uint(x - h);
+}
+
+// Four values of a pool row.
+template <typename KT>
+__device__ __forceinline__ float4 tree_load4(const void *pool, size_t at) {
+    if constexpr (sizeof(KT) == 4) {
+        return *reinterpret_cast<const float4 *>(static_cast<const float *>(pool) + at);
+    } else {
+        const uint2 w = *reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(pool) + at);
+        if constexpr (std::is_same<KT, __half>::value) {
+            const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&w.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&w.y));
+            return make_float4(a.x, a.y, b.x, b.y);
+        }
+        return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u), __uint_as_float(w.y << 16),
+                           __uint_as_float(w.y & 0xffff0000u));
+    }
+}
+
+// Positions [lo, hi) of a request's kv head, and the node of the row that looks.
+struct TreeSpan {
+    uint32_t seq, head, t, lo, hi;
+    TreeSeq s;
+};
+
+// Infinities and NaN among the V values that a row sees.  In products a weight
+// that is 0 in 32 bits, or a split weight's lower term, makes NaN of them; those of
+// drafted nodes, which other rows do not see, are taken as zeros there.  So a
+// column that came out NaN though the row's sum of weights is a number, and all
+// columns where a node's values were zeroed, are looked up here: weights are
+// positive, so such a column is the sum of its values that are not finite.
+// o: n columns from `col` on, un-normalised.  Rare, from global memory.
+template <int D, typename KT>
+__device__ __noinline__ void tree_nonfinite(const TreeParams &p, const TreeSpan &a, uint32_t col, uint32_t n, float *o) {
+    const uint32_t P = a.s.L - min(a.s.T, a.s.L), end = min(a.hi, a.s.L);
+    for (uint32_t c = 0; c < n; c += 4) {
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        for (uint32_t pos = a.lo; pos < end; ++pos) {
+            if (pos >= P && !tree_sees(p, a.s, a.t, pos - P)) continue;
+            const uint32_t page = (uint32_t)p.table[(size_t)a.seq * p.max_pages + (pos >> p.page_shift)];
+            if (page >= p.n_pages) continue;
+            const size_t row = ((size_t)page << p.page_shift) + (pos & ((1u << p.page_shift) - 1));
+            const float4 v = tree_load4<KT>(p.v, (row * p.n_kv + a.head) * D + col + c);
+            const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (!(fabsf(x[e]) < INFINITY)) sum[e] += x[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (sum[e] != 0.f) o[c + e] = sum[e];
+    }
+}
+// For four columns, where they need it.  l: the row's sum of weights; odd: the
+// segment has a node with zeroed values.
+template <int D, typename KT>
+__device__ __forceinline__ void tree_nonfinite4(const TreeParams &p, const TreeSeg &g, uint32_t head, uint32_t row, uint32_t col, float l,
+                                                bool odd, float4 &x) {
+    const float any = (x.x + x.y) + (x.z + x.w);  // inf - inf: looked up for nothing
+    if (__builtin_expect((odd || any != any) && l == l, 0)) {
+        const TreeSpan a = {g.seq, head, (g.row0 + row) / p.group, g.t0 << p.tile_shift, g.t1 << p.tile_shift, g.s};
+        float o[4] = {x.x, x.y, x.z, x.w};
+        tree_nonfinite<D, KT>(p, a, col, 4, o);
+        x = make_float4(o[0], o[1], o[2], o[3]);
+    }
 }
 // 16 bytes global -> shared; bytes = 0 writes zeros and reads nothing.
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, uint32_t bytes) {
@@ -484,6 +562,10 @@ __device__ __forceinline__ bool group_any(uint32_t id, uint32_t threads, bool x)
         : "memory");
     return r != 0;
 }
+// A warp's sum of weights l >= 0 on the way to its CTA's join, with a sign that
+// says whether a drafted node's V values that are not finite were taken as zeros.
+__device__ __forceinline__ float odd_sign(float l, bool odd) { return odd ? -l : l; }
+__device__ __forceinline__ bool sign_odd(float l) { return __float_as_uint(l) >> 31; }
 #endif
 
 }  // namespace bml

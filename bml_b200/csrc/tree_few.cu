@@ -82,6 +82,7 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ TreeShared sh;
     __shared__ uint32_t s_abort;
+    using KT = typename std::conditional<kF16, __half, __nv_bfloat16>::type;
     volatile uint32_t *abort_flag = &s_abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const uint32_t hsub = warp % p.hpu, split = warp / p.hpu;
@@ -93,7 +94,6 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
     const uint32_t pmask = (1u << p.page_shift) - 1;
     // K and V are read once: 131 MB in 30 us with the hint, 34 without (64 x 2000, d = 64)
     const uint64_t policy = l2_policy_evict_first();
-    const size_t prow = (size_t)p.n_kv * D * 2;
 
     if (lane == 0) {
         for (int i = 0; i < C::NST; ++i) mbar_init(&full[i], 1);
@@ -207,6 +207,7 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // rows 2c, 2c + 1; l: this lane's share
+        bool odd = false;  // a node has values taken as zeros
 
 #pragma unroll 1
         for (uint32_t k = sg.t0; k < sg.t1; ++k) {
@@ -221,11 +222,10 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
             }
             if (base >= sg.s.L || !flags[st]) continue;
             const bool edge = base + 16 > P;
-            bool odd = false;
             if (edge) {
                 // V rows past the length become zeros, and so do nodes' values that
-                // are not finite (0 * NaN is not 0); rows that see them get those
-                // added below.
+                // are not finite (0 * NaN is not 0); tree_nonfinite adds those to rows
+                // that see them.
 #pragma unroll 1
                 for (int i = lane; i < 16 * C::KB * 8; i += 32) {
                     const uint32_t r = (i >> 3) & 15;
@@ -243,7 +243,6 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the stage's next copy
-                odd = __any_sync(0xffffffffu, odd);
                 __syncwarp();
             }
             float s[4] = {0.f, 0.f, 0.f, 0.f}, lo[4] = {0.f, 0.f, 0.f, 0.f};
@@ -257,7 +256,8 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
             }
             if (kQ32)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[e] += lo[e];
+                for (int e = 0; e < 4; ++e)
+                    if (fabsf(s[e]) < INFINITY) s[e] += lo[e];  // else an infinite K, whose lower terms are NaN
             // s[0], s[1]: position base + g, rows 2c, 2c + 1; s[2], s[3]: base + g + 8
             if (edge) {
 #pragma unroll
@@ -323,31 +323,6 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
                     mma16816<kF16>(o[j], r, pb[0][0], pb[1][0]);
                 }
             }
-            if (odd) {
-                // rare: the values that became zeros, from global memory
-#pragma unroll 1
-                for (int i = 0; i < 16; ++i) {
-                    const int src = (i & 7) * 4 + c;
-                    const float w0 = __shfl_sync(0xffffffffu, i < 8 ? s[0] : s[2], src);
-                    const float w1 = __shfl_sync(0xffffffffu, i < 8 ? s[1] : s[3], src);
-                    const uint32_t at = base + i;
-                    if (at < P || at >= sg.s.L) continue;
-                    const uint32_t page = (uint32_t)p.table[(size_t)sg.seq * p.max_pages + (at >> p.page_shift)];
-                    if (page >= p.n_pages) continue;
-                    const uint16_t *v = reinterpret_cast<const uint16_t *>(static_cast<const char *>(p.v) +
-                                                                           (((size_t)page << p.page_shift) + (at & pmask)) * prow) +
-                                        (sg.head + hsub) * D;
-#pragma unroll
-                    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const uint16_t y = v[j * 16 + g + h * 8];
-                            if (!odd16<kF16>(y)) continue;
-                            if (w0 > 0.f) o[j][2 * h] += w0 * wide16<kF16>(y);
-                            if (w1 > 0.f) o[j][2 * h + 1] += w1 * wide16<kF16>(y);
-                        }
-                }
-            }
         }
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) {
@@ -357,14 +332,16 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
 
         // ------------------------------------------ the warps of a head meet
         // [warp][row][columns], rows of a warp's head
+        odd = __any_sync(0xffffffffu, odd);
         if (g == 0) {
-            ml[warp * kRows + 2 * c] = make_float2(m0, l0);
-            ml[warp * kRows + 2 * c + 1] = make_float2(m1, l1);
+            ml[warp * kRows + 2 * c] = make_float2(m0, odd_sign(l0, odd));
+            ml[warp * kRows + 2 * c + 1] = make_float2(m1, odd_sign(l1, odd));
         }
         const uint32_t R = kRows * p.hpu;  // a power of two that divides the thread count
         float *part = sg.slot < 2 ? tree_part(p, D, blockIdx.x, sg.slot) : nullptr;
         const uint32_t row = threadIdx.x & (R - 1), h = row / kRows, r = row % kRows;  // this thread's in what follows
         float m = -INFINITY, mu = 0.f, l = 0.f, inv = 0.f;
+        bool some_odd = false;
         size_t at = 0;
 #pragma unroll
         for (int ch = 0; ch < 2; ++ch) {
@@ -384,7 +361,8 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
                     mu = m == -INFINITY ? 0.f : m;
                     for (uint32_t s = 0; s < fp.splits; ++s) {
                         const float2 a = ml[(s * p.hpu + h) * kRows + r];
-                        l += weight(a.x - mu) * a.y;
+                        l += weight(a.x - mu) * fabsf(a.y);
+                        some_odd |= sign_odd(a.y);
                     }
                     if (*abort_flag) l = __int_as_float(0x7fffffff);  // a copy did not arrive: NaN
                     inv = l == 0.f ? 0.f : 1.f / l;
@@ -406,6 +384,7 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
                         acc.w += f * y.w;
                     }
                     const uint32_t col4 = ch * (C::CH / 4) + x4;
+                    tree_nonfinite4<D, KT>(p, sg, sg.head + h, r, col4 * 4, l, some_odd, acc);
                     if (part)
                         reinterpret_cast<float4 *>(part)[col4 * R + row] = acc;
                     else if (kQ32)

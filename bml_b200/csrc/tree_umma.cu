@@ -31,8 +31,8 @@
 // What a row does not see must not reach it: scores are replaced by -inf
 // (bad pages, rows past the length, nodes outside the mask), V rows past the
 // length are zeroed in shared memory before the first P.V that reads them,
-// and so are V rows of drafted nodes with a value that is not finite (0 * NaN
-// is not 0); the epilogue adds those nodes for the rows that see them.
+// and so are values of drafted nodes that are not finite (0 * NaN is not 0);
+// tree_nonfinite adds those to the rows that see them.
 #include <math.h>
 
 #include <type_traits>
@@ -90,7 +90,9 @@ struct alignas(16) UmmaShared {
     uint64_t drain;
     uint32_t tmem, abort;
     uint32_t bad[kBadRing];  // per tile: 16-position blocks on pages outside the pool
-    uint32_t odd[8];         // drafted nodes whose V has a value that is not finite
+    // [segment % 2]: the last segment (from 1 on) with a drafted node whose V has a
+    // value that is not finite.  A chain is less than two segments ahead of the other.
+    uint32_t odd[2];
     float2 ml[256];          // (m, l) of both chains' rows
     TreeShared sched;
     uint64_t seg_full[kBoard];
@@ -142,62 +144,49 @@ __device__ __noinline__ uint4 see_tile(const TreeParams &p, const volatile Board
     return make_uint4(see[0], see[1], see[2], see[3]);
 }
 
-// One V row of a tile before its first P.V: zeros past the length, and where a
-// drafted node's row has a value that is not finite (noted in odd).  row: its
+// One V row of a tile before its first P.V: zeros past the length, and in place
+// of a drafted node's values that are not finite (then *odd = seg).  row: its
 // first 128 bytes; the lanes start at different 16-byte pieces, against bank
 // conflicts.
 template <int KB, bool kF16>
-__device__ __noinline__ void fix_v(uint8_t *row, bool node_row, bool past, uint32_t node, uint32_t *odd) {
+__device__ __noinline__ void fix_v(uint8_t *row, bool node_row, bool past, volatile uint32_t *odd, uint32_t seg) {
     const uint32_t lane = threadIdx.x & 31;
-    bool zero = past;
-    if (node_row && !past) {
-        constexpr uint32_t em = kF16 ? 0x7c00u : 0x7f80u;
-        bool bad = false;
+    if (!node_row) return;
+    constexpr uint32_t em = kF16 ? 0x7c00u : 0x7f80u;
+    auto piece = [&](int u) { return reinterpret_cast<uint4 *>(row + (u >> 3) * BN * 128 + ((u + lane) & 7) * 16); };
+    if (past) {
 #pragma unroll 4
-        for (int u = 0; u < KB * 8; ++u) {
-            const uint4 w = lds128(row + (u >> 3) * BN * 128 + ((u + lane) & 7) * 16);
-            const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+        for (int u = 0; u < KB * 8; ++u) *piece(u) = make_uint4(0, 0, 0, 0);
+        return;
+    }
+    bool bad = false;
+#pragma unroll 4
+    for (int u = 0; u < KB * 8; ++u) {
+        const uint4 w = lds128(reinterpret_cast<const uint8_t *>(piece(u)));
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) bad |= (ws[e] & em) == em || ((ws[e] >> 16) & em) == em;
-        }
-        if (bad) {
-            atomicOr(&odd[node >> 5], 1u << (node & 31));
-            zero = true;
-        }
+        for (int e = 0; e < 4; ++e) bad |= (ws[e] & em) == em || ((ws[e] >> 16) & em) == em;
     }
-    if (zero)
-#pragma unroll 4
-        for (int u = 0; u < KB * 8; ++u)
-            *reinterpret_cast<uint4 *>(row + (u >> 3) * BN * 128 + ((u + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
+    if (!bad) return;
+    *odd = seg;
+#pragma unroll 1
+    for (int u = 0; u < KB * 8; ++u) {
+        const uint4 w = *piece(u);
+        uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ws[e] &= ((ws[e] & em) == em ? 0u : 0xffffu) | ((ws[e] >> 16 & em) == em ? 0u : 0xffff0000u);
+        *piece(u) = make_uint4(ws[0], ws[1], ws[2], ws[3]);
+    }
 }
 
-template <bool kF16>
-__device__ __forceinline__ float one16(uint16_t x) {
-    return kF16 ? __half2float(*reinterpret_cast<const __half *>(&x)) : __uint_as_float((uint32_t)x << 16);
-}
-
-// Adds to o (32 columns of a row of node t from `col` on, relative to maximum
-// m) the drafted nodes whose V rows were zeroed because a value is not finite,
-// where the row sees them.  Rare: everything is recomputed from global memory.
+// tree_nonfinite for 32 columns of a row of node t.
 template <int D, bool kF16>
-__device__ __noinline__ void add_odd(const TreeParams &p, const volatile Board *b, const uint32_t *odd, uint32_t P, uint32_t t,
-                                     size_t q_at, uint32_t col, float m, float *o) {
-    const uint32_t lo = b->t0 * BN, hi = lo + (b->packed & 0xfffffffu) * BN;
-    TreeSeq s;
-    s.first = b->first;
-    s.T = b->T;
-    for (uint32_t node = 0; node < s.T; ++node) {
-        const uint32_t pos = P + node;
-        if (!(odd[node >> 5] >> (node & 31) & 1) || pos < lo || pos >= hi || !tree_sees(p, s, t, node)) continue;
-        const uint32_t page = (uint32_t)p.table[(size_t)b->seq * p.max_pages + (pos >> p.page_shift)];
-        if (page >= p.n_pages) continue;
-        const size_t at = ((((size_t)page << p.page_shift) + (pos & ((1u << p.page_shift) - 1))) * p.n_kv + b->head) * D;
-        const uint16_t *q = static_cast<const uint16_t *>(p.q) + q_at, *k = static_cast<const uint16_t *>(p.k) + at;
-        float sc = 0.f;
-        for (int i = 0; i < D; ++i) sc = fmaf(one16<kF16>(q[i]), one16<kF16>(k[i]), sc);
-        const float w = fast_exp2(sc * p.scale_log2 - m);
-        for (int u = 0; u < 32; ++u) o[u] = fmaf(w, one16<kF16>(static_cast<const uint16_t *>(p.v)[at + col + u]), o[u]);
-    }
+__device__ __noinline__ void add_nonfinite(const TreeParams &p, const volatile Board *b, uint32_t t, uint32_t col, float *o) {
+    TreeSpan a = {b->seq, b->head, t, b->t0 * BN, (b->t0 + (b->packed & 0xfffffffu)) * BN, {}};
+    a.s.first = b->first;
+    a.s.T = b->T;
+    a.s.L = b->L;
+    tree_nonfinite<D, typename std::conditional<kF16, __half, __nv_bfloat16>::type>(p, a, col, 32, o);
 }
 
 template <int D, bool kF16>
@@ -230,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
         sh.abort = 0u;
         fence_mbar_init();
     }
-    if (threadIdx.x < 8) sh.odd[threadIdx.x] = 0u;
+    if (threadIdx.x < 2) sh.odd[threadIdx.x] = 0u;
     if (warp == 0 && lane == 0) {
         prefetch_tmap(&up.tq);
         prefetch_tmap(&up.tk);
@@ -591,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
                     const uint32_t pos = kv0 + r, cv = cnt + v_index(pair, j, n), slot = cv % C::SLOTS;
                     if (__any_sync(0xffffffffu, pos >= P)) {
                         wait_bar(&sh.full[slot], (cv / C::SLOTS) & 1u, abort_flag, p.wait_ns);
-                        fix_v<C::KB, kF16>(ring + slot * C::TILE + r * 128, pos >= P, pos >= b->L, pos - P, sh.odd);
+                        fix_v<C::KB, kF16>(ring + slot * C::TILE + r * 128, pos >= P, pos >= b->L, &sh.odd[segs & 1u], segs + 1);
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     }
                 }
@@ -687,10 +676,13 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
             // Row = wa * O_A + wb * O_B, un-normalised, with maximum m and sum l.
             // One row tile: both chains' (m, l) meet in shared memory, and chain x
             // writes columns x * D / 2 .. of the joined row.
+            // has_a, has_b: the chain saw something (else its O may be anything).
             float wa, wb, m = m_run, l = l_run;
+            bool has_a, has_b = false;
             if (pair) {
                 wait_bar(&sh.o_final[x], (finals >> x) & 1u, abort_flag, p.wait_ns);
-                wa = m_run == -INFINITY ? 0.f : 1.f;
+                has_a = m_run != -INFINITY;
+                wa = 1.f;
                 wb = 0.f;
             } else {
                 sh.ml[x * 128 + r] = make_float2(m_run, l_run);
@@ -700,8 +692,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
                 named_bar_sync(1, 256);
                 const float2 ma = sh.ml[r], mb = sh.ml[128 + r];
                 m = fmaxf(ma.x, mb.x);
-                wa = ma.x == -INFINITY ? 0.f : fast_exp2(ma.x - m);
-                wb = mb.x == -INFINITY ? 0.f : fast_exp2(mb.x - m);  // no tiles: -inf
+                has_a = ma.x != -INFINITY;
+                has_b = mb.x != -INFINITY;  // no tiles: -inf
+                wa = has_a ? fast_exp2(ma.x - m) : 0.f;
+                wb = has_b ? fast_exp2(mb.x - m) : 0.f;
                 l = wa * ma.y + wb * mb.y;
             }
             __syncwarp();
@@ -712,10 +706,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
             const uint32_t gr = b->row0 + row, t = gr / p.group;  // node; q head gr - t * group of the kv head
             const size_t at = valid ? ((size_t)(b->first + t) * p.n_heads + (size_t)b->head * p.group + (gr - t * p.group)) * D : 0;
             float *part = slot_of < 2 ? tree_part(p, D, blockIdx.x, slot_of) : nullptr;
-            uint32_t any_odd = 0;
-            if (kv_first + n * BN > P)
-#pragma unroll
-                for (int w = 0; w < 8; ++w) any_odd |= *(volatile uint32_t *)&sh.odd[w];
+            const bool odd = kv_first + n * BN > P && *(volatile uint32_t *)&sh.odd[segs & 1u] == segs + 1;
             if (warp_live) {
                 const uint32_t first = pair ? 0u : x * (D / 2), n_cols = pair ? D : D / 2;
                 const uint32_t src0 = pair ? o_col : o_base;
@@ -726,21 +717,25 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
                     tmem_ld32(src0 + col, o);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int u = 0; u < 32; ++u) o[u] = wa == 0.f ? 0.f : o[u] * wa;
-                    if (__any_sync(0xffffffffu, wb != 0.f)) {
+                    for (int u = 0; u < 32; ++u) o[u] = has_a ? o[u] * wa : 0.f;
+                    if (__any_sync(0xffffffffu, has_b)) {
                         float o2[32];
                         tmem_ld32(o_base + D + col, o2);
                         tmem_wait_ld();
-                        if (wb != 0.f)
+                        if (has_b)
 #pragma unroll
                             for (int u = 0; u < 32; ++u) o[u] = fmaf(o2[u], wb, o[u]);
                     }
                     if (valid) {
-                        if (any_odd) {
+                        float any[4] = {0.f, 0.f, 0.f, 0.f};  // NaN where a column is not finite
+#pragma unroll
+                        for (int u = 0; u < 32; ++u) any[u & 3] = fmaf(o[u], 0.f, any[u & 3]);
+                        any[0] = (any[0] + any[1]) + (any[2] + any[3]);
+                        if (__builtin_expect((odd || any[0] != any[0]) && l == l, 0)) {
                             float tmp[32];  // its address is taken, o's is not
 #pragma unroll
                             for (int u = 0; u < 32; ++u) tmp[u] = o[u];
-                            add_odd<D, kF16>(p, b, sh.odd, P, t, at, col, m, tmp);
+                            add_nonfinite<D, kF16>(p, b, t, col, tmp);
 #pragma unroll
                             for (int u = 0; u < 32; ++u) o[u] = tmp[u];
                         }
@@ -766,15 +761,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
             }
             tc_fence_before();
             __syncwarp();
-            // The next segment's first P.V may overwrite O, its ml and odd words
-            // be set, once both chains are here.
-            const bool had_edge = kv_first + n * BN > P;
-            if (!pair || had_edge) named_bar_sync(1, 256);
-            if (had_edge) {
-                if (threadIdx.x >= 64 && threadIdx.x < 72) sh.odd[threadIdx.x - 64] = 0u;
-                __syncwarp();
-                named_bar_sync(1, 256);
-            }
+            // The next segment's first P.V may overwrite O, and its ml be set, once both
+            // chains are here.
+            if (!pair) named_bar_sync(1, 256);
             cnt += 2 * n;
             tiles += n;
             done += nt;

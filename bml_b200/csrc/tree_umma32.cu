@@ -40,8 +40,8 @@
 //
 // What a row does not see must not reach it: scores are replaced by -inf (bad
 // pages, rows past the length, nodes outside the mask), V rows past the length
-// and values of drafted nodes that are not finite are split as zeros, and the
-// latter are added at the end for the rows that see them.
+// and values of drafted nodes that are not finite are split as zeros, and
+// tree_nonfinite adds the latter to the rows that see them.
 #include <math.h>
 
 #include "tree.cuh"
@@ -84,7 +84,7 @@ struct alignas(16) XShared {
     uint64_t v_full, v_empty, q_ready, v_ready, s_full, p_ready, o_full, o_free, drain;
     uint32_t tmem, abort;
     uint32_t bad[kBadRing];  // per tile: 16-position blocks on pages outside the pool
-    uint32_t odd[3][8];      // per segment: drafted nodes with a V value that is not finite
+    uint32_t odd[3];  // [segment % 3]: the last segment (from 1 on) with a drafted node's V value that is not finite
     float top[2][BM], sum[2][BM];  // [half][row]: maximum of a tile; l of a segment
     TreeShared sched;
 };
@@ -100,13 +100,17 @@ __device__ __forceinline__ void mma_tf32_ts(uint32_t d_tmem, uint32_t a_tmem, ui
         : "memory");
 }
 
-// 32 values as hi and lo, to tensor memory.
+// 32 values as hi and lo, to tensor memory.  kAny: of any size (else weights).
+template <bool kAny>
 __device__ __forceinline__ void put_split(uint32_t hi_at, uint32_t lo_at, const float *x) {
 #pragma unroll
     for (int c = 0; c < 32; c += 16) {
         uint32_t hi[16], lo[16];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) tf32_split(x[c + k], hi[k], lo[k]);
+        for (int k = 0; k < 16; ++k) {
+            if (kAny) tf32_split_any(x[c + k], hi[k], lo[k]);
+            else tf32_split(x[c + k], hi[k], lo[k]);
+        }
         tmem_st16(hi_at + c, hi);
         tmem_st16(lo_at + c, lo);
     }
@@ -123,30 +127,6 @@ __device__ __forceinline__ uint32_t see_half(const TreeParams &p, const TreeSeq 
         see |= (n0 <= -16 ? 0xffffu : tree_see16(p, s, t, n0) & 0xffffu) << (16 * b);
     }
     return see;
-}
-
-// Adds to o (32 columns from `col` on of a row of node t, relative to maximum m)
-// the values of drafted nodes that are not finite, where the row sees them.
-// Rare: everything is recomputed from global memory.
-template <int D>
-__device__ __noinline__ void add_odd(const TreeParams &p, const TreeSeg &sg, const uint32_t *odd, uint32_t t, size_t q_at,
-                                     uint32_t col, float m, float *o) {
-    const uint32_t lo = sg.t0 * BN, hi = sg.t1 * BN, P = sg.s.L - min(sg.s.T, sg.s.L);
-    for (uint32_t node = 0; node < sg.s.T; ++node) {
-        const uint32_t pos = P + node;
-        if (!(odd[node >> 5] >> (node & 31) & 1) || pos < lo || pos >= hi || !tree_sees(p, sg.s, t, node)) continue;
-        const uint32_t page = (uint32_t)p.table[(size_t)sg.seq * p.max_pages + (pos >> p.page_shift)];
-        if (page >= p.n_pages) continue;
-        const size_t at = ((((size_t)page << p.page_shift) + (pos & ((1u << p.page_shift) - 1))) * p.n_kv + sg.head) * D;
-        const float *q = static_cast<const float *>(p.q) + q_at, *k = static_cast<const float *>(p.k) + at;
-        float sc = 0.f;
-        for (int i = 0; i < D; ++i) sc = fmaf(q[i], k[i], sc);
-        const float w = exp2f(sc * p.scale_log2 - m);
-        for (int u = 0; u < 32; ++u) {
-            const float v = static_cast<const float *>(p.v)[at + col + u];
-            if (!(fabsf(v) < INFINITY) && !(w <= 0.f)) o[u] = fmaf(w, v, o[u]);
-        }
-    }
 }
 
 template <int D>
@@ -176,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
         sh.abort = 0u;
         fence_mbar_init();
     }
-    if (threadIdx.x < 24) sh.odd[threadIdx.x / 8][threadIdx.x % 8] = 0u;
+    if (threadIdx.x < 3) sh.odd[threadIdx.x] = 0u;
     if (warp == 0 && lane == 0) {
         prefetch_tmap(&xp.tk);
         prefetch_tmap(&xp.tv);
@@ -327,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
                 }
                 __syncwarp();
 #pragma unroll
-                for (int c = 0; c < D / 2; c += 32) put_split(at + C::QHI + half * (D / 2) + c, at + C::QLO + half * (D / 2) + c, x + c);
+                for (int c = 0; c < D / 2; c += 32) put_split<true>(at + C::QHI + half * (D / 2) + c, at + C::QLO + half * (D / 2) + c, x + c);
                 tmem_wait_st();
             }
             tc_fence_before();
@@ -389,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
                         s[k + 1] = fast_exp2(z.y);
                         sum[k >> 1 & 1] = __fadd2_rn(sum[k >> 1 & 1], make_float2(s[k], s[k + 1]));
                     }
-                    put_split(hi_at, lo_at, s);
+                    put_split<false>(hi_at, lo_at, s);
                     const float2 both = __fadd2_rn(sum[0], sum[1]);
                     l = fmaf(l, alpha, both.x + both.y);
                     tmem_wait_st();
@@ -424,23 +404,23 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
             }
             if (*abort_flag) l = __int_as_float(0x7fffffff);  // a wait gave up: NaN
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            const uint32_t *odd = sh.odd[segs % 3];  // all V of the segment has been split
+            // all V of the segment has been split
+            const bool odd = sg.t1 * BN > P && *(const volatile uint32_t *)&sh.odd[segs % 3] == segs + 1;
             float *part = sg.slot < 2 ? tree_part(p, D, blockIdx.x, sg.slot) : nullptr;
-            uint32_t any_odd = 0;
-            if (sg.t1 * BN > P)
-#pragma unroll
-                for (int w = 0; w < 8; ++w) any_odd |= *(const volatile uint32_t *)&odd[w];
             if (valid) {
                 const size_t at = tree_row(p, sg, sg.row0 + r, D);
-                if (any_odd) {
-                    const uint32_t t = (sg.row0 + r) / p.group;
-                    const TreeSeg g = sg;  // as are their copies'
+                float any[4] = {0.f, 0.f, 0.f, 0.f};  // NaN where a column is not finite
+#pragma unroll
+                for (int u = 0; u < D / 2; ++u) any[u & 3] = fmaf(o[u], 0.f, any[u & 3]);
+                any[0] = (any[0] + any[1]) + (any[2] + any[3]);
+                if (__builtin_expect((odd || any[0] != any[0]) && l == l, 0)) {
+                    const TreeSpan a = {sg.seq, sg.head, (sg.row0 + r) / p.group, sg.t0 * BN, sg.t1 * BN, sg.s};
 #pragma unroll
                     for (int c = 0; c < D / 2; c += 32) {
                         float tmp[32];  // its address is taken, o's is not
 #pragma unroll
                         for (int u = 0; u < 32; ++u) tmp[u] = o[c + u];
-                        add_odd<D>(p, g, odd, t, at, half * (D / 2) + c, m, tmp);
+                        tree_nonfinite<D, float>(p, a, half * (D / 2) + c, 32, tmp);
 #pragma unroll
                         for (int u = 0; u < 32; ++u) o[c + u] = tmp[u];
                     }
@@ -483,10 +463,10 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
                 const uint32_t e = x + x / kBlock * kBlock;
                 const uint4 y = k[e];
                 uint4 h, l;
-                tf32_split(__uint_as_float(y.x), h.x, l.x);
-                tf32_split(__uint_as_float(y.y), h.y, l.y);
-                tf32_split(__uint_as_float(y.z), h.z, l.z);
-                tf32_split(__uint_as_float(y.w), h.w, l.w);
+                tf32_split_any(__uint_as_float(y.x), h.x, l.x);
+                tf32_split_any(__uint_as_float(y.y), h.y, l.y);
+                tf32_split_any(__uint_as_float(y.z), h.z, l.z);
+                tf32_split_any(__uint_as_float(y.w), h.w, l.w);
                 k[e] = h;
                 k[e + kBlock] = l;
             }
@@ -497,14 +477,11 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
         if (total) split_k(0);
         while (walk.next(p, sg)) {
             const uint32_t P = sg.s.L - min(sg.s.T, sg.s.L);
-            uint32_t *odd = sh.odd[segs % 3];
             for (uint32_t j = sg.t0; j < sg.t1; ++j, ++it) {
                 // V(it) transposed: thread = 4 positions of one column
                 wait_bar(&sh.v_full, it & 1u, abort_flag, p.wait_ns);
                 if (it > 0) wait_bar(&sh.o_full, (it & 1u) ^ 1u, abort_flag, p.wait_ns);  // the last tile's V has been read
                 __syncwarp();
-                // read two segments ago: the rows' warps have since been through a tile of the last one
-                if (j == sg.t0 && cw == 0 && lane < 8) sh.odd[(segs + 1) % 3][lane] = 0u;
                 const float *v = reinterpret_cast<const float *>(smem + C::OFF_V);
                 const uint32_t kv0 = j * BN;
                 const bool edge = kv0 + BN > P;
@@ -521,15 +498,15 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
                             if (pos >= sg.s.L) x[e] = 0.f;
                             else if (pos >= P && !(fabsf(x[e]) < INFINITY)) {
                                 x[e] = 0.f;
-                                atomicOr(&odd[(pos - P) >> 5], 1u << ((pos - P) & 31));
+                                *(volatile uint32_t *)&sh.odd[segs % 3] = segs + 1;
                             }
                         }
                     }
                     uint4 h, l;
-                    tf32_split(x[0], h.x, l.x);
-                    tf32_split(x[1], h.y, l.y);
-                    tf32_split(x[2], h.z, l.z);
-                    tf32_split(x[3], h.w, l.w);
+                    tf32_split_any(x[0], h.x, l.x);
+                    tf32_split_any(x[1], h.y, l.y);
+                    tf32_split_any(x[2], h.z, l.z);
+                    tf32_split_any(x[3], h.w, l.w);
                     const uint32_t to = (quad >> 3) * (D * 128) + d * 128 + (((quad & 7) ^ (d & 7)) << 4);
                     *reinterpret_cast<uint4 *>(smem + C::OFF_VHI + to) = h;
                     *reinterpret_cast<uint4 *>(smem + C::OFF_VLO + to) = l;

@@ -97,6 +97,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
     constexpr int PER = D * 2 / 16; // 16-byte pieces of a row
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ TreeShared sh;
+    using KT = typename std::conditional<kF16, __half, __nv_bfloat16>::type;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const int rw = warp % RW, grp = warp / RW, tig = rw * 32 + lane;
     uint8_t *ring = smem + grp * C::NST * C::STAGE;
@@ -225,6 +226,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
         float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // l: this lane's share
+        bool odd = false;  // a node has values taken as zeros
         const bool live = sg.rows > (uint32_t)rw * 16;
 
         for (uint32_t k = sg.t0; k < sg.t1; ++k) {
@@ -233,10 +235,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
             fetch();  // into the stage that every warp of the group has left
             uint8_t *sk = ring + stage * C::STAGE, *sv = sk + C::SP * C::RS;
             const uint32_t pos = k * kTreeTile + grp * C::SP;
-            bool odd = false;
             if (pos + C::SP > P && pos < sg.s.L) {
                 // Drafted nodes' V values that are not finite become zeros here
-                // (0 * NaN is not 0); rows that see them get them added below.
+                // (0 * NaN is not 0); tree_nonfinite adds them to rows that see them.
                 bool mine = false;
                 for (int i = tig; i < C::SP * PER; i += RW * 32) {
                     if (pos + i / PER < P) continue;
@@ -249,9 +250,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
                         }
                 }
                 if (RW == 1) {
-                    odd = __any_sync(0xffffffffu, mine);
+                    odd |= __any_sync(0xffffffffu, mine);
                     __syncwarp();
-                } else odd = group_any(1 + grp, RW * 32, mine);
+                } else odd |= group_any(1 + grp, RW * 32, mine);
             }
             const uint32_t st = stage;
             stage = stage + 1 == (uint32_t)C::NST ? 0 : stage + 1;
@@ -284,7 +285,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[h][e] += lo[h][e];
+                        for (int e = 0; e < 4; ++e)
+                            if (fabsf(s[h][e]) < INFINITY) s[h][e] += lo[h][e];  // else an infinite K, whose lower terms are NaN
                 if (base + 16 > P) {
                     const uint32_t w0 = v0 ? tree_see16(p, sg.s, t0, (int32_t)(base - P)) : 0u;
                     const uint32_t w1 = v1 ? tree_see16(p, sg.s, t1, (int32_t)(base - P)) : 0u;
@@ -362,31 +364,6 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
                         mma16816<kF16>(o[j + 1], pa[0], r[2], r[3]);
                     }
                 }
-                if (odd) {
-                    // rare: the values that became zeros, from global memory
-#pragma unroll 1
-                    for (int i = 0; i < 16; ++i) {
-                        const int src = (lane & ~3) | ((i & 7) >> 1), h = i >> 3, e = i & 1;
-                        const float y0 = h ? (e ? s[1][1] : s[1][0]) : (e ? s[0][1] : s[0][0]);
-                        const float y1 = h ? (e ? s[1][3] : s[1][2]) : (e ? s[0][3] : s[0][2]);
-                        const float w0 = __shfl_sync(0xffffffffu, y0, src), w1 = __shfl_sync(0xffffffffu, y1, src);
-                        const uint32_t at = base + i;
-                        if (at < P || at >= sg.s.L) continue;
-                        const uint32_t page = (uint32_t)p.table[(size_t)sg.seq * p.max_pages + (at >> p.page_shift)];
-                        if (page >= p.n_pages) continue;
-                        const uint16_t *v = reinterpret_cast<const uint16_t *>(
-                            static_cast<const char *>(p.v) + (((size_t)page << p.page_shift) + (at & pmask)) * prow) + sg.head * D;
-#pragma unroll
-                        for (int j = 0; j < NT; ++j)
-#pragma unroll
-                            for (int z = 0; z < 2; ++z) {
-                                const uint16_t y = v[j * 8 + 2 * c + z];
-                                if (!odd16<kF16>(y)) continue;
-                                if (w0 > 0.f) o[j][z] += w0 * wide16<kF16>(y);
-                                if (w1 > 0.f) o[j][2 + z] += w1 * wide16<kF16>(y);
-                            }
-                    }
-                }
             }
         }
         l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
@@ -396,8 +373,8 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
 
         // ---------------------------------------------------- the groups meet
         if (c == 0) {
-            ml[warp * 16 + g] = make_float2(m0, l0);
-            ml[warp * 16 + g + 8] = make_float2(m1, l1);
+            ml[warp * 16 + g] = make_float2(m0, odd_sign(l0, odd));
+            ml[warp * 16 + g + 8] = make_float2(m1, odd_sign(l1, odd));
         }
         float *part = sg.slot < 2 ? tree_part(p, D, blockIdx.x, sg.slot) : nullptr;
 #pragma unroll
@@ -418,19 +395,22 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
                 for (int q8 = 0; q8 < C::GROUPS; ++q8) m = fmaxf(m, ml[q8 * RW * 16 + r].x);
                 const float mu = m == -INFINITY ? 0.f : m;
                 float l = 0.f;
+                bool some_odd = false;
                 float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int q8 = 0; q8 < C::GROUPS; ++q8) {
                     const float2 a = ml[q8 * RW * 16 + r];
                     const float f = weight(a.x - mu);
                     const float4 y = *reinterpret_cast<const float4 *>(meet + (q8 * RW * 16 + r) * C::CS + x4 * 4);
-                    l += f * a.y;
+                    l += f * fabsf(a.y);
+                    some_odd |= sign_odd(a.y);
                     acc.x += f * y.x;
                     acc.y += f * y.y;
                     acc.z += f * y.z;
                     acc.w += f * y.w;
                 }
                 const uint32_t col4 = ch * (C::CH / 4) + x4;
+                tree_nonfinite4<D, KT>(p, sg, sg.head, r, col4 * 4, l, some_odd, acc);
                 if (part) {
                     reinterpret_cast<float4 *>(part)[col4 * p.rpg + r] = acc;
                     if (col4 == 0) {

@@ -486,7 +486,9 @@ bml_status bml_attn_tree_workspace_size(uint32_t head_dim, int32_t device,
  * positions than its table holds.  Positions on a page outside [0, n_pages)
  * count as masked.  What lies in masked places -- cache rows past kv_lens,
  * nodes that a row does not see, infinities and NaN among them -- does not
- * reach the row.  Token rows outside the requests' are left as they were.
+ * reach the row.  An infinity in V that a row does see makes that column of the
+ * row infinite (NaN beside one of the other sign), whatever its weight.
+ * Token rows outside the requests' are left as they were.
  * 16-bit queries: scores and sums in f32, the softmax weights rounded to the
  * 16-bit type before P.V, one rounding of the output; 32-bit queries: about
  * f32 precision throughout.  Results are the same from run to run on one
