@@ -106,6 +106,8 @@ SIGNATURES = {
     "bml_attn_tree_workspace_size": (_st, [_u32, _i32, C.POINTER(_sz)]),
     "bml_attn_tree": (_st, [_vp, C.c_int, _u32, _u32, _u32, _u32, _vp, _vp, C.c_int, _u32, _u32, _vp, _u32, _vp, _vp,
                             _u32, _vp, _u32, C.c_float, _vp, _vp, _sz, _vp]),
+    "bml_attn_tree_sized": (_st, [_vp, C.c_int, _u32, _u32, _u32, _u32, _vp, _vp, C.c_int, _u32, _u32, _vp, _u32, _vp, _vp,
+                                  _u32, _vp, _u32, C.c_float, _vp, _vp, _sz, _u32, _u32, _vp]),
     "bml_paged_commit": (_st, [_vp, _vp, _u32, _u32, _u32, _u32, _u32, C.c_int, _vp, _u32, _vp, _vp, _vp, _u32, _vp,
                                _u32, _vp, _vp, _vp]),
     "bml_softmax_f32": (_st, [_vp, _u32, _u32, _vp, _vp]),
@@ -136,6 +138,8 @@ SIGNATURES = {
     # include/bml_diag.h (test-only)
     "bml_diag_attn_tree": (_st, [_vp, C.c_int, _u32, _u32, _u32, _u32, _vp, _vp, C.c_int, _u32, _u32, _vp, _u32, _vp,
                                  _vp, _u32, _vp, _u32, C.c_float, _vp, _vp, _sz, C.c_uint64, _u32, _vp]),
+    "bml_diag_attn_tree_form": (_st, [C.c_int, C.c_int, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32,
+                                      C.POINTER(C.c_int)]),
     "bml_diag_exp2": (_st, [_vp, _u32, _vp, _vp]),
     "bml_diag_decode_batched": (_st, [C.POINTER(bml_seq_desc), _u32, _u32, _u32, _u32, C.c_int,
                                       C.c_float, _vp, _vp, _vp, _sz, C.c_int, C.c_uint64, _u32, _vp]),

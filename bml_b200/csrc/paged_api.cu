@@ -195,13 +195,21 @@ BML_API bml_status bml_attn_tree_workspace_size(uint32_t head_dim, int32_t devic
 
 namespace {
 
-// What bml_attn_tree takes, and what only tests set.
+// What the choice of a kernel goes by.
+void tree_rows(bml::TreeArgs &a, uint32_t n_tokens, uint32_t group, uint32_t n_seqs, uint32_t n_live, uint32_t max_nodes) {
+    a.live = n_live && n_live < n_seqs ? n_live : n_seqs;
+    a.rows = (uint32_t)((uint64_t)n_tokens * group / a.live);
+    const uint32_t most = max_nodes < bml::kTreeMaxNodes ? max_nodes : bml::kTreeMaxNodes;
+    a.widest = most * group > a.rows && (a.p.q_type != BML_F32 || a.kv_type == BML_F32) ? most * group : a.rows;
+}
+
+// What bml_attn_tree_sized takes, and what only tests set.
 bml_status attn_tree(const char *fn, const void *q_dev, bml_dtype q_dtype, uint32_t n_tokens, uint32_t n_heads,
                      uint32_t n_kv_heads, uint32_t head_dim, const void *k_pool, const void *v_pool, bml_dtype kv_dtype,
                      uint32_t n_pages, uint32_t page_size, const int32_t *block_table, uint32_t max_pages,
                      const int32_t *kv_lens, const int32_t *node_start, uint32_t n_seqs, const uint64_t *mask,
                      uint32_t n_words, float scale, void *out_dev, void *workspace, size_t workspace_bytes,
-                     uint64_t wait_ns, uint32_t diag, void *stream) {
+                     uint32_t n_live, uint32_t max_nodes, uint64_t wait_ns, uint32_t diag, void *stream) {
     if (!valid_dtype(q_dtype) || !valid_dtype(kv_dtype)) return api_fail(BML_E_INVALID, "%s: unknown dtype", fn);
     if (q_dtype != BML_F32 && q_dtype != kv_dtype)
         return api_fail(BML_E_UNSUPPORTED, "%s: 16-bit queries need pages of their own type", fn);
@@ -231,8 +239,9 @@ bml_status attn_tree(const char *fn, const void *q_dev, bml_dtype q_dtype, uint3
     a.D = head_dim;
     a.kv_type = kv_dtype;
     a.num_sms = sms;
-    a.rows = (uint32_t)((uint64_t)n_tokens * (n_heads / n_kv_heads) / n_seqs);
     bml::TreeParams &p = a.p;
+    p.q_type = q_dtype;
+    tree_rows(a, n_tokens, n_heads / n_kv_heads, n_seqs, n_live, max_nodes);
     p.q = q_dev;
     p.out = out_dev;
     p.k = k_pool;
@@ -249,7 +258,6 @@ bml_status attn_tree(const char *fn, const void *q_dev, bml_dtype q_dtype, uint3
     p.n_words = n_words;
     const double sc = scale < 0.f ? 1.0 / sqrt((double)head_dim) : (double)scale;
     p.scale_log2 = (float)(sc * 1.4426950408889634);
-    p.q_type = q_dtype;
     p.part = static_cast<float *>(workspace);
     p.wait_ns = wait_ns;
     p.diag = diag;
@@ -274,7 +282,18 @@ BML_API bml_status bml_attn_tree(const void *q_dev, bml_dtype q_dtype, uint32_t 
                                  size_t workspace_bytes, void *stream) {
     return attn_tree("bml_attn_tree", q_dev, q_dtype, n_tokens, n_heads, n_kv_heads, head_dim, k_pool, v_pool, kv_dtype, n_pages,
                      page_size, block_table, max_pages, kv_lens, node_start, n_seqs, mask, n_words, scale, out_dev, workspace,
-                     workspace_bytes, bml::kWaitNs, 0u, stream);
+                     workspace_bytes, 0u, 0u, bml::kWaitNs, 0u, stream);
+}
+
+BML_API bml_status bml_attn_tree_sized(const void *q_dev, bml_dtype q_dtype, uint32_t n_tokens, uint32_t n_heads,
+                                       uint32_t n_kv_heads, uint32_t head_dim, const void *k_pool, const void *v_pool,
+                                       bml_dtype kv_dtype, uint32_t n_pages, uint32_t page_size, const int32_t *block_table,
+                                       uint32_t max_pages, const int32_t *kv_lens, const int32_t *node_start, uint32_t n_seqs,
+                                       const uint64_t *mask, uint32_t n_words, float scale, void *out_dev, void *workspace,
+                                       size_t workspace_bytes, uint32_t n_live, uint32_t max_nodes, void *stream) {
+    return attn_tree("bml_attn_tree_sized", q_dev, q_dtype, n_tokens, n_heads, n_kv_heads, head_dim, k_pool, v_pool, kv_dtype,
+                     n_pages, page_size, block_table, max_pages, kv_lens, node_start, n_seqs, mask, n_words, scale, out_dev,
+                     workspace, workspace_bytes, n_live, max_nodes, bml::kWaitNs, 0u, stream);
 }
 
 BML_API bml_status bml_diag_attn_tree(const void *q_dev, bml_dtype q_dtype, uint32_t n_tokens, uint32_t n_heads,
@@ -287,7 +306,28 @@ BML_API bml_status bml_diag_attn_tree(const void *q_dev, bml_dtype q_dtype, uint
     if (flags & ~BML_DIAG_STALL) return api_fail(BML_E_INVALID, "%s: flags 0x%x", fn, flags);
     return attn_tree(fn, q_dev, q_dtype, n_tokens, n_heads, n_kv_heads, head_dim, k_pool, v_pool, kv_dtype, n_pages, page_size,
                      block_table, max_pages, kv_lens, node_start, n_seqs, mask, n_words, scale, out_dev, workspace, workspace_bytes,
-                     wait_ns ? wait_ns : bml::kWaitNs, (flags & BML_DIAG_STALL) ? bml::kTreeStall : 0u, stream);
+                     0u, 0u, wait_ns ? wait_ns : bml::kWaitNs, (flags & BML_DIAG_STALL) ? bml::kTreeStall : 0u, stream);
+}
+
+BML_API bml_status bml_diag_attn_tree_form(bml_dtype q_dtype, bml_dtype kv_dtype, uint32_t n_tokens, uint32_t n_heads,
+                                           uint32_t n_kv_heads, uint32_t head_dim, uint32_t page_size, uint32_t max_pages,
+                                           uint32_t n_seqs, uint32_t n_live, uint32_t max_nodes, int *form) {
+    const char *fn = "bml_diag_attn_tree_form";
+    if (!form || page_shift(page_size) < 0 || n_kv_heads == 0 || n_heads % n_kv_heads || n_seqs == 0)
+        return api_fail(BML_E_INVALID, "%s: bad argument", fn);
+    bml::TreeArgs a = {};
+    a.D = head_dim;
+    a.kv_type = kv_dtype;
+    a.num_sms = sm_count(this_device());
+    a.p.q_type = q_dtype;
+    a.p.n_kv = n_kv_heads;
+    a.p.group = n_heads / n_kv_heads;
+    a.p.max_pages = max_pages;
+    a.p.page_shift = (uint32_t)page_shift(page_size);
+    a.p.scale_log2 = 1.f;
+    tree_rows(a, n_tokens, a.p.group, n_seqs, n_live, max_nodes);
+    *form = (int)bml::tree_form(a);
+    return bml::api_ok();
 }
 
 BML_API bml_status bml_paged_commit(void *k_pool, void *v_pool, uint32_t n_layers, uint32_t n_pages, uint32_t page_size,

@@ -25,7 +25,7 @@ namespace {
 
 using PlanFn = decltype(&bml_paged_plan);
 using AppendFn = decltype(&bml_paged_append);
-using TreeFn = decltype(&bml_attn_tree);
+using TreeFn = decltype(&bml_attn_tree_sized);
 using CommitFn = decltype(&bml_paged_commit);
 PlanFn g_plan = nullptr;
 AppendFn g_append = nullptr;
@@ -188,7 +188,7 @@ PyObject *append_impl(PyObject *const *a) {
     return ret;
 }
 
-// q, k_pool, v_pool, block_table, kv_lens, node_start, mask, scale -> out
+// q, k_pool, v_pool, block_table, kv_lens, node_start, mask, scale, n_live, max_new -> out
 PyObject *tree_impl(PyObject *const *a) {
     const at::Tensor *q = plain(a[0], 3), *k = plain(a[1], 4), *lens = plain(a[4], 1);
     USUAL(q && k && lens);
@@ -206,7 +206,8 @@ PyObject *tree_impl(PyObject *const *a) {
         USUAL(mask && mask->size(0) == n_tokens && mask->size(1) >= 1 && mask->size(1) <= 4);
     }
     const int64_t ws_bytes = tree_bytes(dev.index(), d);
-    USUAL(PyFloat_CheckExact(a[7]) && ws_bytes > 0);
+    int64_t live, most;
+    USUAL(PyFloat_CheckExact(a[7]) && ws_bytes > 0 && integer(a[8], &live) && integer(a[9], &most));
     at::Tensor out = fresh(q->sizes(), q->scalar_type(), dev), ws = fresh({ws_bytes}, at::kByte, dev);
     const bml_status st =
         g_tree(q->const_data_ptr(), (bml_dtype)code(q->scalar_type()), (uint32_t)n_tokens, (uint32_t)q->size(1),
@@ -215,7 +216,7 @@ PyObject *tree_impl(PyObject *const *a) {
                lens->const_data_ptr<int32_t>(), start->const_data_ptr<int32_t>(), (uint32_t)n,
                mask ? reinterpret_cast<const uint64_t *>(mask->const_data_ptr<int64_t>()) : nullptr,
                mask ? (uint32_t)mask->size(1) : 0u, (float)PyFloat_AS_DOUBLE(a[7]), out.mutable_data_ptr(), ws.mutable_data_ptr(),
-               (size_t)ws_bytes, stream_of(dev));
+               (size_t)ws_bytes, (uint32_t)live, (uint32_t)most, stream_of(dev));
     USUAL(st == BML_OK);
     return THPVariable_Wrap(std::move(out));
 }
@@ -287,7 +288,7 @@ PyObject *set_calls(PyObject *, PyObject *const *args, Py_ssize_t n) {
 PyMethodDef methods[] = {
     ENTRY(plan, 10),
     ENTRY(append, 9),
-    ENTRY(tree, 8),
+    ENTRY(tree, 10),
     ENTRY(commit, 8),
     {"set_calls", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&set_calls)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -592,17 +592,17 @@ cudaError_t launch_f32(TreeParams p, int num_sms, cudaStream_t st) {
 }
 
 template <int D, typename KT>
-cudaError_t launch_rows(const TreeParams &p, uint32_t rows, int num_sms, cudaStream_t st) {
+cudaError_t launch_rows(const TreeArgs &a, cudaStream_t st) {
     // above 16 rows one CTA covers 64
-    return rows > 16 ? launch_f32<D, KT, 4>(p, num_sms, st) : launch_f32<D, KT, 1>(p, num_sms, st);
+    return a.fits(16) ? launch_f32<D, KT, 1>(a.p, a.num_sms, st) : launch_f32<D, KT, 4>(a.p, a.num_sms, st);
 }
 
 template <int D>
 cudaError_t launch_kv(const TreeArgs &a, cudaStream_t st) {
     switch (a.kv_type) {
-        case BML_F32: return launch_rows<D, float>(a.p, a.rows, a.num_sms, st);
-        case BML_F16: return launch_rows<D, __half>(a.p, a.rows, a.num_sms, st);
-        case BML_BF16: return launch_rows<D, __nv_bfloat16>(a.p, a.rows, a.num_sms, st);
+        case BML_F32: return launch_rows<D, float>(a, st);
+        case BML_F16: return launch_rows<D, __half>(a, st);
+        case BML_BF16: return launch_rows<D, __nv_bfloat16>(a, st);
     }
     return cudaErrorInvalidValue;
 }
@@ -627,7 +627,7 @@ size_t tree_workspace_bytes(uint32_t D, int num_sms) {
     return (size_t)2 * num_sms * kTreeMaxRows * (D + 2) * sizeof(float);
 }
 
-cudaError_t launch_tree(const TreeArgs &a, cudaStream_t st) {
+TreeForm tree_form(const TreeArgs &a) {
     // All but tree_f32_kernel scale masked scores after they were set to -inf, so a
     // scale of 0 is its.  16-bit pages:  Up to 8 rows a kv head (on average): the
     // form with positions as MMA rows (64 x 4000, d = 64, 8 rows: 49 us, 73 with
@@ -637,19 +637,35 @@ cudaError_t launch_tree(const TreeArgs &a, cudaStream_t st) {
     // rows 82 against 93, 48 rows 78 against 144, 16 rows 82 against 74; but one
     // request of 708 positions, 4 kv heads, 64 rows 15 against 11 us).  How much
     // work there is the host knows only as a bound, the tables' width.
+    // Rows count as TreeArgs::fits says: a caller that knows that most requests are
+    // idle, or one much wider than the others, does not get a form that reads the
+    // wide one's K and V for 8 rows at a time (1 of 131,008 positions and 64 nodes among
+    // 64 places, d = 128: 170 us, 1567 with tree_few.cu).  For 32-bit queries over 16-bit
+    // pages the forms differ little in a row's time and much in a request's, so the
+    // average decides (60 of one token and 4 of 64, 4000 positions: 618 us in row groups
+    // of 32, 917 of 64; the former one 1485 with groups of 64, 2204 with 8).
     // 32-bit pages, more than 16 rows: tcgen05, with d = 64 where there is work
     // (d = 128: 64 requests of 1000 positions, 20 rows 247 us against 391, 1 of 700
     // 19.5 against 17.4, 64 rows 20.7 against 22.1; with 16 rows 247 against 166.
     // d = 64: 64 of 1000, 32 rows 180 against 212; 1 of 700 14.5 against 12.6).
-    const uint64_t most = (((uint64_t)a.p.max_pages << a.p.page_shift) + kTreeTile - 1) / kTreeTile * a.p.n_seqs * a.p.n_kv;
+    const uint64_t most = (((uint64_t)a.p.max_pages << a.p.page_shift) + kTreeTile - 1) / kTreeTile * a.live * a.p.n_kv;
     const bool little = most <= 2ull * a.num_sms;
     if (a.p.scale_log2 > 0.f && a.kv_type != BML_F32) {
-        if (a.rows <= 8) return launch_tree_few(a, st);
-        const bool small = little || a.rows <= (a.D == 128 ? 8u : 16u);
-        if (a.p.q_type == BML_F32 || !tree_umma_fits(a) || (small && a.rows <= 64)) return launch_tree_warp(a, st);
-        return launch_tree_umma(a, st);
+        if (a.fits(8)) return TreeForm::kFew;
+        const bool small = little || a.fits(a.D == 128 ? 8 : 16);
+        return a.p.q_type == BML_F32 || !tree_umma_fits(a) || (small && a.fits(64)) ? TreeForm::kWarp : TreeForm::kUmma;
     }
-    if (a.p.scale_log2 > 0.f && a.rows > 16 && tree_umma_fits(a) && !(a.D == 64 && little)) return launch_tree_umma32(a, st);
+    return a.p.scale_log2 > 0.f && !a.fits(16) && tree_umma_fits(a) && !(a.D == 64 && little) ? TreeForm::kUmma32 : TreeForm::kF32;
+}
+
+cudaError_t launch_tree(const TreeArgs &a, cudaStream_t st) {
+    switch (tree_form(a)) {
+        case TreeForm::kFew: return launch_tree_few(a, st);
+        case TreeForm::kWarp: return launch_tree_warp(a, st);
+        case TreeForm::kUmma: return launch_tree_umma(a, st);
+        case TreeForm::kUmma32: return launch_tree_umma32(a, st);
+        case TreeForm::kF32: break;
+    }
     return a.D == 128 ? launch_kv<128>(a, st) : launch_kv<64>(a, st);
 }
 

@@ -46,9 +46,19 @@ struct TreeArgs {
     TreeParams p;
     uint32_t D;
     bml_dtype kv_type;
-    uint32_t rows;  // rows of a request and kv head, on average
+    // Rows of a request and kv head: on average over the requests with new tokens,
+    // and of the widest request (as far as the caller knows; else the average).
+    uint32_t rows, widest;
+    uint32_t live;  // requests with new tokens, at most
     int num_sms;
+    // Whether a form with r rows a row group is for the batch: it fits the average,
+    // and reads no request's K and V more than four times (32-bit queries over 16-bit
+    // pages: widest is the average, see tree_form).
+    bool fits(uint32_t r) const { return rows <= r && widest <= 4 * r; }
 };
+// The kernels: tree.cu, tree_few.cu, tree_warp.cu, tree_umma.cu, tree_umma32.cu.
+enum class TreeForm { kF32, kFew, kWarp, kUmma, kUmma32 };
+TreeForm tree_form(const TreeArgs &a);
 
 constexpr uint32_t kTreeMaxRows = 256;  // rows of the largest partial slot
 cudaError_t launch_tree_merge(const TreeParams &p, uint32_t D, int grid, cudaStream_t st);

@@ -1,6 +1,6 @@
-// tree_warp.cu -- attention of drafted tokens over a paged cache for few rows
-// (up to 64 a kv head) over 16-bit pages: 16-bit queries of the pages' type, or
-// 32-bit queries.
+// tree_warp.cu -- attention of drafted tokens over a paged cache of 16-bit pages:
+// 16-bit queries of the pages' type with few rows (up to 64 a kv head) or more than
+// 128 q heads a kv head, and 32-bit queries of more than 8 rows, however many.
 //
 // The mathematics and the schedule are those of tree.cu / tree.cuh.  With few
 // rows the work is to stream K and V: 4 * rows FLOP per 2-byte K/V element
@@ -456,9 +456,9 @@ cudaError_t launch_w(TreeParams p, int num_sms, cudaStream_t st) {
 
 template <int D, bool kF16, bool kQ32>
 cudaError_t launch_rows(const TreeArgs &a, cudaStream_t st) {
-    if (a.rows > 32) return launch_w<D, kF16, 4, kQ32>(a.p, a.num_sms, st);
-    if (a.rows > 16) return launch_w<D, kF16, 2, kQ32>(a.p, a.num_sms, st);
-    return launch_w<D, kF16, 1, kQ32>(a.p, a.num_sms, st);
+    if (a.fits(16)) return launch_w<D, kF16, 1, kQ32>(a.p, a.num_sms, st);
+    if (a.fits(32)) return launch_w<D, kF16, 2, kQ32>(a.p, a.num_sms, st);
+    return launch_w<D, kF16, 4, kQ32>(a.p, a.num_sms, st);
 }
 
 template <int D>

@@ -99,7 +99,7 @@ def _load():
     from . import _torch_calls
     lib = L.lib()
     _torch_calls.set_calls(*(C.cast(getattr(lib, f), C.c_void_p).value for f in (
-        "bml_paged_plan", "bml_paged_append", "bml_attn_tree", "bml_paged_commit", "bml_attn_tree_workspace_size")))
+        "bml_paged_plan", "bml_paged_append", "bml_attn_tree_sized", "bml_paged_commit", "bml_attn_tree_workspace_size")))
     _fast = _torch_calls
     return _fast
 
@@ -267,7 +267,7 @@ def tree_workspace_size(head_dim: int, device=None) -> int:
 def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
                    kv_lens: torch.Tensor, node_start: torch.Tensor, mask: torch.Tensor | None = None,
                    scale: float = -1.0, out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
-                   stream=None) -> torch.Tensor:
+                   stream=None, n_live: int = 0, max_new: int = 0) -> torch.Tensor:
     """Attention of every request's new tokens over its pages.  q
     [n_tokens, n_heads, d] holds request i's T tokens in rows
     node_start[i]..node_start[i+1]; a token attends over the request's first
@@ -281,9 +281,14 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
 
     workspace: an uint8 tensor of tree_workspace_size bytes for calls that
     must not allocate; calls that share one must not overlap.  By default
-    scratch comes from torch's allocator, on the call's stream."""
+    scratch comes from torch's allocator, on the call's stream.
+
+    n_live, max_new: how many requests have new tokens, and the most of one,
+    where the host knows it (0: not).  The kernel is chosen by them, else by the
+    average over all requests; results are right whatever they say."""
     if stream is None and out is None and workspace is None:
-        r = (_fast or _load()).tree(q, k_pool, v_pool, block_table, kv_lens, node_start, mask, scale)
+        r = (_fast or _load()).tree(q, k_pool, v_pool, block_table, kv_lens, node_start, mask, scale,
+                                    n_live, max_new)
         if r is not None:
             return r
     a_q = _data(q, "q", 3)
@@ -306,6 +311,8 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
         rows, n_words = mask.shape
         if rows != n_tokens or not 1 <= n_words <= MAX_NODES // 64:
             raise ValueError(f"mask must be [{n_tokens}, 1 to {MAX_NODES // 64}], got {tuple(mask.shape)}")
+    if not (0 <= n_live <= 0x7fffffff and 0 <= max_new <= 0x7fffffff):
+        raise ValueError("n_live and max_new must not be negative")
     ctx = _enter(dev, stream)
     try:
         if out is None:
@@ -317,9 +324,9 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
         else:
             _ints(workspace, "workspace", dev, dtype=torch.uint8)
-        _call("bml_attn_tree", a_q, dtype_code(dtype), n_tokens, n_heads, n_kv, d, a_k, a_v, dtype_code(k_pool.dtype),
+        _call("bml_attn_tree_sized", a_q, dtype_code(dtype), n_tokens, n_heads, n_kv, d, a_k, a_v, dtype_code(k_pool.dtype),
               n_pages, page_size, a_table, max_pages, a_len, a_start, n, a_mask, n_words, scale, out.data_ptr(),
-              workspace.data_ptr(), workspace.shape[0], _raw_stream(dev.index))
+              workspace.data_ptr(), workspace.shape[0], n_live, max_new, _raw_stream(dev.index))
     finally:
         if ctx is not None:
             ctx.__exit__(None, None, None)
@@ -400,7 +407,8 @@ class PagedBatcher:
         self.free, self.used = torch.arange(n_pages, **i32), torch.zeros(1, **i32)
         self._rows: dict = {}    # request -> its row of the tables
         self._plan = None        # of the step that has begun
-        self._new = None         # new tokens of each row (host)
+        self._new = None         # new tokens of each row (host),
+        self._live = self._most = 0  # how many rows have some, the most of one
 
     @property
     def active(self) -> list:
@@ -483,7 +491,7 @@ class PagedBatcher:
         if tree and most > MAX_NODES:
             raise ValueError(f"{most} drafted tokens for a request (at most {MAX_NODES})")
         dev = self.device
-        self._new = counts
+        self._new, self._live, self._most = counts, sum(x > 0 for x in counts), most
         return page_plan(self.lens, torch.tensor(counts, dtype=torch.int32, device=dev), self.owned, self.table,
                          self.free, self.used, self.page_size, sum(counts),
                          torch.tensor(parents, dtype=torch.int32, device=dev) if tree else None,
@@ -520,7 +528,7 @@ class PagedBatcher:
         paged_append(q, k_new, v_new, p.slots, p.positions if self.rope else None, self.k[layer], self.v[layer],
                      theta=self.theta, stream=stream)
         return tree_attention(q, self.k[layer], self.v[layer], self.table, p.kv_lens, p.node_start, mask=p.mask,
-                              scale=self.scale, out=out, stream=stream)
+                              scale=self.scale, out=out, stream=stream, n_live=self._live, max_new=self._most)
 
     def commit(self, paths: dict | None = None) -> None:
         """Ends the step.  paths: request -> the accepted nodes, in order

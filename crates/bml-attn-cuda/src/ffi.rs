@@ -102,6 +102,12 @@ extern "C" {
                          page_size: u32, block_table: *const i32, max_pages: u32, kv_lens: *const i32,
                          node_start: *const i32, n_seqs: u32, mask: *const u64, n_words: u32, scale: f32,
                          out: *mut c_void, ws: *mut c_void, ws_bytes: usize, stream: *mut c_void) -> bml_status;
+    pub fn bml_attn_tree_sized(q: *const c_void, q_dtype: bml_dtype, n_tokens: u32, n_heads: u32, n_kv: u32,
+                               head_dim: u32, k_pool: *const c_void, v_pool: *const c_void, kv: bml_dtype,
+                               n_pages: u32, page_size: u32, block_table: *const i32, max_pages: u32,
+                               kv_lens: *const i32, node_start: *const i32, n_seqs: u32, mask: *const u64,
+                               n_words: u32, scale: f32, out: *mut c_void, ws: *mut c_void, ws_bytes: usize,
+                               n_live: u32, max_nodes: u32, stream: *mut c_void) -> bml_status;
     pub fn bml_paged_commit(k_pool: *mut c_void, v_pool: *mut c_void, n_layers: u32, n_pages: u32, page_size: u32,
                             n_kv: u32, head_dim: u32, kv: bml_dtype, block_table: *const i32, max_pages: u32,
                             lens: *const i32, kv_lens: *const i32, node_start: *const i32, n: u32,

@@ -506,6 +506,23 @@ bml_status bml_attn_tree(const void *q_dev, bml_dtype q_dtype,
                          void *out_dev, void *workspace,
                          size_t workspace_bytes, void *stream);
 
+/* bml_attn_tree for a caller that knows more of its batch: n_live requests have
+ * new tokens (0: not known, all n_seqs), the most of one are max_nodes (0: not
+ * known, the average).  The kernel is chosen by them, where bml_attn_tree has
+ * only the average over all n_seqs; results are right whatever they say. */
+bml_status bml_attn_tree_sized(const void *q_dev, bml_dtype q_dtype,
+                               uint32_t n_tokens, uint32_t n_heads,
+                               uint32_t n_kv_heads, uint32_t head_dim,
+                               const void *k_pool, const void *v_pool,
+                               bml_dtype kv_dtype, uint32_t n_pages,
+                               uint32_t page_size, const int32_t *block_table,
+                               uint32_t max_pages, const int32_t *kv_lens,
+                               const int32_t *node_start, uint32_t n_seqs,
+                               const uint64_t *mask, uint32_t n_words,
+                               float scale, void *out_dev, void *workspace,
+                               size_t workspace_bytes, uint32_t n_live,
+                               uint32_t max_nodes, void *stream);
+
 /* Commits the accepted path of every request's draft: in the K and V pools of
  * all n_layers layers (layer l at pool + l * n_pages * page_size * row), row
  * lens[i] + path[i][k] moves to row lens[i] + k for k < n_accept[i], and

@@ -59,6 +59,15 @@ bml_status bml_diag_attn_tree(const void *q_dev, bml_dtype q_dtype,
                               size_t workspace_bytes, uint64_t wait_ns,
                               uint32_t flags, void *stream);
 
+/* Which kernel bml_attn_tree_sized takes for such a batch: 0 tree.cu, 1
+ * tree_few.cu, 2 tree_warp.cu, 3 tree_umma.cu, 4 tree_umma32.cu.  Host only. */
+bml_status bml_diag_attn_tree_form(bml_dtype q_dtype, bml_dtype kv_dtype,
+                                   uint32_t n_tokens, uint32_t n_heads,
+                                   uint32_t n_kv_heads, uint32_t head_dim,
+                                   uint32_t page_size, uint32_t max_pages,
+                                   uint32_t n_seqs, uint32_t n_live,
+                                   uint32_t max_nodes, int *form);
+
 /* Evaluates 2^x with the device exponential the attention kernels use
  * (ex2.approx on the SFU), so tests can bound its error against CUDA's
  * exp2f.  n must be even.  Asynchronous. */
