@@ -514,13 +514,16 @@ struct TreeSpan {
 // column that came out NaN though the row's sum of weights is a number, and all
 // columns where a node's values were zeroed, are looked up here: weights are
 // positive, so such a column is the sum of its values that are not finite.
-// o: n columns from `col` on, un-normalised.  Rare, from global memory.
+// o: n columns from `col` on, un-normalised; nan: some of them are NaN (else only
+// the end of the request is looked at, and added).  Rare, from global memory.
 template <int D, typename KT>
-__device__ __noinline__ void tree_nonfinite(const TreeParams &p, const TreeSpan &a, uint32_t col, uint32_t n, float *o) {
-    const uint32_t P = a.s.L - min(a.s.T, a.s.L), end = min(a.hi, a.s.L);
+__device__ __noinline__ void tree_nonfinite(const TreeParams &p, const TreeSpan &a, uint32_t col, uint32_t n, bool nan, float *o) {
+    // tree_f32_kernel zeroes in whole blocks, of up to 32 positions: some before the
+    // nodes, and what is not finite may be added twice
+    const uint32_t P = a.s.L - min(a.s.T, a.s.L), begin = nan ? a.lo : max(a.lo, P - min(P, 32u)), end = min(a.hi, a.s.L);
     for (uint32_t c = 0; c < n; c += 4) {
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        for (uint32_t pos = a.lo; pos < end; ++pos) {
+        for (uint32_t pos = begin; pos < end; ++pos) {
             if (pos >= P && !tree_sees(p, a.s, a.t, pos - P)) continue;
             const uint32_t page = (uint32_t)p.table[(size_t)a.seq * p.max_pages + (pos >> p.page_shift)];
             if (page >= p.n_pages) continue;
@@ -533,7 +536,7 @@ __device__ __noinline__ void tree_nonfinite(const TreeParams &p, const TreeSpan 
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (sum[e] != 0.f) o[c + e] = sum[e];
+            if (sum[e] != 0.f) o[c + e] = nan ? sum[e] : o[c + e] + sum[e];
     }
 }
 // For four columns, where they need it.  l: the row's sum of weights; odd: the
@@ -545,10 +548,11 @@ __device__ __forceinline__ void tree_nonfinite4(const TreeParams &p, const TreeS
     if (__builtin_expect((odd || any != any) && l == l, 0)) {
         const TreeSpan a = {g.seq, head, (g.row0 + row) / p.group, g.t0 << p.tile_shift, g.t1 << p.tile_shift, g.s};
         float o[4] = {x.x, x.y, x.z, x.w};
-        tree_nonfinite<D, KT>(p, a, col, 4, o);
+        tree_nonfinite<D, KT>(p, a, col, 4, any != any, o);
         x = make_float4(o[0], o[1], o[2], o[3]);
     }
 }
+
 // 16 bytes global -> shared; bytes = 0 writes zeros and reads nothing.
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");

@@ -181,12 +181,12 @@ __device__ __noinline__ void fix_v(uint8_t *row, bool node_row, bool past, volat
 
 // tree_nonfinite for 32 columns of a row of node t.
 template <int D, bool kF16>
-__device__ __noinline__ void add_nonfinite(const TreeParams &p, const volatile Board *b, uint32_t t, uint32_t col, float *o) {
+__device__ __noinline__ void add_nonfinite(const TreeParams &p, const volatile Board *b, uint32_t t, uint32_t col, bool nan, float *o) {
     TreeSpan a = {b->seq, b->head, t, b->t0 * BN, (b->t0 + (b->packed & 0xfffffffu)) * BN, {}};
     a.s.first = b->first;
     a.s.T = b->T;
     a.s.L = b->L;
-    tree_nonfinite<D, typename std::conditional<kF16, __half, __nv_bfloat16>::type>(p, a, col, 32, o);
+    tree_nonfinite<D, typename std::conditional<kF16, __half, __nv_bfloat16>::type>(p, a, col, 32, nan, o);
 }
 
 template <int D, bool kF16>
@@ -735,7 +735,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
                             float tmp[32];  // its address is taken, o's is not
 #pragma unroll
                             for (int u = 0; u < 32; ++u) tmp[u] = o[u];
-                            add_nonfinite<D, kF16>(p, b, t, col, tmp);
+                            add_nonfinite<D, kF16>(p, b, t, col, any[0] != any[0], tmp);
 #pragma unroll
                             for (int u = 0; u < 32; ++u) o[u] = tmp[u];
                         }

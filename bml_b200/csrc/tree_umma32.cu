@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
                         float tmp[32];  // its address is taken, o's is not
 #pragma unroll
                         for (int u = 0; u < 32; ++u) tmp[u] = o[c + u];
-                        tree_nonfinite<D, float>(p, a, half * (D / 2) + c, 32, tmp);
+                        tree_nonfinite<D, float>(p, a, half * (D / 2) + c, 32, any[0] != any[0], tmp);
 #pragma unroll
                         for (int u = 0; u < 32; ++u) o[c + u] = tmp[u];
                     }
