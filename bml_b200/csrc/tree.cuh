@@ -55,6 +55,13 @@ struct TreeArgs {
     // and reads no request's K and V more than four times (32-bit queries over 16-bit
     // pages: widest is the average, see tree_form).
     bool fits(uint32_t r) const { return rows <= r && widest <= 4 * r; }
+    // Tiles of kTreeTile positions of all requests and kv heads, at most: the lengths
+    // are on the device, so the tables' width stands for them.
+    uint64_t most_tiles() const {
+        return (((uint64_t)p.max_pages << p.page_shift) + kTreeTile - 1) / kTreeTile * live * p.n_kv;
+    }
+    // Whether row groups of 16 make no more of such tiles than two an SM.
+    bool little16() const { return most_tiles() * ((rows + 15) / 16) <= 2ull * num_sms; }
 };
 // The kernels: tree.cu, tree_few.cu, tree_warp.cu, tree_umma.cu, tree_umma32.cu.
 enum class TreeForm { kF32, kFew, kWarp, kUmma, kUmma32 };

@@ -52,3 +52,16 @@ def test_narrow_batches_keep_their_kernel(L):
     assert form(L, "bf16", "bf16", 8, 8, 64, 64, n_live=1, max_new=8, positions=704, n_kv=4) == "warp"
     # and without a hint the average over all requests
     assert form(L, "bf16", "bf16", 64, 4, 128, 64) == form(L, "bf16", "bf16", 64, 4, 128, 64, 64, 1)
+
+
+def test_32_bit_pages_by_the_work(L):
+    """Few rows, or little work for the longer start of the tcgen05 form, take row groups of 16."""
+    one = dict(group=4, d=128, n_seqs=1)
+    assert form(L, "f32", "f32", 5, positions=704, **one) == "f32"
+    assert form(L, "f32", "f32", 30, positions=704, **one) == "umma32"
+    assert form(L, "f32", "f32", 5, positions=2048, **one) == "f32"
+    assert form(L, "f32", "f32", 16, positions=2048, **one) == "umma32"
+    assert form(L, "f32", "f32", 5, positions=131072, **one) == "umma32"
+    assert form(L, "f32", "f32", 4, positions=131072, **one) == "f32"
+    assert form(L, "f32", "f32", 16, 8, 64, 1, positions=704, n_kv=4) == "f32"
+    assert form(L, "f32", "f32", 16, 8, 64, 1, positions=4096, n_kv=4) == "umma32"
