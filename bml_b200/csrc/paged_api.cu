@@ -81,6 +81,13 @@ bool overlap(std::initializer_list<Span> written, std::initializer_list<Span> re
         }
     return false;
 }
+// Whether two of the arrays that a call writes overlap.
+bool overlap(std::initializer_list<Span> written) {
+    for (const Span *a = written.begin(); a != written.end(); ++a)
+        for (const Span *b = a + 1; b != written.end(); ++b)
+            if (overlap({*a}, {*b})) return true;
+    return false;
+}
 
 }  // namespace
 
@@ -106,10 +113,12 @@ BML_API bml_status bml_paged_plan(const int32_t *lens, const int32_t *n_new, con
     }
     const uint64_t n4 = 4ull * n, t4 = 4ull * n_tokens;
     const bool drafts = n_tokens && parents;
-    if (overlap({{node_start, n4 + 4}, {kv_lens, n4}, {owned_out, n4}, {free_used_out, 4}, {status, n4}, {slots, 2 * t4},
-                 {positions, t4}, {drafts ? mask : nullptr, 2 * t4 * n_words}, {block_table, n4 * max_pages}},
-                {{lens, n4}, {n_new, n4}, {owned, n4}, {free_pages, 4ull * n_free}, {free_used, 4}, {drafts ? parents : nullptr, t4}}))
+    const std::initializer_list<Span> written = {{node_start, n4 + 4}, {kv_lens, n4}, {owned_out, n4}, {free_used_out, 4}, {status, n4},
+                                                 {slots, 2 * t4}, {positions, t4}, {drafts ? mask : nullptr, 2 * t4 * n_words},
+                                                 {block_table, n4 * max_pages}};
+    if (overlap(written, {{lens, n4}, {n_new, n4}, {owned, n4}, {free_pages, 4ull * n_free}, {free_used, 4}, {drafts ? parents : nullptr, t4}}))
         return api_fail(BML_E_INVALID, "%s: results need buffers of their own, not those of lens, n_new, owned, parents or the free list", fn);
+    if (overlap(written)) return api_fail(BML_E_INVALID, "%s: results overlap one another", fn);
     bml::PlanParams p = {};
     p.lens = lens;
     p.n_new = n_new;
@@ -163,6 +172,13 @@ BML_API bml_status bml_paged_append(const void *q_dev, const void *k_dev, const 
         const uint64_t bytes = (uint64_t)n_tokens * n_heads * head_dim * bml::dtype_size(src_dtype);
         if ((a < b ? b - a : a - b) < bytes) return api_fail(BML_E_INVALID, "%s: q_out overlaps q", fn);
     }
+    // tokens are read and stored by CTAs of their own
+    const uint64_t row = (uint64_t)n_kv_heads * head_dim, src = (uint64_t)n_tokens * row * bml::dtype_size(src_dtype);
+    const uint64_t qb = (uint64_t)n_tokens * n_heads * head_dim * bml::dtype_size(src_dtype), pool = n_rows * row * bml::dtype_size(kv_dtype);
+    if (overlap({{k_pool, pool}, {v_pool, pool}, {q_out_dev, qb}},
+                {{k_dev, src}, {v_dev, src}, {slots, 8ull * n_tokens}, {positions, 4ull * n_tokens}}) ||
+        overlap({{k_pool, pool}, {v_pool, pool}}, {{q_dev, qb}}) || overlap({{k_pool, pool}, {v_pool, pool}, {q_out_dev, qb}}))
+        return api_fail(BML_E_INVALID, "%s: the pools and q_out must not overlap one another or what is read", fn);
     bml::PagedAppendParams p = {};
     p.q = q_dev;
     p.q_out = q_out_dev;
@@ -235,6 +251,13 @@ bml_status attn_tree(const char *fn, const void *q_dev, bml_dtype q_dtype, uint3
     const uintptr_t qa = reinterpret_cast<uintptr_t>(q_dev), oa = reinterpret_cast<uintptr_t>(out_dev);
     if ((qa < oa ? oa - qa : qa - oa) < (uint64_t)n_tokens * n_heads * head_dim * es)
         return api_fail(BML_E_INVALID, "%s: out overlaps q", fn);
+    const uint64_t qb = (uint64_t)n_tokens * n_heads * head_dim * es, n4 = 4ull * n_seqs;
+    const uint64_t pool = (uint64_t)n_pages * page_size * n_kv_heads * head_dim * bml::dtype_size(kv_dtype);
+    const std::initializer_list<Span> written = {{out_dev, qb}, {workspace, bml::tree_workspace_bytes(head_dim, sms)}};
+    if (overlap(written, {{q_dev, qb}, {k_pool, pool}, {v_pool, pool}, {block_table, n4 * max_pages}, {kv_lens, n4}, {node_start, n4 + 4},
+                          {mask, 8ull * n_tokens * n_words}}) ||
+        overlap(written))
+        return api_fail(BML_E_INVALID, "%s: out and workspace must not overlap one another or what is read", fn);
     bml::TreeArgs a = {};
     a.D = head_dim;
     a.kv_type = kv_dtype;
@@ -349,6 +372,8 @@ BML_API bml_status bml_paged_commit(void *k_pool, void *v_pool, uint32_t n_layer
     if (overlap({{lens_out, 4ull * n}}, {{lens, 4ull * n}, {kv_lens, 4ull * n}, {node_start, 4ull * n + 4}, {n_accept, 4ull * n},
                                           {path, 4ull * n * max_path}, {block_table, 4ull * n * max_pages}}))
         return api_fail(BML_E_INVALID, "%s: lens_out needs a buffer of its own", fn);
+    const uint64_t pool = (uint64_t)n_layers * n_pages * page_size * row;
+    if (overlap({{k_pool, pool}}, {{v_pool, pool}})) return api_fail(BML_E_INVALID, "%s: k_pool and v_pool overlap", fn);
     bml::CommitParams p = {};
     p.k_pool = static_cast<char *>(k_pool);
     p.v_pool = static_cast<char *>(v_pool);

@@ -455,7 +455,8 @@ bml_status bml_paged_plan(const int32_t *lens, const int32_t *n_new,
  * slot is outside [0, n_rows) is skipped: nothing of it is written.  Angles
  * are f64, the rotation f32; results are rounded once to the destination's
  * type.  Slots of one call must differ (of two tokens with the same slot,
- * either's values may be stored).  head_dim even; pointers aligned to two
+ * either's values may be stored), and the two pools, q_out and what is read must
+ * not overlap.  head_dim even; pointers aligned to two
  * elements; theta at least 2^-16; negative positions count as 0.
  * Asynchronous. */
 bml_status bml_paged_append(const void *q_dev, const void *k_dev,
@@ -479,7 +480,8 @@ bml_status bml_attn_tree_workspace_size(uint32_t head_dim, int32_t device,
  *   q_dev, out_dev: [n_tokens][n_heads][head_dim] in q_dtype: BML_F32 with
  *       pages of any type, or the pages' own 16-bit type;
  *   workspace: bml_attn_tree_workspace_size bytes, 16-byte aligned, no
- *       contents needed; calls that share one must not overlap in time.
+ *       contents needed; calls that share one must not overlap in time.  It and
+ *       out_dev overlap nothing that the call reads.
  * At most 256 nodes a request (64 * n_words with a mask).  Rows that see
  * nothing are zero; so are all rows of a request with kv_lens[i] < T (one
  * that bml_paged_plan refused), with more nodes than that, or with more
@@ -530,7 +532,8 @@ bml_status bml_attn_tree_sized(const void *q_dev, bml_dtype q_dtype,
  * strictly increasing node indices; an entry that is not larger than the one
  * before, or not below the request's node count, ends the path there, and the
  * count with it.  A request with kv_lens[i] != lens[i] + its node count (one
- * that the plan refused) commits nothing.  lens_out is its own buffer.
+ * that the plan refused) commits nothing.  lens_out is its own buffer, and the
+ * two pools must not overlap.
  * Asynchronous. */
 bml_status bml_paged_commit(void *k_pool, void *v_pool, uint32_t n_layers,
                             uint32_t n_pages, uint32_t page_size,
