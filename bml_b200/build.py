@@ -15,6 +15,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libbmlattn.so")
 CALLS = os.path.join(HERE, "_torch_calls.so")
 CALLS_SRC = os.path.join(CSRC, "torch_calls.cpp")
+CALLS_FOR = os.path.join(HERE, "_torch_calls.torch")  # the torch version that CALLS was built with
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -38,7 +39,32 @@ def headers() -> list[str]:
 
 
 def needs_build() -> bool:
-    return _older(LIB, sources() + headers()) or _older(CALLS, [CALLS_SRC, *headers()])
+    return _older(LIB, sources() + headers()) or _calls_stale()
+
+
+def _torch_version() -> str | None:
+    """None without torch or a C++ compiler: then only the C library is built."""
+    try:
+        import torch
+    except ImportError:
+        return None
+    return torch.__version__ if shutil.which(_cxx()) else None
+
+
+def _cxx() -> str:
+    return os.environ.get("CXX", "g++")
+
+
+def _calls_stale() -> bool:
+    """Whether the binding is to be built: it is older than its sources, or for
+    another torch, whose C++ classes it takes apart."""
+    want = _torch_version()
+    if want is None:
+        return False
+    if _older(CALLS, [CALLS_SRC, *headers()]) or not os.path.exists(CALLS_FOR):
+        return True
+    with open(CALLS_FOR) as f:
+        return f.read() != want
 
 
 def _older(target: str, deps: list[str]) -> bool:
@@ -58,7 +84,7 @@ def _build_calls(verbose: bool) -> None:
     cuda = os.path.dirname(os.path.dirname(nvcc_path()))
     inc = [os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
            sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+    cmd = [_cxx(), "-O2", f'-DBML_TORCH_VERSION="{torch.__version__}"', "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *(f"-I{d}" for d in inc),
            "-o", CALLS + ".tmp", CALLS_SRC, "-L" + os.path.join(root, "lib"),
            *(f"-l{x}" for x in ("c10", "c10_cuda", "torch_cpu", "torch_cuda", "torch", "torch_python"))]
@@ -66,6 +92,8 @@ def _build_calls(verbose: bool) -> None:
         print(" ".join(cmd), file=sys.stderr)
     subprocess.run(cmd, check=True)
     os.replace(CALLS + ".tmp", CALLS)
+    with open(CALLS_FOR, "w") as f:
+        f.write(torch.__version__)
 
 
 def _object(src: str, newest_header: float, force: bool, verbose: bool) -> str:
@@ -82,7 +110,8 @@ def _object(src: str, newest_header: float, force: bool, verbose: bool) -> str:
 
 def build(force: bool = False, verbose: bool = False) -> str:
     """Compiles every csrc/*.cu to an object (in parallel, each only when it
-    or a header changed) and links libbmlattn.so; then _torch_calls.so."""
+    or a header changed) and links libbmlattn.so; and _torch_calls.so, unless
+    torch or the C++ compiler is missing (the C library needs neither)."""
     if not force and not needs_build():
         return LIB
     from concurrent.futures import ThreadPoolExecutor
@@ -90,7 +119,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     newest = max((os.path.getmtime(h) for h in headers()), default=0.0)
     srcs = sources()
     with ThreadPoolExecutor(max_workers=min(len(srcs), os.cpu_count() or 4) + 1) as ex:
-        calls = ex.submit(_build_calls, verbose) if force or _older(CALLS, [CALLS_SRC, *headers()]) else None
+        calls = ex.submit(_build_calls, verbose) if _torch_version() and (force or _calls_stale()) else None
         if force or _older(LIB, srcs + headers()):
             objs = list(ex.map(lambda f: _object(f, newest, force, verbose), srcs))
             subprocess.run([nvcc_path(), *ARCH, "-shared", "-o", LIB + ".tmp", *objs], check=True)

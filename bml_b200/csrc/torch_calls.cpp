@@ -6,7 +6,8 @@
 // Every function returns None when anything is not the usual case (an argument
 // that is not a plain contiguous tensor of the right type and shape, another
 // device, a C call that refused); paged.py then takes its own way, which checks
-// again, says what is wrong, or makes the call.  A refused C call has launched
+// again, says what is wrong, or makes the call.  It takes every call where this
+// module is missing or was built for another torch.  A refused C call has launched
 // nothing.  The entry points of libbmlattn.so are handed over by set_calls().
 //
 // Host time of a call beside a B200, against the way through ctypes: page_plan 5.3
@@ -298,4 +299,13 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_calls", nullptr, -1, method
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__torch_calls(void) { return PyModule_Create(&module); }
+// built_for: the torch version, which paged.py compares: the classes above are
+// that version's.
+PyMODINIT_FUNC PyInit__torch_calls(void) {
+    PyObject *m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "built_for", BML_TORCH_VERSION) < 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

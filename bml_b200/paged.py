@@ -20,7 +20,7 @@ one; `stream` defaults to that device's current stream.
 from __future__ import annotations
 
 import ctypes as C
-import os
+import warnings
 
 import torch
 
@@ -90,14 +90,32 @@ def _enter(device: torch.device, stream):
 _fast = None  # csrc/torch_calls.cpp: the usual calls without Python's share of the time
 
 
+class _Wrappers:
+    """In that module's place: leaves every call to the wrappers below."""
+
+    @staticmethod
+    def plan(*args):
+        return None
+
+    append = tree = commit = plan
+
+
 def _load():
-    """Loads that module and gives it the library's entry points."""
+    """Loads that module and gives it the library's entry points.  One that is
+    missing or was built for another torch is not used: the calls are the same
+    through ctypes, 4 to 15 us slower on the host."""
     global _fast
-    path = os.path.join(L.HERE, "_torch_calls.so")
-    if not os.path.exists(path):
-        raise RuntimeError(f"{path} is missing: build it with `python -m bml_b200.build`")
-    from . import _torch_calls
     lib = L.lib()
+    try:
+        from . import _torch_calls
+        found = _torch_calls.built_for
+    except (ImportError, AttributeError) as e:  # none, symbols that this torch lacks, or an older build
+        found = str(e)
+    if found != torch.__version__:
+        warnings.warn(f"bml_b200/_torch_calls.so is not for torch {torch.__version__} ({found}): paged calls go through ctypes; "
+                      "build it with `python -m bml_b200.build`", RuntimeWarning, stacklevel=3)
+        _fast = _Wrappers
+        return _fast
     _torch_calls.set_calls(*(C.cast(getattr(lib, f), C.c_void_p).value for f in (
         "bml_paged_plan", "bml_paged_append", "bml_attn_tree_sized", "bml_paged_commit", "bml_attn_tree_workspace_size")))
     _fast = _torch_calls
