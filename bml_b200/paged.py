@@ -179,8 +179,8 @@ def page_plan(lens: torch.Tensor, n_new: torch.Tensor, owned: torch.Tensor, bloc
     if rows != n:
         raise ValueError(f"block_table must be [{n}, max_pages], got {tuple(block_table.shape)}")
     a_free, a_used = _ints(free_pages, "free_pages", dev), _ints(free_used, "free_used", dev, (1,))
-    if n_tokens < 0:
-        raise ValueError("n_tokens must not be negative")
+    if not (0 <= n_tokens < 1 << 31 and 0 <= page_size < 1 << 31):  # ctypes would cut them to 32 bits
+        raise ValueError(f"n_tokens {n_tokens} and page_size {page_size} must be 0 to 2^31 - 1")
     a_parents = None
     if parents is not None:
         a_parents = _ints(parents, "parents", dev, (n_tokens,))
