@@ -294,8 +294,9 @@ def tree_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, 
     without a mask, over itself and those before it (T = 1: plain decode).
     q is f32, or of the pools' 16-bit type; the result has q's type.  At most
     256 new tokens a request (64 a mask word).  Rows that see nothing, and
-    those of requests that page_plan refused, are zero.  scale < 0 selects
-    1/sqrt(d).
+    those of requests that page_plan refused or that have more new tokens, are
+    zero; rows behind the last request's are not written (in a result that the
+    call allocates they hold anything).  scale < 0 selects 1/sqrt(d).
 
     workspace: an uint8 tensor of tree_workspace_size bytes for calls that
     must not allocate; calls that share one must not overlap.  By default
@@ -550,12 +551,12 @@ class PagedBatcher:
 
     def commit(self, paths: dict | None = None) -> None:
         """Ends the step.  paths: request -> the accepted nodes, in order
-        (strictly increasing); a request that is not named, or None, keeps
-        all its new tokens (right for chains)."""
+        (strictly increasing; [] for none of them); a request that is not named,
+        or whose path is None, keeps all its new tokens (right for chains)."""
         if self._plan is None:
             raise RuntimeError("no step has begun")
         p, paths = self._plan, paths or {}
-        want = {self._rows[r]: [int(a) for a in x] for r, x in paths.items()}
+        want = {self._rows[r]: [int(a) for a in x] for r, x in paths.items() if x is not None}
         for row, x in want.items():
             if any(b <= a for a, b in zip([-1] + x, x)) or (x and x[-1] >= self._new[row]):
                 raise ValueError(f"path {x} is not strictly increasing below {self._new[row]}")
