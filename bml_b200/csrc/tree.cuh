@@ -493,6 +493,30 @@ __device__ __forceinline__ void tf32_split_any(float x, uint32_t &hi, uint32_t &
     lo = __float_as_uint(x - h);
 }
 
+template <bool kF16>
+__device__ __forceinline__ bool odd16(uint16_t x) {  // not finite
+    constexpr uint16_t em = kF16 ? 0x7c00u : 0x7f80u;
+    return (x & em) == em;
+}
+template <bool kF16>
+__device__ __forceinline__ float wide16(uint16_t x) {
+    return kF16 ? __half2float(*reinterpret_cast<const __half *>(&x)) : __uint_as_float((uint32_t)x << 16);
+}
+
+// x as TERMS 16-bit terms, the largest first: x is their sum to 24 (three
+// bf16) or 22 bits (two f16).
+template <bool kF16, int TERMS>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&t)[TERMS]) {
+#pragma unroll
+    for (int i = 0; i < TERMS; ++i) {
+        t[i] = pack2<kF16>(x, y);
+        if (i + 1 < TERMS) {
+            x -= wide16<kF16>((uint16_t)t[i]);
+            y -= wide16<kF16>((uint16_t)(t[i] >> 16));
+        }
+    }
+}
+
 // Four values of a pool row.
 template <typename KT>
 __device__ __forceinline__ float4 tree_load4(const void *pool, size_t at) {

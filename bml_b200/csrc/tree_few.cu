@@ -52,28 +52,6 @@ struct FewParams {
     uint32_t splits;  // warps of a head
 };
 
-template <bool kF16>
-__device__ __forceinline__ bool odd16(uint16_t x) {  // not finite
-    constexpr uint16_t em = kF16 ? 0x7c00u : 0x7f80u;
-    return (x & em) == em;
-}
-template <bool kF16>
-__device__ __forceinline__ float wide16(uint16_t x) {
-    return kF16 ? __half2float(*reinterpret_cast<const __half *>(&x)) : __uint_as_float((uint32_t)x << 16);
-}
-// x and y as TERMS 16-bit terms, the largest first
-template <bool kF16, int TERMS>
-__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&t)[TERMS]) {
-#pragma unroll
-    for (int i = 0; i < TERMS; ++i) {
-        t[i] = pack2<kF16>(x, y);
-        if (i + 1 < TERMS) {
-            x -= wide16<kF16>((uint16_t)t[i]);
-            y -= wide16<kF16>((uint16_t)(t[i] >> 16));
-        }
-    }
-}
-
 template <int D, bool kF16, bool kQ32>
 __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kernel(const __grid_constant__ FewParams fp) {
     using C = NCfg<D, kF16, kQ32>;

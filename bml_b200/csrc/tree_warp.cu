@@ -55,40 +55,6 @@ struct WCfg {
     static constexpr int SMEM = OFF_Q + (kQ32 ? RW * 16 * D * 2 * TERMS : 0);
 };
 
-template <bool kF16>
-__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
-    if (kF16) {
-        __half2 h = __floats2half2_rn(lo, hi);
-        return *reinterpret_cast<uint32_t *>(&h);
-    }
-    __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<uint32_t *>(&h);
-}
-
-template <bool kF16>
-__device__ __forceinline__ bool odd16(uint16_t x) {  // not finite
-    constexpr uint16_t em = kF16 ? 0x7c00u : 0x7f80u;
-    return (x & em) == em;
-}
-template <bool kF16>
-__device__ __forceinline__ float wide16(uint16_t x) {
-    return kF16 ? __half2float(*reinterpret_cast<const __half *>(&x)) : __uint_as_float((uint32_t)x << 16);
-}
-
-// x as TERMS 16-bit terms, the largest first: x is their sum to 24 (three
-// bf16) or 22 bits (two f16).
-template <bool kF16, int TERMS>
-__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&t)[TERMS]) {
-#pragma unroll
-    for (int i = 0; i < TERMS; ++i) {
-        t[i] = pack16<kF16>(x, y);
-        if (i + 1 < TERMS) {
-            x -= wide16<kF16>((uint16_t)t[i]);
-            y -= wide16<kF16>((uint16_t)(t[i] >> 16));
-        }
-    }
-}
-
 template <int D, bool kF16, int RW, bool kQ32>
 __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_constant__ TreeParams p) {
     using C = WCfg<D, kF16, RW, kQ32>;
@@ -425,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
                             make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
                     else
                         *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + at) =
-                            make_uint2(pack16<kF16>(acc.x * inv, acc.y * inv), pack16<kF16>(acc.z * inv, acc.w * inv));
+                            make_uint2(pack2<kF16>(acc.x * inv, acc.y * inv), pack2<kF16>(acc.z * inv, acc.w * inv));
                 }
             }
             __syncthreads();

@@ -217,17 +217,6 @@ __device__ __forceinline__ uint32_t drop_tiny(uint32_t w) {
     return w;
 }
 
-// two f32 -> one 32-bit word of 16-bit values, lo in the low half
-template <bool kF16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    if (kF16) {
-        __half2 h = __floats2half2_rn(lo, hi);
-        return *reinterpret_cast<uint32_t *>(&h);
-    }
-    __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<uint32_t *>(&h);
-}
-
 PFN_cuTensorMapEncodeTiled_v12000 get_encode() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     static std::once_flag once;

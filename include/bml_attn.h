@@ -491,6 +491,8 @@ bml_status bml_attn_tree_workspace_size(uint32_t head_dim, int32_t device,
  * reach the row.  An infinity in V that a row does see makes that column of the
  * row infinite (NaN beside one of the other sign), whatever its weight.
  * Token rows outside the requests' are left as they were.
+ * Sums are divided by the weights' sum at the end: where 2^8 times the sum of |v|
+ * that a row sees leaves f32's range, that column is infinite or NaN.
  * 16-bit queries: scores and sums in f32, the softmax weights rounded to the
  * 16-bit type before P.V, one rounding of the output; 32-bit queries: about
  * f32 precision throughout.  Results are the same from run to run on one
