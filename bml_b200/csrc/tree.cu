@@ -596,7 +596,7 @@ cudaError_t launch_rows(const TreeArgs &a, cudaStream_t st) {
     // Row groups of 16, whose units are more and spread better, or of 64, which read K
     // and V less often (above 16 rows this kernel is for little work, a scale of 0, and
     // groups of more than 128 q heads).
-    return a.fits(16) || a.little16() ? launch_f32<D, KT, 1>(a.p, a.num_sms, st) : launch_f32<D, KT, 4>(a.p, a.num_sms, st);
+    return a.groups16() ? launch_f32<D, KT, 1>(a.p, a.num_sms, st) : launch_f32<D, KT, 4>(a.p, a.num_sms, st);
 }
 
 template <int D>
@@ -646,6 +646,20 @@ TreeForm tree_form(const TreeArgs &a) {
     // pages the forms differ little in a row's time and much in a request's, so the
     // average decides (60 of one token and 4 of 64, 4000 positions: 618 us in row groups
     // of 32, 917 of 64; the former one 1485 with groups of 64, 2204 with 8).
+    // 32-bit pages: row groups of 16 up to 16 rows, 32 with d = 64 (64 requests of 1000
+    // positions, d = 128: 16 rows 172 us, 256 on tcgen05, 20 rows 321 and 256; d = 64: 32
+    // rows 94 and 103; 4 of 2000, 24 rows 18.1 and 23.1, 40 rows 23.4 and 23.6) and where
+    // they make little work for its longer start: one request of 700 positions, d = 128: 20
+    // rows 13.8 us, 18.2 on tcgen05, 64 rows 19.0 and 19.4, 120 rows 25.8 and 21.2; of
+    // 2000: 20 rows 18.8 and 24.8, 64 rows 29.7 and 26.1; d = 64, 700: 128 rows 12.3 and
+    // 14.7, 240 rows 15.6 and 15.0; 2000: 64 rows 13.2 and 13.7, 128 rows 18.3 and 15.4.
+    // Rows count as TreeArgs::fits says: a caller that knows that most requests are
+    // idle, or one much wider than the others, does not get a form that reads the
+    // wide one's K and V for 8 rows at a time (1 of 131,008 positions and 64 nodes among
+    // 64 places, d = 128: 170 us, 1567 with tree_few.cu).  For 32-bit queries over 16-bit
+    // pages the forms differ little in a row's time and much in a request's, so the
+    // average decides (60 of one token and 4 of 64, 4000 positions: 618 us in row groups
+    // of 32, 917 of 64; the former one 1485 with groups of 64, 2204 with 8).
     // 32-bit pages: row groups of 16 up to 16 rows (d = 128, 64 requests of 1000
     // positions: 166 us, 247 on tcgen05; with 20 rows 391 against 247) and where they
     // make little work for its longer start; one request of 700 positions, d = 128: 20
@@ -669,7 +683,7 @@ TreeForm tree_form(const TreeArgs &a) {
         const bool small = little || a.fits(a.D == 128 ? 8 : 16);
         return a.p.q_type == BML_F32 || !tree_umma_fits(a) || (small && a.fits(64)) ? TreeForm::kWarp : TreeForm::kUmma;
     }
-    return a.p.scale_log2 > 0.f && !a.fits(16) && tree_umma_fits(a) && !a.little16() ? TreeForm::kUmma32 : TreeForm::kF32;
+    return a.p.scale_log2 > 0.f && tree_umma_fits(a) && !a.groups16() ? TreeForm::kUmma32 : TreeForm::kF32;
 }
 
 cudaError_t launch_tree(const TreeArgs &a, cudaStream_t st) {

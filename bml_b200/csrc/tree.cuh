@@ -60,8 +60,9 @@ struct TreeArgs {
     uint64_t most_tiles() const {
         return (((uint64_t)p.max_pages << p.page_shift) + kTreeTile - 1) / kTreeTile * live * p.n_kv;
     }
-    // Whether row groups of 16 make no more of such tiles than two an SM.
-    bool little16() const { return most_tiles() * ((rows + 15) / 16) <= 2ull * num_sms; }
+    // 32-bit pages: whether row groups of 16 are for the batch, also where they make
+    // no more of such tiles than two an SM (see tree_form).
+    bool groups16() const { return fits(D == 64 ? 32 : 16) || most_tiles() * ((rows + 15) / 16) <= 2ull * num_sms; }
 };
 // The kernels: tree.cu, tree_few.cu, tree_warp.cu, tree_umma.cu, tree_umma32.cu.
 enum class TreeForm { kF32, kFew, kWarp, kUmma, kUmma32 };

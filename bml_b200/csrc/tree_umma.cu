@@ -25,8 +25,10 @@
 // room for the walk.
 //
 // Measured on B200, 32 requests of 8000 positions, 32 / 8 heads, d = 128: 32
-// nodes (128 rows) 180 us, 5.9 TB/s; 64 nodes (256 rows) 280 us, 960 TFLOP/s,
-// where the tensor pipe and the exponentials share the time as in prefill.cu.
+// nodes (128 rows) 186 us, 5.7 TB/s; 64 nodes (256 rows) 287 us, 940 TFLOP/s.
+// 32 requests of 1024 to 8192, 16 to 64 nodes: tensor pipe busy 48% of the active
+// cycles, the exponentials' unit 34%, issue 33%, each K and V byte read once: no
+// unit is full, the chains wait for their softmax as in prefill.cu.
 //
 // What a row does not see must not reach it: scores are replaced by -inf
 // (bad pages, rows past the length, nodes outside the mask), V rows past the

@@ -65,3 +65,6 @@ def test_32_bit_pages_by_the_work(L):
     assert form(L, "f32", "f32", 4, positions=131072, **one) == "f32"
     assert form(L, "f32", "f32", 16, 8, 64, 1, positions=704, n_kv=4) == "f32"
     assert form(L, "f32", "f32", 16, 8, 64, 1, positions=4096, n_kv=4) == "umma32"
+    # d = 64: two row groups of 16 at any size
+    assert form(L, "f32", "f32", 64 * 4, 8, 64, 64, n_kv=4) == "f32"
+    assert form(L, "f32", "f32", 64 * 5, 8, 64, 64, n_kv=4) == "umma32"
