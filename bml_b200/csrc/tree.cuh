@@ -505,15 +505,19 @@ __device__ __forceinline__ float wide16(uint16_t x) {
 }
 
 // x as TERMS 16-bit terms, the largest first: x is their sum to 24 (three
-// bf16) or 22 bits (two f16).
+// bf16) or 22 bits (two f16).  f16's smallest step is 2^-24, so its second term
+// is kept kTermScale times as large: 22 bits down to 2^-14, and a step of 2^-36
+// below that (2^-24 without).
+template <bool kF16>
+constexpr float kTermScale = kF16 ? 4096.f : 1.f;
 template <bool kF16, int TERMS>
 __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&t)[TERMS]) {
 #pragma unroll
     for (int i = 0; i < TERMS; ++i) {
         t[i] = pack2<kF16>(x, y);
         if (i + 1 < TERMS) {
-            x -= wide16<kF16>((uint16_t)t[i]);
-            y -= wide16<kF16>((uint16_t)(t[i] >> 16));
+            x = (x - wide16<kF16>((uint16_t)t[i])) * kTermScale<kF16>;
+            y = (y - wide16<kF16>((uint16_t)(t[i] >> 16))) * kTermScale<kF16>;
         }
     }
 }

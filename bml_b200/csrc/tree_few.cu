@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
             if (kQ32)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if (fabsf(s[e]) < INFINITY) s[e] += lo[e];  // else an infinite K, whose lower terms are NaN
+                    if (fabsf(s[e]) < INFINITY) s[e] = fmaf(lo[e], 1.f / kTermScale<kF16>, s[e]);  // else an infinite K, whose lower terms are NaN
             // s[0], s[1]: position base + g, rows 2c, 2c + 1; s[2], s[3]: base + g + 8
             if (edge) {
 #pragma unroll
@@ -271,7 +271,9 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
                     o[j][3] *= f1;
                 }
             }
-            const float u0 = m0 == -INFINITY ? 0.f : m0, u1 = m1 == -INFINITY ? 0.f : m1;
+            // two f16 terms: weights up to 2^15 (l and o are as much larger), away from f16's smallest step
+            constexpr float up = kQ32 && kF16 ? 7.f : 0.f;
+            const float u0 = (m0 == -INFINITY ? 0.f : m0) - up, u1 = (m1 == -INFINITY ? 0.f : m1) - up;
             s[0] = weight(s[0] - u0);
             s[1] = weight(s[1] - u1);
             s[2] = weight(s[2] - u0);
@@ -296,7 +298,12 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
                 if (kQ32) {
                     float x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int z = TERMS - 1; z >= 0; --z) mma16816<kF16>(x, r, pb[0][z], pb[1][z]);
+                    for (int z = TERMS - 1; z >= 0; --z) {
+                        mma16816<kF16>(x, r, pb[0][z], pb[1][z]);
+                        if (kF16 && z)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) x[e] *= 1.f / kTermScale<kF16>;
+                    }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[j][e] += x[e];
                 } else {

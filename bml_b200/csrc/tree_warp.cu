@@ -21,7 +21,7 @@
 // 32-bit queries (kQ32) are split into 16-bit terms of the pages' type, so
 // that products are exact in the f32 sums: three bf16 terms hold all 24 bits;
 // two f16 terms hold 22 of a row that is first scaled by a power of two to a
-// largest value in [2^10, 2^11) (f16's range is small).  The softmax weights
+// largest value in [2^10, 2^11) (f16's range is small; split_pair).  The softmax weights
 // are split the same way, and each block's P.V is summed apart and added to O
 // with a rounding, since the matrix unit's own accumulation truncates.
 #include <math.h>
@@ -252,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (fabsf(s[h][e]) < INFINITY) s[h][e] += lo[h][e];  // else an infinite K, whose lower terms are NaN
+                            if (fabsf(s[h][e]) < INFINITY) s[h][e] = fmaf(lo[h][e], 1.f / kTermScale<kF16>, s[h][e]);  // else an infinite K, whose lower terms are NaN
                 if (base + 16 > P) {
                     const uint32_t w0 = v0 ? tree_see16(p, sg.s, t0, (int32_t)(base - P)) : 0u;
                     const uint32_t w1 = v1 ? tree_see16(p, sg.s, t1, (int32_t)(base - P)) : 0u;
@@ -287,7 +287,9 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
                         o[j][3] *= f1;
                     }
                 }
-                const float u0 = m0 == -INFINITY ? 0.f : m0, u1 = m1 == -INFINITY ? 0.f : m1;
+                // two f16 terms: weights up to 2^15 (l and o are as much larger), away from f16's smallest step
+                constexpr float up = kQ32 && kF16 ? 7.f : 0.f;
+                const float u0 = (m0 == -INFINITY ? 0.f : m0) - up, u1 = (m1 == -INFINITY ? 0.f : m1) - up;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -319,6 +321,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
                         for (int z = TERMS - 1; z >= 0; --z) {
                             mma16816<kF16>(x[0], pa[z], r[0], r[1]);
                             mma16816<kF16>(x[1], pa[z], r[2], r[3]);
+                            if (kF16 && z)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    x[0][e] *= 1.f / kTermScale<kF16>;
+                                    x[1][e] *= 1.f / kTermScale<kF16>;
+                                }
                         }
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {

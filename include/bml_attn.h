@@ -495,7 +495,8 @@ bml_status bml_attn_tree_workspace_size(uint32_t head_dim, int32_t device,
  * that a row sees leaves f32's range, that column is infinite or NaN.
  * 16-bit queries: scores and sums in f32, the softmax weights rounded to the
  * 16-bit type before P.V, one rounding of the output; 32-bit queries: about
- * f32 precision throughout.  Results are the same from run to run on one
+ * f32 precision throughout (over f16 pages a weight has steps of 2^-44 of the
+ * row's largest).  Results are the same from run to run on one
  * device.  Should a wait inside a kernel run into its limit (2 s), the rows that
  * its CTA had not written yet become NaN.  head_dim 64 or 128.  Asynchronous. */
 bml_status bml_attn_tree(const void *q_dev, bml_dtype q_dtype,
