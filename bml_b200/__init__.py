@@ -16,6 +16,10 @@ package is its host-side mirror of the reference interface:
   page_plan / paged_append / tree_attention / paged_commit, PagedBatcher
                      the paged KV cache and the attention of drafted tokens
                      over it (no reference counterpart)
+  chunk_attention / verify_drafts / page_fork / page_free / page_compact
+                     prompts in chunks over pages, the verification of drafted
+                     tokens, and pages shared, returned and packed (no
+                     reference counterpart)
   read_tensor_f32 / WeightTensor.matmul_f64
                      gguf_compiler.rs:351-470 and :1239-1255 on the device
 """
@@ -24,6 +28,7 @@ from .attention import (SeqBatch, Workspace, decode_batched, decode_partial,  # 
                         merge_lse, merge_lse_packed, prefill, softmax_f32)
 from .kv_cache import HashConsedKV  # noqa: F401
 from .batching import AtCapacity, DecodeBatcher, MAX_PENDING_REQUESTS  # noqa: F401
-from .paged import (OutOfPages, PagedBatcher, PagePlan, page_plan, paged_append, paged_commit,  # noqa: F401
-                    tree_attention, tree_workspace_size)
+from .paged import (OutOfPages, PagedBatcher, PagePlan, PageRefused, PageUpdate, chunk_attention,  # noqa: F401
+                    chunk_workspace_size, page_compact, page_fork, page_free, page_plan, paged_append, paged_commit,
+                    tree_attention, tree_workspace_size, verify_drafts)
 from .weights import WeightTensor, matmul_f64, read_tensor_f32  # noqa: F401

@@ -110,6 +110,16 @@ SIGNATURES = {
                                   _u32, _vp, _u32, C.c_float, _vp, _vp, _sz, _u32, _u32, _vp]),
     "bml_paged_commit": (_st, [_vp, _vp, _u32, _u32, _u32, _u32, _u32, C.c_int, _vp, _u32, _vp, _vp, _vp, _u32, _vp,
                                _u32, _vp, _vp, _vp]),
+    "bml_attn_chunk_workspace_size": (_st, [_u32, _u32, _u32, _i32, C.POINTER(_sz)]),
+    "bml_attn_chunk": (_st, [_vp, C.c_int, _u32, _u32, _u32, _u32, _vp, _vp, C.c_int, _u32, _u32, _vp, _u32, _vp, _vp,
+                             _u32, C.c_float, _vp, _vp, _sz, _vp]),
+    "bml_verify_drafts": (_st, [_vp, _vp, C.c_int, _u32, _vp, _vp, _u32, _vp, _u32, _vp, _vp, _u32, _vp, _vp, _vp, _vp]),
+    "bml_page_fork": (_st, [_vp, _vp, _u32, _u32, _u32, _u32, _u32, C.c_int, _vp, _vp, _u32, _vp, _vp, _u32, _vp, _u32, _vp,
+                            _vp, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "bml_page_free": (_st, [_vp, _vp, _vp, _u32, _vp, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                            _vp]),
+    "bml_page_compact": (_st, [_vp, _vp, _u32, _u32, _u32, _u32, _u32, C.c_int, _vp, _u32, _vp, _u32, _vp, _vp, _vp, _vp,
+                               _vp, _vp, _sz, _vp]),
     "bml_softmax_f32": (_st, [_vp, _u32, _u32, _vp, _vp]),
     # include/bml_weights.h
     "bml_read_tensor_f32": (_st, [_vp, C.c_uint64, _i32, C.c_uint64, _vp, C.POINTER(C.c_uint64), _vp]),
@@ -138,6 +148,8 @@ SIGNATURES = {
     # include/bml_diag.h (test-only)
     "bml_diag_attn_tree": (_st, [_vp, C.c_int, _u32, _u32, _u32, _u32, _vp, _vp, C.c_int, _u32, _u32, _vp, _u32, _vp,
                                  _vp, _u32, _vp, _u32, C.c_float, _vp, _vp, _sz, C.c_uint64, _u32, _vp]),
+    "bml_diag_attn_chunk": (_st, [_vp, C.c_int, _u32, _u32, _u32, _u32, _vp, _vp, C.c_int, _u32, _u32, _vp, _u32, _vp,
+                                  _vp, _u32, C.c_float, _vp, _vp, _sz, C.c_uint64, _u32, _vp]),
     "bml_diag_attn_tree_form": (_st, [C.c_int, C.c_int, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32, _u32,
                                       C.POINTER(C.c_int)]),
     "bml_diag_exp2": (_st, [_vp, _u32, _vp, _vp]),

@@ -1,0 +1,118 @@
+// chunk.cu -- attention of chunks of any number of new tokens over a paged cache.
+//
+// Row t of a request's T new tokens sees the positions 0 .. P + t, P = L - T.  A
+// chunk is cut into pieces of W consecutive tokens: piece k is a request of its
+// own, W tokens behind P + k W positions on the same row of the block table, and
+// the kernels of drafted tokens (tree*.cu) compute it.  W * group is at most 256
+// rows, the largest row group, so no piece is read twice and the masked part of
+// one is at most W positions wide.  How many pieces a batch has is on the device;
+// n_seqs + n_tokens / W bound it, and those that are none have no tokens.
+#include "tree.cuh"
+
+namespace bml {
+
+namespace {
+
+constexpr int kThreads = 1024;
+constexpr uint32_t kPieceRows = 256;
+
+struct PieceParams {
+    const int32_t *node_start, *kv_lens;  // [n + 1], [n]
+    uint32_t n, n_tokens, width, most;    // width: tokens of a piece; most: pieces
+    uint64_t room;                        // positions of a row of the block table
+    int32_t *first;                       // [n + 1]: a request's first piece
+    int32_t *start, *lens, *row_of;       // [most + 1], [most], [most]: the pieces
+};
+
+// One CTA: pieces of each request, their prefix sums, then a piece a thread.
+__global__ void __launch_bounds__(kThreads) chunk_pieces_kernel(const PieceParams p) {
+    __shared__ uint32_t sums[kThreads / 32];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    auto tokens = [&](uint32_t i) -> uint32_t {
+        const int32_t a = p.node_start[i], b = p.node_start[i + 1];
+        return a >= 0 && b > a && (uint32_t)b <= p.n_tokens ? (uint32_t)(b - a) : 0u;
+    };
+    uint32_t base = 0;
+    for (uint32_t i0 = 0; i0 < p.n; i0 += kThreads) {
+        const uint32_t i = i0 + threadIdx.x, x = i < p.n ? (tokens(i) + p.width - 1) / p.width : 0u;
+        uint32_t inc = x;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= (uint32_t)o) inc += y;
+        }
+        if (lane == 31) sums[warp] = inc;
+        __syncthreads();
+        uint32_t before = 0, all = 0;
+        for (uint32_t w = 0; w < kThreads / 32; ++w) {
+            if (w < warp) before += sums[w];
+            all += sums[w];
+        }
+        if (i < p.n) p.first[i] = (int32_t)min(base + before + inc - x, p.most);
+        base = min(base + all, p.most);  // more only with a node_start that does not ascend
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) p.first[p.n] = (int32_t)base;
+    __syncthreads();
+    const int32_t end = min(max(p.node_start[p.n], 0), (int32_t)p.n_tokens);
+    for (uint32_t v = threadIdx.x; v <= p.most; v += kThreads) {
+        int32_t start = end, len = 0;
+        uint32_t row = 0;
+        if (v < base) {
+            uint32_t lo = 0, hi = p.n;  // the last request whose first piece is at most v
+            while (hi - lo > 1) {
+                const uint32_t mid = (lo + hi) >> 1;
+                if ((uint32_t)p.first[mid] <= v) lo = mid;
+                else hi = mid;
+            }
+            const uint32_t T = tokens(lo), k = (v - (uint32_t)p.first[lo]) * p.width;
+            const int32_t L = p.kv_lens[lo];
+            row = lo;
+            start = p.node_start[lo] + (int32_t)min(k, T);
+            // a refused request, or one whose positions its row does not hold: none
+            if (L >= (int32_t)T && (uint64_t)L <= p.room) len = L - (int32_t)T + (int32_t)min(k + p.width, T);
+        }
+        p.start[v] = start;
+        if (v < p.most) {
+            p.lens[v] = len;
+            p.row_of[v] = (int32_t)row;
+        }
+    }
+}
+
+}  // namespace
+
+size_t chunk_work_bytes(uint64_t n_tokens, uint64_t n_seqs) {
+    // pieces of one token at the least (groups of more than 128 q heads)
+    return (3 * (n_tokens + n_seqs) + n_seqs + 2) * sizeof(int32_t);
+}
+
+cudaError_t launch_chunk(const TreeArgs &args, int32_t *work, cudaStream_t st) {
+    TreeArgs a = args;
+    TreeParams &p = a.p;
+    PieceParams pp = {};
+    pp.node_start = p.node_start;
+    pp.kv_lens = p.kv_lens;
+    pp.n = p.n_seqs;
+    pp.n_tokens = p.n_tokens;
+    pp.width = p.group < kPieceRows ? kPieceRows / p.group : 1;
+    pp.most = p.n_seqs + p.n_tokens / pp.width;
+    pp.room = (uint64_t)p.max_pages << p.page_shift;
+    pp.first = work;
+    pp.start = pp.first + p.n_seqs + 1;
+    pp.lens = pp.start + pp.most + 1;
+    pp.row_of = pp.lens + pp.most;
+    cudaError_t e = launch_after(chunk_pieces_kernel, dim3(1), kThreads, 0, st, pp);
+    tree_rows(a, p.n_tokens, p.group, pp.most, 0u, 0u);
+    for (uint32_t base = 0; base < pp.most && e == cudaSuccess; base += kTreeMaxSeqs) {
+        p.n_seqs = pp.most - base < kTreeMaxSeqs ? pp.most - base : kTreeMaxSeqs;
+        p.node_start = pp.start + base;
+        p.kv_lens = pp.lens + base;
+        p.row_of = pp.row_of + base;
+        e = launch_tree(a, st);
+    }
+    return e;
+}
+
+}  // namespace bml

@@ -4,92 +4,9 @@
 // the kernels themselves.
 #include <math.h>
 
-#include <atomic>
-#include <initializer_list>
-
 #include "../../include/bml_diag.h"
+#include "paged_check.cuh"
 #include "tree.cuh"
-
-#define BML_API extern "C" __attribute__((visibility("default")))
-
-namespace bml {
-bml_status api_fail(bml_status code, const char *fmt, ...);
-bml_status api_ok();
-bml_status api_cuda_fail(cudaError_t e, const char *where);
-}  // namespace bml
-
-namespace {
-
-using bml::api_fail;
-
-int sm_count(int device) {
-    static std::atomic<int> known[64];
-    const bool keep = device >= 0 && device < 64;
-    if (keep && known[device].load(std::memory_order_relaxed) > 0) return known[device].load(std::memory_order_relaxed);
-    int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) {
-        (void)cudaGetLastError();
-        return 148;
-    }
-    if (keep) known[device].store(n, std::memory_order_relaxed);
-    return n;
-}
-
-int this_device() {
-    int d = 0;
-    if (cudaGetDevice(&d) != cudaSuccess) {
-        (void)cudaGetLastError();
-        d = 0;
-    }
-    return d;
-}
-
-bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-bool valid_dtype(int t) { return t == BML_F32 || t == BML_F16 || t == BML_BF16; }
-
-// log2 of a page size, or -1
-int page_shift(uint32_t page_size) {
-    for (int s = 4; s <= 10; ++s)
-        if (page_size == 1u << s) return s;
-    return -1;
-}
-
-bml_status check_pages(uint32_t page_size, uint32_t max_pages, const char *fn) {
-    if (page_shift(page_size) < 0) return api_fail(BML_E_INVALID, "%s: page_size %u is not a power of two from 16 to 1024", fn, page_size);
-    if (max_pages == 0 || (uint64_t)max_pages * page_size >= (1ull << 31))
-        return api_fail(BML_E_INVALID, "%s: %u pages of %u positions a request", fn, max_pages, page_size);
-    return BML_OK;
-}
-
-bml_status ints(const char *fn, std::initializer_list<const void *> ps) {
-    for (const void *p : ps)
-        if (!p || !aligned(p, 4)) return api_fail(BML_E_INVALID, "%s: null or misaligned int32 array", fn);
-    return BML_OK;
-}
-
-// Whether an array that a call writes overlaps one that it reads: its CTAs do
-// not wait for one another.
-struct Span {
-    const void *p;
-    uint64_t bytes;
-};
-bool overlap(std::initializer_list<Span> written, std::initializer_list<Span> read) {
-    for (const Span &w : written)
-        for (const Span &r : read) {
-            const uintptr_t a = reinterpret_cast<uintptr_t>(w.p), b = reinterpret_cast<uintptr_t>(r.p);
-            if (a && b && a < b + r.bytes && b < a + w.bytes) return true;
-        }
-    return false;
-}
-// Whether two of the arrays that a call writes overlap.
-bool overlap(std::initializer_list<Span> written) {
-    for (const Span *a = written.begin(); a != written.end(); ++a)
-        for (const Span *b = a + 1; b != written.end(); ++b)
-            if (overlap({*a}, {*b})) return true;
-    return false;
-}
-
-}  // namespace
 
 BML_API bml_status bml_paged_plan(const int32_t *lens, const int32_t *n_new, const int32_t *owned, uint32_t n,
                                   const int32_t *free_pages, uint32_t n_free, const int32_t *free_used,
@@ -211,16 +128,8 @@ BML_API bml_status bml_attn_tree_workspace_size(uint32_t head_dim, int32_t devic
 
 namespace {
 
-// What the choice of a kernel goes by.
-void tree_rows(bml::TreeArgs &a, uint32_t n_tokens, uint32_t group, uint32_t n_seqs, uint32_t n_live, uint32_t max_nodes) {
-    a.live = n_live && n_live < n_seqs ? n_live : n_seqs;
-    a.rows = (uint32_t)((uint64_t)n_tokens * group / a.live);
-    const uint32_t most = max_nodes < bml::kTreeMaxNodes ? max_nodes : bml::kTreeMaxNodes;
-    a.widest = most * group > a.rows && (a.p.q_type != BML_F32 || a.kv_type == BML_F32) ? most * group : a.rows;
-}
-
-// What bml_attn_tree_sized takes, and what only tests set.
-bml_status attn_tree(const char *fn, const void *q_dev, bml_dtype q_dtype, uint32_t n_tokens, uint32_t n_heads,
+// What bml_attn_tree_sized takes, and what only tests set.  chunk: bml_attn_chunk.
+bml_status attn_tree(const char *fn, bool chunk, const void *q_dev, bml_dtype q_dtype, uint32_t n_tokens, uint32_t n_heads,
                      uint32_t n_kv_heads, uint32_t head_dim, const void *k_pool, const void *v_pool, bml_dtype kv_dtype,
                      uint32_t n_pages, uint32_t page_size, const int32_t *block_table, uint32_t max_pages,
                      const int32_t *kv_lens, const int32_t *node_start, uint32_t n_seqs, const uint64_t *mask,
@@ -245,15 +154,15 @@ bml_status attn_tree(const char *fn, const void *q_dev, bml_dtype q_dtype, uint3
         !aligned(mask, 8))
         return api_fail(BML_E_INVALID, "%s: pointers must be 16-byte aligned (mask 8)", fn);
     const int sms = sm_count(this_device());
-    if (workspace_bytes < bml::tree_workspace_bytes(head_dim, sms))
-        return api_fail(BML_E_INVALID, "%s: workspace of %zu bytes, need %zu", fn, workspace_bytes, bml::tree_workspace_bytes(head_dim, sms));
+    const size_t parts = bml::tree_workspace_bytes(head_dim, sms), need = parts + (chunk ? bml::chunk_work_bytes(n_tokens, n_seqs) : 0);
+    if (workspace_bytes < need) return api_fail(BML_E_INVALID, "%s: workspace of %zu bytes, need %zu", fn, workspace_bytes, need);
     const size_t es = bml::dtype_size(q_dtype);
     const uintptr_t qa = reinterpret_cast<uintptr_t>(q_dev), oa = reinterpret_cast<uintptr_t>(out_dev);
     if ((qa < oa ? oa - qa : qa - oa) < (uint64_t)n_tokens * n_heads * head_dim * es)
         return api_fail(BML_E_INVALID, "%s: out overlaps q", fn);
     const uint64_t qb = (uint64_t)n_tokens * n_heads * head_dim * es, n4 = 4ull * n_seqs;
     const uint64_t pool = (uint64_t)n_pages * page_size * n_kv_heads * head_dim * bml::dtype_size(kv_dtype);
-    const std::initializer_list<Span> written = {{out_dev, qb}, {workspace, bml::tree_workspace_bytes(head_dim, sms)}};
+    const std::initializer_list<Span> written = {{out_dev, qb}, {workspace, need}};
     if (overlap(written, {{q_dev, qb}, {k_pool, pool}, {v_pool, pool}, {block_table, n4 * max_pages}, {kv_lens, n4}, {node_start, n4 + 4},
                           {mask, 8ull * n_tokens * n_words}}) ||
         overlap(written))
@@ -264,7 +173,7 @@ bml_status attn_tree(const char *fn, const void *q_dev, bml_dtype q_dtype, uint3
     a.num_sms = sms;
     bml::TreeParams &p = a.p;
     p.q_type = q_dtype;
-    tree_rows(a, n_tokens, n_heads / n_kv_heads, n_seqs, n_live, max_nodes);
+    bml::tree_rows(a, n_tokens, n_heads / n_kv_heads, n_seqs, n_live, max_nodes);
     p.q = q_dev;
     p.out = out_dev;
     p.k = k_pool;
@@ -284,6 +193,13 @@ bml_status attn_tree(const char *fn, const void *q_dev, bml_dtype q_dtype, uint3
     p.part = static_cast<float *>(workspace);
     p.wait_ns = wait_ns;
     p.diag = diag;
+    if (chunk) {
+        p.n_seqs = n_seqs;
+        p.table = block_table;
+        p.kv_lens = kv_lens;
+        const cudaError_t e = bml::launch_chunk(a, reinterpret_cast<int32_t *>(static_cast<char *>(workspace) + parts), static_cast<cudaStream_t>(stream));
+        return e == cudaSuccess ? bml::api_ok() : bml::api_cuda_fail(e, fn);
+    }
     for (uint32_t base = 0; base < n_seqs; base += bml::kTreeMaxSeqs) {
         p.n_seqs = n_seqs - base < bml::kTreeMaxSeqs ? n_seqs - base : bml::kTreeMaxSeqs;
         p.table = block_table + (size_t)base * max_pages;
@@ -303,7 +219,7 @@ BML_API bml_status bml_attn_tree(const void *q_dev, bml_dtype q_dtype, uint32_t 
                                  uint32_t max_pages, const int32_t *kv_lens, const int32_t *node_start, uint32_t n_seqs,
                                  const uint64_t *mask, uint32_t n_words, float scale, void *out_dev, void *workspace,
                                  size_t workspace_bytes, void *stream) {
-    return attn_tree("bml_attn_tree", q_dev, q_dtype, n_tokens, n_heads, n_kv_heads, head_dim, k_pool, v_pool, kv_dtype, n_pages,
+    return attn_tree("bml_attn_tree", false, q_dev, q_dtype, n_tokens, n_heads, n_kv_heads, head_dim, k_pool, v_pool, kv_dtype, n_pages,
                      page_size, block_table, max_pages, kv_lens, node_start, n_seqs, mask, n_words, scale, out_dev, workspace,
                      workspace_bytes, 0u, 0u, bml::kWaitNs, 0u, stream);
 }
@@ -314,9 +230,38 @@ BML_API bml_status bml_attn_tree_sized(const void *q_dev, bml_dtype q_dtype, uin
                                        uint32_t max_pages, const int32_t *kv_lens, const int32_t *node_start, uint32_t n_seqs,
                                        const uint64_t *mask, uint32_t n_words, float scale, void *out_dev, void *workspace,
                                        size_t workspace_bytes, uint32_t n_live, uint32_t max_nodes, void *stream) {
-    return attn_tree("bml_attn_tree_sized", q_dev, q_dtype, n_tokens, n_heads, n_kv_heads, head_dim, k_pool, v_pool, kv_dtype,
+    return attn_tree("bml_attn_tree_sized", false, q_dev, q_dtype, n_tokens, n_heads, n_kv_heads, head_dim, k_pool, v_pool, kv_dtype,
                      n_pages, page_size, block_table, max_pages, kv_lens, node_start, n_seqs, mask, n_words, scale, out_dev,
                      workspace, workspace_bytes, n_live, max_nodes, bml::kWaitNs, 0u, stream);
+}
+
+BML_API bml_status bml_attn_chunk_workspace_size(uint32_t head_dim, uint32_t n_tokens, uint32_t n_seqs, int32_t device, size_t *bytes) {
+    const bml_status st = bml_attn_tree_workspace_size(head_dim, device, bytes);
+    if (st == BML_OK) *bytes += bml::chunk_work_bytes(n_tokens, n_seqs);
+    return st;
+}
+
+BML_API bml_status bml_attn_chunk(const void *q_dev, bml_dtype q_dtype, uint32_t n_tokens, uint32_t n_heads,
+                                  uint32_t n_kv_heads, uint32_t head_dim, const void *k_pool, const void *v_pool,
+                                  bml_dtype kv_dtype, uint32_t n_pages, uint32_t page_size, const int32_t *block_table,
+                                  uint32_t max_pages, const int32_t *kv_lens, const int32_t *node_start, uint32_t n_seqs,
+                                  float scale, void *out_dev, void *workspace, size_t workspace_bytes, void *stream) {
+    return attn_tree("bml_attn_chunk", true, q_dev, q_dtype, n_tokens, n_heads, n_kv_heads, head_dim, k_pool, v_pool, kv_dtype, n_pages,
+                     page_size, block_table, max_pages, kv_lens, node_start, n_seqs, nullptr, 0u, scale, out_dev, workspace,
+                     workspace_bytes, 0u, 0u, bml::kWaitNs, 0u, stream);
+}
+
+BML_API bml_status bml_diag_attn_chunk(const void *q_dev, bml_dtype q_dtype, uint32_t n_tokens, uint32_t n_heads,
+                                       uint32_t n_kv_heads, uint32_t head_dim, const void *k_pool, const void *v_pool,
+                                       bml_dtype kv_dtype, uint32_t n_pages, uint32_t page_size, const int32_t *block_table,
+                                       uint32_t max_pages, const int32_t *kv_lens, const int32_t *node_start, uint32_t n_seqs,
+                                       float scale, void *out_dev, void *workspace, size_t workspace_bytes, uint64_t wait_ns,
+                                       uint32_t flags, void *stream) {
+    const char *fn = "bml_diag_attn_chunk";
+    if (flags & ~BML_DIAG_STALL) return api_fail(BML_E_INVALID, "%s: flags 0x%x", fn, flags);
+    return attn_tree(fn, true, q_dev, q_dtype, n_tokens, n_heads, n_kv_heads, head_dim, k_pool, v_pool, kv_dtype, n_pages, page_size,
+                     block_table, max_pages, kv_lens, node_start, n_seqs, nullptr, 0u, scale, out_dev, workspace, workspace_bytes,
+                     0u, 0u, wait_ns ? wait_ns : bml::kWaitNs, (flags & BML_DIAG_STALL) ? bml::kTreeStall : 0u, stream);
 }
 
 BML_API bml_status bml_diag_attn_tree(const void *q_dev, bml_dtype q_dtype, uint32_t n_tokens, uint32_t n_heads,
@@ -327,7 +272,7 @@ BML_API bml_status bml_diag_attn_tree(const void *q_dev, bml_dtype q_dtype, uint
                                       size_t workspace_bytes, uint64_t wait_ns, uint32_t flags, void *stream) {
     const char *fn = "bml_diag_attn_tree";
     if (flags & ~BML_DIAG_STALL) return api_fail(BML_E_INVALID, "%s: flags 0x%x", fn, flags);
-    return attn_tree(fn, q_dev, q_dtype, n_tokens, n_heads, n_kv_heads, head_dim, k_pool, v_pool, kv_dtype, n_pages, page_size,
+    return attn_tree(fn, false, q_dev, q_dtype, n_tokens, n_heads, n_kv_heads, head_dim, k_pool, v_pool, kv_dtype, n_pages, page_size,
                      block_table, max_pages, kv_lens, node_start, n_seqs, mask, n_words, scale, out_dev, workspace, workspace_bytes,
                      0u, 0u, wait_ns ? wait_ns : bml::kWaitNs, (flags & BML_DIAG_STALL) ? bml::kTreeStall : 0u, stream);
 }
@@ -348,7 +293,7 @@ BML_API bml_status bml_diag_attn_tree_form(bml_dtype q_dtype, bml_dtype kv_dtype
     a.p.max_pages = max_pages;
     a.p.page_shift = (uint32_t)page_shift(page_size);
     a.p.scale_log2 = 1.f;
-    tree_rows(a, n_tokens, a.p.group, n_seqs, n_live, max_nodes);
+    bml::tree_rows(a, n_tokens, a.p.group, n_seqs, n_live, max_nodes);
     *form = (int)bml::tree_form(a);
     return bml::api_ok();
 }

@@ -1,7 +1,6 @@
 // torch_calls.cpp -- the usual calls of bml_b200/paged.py without Python's
-// share of the time: argument checks, output allocation and the C call of
-// page_plan, paged_append, tree_attention and paged_commit for plain CUDA
-// tensors on the current device and stream.
+// share of the time: argument checks, output allocation and the C call of its
+// functions for plain CUDA tensors on the current device and stream.
 //
 // Every function returns None when anything is not the usual case (an argument
 // that is not a plain contiguous tensor of the right type and shape, another
@@ -33,6 +32,12 @@ AppendFn g_append = nullptr;
 TreeFn g_tree = nullptr;
 CommitFn g_commit = nullptr;
 decltype(&bml_attn_tree_workspace_size) g_tree_bytes = nullptr;
+decltype(&bml_attn_chunk) g_chunk = nullptr;
+decltype(&bml_attn_chunk_workspace_size) g_chunk_bytes = nullptr;
+decltype(&bml_verify_drafts) g_verify = nullptr;
+decltype(&bml_page_fork) g_fork = nullptr;
+decltype(&bml_page_free) g_free = nullptr;
+decltype(&bml_page_compact) g_compact = nullptr;
 
 // Scratch bytes of tree_attention, asked for once a device and head size; -1: refused.
 int64_t tree_bytes(int device, int64_t d) {
@@ -247,6 +252,165 @@ PyObject *commit_impl(PyObject *const *a) {
     return THPVariable_Wrap(std::move(out));
 }
 
+// q, k_pool, v_pool, block_table, kv_lens, node_start, scale -> out
+PyObject *chunk_impl(PyObject *const *a) {
+    const at::Tensor *q = plain(a[0], 3), *k = plain(a[1], 4), *lens = plain(a[4], 1);
+    USUAL(q && k && lens);
+    const c10::Device dev = q->device();
+    const at::Tensor *v = typed(a[2], 4, k->scalar_type(), dev), *table = typed(a[3], 2, at::kInt, dev);
+    const at::Tensor *start = typed(a[5], 1, at::kInt, dev);
+    USUAL(here(dev) && k->device() == dev && lens->device() == dev && lens->scalar_type() == at::kInt && v && table && start &&
+          code(q->scalar_type()) >= 0 && code(k->scalar_type()) >= 0 && PyFloat_CheckExact(a[6]));
+    const int64_t n = lens->size(0), n_tokens = q->size(0), d = q->size(2);
+    USUAL(v->sizes() == k->sizes() && k->size(3) == d && start->size(0) == n + 1 && table->size(0) == n && n > 0 && n_tokens > 0 &&
+          n < (1ll << 31) && n_tokens < (1ll << 31) && k->size(0) < (1ll << 31) && k->size(1) < (1ll << 31) && table->size(1) < (1ll << 31));
+    size_t ws_bytes = 0;
+    USUAL(g_chunk_bytes((uint32_t)d, (uint32_t)n_tokens, (uint32_t)n, dev.index(), &ws_bytes) == BML_OK);
+    at::Tensor out = fresh(q->sizes(), q->scalar_type(), dev), ws = fresh({(int64_t)ws_bytes}, at::kByte, dev);
+    const bml_status st =
+        g_chunk(q->const_data_ptr(), (bml_dtype)code(q->scalar_type()), (uint32_t)n_tokens, (uint32_t)q->size(1), (uint32_t)k->size(2),
+                (uint32_t)d, k->const_data_ptr(), v->const_data_ptr(), (bml_dtype)code(k->scalar_type()), (uint32_t)k->size(0),
+                (uint32_t)k->size(1), table->const_data_ptr<int32_t>(), (uint32_t)table->size(1), lens->const_data_ptr<int32_t>(),
+                start->const_data_ptr<int32_t>(), (uint32_t)n, (float)PyFloat_AS_DOUBLE(a[6]), out.mutable_data_ptr(),
+                ws.mutable_data_ptr(), ws_bytes, stream_of(dev));
+    USUAL(st == BML_OK);
+    return THPVariable_Wrap(std::move(out));
+}
+
+// Consecutive pieces of an int32 buffer, as a tuple of vectors.
+PyObject *pieces(const at::Tensor &buf, std::initializer_list<int64_t> sizes) {
+    static const caffe2::TypeMeta i32 = caffe2::TypeMeta::Make<int32_t>();
+    PyObject *out = PyTuple_New((Py_ssize_t)sizes.size());
+    if (!out) return nullptr;
+    int64_t at = 0;
+    Py_ssize_t i = 0;
+    for (int64_t n : sizes) {
+        PyTuple_SET_ITEM(out, i++, piece(buf, i32, at, {n}));
+        at += n;
+    }
+    return out;
+}
+
+// target, draft, tokens, parents, node_start, u, u_next, max_path -> path, n_accept, next
+PyObject *verify_impl(PyObject *const *a) {
+    const at::Tensor *p = plain(a[0], 2);
+    USUAL(p && code(p->scalar_type()) >= 0);
+    const c10::Device dev = p->device();
+    const at::Tensor *q = nullptr, *tok = typed(a[2], 1, at::kInt, dev), *par = typed(a[3], 1, at::kInt, dev);
+    const at::Tensor *start = typed(a[4], 1, at::kInt, dev), *u = typed(a[5], 1, at::kFloat, dev), *un = typed(a[6], 1, at::kFloat, dev);
+    int64_t most;
+    USUAL(here(dev) && tok && par && start && u && un && integer(a[7], &most) && most > 0);
+    if (a[1] != Py_None) {
+        q = typed(a[1], 2, p->scalar_type(), dev);
+        USUAL(q && q->sizes() == p->sizes());
+    }
+    const int64_t rows = p->size(0), n = start->size(0) - 1;
+    USUAL(n > 0 && n < (1ll << 31) && rows < (1ll << 31) && p->size(1) < (1ll << 31) && tok->size(0) == rows && par->size(0) == rows &&
+          u->size(0) == rows && un->size(0) == n);
+    at::Tensor all = fresh({n * (most + 2)}, at::kInt, dev);
+    int32_t *path = all.mutable_data_ptr<int32_t>();
+    const bml_status st =
+        g_verify(p->const_data_ptr(), q ? q->const_data_ptr() : nullptr, (bml_dtype)code(p->scalar_type()), (uint32_t)p->size(1),
+                 tok->const_data_ptr<int32_t>(), par->const_data_ptr<int32_t>(), (uint32_t)rows, start->const_data_ptr<int32_t>(),
+                 (uint32_t)n, u->const_data_ptr<float>(), un->const_data_ptr<float>(), (uint32_t)most, path, path + n * most,
+                 path + n * most + n, stream_of(dev));
+    USUAL(st == BML_OK);
+    static const caffe2::TypeMeta i32 = caffe2::TypeMeta::Make<int32_t>();
+    PyObject *out = PyTuple_New(3);
+    if (!out) return nullptr;
+    PyTuple_SET_ITEM(out, 0, piece(all, i32, 0, {n, most}));
+    PyTuple_SET_ITEM(out, 1, piece(all, i32, n * most, {n}));
+    PyTuple_SET_ITEM(out, 2, piece(all, i32, n * most + n, {n}));
+    return out;
+}
+
+// Whether a layered pool's sizes fit the C calls'.
+bool sizes32(const at::Tensor *k) {
+    for (int64_t s : k->sizes())
+        if (s >= (1ll << 31)) return false;
+    return true;
+}
+
+// k_pools, v_pools, src, dst, lens, owned, block_table, shared, free_pages, free_used
+//   -> lens, owned, shared, free_used, status
+PyObject *fork_impl(PyObject *const *a) {
+    const at::Tensor *k = plain(a[0], 5);
+    USUAL(k && code(k->scalar_type()) >= 0 && sizes32(k));
+    const c10::Device dev = k->device();
+    const at::Tensor *v = typed(a[1], 5, k->scalar_type(), dev), *src = typed(a[2], 1, at::kInt, dev), *dst = typed(a[3], 1, at::kInt, dev);
+    const at::Tensor *lens = typed(a[4], 1, at::kInt, dev), *owned = typed(a[5], 1, at::kInt, dev), *table = typed(a[6], 2, at::kInt, dev);
+    const at::Tensor *shared = typed(a[7], 1, at::kInt, dev), *free = typed(a[8], 1, at::kInt, dev), *used = typed(a[9], 1, at::kInt, dev);
+    USUAL(here(dev) && v && src && dst && lens && owned && table && shared && free && used);
+    const int64_t n = lens->size(0), m = src->size(0), pages = k->size(1);
+    USUAL(v->sizes() == k->sizes() && n > 0 && n < (1ll << 31) && m < (1ll << 31) && dst->size(0) == m && owned->size(0) == n &&
+          table->size(0) == n && table->size(1) < (1ll << 31) && shared->size(0) == pages && free->size(0) < (1ll << 31) &&
+          used->size(0) == 1);
+    at::Tensor all = fresh({2 * n + pages + 1 + m}, at::kInt, dev);
+    int32_t *o = all.mutable_data_ptr<int32_t>();
+    const bml_status st =
+        g_fork(k->mutable_data_ptr(), v->mutable_data_ptr(), (uint32_t)k->size(0), (uint32_t)pages, (uint32_t)k->size(2),
+               (uint32_t)k->size(3), (uint32_t)k->size(4), (bml_dtype)code(k->scalar_type()), src->const_data_ptr<int32_t>(),
+               dst->const_data_ptr<int32_t>(), (uint32_t)m, lens->const_data_ptr<int32_t>(), owned->const_data_ptr<int32_t>(), (uint32_t)n,
+               table->mutable_data_ptr<int32_t>(), (uint32_t)table->size(1), shared->const_data_ptr<int32_t>(),
+               free->const_data_ptr<int32_t>(), (uint32_t)free->size(0), used->const_data_ptr<int32_t>(), o, o + n, o + 2 * n,
+               o + 2 * n + pages, o + 2 * n + pages + 1, stream_of(dev));
+    USUAL(st == BML_OK);
+    return pieces(all, {n, n, pages, 1, m});
+}
+
+// keep, lens, owned, block_table, page_size, shared, free_pages, free_used
+//   -> lens, owned, shared, free_pages, free_used, status
+PyObject *free_impl(PyObject *const *a) {
+    const at::Tensor *lens = plain(a[1], 1);
+    USUAL(lens && lens->scalar_type() == at::kInt);
+    const c10::Device dev = lens->device();
+    const int64_t n = lens->size(0);
+    const at::Tensor *keep = typed(a[0], 1, at::kInt, dev), *owned = typed(a[2], 1, at::kInt, dev), *table = typed(a[3], 2, at::kInt, dev);
+    const at::Tensor *shared = typed(a[5], 1, at::kInt, dev), *free = typed(a[6], 1, at::kInt, dev), *used = typed(a[7], 1, at::kInt, dev);
+    int64_t page;
+    USUAL(here(dev) && n > 0 && n < (1ll << 31) && keep && owned && table && shared && free && used && integer(a[4], &page));
+    const int64_t pages = shared->size(0), n_free = free->size(0);
+    USUAL(keep->size(0) == n && owned->size(0) == n && table->size(0) == n && table->size(1) < (1ll << 31) && pages < (1ll << 31) &&
+          n_free < (1ll << 31) && used->size(0) == 1);
+    at::Tensor all = fresh({3 * n + pages + n_free + 1}, at::kInt, dev);
+    int32_t *o = all.mutable_data_ptr<int32_t>();
+    const bml_status st =
+        g_free(keep->const_data_ptr<int32_t>(), lens->const_data_ptr<int32_t>(), owned->const_data_ptr<int32_t>(), (uint32_t)n,
+               table->const_data_ptr<int32_t>(), (uint32_t)table->size(1), (uint32_t)page, shared->const_data_ptr<int32_t>(),
+               (uint32_t)pages, free->const_data_ptr<int32_t>(), (uint32_t)n_free, used->const_data_ptr<int32_t>(), o, o + n, o + 2 * n,
+               o + 2 * n + pages, o + 2 * n + pages + n_free, o + 2 * n + pages + n_free + 1, stream_of(dev));
+    USUAL(st == BML_OK);
+    return pieces(all, {n, n, pages, n_free, 1, n});
+}
+
+// k_pools, v_pools, owned, block_table, shared -> block_table, shared, free_pages, free_used
+PyObject *compact_impl(PyObject *const *a) {
+    const at::Tensor *k = plain(a[0], 5);
+    USUAL(k && code(k->scalar_type()) >= 0 && sizes32(k));
+    const c10::Device dev = k->device();
+    const at::Tensor *v = typed(a[1], 5, k->scalar_type(), dev), *owned = typed(a[2], 1, at::kInt, dev);
+    const at::Tensor *table = typed(a[3], 2, at::kInt, dev), *shared = typed(a[4], 1, at::kInt, dev);
+    USUAL(here(dev) && v && owned && table && shared && v->sizes() == k->sizes());
+    const int64_t n = owned->size(0), wide = table->size(1), pages = k->size(1);
+    USUAL(n > 0 && n < (1ll << 31) && table->size(0) == n && wide < (1ll << 31) && shared->size(0) == pages);
+    at::Tensor all = fresh({n * wide + 2 * pages + 1}, at::kInt, dev), work = fresh({3 * pages + 1}, at::kInt, dev);
+    int32_t *o = all.mutable_data_ptr<int32_t>(), *s = o + n * wide;
+    const bml_status st =
+        g_compact(k->mutable_data_ptr(), v->mutable_data_ptr(), (uint32_t)k->size(0), (uint32_t)pages, (uint32_t)k->size(2),
+                  (uint32_t)k->size(3), (uint32_t)k->size(4), (bml_dtype)code(k->scalar_type()), owned->const_data_ptr<int32_t>(),
+                  (uint32_t)n, table->const_data_ptr<int32_t>(), (uint32_t)wide, shared->const_data_ptr<int32_t>(), o, s, s + pages,
+                  s + 2 * pages, work.mutable_data_ptr(), (size_t)(4 * (3 * pages + 1)), stream_of(dev));
+    USUAL(st == BML_OK);
+    static const caffe2::TypeMeta i32 = caffe2::TypeMeta::Make<int32_t>();
+    PyObject *out = PyTuple_New(4);
+    if (!out) return nullptr;
+    PyTuple_SET_ITEM(out, 0, piece(all, i32, 0, {n, wide}));
+    PyTuple_SET_ITEM(out, 1, piece(all, i32, n * wide, {pages}));
+    PyTuple_SET_ITEM(out, 2, piece(all, i32, n * wide + pages, {pages}));
+    PyTuple_SET_ITEM(out, 3, piece(all, i32, n * wide + 2 * pages, {1}));
+    return out;
+}
+
 // No C++ exception leaves: an allocation that fails is left to paged.py, which
 // meets it again and raises it.
 template <PyObject *(*F)(PyObject *const *), Py_ssize_t kArgs>
@@ -263,12 +427,13 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
 }
 
 PyObject *set_calls(PyObject *, PyObject *const *args, Py_ssize_t n) {
-    if (n != 5) {
-        PyErr_SetString(PyExc_TypeError, "five addresses expected");
+    constexpr Py_ssize_t kCalls = 11;
+    if (n != kCalls) {
+        PyErr_Format(PyExc_TypeError, "%zd addresses expected", kCalls);
         return nullptr;
     }
-    void *p[5];
-    for (int i = 0; i < 5; ++i) {
+    void *p[kCalls];
+    for (Py_ssize_t i = 0; i < kCalls; ++i) {
         p[i] = PyLong_AsVoidPtr(args[i]);
         if (!p[i]) {
             if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null address");
@@ -280,6 +445,12 @@ PyObject *set_calls(PyObject *, PyObject *const *args, Py_ssize_t n) {
     g_tree = reinterpret_cast<TreeFn>(p[2]);
     g_commit = reinterpret_cast<CommitFn>(p[3]);
     g_tree_bytes = reinterpret_cast<decltype(g_tree_bytes)>(p[4]);
+    g_chunk = reinterpret_cast<decltype(g_chunk)>(p[5]);
+    g_chunk_bytes = reinterpret_cast<decltype(g_chunk_bytes)>(p[6]);
+    g_verify = reinterpret_cast<decltype(g_verify)>(p[7]);
+    g_fork = reinterpret_cast<decltype(g_fork)>(p[8]);
+    g_free = reinterpret_cast<decltype(g_free)>(p[9]);
+    g_compact = reinterpret_cast<decltype(g_compact)>(p[10]);
     Py_RETURN_NONE;
 }
 
@@ -291,6 +462,11 @@ PyMethodDef methods[] = {
     ENTRY(append, 9),
     ENTRY(tree, 10),
     ENTRY(commit, 8),
+    ENTRY(chunk, 7),
+    ENTRY(verify, 8),
+    ENTRY(fork, 10),
+    ENTRY(free, 8),
+    ENTRY(compact, 5),
     {"set_calls", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&set_calls)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

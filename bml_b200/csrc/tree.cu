@@ -134,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_f32_kernel(const __grid_cons
         const uint32_t P = sg.s.L - min(sg.s.T, sg.s.L);  // committed positions
         const uint32_t pos0 = sg.t0 * C::TILE;
         const uint32_t n_steps = sg.t1 - sg.t0;
-        const int32_t *table = p.table + (size_t)sg.seq * p.max_pages;
+        const int32_t *table = tree_table(p, sg.seq);
         auto step_pos = [&](uint32_t k) { return pos0 + (k * C::GROUPS + grp) * C::SP; };
         // the group's copies of step k into stage k % NST
         auto fetch = [&](uint32_t k) {

@@ -20,6 +20,7 @@ struct TreeParams {
     const void *k, *v;  // pools [n_pages][page][n_kv][D]
     const int32_t *table;  // [n_seqs][max_pages]
     const int32_t *kv_lens, *node_start;
+    const int32_t *row_of;  // [n_seqs]: a request's row of table (pieces of a chunk share one); null: its own index
     const uint64_t *mask;  // [n_tokens][n_words] or null: node t sees nodes 0..t
     uint32_t n_seqs, n_tokens, n_heads, n_kv, group, max_pages, n_pages, page_shift, n_words;
     float scale_log2;
@@ -94,6 +95,17 @@ cudaError_t launch_tree_few(const TreeArgs &a, cudaStream_t st);
 cudaError_t launch_tree_umma(const TreeArgs &a, cudaStream_t st);
 cudaError_t launch_tree_umma32(const TreeArgs &a, cudaStream_t st);
 
+// Chunks of any number of new tokens (chunk.cu).  work: chunk_work_bytes of scratch.
+cudaError_t launch_chunk(const TreeArgs &a, int32_t *work, cudaStream_t st);
+size_t chunk_work_bytes(uint64_t n_tokens, uint64_t n_seqs);
+// What the choice of a kernel goes by.
+inline void tree_rows(TreeArgs &a, uint32_t n_tokens, uint32_t group, uint32_t n_seqs, uint32_t n_live, uint32_t max_nodes) {
+    a.live = n_live && n_live < n_seqs ? n_live : n_seqs;
+    a.rows = (uint32_t)((uint64_t)n_tokens * group / a.live);
+    const uint32_t most = max_nodes < kTreeMaxNodes ? max_nodes : kTreeMaxNodes;
+    a.widest = most * group > a.rows && (a.p.q_type != BML_F32 || a.kv_type == BML_F32) ? most * group : a.rows;
+}
+
 // Sets what follows from the other fields, and says whether the schedule can
 // count the launch's tiles in 32 bits, whatever the lengths on the device are.
 inline uint64_t tree_most_units(const TreeParams &p) {
@@ -132,6 +144,10 @@ struct TreeSeq {
 template <bool kW>
 __device__ __forceinline__ uint32_t tree_weight(const TreeParams &p, uint32_t rows) {
     return !kW ? 1u : rows > p.heavy_rows ? p.heavy : p.light;
+}
+
+__device__ __forceinline__ const int32_t *tree_table(const TreeParams &p, uint32_t seq) {
+    return p.table + (size_t)(p.row_of ? (uint32_t)p.row_of[seq] : seq) * p.max_pages;
 }
 
 // What the device holds of a request: rows [a, b), positions.
@@ -561,7 +577,7 @@ __device__ __noinline__ void tree_nonfinite(const TreeParams &p, const TreeSpan 
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
         for (uint32_t pos = begin; pos < end; ++pos) {
             if (pos >= P && !tree_sees(p, a.s, a.t, pos - P)) continue;
-            const uint32_t page = (uint32_t)p.table[(size_t)a.seq * p.max_pages + (pos >> p.page_shift)];
+            const uint32_t page = (uint32_t)tree_table(p, a.seq)[pos >> p.page_shift];
             if (page >= p.n_pages) continue;
             const size_t row = ((size_t)page << p.page_shift) + (pos & ((1u << p.page_shift) - 1));
             const float4 v = tree_load4<KT>(p.v, (row * p.n_kv + a.head) * D + col + c);

@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(NCfg<D, kF16, kQ32>::NW * 32, 1) tree_few_kern
             if (!fw.next(p, fs)) return;
             f_left = fs.t1 - fs.t0;
             f_pos = fs.t0 * p.tile + split * 16;
-            f_table = p.table + (size_t)fs.seq * p.max_pages;
+            f_table = tree_table(p, fs.seq);
             f_page = page_at(f_pos);
         }
         if (lane == 0 && live) {

@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma_kernel(const __grid_con
         while (live && walk.next(p, sg)) {
             const bool pair = sg.rows > up.rt;
             const uint32_t n = sg.t1 - sg.t0;
-            const int32_t *table = p.table + (size_t)sg.seq * p.max_pages;
+            const int32_t *table = tree_table(p, sg.seq);
             // Table entries come 32 boxes at a time, one window ahead: lane l
             // holds the first row of box 32 w + l of the segment (-1: past the
             // length, -2: a page outside the pool).

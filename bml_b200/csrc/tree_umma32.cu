@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
         const bool mine = part < parts && lane < 20;
         bool live = !(p.diag & kTreeStall);
         while (live && walk.next(p, sg)) {
-            const int32_t *table = p.table + (size_t)sg.seq * p.max_pages;
+            const int32_t *table = tree_table(p, sg.seq);
             // a lane's first row in the pool of tile j (-1: past the length, -2: a page outside the pool)
             auto row_of = [&](uint32_t j) -> int {
                 const uint32_t pos = j * BN + part * xp.box_rows;

@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_warp_kernel(const __grid_con
         }
         if (f_left) {
             uint8_t *dk = ring + f_stage * C::STAGE, *dv = dk + C::SP * C::RS;
-            const int32_t *table = p.table + (size_t)fs.seq * p.max_pages;
+            const int32_t *table = tree_table(p, fs.seq);
 #pragma unroll
             for (int b = 0; b < C::SP / 16; ++b) {  // 16 positions share a page
                 const uint32_t pos = f_pos + b * 16;

@@ -1,0 +1,383 @@
+// verify.cu -- verification of drafted tokens: which path of a request's draft
+// the target model's probabilities keep, and the token that follows it.
+//
+// Node 0 is the pending token and is kept.  At a kept node, with target row p and
+// draft row q (the distribution that its children were drawn from, independently),
+// the children are tried in node order against the residual r_k:
+//   r_0 = p,  child x kept iff u < r_k(x) / q(x),  else r_(k+1) = norm(max(r_k - q, 0)).
+// The residuals are never formed.  With c_0 = 0, S_0 = 1,
+//   r_k = max(p - c_k q, 0) / S_k,  c_(k+1) = c_k + S_k,  S_(k+1) = sum_v max(p - c_(k+1) q, 0),
+// since norm(max(r_k - q, 0)) is max(p - c_k q - S_k q, 0) up to a factor: so a
+// rejection costs one pass over the two rows, and only where another child follows.
+// Tokens that were picked (no draft rows): q is 1 at the token, so S loses p(x)
+// and p(x) becomes 0, without a pass.
+// The token behind the path is the first v with C(v) > u_next C(V - 1), C the
+// prefix sums of max(p - c q, 0).  In exact arithmetic something is left of a
+// residual whenever a child is rejected; of rows rounded to 16 bits p <= q may hold
+// everywhere (0.996 and 1 at one token), and the token is drawn from p then.
+//
+// Whether a number is below another decides about tokens, so sums are f64: of
+// f32 or 16-bit inputs, their order changes them by 1e-16 relatively.
+//
+// A cluster of 1 to 8 CTAs serves a request; each walks the tree by itself (the
+// probabilities of drafted tokens are looked up at once at the start) and sums
+// its part of a row; the sums meet in distributed shared memory.  What bounds it:
+// latency for one request (launch, two dependent loads, a row pass), HBM for a
+// batch over a large vocabulary.
+#include <cooperative_groups.h>
+
+#include "pages.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace bml {
+
+namespace {
+
+constexpr int kThreads = 512;
+constexpr uint32_t kWarps = kThreads / 32;
+constexpr uint32_t kNodes = kTreeMaxNodes;
+constexpr uint32_t kMostCluster = 8;
+
+struct VerifyShared {
+    int32_t token[kNodes];
+    float pv[kNodes], qv[kNodes], u[kNodes];
+    uint32_t below[kNodes][kNodes / 32];  // children of a node, by node
+    double part[2][kMostCluster];         // pass parity: the CTAs' sums
+    double warp[kWarps];
+    double all[kMostCluster * kWarps];    // the last pass: every warp's sum
+    uint32_t out[kNodes];                 // tokens that are taken out of p
+};
+
+// A probability; what is not a positive number counts as 0.
+template <typename T>
+__device__ __forceinline__ float prob(T x) {
+    const float f = (float)x;
+    return f > 0.f && f < INFINITY ? f : 0.f;
+}
+
+template <typename T>
+struct Vec {
+    static constexpr int N = 16 / sizeof(T);
+    T v[N];
+};
+
+// The N values of a row from element e0 on (from a 16-byte boundary where `whole`),
+// zeros outside [0, vocab).
+template <typename T>
+__device__ __forceinline__ void load_vec(const T *row, int64_t e0, uint32_t vocab, bool aligned, float (&x)[Vec<T>::N]) {
+    constexpr int N = Vec<T>::N;
+    if (aligned && e0 >= 0 && e0 + N <= (int64_t)vocab) {
+        const uint4 z = __ldg(reinterpret_cast<const uint4 *>(row + e0));
+        const T *t = reinterpret_cast<const T *>(&z);
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = prob(t[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = e0 + i >= 0 && e0 + i < (int64_t)vocab ? prob(row[e0 + i]) : 0.f;
+    }
+}
+
+// What a row pass sums: max(p - c q, 0), or p without some tokens.
+template <typename T, bool kDraft>
+struct Row {
+    static constexpr int N = Vec<T>::N;
+    const T *p, *q;
+    uint32_t vocab;
+    double c;
+    const uint32_t *out;
+    uint32_t n_out;
+    int shift;  // elements from the row's start back to a 16-byte boundary
+    bool q_ok;  // q's row lies on the same place of one
+    __device__ __forceinline__ void at(const T *pr, const T *qr) {
+        p = pr;
+        q = qr;
+        shift = (int)((reinterpret_cast<uintptr_t>(pr) & 15u) / sizeof(T));
+        q_ok = kDraft && ((reinterpret_cast<uintptr_t>(pr) ^ reinterpret_cast<uintptr_t>(qr)) & 15u) == 0;
+    }
+    __device__ __forceinline__ uint32_t vecs() const { return (vocab + shift + N - 1) / N; }
+    // vector k's weights
+    __device__ __forceinline__ void load(uint32_t k, float (&x)[N], float (&y)[N]) const {
+        const int64_t e0 = (int64_t)k * N - shift;
+        load_vec<T>(p, e0, vocab, true, x);
+        if (kDraft) load_vec<T>(q, e0, vocab, q_ok, y);
+    }
+    __device__ __forceinline__ void weigh(uint32_t k, const float (&x)[N], const float (&y)[N], double (&w)[N]) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = kDraft ? fmax((double)x[i] - c * (double)y[i], 0.0) : (double)x[i];
+        if (!kDraft)
+            for (uint32_t o = 0; o < n_out; ++o) {
+                const int64_t i = (int64_t)out[o] - ((int64_t)k * N - shift);
+#pragma unroll
+                for (int j = 0; j < N; ++j)
+                    if (i == j) w[j] = 0.0;
+            }
+    }
+};
+
+// Sum of vectors [k0, k1) by a warp; every lane gets it.
+template <typename T, bool kDraft>
+__device__ __forceinline__ double warp_pass(const Row<T, kDraft> &r, uint32_t k0, uint32_t k1) {
+    constexpr int N = Vec<T>::N, kAtOnce = 4;
+    const uint32_t lane = threadIdx.x & 31;
+    double s[2] = {0.0, 0.0};
+    for (uint32_t k = k0 + lane; k < k1; k += 32 * kAtOnce) {
+        float x[kAtOnce][N], y[kAtOnce][N];
+#pragma unroll
+        for (int a = 0; a < kAtOnce; ++a)
+            if (k + a * 32 < k1) r.load(k + a * 32, x[a], y[a]);
+#pragma unroll
+        for (int a = 0; a < kAtOnce; ++a)
+            if (k + a * 32 < k1) {
+                double w[N];
+                r.weigh(k + a * 32, x[a], y[a], w);
+#pragma unroll
+                for (int i = 0; i < N; ++i) s[i & 1] += w[i];
+            }
+    }
+    double t = s[0] + s[1];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    return t;
+}
+
+// The first element of vectors [k0, k1) whose prefix sum, from `base` on, is above
+// tau; where rounding leaves none, the last element with a weight.  One warp.
+template <typename T, bool kDraft>
+__device__ __noinline__ int32_t warp_find(const Row<T, kDraft> &r, uint32_t k0, uint32_t k1, double base, double tau) {
+    constexpr int N = Vec<T>::N;
+    const uint32_t lane = threadIdx.x & 31;
+    int32_t last = -1;
+    for (uint32_t kb = k0; kb < k1; kb += 32) {
+        const uint32_t k = kb + lane;
+        float x[N], y[N];
+        double w[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) w[i] = 0.0;
+        if (k < k1) {
+            r.load(k, x, y);
+            r.weigh(k, x, y, w);
+        }
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum += w[i];
+        double inc = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double a = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= (uint32_t)o) inc += a;
+        }
+        double at = base + (inc - sum);
+        int32_t hit = -1, seen = -1;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            at += w[i];
+            const int32_t e = (int32_t)((int64_t)k * N - r.shift + i);
+            if (w[i] > 0.0) {
+                seen = e;
+                if (hit < 0 && at > tau) hit = e;
+            }
+        }
+        const uint32_t hits = __ballot_sync(0xffffffffu, hit >= 0), some = __ballot_sync(0xffffffffu, seen >= 0);
+        if (hits) return __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1);
+        if (some) last = __shfl_sync(0xffffffffu, seen, 31 - __clz(some));
+        base += __shfl_sync(0xffffffffu, inc, 31);
+    }
+    return last;
+}
+
+template <typename T, bool kDraft>
+__global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant__ VerifyParams p) {
+    __shared__ VerifyShared sh;
+    cg::cluster_group cl = cg::this_cluster();
+    const uint32_t C = cl.num_blocks(), rank = cl.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t i = blockIdx.x / C;
+    const T *target = static_cast<const T *>(p.target), *draft = static_cast<const T *>(p.draft);
+    for (uint32_t k = threadIdx.x; k < kNodes * (kNodes / 32); k += kThreads) (&sh.below[0][0])[k] = 0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int32_t a = p.node_start[i], b = p.node_start[i + 1];
+    const bool ok = a >= 0 && b > a && (uint32_t)b <= p.n_tokens && b - a <= (int32_t)kNodes;
+    const uint32_t T_nodes = ok ? (uint32_t)(b - a) : 0u;
+    __syncthreads();
+    if (threadIdx.x < T_nodes) {
+        const uint32_t j = threadIdx.x;
+        const int32_t up = p.parents[a + j], tok = p.tokens[a + j];
+        const bool child = up >= 0 && up < (int32_t)j && (uint32_t)tok < p.vocab;
+        sh.token[j] = tok;
+        sh.u[j] = p.u[a + j];
+        sh.pv[j] = sh.qv[j] = 0.f;
+        if (child) {
+            const size_t at = (size_t)(a + up) * p.vocab + tok;
+            sh.pv[j] = prob(target[at]);
+            if (kDraft) sh.qv[j] = prob(draft[at]);
+            atomicOr(&sh.below[up][j >> 5], 1u << (j & 31));
+        }
+    }
+    cl.sync();  // also: every CTA of the cluster runs, so its shared memory may be written
+
+    int32_t *path = p.path + (size_t)i * p.max_path;
+    const bool writes = rank == 0 && threadIdx.x == 0;
+    Row<T, kDraft> row;
+    row.vocab = p.vocab;
+    row.c = 0.0;
+    row.out = sh.out;
+    row.n_out = 0;
+    const uint32_t slice = C * kWarps, me = rank * kWarps + warp;
+    uint32_t passes = 0, kept = 0, t = 0;
+    auto bounds = [&](uint32_t n, uint32_t &k0, uint32_t &k1) {  // of the warp's piece of n vectors
+        const uint32_t each = (n + slice - 1) / slice;
+        k0 = min(me * each, n);
+        k1 = min(k0 + each, n);
+    };
+    // sum of a row over all CTAs, the same in each
+    auto total = [&](const auto &r) {
+        uint32_t k0, k1;
+        bounds(r.vecs(), k0, k1);
+        const double w = warp_pass(r, k0, k1);
+        if (lane == 0) sh.warp[warp] = w;
+        __syncthreads();
+        if (threadIdx.x < C) {
+            double s = 0.0;
+            for (uint32_t x = 0; x < kWarps; ++x) s += sh.warp[x];
+            *cl.map_shared_rank(&sh.part[passes & 1][rank], threadIdx.x) = s;
+        }
+        cl.sync();
+        double s = 0.0;
+        for (uint32_t x = 0; x < C; ++x) s += sh.part[passes & 1][x];
+        ++passes;
+        return s;
+    };
+
+    if (T_nodes && p.max_path) {
+        if (writes) path[0] = 0;
+        kept = 1;
+        while (true) {
+            row.c = 0.0;
+            row.n_out = 0;
+            if (kept == p.max_path) break;  // its children are not looked at
+            row.at(target + (size_t)(a + t) * p.vocab, kDraft ? draft + (size_t)(a + t) * p.vocab : nullptr);
+            double mass = 1.0;
+            bool known = true;  // mass is that of the residual
+            uint32_t next = 0;
+            for (uint32_t w = 0; w < kNodes / 32 && !next; ++w)
+                for (uint32_t m = sh.below[t][w]; m; m &= m - 1) {
+                    const uint32_t j = w * 32 + __ffs(m) - 1;
+                    const double u = sh.u[j], pv = sh.pv[j], qv = sh.qv[j];
+                    double r = pv;
+                    if (kDraft) {
+                        if (!known) mass = total(row);
+                        known = true;
+                        r = fmax(pv - row.c * qv, 0.0);
+                    } else {
+                        for (uint32_t o = 0; o < row.n_out; ++o)
+                            if (sh.out[o] == (uint32_t)sh.token[j]) r = 0.0;  // has been rejected
+                    }
+                    if ((kDraft ? u * qv * mass : u * mass) < r) {
+                        next = j;
+                        break;
+                    }
+                    if (kDraft) {
+                        row.c += mass;
+                        known = false;
+                    } else {
+                        mass -= r;
+                        __syncthreads();
+                        if (threadIdx.x == 0) sh.out[row.n_out] = (uint32_t)sh.token[j];
+                        __syncthreads();
+                        ++row.n_out;
+                    }
+                }
+            if (!next) break;
+            t = next;
+            if (writes) path[kept] = (int32_t)t;
+            ++kept;
+        }
+    }
+    if (writes) p.n_accept[i] = (int32_t)kept;
+    if (rank == 0)
+        for (uint32_t k = kept + threadIdx.x; k < p.max_path; k += kThreads) path[k] = -1;
+
+    // the token behind node t, from the residual
+    if (kept) {
+        row.at(target + (size_t)(a + t) * p.vocab, kDraft ? draft + (size_t)(a + t) * p.vocab : nullptr);
+        for (int again = 0; again < 2; ++again) {
+            uint32_t k0, k1;
+            bounds(row.vecs(), k0, k1);
+            const double w = warp_pass(row, k0, k1);
+            if (lane < C) *cl.map_shared_rank(&sh.all[me], lane) = w;
+            cl.sync();
+            double before = 0.0, sum = 0.0;
+            for (uint32_t x = 0; x < slice; ++x) {
+                if (x == me) before = sum;
+                sum += sh.all[x];
+            }
+            if (sum > 0.0) {
+                const double tau = (double)p.u_next[i] * sum;
+                // the first piece that ends above tau, or the last one with a weight
+                uint32_t piece = 0, heavy = 0;
+                double run = 0.0;
+                bool found = false;
+                for (uint32_t x = 0; x < slice; ++x) {
+                    const double y = sh.all[x];
+                    run += y;
+                    if (y > 0.0) heavy = x;
+                    if (!found && y > 0.0 && run > tau) {
+                        found = true;
+                        piece = x;
+                    }
+                }
+                if (!found) piece = heavy;
+                if (piece == me) {
+                    const int32_t token = warp_find(row, k0, k1, before, tau);
+                    if (lane == 0) p.next[i] = token;
+                }
+                break;
+            }
+            cl.sync();  // sh.all has been read
+            // nothing is left: by rounding, unless q sums to more than twice p (no
+            // distribution) or p itself has nothing
+            bool drawn = !again;
+            if (kDraft && drawn) {
+                Row<T, false> one;
+                one.vocab = p.vocab;
+                one.n_out = 0;
+                one.at(row.q, nullptr);
+                const double sq = total(one);
+                one.at(row.p, nullptr);
+                drawn = sq <= 2.0 * total(one);
+            }
+            if (!drawn) {
+                if (writes) p.next[i] = (int32_t)p.vocab - 1;
+                break;
+            }
+            row.c = 0.0;
+            row.n_out = 0;
+        }
+    } else if (writes) {
+        p.next[i] = -1;
+    }
+    cl.sync();  // no CTA leaves while another writes into its shared memory
+}
+
+template <typename T>
+cudaError_t verify_t(const VerifyParams &p, cudaStream_t st) {
+    // as many CTAs a request as leave two for each SM (a CTA's row pass is bound by
+    // what one SM can read)
+    uint32_t cluster = kMostCluster;
+    while (cluster > 1 && (uint64_t)p.n * cluster > 2ull * p.num_sms) cluster /= 2;
+    auto kern = p.draft ? verify_kernel<T, true> : verify_kernel<T, false>;
+    return launch_clusters(kern, cluster, dim3(p.n * cluster), kThreads, 0, st, p);
+}
+
+}  // namespace
+
+cudaError_t launch_verify_drafts(const VerifyParams &p, cudaStream_t st) {
+    switch (p.type) {
+        case BML_F32: return verify_t<float>(p, st);
+        case BML_F16: return verify_t<__half>(p, st);
+        case BML_BF16: return verify_t<__nv_bfloat16>(p, st);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace bml

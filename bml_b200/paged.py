@@ -10,8 +10,14 @@ decode.  A step is
 
   page_plan       pages, slots, positions, ancestor masks   (once a step)
   paged_append    RoPE of q and k, K and V rows stored      (every layer)
-  tree_attention  attention of the new tokens               (every layer)
+  tree_attention  attention of the new tokens               (every layer);
+  chunk_attention in its place where prompts come in chunks
+  verify_drafts   the path that the target's probabilities keep, and the next
+                  token                                     (once a step)
   paged_commit    the accepted path moved to the front      (once a step)
+
+and between steps page_fork lets requests share another's pages, page_free
+returns pages of requests that end, page_compact packs the pool.
 
 None of the calls waits for the GPU, and all can be captured in a CUDA
 graph.  Tensors of a call live on one device, which need not be the current
@@ -32,8 +38,15 @@ MAX_NODES = 256  # drafted tokens of one request in tree_attention
 PLAN_NO_PAGES, PLAN_BAD, PLAN_NO_ROOM = 1, 2, 4  # status values of a plan
 
 
-class OutOfPages(RuntimeError):
-    """A plan that refused a request (its status says why)."""
+PAGE_SHARED = 8  # status value of a page_free
+
+
+class PageRefused(RuntimeError):
+    """A call that refused a request (its status says why)."""
+
+
+class OutOfPages(PageRefused):
+    """A plan or a fork that refused a request (its status says why)."""
 
 
 # A call costs the host several microseconds and the GPU often less, so the
@@ -98,6 +111,7 @@ class _Wrappers:
         return None
 
     append = tree = commit = plan
+    chunk = verify = fork = free = compact = plan
 
 
 def _load():
@@ -117,7 +131,9 @@ def _load():
         _fast = _Wrappers
         return _fast
     _torch_calls.set_calls(*(C.cast(getattr(lib, f), C.c_void_p).value for f in (
-        "bml_paged_plan", "bml_paged_append", "bml_attn_tree_sized", "bml_paged_commit", "bml_attn_tree_workspace_size")))
+        "bml_paged_plan", "bml_paged_append", "bml_attn_tree_sized", "bml_paged_commit", "bml_attn_tree_workspace_size",
+        "bml_attn_chunk", "bml_attn_chunk_workspace_size", "bml_verify_drafts", "bml_page_fork", "bml_page_free",
+        "bml_page_compact")))
     _fast = _torch_calls
     return _fast
 
@@ -392,15 +408,256 @@ def paged_commit(k_pools: torch.Tensor, v_pools: torch.Tensor, block_table: torc
     return new
 
 
+def chunk_workspace_size(head_dim: int, n_tokens: int, n_requests: int, device=None) -> int:
+    """Scratch bytes of chunk_attention for a batch of that size."""
+    dev = torch.cuda.current_device() if device is None else torch.device(device).index or 0
+    size = C.c_size_t()
+    L.call("bml_attn_chunk_workspace_size", head_dim, n_tokens, n_requests, dev, C.byref(size))
+    return size.value
+
+
+def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
+                    kv_lens: torch.Tensor, node_start: torch.Tensor, scale: float = -1.0,
+                    out: torch.Tensor | None = None, workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Attention of chunks of new tokens over pages: tree_attention without a
+    mask, for any number of new tokens a request -- a prompt or a part of one,
+    beside requests that decode one token.  The j-th of request i's T new tokens
+    (row node_start[i] + j of q) attends over positions 0 to kv_lens[i] - T + j.
+    Types, results, refused requests and rows behind the last request's are
+    tree_attention's.  workspace: an uint8 tensor of chunk_workspace_size bytes
+    for calls that must not allocate; calls that share one must not overlap."""
+    if stream is None and out is None and workspace is None:
+        r = (_fast or _load()).chunk(q, k_pool, v_pool, block_table, kv_lens, node_start, scale)
+        if r is not None:
+            return r
+    a_q = _data(q, "q", 3)
+    shape, dev, dtype = q.shape, q.device, q.dtype
+    n_tokens, n_heads, d = shape
+    a_k, a_v, pool = _pools(k_pool, v_pool, 4, dev)
+    n_pages, page_size, n_kv, pd = pool
+    if pd != d:
+        raise ValueError(f"q {tuple(shape)} does not match the pools {tuple(pool)}")
+    a_len = _ints(kv_lens, "kv_lens", dev)
+    n = kv_lens.shape[0]
+    a_start = _ints(node_start, "node_start", dev, (n + 1,))
+    a_table = _ints(block_table, "block_table", dev, ndim=2)
+    rows, max_pages = block_table.shape
+    if rows != n:
+        raise ValueError(f"block_table must be [{n}, max_pages], got {tuple(block_table.shape)}")
+    ctx = _enter(dev, stream)
+    try:
+        if out is None:
+            out = torch.empty_like(q)
+        elif _data(out, "out", 3, dtype, dev) and out.shape != shape:
+            raise ValueError(f"out {tuple(out.shape)} does not match q {tuple(shape)}")
+        if workspace is None:
+            workspace = torch.empty(chunk_workspace_size(d, n_tokens, n, dev), dtype=torch.uint8, device=dev)
+        else:
+            _ints(workspace, "workspace", dev, dtype=torch.uint8)
+        _call("bml_attn_chunk", a_q, dtype_code(dtype), n_tokens, n_heads, n_kv, d, a_k, a_v, dtype_code(k_pool.dtype),
+              n_pages, page_size, a_table, max_pages, a_len, a_start, n, scale, out.data_ptr(), workspace.data_ptr(),
+              workspace.shape[0], _raw_stream(dev.index))
+    finally:
+        if ctx is not None:
+            ctx.__exit__(None, None, None)
+    return out
+
+
+def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torch.Tensor, parents: torch.Tensor,
+                  node_start: torch.Tensor, u: torch.Tensor, u_next: torch.Tensor, max_path: int = MAX_NODES,
+                  stream=None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Which path of each request's draft the target model keeps, and the token
+    that follows it, so that tokens are distributed as the target's.  Request
+    i's nodes are rows node_start[i]..node_start[i+1]; node 0 is its pending token
+    and always kept, a node whose parent is an earlier node is a drafted child of
+    it, any other is never kept.  target [n_tokens, vocab]: the target's
+    probabilities behind each node; draft: those (of the same type) that each
+    node's children were drawn from, independently, or None for tokens that were
+    picked; tokens, parents int32 [n_tokens]; u [n_tokens] and u_next [n] f32:
+    random numbers in [0, 1).
+
+    Returns path int32 [n, max_path] (-1 behind its end) and n_accept [n], as
+    paged_commit takes them, and the next tokens int32 [n].  At a kept node its
+    children are tried in node order: x is kept with probability min(1, r(x) /
+    q(x)), r the target's probabilities at first and norm(max(r - q, 0)) after
+    each rejection; if none is, the next token is drawn from r.  A path of
+    max_path nodes ends there.  A request without nodes, or with more than 256,
+    has n_accept 0 and next -1.  include/bml_attn.h has the formulas."""
+    if stream is None:
+        r = (_fast or _load()).verify(target, draft, tokens, parents, node_start, u, u_next, max_path)
+        if r is not None:
+            return r
+    a_t = _data(target, "target", 2)
+    dev, dtype = target.device, target.dtype
+    rows, vocab = target.shape
+    a_d = None
+    if draft is not None:
+        a_d = _data(draft, "draft", 2, dtype, dev)
+        if draft.shape != target.shape:
+            raise ValueError(f"draft {tuple(draft.shape)} does not match target {tuple(target.shape)}")
+    a_tok, a_par = _ints(tokens, "tokens", dev, (rows,)), _ints(parents, "parents", dev, (rows,))
+    a_start = _ints(node_start, "node_start", dev)
+    n = node_start.shape[0] - 1
+    a_u, a_next = _ints(u, "u", dev, (rows,), dtype=torch.float32), _ints(u_next, "u_next", dev, (n,), dtype=torch.float32)
+    if not 1 <= max_path < 1 << 31:
+        raise ValueError(f"max_path must be 1 to 2^31 - 1, got {max_path}")
+    ctx = _enter(dev, stream)
+    try:
+        path = torch.empty((n, max_path), dtype=torch.int32, device=dev)
+        count, token = torch.empty((2, n), dtype=torch.int32, device=dev).unbind()
+        _call("bml_verify_drafts", a_t, a_d, dtype_code(dtype), vocab, a_tok, a_par, rows, a_start, n, a_u, a_next,
+              max_path, path.data_ptr(), count.data_ptr(), token.data_ptr(), _raw_stream(dev.index))
+    finally:
+        if ctx is not None:
+            ctx.__exit__(None, None, None)
+    return path, count, token
+
+
+class PageUpdate:
+    """What page_fork, page_free and page_compact make of the pages' state: the
+    arrays that the call replaces (None: it leaves that one as it is).
+
+    lens, owned int32 [n], shared int32 [n_pages], free_pages int32 [n_free],
+    free_used int32 [1], block_table int32 [n, max_pages], status int32."""
+
+    __slots__ = ("lens", "owned", "shared", "free_pages", "free_used", "block_table", "status")
+
+    def __init__(self, lens=None, owned=None, shared=None, free_pages=None, free_used=None, block_table=None, status=None):
+        self.lens, self.owned, self.shared, self.free_pages = lens, owned, shared, free_pages
+        self.free_used, self.block_table, self.status = free_used, block_table, status
+
+    def check(self) -> None:
+        """Raises OutOfPages or PageRefused if something was refused.  Waits for the GPU."""
+        bad = [] if self.status is None else self.status.nonzero().flatten().tolist()
+        if bad:
+            status = self.status[bad].tolist()
+            raise (OutOfPages if PLAN_NO_PAGES in status else PageRefused)(f"entries {bad} refused, status {status}")
+
+
+def page_fork(k_pools: torch.Tensor, v_pools: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, lens: torch.Tensor,
+              owned: torch.Tensor, block_table: torch.Tensor, shared: torch.Tensor, free_pages: torch.Tensor,
+              free_used: torch.Tensor, stream=None) -> PageUpdate:
+    """Lets row dst[j] of the tables continue the positions of row src[j], in the
+    pools [n_layers, n_pages, page_size, n_kv, d] of all layers: full pages are
+    shared (shared [n_pages] counts a page's holders beyond the first), the rows of
+    a part-filled one are copied to a page of the free list.  src, dst [m], lens,
+    owned [n], block_table [n, max_pages] (rows dst written), free_pages, free_used
+    [1]: int32, as page_plan takes them.  dst must be idle rows.  Returns the next
+    lens, owned, shared and free_used, and a status per fork."""
+    if stream is None:
+        r = (_fast or _load()).fork(k_pools, v_pools, src, dst, lens, owned, block_table, shared, free_pages, free_used)
+        if r is not None:
+            return PageUpdate(r[0], r[1], r[2], None, r[3], None, r[4])
+    a_k, a_v, pool = _pools(k_pools, v_pools, 5)
+    layers, n_pages, page_size, n_kv, d = pool
+    dev = k_pools.device
+    a_src = _ints(src, "src", dev)
+    m = src.shape[0]
+    a_dst = _ints(dst, "dst", dev, (m,))
+    a_lens = _ints(lens, "lens", dev)
+    n = lens.shape[0]
+    a_owned, a_table = _ints(owned, "owned", dev, (n,)), _ints(block_table, "block_table", dev, ndim=2)
+    if block_table.shape[0] != n:
+        raise ValueError(f"block_table must be [{n}, max_pages], got {tuple(block_table.shape)}")
+    a_shared = _ints(shared, "shared", dev, (n_pages,))
+    a_free, a_used = _ints(free_pages, "free_pages", dev), _ints(free_used, "free_used", dev, (1,))
+    ctx = _enter(dev, stream)
+    try:
+        buf = torch.empty(2 * n + n_pages + 1 + m, dtype=torch.int32, device=dev)
+        out = torch.unsafe_split_with_sizes(buf, (n, n, n_pages, 1, m))
+        _call("bml_page_fork", a_k, a_v, layers, n_pages, page_size, n_kv, d, dtype_code(k_pools.dtype), a_src, a_dst, m,
+              a_lens, a_owned, n, a_table, block_table.shape[1], a_shared, a_free, free_pages.shape[0], a_used,
+              *(x.data_ptr() for x in out), _raw_stream(dev.index))
+    finally:
+        if ctx is not None:
+            ctx.__exit__(None, None, None)
+    return PageUpdate(out[0], out[1], out[2], None, out[3], None, out[4])
+
+
+def page_free(keep: torch.Tensor, lens: torch.Tensor, owned: torch.Tensor, block_table: torch.Tensor, page_size: int,
+              shared: torch.Tensor, free_pages: torch.Tensor, free_used: torch.Tensor, stream=None) -> PageUpdate:
+    """Ends or rolls back requests: request i keeps min(lens[i], keep[i])
+    positions (negative: everything) and the pages that hold them; pages that
+    all their holders have released return to the free list, whose taken part is
+    parted into pages still held and freed ones.  Refused (status 8) where keep ends
+    inside a page that others hold.  keep, lens, owned [n], block_table [n,
+    max_pages], shared [n_pages], free_pages, free_used [1] are int32.  Returns the
+    next lens, owned, shared, free_pages and free_used, and a status per request."""
+    if stream is None:
+        r = (_fast or _load()).free(keep, lens, owned, block_table, page_size, shared, free_pages, free_used)
+        if r is not None:
+            return PageUpdate(r[0], r[1], r[2], r[3], r[4], None, r[5])
+    dev = lens.device if isinstance(lens, torch.Tensor) else None
+    if dev is None or dev.type != "cuda":
+        _bad(lens, "lens", torch.int32, 1)
+    a_lens = _ints(lens, "lens", dev)
+    n = lens.shape[0]
+    a_keep, a_owned = _ints(keep, "keep", dev, (n,)), _ints(owned, "owned", dev, (n,))
+    a_table = _ints(block_table, "block_table", dev, ndim=2)
+    if block_table.shape[0] != n:
+        raise ValueError(f"block_table must be [{n}, max_pages], got {tuple(block_table.shape)}")
+    a_shared, a_free = _ints(shared, "shared", dev), _ints(free_pages, "free_pages", dev)
+    a_used = _ints(free_used, "free_used", dev, (1,))
+    n_pages, n_free = shared.shape[0], free_pages.shape[0]
+    if not 0 <= page_size < 1 << 31:  # ctypes would cut it to 32 bits
+        raise ValueError(f"page_size {page_size} must be 0 to 2^31 - 1")
+    ctx = _enter(dev, stream)
+    try:
+        buf = torch.empty(3 * n + n_pages + n_free + 1, dtype=torch.int32, device=dev)
+        out = torch.unsafe_split_with_sizes(buf, (n, n, n_pages, n_free, 1, n))
+        _call("bml_page_free", a_keep, a_lens, a_owned, n, a_table, block_table.shape[1], page_size, a_shared, n_pages,
+              a_free, n_free, a_used, *(x.data_ptr() for x in out), _raw_stream(dev.index))
+    finally:
+        if ctx is not None:
+            ctx.__exit__(None, None, None)
+    return PageUpdate(out[0], out[1], out[2], out[3], out[4], None, out[5])
+
+
+def page_compact(k_pools: torch.Tensor, v_pools: torch.Tensor, owned: torch.Tensor, block_table: torch.Tensor,
+                 shared: torch.Tensor, stream=None) -> PageUpdate:
+    """Packs the pools [n_layers, n_pages, page_size, n_kv, d]: the H held pages (the
+    first owned[i] entries of each row of block_table) come to lie at 0 to H - 1.
+    Those behind move, in ascending order, into the pages below H that nobody holds.
+    owned [n], block_table [n, max_pages], shared [n_pages] are int32.  Returns the
+    next block_table, shared, free_pages (0, 1, 2, ...) and free_used (H)."""
+    if stream is None:
+        r = (_fast or _load()).compact(k_pools, v_pools, owned, block_table, shared)
+        if r is not None:
+            return PageUpdate(None, None, r[1], r[2], r[3], r[0])
+    a_k, a_v, pool = _pools(k_pools, v_pools, 5)
+    layers, n_pages, page_size, n_kv, d = pool
+    dev = k_pools.device
+    a_owned, a_table = _ints(owned, "owned", dev), _ints(block_table, "block_table", dev, ndim=2)
+    n, max_pages = owned.shape[0], block_table.shape[1]
+    if block_table.shape[0] != n:
+        raise ValueError(f"block_table must be [{n}, max_pages], got {tuple(block_table.shape)}")
+    a_shared = _ints(shared, "shared", dev, (n_pages,))
+    ctx = _enter(dev, stream)
+    try:
+        table, work = torch.empty_like(block_table), torch.empty(3 * n_pages + 1, dtype=torch.int32, device=dev)
+        out = torch.unsafe_split_with_sizes(torch.empty(2 * n_pages + 1, dtype=torch.int32, device=dev),
+                                            (n_pages, n_pages, 1))
+        _call("bml_page_compact", a_k, a_v, layers, n_pages, page_size, n_kv, d, dtype_code(k_pools.dtype), a_owned, n,
+              a_table, max_pages, a_shared, table.data_ptr(), *(x.data_ptr() for x in out), work.data_ptr(),
+              4 * work.shape[0], _raw_stream(dev.index))
+    finally:
+        if ctx is not None:
+            ctx.__exit__(None, None, None)
+    return PageUpdate(None, None, out[0], out[1], out[2], table)
+
+
 class PagedBatcher:
     """DecodeBatcher over a paged cache, with drafts: requests join and leave
     between steps, a step brings each request any number of new tokens -- one
     to decode, a chain, or a tree of drafted tokens -- and commit() keeps the
-    accepted ones.
+    accepted ones.  Prompts may come in chunks of any length beside them.
 
     Per step: ``begin(new)`` plans it; for every layer ``step(layer, q, k, v)``
-    stores the tokens and returns their attention; ``commit(paths)`` ends it.
-    Token rows are the requests' tokens in the order of ``active``."""
+    stores the tokens and returns their attention; ``commit(paths)`` ends it, or
+    ``verify(...)``, which finds the paths on the GPU.  Token rows are the
+    requests' tokens in the order of ``active``.  Between steps ``fork`` lets
+    requests continue another's positions, ``truncate`` rolls one back, and
+    ``compact`` packs the pool."""
 
     def __init__(self, n_layers: int, n_heads: int, n_kv_heads: int, head_dim: int, n_pages: int,
                  page_size: int = 64, max_positions: int = 8192, dtype: torch.dtype = torch.bfloat16, device=None,
@@ -424,10 +681,12 @@ class PagedBatcher:
         self.table = torch.full((max_requests, -(-max_positions // page_size)), -1, **i32)
         self.lens, self.owned = torch.zeros(max_requests, **i32), torch.zeros(max_requests, **i32)
         self.free, self.used = torch.arange(n_pages, **i32), torch.zeros(1, **i32)
+        self.shared = torch.zeros(n_pages, **i32)  # holders of a page beyond the first
         self._rows: dict = {}    # request -> its row of the tables
         self._plan = None        # of the step that has begun
         self._new = None         # new tokens of each row (host),
         self._live = self._most = 0  # how many rows have some, the most of one
+        self._parents = []       # of the step's tokens (host)
 
     @property
     def active(self) -> list:
@@ -474,27 +733,62 @@ class PagedBatcher:
         """Lengths of the refused requests (kv_lens gives them as 0)."""
         return torch.where(plan.status != 0, self.lens, torch.zeros_like(self.lens))
 
-    def remove(self, rid) -> None:
-        """Drops a request and returns its pages.  Waits for the GPU."""
+    def _between_steps(self) -> None:
         if self._plan is not None:
             raise RuntimeError("a step has begun: commit it first")
-        row = self._rows.pop(rid)
-        n, used = int(self.owned[row]), int(self.used)
-        self.free[used - n:used] = self._held(row, n)
-        self.used = self.used - n
-        self.owned[row] = 0
-        self.lens[row] = 0
 
-    def _held(self, row: int, n: int) -> torch.Tensor:
-        """The row's pages moved to the end of the taken part of the free
-        list: the list holds each page once, so those pages swap places with
-        the ones that lie there."""
-        pages = self.table[row, :n].clone()
-        used = int(self.used)
-        taken = self.free[:used]
-        keep = taken[~torch.isin(taken, pages)]
-        self.free[:used - n] = keep
-        return pages
+    def _keep(self, rows: dict, check: bool) -> None:
+        """Releases what the given rows hold behind so many positions."""
+        keep = [rows.get(r, -1) for r in range(self.max_requests)]
+        p = page_free(torch.tensor(keep, dtype=torch.int32, device=self.device), self.lens, self.owned, self.table,
+                      self.page_size, self.shared, self.free, self.used)
+        if check:
+            p.check()
+        self.lens, self.owned, self.shared = p.lens, p.owned, p.shared
+        self.free, self.used = p.free_pages, p.free_used
+
+    def remove(self, rid) -> None:
+        """Drops a request and returns the pages that no other one shares."""
+        self._between_steps()
+        self._keep({self._rows.pop(rid): 0}, False)
+
+    def truncate(self, rid, n: int) -> None:
+        """Rolls a request back to its first n positions.  PageRefused where that
+        ends inside a page that it shares.  Waits for the GPU."""
+        self._between_steps()
+        if n < 0:
+            raise ValueError(f"{n} positions")
+        self._keep({self._rows[rid]: n}, True)
+
+    def fork(self, rid, new) -> None:
+        """Admits a request, or a list of them, that continues the positions of
+        `rid`: its full pages are shared, a part-filled one is copied.  OutOfPages
+        where the pool has no page for that; then none is admitted.  Waits for
+        the GPU."""
+        self._between_steps()
+        new = list(new) if isinstance(new, (list, tuple)) else [new]
+        row = self._rows[rid]
+        if len(set(new)) < len(new) or any(r in self._rows for r in new):
+            raise KeyError(f"requests {new!r}: one is already active, or named twice")
+        if len(self._rows) + len(new) > self.max_requests:
+            raise AtCapacity(f"{len(self._rows)} requests active (max {self.max_requests}), {len(new)} more")
+        if not new:
+            return
+        free = sorted(set(range(self.max_requests)) - set(self._rows.values()))[:len(new)]
+        i32 = dict(dtype=torch.int32, device=self.device)
+        p = page_fork(self.k, self.v, torch.tensor([row] * len(new), **i32), torch.tensor(free, **i32), self.lens, self.owned,
+                      self.table, self.shared, self.free, self.used)
+        p.check()
+        self.lens, self.owned, self.shared, self.used = p.lens, p.owned, p.shared, p.free_used
+        self._rows.update(zip(new, free))
+
+    def compact(self) -> torch.Tensor:
+        """Moves the held pages to the pool's front and returns their number
+        (int32 [1] on the GPU): pages from there on are free."""
+        self._between_steps()
+        p = page_compact(self.k, self.v, self.owned, self.table, self.shared)
+        self.table, self.shared, self.free, self.used = p.block_table, p.shared, p.free_pages, p.free_used
+        return self.used
 
     def _planned(self, new: dict) -> PagePlan:
         counts, parents = [0] * self.max_requests, []
@@ -510,20 +804,24 @@ class PagedBatcher:
         if tree and most > MAX_NODES:
             raise ValueError(f"{most} drafted tokens for a request (at most {MAX_NODES})")
         dev = self.device
-        self._new, self._live, self._most = counts, sum(x > 0 for x in counts), most
+        self._new, self._live, self._most, self._parents = counts, sum(x > 0 for x in counts), most, parents
         return page_plan(self.lens, torch.tensor(counts, dtype=torch.int32, device=dev), self.owned, self.table,
                          self.free, self.used, self.page_size, sum(counts),
                          torch.tensor(parents, dtype=torch.int32, device=dev) if tree else None,
                          n_words=max(1, -(-most // 64)) if tree else 1)
 
-    def begin(self, new: dict, check: bool = True) -> PagePlan:
+    def begin(self, new: dict, check: bool = True, chunks: bool = False) -> PagePlan:
         """Plans a step.  new: request -> its number of new tokens (a chain),
         or the list of its drafted tokens' parents (-1: a child of the last
         committed token).  check: wait for the plan and raise OutOfPages if a
-        request was refused; False leaves that to the caller (plan.status)."""
+        request was refused; False leaves that to the caller (plan.status).
+        chunks: chains may have more than 256 tokens (chunks of prompts); then no
+        request of the step brings a tree."""
         if self._plan is not None:
             raise RuntimeError("a step has begun: commit it first")
-        if any((x if isinstance(x, int) else len(x)) > MAX_NODES for x in new.values()):
+        if chunks and any(not isinstance(x, int) for x in new.values()):
+            raise ValueError("a step of chunks has no trees")
+        if not chunks and any((x if isinstance(x, int) else len(x)) > MAX_NODES for x in new.values()):
             raise ValueError(f"at most {MAX_NODES} new tokens a request")
         if any(isinstance(x, int) and x < 0 for x in new.values()):
             raise ValueError("a negative number of new tokens")
@@ -546,6 +844,9 @@ class PagedBatcher:
         p = self._plan
         paged_append(q, k_new, v_new, p.slots, p.positions if self.rope else None, self.k[layer], self.v[layer],
                      theta=self.theta, stream=stream)
+        if self._most > MAX_NODES:
+            return chunk_attention(q, self.k[layer], self.v[layer], self.table, p.kv_lens, p.node_start, scale=self.scale,
+                                   out=out, stream=stream)
         return tree_attention(q, self.k[layer], self.v[layer], self.table, p.kv_lens, p.node_start, mask=p.mask,
                               scale=self.scale, out=out, stream=stream, n_live=self._live, max_new=self._most)
 
@@ -568,6 +869,32 @@ class PagedBatcher:
         self.lens = paged_commit(self.k, self.v, self.table, self.lens, p.kv_lens, p.node_start, path, count)
         self.owned, self.used = p.owned, p.free_used
         self._plan = None
+
+    def verify(self, target: torch.Tensor, draft: torch.Tensor | None, tokens: torch.Tensor, u: torch.Tensor,
+               u_next: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Ends a step of drafts with the paths that the target's probabilities
+        keep (verify_drafts), without waiting for the GPU.  The first token of each
+        request is its pending one, the others hang below it.  target, draft
+        [n_tokens, vocab], tokens int32, u f32 [n_tokens]: by token row; u_next f32
+        [max_requests]: by the requests' places.  Returns path, n_accept and the
+        next tokens, by place (place(rid)); idle places have n_accept 0, next -1."""
+        if self._plan is None:
+            raise RuntimeError("no step has begun")
+        p, most = self._plan, max(1, self._most)
+        if most > MAX_NODES:
+            raise ValueError(f"{most} tokens for a request (at most {MAX_NODES} can be verified)")
+        parents = self._parents if p.mask is not None else [a - 1 for t in self._new for a in range(t)]
+        path, count, token = verify_drafts(target, draft, tokens,
+                                           torch.tensor(parents, dtype=torch.int32, device=self.device), p.node_start, u,
+                                           u_next, max_path=most)
+        self.lens = paged_commit(self.k, self.v, self.table, self.lens, p.kv_lens, p.node_start, path, count)
+        self.owned, self.used = p.owned, p.free_used
+        self._plan = None
+        return path, count, token
+
+    def place(self, rid) -> int:
+        """The request's row in the batch's tables."""
+        return self._rows[rid]
 
     def cache(self, rid, layer: int):
         """(K, V) copies [length, n_kv, d] of a request's layer, in position

@@ -113,6 +113,33 @@ extern "C" {
                             lens: *const i32, kv_lens: *const i32, node_start: *const i32, n: u32,
                             path: *const i32, max_path: u32, n_accept: *const i32, lens_out: *mut i32,
                             stream: *mut c_void) -> bml_status;
+    pub fn bml_attn_chunk_workspace_size(head_dim: u32, n_tokens: u32, n_seqs: u32, device: i32,
+                                         bytes: *mut usize) -> bml_status;
+    pub fn bml_attn_chunk(q: *const c_void, q_dtype: bml_dtype, n_tokens: u32, n_heads: u32, n_kv: u32,
+                          head_dim: u32, k_pool: *const c_void, v_pool: *const c_void, kv: bml_dtype, n_pages: u32,
+                          page_size: u32, block_table: *const i32, max_pages: u32, kv_lens: *const i32,
+                          node_start: *const i32, n_seqs: u32, scale: f32, out: *mut c_void, ws: *mut c_void,
+                          ws_bytes: usize, stream: *mut c_void) -> bml_status;
+    pub fn bml_verify_drafts(target: *const c_void, draft: *const c_void, dtype: bml_dtype, vocab: u32,
+                             tokens: *const i32, parents: *const i32, n_tokens: u32, node_start: *const i32, n: u32,
+                             u: *const f32, u_next: *const f32, max_path: u32, path: *mut i32, n_accept: *mut i32,
+                             next: *mut i32, stream: *mut c_void) -> bml_status;
+    pub fn bml_page_fork(k_pool: *mut c_void, v_pool: *mut c_void, n_layers: u32, n_pages: u32, page_size: u32,
+                         n_kv: u32, head_dim: u32, kv: bml_dtype, src: *const i32, dst: *const i32, m: u32,
+                         lens: *const i32, owned: *const i32, n: u32, block_table: *mut i32, max_pages: u32,
+                         shared: *const i32, free_pages: *const i32, n_free: u32, free_used: *const i32,
+                         lens_out: *mut i32, owned_out: *mut i32, shared_out: *mut i32, free_used_out: *mut i32,
+                         status: *mut i32, stream: *mut c_void) -> bml_status;
+    pub fn bml_page_free(keep: *const i32, lens: *const i32, owned: *const i32, n: u32, block_table: *const i32,
+                         max_pages: u32, page_size: u32, shared: *const i32, n_pages: u32, free_pages: *const i32,
+                         n_free: u32, free_used: *const i32, lens_out: *mut i32, owned_out: *mut i32,
+                         shared_out: *mut i32, free_out: *mut i32, free_used_out: *mut i32, status: *mut i32,
+                         stream: *mut c_void) -> bml_status;
+    pub fn bml_page_compact(k_pool: *mut c_void, v_pool: *mut c_void, n_layers: u32, n_pages: u32, page_size: u32,
+                            n_kv: u32, head_dim: u32, kv: bml_dtype, owned: *const i32, n: u32,
+                            block_table: *const i32, max_pages: u32, shared: *const i32, table_out: *mut i32,
+                            shared_out: *mut i32, free_out: *mut i32, free_used_out: *mut i32, ws: *mut c_void,
+                            ws_bytes: usize, stream: *mut c_void) -> bml_status;
     pub fn bml_softmax_f32(x: *const f32, n_rows: u32, n: u32, out: *mut f32,
                            stream: *mut c_void) -> bml_status;
     pub fn bml_attn_workspace_check(ws: *mut c_void, bytes: usize, stream: *mut c_void) -> bml_status;

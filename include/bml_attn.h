@@ -528,6 +528,67 @@ bml_status bml_attn_tree_sized(const void *q_dev, bml_dtype q_dtype,
                                size_t workspace_bytes, uint32_t n_live,
                                uint32_t max_nodes, void *stream);
 
+/* Scratch bytes of bml_attn_chunk on `device` for a batch of that size. */
+bml_status bml_attn_chunk_workspace_size(uint32_t head_dim, uint32_t n_tokens,
+                                         uint32_t n_seqs, int32_t device,
+                                         size_t *bytes);
+
+/* Attention of chunks of new tokens over pages: bml_attn_tree without a mask,
+ * for any number of new tokens a request -- a prompt or a part of one, beside
+ * requests that decode one token.  Token row t of request i (the j-th of its T,
+ * j = t - node_start[i]) attends over the positions [0, kv_lens[i] - T + j].
+ * Types, layouts, refused requests, masked places, infinities, precision and the
+ * limit of waits are bml_attn_tree's; workspace: bml_attn_chunk_workspace_size
+ * bytes, 16-byte aligned, no contents needed, not shared by calls that overlap
+ * in time.  Up to 256 tokens a request, where most have few, bml_attn_tree_sized
+ * is the faster call.  head_dim 64 or 128.  Asynchronous. */
+bml_status bml_attn_chunk(const void *q_dev, bml_dtype q_dtype,
+                          uint32_t n_tokens, uint32_t n_heads,
+                          uint32_t n_kv_heads, uint32_t head_dim,
+                          const void *k_pool, const void *v_pool,
+                          bml_dtype kv_dtype, uint32_t n_pages,
+                          uint32_t page_size, const int32_t *block_table,
+                          uint32_t max_pages, const int32_t *kv_lens,
+                          const int32_t *node_start, uint32_t n_seqs,
+                          float scale, void *out_dev, void *workspace,
+                          size_t workspace_bytes, void *stream);
+
+/* Verification of drafted tokens: which path of each request's draft is kept,
+ * and the token that follows it, so that tokens are distributed as the target
+ * model's.  Nodes are those of bml_paged_plan: token row t of request i is node
+ * j = t - node_start[i]; node 0 is the pending token (chosen before, not in the
+ * cache yet) and is always kept; a node whose parent is an earlier node of its
+ * request is a drafted child of that node, any other never kept.
+ *   target [n_tokens][vocab]: the target model's probabilities behind each node;
+ *   draft [n_tokens][vocab]: those that each node's children were drawn from,
+ *       independently of one another (rows of nodes without children are not
+ *       read); NULL: the tokens were picked, not drawn (the likeliest ones);
+ *   u [n_tokens], u_next [n]: random numbers, uniform in [0, 1);
+ *   path [n][max_path], n_accept [n]: the kept nodes in order, as
+ *       bml_paged_commit takes them; -1 behind them;
+ *   next [n]: the token behind the path, the next step's pending token.
+ * At a kept node with rows p and q its children are tried in node order: the
+ * k-th, of token x, is kept if u q(x) S_k < max(p(x) - c_k q(x), 0), where
+ * c_0 = 0, S_0 = 1, and after a rejection c_(k+1) = c_k + S_k, S_(k+1) =
+ * sum_v max(p(v) - c_(k+1) q(v), 0).  If none is, the path ends there and next
+ * is the smallest v with C(v) > u_next * C(vocab - 1), C the prefix sums of
+ * max(p - c q, 0) with the last c.  Without draft: kept if u S < p(x), and a
+ * rejected x leaves p (S loses p(x), and it is neither kept nor drawn).  Where
+ * nothing of positive weight is left, which rounding can do to 16-bit rows, next
+ * is drawn from p itself; if p has nothing either, or q sums to more than twice p
+ * (no distribution), it is vocab - 1.  Sums are f64.  A path of max_path nodes ends there, its last
+ * node's children untried.  Probabilities that are not positive finite numbers
+ * count as 0; a child whose token is outside [0, vocab) is never tried.  A request
+ * without nodes, or with more than 256, has n_accept 0 and next -1.  target and
+ * draft are of one type, rows need no alignment beyond it.  Asynchronous. */
+bml_status bml_verify_drafts(const void *target, const void *draft,
+                             bml_dtype dtype, uint32_t vocab,
+                             const int32_t *tokens, const int32_t *parents,
+                             uint32_t n_tokens, const int32_t *node_start,
+                             uint32_t n, const float *u, const float *u_next,
+                             uint32_t max_path, int32_t *path,
+                             int32_t *n_accept, int32_t *next, void *stream);
+
 /* Commits the accepted path of every request's draft: in the K and V pools of
  * all n_layers layers (layer l at pool + l * n_pages * page_size * row), row
  * lens[i] + path[i][k] moves to row lens[i] + k for k < n_accept[i], and
@@ -546,6 +607,81 @@ bml_status bml_paged_commit(void *k_pool, void *v_pool, uint32_t n_layers,
                             const int32_t *kv_lens, const int32_t *node_start,
                             uint32_t n, const int32_t *path, uint32_t max_path,
                             const int32_t *n_accept, int32_t *lens_out,
+                            void *stream);
+
+/* Pages held by several requests.  shared [n_pages] int32 counts a page's
+ * holders beyond the first (0: one holder, or none), so bml_paged_plan's new
+ * pages need no entry: an array of zeros at the start.  Shared pages are full
+ * ones, behind which nobody writes: a request's part-filled page is always its
+ * own.  The calls below, like the plan, leave lens, owned, shared and the free
+ * list's count as they are and write their next values into buffers of their
+ * own, which must not overlap one another or what is read.  n, m <= 4096.
+ *
+ * Forks: row dst[j] of the tables continues the lens[src[j]] positions of row
+ * src[j] (several samples of one prompt, beams).  Full pages are shared; the rows
+ * of a part-filled one are copied in all layers to a page of the free list, taken
+ * in the order of j.  dst must be an idle row (lens and owned 0).
+ *   block_table: row dst[j] written, nothing else;
+ *   lens_out, owned_out [n], shared_out [n_pages], free_used_out [1];
+ *   status [m]: 0, or why fork j is refused: 1 not enough free pages (for it and
+ *       the forks before it), 2 a row outside [0, n), a dst that is not idle or
+ *       that an earlier fork names, or a src whose pages do not hold its positions.
+ *       A refused fork changes nothing.
+ * Layers lie as in bml_paged_commit.  Asynchronous. */
+bml_status bml_page_fork(void *k_pool, void *v_pool, uint32_t n_layers,
+                         uint32_t n_pages, uint32_t page_size,
+                         uint32_t n_kv_heads, uint32_t head_dim,
+                         bml_dtype kv_dtype, const int32_t *src,
+                         const int32_t *dst, uint32_t m, const int32_t *lens,
+                         const int32_t *owned, uint32_t n,
+                         int32_t *block_table, uint32_t max_pages,
+                         const int32_t *shared, const int32_t *free_pages,
+                         uint32_t n_free, const int32_t *free_used,
+                         int32_t *lens_out, int32_t *owned_out,
+                         int32_t *shared_out, int32_t *free_used_out,
+                         int32_t *status, void *stream);
+
+/* Ends or rolls back requests: request i keeps min(lens[i], keep[i]) positions
+ * and the pages that hold them, and releases the pages behind (0: all of them;
+ * its length or more: spare pages only; negative: it is left as it is).  A page
+ * that all its holders have released is free again.
+ *   free_out [n_free]: free_pages with the taken part [0, *free_used) parted into
+ *       the pages that are still held and, behind *free_used_out, the freed ones,
+ *       each in the order they had;
+ *   lens_out, owned_out [n], shared_out [n_pages], free_used_out [1];
+ *   status [n]: 8 where keep ends inside a page that others hold: the request is
+ *       left as it is (its next token would be written there); else 0.
+ * block_table is not written: entries from owned_out on mean nothing.
+ * Asynchronous. */
+bml_status bml_page_free(const int32_t *keep, const int32_t *lens,
+                         const int32_t *owned, uint32_t n,
+                         const int32_t *block_table, uint32_t max_pages,
+                         uint32_t page_size, const int32_t *shared,
+                         uint32_t n_pages, const int32_t *free_pages,
+                         uint32_t n_free, const int32_t *free_used,
+                         int32_t *lens_out, int32_t *owned_out,
+                         int32_t *shared_out, int32_t *free_out,
+                         int32_t *free_used_out, int32_t *status,
+                         void *stream);
+
+/* Packs a pool: the H held pages (the first owned[i] entries of each table row)
+ * come to lie at [0, H), in all layers.  Held pages from H on move, in ascending
+ * order, into the pages below H that nobody holds, in ascending order; the
+ * others stay.  The tables (table_out [n][max_pages], other entries copied) and
+ * shared counts (shared_out [n_pages], 0 for free pages) follow, free_out
+ * [n_pages] becomes 0, 1, 2, ... and free_used_out H: the free list is that of
+ * the whole pool.  Pages from H on keep what they held.  workspace: 12 * n_pages
+ * + 4 bytes, no contents needed, not shared by calls that overlap in time.
+ * Asynchronous. */
+bml_status bml_page_compact(void *k_pool, void *v_pool, uint32_t n_layers,
+                            uint32_t n_pages, uint32_t page_size,
+                            uint32_t n_kv_heads, uint32_t head_dim,
+                            bml_dtype kv_dtype, const int32_t *owned,
+                            uint32_t n, const int32_t *block_table,
+                            uint32_t max_pages, const int32_t *shared,
+                            int32_t *table_out, int32_t *shared_out,
+                            int32_t *free_out, int32_t *free_used_out,
+                            void *workspace, size_t workspace_bytes,
                             void *stream);
 
 /* ------------------------------------------------------------------------ */

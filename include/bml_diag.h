@@ -23,7 +23,8 @@ extern "C" {
 #define BML_DIAG_DECODE_DEFAULT 0   /* what bml_attn_decode_batched picks */
 #define BML_DIAG_DECODE_CUDA_CORE 1 /* the CUDA-core kernel, for any dtype */
 
-/* Behaviour flags of bml_diag_decode_batched and bml_diag_attn_tree. */
+/* Behaviour flags of bml_diag_decode_batched, bml_diag_attn_tree and
+ * bml_diag_attn_chunk. */
 #define BML_DIAG_STALL 1u /* the kernel's producer fills no stage, so its
                              consumers' first wait runs out */
 
@@ -41,6 +42,19 @@ bml_status bml_diag_decode_batched(const bml_seq_desc *seqs_host,
                                    void *workspace, size_t workspace_bytes,
                                    int kernel, uint64_t wait_ns,
                                    uint32_t flags, void *stream);
+
+/* bml_attn_chunk in the same way as bml_diag_attn_tree below. */
+bml_status bml_diag_attn_chunk(const void *q_dev, bml_dtype q_dtype,
+                               uint32_t n_tokens, uint32_t n_heads,
+                               uint32_t n_kv_heads, uint32_t head_dim,
+                               const void *k_pool, const void *v_pool,
+                               bml_dtype kv_dtype, uint32_t n_pages,
+                               uint32_t page_size, const int32_t *block_table,
+                               uint32_t max_pages, const int32_t *kv_lens,
+                               const int32_t *node_start, uint32_t n_seqs,
+                               float scale, void *out_dev, void *workspace,
+                               size_t workspace_bytes, uint64_t wait_ns,
+                               uint32_t flags, void *stream);
 
 /* bml_attn_tree with the limit of every bounded device wait (nanoseconds; 0
  * selects the default 2 s) and behaviour flags chosen by the caller.  With
