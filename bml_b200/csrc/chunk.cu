@@ -1,4 +1,6 @@
-// chunk.cu -- attention of chunks of any number of new tokens over a paged cache.
+// chunk.cu -- attention of chunks of any number of new tokens over a paged cache,
+// where chunk_umma.cu does not take them: 32-bit queries, a scale of 0, groups of
+// more than 128 q heads.
 //
 // Row t of a request's T new tokens sees the positions 0 .. P + t, P = L - T.  A
 // chunk is cut into pieces of W consecutive tokens: piece k is a request of its
@@ -89,6 +91,7 @@ size_t chunk_work_bytes(uint64_t n_tokens, uint64_t n_seqs) {
 }
 
 cudaError_t launch_chunk(const TreeArgs &args, int32_t *work, cudaStream_t st) {
+    if (chunk_umma_fits(args)) return launch_chunk_umma(args, st);
     TreeArgs a = args;
     TreeParams &p = a.p;
     PieceParams pp = {};

@@ -95,8 +95,10 @@ cudaError_t launch_tree_few(const TreeArgs &a, cudaStream_t st);
 cudaError_t launch_tree_umma(const TreeArgs &a, cudaStream_t st);
 cudaError_t launch_tree_umma32(const TreeArgs &a, cudaStream_t st);
 
-// Chunks of any number of new tokens (chunk.cu).  work: chunk_work_bytes of scratch.
+// Chunks of any number of new tokens (chunk.cu; chunk_umma.cu where it fits).  work: chunk_work_bytes of scratch.
 cudaError_t launch_chunk(const TreeArgs &a, int32_t *work, cudaStream_t st);
+bool chunk_umma_fits(const TreeArgs &a);
+cudaError_t launch_chunk_umma(const TreeArgs &a, cudaStream_t st);
 size_t chunk_work_bytes(uint64_t n_tokens, uint64_t n_seqs);
 // What the choice of a kernel goes by.
 inline void tree_rows(TreeArgs &a, uint32_t n_tokens, uint32_t group, uint32_t n_seqs, uint32_t n_live, uint32_t max_nodes) {

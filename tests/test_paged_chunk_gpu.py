@@ -51,6 +51,24 @@ def test_many_requests(cuda, qt, ct):
         assert torch.equal(got[:sum(nodes)], attend(c)[:sum(nodes)])
 
 
+@pytest.mark.parametrize("qt,ct", [("bf16", "bf16"), ("f16", "f16"), ("f32", "bf16")])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("kind", ["tokens", "chunks", "both", "short"])
+def test_many_tiles_and_segments(cuda, qt, ct, d, kind):
+    """Each SM gets long runs of tiles of few rows, many short segments, or row
+    groups of one and of two row tiles in turns, of odd and even tile counts."""
+    rng = np.random.default_rng(["tokens", "chunks", "both", "short"].index(kind))
+    n, long, sizes = {"tokens": (60, 4000, [1]), "chunks": (24, 1500, [200, 333, 65]), "both": (90, 1700, [1, 1, 40, 33, 64, 100, 130]),
+                      "short": (400, 200, [1, 2, 70])}[kind]
+    lens = [int(x) for x in rng.integers(0, long, n)]
+    nodes = [int(rng.choice(sizes)) for _ in range(n)]
+    c = Paged(lens, nodes, 16, 4, d, 32, qt, ct, seed=n + d)
+    got = attend(c)
+    check(c, got, sees_of(c), qt, only=range(0, n, 7 if kind == "short" else 3))
+    for _ in range(3):
+        assert torch.equal(attend(c), got)
+
+
 @pytest.mark.parametrize("qt,ct,d", [("bf16", "bf16", 128), ("f16", "f16", 64), ("f32", "f32", 128), ("f32", "bf16", 64)])
 def test_long(cuda, qt, ct, d):
     """One long request that many CTAs share, a long fresh prompt, and a single
