@@ -85,13 +85,14 @@ __global__ void __launch_bounds__(kThreads) chunk_pieces_kernel(const PieceParam
 
 }  // namespace
 
-size_t chunk_work_bytes(uint64_t n_tokens, uint64_t n_seqs) {
+size_t chunk_work_bytes(uint64_t n_tokens, uint64_t n_seqs, int num_sms) {
     // pieces of one token at the least (groups of more than 128 q heads)
-    return (3 * (n_tokens + n_seqs) + n_seqs + 2) * sizeof(int32_t);
+    const size_t pieces = (3 * (n_tokens + n_seqs) + n_seqs + 2) * sizeof(int32_t), cuts = chunk_umma_bytes(n_tokens, num_sms);
+    return pieces > cuts ? pieces : cuts;
 }
 
 cudaError_t launch_chunk(const TreeArgs &args, int32_t *work, cudaStream_t st) {
-    if (chunk_umma_fits(args)) return launch_chunk_umma(args, st);
+    if (chunk_umma_fits(args)) return launch_chunk_umma(args, work, st);
     TreeArgs a = args;
     TreeParams &p = a.p;
     PieceParams pp = {};

@@ -84,6 +84,14 @@ struct ChunkParams {
     uint32_t rt;        // rows of a row tile: 128 / group * group
     uint32_t tpg;       // tokens of a row group: 2 * (128 / group)
     uint32_t box_rows;  // min(page, 128)
+    uint32_t most_phases;
+    struct ChunkCut *cuts;  // [most_phases * CTAs]
+};
+// What the merge reads of the unit that is divided behind piece i of the line and
+// begins in it (rows 0: there is none): rows row0 .. of a request's kv head, with
+// partial results of the pieces i .. last.
+struct ChunkCut {
+    uint32_t first, head, row0, rows, last, pad[3];
 };
 
 // ---------------------------------------------------------------------------
@@ -109,10 +117,8 @@ struct ChunkSeq {
 
 __device__ __forceinline__ uint64_t chunk_weight(const ChunkParams &p, uint32_t rows) { return rows > p.rt ? kHeavy : kLight; }
 
-// kEarly: before griddepcontrol.wait (the merge, which reads past L1).
-template <bool kEarly>
 __device__ __forceinline__ ChunkSeq chunk_seq(const ChunkParams &p, uint32_t i) {
-    const TreeRaw raw = tree_raw<kEarly>(p.t, i);
+    const TreeRaw raw = tree_raw<false>(p.t, i);
     ChunkSeq s;
     const bool rows_ok = raw.a >= 0 && raw.b > raw.a && (uint32_t)raw.b <= p.t.n_tokens;
     s.first = rows_ok ? (uint32_t)raw.a : 0u;
@@ -136,9 +142,9 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const ChunkParams &p, uint32_t i) 
 struct ChunkCuts {
     uint64_t each, more;
     uint32_t active;
-    __device__ __forceinline__ ChunkCuts(uint64_t total, uint32_t grid) {
+    __device__ __forceinline__ ChunkCuts(uint64_t total, uint32_t pieces) {
         const uint64_t most = total / (kHeavy * BN);
-        active = most < 1 ? (total ? 1u : 0u) : most < grid ? (uint32_t)most : grid;
+        active = most < 1 ? (total ? 1u : 0u) : most < pieces ? (uint32_t)most : pieces;
         each = active ? total / active : 0u;
         more = total - each * active;
     }
@@ -149,49 +155,79 @@ struct ChunkCuts {
     }
 };
 
+constexpr uint32_t kMostPhases = 4;
+// K and V bytes of the requests with several row groups that a phase is meant to
+// have: well within the half of L2 that is near to an SM.
+constexpr uint64_t kPhaseBytes = 48ull << 20;
+
 struct ChunkScan {
-    uint64_t sums[32];
-    uint64_t base;
-    uint32_t seq;
+    uint64_t sums[32], bytes[32];
+};
+// Where a CTA's pieces begin: the request that holds a piece's first place, and the
+// request's first place.
+struct ChunkStarts {
+    uint64_t base[kMostPhases];
+    uint32_t seq[kMostPhases];
 };
 
-// The total of the line and, for CTA cut b, the request that holds the cut's place
-// and its first place.  Every thread of the CTA calls it.
-template <bool kEarly>
-__device__ __forceinline__ uint64_t chunk_find(const ChunkParams &p, ChunkScan *sh, uint32_t b, uint32_t grid) {
+// The line's length and its number of phases, and where the CTA's pieces begin.
+// Every thread of the CTA calls it; `starts` is for all of them behind the next
+// barrier.
+struct ChunkLine {
+    uint64_t total;
+    uint32_t phases;
+};
+__device__ __forceinline__ ChunkLine chunk_find(const ChunkParams &p, uint32_t D, ChunkScan *sh, ChunkStarts *starts) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = p.t.n_seqs;
     const uint32_t per = (n + blockDim.x - 1) / blockDim.x, i0 = min(threadIdx.x * per, n), i1 = min(i0 + per, n);
-    uint64_t mine = 0;
-    for (uint32_t i = i0; i < i1; ++i) mine += chunk_seq<kEarly>(p, i).places * p.t.n_kv;
+    uint64_t mine = 0, again = 0;  // again: positions that are read more than once
+    for (uint32_t i = i0; i < i1; ++i) {
+        const ChunkSeq s = chunk_seq(p, i);
+        mine += s.places * p.t.n_kv;
+        if (s.groups > 1 && s.ok) again += (uint32_t)s.P + s.T;
+    }
     uint64_t inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const uint64_t a = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= (uint32_t)o) inc += a;
     }
-    if (lane == 31) sh->sums[warp] = inc;
-    if (threadIdx.x == 0) sh->seq = n;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) again += __shfl_xor_sync(0xffffffffu, again, o);
+    if (lane == 31) {
+        sh->sums[warp] = inc;
+        sh->bytes[warp] = again;
+    }
+    if (threadIdx.x < kMostPhases) starts->seq[threadIdx.x] = n;
     __syncthreads();
-    uint64_t at = inc - mine, total = 0;
+    uint64_t at = inc - mine;
+    ChunkLine line = {0, 1};
+    again = 0;
     for (uint32_t w = 0; w < blockDim.x / 32; ++w) {
         if (w < warp) at += sh->sums[w];
-        total += sh->sums[w];
+        line.total += sh->sums[w];
+        again += sh->bytes[w];
     }
-    const ChunkCuts cuts(total, grid);
-    const uint64_t w0 = cuts.at(b);
-    if (b < cuts.active && w0 >= at && w0 < at + mine) {
-        uint32_t i = i0;
-        while (i + 1 < i1) {
-            const uint64_t x = chunk_seq<kEarly>(p, i).places * p.t.n_kv;
-            if (w0 < at + x) break;
-            at += x;
-            ++i;
+    again *= 4ull * D * p.t.n_kv;
+    while (line.phases < p.most_phases && again > kPhaseBytes * line.phases) ++line.phases;
+    const ChunkCuts cuts(line.total, line.phases * gridDim.x);
+    for (uint32_t k = 0; k < line.phases; ++k) {
+        const uint32_t piece = k * gridDim.x + blockIdx.x;
+        const uint64_t w0 = cuts.at(piece);
+        if (piece < cuts.active && w0 >= at && w0 < at + mine) {
+            uint64_t base = at;
+            uint32_t i = i0;
+            while (i + 1 < i1) {
+                const uint64_t x = chunk_seq(p, i).places * p.t.n_kv;
+                if (w0 < base + x) break;
+                base += x;
+                ++i;
+            }
+            starts->seq[k] = i;
+            starts->base[k] = base;
         }
-        sh->seq = i;
-        sh->base = at;
     }
-    __syncthreads();
-    return total;
+    return line;
 }
 
 // Consecutive tiles of one unit.
@@ -201,27 +237,29 @@ struct ChunkSeg {
     uint32_t tiles;
     uint64_t u0, w;      // the place of the unit's first tile, a tile's weight
     uint32_t row0, rows;
-    uint32_t slot;       // partial slot of the CTA: 0 the unit began before, 1 it ends after, 2 whole
+    uint32_t slot;       // partial slot of the piece: 0 the unit began before, 1 it ends after, 2 whole
     ChunkSeq s;
 };
 
+// The segments of a CTA's pieces in order.
 struct ChunkWalk {
     uint64_t pos, end, base;
-    uint32_t seq;
+    uint32_t seq, phase;
+    ChunkLine line;
     ChunkSeq s;
-    template <bool kEarly>
-    __device__ __forceinline__ void begin(const ChunkParams &p, const ChunkScan *sh, uint64_t total, uint32_t b, uint32_t grid) {
-        const ChunkCuts cuts(total, grid);
-        seq = sh->seq;
-        base = sh->base;
+    __device__ __forceinline__ uint32_t piece() const { return phase * gridDim.x + blockIdx.x; }
+    __device__ __forceinline__ void begin(const ChunkParams &p, const ChunkStarts *starts) {
+        const ChunkCuts cuts(line.total, line.phases * gridDim.x);
+        seq = starts->seq[phase];
+        base = starts->base[phase];
         pos = end = 0;
-        if (b < cuts.active && seq < p.t.n_seqs) {
-            pos = cuts.at(b);
-            end = cuts.at(b + 1);
-            s = chunk_seq<kEarly>(p, seq);
+        if (piece() < cuts.active && seq < p.t.n_seqs) {
+            pos = cuts.at(piece());
+            end = cuts.at(piece() + 1);
+            s = chunk_seq(p, seq);
         }
     }
-    template <bool kEarly>
+    // the next segment of the piece
     __device__ __forceinline__ bool next(const ChunkParams &p, ChunkSeg &g) {
         while (pos < end) {
             while (pos - base >= s.places * p.t.n_kv) {
@@ -230,9 +268,11 @@ struct ChunkWalk {
                     pos = end;
                     return false;
                 }
-                s = chunk_seq<kEarly>(p, seq);
+                s = chunk_seq(p, seq);
             }
-            const uint64_t off = pos - base, head = off / s.places, in_head = off - head * s.places;
+            const uint64_t off = pos - base;
+            const uint32_t head = p.t.n_kv == 1 ? 0u : (uint32_t)(off / s.places);
+            const uint64_t in_head = off - head * s.places;
             uint32_t lo = 0, hi = s.groups;  // the last row group that begins at in_head or before
             while (hi - lo > 1) {
                 const uint32_t mid = (lo + hi) >> 1;
@@ -247,10 +287,11 @@ struct ChunkWalk {
             g.w = chunk_weight(p, g.rows);
             const uint64_t in = in_head - s.before(lo), len = kLead + g.w * (last + 127u);
             const uint64_t out = min(in + (end - pos), len);
-            // tiles that begin in [in, out)
+            // tiles that begin in [0, x): a tile's places, 128 w, divided in two steps
             auto first_at = [&](uint64_t x) {
-                const uint64_t t = x <= kLead ? 0u : (x - kLead + g.w * BN - 1) / (g.w * BN);
-                return (uint32_t)min(t, (uint64_t)g.tiles);
+                if (x <= kLead) return 0u;
+                const uint32_t y = (uint32_t)((x - kLead + BN - 1) / BN);  // below 2^31 * 5 / 128
+                return min(g.w == kHeavy ? (y + (uint32_t)kHeavy - 1) / (uint32_t)kHeavy : (y + (uint32_t)kLight - 1) / (uint32_t)kLight, g.tiles);
             };
             g.t0 = first_at(in);
             g.t1 = first_at(out);
@@ -259,7 +300,7 @@ struct ChunkWalk {
             if (g.t0 >= g.t1) continue;  // no tile begins here
             g.seq = seq;
             g.s = s;
-            g.head = (uint32_t)head;
+            g.head = head;
             g.slot = g.t0 > 0 ? 0u : (g.t1 < g.tiles ? 1u : 2u);
             return true;
         }
@@ -268,8 +309,12 @@ struct ChunkWalk {
 };
 
 __device__ __forceinline__ size_t chunk_slot(const ChunkParams &p, uint32_t D) { return ((size_t)2 * p.rt * (D + 2) + 3) & ~(size_t)3; }
-__device__ __forceinline__ float *chunk_part(const ChunkParams &p, uint32_t D, uint32_t b, uint32_t which) {
-    return p.t.part + (2 * (size_t)b + which) * chunk_slot(p, D);
+// Partial slot i: 2 * piece + (0: the unit began before the piece, 1: it ends after).
+__device__ __forceinline__ float *chunk_part(const ChunkParams &p, uint32_t D, uint32_t i) { return p.t.part + i * chunk_slot(p, D); }
+// The record of a segment that is its unit's first and not its last.
+__device__ __forceinline__ ChunkCut chunk_cut(const ChunkParams &p, const ChunkLine &line, const ChunkSeg &g) {
+    const ChunkCuts cuts(line.total, line.phases * gridDim.x);
+    return {g.s.first, g.head, g.row0, g.rows, cuts.owner(g.u0 + (uint64_t)(g.tiles - 1) * g.w * BN), {}};
 }
 // Element index of row r (token * group + g) of a request's kv head in q and out.
 __device__ __forceinline__ size_t chunk_row(const ChunkParams &p, uint32_t first, uint32_t head, uint32_t r, uint32_t D) {
@@ -285,8 +330,10 @@ struct Board {
     uint32_t seq, first, T;
     int32_t P;
     uint32_t head, row0, t0;
-    uint32_t packed;  // tiles | slot << 28 | 1 << 31; 0: no more segments
+    uint32_t n;     // tiles; 0: no more segments
+    uint32_t part;  // partial slot, kWhole: none
 };
+constexpr uint32_t kWhole = 0xffffffffu;
 
 // Small shared arrays behind the ring.
 struct alignas(16) ChunkShared {
@@ -304,6 +351,7 @@ struct alignas(16) ChunkShared {
     // chains have read it, so none is more than STAGES + 1 segments ahead.
     uint32_t odd[2][8];
     Board board[kBoard];
+    ChunkStarts starts;
     union {
         // [chain][half][row]: maxima on the way to the other half of the row, sums at a
         // segment's end.  One buffer is enough: a thread writes the next tile's value
@@ -392,25 +440,29 @@ __device__ __noinline__ void add_nonfinite(const TreeParams &p, uint32_t seq, ui
 }
 
 // A wait of the CTA gave up: NaN in the rows of all its segments (in the sums of
-// those that the merge joins).
-__device__ __noinline__ void chunk_give_up(const ChunkParams &p, ChunkScan *sh, uint32_t D) {
-    __syncthreads();
-    const uint64_t total = chunk_find<false>(p, sh, blockIdx.x, gridDim.x);
+// those that the merge joins).  `walk` as at the start.
+__device__ __noinline__ void chunk_give_up(const ChunkParams &p, const ChunkStarts *starts, ChunkLine line, uint32_t D) {
     ChunkWalk walk;
-    walk.begin<false>(p, sh, total, blockIdx.x, gridDim.x);
+    walk.line = line;
     ChunkSeg g;
     const uint32_t R = 2 * p.rt;
-    while (walk.next<false>(p, g)) {
-        float *part = g.slot < 2 ? chunk_part(p, D, blockIdx.x, g.slot) : nullptr;
-        for (uint32_t r = threadIdx.x; r < g.rows; r += blockDim.x) {
-            if (part) {
-                part[(size_t)R * D + r] = 0.f;
-                part[(size_t)R * (D + 1) + r] = __int_as_float(0x7fffffff);
-            } else {
-                uint4 *out = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.t.out) + chunk_row(p, g.s.first, g.head, g.row0 + r, D));
-                for (uint32_t u = 0; u < D / 8; ++u) out[u] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+    for (walk.phase = 0; walk.phase < line.phases; ++walk.phase) {
+        walk.begin(p, starts);
+        ChunkCut cut = {};
+        while (walk.next(p, g)) {
+            float *part = g.slot < 2 ? chunk_part(p, D, 2 * walk.piece() + g.slot) : nullptr;
+            if (g.slot == 1) cut = chunk_cut(p, line, g);
+            for (uint32_t r = threadIdx.x; r < g.rows; r += blockDim.x) {
+                if (part) {
+                    part[(size_t)R * D + r] = 0.f;
+                    part[(size_t)R * (D + 1) + r] = __int_as_float(0x7fffffff);
+                } else {
+                    uint4 *out = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p.t.out) + chunk_row(p, g.s.first, g.head, g.row0 + r, D));
+                    for (uint32_t u = 0; u < D / 8; ++u) out[u] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+                }
             }
         }
+        if (threadIdx.x == 0) p.cuts[walk.piece()] = cut;
     }
 }
 
@@ -464,10 +516,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_umma_kernel(const __grid_co
     }
     tc_fence_before();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const uint64_t total = chunk_find<false>(cp, &sh.scan, blockIdx.x, gridDim.x);
-    ChunkWalk walk;
-    if (warp == 2) walk.begin<false>(cp, &sh.scan, total, blockIdx.x, gridDim.x);
-    __syncthreads();  // the set-up above, and the scan's shared memory read
+    const ChunkLine line = chunk_find(cp, D, &sh.scan, &sh.starts);
+    __syncthreads();  // the set-up above, the CTA's starts, and the scan's shared memory read
     tc_fence_after();
     const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may take its place; it waits for this grid
@@ -492,8 +542,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_umma_kernel(const __grid_co
         b.head = v->head;
         b.row0 = v->row0;
         b.t0 = v->t0;
-        b.packed = v->packed;
-        return b.packed != 0u;
+        b.n = v->n;
+        b.part = v->part;
+        return b.n != 0u;
     };
     auto segment_done = [&]() {
         __syncwarp();
@@ -519,7 +570,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_umma_kernel(const __grid_co
             live = live && __all_sync(0xffffffffu, wait_bar(bar, parity, abort_flag, p.wait_ns));
         };
         auto copy = [&](const Board &b) {
-            const uint32_t n = b.packed & 0xfffffffu, rows = min(b.T * p.group - b.row0, 2 * cp.rt);
+            const uint32_t n = b.n, rows = min(b.T * p.group - b.row0, 2 * cp.rt);
             const bool pair = rows > cp.rt, alone = b.T <= cp.tpg;
             const uint32_t t_end = min(b.T, b.row0 / p.group + cp.tpg);
             const uint32_t lim = b.P < 0 ? 0u : (uint32_t)b.P + t_end;  // positions that the unit sees
@@ -586,12 +637,29 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_umma_kernel(const __grid_co
                 ++segs;
             }
         } else {
+            if (lane >= line.phases && lane < cp.most_phases) cp.cuts[lane * gridDim.x + blockIdx.x] = ChunkCut{};
+            ChunkWalk walk;
+            walk.line = line;
+            walk.phase = 0;
+            walk.begin(cp, &sh.starts);
             ChunkSeg sg;
+            ChunkCut cut = {};
             bool more = true;
             while (more) {
-                more = live && !*abort_flag && walk.next<false>(cp, sg);
+                more = live && !*abort_flag;
+                while (more && !walk.next(cp, sg)) {
+                    if (lane == 0) cp.cuts[walk.piece()] = cut;
+                    cut = {};
+                    if (++walk.phase >= line.phases) more = false;
+                    else walk.begin(cp, &sh.starts);
+                }
                 more = __shfl_sync(0xffffffffu, more, 0);
-                b = more ? Board{sg.seq, sg.s.first, sg.s.T, sg.s.P, sg.head, sg.row0, sg.t0, (sg.t1 - sg.t0) | sg.slot << 28 | 1u << 31} : Board{};
+                b = Board{};
+                if (more) {
+                    b = Board{sg.seq, sg.s.first, sg.s.T, sg.s.P, sg.head, sg.row0, sg.t0, sg.t1 - sg.t0,
+                              sg.slot < 2 ? 2 * walk.piece() + sg.slot : kWhole};
+                    if (sg.slot == 1) cut = chunk_cut(cp, line, sg);
+                }
                 // not cut short by the abort flag: the others still read what lies there
                 if (entry >= kBoard && !mbar_drain(&sh.seg_empty[entry % kBoard], (entry / kBoard - 1) & 1u, 8 * p.wait_ns)) *abort_flag = 1u;
                 __syncwarp();
@@ -722,7 +790,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_umma_kernel(const __grid_co
         };
         Board b;
         for (; segment(b); segment_done()) {
-            const uint32_t n = uniform(b.packed & 0xfffffffu);
+            const uint32_t n = uniform(b.n);
             if (live) work(uniform(min(b.T * p.group - b.row0, 2 * cp.rt)) > cp.rt, n);
             tiles += n;
             ++segs;
@@ -743,7 +811,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_umma_kernel(const __grid_co
         uint32_t finals = 0;  // phase parity of o_final[x]
         Board b;
         for (; segment(b); segment_done()) {
-            const uint32_t n = b.packed & 0xfffffffu, slot_of = b.packed >> 28 & 7u;
+            const uint32_t n = b.n;
             const uint32_t rows = min(b.T * p.group - b.row0, 2 * cp.rt);
             const bool pair = rows > cp.rt;
             const uint32_t nt = pair ? n : (x ? n / 2 : (n + 1) / 2);
@@ -915,7 +983,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_umma_kernel(const __grid_co
             tc_fence_after();
             const float inv = l == 0.f ? 0.f : 1.f / l;
             const size_t at = valid ? chunk_row(cp, b.first, b.head, b.row0 + row, D) : 0;
-            float *part = slot_of < 2 ? chunk_part(cp, D, blockIdx.x, slot_of) : nullptr;
+            float *part = b.part != kWhole ? chunk_part(cp, D, b.part) : nullptr;
             const uint32_t hi = min(kv_first + n * BN, (uint32_t)max(last + 1, 0));
             // either chain: of two that look at the same tile, the second may find zeros
             const bool odd = *(volatile uint32_t *)&sh.odd[0][segs & 7u] == segs + 1 || *(volatile uint32_t *)&sh.odd[1][segs & 7u] == segs + 1;
@@ -983,7 +1051,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_umma_kernel(const __grid_co
 
     tc_fence_before();
     __syncthreads();
-    if (*abort_flag) chunk_give_up(cp, &sh.scan, D);
+    if (*abort_flag) chunk_give_up(cp, &sh.starts, line, D);
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS) : "memory");
@@ -991,41 +1059,28 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_umma_kernel(const __grid_co
 }
 
 // ---------------------------------------------------------------------------
-// Merge of the units that a cut divides: CTA (x, y) serves the unit that cut x + 1
-// divides, if that is the first cut in it, and takes the unit's tasks y, y +
-// gridDim.y, ...  A task is 8 rows x 32 columns of a warp.  Segments are added in a
-// fixed order, so a result does not depend on timing.
+// Merge of the units that a cut divides: CTA (x, y) serves the one that begins in
+// piece x and is divided behind it, and takes its tasks y, y + gridDim.y, ...  A task
+// is 8 rows x 32 columns of a warp.  Segments are added in a fixed order, so a result
+// does not depend on timing.
 // ---------------------------------------------------------------------------
 constexpr int kMergeThreads = 256;
 
 template <int D, bool kF16>
-__global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const __grid_constant__ ChunkParams cp, uint32_t grid) {
-    __shared__ ChunkScan sh;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, b = blockIdx.x + 1;
-    // the lengths are inputs of the call, not results of the kernel before, and that
-    // kernel has waited for their writer
-    const uint64_t total = chunk_find<true>(cp, &sh, b, grid);
-    ChunkWalk walk;
-    walk.begin<true>(cp, &sh, total, b, grid);
-    ChunkSeg g;
-    bool mine = walk.next<true>(cp, g) && g.t0 > 0;
-    uint32_t last = 0;  // the CTAs with a segment of the unit: b - 1 to last
-    if (mine) {
-        const ChunkCuts cuts(total, grid);
-        last = cuts.owner(g.u0 + (uint64_t)(g.tiles - 1) * g.w * BN);
-        mine = last >= b && cuts.owner(g.u0) == b - 1;
-    }
+__global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const __grid_constant__ ChunkParams cp) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the segments' partials are written
-    if (!mine) return;
+    const ChunkCut g = cp.cuts[blockIdx.x];
+    const uint32_t from = blockIdx.x, last = g.last;
     const uint32_t R = 2 * cp.rt, tasks = (g.rows + 7) / 8 * (D / 32);
     for (uint32_t task = blockIdx.y * (kMergeThreads / 32) + warp; task < tasks; task += gridDim.y * (kMergeThreads / 32)) {
         const uint32_t row = task / (D / 32) * 8 + (lane & 7), x4 = task % (D / 32) * 8 + (lane >> 3);
         if (row >= g.rows) continue;
-        auto part = [&](uint32_t s) { return chunk_part(cp, D, s, s == b - 1 ? 1u : 0u); };
+        auto part = [&](uint32_t s) { return chunk_part(cp, D, 2 * s + (s == from ? 1u : 0u)); };
         float m = -INFINITY, l = 0.f;
         float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
         constexpr uint32_t kBatch = 4;  // segments whose loads are in flight together
-        for (uint32_t s0 = b - 1; s0 <= last; s0 += kBatch) {
+        for (uint32_t s0 = from; s0 <= last; s0 += kBatch) {
             float f[kBatch], ls[kBatch];
             float4 y[kBatch][2];
 #pragma unroll
@@ -1062,7 +1117,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const __grid
             m = mn;
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        uint16_t *out = static_cast<uint16_t *>(cp.t.out) + chunk_row(cp, g.s.first, g.head, g.row0 + row, D) + x4 * 4;
+        uint16_t *out = static_cast<uint16_t *>(cp.t.out) + chunk_row(cp, g.first, g.head, g.row0 + row, D) + x4 * 4;
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
             const float any = (acc[z].x + acc[z].y) + (acc[z].z + acc[z].w);
@@ -1070,7 +1125,7 @@ __global__ void __launch_bounds__(kMergeThreads) chunk_merge_kernel(const __grid
                 // a segment's infinity met a weight that is 0 in 32 bits: such a column is
                 // the sum of the segments' values that are not finite
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                for (uint32_t s = b - 1; s <= last; ++s) {
+                for (uint32_t s = from; s <= last; ++s) {
                     const float4 v = reinterpret_cast<const float4 *>(part(s))[(size_t)(x4 + 4 * z) * R + row];
                     const float xs[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -1112,19 +1167,25 @@ cudaError_t launch_c(const ChunkParams &cp, int num_sms, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     e = launch_after(kern, dim3(num_sms), kThreads, C::SMEM, st, cp);
     if (e != cudaSuccess || num_sms < 2) return e;
-    return launch_after(chunk_merge_kernel<D, kF16>, dim3(num_sms - 1, 2), kMergeThreads, 0, st, cp, (uint32_t)num_sms);
+    return launch_after(chunk_merge_kernel<D, kF16>, dim3(num_sms * cp.most_phases - 1, 8), kMergeThreads, 0, st, cp);
 }
 
 }  // namespace
+
+// Phases that a batch of so many tokens may take: more need more partial results.
+uint32_t chunk_phases(uint64_t n_tokens) { return n_tokens >= 1024 ? kMostPhases : 1; }
+size_t chunk_umma_bytes(uint64_t n_tokens, int num_sms) { return sizeof(ChunkCut) * chunk_phases(n_tokens) * num_sms; }
 
 bool chunk_umma_fits(const TreeArgs &a) {
     // positions and tokens are compared in 32 bits with a sign
     return a.p.q_type != BML_F32 && a.p.scale_log2 > 0.f && a.p.group <= (uint32_t)BM && a.p.n_tokens <= 1u << 30;
 }
 
-cudaError_t launch_chunk_umma(const TreeArgs &a, cudaStream_t st) {
+cudaError_t launch_chunk_umma(const TreeArgs &a, int32_t *work, cudaStream_t st) {
     static thread_local ChunkParams cp;
     cp.t = a.p;
+    cp.most_phases = chunk_phases(a.p.n_tokens);
+    cp.cuts = reinterpret_cast<ChunkCut *>(work);
     const uint32_t group = a.p.group, page = 1u << a.p.page_shift;
     const bool f16 = a.kv_type == BML_F16;
     cp.rt = BM / group * group;

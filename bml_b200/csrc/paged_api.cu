@@ -154,7 +154,8 @@ bml_status attn_tree(const char *fn, bool chunk, const void *q_dev, bml_dtype q_
         !aligned(mask, 8))
         return api_fail(BML_E_INVALID, "%s: pointers must be 16-byte aligned (mask 8)", fn);
     const int sms = sm_count(this_device());
-    const size_t parts = bml::tree_workspace_bytes(head_dim, sms), need = parts + (chunk ? bml::chunk_work_bytes(n_tokens, n_seqs) : 0);
+    const size_t parts = bml::tree_workspace_bytes(head_dim, sms) * (chunk ? bml::chunk_phases(n_tokens) : 1);
+    const size_t need = parts + (chunk ? bml::chunk_work_bytes(n_tokens, n_seqs, sms) : 0);
     if (workspace_bytes < need) return api_fail(BML_E_INVALID, "%s: workspace of %zu bytes, need %zu", fn, workspace_bytes, need);
     const size_t es = bml::dtype_size(q_dtype);
     const uintptr_t qa = reinterpret_cast<uintptr_t>(q_dev), oa = reinterpret_cast<uintptr_t>(out_dev);
@@ -237,7 +238,7 @@ BML_API bml_status bml_attn_tree_sized(const void *q_dev, bml_dtype q_dtype, uin
 
 BML_API bml_status bml_attn_chunk_workspace_size(uint32_t head_dim, uint32_t n_tokens, uint32_t n_seqs, int32_t device, size_t *bytes) {
     const bml_status st = bml_attn_tree_workspace_size(head_dim, device, bytes);
-    if (st == BML_OK) *bytes += bml::chunk_work_bytes(n_tokens, n_seqs);
+    if (st == BML_OK) *bytes = *bytes * bml::chunk_phases(n_tokens) + bml::chunk_work_bytes(n_tokens, n_seqs, sm_count(device));
     return st;
 }
 

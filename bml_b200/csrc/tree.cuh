@@ -98,8 +98,10 @@ cudaError_t launch_tree_umma32(const TreeArgs &a, cudaStream_t st);
 // Chunks of any number of new tokens (chunk.cu; chunk_umma.cu where it fits).  work: chunk_work_bytes of scratch.
 cudaError_t launch_chunk(const TreeArgs &a, int32_t *work, cudaStream_t st);
 bool chunk_umma_fits(const TreeArgs &a);
-cudaError_t launch_chunk_umma(const TreeArgs &a, cudaStream_t st);
-size_t chunk_work_bytes(uint64_t n_tokens, uint64_t n_seqs);
+cudaError_t launch_chunk_umma(const TreeArgs &a, int32_t *work, cudaStream_t st);
+size_t chunk_umma_bytes(uint64_t n_tokens, int num_sms);
+uint32_t chunk_phases(uint64_t n_tokens);  // the partial results are so many times tree_workspace_bytes
+size_t chunk_work_bytes(uint64_t n_tokens, uint64_t n_seqs, int num_sms);
 // What the choice of a kernel goes by.
 inline void tree_rows(TreeArgs &a, uint32_t n_tokens, uint32_t group, uint32_t n_seqs, uint32_t n_live, uint32_t max_nodes) {
     a.live = n_live && n_live < n_seqs ? n_live : n_seqs;
