@@ -99,7 +99,7 @@ struct ChunkCut {
 // ---------------------------------------------------------------------------
 // A tile of two row tiles against one of one, and a unit's start and end in places
 // (of a 128th of a weight).
-constexpr uint64_t kHeavy = 5, kLight = 3, kLead = 20 * 128;
+constexpr uint64_t kHeavy = 2, kLight = 1, kLead = 8 * 128;
 
 struct ChunkSeq {
     uint32_t first, T;   // token rows
@@ -136,51 +136,50 @@ __device__ __forceinline__ ChunkSeq chunk_seq(const ChunkParams &p, uint32_t i) 
     return s;
 }
 
-// The line of `total` places cut for up to `grid` CTAs, at least a heavy tile each:
-// the first `more` take one more than the others.  A tile belongs to the CTA in
-// whose part it begins.
-struct ChunkCuts {
-    uint64_t each, more;
-    uint32_t active;
-    __device__ __forceinline__ ChunkCuts(uint64_t total, uint32_t pieces) {
-        const uint64_t most = total / (kHeavy * BN);
-        active = most < 1 ? (total ? 1u : 0u) : most < pieces ? (uint32_t)most : pieces;
-        each = active ? total / active : 0u;
-        more = total - each * active;
-    }
-    __device__ __forceinline__ uint64_t at(uint32_t b) const { return each * b + min((uint64_t)b, more); }
-    __device__ __forceinline__ uint32_t owner(uint64_t w) const {
-        const uint64_t wide = more * (each + 1);
-        return (uint32_t)(w < wide ? w / (each + 1) : more + (w - wide) / each);
-    }
-};
+// Out of line, and in 32 bits where they are enough: a launch meets this code cold.
+__device__ __noinline__ uint64_t chunk_div(uint64_t a, uint64_t b) {
+    if (((a | b) >> 32) == 0) return (uint32_t)a / (uint32_t)b;
+    return a / b;
+}
 
 constexpr uint32_t kMostPhases = 4;
 // K and V bytes of the requests with several row groups that a phase is meant to
-// have: well within the half of L2 that is near to an SM.
-constexpr uint64_t kPhaseBytes = 48ull << 20;
+// have.  Measured on B200 (L2 of 126 MB): 134 MB in one phase 958 us, in two 892, in
+// three 870 to 895; 74 MB in one 170, in two 185.
+constexpr uint64_t kPhaseBytes = 80ull << 20;
 
-struct ChunkScan {
-    uint64_t sums[32], bytes[32];
+// The line of `total` places, cut into `active` pieces (a CTA's of each phase, at
+// least a heavy tile each): the first `more` take one place more than the others.  A
+// tile belongs to the piece in which it begins.
+struct ChunkLine {
+    uint64_t total, each, more;
+    uint32_t phases, active;
+    __device__ __forceinline__ void cut(uint32_t pieces) {
+        active = total >= pieces * kHeavy * BN ? pieces : max((uint32_t)total / (uint32_t)(kHeavy * BN), total ? 1u : 0u);
+        each = active ? chunk_div(total, active) : 0u;
+        more = total - each * active;
+    }
+    __device__ __forceinline__ uint64_t at(uint32_t piece) const { return each * piece + min((uint64_t)piece, more); }
+    __device__ __forceinline__ uint32_t owner(uint64_t w) const {
+        const uint64_t wide = more * (each + 1);
+        return (uint32_t)(w < wide ? chunk_div(w, each + 1) : more + chunk_div(w - wide, each));
+    }
 };
-// Where a CTA's pieces begin: the request that holds a piece's first place, and the
-// request's first place.
+
+// What the schedule's warp finds at the start: the line, and for each of the CTA's
+// pieces the request that holds its first place, and that request's first place.
 struct ChunkStarts {
+    ChunkLine line;
     uint64_t base[kMostPhases];
     uint32_t seq[kMostPhases];
 };
 
-// The line's length and its number of phases, and where the CTA's pieces begin.
-// Every thread of the CTA calls it; `starts` is for all of them behind the next
-// barrier.
-struct ChunkLine {
-    uint64_t total;
-    uint32_t phases;
-};
-__device__ __forceinline__ ChunkLine chunk_find(const ChunkParams &p, uint32_t D, ChunkScan *sh, ChunkStarts *starts) {
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = p.t.n_seqs;
-    const uint32_t per = (n + blockDim.x - 1) / blockDim.x, i0 = min(threadIdx.x * per, n), i1 = min(i0 + per, n);
+// By one warp: a lane takes a run of requests.
+__device__ __forceinline__ void chunk_find(const ChunkParams &p, uint32_t D, ChunkStarts *out) {
+    const uint32_t lane = threadIdx.x & 31, n = p.t.n_seqs;
+    const uint32_t per = (n + 31) / 32, i0 = min(lane * per, n), i1 = min(i0 + per, n);
     uint64_t mine = 0, again = 0;  // again: positions that are read more than once
+#pragma unroll 4
     for (uint32_t i = i0; i < i1; ++i) {
         const ChunkSeq s = chunk_seq(p, i);
         mine += s.places * p.t.n_kv;
@@ -189,33 +188,24 @@ __device__ __forceinline__ ChunkLine chunk_find(const ChunkParams &p, uint32_t D
     uint64_t inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t a = __shfl_up_sync(0xffffffffu, inc, o);
+        const uint64_t a = __shfl_up_sync(0xffffffffu, inc, o), c = __shfl_xor_sync(0xffffffffu, again, o);
         if (lane >= (uint32_t)o) inc += a;
+        again += c;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) again += __shfl_xor_sync(0xffffffffu, again, o);
-    if (lane == 31) {
-        sh->sums[warp] = inc;
-        sh->bytes[warp] = again;
-    }
-    if (threadIdx.x < kMostPhases) starts->seq[threadIdx.x] = n;
-    __syncthreads();
-    uint64_t at = inc - mine;
-    ChunkLine line = {0, 1};
-    again = 0;
-    for (uint32_t w = 0; w < blockDim.x / 32; ++w) {
-        if (w < warp) at += sh->sums[w];
-        line.total += sh->sums[w];
-        again += sh->bytes[w];
-    }
+    ChunkLine line;
+    line.total = __shfl_sync(0xffffffffu, inc, 31);
+    line.phases = 1;
     again *= 4ull * D * p.t.n_kv;
     while (line.phases < p.most_phases && again > kPhaseBytes * line.phases) ++line.phases;
-    const ChunkCuts cuts(line.total, line.phases * gridDim.x);
+    line.cut(line.phases * gridDim.x);
+    if (lane < kMostPhases) out->seq[lane] = n;
+    if (lane == 0) out->line = line;
+    __syncwarp();
     for (uint32_t k = 0; k < line.phases; ++k) {
         const uint32_t piece = k * gridDim.x + blockIdx.x;
-        const uint64_t w0 = cuts.at(piece);
-        if (piece < cuts.active && w0 >= at && w0 < at + mine) {
-            uint64_t base = at;
+        const uint64_t w0 = line.at(piece);
+        uint64_t base = inc - mine;
+        if (piece < line.active && w0 >= base && w0 < inc) {
             uint32_t i = i0;
             while (i + 1 < i1) {
                 const uint64_t x = chunk_seq(p, i).places * p.t.n_kv;
@@ -223,11 +213,11 @@ __device__ __forceinline__ ChunkLine chunk_find(const ChunkParams &p, uint32_t D
                 base += x;
                 ++i;
             }
-            starts->seq[k] = i;
-            starts->base[k] = base;
+            out->seq[k] = i;
+            out->base[k] = base;
         }
     }
-    return line;
+    __syncwarp();
 }
 
 // Consecutive tiles of one unit.
@@ -249,13 +239,12 @@ struct ChunkWalk {
     ChunkSeq s;
     __device__ __forceinline__ uint32_t piece() const { return phase * gridDim.x + blockIdx.x; }
     __device__ __forceinline__ void begin(const ChunkParams &p, const ChunkStarts *starts) {
-        const ChunkCuts cuts(line.total, line.phases * gridDim.x);
         seq = starts->seq[phase];
         base = starts->base[phase];
         pos = end = 0;
-        if (piece() < cuts.active && seq < p.t.n_seqs) {
-            pos = cuts.at(piece());
-            end = cuts.at(piece() + 1);
+        if (seq < p.t.n_seqs) {
+            pos = line.at(piece());
+            end = line.at(piece() + 1);
             s = chunk_seq(p, seq);
         }
     }
@@ -271,7 +260,7 @@ struct ChunkWalk {
                 s = chunk_seq(p, seq);
             }
             const uint64_t off = pos - base;
-            const uint32_t head = p.t.n_kv == 1 ? 0u : (uint32_t)(off / s.places);
+            const uint32_t head = (uint32_t)chunk_div(off, s.places);
             const uint64_t in_head = off - head * s.places;
             uint32_t lo = 0, hi = s.groups;  // the last row group that begins at in_head or before
             while (hi - lo > 1) {
@@ -313,8 +302,7 @@ __device__ __forceinline__ size_t chunk_slot(const ChunkParams &p, uint32_t D) {
 __device__ __forceinline__ float *chunk_part(const ChunkParams &p, uint32_t D, uint32_t i) { return p.t.part + i * chunk_slot(p, D); }
 // The record of a segment that is its unit's first and not its last.
 __device__ __forceinline__ ChunkCut chunk_cut(const ChunkParams &p, const ChunkLine &line, const ChunkSeg &g) {
-    const ChunkCuts cuts(line.total, line.phases * gridDim.x);
-    return {g.s.first, g.head, g.row0, g.rows, cuts.owner(g.u0 + (uint64_t)(g.tiles - 1) * g.w * BN), {}};
+    return {g.s.first, g.head, g.row0, g.rows, line.owner(g.u0 + (uint64_t)(g.tiles - 1) * g.w * BN), {}};
 }
 // Element index of row r (token * group + g) of a request's kv head in q and out.
 __device__ __forceinline__ size_t chunk_row(const ChunkParams &p, uint32_t first, uint32_t head, uint32_t r, uint32_t D) {
@@ -352,14 +340,11 @@ struct alignas(16) ChunkShared {
     uint32_t odd[2][8];
     Board board[kBoard];
     ChunkStarts starts;
-    union {
-        // [chain][half][row]: maxima on the way to the other half of the row, sums at a
-        // segment's end.  One buffer is enough: a thread writes the next tile's value
-        // only after that tile's S, which is computed only after both halves have
-        // released this tile's P, that is, read its values.
-        float row[2][2][128];
-        ChunkScan scan;
-    };
+    // [chain][half][row]: maxima on the way to the other half of the row, sums at a
+    // segment's end.  One buffer is enough: a thread writes the next tile's value only
+    // after that tile's S, which is computed only after both halves have released this
+    // tile's P, that is, read its values.
+    float row[2][2][128];
 };
 static_assert(sizeof(ChunkShared) <= 3 * 1024, "small arrays");
 
@@ -441,8 +426,9 @@ __device__ __noinline__ void add_nonfinite(const TreeParams &p, uint32_t seq, ui
 
 // A wait of the CTA gave up: NaN in the rows of all its segments (in the sums of
 // those that the merge joins).  `walk` as at the start.
-__device__ __noinline__ void chunk_give_up(const ChunkParams &p, const ChunkStarts *starts, ChunkLine line, uint32_t D) {
+__device__ __noinline__ void chunk_give_up(const ChunkParams &p, const ChunkStarts *starts, uint32_t D) {
     ChunkWalk walk;
+    const ChunkLine line = starts->line;
     walk.line = line;
     ChunkSeg g;
     const uint32_t R = 2 * p.rt;
@@ -516,8 +502,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_umma_kernel(const __grid_co
     }
     tc_fence_before();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const ChunkLine line = chunk_find(cp, D, &sh.scan, &sh.starts);
-    __syncthreads();  // the set-up above, the CTA's starts, and the scan's shared memory read
+    if (warp == 2) chunk_find(cp, D, &sh.starts);
+    __syncthreads();  // the set-up above
     tc_fence_after();
     const uint32_t tmem = *(volatile uint32_t *)&sh.tmem;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the merge may take its place; it waits for this grid
@@ -637,6 +623,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_umma_kernel(const __grid_co
                 ++segs;
             }
         } else {
+            const ChunkLine line = sh.starts.line;
             if (lane >= line.phases && lane < cp.most_phases) cp.cuts[lane * gridDim.x + blockIdx.x] = ChunkCut{};
             ChunkWalk walk;
             walk.line = line;
@@ -873,20 +860,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_umma_kernel(const __grid_co
                 const float2 c2 = make_float2(c, c);
                 float2 nm2, sum2[2];
                 uint32_t w[16];
-                // P = 2^(s c - m) of 32 scores as packed 16-bit pairs
+                // P = 2^(s c - m) of 32 scores as packed 16-bit pairs.  All on the SFU: a share
+                // of them on the FMA pipe (prefill.cu) costs 5% here, where two threads share
+                // a row and the SFU is busy half of the time.
                 auto weights = [&](int q) {
 #pragma unroll
                     for (int k = 0; k < 32; k += 2) {
                         float2 e = __ffma2_rn(make_float2(sv[q * 32 + k], sv[q * 32 + k + 1]), c2, nm2);
-                        if (((k >> 1) & 7) == 7) {  // an eighth on the FMA pipe
-                            e = exp2_poly_pair<true>(e);
-                        } else {
-                            e.x = fast_exp2(e.x);
-                            e.y = fast_exp2(e.y);
-                        }
+                        e.x = fast_exp2(e.x);
+                        e.y = fast_exp2(e.y);
                         sum2[(k >> 1) & 1] = __fadd2_rn(sum2[(k >> 1) & 1], e);
                         w[k >> 1] = pack2<kF16>(e.x, e.y);
-                        if (!kF16 && ((k >> 1) & 7) == 7) w[k >> 1] = drop_tiny(w[k >> 1]);
                     }
                 };
                 auto reference = [&]() {
@@ -904,8 +888,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_umma_kernel(const __grid_co
                     mx4[k] = fmaxf(a, sv[k + 60]);
                 }
                 const float mine = fmaxf(fmax3(mx4[0], mx4[1], mx4[2]), mx4[3]) * c;  // c > 0
+                // (also in a segment's first tile, which knows no maximum so far: a branch here
+                // would keep the two apart, 12% of the long chunk's time)
                 weights(0);
-                // the first that the row sees: m_run is -inf
                 if (pair_any(pair_bar, mine > m_run + kRescaleThreshold)) {
                     sh.row[x][h][r] = mine;
                     named_bar_sync(pair_bar, 64);
@@ -936,8 +921,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_umma_kernel(const __grid_co
                 // halves have written it
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    if (q > 0) weights(q);
                     tmem_st16(s_col + h * 32 + q * 16, w);
+                    if (q == 0) weights(1);  // while the first are stored
                     tmem_wait_st();
                     tc_fence_before();
                     __syncwarp();
@@ -1051,7 +1036,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_umma_kernel(const __grid_co
 
     tc_fence_before();
     __syncthreads();
-    if (*abort_flag) chunk_give_up(cp, &sh.starts, line, D);
+    if (*abort_flag) chunk_give_up(cp, &sh.starts, D);
     if (warp == 1) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM_COLS) : "memory");
