@@ -21,6 +21,7 @@ namespace {
 
 constexpr uint32_t kBook = 8;  // CTAs of the bookkeeping cluster
 constexpr int kThreads = 512;
+constexpr int kFreeThreads = 1024;
 
 // Block-wide exclusive sum; every thread gets the total.  sums: one per warp.
 __device__ __forceinline__ uint32_t block_before(uint32_t x, uint32_t *sums, uint32_t *total) {
@@ -203,57 +204,95 @@ __device__ __forceinline__ FreeOne free_one(const FreeParams &p, uint32_t i) {
     return r;
 }
 
-__global__ void __launch_bounds__(kThreads) page_free_kernel(const __grid_constant__ FreeParams p) {
-    __shared__ uint32_t sums[kThreads / 32], s_gone[kBook];
+// Independent loads of a loop's next kAtOnce elements, so that they are in flight
+// together (131,000 pages, 512 requests: 71 us with one at a time).
+constexpr uint32_t kAtOnce = 4;
+
+__global__ void __launch_bounds__(kFreeThreads) page_free_kernel(const __grid_constant__ FreeParams p) {
+    __shared__ uint32_t sums[kFreeThreads / 32], s_gone[kBook];
     cg::cluster_group cl = cg::this_cluster();
     const uint32_t rank = cl.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t me = rank * kThreads + threadIdx.x, all = kBook * kThreads;
+    const uint32_t me = rank * kFreeThreads + threadIdx.x, all = kBook * kFreeThreads;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t used = (uint32_t)min(max(*p.free_used, 0), (int32_t)p.n_free);
-    for (uint32_t i = me; i < p.n_pages; i += all) p.shared_out[i] = max(p.shared[i], 0);
+    auto copy = [&](const int32_t *from, int32_t *to, uint32_t first, uint32_t end, int32_t least) {
+        for (uint32_t i0 = first + me; i0 < end; i0 += all * kAtOnce) {
+            int32_t x[kAtOnce];
+#pragma unroll
+            for (uint32_t k = 0; k < kAtOnce; ++k)
+                if (i0 + k * all < end) x[k] = from[i0 + k * all];
+#pragma unroll
+            for (uint32_t k = 0; k < kAtOnce; ++k)
+                if (i0 + k * all < end) to[i0 + k * all] = max(x[k], least);
+        }
+    };
+    copy(p.shared, p.shared_out, 0, p.n_pages, 0);
     for (uint32_t i = me; i < p.n; i += all) {
         const FreeOne r = free_one(p, i);
         p.lens_out[i] = r.len;
         p.owned_out[i] = r.stay;
         p.status[i] = r.status;
     }
-    for (uint32_t i = used + me; i < p.n_free; i += all) p.free_out[i] = p.free_pages[i];
+    copy(p.free_pages, p.free_out, used, p.n_free, INT32_MIN);
     cl.sync();
-    for (uint32_t i = rank * (kThreads / 32) + warp; i < p.n; i += kBook * (kThreads / 32)) {
-        const FreeOne r = free_one(p, i);
-        const uint32_t drop = r.stay < r.owned ? (uint32_t)(r.owned - r.stay) : 0u;  // then owned is at most max_pages
-        for (uint32_t k = lane; k < drop; k += 32) {
-            const uint32_t page = (uint32_t)p.table[(size_t)i * p.max_pages + r.stay + k];
-            if (page < p.n_pages) atomicSub(&p.shared_out[page], 1);
+    for (uint32_t i = rank * (kFreeThreads / 32) + warp; i < p.n; i += kBook * (kFreeThreads / 32)) {
+        const int32_t stay = __ldcg(p.owned_out + i), owned = p.owned[i];
+        const uint32_t drop = stay < owned ? (uint32_t)(owned - stay) : 0u;  // then owned is at most max_pages
+        const int32_t *row = p.table + (size_t)i * p.max_pages + stay;
+        for (uint32_t k0 = lane; k0 < drop; k0 += 32 * kAtOnce) {
+            uint32_t page[kAtOnce];
+#pragma unroll
+            for (uint32_t k = 0; k < kAtOnce; ++k) page[k] = k0 + 32 * k < drop ? (uint32_t)row[k0 + 32 * k] : 0xffffffffu;
+#pragma unroll
+            for (uint32_t k = 0; k < kAtOnce; ++k)
+                if (page[k] < p.n_pages) atomicSub(&p.shared_out[page[k]], 1);
         }
     }
     cl.sync();
-    // a run of the list for each CTA: its gone pages counted, then both kinds placed
-    const uint32_t run = (used + kBook - 1) / kBook, a = min(rank * run, used), b = min(a + run, used);
-    auto gone = [&](uint32_t page) { return page < p.n_pages && __ldcg(&p.shared_out[page]) < 0; };
+    // a run of the taken part for each thread: its gone pages counted, then both kinds placed
+    const uint32_t run = (used + all - 1) / all, a = min(me * run, used), b = min(a + run, used);
     uint32_t mine = 0;
-    for (uint32_t i = a + threadIdx.x; i < b; i += kThreads) mine += gone((uint32_t)p.free_pages[i]);
-    mine = block_sum(mine, sums);
-    cluster_gather(cl, mine, s_gone);
-    uint32_t before = 0, total = 0;
+    int32_t page[kAtOnce];
+    bool gone[kAtOnce];
+    auto look = [&](uint32_t i0) {
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k) page[k] = i0 + k < b ? p.free_pages[i0 + k] : -1;
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k) gone[k] = (uint32_t)page[k] < p.n_pages && __ldcg(&p.shared_out[page[k]]) < 0;
+    };
+    for (uint32_t i0 = a; i0 < b; i0 += kAtOnce) {
+        look(i0);
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k) mine += i0 + k < b && gone[k];
+    }
+    uint32_t cta;
+    uint32_t before = block_before(mine, sums, &cta);
+    cluster_gather(cl, cta, s_gone);
+    uint32_t total = 0;
     for (uint32_t r = 0; r < kBook; ++r) {
         if (r < rank) before += s_gone[r];
         total += s_gone[r];
     }
     const uint32_t left = used - total;
     if (me == 0) *p.free_used_out = (int32_t)left;
-    for (uint32_t i0 = a; i0 < b; i0 += kThreads) {
-        const uint32_t i = i0 + threadIdx.x;
-        const int32_t page = i < b ? p.free_pages[i] : -1;
-        const bool g = i < b && gone((uint32_t)page);
-        uint32_t some;
-        const uint32_t at = before + block_before(g, sums, &some);  // gone pages ahead of i
-        if (i < b) p.free_out[g ? left + at : i - at] = page;
-        before += some;
+    for (uint32_t i0 = a; i0 < b; i0 += kAtOnce) {
+        if (run > kAtOnce) look(i0);  // else as it is
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k)
+            if (i0 + k < b) {
+                p.free_out[gone[k] ? left + before : i0 + k - before] = page[k];
+                before += gone[k];
+            }
     }
     cl.sync();  // every flag has been read
-    for (uint32_t i = me; i < p.n_pages; i += all)
-        if (__ldcg(&p.shared_out[i]) < 0) p.shared_out[i] = 0;
+    for (uint32_t i0 = me; i0 < p.n_pages; i0 += all * kAtOnce) {
+        int32_t x[kAtOnce];
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k) x[k] = i0 + k * all < p.n_pages ? __ldcg(&p.shared_out[i0 + k * all]) : 0;
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k)
+            if (x[k] < 0) p.shared_out[i0 + k * all] = 0;
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -385,7 +424,7 @@ cudaError_t launch_page_fork(const ForkParams &p, cudaStream_t st) {
 }
 
 cudaError_t launch_page_free(const FreeParams &p, cudaStream_t st) {
-    return launch_clusters(page_free_kernel, kBook, dim3(kBook), kThreads, 0, st, p);
+    return launch_clusters(page_free_kernel, kBook, dim3(kBook), kFreeThreads, 0, st, p);
 }
 
 cudaError_t launch_page_compact(const CompactParams &p, cudaStream_t st) {

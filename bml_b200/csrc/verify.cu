@@ -34,10 +34,11 @@ namespace bml {
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr uint32_t kWarps = kThreads / 32;
 constexpr uint32_t kNodes = kTreeMaxNodes;
 constexpr uint32_t kMostCluster = 8;
+static_assert(kMostCluster * kWarps <= 64, "two pieces a lane");
 
 struct VerifyShared {
     int32_t token[kNodes];
@@ -45,7 +46,7 @@ struct VerifyShared {
     uint32_t below[kNodes][kNodes / 32];  // children of a node, by node
     double part[2][kMostCluster];         // pass parity: the CTAs' sums
     double warp[kWarps];
-    double all[kMostCluster * kWarps];    // the last pass: every warp's sum
+    double all[kMostCluster * kWarps], all_q[kMostCluster * kWarps];  // the last pass: every warp's sum
     uint32_t out[kNodes];                 // tokens that are taken out of p
 };
 
@@ -56,27 +57,43 @@ __device__ __forceinline__ float prob(T x) {
     return f > 0.f && f < INFINITY ? f : 0.f;
 }
 
+// f64 of a number from 0 to below 2, by integer operations: the exponent's bias grows
+// by 1023 - 127.  0 becomes 2^-127, and a subnormal f32 something below 2^-126; both
+// are nothing beside a row's sum.
+__device__ __forceinline__ double widen(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return __hiloint2double((int)((b >> 3) + 0x38000000u), (int)(b << 29));
+}
+
 template <typename T>
-struct Vec {
+struct alignas(16) Vec {
     static constexpr int N = 16 / sizeof(T);
     T v[N];
 };
 
 // The N values of a row from element e0 on (from a 16-byte boundary where `whole`),
-// zeros outside [0, vocab).
+// zeros outside [0, vocab), as they are stored: fewer registers than widened.
 template <typename T>
-__device__ __forceinline__ void load_vec(const T *row, int64_t e0, uint32_t vocab, bool aligned, float (&x)[Vec<T>::N]) {
+__device__ __forceinline__ Vec<T> load_vec(const T *row, int64_t e0, uint32_t vocab, bool whole) {
     constexpr int N = Vec<T>::N;
-    if (aligned && e0 >= 0 && e0 + N <= (int64_t)vocab) {
+    Vec<T> x;
+    if (whole && e0 >= 0 && e0 + N <= (int64_t)vocab) {
         const uint4 z = __ldg(reinterpret_cast<const uint4 *>(row + e0));
-        const T *t = reinterpret_cast<const T *>(&z);
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = prob(t[i]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = e0 + i >= 0 && e0 + i < (int64_t)vocab ? prob(row[e0 + i]) : 0.f;
+        return *reinterpret_cast<const Vec<T> *>(&z);
     }
+#pragma unroll
+    for (int i = 0; i < N; ++i) x.v[i] = e0 + i >= 0 && e0 + i < (int64_t)vocab ? row[e0 + i] : T(0.f);
+    return x;
 }
+// All its bits in one word; with a bit of kOdd set, some value is negative, 2 or more,
+// infinite or NaN.
+template <typename T>
+__device__ __forceinline__ uint32_t bits(const Vec<T> &x) {
+    const uint4 z = *reinterpret_cast<const uint4 *>(&x);
+    return z.x | z.y | z.z | z.w;
+}
+template <typename T>
+constexpr uint32_t kOdd = sizeof(T) == 4 ? 0xc0000000u : 0xc000c000u;
 
 // What a row pass sums: max(p - c q, 0), or p without some tokens.
 template <typename T, bool kDraft>
@@ -96,18 +113,24 @@ struct Row {
         q_ok = kDraft && ((reinterpret_cast<uintptr_t>(pr) ^ reinterpret_cast<uintptr_t>(qr)) & 15u) == 0;
     }
     __device__ __forceinline__ uint32_t vecs() const { return (vocab + shift + N - 1) / N; }
-    // vector k's weights
-    __device__ __forceinline__ void load(uint32_t k, float (&x)[N], float (&y)[N]) const {
-        const int64_t e0 = (int64_t)k * N - shift;
-        load_vec<T>(p, e0, vocab, true, x);
-        if (kDraft) load_vec<T>(q, e0, vocab, q_ok, y);
-    }
-    __device__ __forceinline__ void weigh(uint32_t k, const float (&x)[N], const float (&y)[N], double (&w)[N]) const {
+    __device__ __forceinline__ int64_t first(uint32_t k) const { return (int64_t)k * N - shift; }
+    // vector k's weights, whatever the values are
+    __device__ __forceinline__ void weigh(uint32_t k, double (&w)[N]) const {
+        const Vec<T> x = load_vec<T>(p, first(k), vocab, true);
 #pragma unroll
-        for (int i = 0; i < N; ++i) w[i] = kDraft ? fmax((double)x[i] - c * (double)y[i], 0.0) : (double)x[i];
+        for (int i = 0; i < N; ++i) w[i] = (double)prob(x.v[i]);
+        if (kDraft && c != 0.0) {
+            const Vec<T> y = load_vec<T>(q, first(k), vocab, q_ok);
+#pragma unroll
+            for (int i = 0; i < N; ++i) w[i] = fmax(w[i] - c * (double)prob(y.v[i]), 0.0);
+        }
+        drop(k, w);
+    }
+    // zeros for the tokens that are taken out
+    __device__ __forceinline__ void drop(uint32_t k, double (&w)[N]) const {
         if (!kDraft)
             for (uint32_t o = 0; o < n_out; ++o) {
-                const int64_t i = (int64_t)out[o] - ((int64_t)k * N - shift);
+                const int64_t i = (int64_t)out[o] - first(k);
 #pragma unroll
                 for (int j = 0; j < N; ++j)
                     if (i == j) w[j] = 0.0;
@@ -115,30 +138,77 @@ struct Row {
     }
 };
 
-// Sum of vectors [k0, k1) by a warp; every lane gets it.
+__device__ __forceinline__ double warp_sum(double t) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    return t;
+}
+
+// Sum of vectors [k0, k1) by a warp, value by value.
+template <typename T, bool kDraft>
+__device__ __noinline__ double slow_pass(const Row<T, kDraft> &r, uint32_t k0, uint32_t k1) {
+    double s = 0.0;
+    for (uint32_t k = k0 + (threadIdx.x & 31); k < k1; k += 32) {
+        double w[Row<T, kDraft>::N];
+        r.weigh(k, w);
+#pragma unroll
+        for (int i = 0; i < Row<T, kDraft>::N; ++i) s += w[i];
+    }
+    return warp_sum(s);
+}
+
+// Sum of vectors [k0, k1) by a warp; every lane gets it.  Instructions bound this (48
+// requests, 128,000 f32: 30 an element, with every value looked at, made a pass 8 us,
+// these 11 make it 3): the values are probabilities, so one OR of their bits says for
+// many at once that none is negative, infinite or NaN; else all is summed again value
+// by value.  q is widened by integer operations beside the conversion unit, which
+// takes p.
 template <typename T, bool kDraft>
 __device__ __forceinline__ double warp_pass(const Row<T, kDraft> &r, uint32_t k0, uint32_t k1) {
     constexpr int N = Vec<T>::N, kAtOnce = 4;
     const uint32_t lane = threadIdx.x & 31;
     double s[2] = {0.0, 0.0};
-    for (uint32_t k = k0 + lane; k < k1; k += 32 * kAtOnce) {
-        float x[kAtOnce][N], y[kAtOnce][N];
+    uint32_t all = 0;
+    if (kDraft && r.c != 0.0) {
+        if (!r.q_ok) return slow_pass(r, k0, k1);
+        for (uint32_t k = k0 + lane; k < k1; k += 32 * kAtOnce) {
+            Vec<T> x[kAtOnce], y[kAtOnce];
 #pragma unroll
-        for (int a = 0; a < kAtOnce; ++a)
-            if (k + a * 32 < k1) r.load(k + a * 32, x[a], y[a]);
+            for (int a = 0; a < kAtOnce; ++a) {
+                const bool in = k + a * 32 < k1;  // else zeros
+                x[a] = load_vec<T>(r.p, r.first(k + a * 32), in ? r.vocab : 0u, true);
+                y[a] = load_vec<T>(r.q, r.first(k + a * 32), in ? r.vocab : 0u, true);
+            }
 #pragma unroll
-        for (int a = 0; a < kAtOnce; ++a)
-            if (k + a * 32 < k1) {
+            for (int a = 0; a < kAtOnce; ++a) {
+                all |= bits(x[a]) | bits(y[a]);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const double d = fma(-r.c, widen((float)y[a].v[i]), (double)(float)x[a].v[i]);
+                    const int hi = __double2hiint(d), keep = ~(hi >> 31);  // 0 where d is negative
+                    s[i & 1] += __hiloint2double(hi & keep, __double2loint(d) & keep);
+                }
+            }
+        }
+    } else {
+        for (uint32_t k = k0 + lane; k < k1; k += 32 * kAtOnce) {
+            Vec<T> x[kAtOnce];
+#pragma unroll
+            for (int a = 0; a < kAtOnce; ++a) x[a] = load_vec<T>(r.p, r.first(k + a * 32), k + a * 32 < k1 ? r.vocab : 0u, true);
+#pragma unroll
+            for (int a = 0; a < kAtOnce; ++a) {
+                all |= bits(x[a]);
                 double w[N];
-                r.weigh(k + a * 32, x[a], y[a], w);
+#pragma unroll
+                for (int i = 0; i < N; ++i) w[i] = (double)(float)x[a].v[i];
+                r.drop(k + a * 32, w);
 #pragma unroll
                 for (int i = 0; i < N; ++i) s[i & 1] += w[i];
             }
+        }
     }
-    double t = s[0] + s[1];
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    return t;
+    if (__any_sync(0xffffffffu, all & kOdd<T>)) return slow_pass(r, k0, k1);
+    return warp_sum(s[0] + s[1]);
 }
 
 // The first element of vectors [k0, k1) whose prefix sum, from `base` on, is above
@@ -150,14 +220,10 @@ __device__ __noinline__ int32_t warp_find(const Row<T, kDraft> &r, uint32_t k0, 
     int32_t last = -1;
     for (uint32_t kb = k0; kb < k1; kb += 32) {
         const uint32_t k = kb + lane;
-        float x[N], y[N];
         double w[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) w[i] = 0.0;
-        if (k < k1) {
-            r.load(k, x, y);
-            r.weigh(k, x, y, w);
-        }
+        if (k < k1) r.weigh(k, w);
         double sum = 0.0;
 #pragma unroll
         for (int i = 0; i < N; ++i) sum += w[i];
@@ -172,7 +238,7 @@ __device__ __noinline__ int32_t warp_find(const Row<T, kDraft> &r, uint32_t k0, 
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             at += w[i];
-            const int32_t e = (int32_t)((int64_t)k * N - r.shift + i);
+            const int32_t e = (int32_t)(r.first(k) + i);
             if (w[i] > 0.0) {
                 seen = e;
                 if (hit < 0 && at > tau) hit = e;
@@ -187,7 +253,7 @@ __device__ __noinline__ int32_t warp_find(const Row<T, kDraft> &r, uint32_t k0, 
 }
 
 template <typename T, bool kDraft>
-__global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant__ VerifyParams p) {
+__global__ void __launch_bounds__(kThreads, 3) verify_kernel(const __grid_constant__ VerifyParams p) {
     __shared__ VerifyShared sh;
     cg::cluster_group cl = cg::this_cluster();
     const uint32_t C = cl.num_blocks(), rank = cl.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -224,16 +290,19 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
     row.n_out = 0;
     const uint32_t slice = C * kWarps, me = rank * kWarps + warp;
     uint32_t passes = 0, kept = 0, t = 0;
-    auto bounds = [&](uint32_t n, uint32_t &k0, uint32_t &k1) {  // of the warp's piece of n vectors
+    uint32_t k0 = 0, k1 = 0;  // the warp's piece of the row
+    auto piece_of = [&](uint32_t n) {  // of n vectors
         const uint32_t each = (n + slice - 1) / slice;
         k0 = min(me * each, n);
         k1 = min(k0 + each, n);
     };
-    // sum of a row over all CTAs, the same in each
-    auto total = [&](const auto &r) {
-        uint32_t k0, k1;
-        bounds(r.vecs(), k0, k1);
-        const double w = warp_pass(r, k0, k1);
+    auto go = [&](uint32_t node) {
+        row.at(target + (size_t)(a + node) * p.vocab, kDraft ? draft + (size_t)(a + node) * p.vocab : nullptr);
+        piece_of(row.vecs());
+    };
+    // sum of the row over all CTAs, the same in each
+    auto total = [&]() {
+        const double w = warp_pass(row, k0, k1);
         if (lane == 0) sh.warp[warp] = w;
         __syncthreads();
         if (threadIdx.x < C) {
@@ -255,7 +324,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
             row.c = 0.0;
             row.n_out = 0;
             if (kept == p.max_path) break;  // its children are not looked at
-            row.at(target + (size_t)(a + t) * p.vocab, kDraft ? draft + (size_t)(a + t) * p.vocab : nullptr);
+            go(t);
             double mass = 1.0;
             bool known = true;  // mass is that of the residual
             uint32_t next = 0;
@@ -265,7 +334,7 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
                     const double u = sh.u[j], pv = sh.pv[j], qv = sh.qv[j];
                     double r = pv;
                     if (kDraft) {
-                        if (!known) mass = total(row);
+                        if (!known) mass = total();
                         known = true;
                         r = fmax(pv - row.c * qv, 0.0);
                     } else {
@@ -299,57 +368,55 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
 
     // the token behind node t, from the residual
     if (kept) {
-        row.at(target + (size_t)(a + t) * p.vocab, kDraft ? draft + (size_t)(a + t) * p.vocab : nullptr);
+        go(t);
         for (int again = 0; again < 2; ++again) {
-            uint32_t k0, k1;
-            bounds(row.vecs(), k0, k1);
+            double q_sum = 0.0;
             const double w = warp_pass(row, k0, k1);
-            if (lane < C) *cl.map_shared_rank(&sh.all[me], lane) = w;
-            cl.sync();
-            double before = 0.0, sum = 0.0;
-            for (uint32_t x = 0; x < slice; ++x) {
-                if (x == me) before = sum;
-                sum += sh.all[x];
+            if (kDraft && again) {  // q on its own: it may lie on another place of 16 bytes
+                Row<T, kDraft> q_row = row;
+                q_row.at(row.q, row.q);
+                piece_of(q_row.vecs());
+                q_sum = warp_pass(q_row, k0, k1);
+                piece_of(row.vecs());
             }
-            if (sum > 0.0) {
-                const double tau = (double)p.u_next[i] * sum;
+            if (lane < C) {
+                *cl.map_shared_rank(&sh.all[me], lane) = w;
+                if (again) *cl.map_shared_rank(&sh.all_q[me], lane) = q_sum;
+            }
+            cl.sync();
+            // prefix sums of the pieces, two a lane, by every warp
+            const double y0 = 2 * lane < slice ? sh.all[2 * lane] : 0.0, y1 = 2 * lane + 1 < slice ? sh.all[2 * lane + 1] : 0.0;
+            double inc = y0 + y1;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double v = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= (uint32_t)o) inc += v;
+            }
+            const double sum = __shfl_sync(0xffffffffu, inc, 31), begin = inc - (y0 + y1);
+            bool drawn = sum > 0.0;
+            if (kDraft && again) {
+                q_sum = 0.0;
+                for (uint32_t x = 0; x < slice; ++x) q_sum += sh.all_q[x];
+                drawn = drawn && q_sum <= 2.0 * sum;
+            }
+            if (drawn) {
                 // the first piece that ends above tau, or the last one with a weight
-                uint32_t piece = 0, heavy = 0;
-                double run = 0.0;
-                bool found = false;
-                for (uint32_t x = 0; x < slice; ++x) {
-                    const double y = sh.all[x];
-                    run += y;
-                    if (y > 0.0) heavy = x;
-                    if (!found && y > 0.0 && run > tau) {
-                        found = true;
-                        piece = x;
-                    }
-                }
-                if (!found) piece = heavy;
+                const double tau = (double)p.u_next[i] * sum;
+                const bool in0 = y0 > 0.0 && begin + y0 > tau, in1 = y1 > 0.0 && inc > tau;
+                const uint32_t hits = __ballot_sync(0xffffffffu, in0 || in1), some = __ballot_sync(0xffffffffu, y0 > 0.0 || y1 > 0.0);
+                const uint32_t who = hits ? __ffs(hits) - 1 : 31 - __clz(some);
+                const uint32_t piece = __shfl_sync(0xffffffffu, 2 * lane + (hits ? !in0 : y1 > 0.0), who);
+                const double before = __shfl_sync(0xffffffffu, hits ? (in0 ? begin : begin + y0) : (y1 > 0.0 ? begin + y0 : begin), who);
                 if (piece == me) {
                     const int32_t token = warp_find(row, k0, k1, before, tau);
                     if (lane == 0) p.next[i] = token;
                 }
                 break;
             }
+            // Nothing is left of the residual: by rounding, and the token is p's, unless q
+            // sums to more than twice p (no distribution) or p itself has nothing.
+            if (again && writes) p.next[i] = (int32_t)p.vocab - 1;
             cl.sync();  // sh.all has been read
-            // nothing is left: by rounding, unless q sums to more than twice p (no
-            // distribution) or p itself has nothing
-            bool drawn = !again;
-            if (kDraft && drawn) {
-                Row<T, false> one;
-                one.vocab = p.vocab;
-                one.n_out = 0;
-                one.at(row.q, nullptr);
-                const double sq = total(one);
-                one.at(row.p, nullptr);
-                drawn = sq <= 2.0 * total(one);
-            }
-            if (!drawn) {
-                if (writes) p.next[i] = (int32_t)p.vocab - 1;
-                break;
-            }
             row.c = 0.0;
             row.n_out = 0;
         }
@@ -361,10 +428,9 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const __grid_constant_
 
 template <typename T>
 cudaError_t verify_t(const VerifyParams &p, cudaStream_t st) {
-    // as many CTAs a request as leave two for each SM (a CTA's row pass is bound by
-    // what one SM can read)
+    // as many CTAs a request as all fit the SMs at once, three on each
     uint32_t cluster = kMostCluster;
-    while (cluster > 1 && (uint64_t)p.n * cluster > 2ull * p.num_sms) cluster /= 2;
+    while (cluster > 1 && (uint64_t)p.n * cluster > 3ull * p.num_sms) cluster /= 2;
     auto kern = p.draft ? verify_kernel<T, true> : verify_kernel<T, false>;
     return launch_clusters(kern, cluster, dim3(p.n * cluster), kThreads, 0, st, p);
 }

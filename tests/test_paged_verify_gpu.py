@@ -237,6 +237,27 @@ def test_unaligned_rows(cuda):
             assert [x.tolist() for x in got] == want
 
 
+def test_unaligned_rows_with_nothing_left(cuda):
+    """q is summed where it lies: draft rows on another boundary than the target's, a
+    residual that is empty, and values that are looked at one by one."""
+    import bml_b200
+    for dt in DT:
+        for bump in (0.0, 0.5, float("nan"), float("inf"), -1.0, 7.0):
+            b = batch([4, 5], 1003, dt, True, 13)
+            b["q"][:4] = b["p"][:4].float() + bump if bump == bump and bump >= 0 and bump != float("inf") else b["p"][:4].float()
+            if bump != bump or bump in (float("inf"), -1.0):
+                b["q"][:, 5::7] = bump
+                b["p"][:, 6::9] = bump
+            b["u"][:] = 1.0
+            want = check(b)
+            for a, c in ((1, 0), (0, 3), (2, 5), (4, 4)):
+                p, q = (torch.empty(9 * 1003 + 8, dtype=DT[dt], device="cuda")[k:k + 9 * 1003].view(9, 1003) for k in (a, c))
+                p.copy_(b["p"])
+                q.copy_(b["q"])
+                got = bml_b200.verify_drafts(p, q, ints(b["tokens"]), ints(b["parents"]), ints([0, 4, 9]), b["u"].cuda(), b["un"].cuda())
+                assert tuple(x.tolist() for x in got) == tuple(want)
+
+
 def test_first_token_is_distributed_as_the_target(cuda):
     """The first token behind the pending one -- a kept draft or the drawn one --
     over 200,000 requests with the same rows: each count is binomial, so within
