@@ -117,7 +117,7 @@ SIGNATURES = {
     "bml_page_fork": (_st, [_vp, _vp, _u32, _u32, _u32, _u32, _u32, C.c_int, _vp, _vp, _u32, _vp, _vp, _u32, _vp, _u32, _vp,
                             _vp, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "bml_page_free": (_st, [_vp, _vp, _vp, _u32, _vp, _u32, _u32, _vp, _u32, _vp, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
-                            _vp]),
+                            _vp, _sz, _vp]),
     "bml_page_compact": (_st, [_vp, _vp, _u32, _u32, _u32, _u32, _u32, C.c_int, _vp, _u32, _vp, _u32, _vp, _vp, _vp, _vp,
                                _vp, _vp, _sz, _vp]),
     "bml_softmax_f32": (_st, [_vp, _u32, _u32, _vp, _vp]),

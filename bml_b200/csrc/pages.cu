@@ -22,6 +22,7 @@ namespace {
 constexpr uint32_t kBook = 8;  // CTAs of the bookkeeping cluster
 constexpr int kThreads = 512;
 constexpr int kFreeThreads = 1024;
+constexpr uint32_t kWidePages = 16384;
 
 // Block-wide exclusive sum; every thread gets the total.  sums: one per warp.
 __device__ __forceinline__ uint32_t block_before(uint32_t x, uint32_t *sums, uint32_t *total) {
@@ -295,6 +296,89 @@ __global__ void __launch_bounds__(kFreeThreads) page_free_kernel(const __grid_co
     }
 }
 
+// The same over all SMs for long lists: a launch a step in place of a cluster barrier.
+// work: the gone pages of each tile of the taken part, then a bit for each entry, so
+// that the last step need not look a page up while another CTA clears it.
+constexpr int kWideThreads = 256;
+struct FreeTile {
+    uint32_t a, b, used;
+    __device__ __forceinline__ explicit FreeTile(const FreeParams &p) {
+        used = (uint32_t)min(max(*p.free_used, 0), (int32_t)p.n_free);
+        a = (uint32_t)min((uint64_t)blockIdx.x * p.tile, (uint64_t)used);
+        b = (uint32_t)min((uint64_t)a + p.tile, (uint64_t)used);
+    }
+};
+
+__global__ void __launch_bounds__(kWideThreads) free_start_kernel(const __grid_constant__ FreeParams p) {
+    const uint32_t me = blockIdx.x * kWideThreads + threadIdx.x, all = gridDim.x * kWideThreads;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t used = (uint32_t)min(max(*p.free_used, 0), (int32_t)p.n_free);
+    for (uint32_t i = me; i < p.n_pages; i += all) p.shared_out[i] = max(p.shared[i], 0);
+    for (uint64_t i = (uint64_t)used + me; i < p.n_free; i += all) p.free_out[i] = p.free_pages[i];
+    for (uint32_t i = me; i < p.n; i += all) {
+        const FreeOne r = free_one(p, i);
+        p.lens_out[i] = r.len;
+        p.owned_out[i] = r.stay;
+        p.status[i] = r.status;
+    }
+}
+
+__global__ void __launch_bounds__(kWideThreads) free_release_kernel(const __grid_constant__ FreeParams p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const uint32_t i = blockIdx.x;
+    const int32_t stay = p.owned_out[i], owned = p.owned[i];
+    const uint32_t drop = stay < owned ? (uint32_t)(owned - stay) : 0u;  // then owned is at most max_pages
+    const int32_t *row = p.table + (size_t)i * p.max_pages + stay;
+    for (uint32_t k = threadIdx.x; k < drop; k += kWideThreads) {
+        const uint32_t page = (uint32_t)row[k];
+        if (page < p.n_pages) atomicSub(&p.shared_out[page], 1);
+    }
+}
+
+__global__ void __launch_bounds__(kWideThreads) free_count_kernel(const __grid_constant__ FreeParams p) {
+    __shared__ uint32_t sums[kWideThreads / 32];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const FreeTile t(p);
+    uint32_t mine = 0;
+    for (uint32_t i0 = t.a; i0 < t.b; i0 += kWideThreads) {
+        const uint32_t i = i0 + threadIdx.x, page = i < t.b ? (uint32_t)p.free_pages[i] : 0xffffffffu;
+        const uint32_t word = __ballot_sync(0xffffffffu, page < p.n_pages && p.shared_out[page] < 0);
+        if ((threadIdx.x & 31) == 0 && i < t.b) {
+            p.work[kFreeTiles + i / 32] = word;
+            mine += __popc(word);
+        }
+    }
+    mine = block_sum(mine, sums);
+    if (threadIdx.x == 0) p.work[blockIdx.x] = mine;
+}
+
+__global__ void __launch_bounds__(kWideThreads) free_place_kernel(const __grid_constant__ FreeParams p) {
+    __shared__ uint32_t sums[kWideThreads / 32];
+    const uint32_t lane = threadIdx.x & 31, me = blockIdx.x * kWideThreads + threadIdx.x, all = gridDim.x * kWideThreads;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const FreeTile t(p);
+    uint32_t before = 0, total = 0;
+    for (uint32_t i = threadIdx.x; i < gridDim.x; i += kWideThreads) {
+        const uint32_t x = p.work[i];
+        total += x;
+        if (i < blockIdx.x) before += x;
+    }
+    total = block_sum(total, sums);
+    before = block_sum(before, sums);
+    const uint32_t left = t.used - total;
+    if (me == 0) *p.free_used_out = (int32_t)left;
+    for (uint32_t i0 = t.a; i0 < t.b; i0 += kWideThreads) {
+        const uint32_t i = i0 + threadIdx.x, word = i < t.b ? p.work[kFreeTiles + i / 32] : 0u;
+        uint32_t some;
+        const uint32_t warps = block_before(lane == 0 ? __popc(word) : 0u, sums, &some);  // lane 0: of the warps before
+        const uint32_t at = before + __shfl_sync(0xffffffffu, warps, 0) + __popc(word & ((1u << lane) - 1));
+        if (i < t.b) p.free_out[(word >> lane & 1u) ? left + at : i - at] = p.free_pages[i];
+        before += some;
+    }
+    for (uint32_t i = me; i < p.n_pages; i += all)
+        if (p.shared_out[i] < 0) p.shared_out[i] = 0;
+}
+
 // ---------------------------------------------------------------------------
 // page_compact
 //
@@ -404,6 +488,72 @@ __global__ void __launch_bounds__(kThreads) page_move_kernel(const __grid_consta
     }
 }
 
+// Both in one launch for a small pool: every CTA finds all the moves, from bits in
+// shared memory, and makes its share of them.
+constexpr uint32_t kSmallPages = 8192, kSmallEntries = 16384;
+
+template <typename U>
+__global__ void __launch_bounds__(kThreads) page_compact_kernel(const __grid_constant__ CompactParams p, uint32_t piece) {
+    constexpr uint32_t kWords = kSmallPages / 32, kAtOnce = 8;
+    static_assert(kWords <= kThreads, "a word a thread");
+    __shared__ uint32_t held_bits[kWords], before[kWords], sums[kThreads / 32];
+    __shared__ uint16_t from[kSmallPages / 2], to[kSmallPages / 2];  // as many movers as holes below them
+    const uint32_t n = p.pool.n_pages, tid = threadIdx.x, me = blockIdx.x * kThreads + tid, all = gridDim.x * kThreads;
+    const uint32_t entries = p.n * p.max_pages;
+    if (tid < kWords) held_bits[tid] = 0;
+    __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    auto held_entry = [&](uint32_t e) { return (int32_t)(e % p.max_pages) < p.owned[e / p.max_pages]; };
+    for (uint32_t e0 = tid; e0 < entries; e0 += kThreads * kAtOnce) {
+        uint32_t page[kAtOnce];
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k) {
+            const uint32_t e = e0 + k * kThreads;
+            page[k] = e < entries && held_entry(e) ? (uint32_t)p.table[e] : 0xffffffffu;
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k)
+            if (page[k] < n) atomicOr(&held_bits[page[k] >> 5], 1u << (page[k] & 31));
+    }
+    __syncthreads();
+    const uint32_t word = tid < kWords ? held_bits[tid] : 0u;
+    uint32_t held;
+    const uint32_t first = block_before(__popc(word), sums, &held);  // held pages before this word
+    if (tid < kWords) before[tid] = first;
+    __syncthreads();
+    // pages below i that are held
+    auto rank = [&](uint32_t i) { return before[i >> 5] + __popc(held_bits[i >> 5] & ((1u << (i & 31)) - 1)); };
+    const uint32_t stay = held < n ? rank(held) : held;  // held pages below H; H is n only if all are
+    const uint32_t moves = held - stay;
+    for (uint32_t i = tid; i < n; i += kThreads) {
+        const bool h = held_bits[i >> 5] >> (i & 31) & 1u;
+        if (h && i >= held) from[rank(i) - stay] = (uint16_t)i;
+        if (!h && i < held) to[i - rank(i)] = (uint16_t)i;
+    }
+    __syncthreads();
+
+    for (uint32_t e = me; e < entries; e += all) {
+        const int32_t page = p.table[e];
+        int32_t place = page;
+        if ((uint32_t)page < n && (uint32_t)page >= held && held_entry(e)) place = to[rank((uint32_t)page) - stay];
+        p.table_out[e] = place;
+    }
+    for (uint32_t i = me; i < n; i += all) {
+        p.free_out[i] = (int32_t)i;
+        if (held_bits[i >> 5] >> (i & 31) & 1u) p.shared_out[i < held ? i : to[rank(i) - stay]] = p.shared[i];
+        if (i >= held) p.shared_out[i] = 0;
+    }
+    if (me == 0) *p.free_used_out = (int32_t)held;
+    const uint64_t page_bytes = (uint64_t)p.pool.row_bytes << p.pool.page_shift;
+    const uint64_t pieces = (page_bytes + piece - 1) / piece, per = pieces * 2 * p.pool.n_layers, items = per * moves;
+    for (uint64_t it = blockIdx.x; it < items; it += gridDim.x) {
+        const uint64_t m = it / per, lw = (it - m * per) / pieces, off = (it - m * per - lw * pieces) * piece;
+        char *base = ((lw & 1) ? p.pool.v_pool : p.pool.k_pool) + (lw >> 1) * p.pool.layer_bytes + off;
+        const uint64_t left = page_bytes - off;
+        copy_cta<U>(base + to[m] * page_bytes, base + from[m] * page_bytes, (uint32_t)(left < piece ? left : piece));
+    }
+}
+
 bool wide(const PoolParams &p) {
     return p.row_bytes % 16 == 0 && ((reinterpret_cast<uintptr_t>(p.k_pool) | reinterpret_cast<uintptr_t>(p.v_pool)) & 15u) == 0;
 }
@@ -424,15 +574,27 @@ cudaError_t launch_page_fork(const ForkParams &p, cudaStream_t st) {
 }
 
 cudaError_t launch_page_free(const FreeParams &p, cudaStream_t st) {
-    return launch_clusters(page_free_kernel, kBook, dim3(kBook), kFreeThreads, 0, st, p);
+    if (p.n_pages < kWidePages && p.n_free < kWidePages)
+        return launch_clusters(page_free_kernel, kBook, dim3(kBook), kFreeThreads, 0, st, p);
+    FreeParams q = p;
+    q.tile = (p.n_free + kFreeTiles - 1) / kFreeTiles;  // in whole words of the bits
+    q.tile = q.tile < kWideThreads ? kWideThreads : (q.tile + 31) / 32 * 32;
+    const uint32_t tiles = (p.n_free + q.tile - 1) / q.tile, grid = tiles < kFreeTiles / 4 ? kFreeTiles / 4 : tiles;
+    cudaError_t e = launch_after(free_start_kernel, dim3((uint32_t)p.num_sms * 2), kWideThreads, 0, st, q);
+    if (e == cudaSuccess) e = launch_after(free_release_kernel, dim3(p.n), kWideThreads, 0, st, q);
+    if (e == cudaSuccess) e = launch_after(free_count_kernel, dim3(grid), kWideThreads, 0, st, q);
+    if (e == cudaSuccess) e = launch_after(free_place_kernel, dim3(grid), kWideThreads, 0, st, q);
+    return e;
 }
 
 cudaError_t launch_page_compact(const CompactParams &p, cudaStream_t st) {
-    const cudaError_t e = launch_clusters(page_moves_kernel, kBook, dim3(kBook), kThreads, 0, st, p);
-    if (e != cudaSuccess) return e;
     // pieces of a page that a CTA copies in one round: eight units a thread
     const bool w = wide(p.pool);
     const uint32_t piece = kThreads * 8 * (w ? 16 : 2);
+    if (p.pool.n_pages <= kSmallPages && (uint64_t)p.n * p.max_pages <= kSmallEntries)
+        return launch_after(w ? page_compact_kernel<uint4> : page_compact_kernel<uint16_t>, dim3((uint32_t)p.num_sms * 4), kThreads, 0, st, p, piece);
+    const cudaError_t e = launch_clusters(page_moves_kernel, kBook, dim3(kBook), kThreads, 0, st, p);
+    if (e != cudaSuccess) return e;
     return launch_after(w ? page_move_kernel<uint4> : page_move_kernel<uint16_t>, dim3((uint32_t)p.num_sms * 4), kThreads, 0, st, p, piece);
 }
 

@@ -60,7 +60,12 @@ struct FreeParams {
     uint32_t n_free;
     const int32_t *free_used;
     int32_t *lens_out, *owned_out, *shared_out, *free_out, *free_used_out, *status;
+    uint32_t *work;  // free_work_bytes(n_free)
+    uint32_t tile;   // entries of the free list a CTA, set by the launch
+    int num_sms;
 };
+constexpr uint32_t kFreeTiles = 1024;  // at most
+constexpr uint64_t free_work_bytes(uint32_t n_free) { return 4ull * (kFreeTiles + (n_free + 31ull) / 32); }
 cudaError_t launch_page_free(const FreeParams &p, cudaStream_t st);
 
 struct CompactParams {

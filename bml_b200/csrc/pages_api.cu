@@ -86,24 +86,28 @@ BML_API bml_status bml_page_free(const int32_t *keep, const int32_t *lens, const
                                  const int32_t *block_table, uint32_t max_pages, uint32_t page_size, const int32_t *shared,
                                  uint32_t n_pages, const int32_t *free_pages, uint32_t n_free, const int32_t *free_used,
                                  int32_t *lens_out, int32_t *owned_out, int32_t *shared_out, int32_t *free_out,
-                                 int32_t *free_used_out, int32_t *status, void *stream) {
+                                 int32_t *free_used_out, int32_t *status, void *workspace, size_t workspace_bytes,
+                                 void *stream) {
     const char *fn = "bml_page_free";
     if (bml_status st = count(fn, "requests", n)) return st;
     if (bml_status st = check_pages(page_size, max_pages, fn)) return st;
     if (n_pages == 0 || (uint64_t)n_pages * page_size >= (1ull << 31))
         return api_fail(BML_E_INVALID, "%s: %u pages of %u positions", fn, n_pages, page_size);
-    if (bml_status st = ints(fn, {keep, lens, owned, block_table, shared, free_used, lens_out, owned_out, shared_out, free_used_out, status}))
+    if (bml_status st = ints(fn, {keep, lens, owned, block_table, shared, free_used, lens_out, owned_out, shared_out, free_used_out, status,
+                              static_cast<const int32_t *>(workspace)}))
         return st;
     if (n_free > 0x7fffffffu) return api_fail(BML_E_INVALID, "%s: count above 2^31 - 1", fn);
+    const uint64_t need = bml::free_work_bytes(n_free);
+    if (workspace_bytes < need) return api_fail(BML_E_INVALID, "%s: workspace of %zu bytes, need %llu", fn, workspace_bytes, (unsigned long long)need);
     if (n_free)
         if (bml_status st = ints(fn, {free_pages, free_out})) return st;
     const uint64_t n4 = 4ull * n, p4 = 4ull * n_pages, f4 = 4ull * n_free;
     const std::initializer_list<Span> written = {{lens_out, n4}, {owned_out, n4}, {shared_out, p4}, {n_free ? free_out : nullptr, f4},
-                                                 {free_used_out, 4}, {status, n4}};
+                                                 {free_used_out, 4}, {status, n4}, {workspace, need}};
     if (overlap(written, {{keep, n4}, {lens, n4}, {owned, n4}, {block_table, n4 * max_pages}, {shared, p4}, {n_free ? free_pages : nullptr, f4},
                           {free_used, 4}}) ||
         overlap(written))
-        return api_fail(BML_E_INVALID, "%s: results must not overlap one another or what is read", fn);
+        return api_fail(BML_E_INVALID, "%s: results and workspace must not overlap one another or what is read", fn);
     bml::FreeParams p = {};
     p.keep = keep;
     p.lens = lens;
@@ -123,6 +127,8 @@ BML_API bml_status bml_page_free(const int32_t *keep, const int32_t *lens, const
     p.free_out = free_out;
     p.free_used_out = free_used_out;
     p.status = status;
+    p.work = static_cast<uint32_t *>(workspace);
+    p.num_sms = sm_count(this_device());
     return done(bml::launch_page_free(p, static_cast<cudaStream_t>(stream)), fn);
 }
 

@@ -372,13 +372,15 @@ PyObject *free_impl(PyObject *const *a) {
     const int64_t pages = shared->size(0), n_free = free->size(0);
     USUAL(keep->size(0) == n && owned->size(0) == n && table->size(0) == n && table->size(1) < (1ll << 31) && pages < (1ll << 31) &&
           n_free < (1ll << 31) && used->size(0) == 1);
-    at::Tensor all = fresh({3 * n + pages + n_free + 1}, at::kInt, dev);
+    const int64_t work = 1024 + (n_free + 31) / 32;
+    at::Tensor all = fresh({3 * n + pages + n_free + 1 + work}, at::kInt, dev);
     int32_t *o = all.mutable_data_ptr<int32_t>();
     const bml_status st =
         g_free(keep->const_data_ptr<int32_t>(), lens->const_data_ptr<int32_t>(), owned->const_data_ptr<int32_t>(), (uint32_t)n,
                table->const_data_ptr<int32_t>(), (uint32_t)table->size(1), (uint32_t)page, shared->const_data_ptr<int32_t>(),
                (uint32_t)pages, free->const_data_ptr<int32_t>(), (uint32_t)n_free, used->const_data_ptr<int32_t>(), o, o + n, o + 2 * n,
-               o + 2 * n + pages, o + 2 * n + pages + n_free, o + 2 * n + pages + n_free + 1, stream_of(dev));
+               o + 2 * n + pages, o + 2 * n + pages + n_free, o + 2 * n + pages + n_free + 1, o + 3 * n + pages + n_free + 1, 4 * (size_t)work,
+               stream_of(dev));
     USUAL(st == BML_OK);
     return pieces(all, {n, n, pages, n_free, 1, n});
 }

@@ -603,10 +603,11 @@ def page_free(keep: torch.Tensor, lens: torch.Tensor, owned: torch.Tensor, block
         raise ValueError(f"page_size {page_size} must be 0 to 2^31 - 1")
     ctx = _enter(dev, stream)
     try:
-        buf = torch.empty(3 * n + n_pages + n_free + 1, dtype=torch.int32, device=dev)
-        out = torch.unsafe_split_with_sizes(buf, (n, n, n_pages, n_free, 1, n))
+        work = 1024 + (n_free + 31) // 32
+        buf = torch.empty(3 * n + n_pages + n_free + 1 + work, dtype=torch.int32, device=dev)
+        out = torch.unsafe_split_with_sizes(buf, (n, n, n_pages, n_free, 1, n, work))
         _call("bml_page_free", a_keep, a_lens, a_owned, n, a_table, block_table.shape[1], page_size, a_shared, n_pages,
-              a_free, n_free, a_used, *(x.data_ptr() for x in out), _raw_stream(dev.index))
+              a_free, n_free, a_used, *(x.data_ptr() for x in out), 4 * work, _raw_stream(dev.index))
     finally:
         if ctx is not None:
             ctx.__exit__(None, None, None)

@@ -134,7 +134,7 @@ extern "C" {
                          max_pages: u32, page_size: u32, shared: *const i32, n_pages: u32, free_pages: *const i32,
                          n_free: u32, free_used: *const i32, lens_out: *mut i32, owned_out: *mut i32,
                          shared_out: *mut i32, free_out: *mut i32, free_used_out: *mut i32, status: *mut i32,
-                         stream: *mut c_void) -> bml_status;
+                         ws: *mut c_void, ws_bytes: usize, stream: *mut c_void) -> bml_status;
     pub fn bml_page_compact(k_pool: *mut c_void, v_pool: *mut c_void, n_layers: u32, n_pages: u32, page_size: u32,
                             n_kv: u32, head_dim: u32, kv: bml_dtype, owned: *const i32, n: u32,
                             block_table: *const i32, max_pages: u32, shared: *const i32, table_out: *mut i32,

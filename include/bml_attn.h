@@ -652,7 +652,8 @@ bml_status bml_page_fork(void *k_pool, void *v_pool, uint32_t n_layers,
  *   status [n]: 8 where keep ends inside a page that others hold: the request is
  *       left as it is (its next token would be written there); else 0.
  * block_table is not written: entries from owned_out on mean nothing.
- * Asynchronous. */
+ * workspace: 4096 + 4 * ceil(n_free / 32) bytes, no contents needed, not shared by
+ * calls that overlap in time.  Asynchronous. */
 bml_status bml_page_free(const int32_t *keep, const int32_t *lens,
                          const int32_t *owned, uint32_t n,
                          const int32_t *block_table, uint32_t max_pages,
@@ -662,7 +663,7 @@ bml_status bml_page_free(const int32_t *keep, const int32_t *lens,
                          int32_t *lens_out, int32_t *owned_out,
                          int32_t *shared_out, int32_t *free_out,
                          int32_t *free_used_out, int32_t *status,
-                         void *stream);
+                         void *workspace, size_t workspace_bytes, void *stream);
 
 /* Packs a pool: the H held pages (the first owned[i] entries of each table row)
  * come to lie at [0, H), in all layers.  Held pages from H on move, in ascending

@@ -393,3 +393,62 @@ def test_batcher_shares_and_returns_pages(cuda):
     b2.commit()
     with pytest.raises(ValueError):
         b2.truncate("a", -1)
+
+
+@pytest.mark.parametrize("n,page,per,spare", [(600, 16, 60, 0), (4096, 16, 12, 5), (1, 16, 20000, 30), (64, 16, 6000, 200000)])
+def test_free_of_a_long_list(cuda, n, page, per, spare):
+    """The form over all SMs: short and long tiles of the list, one request and many."""
+    rng = np.random.default_rng(n)
+    s = State([int(x) for x in rng.integers(per * page // 2, per * page, n)], page, spare=spare, seed=n, share=n < 1000)
+    for step in range(3):
+        keep = [int(rng.choice([-1, 0, a, a // 2, a // 2 // page * page, a + 100])) for a in s.lens]
+        p = call_free(s, keep)
+        want = want_free(s, keep)
+        for got, w in zip((p.lens, p.owned, p.shared, p.free_pages), want):
+            assert (got.cpu().numpy() == np.asarray(w)).all()
+        assert p.free_used.tolist() == [want[4]] and p.status.tolist() == want[5]
+        s.lens, s.owned, s.shared, s.free, s.used = want[0], want[1], want[2], want[3], want[4]
+
+
+@pytest.mark.parametrize("n_pages,n_free", [(20000, 7), (8, 20007), (20000, 0)])
+def test_free_of_long_state_that_does_not_hold_together(cuda, n_pages, n_free):
+    import bml_b200
+    big = 0x7fffffff
+    free = (([1, -7, big, 5, 5, 0, 2] * (n_free // 7 + 1))[:n_free]) if n_free else []
+    p = bml_b200.page_free(ints([0, 0, 0, 5, -1]), ints([100, -5, 20, 30, 40]), ints([9, 2, -3, big, 2]),
+                           ints([[5, -1, big, 5, 5, 7, 0, 0, 9]] * 5), 16, ints(([0, 3, -4] + [0] * n_pages)[:n_pages]),
+                           ints(free), ints([big]))
+    assert p.lens.tolist() == [0, -5, 20, 30, 40] and p.owned.tolist() == [0, 2, -3, big, 2]
+    assert p.shared.tolist() == [0, 3] + [0] * (n_pages - 2)
+    assert p.free_pages.tolist() == [x for x in free if x not in (5, 0)] + [x for x in free if x in (5, 0)]
+    assert p.free_used.tolist() == [len([x for x in free if x not in (5, 0)])]
+
+
+@pytest.mark.parametrize("n_pages,n,max_pages,held", [
+    (8192, 16, 1024, 8192), (8192, 16, 1024, 5000), (8193, 16, 1024, 5000), (8192, 17, 1024, 4096), (8160, 2, 8192, 1),
+    (33, 4096, 4, 20), (1, 1, 1, 1), (31, 1, 31, 31)])
+def test_compact_at_the_edges_of_its_forms(cuda, n_pages, n, max_pages, held):
+    import bml_b200
+    rng = np.random.default_rng(held)
+    order = rng.permutation(n_pages)[:held]
+    table = np.full((n, max_pages), n_pages)
+    owned = [held // n + (i < held % n) for i in range(n)]
+    at = 0
+    for i, k in enumerate(owned):
+        table[i, :k] = order[at:at + k]
+        at += k
+    pools = [torch.arange(n_pages, device="cuda", dtype=torch.float16)[None, :, None, None, None].repeat(2, 1, 16, 1, 8) for _ in "kv"]
+    mark = pools[0][:, :, 0, 0, 0].clone()
+    u = bml_b200.page_compact(*pools, ints(owned), ints(table), ints(np.arange(n_pages) % 7))
+    new = u.block_table.cpu().numpy()
+    low = np.sort(order)
+    move = dict(zip(low[low >= held], np.setdiff1d(np.arange(held), low)))
+    want = np.array([[move.get(x, x) for x in row] for row in table])
+    assert (new == want).all() and u.free_used.tolist() == [held] and u.free_pages.tolist() == list(range(n_pages))
+    shared = np.zeros(n_pages, int)
+    shared[[move.get(x, x) for x in order]] = order % 7
+    assert (u.shared.cpu().numpy() == shared).all()
+    for a, b in move.items():
+        mark[:, b] = mark[:, a]
+    for p in pools:
+        assert torch.equal(p, mark[:, :, None, None, None].expand_as(p))

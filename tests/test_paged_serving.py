@@ -37,14 +37,14 @@ fork = caller("bml_page_fork", "k v layers n_pages page n_kv d dt src dst m lens
                                                      "owned2", "shared2", "used2", "status"),
               layers=2, n_pages=4, page=16, n_kv=2, d=64, dt=2, m=2, n=3, max_pages=8, n_free=4)
 free = caller("bml_page_free", "keep lens owned n table max_pages page shared n_pages free n_free used lens2 owned2 shared2 free2 used2 "
-              "status stream", ("keep", "lens", "owned", "table", "shared", "free", "used", "lens2", "owned2", "shared2", "free2", "used2",
-                                "status"), n=3, max_pages=8, page=16, n_pages=4, n_free=4)
+              "status ws ws_bytes stream", ("keep", "lens", "owned", "table", "shared", "free", "used", "lens2", "owned2", "shared2", "free2",
+                                            "used2", "status", "ws"), n=3, max_pages=8, page=16, n_pages=4, n_free=4, ws_bytes=4100)
 compact = caller("bml_page_compact", "k v layers n_pages page n_kv d dt owned n table max_pages shared table2 shared2 free2 used2 ws "
                  "ws_bytes stream", ("k", "v", "owned", "table", "shared", "table2", "shared2", "free2", "used2", "ws"),
                  layers=2, n_pages=4, page=16, n_kv=2, d=64, dt=2, n=3, max_pages=8, ws_bytes=52)
 WRITTEN = {chunk: ("out", "ws"), verify: ("path", "count", "next"),
            fork: ("k", "v", "table", "lens2", "owned2", "shared2", "used2", "status"),
-           free: ("lens2", "owned2", "shared2", "free2", "used2", "status"),
+           free: ("lens2", "owned2", "shared2", "free2", "used2", "status", "ws"),
            compact: ("k", "v", "table2", "shared2", "free2", "used2", "ws")}
 
 
@@ -63,7 +63,7 @@ WRITTEN = {chunk: ("out", "ws"), verify: ("path", "count", "next"),
     (fork, dict(status=None)), (fork, dict(free=None)), (fork, dict(lens2=None)), (fork, dict(n_free=1 << 31)), (fork, dict(shared=A + 1)),
     (free, dict(n=0)), (free, dict(n=4097)), (free, dict(page=0)), (free, dict(max_pages=1 << 27)), (free, dict(n_pages=0)),
     (free, dict(n_pages=1 << 27)), (free, dict(keep=None)), (free, dict(free=None)), (free, dict(free2=None)), (free, dict(n_free=1 << 31)),
-    (free, dict(status=A + 2)), (compact, dict(n=0)), (compact, dict(n=4097)), (compact, dict(page=17)), (compact, dict(n_pages=0)),
+    (free, dict(status=A + 2)), (free, dict(ws=None)), (free, dict(ws=A + 2)), (free, dict(ws_bytes=4099)), (compact, dict(n=0)), (compact, dict(n=4097)), (compact, dict(page=17)), (compact, dict(n_pages=0)),
     (compact, dict(dt=-1)), (compact, dict(owned=None)), (compact, dict(ws=None)), (compact, dict(ws_bytes=51)), (compact, dict(k=None)),
     (compact, dict(d=1 << 30)), (compact, dict(table2=A + 3)),
 ])
@@ -91,7 +91,9 @@ def test_unsupported_and_nothing_to_do(L):
     assert lib.bml_attn_chunk_workspace_size(64, 1, 1, 0, None) == L.BML_E_INVALID
     assert lib.bml_attn_chunk_workspace_size(64, 5000, 7, 0, C.byref(n)) == L.BML_OK
     assert lib.bml_attn_tree_workspace_size(64, 0, C.byref(m)) == L.BML_OK
-    assert m.value < n.value < m.value + (1 << 17)
+    assert m.value < n.value < 4 * m.value + (1 << 17)   # the results of a long line's pieces, of up to four passes over it
+    assert lib.bml_attn_chunk_workspace_size(64, 1000, 7, 0, C.byref(n)) == L.BML_OK
+    assert m.value < n.value < m.value + (1 << 17)       # of one pass
     assert chunk(lib, ws_bytes=m.value) == L.BML_E_INVALID
 
 
