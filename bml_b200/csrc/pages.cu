@@ -467,8 +467,41 @@ __global__ void __launch_bounds__(kThreads) page_moves_kernel(const __grid_const
     }
 }
 
+// Pages from[m] to to[m], in all layers, K and V.  A CTA copies a unit a thread of a
+// page (a piece) at a time, kInFlight pieces in flight.
+template <typename U, typename I>
+__device__ __forceinline__ void move_pages(const PoolParams &p, const I *from, const I *to, uint32_t moves) {
+    constexpr uint32_t kInFlight = 8;
+    const uint64_t page_bytes = (uint64_t)p.row_bytes << p.page_shift;  // below 2^31
+    const uint32_t units = (uint32_t)(page_bytes / sizeof(U)), pieces = (units + kThreads - 1) / kThreads, both = 2 * p.n_layers;
+    // (move, layer and side, piece) as digits, advanced by the grid's
+    const uint32_t dp = gridDim.x % pieces, dl = gridDim.x / pieces % both, dm = gridDim.x / pieces / both;
+    uint32_t at = blockIdx.x % pieces, lw = blockIdx.x / pieces % both, m = blockIdx.x / pieces / both;
+    while (m < moves) {
+        U x[kInFlight], *d[kInFlight];
+#pragma unroll
+        for (uint32_t k = 0; k < kInFlight; ++k) {
+            const uint32_t u = at * kThreads + threadIdx.x;
+            d[k] = nullptr;
+            if (m < moves && u < units) {
+                char *base = ((lw & 1) ? p.v_pool : p.k_pool) + (lw >> 1) * p.layer_bytes;
+                d[k] = reinterpret_cast<U *>(base + (uint32_t)to[m] * page_bytes) + u;
+                x[k] = __ldcs(reinterpret_cast<const U *>(base + (uint32_t)from[m] * page_bytes) + u);
+            }
+            at += dp;
+            lw += dl + (at >= pieces);
+            at -= at >= pieces ? pieces : 0;
+            m += dm + (lw >= both);
+            lw -= lw >= both ? both : 0;
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kInFlight; ++k)
+            if (d[k]) __stcs(d[k], x[k]);
+    }
+}
+
 template <typename U>
-__global__ void __launch_bounds__(kThreads) page_move_kernel(const __grid_constant__ CompactParams p, uint32_t piece) {
+__global__ void __launch_bounds__(kThreads) page_move_kernel(const __grid_constant__ CompactParams p) {
     const uint32_t n = p.pool.n_pages;
     const int32_t *where = p.work, *from = where + n, *to = from + n;
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -478,14 +511,7 @@ __global__ void __launch_bounds__(kThreads) page_move_kernel(const __grid_consta
         const int32_t page = p.table[e];
         p.table_out[e] = (int32_t)k < p.owned[i] && (uint32_t)page < n ? where[page] : page;
     }
-    const uint64_t page_bytes = (uint64_t)p.pool.row_bytes << p.pool.page_shift;
-    const uint64_t pieces = (page_bytes + piece - 1) / piece, per = pieces * 2 * p.pool.n_layers, items = per * (uint32_t)to[n];
-    for (uint64_t it = blockIdx.x; it < items; it += gridDim.x) {
-        const uint64_t m = it / per, lw = (it - m * per) / pieces, off = (it - m * per - lw * pieces) * piece;
-        char *base = ((lw & 1) ? p.pool.v_pool : p.pool.k_pool) + (lw >> 1) * p.pool.layer_bytes + off;
-        const uint64_t left = page_bytes - off;
-        copy_cta<U>(base + (uint32_t)to[m] * page_bytes, base + (uint32_t)from[m] * page_bytes, (uint32_t)(left < piece ? left : piece));
-    }
+    move_pages<U>(p.pool, from, to, (uint32_t)to[n]);
 }
 
 // Both in one launch for a small pool: every CTA finds all the moves, from bits in
@@ -493,7 +519,7 @@ __global__ void __launch_bounds__(kThreads) page_move_kernel(const __grid_consta
 constexpr uint32_t kSmallPages = 8192, kSmallEntries = 16384;
 
 template <typename U>
-__global__ void __launch_bounds__(kThreads) page_compact_kernel(const __grid_constant__ CompactParams p, uint32_t piece) {
+__global__ void __launch_bounds__(kThreads) page_compact_kernel(const __grid_constant__ CompactParams p) {
     constexpr uint32_t kWords = kSmallPages / 32, kAtOnce = 8;
     static_assert(kWords <= kThreads, "a word a thread");
     __shared__ uint32_t held_bits[kWords], before[kWords], sums[kThreads / 32];
@@ -544,14 +570,7 @@ __global__ void __launch_bounds__(kThreads) page_compact_kernel(const __grid_con
         if (i >= held) p.shared_out[i] = 0;
     }
     if (me == 0) *p.free_used_out = (int32_t)held;
-    const uint64_t page_bytes = (uint64_t)p.pool.row_bytes << p.pool.page_shift;
-    const uint64_t pieces = (page_bytes + piece - 1) / piece, per = pieces * 2 * p.pool.n_layers, items = per * moves;
-    for (uint64_t it = blockIdx.x; it < items; it += gridDim.x) {
-        const uint64_t m = it / per, lw = (it - m * per) / pieces, off = (it - m * per - lw * pieces) * piece;
-        char *base = ((lw & 1) ? p.pool.v_pool : p.pool.k_pool) + (lw >> 1) * p.pool.layer_bytes + off;
-        const uint64_t left = page_bytes - off;
-        copy_cta<U>(base + to[m] * page_bytes, base + from[m] * page_bytes, (uint32_t)(left < piece ? left : piece));
-    }
+    move_pages<U>(p.pool, from, to, moves);
 }
 
 bool wide(const PoolParams &p) {
@@ -588,14 +607,12 @@ cudaError_t launch_page_free(const FreeParams &p, cudaStream_t st) {
 }
 
 cudaError_t launch_page_compact(const CompactParams &p, cudaStream_t st) {
-    // pieces of a page that a CTA copies in one round: eight units a thread
     const bool w = wide(p.pool);
-    const uint32_t piece = kThreads * 8 * (w ? 16 : 2);
     if (p.pool.n_pages <= kSmallPages && (uint64_t)p.n * p.max_pages <= kSmallEntries)
-        return launch_after(w ? page_compact_kernel<uint4> : page_compact_kernel<uint16_t>, dim3((uint32_t)p.num_sms * 4), kThreads, 0, st, p, piece);
+        return launch_after(w ? page_compact_kernel<uint4> : page_compact_kernel<uint16_t>, dim3((uint32_t)p.num_sms * 4), kThreads, 0, st, p);
     const cudaError_t e = launch_clusters(page_moves_kernel, kBook, dim3(kBook), kThreads, 0, st, p);
     if (e != cudaSuccess) return e;
-    return launch_after(w ? page_move_kernel<uint4> : page_move_kernel<uint16_t>, dim3((uint32_t)p.num_sms * 4), kThreads, 0, st, p, piece);
+    return launch_after(w ? page_move_kernel<uint4> : page_move_kernel<uint16_t>, dim3((uint32_t)p.num_sms * 4), kThreads, 0, st, p);
 }
 
 }  // namespace bml
