@@ -558,8 +558,11 @@ cudaError_t launch_x(const TreeArgs &a, cudaStream_t st) {
     xp.t.heavy_rows = 0xffffffffu;
     xp.t.heavy = xp.t.light = 1;
     // 4 requests of 500 to 3000 positions: 37.4 us, 38.6 without a lead, 39.3 with 3; 40
-    // of 50 to 1000: 52.8, 60.7, 55.8
-    xp.t.lead = 1;
+    // of 50 to 1000: 52.8, 60.7, 55.8.  The pieces of chunks are many units of unlike
+    // lengths (1600 fresh tokens with lead 1, 2, 3, 4: d = 128 273, 193, 196, 203 us, d =
+    // 64 143, 134, 140, 144; 3 requests of 626, 459, 502 behind 241, 310, 105: d = 128
+    // 170, 160, 151, 153, d = 64 111, 102, 103, 105).
+    xp.t.lead = !a.p.row_of ? 1 : D == 128 ? 3 : 2;
     if (!tree_line(xp.t)) return cudaErrorNotSupported;
     const uint64_t rows = (uint64_t)a.p.n_pages << a.p.page_shift;
     if (!pool_map(&xp.tk, a.p.k, D, a.p.n_kv, rows, 32, xp.box_rows, CU_TENSOR_MAP_SWIZZLE_128B) ||
