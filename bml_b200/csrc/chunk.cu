@@ -1,6 +1,6 @@
 // chunk.cu -- attention of chunks of any number of new tokens over a paged cache,
 // where chunk_umma.cu does not take them: 32-bit queries, a scale of 0, groups of
-// more than 128 q heads.
+// more than 128 q heads, and batches of few tokens.
 //
 // Row t of a request's T new tokens sees the positions 0 .. P + t, P = L - T.  A
 // chunk is cut into pieces of W consecutive tokens: piece k is a request of its
@@ -17,6 +17,18 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr uint32_t kPieceRows = 256;
+// 32-bit queries over 16-bit pages: tree_umma32.cu from so many rows a request or piece
+// on (on average).  3 requests of 706 fresh tokens, d = 128, group 4: 163 us, 271 with
+// tree_warp.cu; 8 of 64 tokens behind 1000: 88 and 131; 32 of 16 behind 2000: 222 and
+// 220, of 8: 217 and 128.
+constexpr uint32_t kTf32Rows = 80;
+// Batches of so few tokens are a call of tree*.cu as they are, no request having more
+// than such a call takes: no pieces are made (32-bit queries: 3 us less), and with
+// 16-bit queries those kernels start sooner than chunk_umma.cu (bf16, d = 128, one
+// token behind 1000 positions 11.9 us, 15.3 there; 64 tokens 18.9 and 25.2; d = 64,
+// 8 of one token 9.6 and 16.0; one request of 128 tokens 24.7 and 28.2, d = 64 20.0 and 22.5; but 32 of one token 44.8 and 37.4, 3 of 80 tokens 31.7 and
+// 30.0).
+constexpr uint32_t kFewTokens = 64, kFewSeqs = 8;
 
 struct PieceParams {
     const int32_t *node_start, *kv_lens;  // [n + 1], [n]
@@ -92,9 +104,15 @@ size_t chunk_work_bytes(uint64_t n_tokens, uint64_t n_seqs, int num_sms) {
 }
 
 cudaError_t launch_chunk(const TreeArgs &args, int32_t *work, cudaStream_t st) {
-    if (chunk_umma_fits(args)) return launch_chunk_umma(args, work, st);
     TreeArgs a = args;
     TreeParams &p = a.p;
+    const bool umma = chunk_umma_fits(args), tf32_fits = p.q_type == BML_F32 && p.scale_log2 > 0.f && tree_umma_fits(a);
+    const bool few = p.n_seqs <= kFewSeqs;
+    if (umma ? few && p.n_tokens <= (p.n_seqs == 1 ? kTreeMaxNodes / 2 : kFewTokens) && !p.diag : p.n_tokens <= kTreeMaxNodes && p.n_seqs <= kTreeMaxSeqs) {
+        tree_rows(a, p.n_tokens, p.group, p.n_seqs, 0u, few ? p.n_tokens : 0u);
+        return !umma && a.kv_type != BML_F32 && tf32_fits && a.rows >= kTf32Rows ? launch_tree_umma32(a, st) : launch_tree(a, st);
+    }
+    if (umma) return launch_chunk_umma(args, work, st);
     PieceParams pp = {};
     pp.node_start = p.node_start;
     pp.kv_lens = p.kv_lens;
@@ -109,12 +127,13 @@ cudaError_t launch_chunk(const TreeArgs &args, int32_t *work, cudaStream_t st) {
     pp.row_of = pp.lens + pp.most;
     cudaError_t e = launch_after(chunk_pieces_kernel, dim3(1), kThreads, 0, st, pp);
     tree_rows(a, p.n_tokens, p.group, pp.most, 0u, 0u);
+    const bool tf32 = a.kv_type != BML_F32 && tf32_fits && a.rows >= kTf32Rows;
     for (uint32_t base = 0; base < pp.most && e == cudaSuccess; base += kTreeMaxSeqs) {
         p.n_seqs = pp.most - base < kTreeMaxSeqs ? pp.most - base : kTreeMaxSeqs;
         p.node_start = pp.start + base;
         p.kv_lens = pp.lens + base;
         p.row_of = pp.row_of + base;
-        e = launch_tree(a, st);
+        e = tf32 ? launch_tree_umma32(a, st) : launch_tree(a, st);
     }
     return e;
 }

@@ -56,25 +56,29 @@ constexpr int kRowWarps = 8, kSplitWarps = 6;
 constexpr int kThreads = 32 * (2 + kRowWarps + kSplitWarps);  // 512: up to 128 registers a thread
 constexpr int kBadRing = 16;  // tiles whose page flags are kept
 
-template <int D>
+template <int D, typename T>
 struct XCfg {
-    static constexpr int KB = D / 32;          // 128-byte column blocks of a K row
-    static constexpr int TILE = BN * D * 4;    // a K or V tile
-    static constexpr int OFF_K = 0;            // two stages: per column block 64 rows hi (in place), 64 rows lo
+    static constexpr bool kWide = sizeof(T) == 4;
+    static constexpr int KR = D * sizeof(T) / 128;   // 128-byte column blocks of a K row
+    static constexpr int TILE = BN * D * 4;          // a K or V tile of 32-bit values
+    static constexpr int RAW = BN * D * sizeof(T);   // and as it arrives
+    static constexpr int OFF_K = 0;                  // two stages: per column block 64 rows hi (32 bits: in place), 64 rows lo
     static constexpr int OFF_V = 4 * TILE;
-    static constexpr int OFF_VHI = 5 * TILE;   // [2 blocks of 32 positions][D][128 B]
-    static constexpr int OFF_VLO = 6 * TILE;
-    static constexpr int OFF_SH = 7 * TILE;
+    static constexpr int OFF_VHI = OFF_V + RAW;      // [2 blocks of 32 positions][D][128 B]
+    static constexpr int OFF_VLO = OFF_VHI + TILE;   // 32 bits only: 16 are exact in TF32
+    static constexpr int OFF_KR = OFF_VLO;           // 16 bits only: two stages of K as it arrives
+    static constexpr int OFF_SH = OFF_VLO + TILE;
     static constexpr int SMEM = OFF_SH + 3 * 1024;
     // tensor memory columns
     static constexpr uint32_t QHI = 0, QLO = D, OC = 2 * D;
     static constexpr uint32_t SC = 3 * D, PLO = SC + BN;  // S: Q hi * K hi, and the other two products; then P
     static constexpr uint32_t TMEM_COLS = 512;
 };
-static_assert(XCfg<128>::SMEM <= 227 * 1024 && XCfg<128>::PLO + BN == 512, "shared and tensor memory");
+static_assert(XCfg<128, float>::SMEM <= 227 * 1024 && XCfg<128, float>::PLO + BN == 512, "shared and tensor memory");
+static_assert(2 * XCfg<128, __half>::RAW <= XCfg<128, __half>::TILE, "K as it arrives");
 
 struct XParams {
-    CUtensorMap tk, tv;  // (d, n_kv, rows); box (32, 1, box_rows) swizzled, (d, 1, box_rows) plain
+    CUtensorMap tk, tv;  // (d, n_kv, rows); box (128 bytes, 1, box_rows) swizzled, (d, 1, box_rows) plain
     TreeParams t;
     uint32_t box_rows;  // min(page, 64)
 };
@@ -129,9 +133,9 @@ __device__ __forceinline__ uint32_t see_half(const TreeParams &p, const TreeSeq 
     return see;
 }
 
-template <int D>
+template <int D, typename T>
 __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_constant__ XParams xp) {
-    using C = XCfg<D>;
+    using C = XCfg<D, T>;
     const TreeParams &p = xp.t;
     extern __shared__ __align__(1024) uint8_t smem[];
     XShared &sh = *reinterpret_cast<XShared *>(smem + C::OFF_SH);
@@ -180,12 +184,12 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
 
     if (warp == 0) {
         // --------------------------------------------------------------- producer
-        // Lanes 0-15 issue K's boxes (column block lane % KB of part lane / KB),
+        // Lanes 0-15 issue K's boxes (column block lane % KR of part lane / KR),
         // lanes 16-19 V's (part lane - 16).
         const uint64_t policy = l2_policy_evict_first();
         const uint32_t parts = BN / xp.box_rows, ps_mask = (1u << p.page_shift) - 1;
         const bool is_k = lane < 16;
-        const uint32_t part = is_k ? lane / C::KB : lane - 16, kb = is_k ? lane % C::KB : 0u;
+        const uint32_t part = is_k ? lane / C::KR : lane - 16, kb = is_k ? lane % C::KR : 0u;
         const bool mine = part < parts && lane < 20;
         bool live = !(p.diag & kTreeStall);
         while (live && walk.next(p, sg)) {
@@ -209,23 +213,25 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
                 if (lane == 0) *(volatile uint32_t *)&sh.bad[it % kBadRing] = flag;
                 // a page outside the pool is read past the map's end: zeros
                 const int at = row == -2 ? (int)(p.n_pages << p.page_shift) : row;
-                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, row != -1 && !is_k)) * xp.box_rows * D * 4;
+                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, row != -1 && !is_k)) * xp.box_rows * D * (uint32_t)sizeof(T);
                 const bool once = sg.s.groups == 1;  // K and V are read once
                 auto copy = [&](bool k, uint64_t *full, uint8_t *dst) {
                     if (lane == 0) mbar_arrive_expect_tx(full, bytes);
                     __syncwarp();
                     if (row != -1 && is_k == k) {
-                        if (once) tma_load_3d_hint(dst, k ? &xp.tk : &xp.tv, (int)kb * 32, (int)sg.head, at, full, policy);
-                        else tma_load_3d(dst, k ? &xp.tk : &xp.tv, (int)kb * 32, (int)sg.head, at, full);
+                        if (once) tma_load_3d_hint(dst, k ? &xp.tk : &xp.tv, (int)(kb * 128 / sizeof(T)), (int)sg.head, at, full, policy);
+                        else tma_load_3d(dst, k ? &xp.tk : &xp.tv, (int)(kb * 128 / sizeof(T)), (int)sg.head, at, full);
                     }
                     __syncwarp();
                 };
                 if (use > 0) live = __all_sync(0xffffffffu, wait_bar(&sh.k_empty[st], (use & 1u) ^ 1u, abort_flag, p.wait_ns));
                 if (!live) break;
-                copy(true, &sh.k_full[st], smem + C::OFF_K + st * 2 * C::TILE + kb * 2 * BN * 128 + part * xp.box_rows * 128);
+                copy(true, &sh.k_full[st],
+                     (C::kWide ? smem + C::OFF_K + st * 2 * C::TILE + kb * 2 * BN * 128 : smem + C::OFF_KR + st * C::RAW + kb * BN * 128) +
+                         part * xp.box_rows * 128);
                 if (it > 0) live = __all_sync(0xffffffffu, wait_bar(&sh.v_empty, (it & 1u) ^ 1u, abort_flag, p.wait_ns));
                 if (!live) break;
-                copy(false, &sh.v_full, smem + C::OFF_V + part * xp.box_rows * D * 4);
+                copy(false, &sh.v_full, smem + C::OFF_V + part * xp.box_rows * D * sizeof(T));
             }
         }
         // No copy may outlive the CTA: all have landed unless a wait gave up,
@@ -275,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
                 wait_all(&sh.p_ready, par);
                 if (!live) break;
                 chain(tmem + C::OC, tmem + C::PLO, d_vhi, D * 128, idesc_pv, BN / 8, true);
-                chain(tmem + C::OC, tmem + C::SC, d_vlo, D * 128, idesc_pv, BN / 8, false);
+                if (C::kWide) chain(tmem + C::OC, tmem + C::SC, d_vlo, D * 128, idesc_pv, BN / 8, false);
                 chain(tmem + C::OC, tmem + C::SC, d_vhi, D * 128, idesc_pv, BN / 8, false);
                 if (elect_one()) tc_commit(&sh.o_full);
                 __syncwarp();
@@ -420,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
                         float tmp[32];  // its address is taken, o's is not
 #pragma unroll
                         for (int u = 0; u < 32; ++u) tmp[u] = o[c + u];
-                        tree_nonfinite<D, float>(p, a, half * (D / 2) + c, 32, any[0] != any[0], tmp);
+                        tree_nonfinite<D, T>(p, a, half * (D / 2) + c, 32, any[0] != any[0], tmp);
 #pragma unroll
                         for (int u = 0; u < 32; ++u) o[c + u] = tmp[u];
                     }
@@ -447,6 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
         // --------------------------------------------------------- K and V split
         const uint32_t cw = warp - 2 - kRowWarps, tid = cw * 32 + lane;
         constexpr uint32_t kN = kSplitWarps * 32;
+        constexpr bool kF16 = std::is_same<T, __half>::value;
         uint32_t total = 0;  // tiles of this CTA
         {
             TreeWalk<false> w(range);
@@ -457,9 +464,31 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
             wait_bar(&sh.k_full[i & 1u], (i >> 1) & 1u, abort_flag, p.wait_ns);
             __syncwarp();
             uint4 *k = reinterpret_cast<uint4 *>(smem + C::OFF_K + (i & 1u) * 2 * C::TILE);
+            constexpr uint32_t kBlock = BN * 8;  // 16-byte pieces of a block's hi (or lo) rows
+            if constexpr (!C::kWide) {
+                const uint4 *raw = reinterpret_cast<const uint4 *>(smem + C::OFF_KR + (i & 1u) * C::RAW);
+                // eight rows' pieces of one column a quarter warp: other banks, swizzled as they are
+#pragma unroll 2
+                for (uint32_t x = tid; x < C::RAW / 16; x += kN) {
+                    const uint32_t row = (x & 7) + x / D * 8, c = x / 8 % (D / 8);  // eight columns from 8 c on
+                    const uint4 y = raw[c / 8 * (BN * 8) + row * 8 + ((c ^ row) & 7)];
+                    const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+                    uint32_t h[8], l[8];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        tf32_split_any(wide16<kF16>((uint16_t)w[u]), h[2 * u], l[2 * u]);
+                        tf32_split_any(wide16<kF16>((uint16_t)(w[u] >> 16)), h[2 * u + 1], l[2 * u + 1]);
+                    }
+#pragma unroll
+                    for (uint32_t u = 0; u < 2; ++u) {
+                        const uint32_t e = c / 4 * (2 * kBlock) + row * 8 + ((c % 4 * 2 + u) ^ (row & 7));
+                        k[e] = make_uint4(h[4 * u], h[4 * u + 1], h[4 * u + 2], h[4 * u + 3]);
+                        k[e + kBlock] = make_uint4(l[4 * u], l[4 * u + 1], l[4 * u + 2], l[4 * u + 3]);
+                    }
+                }
+            }
 #pragma unroll 4
-            for (uint32_t x = tid; x < C::TILE / 16; x += kN) {
-                constexpr uint32_t kBlock = BN * 8;  // 16-byte pieces of a block's hi (or lo) rows
+            for (uint32_t x = tid; C::kWide && x < C::TILE / 16; x += kN) {
                 const uint32_t e = x + x / kBlock * kBlock;
                 const uint4 y = k[e];
                 uint4 h, l;
@@ -482,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
                 wait_bar(&sh.v_full, it & 1u, abort_flag, p.wait_ns);
                 if (it > 0) wait_bar(&sh.o_full, (it & 1u) ^ 1u, abort_flag, p.wait_ns);  // the last tile's V has been read
                 __syncwarp();
-                const float *v = reinterpret_cast<const float *>(smem + C::OFF_V);
+                const T *v = reinterpret_cast<const T *>(smem + C::OFF_V);
                 const uint32_t kv0 = j * BN;
                 const bool edge = kv0 + BN > P;
 #pragma unroll 4
@@ -490,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
                     const uint32_t quad = u % (BN / 4), d = u / (BN / 4) * 32 + lane;
                     float x[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] = v[(quad * 4 + e) * D + d];
+                    for (int e = 0; e < 4; ++e) x[e] = (float)v[(quad * 4 + e) * D + d];
                     if (edge) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
@@ -502,14 +531,18 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
                             }
                         }
                     }
-                    uint4 h, l;
-                    tf32_split_any(x[0], h.x, l.x);
-                    tf32_split_any(x[1], h.y, l.y);
-                    tf32_split_any(x[2], h.z, l.z);
-                    tf32_split_any(x[3], h.w, l.w);
                     const uint32_t to = (quad >> 3) * (D * 128) + d * 128 + (((quad & 7) ^ (d & 7)) << 4);
+                    uint4 h, l;
+                    if (C::kWide) {
+                        tf32_split_any(x[0], h.x, l.x);
+                        tf32_split_any(x[1], h.y, l.y);
+                        tf32_split_any(x[2], h.z, l.z);
+                        tf32_split_any(x[3], h.w, l.w);
+                        *reinterpret_cast<uint4 *>(smem + C::OFF_VLO + to) = l;
+                    } else {
+                        h = make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
+                    }
                     *reinterpret_cast<uint4 *>(smem + C::OFF_VHI + to) = h;
-                    *reinterpret_cast<uint4 *>(smem + C::OFF_VLO + to) = l;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -532,22 +565,26 @@ __global__ void __launch_bounds__(kThreads, 1) tree_umma32_kernel(const __grid_c
 }
 
 // (d, n_kv, rows) view of a pool.
+template <typename T>
 bool pool_map(CUtensorMap *map, const void *base, uint32_t d, uint32_t n_kv, uint64_t rows, uint32_t box_d, uint32_t box_rows,
               CUtensorMapSwizzle swizzle) {
     auto enc = get_encode();
     if (!enc) return false;
     cuuint64_t dims[3] = {d, n_kv, rows};
-    cuuint64_t strides[2] = {(cuuint64_t)d * 4, (cuuint64_t)d * n_kv * 4};
+    cuuint64_t strides[2] = {(cuuint64_t)d * sizeof(T), (cuuint64_t)d * n_kv * sizeof(T)};
     cuuint32_t box[3] = {box_d, 1, box_rows};
     cuuint32_t estr[3] = {1, 1, 1};
-    return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<void *>(base), dims, strides, box, estr,
+    constexpr CUtensorMapDataType type = sizeof(T) == 4                      ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                         : std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                          : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return enc(map, type, 3, const_cast<void *>(base), dims, strides, box, estr,
                CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D>
+template <int D, typename T>
 cudaError_t launch_x(const TreeArgs &a, cudaStream_t st) {
-    using C = XCfg<D>;
+    using C = XCfg<D, T>;
     static thread_local XParams xp;
     xp.t = a.p;
     const uint32_t page = 1u << a.p.page_shift;
@@ -565,10 +602,10 @@ cudaError_t launch_x(const TreeArgs &a, cudaStream_t st) {
     xp.t.lead = !a.p.row_of ? 1 : D == 128 ? 3 : 2;
     if (!tree_line(xp.t)) return cudaErrorNotSupported;
     const uint64_t rows = (uint64_t)a.p.n_pages << a.p.page_shift;
-    if (!pool_map(&xp.tk, a.p.k, D, a.p.n_kv, rows, 32, xp.box_rows, CU_TENSOR_MAP_SWIZZLE_128B) ||
-        !pool_map(&xp.tv, a.p.v, D, a.p.n_kv, rows, D, xp.box_rows, CU_TENSOR_MAP_SWIZZLE_NONE))
+    if (!pool_map<T>(&xp.tk, a.p.k, D, a.p.n_kv, rows, 128 / sizeof(T), xp.box_rows, CU_TENSOR_MAP_SWIZZLE_128B) ||
+        !pool_map<T>(&xp.tv, a.p.v, D, a.p.n_kv, rows, D, xp.box_rows, CU_TENSOR_MAP_SWIZZLE_NONE))
         return cudaErrorInvalidValue;
-    auto kern = tree_umma32_kernel<D>;
+    auto kern = tree_umma32_kernel<D, T>;
     static SmemSet set;  // one for each instantiation
     cudaError_t e = set.allow(kern, C::SMEM);
     if (e != cudaSuccess) return e;
@@ -579,6 +616,13 @@ cudaError_t launch_x(const TreeArgs &a, cudaStream_t st) {
 
 }  // namespace
 
-cudaError_t launch_tree_umma32(const TreeArgs &a, cudaStream_t st) { return a.D == 128 ? launch_x<128>(a, st) : launch_x<64>(a, st); }
+cudaError_t launch_tree_umma32(const TreeArgs &a, cudaStream_t st) {
+    const bool d128 = a.D == 128;
+    switch (a.kv_type) {
+        case BML_F16: return d128 ? launch_x<128, __half>(a, st) : launch_x<64, __half>(a, st);
+        case BML_BF16: return d128 ? launch_x<128, __nv_bfloat16>(a, st) : launch_x<64, __nv_bfloat16>(a, st);
+        default: return d128 ? launch_x<128, float>(a, st) : launch_x<64, float>(a, st);
+    }
+}
 
 }  // namespace bml
