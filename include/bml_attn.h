@@ -403,9 +403,14 @@ bml_status bml_kvsplit_destroy(bml_kvsplit *h);
  *   bml_paged_plan      pages for the new tokens, their slots, positions and
  *                       (for drafts) ancestor masks -- once a step
  *   bml_paged_append    RoPE of q and k, K and V rows stored -- every layer
- *   bml_attn_tree       attention of the new tokens -- every layer
+ *   bml_attn_tree       attention of the new tokens -- every layer; or
+ *   bml_attn_chunk      the same for any number of them, without drafts
+ *   bml_verify_drafts   which drafted tokens the target model keeps
  *   bml_paged_commit    the rows of the accepted path moved to the front,
  *                       all layers, new lengths -- once a step
+ * and between steps bml_page_fork (requests that share another's pages),
+ * bml_page_free (pages of requests that end or are rolled back) and
+ * bml_page_compact (the pool packed to its front).
  * page_size is a power of two from 16 to 1024 and max_pages * page_size
  * below 2^31 in every call. */
 
