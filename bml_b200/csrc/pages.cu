@@ -22,6 +22,10 @@ namespace {
 constexpr uint32_t kBook = 8;  // CTAs of the bookkeeping cluster
 constexpr int kThreads = 512;
 constexpr int kFreeThreads = 1024;
+// From so many pages, or entries of the free list, on a release goes over all SMs.  512
+// requests, 131,000 pages: 43 us by the cluster, 10.4 over all SMs; 32,768 pages 12.3 and
+// 7.6; 16,384 9.2 and 7.3; 4096 7.7 and 6.8.  But four launches take the host 11.5 us,
+// one 5.7.
 constexpr uint32_t kWidePages = 16384;
 
 // Block-wide exclusive sum; every thread gets the total.  sums: one per warp.
@@ -515,13 +519,16 @@ __global__ void __launch_bounds__(kThreads) page_move_kernel(const __grid_consta
 }
 
 // Both in one launch for a small pool: every CTA finds all the moves, from bits in
-// shared memory, and makes its share of them.
+// shared memory, and makes its share of them.  6 requests of 16 pages in 200, 22 layers:
+// 7.8 us, 14.7 in two launches; 32 of 60 in 4000, 4 layers 22.7 and 31.5; 128 of 32 in
+// 8192, one layer 15.1 and 22.3.  A CTA an SM: its search costs more than its copies gain
+// from more of them (the first case with two 10.0 us, with four 13.7).
 constexpr uint32_t kSmallPages = 8192, kSmallEntries = 16384;
 
 template <typename U>
 __global__ void __launch_bounds__(kThreads) page_compact_kernel(const __grid_constant__ CompactParams p) {
     constexpr uint32_t kWords = kSmallPages / 32, kAtOnce = 8;
-    static_assert(kWords <= kThreads, "a word a thread");
+    static_assert(kWords <= kThreads, "a word a thread");  // and 16-bit page numbers
     __shared__ uint32_t held_bits[kWords], before[kWords], sums[kThreads / 32];
     __shared__ uint16_t from[kSmallPages / 2], to[kSmallPages / 2];  // as many movers as holes below them
     const uint32_t n = p.pool.n_pages, tid = threadIdx.x, me = blockIdx.x * kThreads + tid, all = gridDim.x * kThreads;
@@ -609,7 +616,7 @@ cudaError_t launch_page_free(const FreeParams &p, cudaStream_t st) {
 cudaError_t launch_page_compact(const CompactParams &p, cudaStream_t st) {
     const bool w = wide(p.pool);
     if (p.pool.n_pages <= kSmallPages && (uint64_t)p.n * p.max_pages <= kSmallEntries)
-        return launch_after(w ? page_compact_kernel<uint4> : page_compact_kernel<uint16_t>, dim3((uint32_t)p.num_sms * 4), kThreads, 0, st, p);
+        return launch_after(w ? page_compact_kernel<uint4> : page_compact_kernel<uint16_t>, dim3((uint32_t)p.num_sms), kThreads, 0, st, p);
     const cudaError_t e = launch_clusters(page_moves_kernel, kBook, dim3(kBook), kThreads, 0, st, p);
     if (e != cudaSuccess) return e;
     return launch_after(w ? page_move_kernel<uint4> : page_move_kernel<uint16_t>, dim3((uint32_t)p.num_sms * 4), kThreads, 0, st, p);

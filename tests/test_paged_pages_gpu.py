@@ -452,3 +452,9 @@ def test_compact_at_the_edges_of_its_forms(cuda, n_pages, n, max_pages, held):
         mark[:, b] = mark[:, a]
     for p in pools:
         assert torch.equal(p, mark[:, :, None, None, None].expand_as(p))
+
+
+@pytest.mark.parametrize("n_pages,n,max_pages,held", [(2048, 8, 1024, 2048), (2048, 8, 1024, 1100), (2049, 8, 1024, 1100),
+                                                      (2048, 9, 1024, 1100), (2047, 1, 8192, 700)])
+def test_compact_between_its_forms(cuda, n_pages, n, max_pages, held):
+    test_compact_at_the_edges_of_its_forms(None, n_pages, n, max_pages, held)
