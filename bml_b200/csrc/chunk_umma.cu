@@ -41,6 +41,11 @@
 //     scores against the maximum so far while the maximum is found beside them, and
 //     only where that grew by more than 2^8 in either half (the result is exact for any
 //     fixed reference) takes them anew, from tensor memory, and rescales O.
+//
+// Measured on B200, d = 128, group 4: 2048 tokens behind 30,720 positions 870 us (1.22
+// PFLOP/s, at the power cap), 4 requests of 512 behind 4000 155 us (920 TFLOP/s; tensor
+// pipe 50% of active cycles, exponentials 51%: a chain's softmax and MMAs wait for each
+// other); d = 64, 300 tokens behind 700 21 us, most of it start and end.
 #include <math.h>
 
 #include <type_traits>

@@ -89,7 +89,9 @@ __device__ __forceinline__ void copy_cta(char *dst, const char *src, uint32_t by
 //   free[used + (part-filled pages of the forks before)], since both requests
 //   will write behind their rows.
 // Every CTA redoes the plan (a few loads a fork, one scan); cluster 0 keeps the
-// books, and all copy.  Memory-bound in the copies.
+// books, and all copy.  Memory-bound in the copies: 48 forks, 32 layers, rows of 2 KB
+// 81 us (6.2 TB/s; four CTAs an SM: 87 with one, 97 with two); 8 forks of one prompt 7 us,
+// launch and the plan's dependent loads.
 // ---------------------------------------------------------------------------
 struct ForkOne {
     int32_t len;       // positions; -1: refused
@@ -390,7 +392,8 @@ __global__ void __launch_bounds__(kWideThreads) free_place_kernel(const __grid_c
 // holds, both in ascending order; sources and destinations are disjoint, so the
 // moves need no order.  Tables and shared counts follow the pages, and the free
 // list becomes 0, 1, 2, ... with H taken.  The first kernel finds the moves, the
-// second makes them.
+// second makes them.  Memory-bound: 32 requests, 32 layers, pages of 131 KB 551 us (6.1
+// TB/s).
 // work: where[n_pages] (mark, then a page's new place), from[n_pages], to[n_pages],
 // the number of moves.
 // ---------------------------------------------------------------------------

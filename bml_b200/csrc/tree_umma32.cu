@@ -1,6 +1,7 @@
-// tree_umma32.cu -- attention of drafted tokens over a paged cache of 32-bit
-// values on tcgen05 tensor cores (sm_100a): results to about f32 precision
-// from TF32 products.
+// tree_umma32.cu -- attention of drafted tokens with 32-bit queries over a paged
+// cache on tcgen05 tensor cores (sm_100a): results to about f32 precision from TF32
+// products.  Pages hold 32-bit values, or, for chunks of new tokens (chunk.cu), 16-bit
+// ones.
 //
 // The mathematics and the schedule are those of tree.cu / tree.cuh: a CTA (one
 // per SM) works through its even share of the line of 64-position tiles,
@@ -37,6 +38,12 @@
 // has no second buffer; copies, splits and MMA operands pass 3600 cycles' worth
 // of shared memory.  4 requests of 618 to 2671 positions, 32 to 84 rows: 43 us,
 // 75.6 with tree.cu's kernel.
+//
+// 16-bit pages: values are exact in TF32, so V has no lo part (and one chain of P V
+// less: 0.7 us).  K's is kept, zeros but for infinities and NaN, since Q hi * K takes an
+// MMA of 128 columns' time without it too.  K arrives in 16 bits beside its stages, the
+// same split warps widen it.  3 requests of 706 fresh tokens, d = 128, group 4: 163 us,
+// 271 with tree_warp.cu (mma.sync).
 //
 // What a row does not see must not reach it: scores are replaced by -inf (bad
 // pages, rows past the length, nodes outside the mask), V rows past the length

@@ -22,8 +22,10 @@
 // A cluster of 1 to 8 CTAs serves a request; each walks the tree by itself (the
 // probabilities of drafted tokens are looked up at once at the start) and sums
 // its part of a row; the sums meet in distributed shared memory.  What bounds it:
-// latency for one request (launch, two dependent loads, a row pass), HBM for a
-// batch over a large vocabulary.
+// latency for one request (launch, two dependent loads, a row pass: 8 picked nodes over
+// 32,001 tokens 7.3 us); for a batch over a large vocabulary its passes one after
+// another, 3 us each over 49 MB (48 requests, 2 to 32 drawn nodes, 128,000 f32 29 us; HBM
+// alone 7.5).
 #include <cooperative_groups.h>
 
 #include "pages.cuh"
