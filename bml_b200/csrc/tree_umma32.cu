@@ -40,7 +40,7 @@
 // 75.6 with tree.cu's kernel.
 //
 // 16-bit pages: values are exact in TF32, so V has no lo part (and one chain of P V
-// less: 0.7 us).  K's is kept, zeros but for infinities and NaN, since Q hi * K takes an
+// less: 0.25 us).  K's is kept, zeros but for infinities and NaN, since Q hi * K takes an
 // MMA of 128 columns' time without it too.  K arrives in 16 bits beside its stages, the
 // same split warps widen it.  3 requests of 706 fresh tokens, d = 128, group 4: 163 us,
 // 271 with tree_warp.cu (mma.sync).

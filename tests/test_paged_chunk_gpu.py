@@ -195,6 +195,57 @@ def test_infinities_far_from_the_chunk(cuda, qt, ct):
     assert ((got.double() - want).abs() <= tol(qt, want, ab, bm)).all()
 
 
+@pytest.mark.parametrize("qt,ct", TYPES)
+@pytest.mark.parametrize("n,total", [(1, 128), (1, 129), (8, 64), (8, 65), (9, 64), (1, 256), (1, 257), (30, 256), (30, 257), (1024, 200),
+                                     (1025, 200)])
+def test_between_the_forms_for_few_tokens(cuda, qt, ct, n, total):
+    """Around the sizes where another kernel takes the call: idle requests, a wide
+    one, a refused one; rows behind the last request's stay as they were."""
+    rng = np.random.default_rng(n + total)
+    nodes = [0] * n
+    for i in rng.integers(0, n, total // 2) if n > 1 else []:
+        nodes[int(i)] += 1
+    nodes[n // 2] += total - sum(nodes)
+    c = Paged([int(x) for x in rng.integers(0, 30 if n > 100 else 700, n)], nodes, 8, 2, 64 if n % 2 else 128, 16, qt, ct, seed=n,
+              spare_rows=3)
+    bad = int(np.argmax([0 if i == n // 2 else x for i, x in enumerate(nodes)])) if n > 1 else -1
+    if bad >= 0:
+        c.kv_lens[bad] = 0
+    out = torch.full_like(c.q, 7.0)
+    got = attend(c, out=out)
+    assert got is out and (out[total:] == 7.0).all()
+    check(c, got, sees_of(c), qt, only=[i for i in range(n) if i != bad][::1 if n < 100 else 9] + [n // 2])
+    if bad >= 0:
+        assert (got[int(c.start[bad]):int(c.start[bad]) + nodes[bad]] == 0).all()
+
+
+@pytest.mark.parametrize("qt,ct", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("nodes", [[300, 5], [60, 40], [1, 3]])
+def test_keys_of_minus_infinite_scores(cuda, qt, ct, d, nodes):
+    """An infinite key whose scores are -inf has weight 0 (and no lower term of a split
+    operand makes NaN of it); one whose scores are +inf makes its rows NaN."""
+    inf = float("inf")
+    c = Paged([700, 90], nodes, 8, 2, d, 32, qt, ct, seed=61)
+    c.q[:, :, 3] = -c.q[:, :, 3].abs() - 0.4
+    places = ((0, 17), (0, 640), (1, 89))
+    for i, pos in places:
+        c.k[int(c.table[i, pos // 32]), pos % 32, :, 3] = inf
+        c.ks[i][pos, :, 3] = 0
+    got = attend(c)
+    for i in range(2):
+        see = chain(nodes[i], c.lens[i])
+        for j, pos in places:
+            if i == j:
+                see[:, pos] = False
+        want, ab, bm = c.want(i, see)
+        have = got[int(c.start[i]):int(c.start[i]) + nodes[i]].double()
+        assert torch.isfinite(have).all() and ((have - want).abs() <= tol(qt, want, ab, bm)).all()
+    c.k[int(c.table[0, 0]), 17, 0, 3] = -inf      # scores of the first kv head's rows
+    got = attend(c)[:nodes[0]]
+    assert torch.isnan(got[:, :4]).all() and torch.isfinite(got[:, 4:]).all()
+
+
 def test_offsets_past_32_bits(cuda):
     """Pages at the end of a pool of more than 2^31 elements (4.5 GB)."""
     c = Paged([200, 31], [290, 1], 8, 8, 128, 64, "bf16", "bf16", seed=14)
