@@ -112,7 +112,7 @@ SIGNATURES = {
                                _u32, _vp, _vp, _vp]),
     "bml_attn_chunk_workspace_size": (_st, [_u32, _u32, _u32, _i32, C.POINTER(_sz)]),
     "bml_attn_chunk": (_st, [_vp, C.c_int, _u32, _u32, _u32, _u32, _vp, _vp, C.c_int, _u32, _u32, _vp, _u32, _vp, _vp,
-                             _u32, C.c_float, _vp, _vp, _sz, _vp]),
+                             _u32, C.c_float, _vp, _vp, _sz, _u32, _u32, _vp]),
     "bml_verify_drafts": (_st, [_vp, _vp, C.c_int, _u32, _vp, _vp, _u32, _vp, _u32, _vp, _vp, _u32, _vp, _vp, _vp, _vp]),
     "bml_page_fork": (_st, [_vp, _vp, _u32, _u32, _u32, _u32, _u32, C.c_int, _vp, _vp, _u32, _vp, _vp, _u32, _vp, _u32, _vp,
                             _vp, _u32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),

@@ -27,7 +27,7 @@ constexpr uint32_t kTf32Rows = 80;
 // 16-bit queries those kernels start sooner than chunk_umma.cu (bf16, d = 128, one
 // token behind 1000 positions 11.9 us, 15.3 there; 64 tokens 18.9 and 25.2; d = 64,
 // 8 of one token 9.6 and 16.0; one request of 128 tokens 24.7 and 28.2, d = 64 20.0 and 22.5; but 32 of one token 44.8 and 37.4, 3 of 80 tokens 31.7 and
-// 30.0).
+// 30.0, and 64 tokens of one among 64 idle requests 40.0 and 25.4).
 constexpr uint32_t kFewTokens = 64, kFewSeqs = 8;
 
 struct PieceParams {
@@ -107,9 +107,10 @@ cudaError_t launch_chunk(const TreeArgs &args, int32_t *work, cudaStream_t st) {
     TreeArgs a = args;
     TreeParams &p = a.p;
     const bool umma = chunk_umma_fits(args), tf32_fits = p.q_type == BML_F32 && p.scale_log2 > 0.f && tree_umma_fits(a);
-    const bool few = p.n_seqs <= kFewSeqs;
-    if (umma ? few && p.n_tokens <= (p.n_seqs == 1 ? kTreeMaxNodes / 2 : kFewTokens) && !p.diag : p.n_tokens <= kTreeMaxNodes && p.n_seqs <= kTreeMaxSeqs) {
-        tree_rows(a, p.n_tokens, p.group, p.n_seqs, 0u, few ? p.n_tokens : 0u);
+    const uint32_t live = args.live;
+    if (umma ? p.n_seqs <= kFewSeqs && p.n_tokens <= (p.n_seqs == 1 ? kTreeMaxNodes / 2 : kFewTokens) && !p.diag
+             : p.n_tokens <= kTreeMaxNodes && p.n_seqs <= kTreeMaxSeqs) {
+        tree_rows(a, p.n_tokens, p.group, p.n_seqs, live, a.max_new ? a.max_new : live <= kFewSeqs ? p.n_tokens : 0u);
         return !umma && a.kv_type != BML_F32 && tf32_fits && a.rows >= kTf32Rows ? launch_tree_umma32(a, st) : launch_tree(a, st);
     }
     if (umma) return launch_chunk_umma(args, work, st);
@@ -126,7 +127,8 @@ cudaError_t launch_chunk(const TreeArgs &args, int32_t *work, cudaStream_t st) {
     pp.lens = pp.start + pp.most + 1;
     pp.row_of = pp.lens + pp.most;
     cudaError_t e = launch_after(chunk_pieces_kernel, dim3(1), kThreads, 0, st, pp);
-    tree_rows(a, p.n_tokens, p.group, pp.most, 0u, 0u);
+    // how many pieces have tokens, and the most of one, as far as the caller said it
+    tree_rows(a, p.n_tokens, p.group, pp.most, live + p.n_tokens / pp.width, a.max_new < pp.width ? a.max_new : pp.width);
     const bool tf32 = a.kv_type != BML_F32 && tf32_fits && a.rows >= kTf32Rows;
     for (uint32_t base = 0; base < pp.most && e == cudaSuccess; base += kTreeMaxSeqs) {
         p.n_seqs = pp.most - base < kTreeMaxSeqs ? pp.most - base : kTreeMaxSeqs;

@@ -175,6 +175,7 @@ bml_status attn_tree(const char *fn, bool chunk, const void *q_dev, bml_dtype q_
     bml::TreeParams &p = a.p;
     p.q_type = q_dtype;
     bml::tree_rows(a, n_tokens, n_heads / n_kv_heads, n_seqs, n_live, max_nodes);
+    a.max_new = max_nodes;
     p.q = q_dev;
     p.out = out_dev;
     p.k = k_pool;
@@ -246,10 +247,11 @@ BML_API bml_status bml_attn_chunk(const void *q_dev, bml_dtype q_dtype, uint32_t
                                   uint32_t n_kv_heads, uint32_t head_dim, const void *k_pool, const void *v_pool,
                                   bml_dtype kv_dtype, uint32_t n_pages, uint32_t page_size, const int32_t *block_table,
                                   uint32_t max_pages, const int32_t *kv_lens, const int32_t *node_start, uint32_t n_seqs,
-                                  float scale, void *out_dev, void *workspace, size_t workspace_bytes, void *stream) {
+                                  float scale, void *out_dev, void *workspace, size_t workspace_bytes, uint32_t n_live,
+                                  uint32_t max_new, void *stream) {
     return attn_tree("bml_attn_chunk", true, q_dev, q_dtype, n_tokens, n_heads, n_kv_heads, head_dim, k_pool, v_pool, kv_dtype, n_pages,
                      page_size, block_table, max_pages, kv_lens, node_start, n_seqs, nullptr, 0u, scale, out_dev, workspace,
-                     workspace_bytes, 0u, 0u, bml::kWaitNs, 0u, stream);
+                     workspace_bytes, n_live, max_new, bml::kWaitNs, 0u, stream);
 }
 
 BML_API bml_status bml_diag_attn_chunk(const void *q_dev, bml_dtype q_dtype, uint32_t n_tokens, uint32_t n_heads,

@@ -265,6 +265,8 @@ PyObject *chunk_impl(PyObject *const *a) {
     USUAL(v->sizes() == k->sizes() && k->size(3) == d && start->size(0) == n + 1 && table->size(0) == n && n > 0 && n_tokens > 0 &&
           n < (1ll << 31) && n_tokens < (1ll << 31) && k->size(0) < (1ll << 31) && k->size(1) < (1ll << 31) && table->size(1) < (1ll << 31));
     size_t ws_bytes = 0;
+    int64_t live, most;
+    USUAL(integer(a[7], &live) && integer(a[8], &most));
     USUAL(g_chunk_bytes((uint32_t)d, (uint32_t)n_tokens, (uint32_t)n, dev.index(), &ws_bytes) == BML_OK);
     at::Tensor out = fresh(q->sizes(), q->scalar_type(), dev), ws = fresh({(int64_t)ws_bytes}, at::kByte, dev);
     const bml_status st =
@@ -272,7 +274,7 @@ PyObject *chunk_impl(PyObject *const *a) {
                 (uint32_t)d, k->const_data_ptr(), v->const_data_ptr(), (bml_dtype)code(k->scalar_type()), (uint32_t)k->size(0),
                 (uint32_t)k->size(1), table->const_data_ptr<int32_t>(), (uint32_t)table->size(1), lens->const_data_ptr<int32_t>(),
                 start->const_data_ptr<int32_t>(), (uint32_t)n, (float)PyFloat_AS_DOUBLE(a[6]), out.mutable_data_ptr(),
-                ws.mutable_data_ptr(), ws_bytes, stream_of(dev));
+                ws.mutable_data_ptr(), ws_bytes, (uint32_t)live, (uint32_t)most, stream_of(dev));
     USUAL(st == BML_OK);
     return THPVariable_Wrap(std::move(out));
 }
@@ -464,7 +466,7 @@ PyMethodDef methods[] = {
     ENTRY(append, 9),
     ENTRY(tree, 10),
     ENTRY(commit, 8),
-    ENTRY(chunk, 7),
+    ENTRY(chunk, 9),
     ENTRY(verify, 8),
     ENTRY(fork, 10),
     ENTRY(free, 8),

@@ -50,7 +50,8 @@ struct TreeArgs {
     // Rows of a request and kv head: on average over the requests with new tokens,
     // and of the widest request (as far as the caller knows; else the average).
     uint32_t rows, widest;
-    uint32_t live;  // requests with new tokens, at most
+    uint32_t live;     // requests with new tokens, at most
+    uint32_t max_new;  // new tokens of a request at most, 0: not known (launch_chunk)
     int num_sms;
     // Whether a form with r rows a row group is for the batch: it fits the average,
     // and reads no request's K and V more than four times (32-bit queries over 16-bit

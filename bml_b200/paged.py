@@ -418,16 +418,18 @@ def chunk_workspace_size(head_dim: int, n_tokens: int, n_requests: int, device=N
 
 def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
                     kv_lens: torch.Tensor, node_start: torch.Tensor, scale: float = -1.0,
-                    out: torch.Tensor | None = None, workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+                    out: torch.Tensor | None = None, workspace: torch.Tensor | None = None, stream=None, n_live: int = 0,
+                    max_new: int = 0) -> torch.Tensor:
     """Attention of chunks of new tokens over pages: tree_attention without a
     mask, for any number of new tokens a request -- a prompt or a part of one,
     beside requests that decode one token.  The j-th of request i's T new tokens
     (row node_start[i] + j of q) attends over positions 0 to kv_lens[i] - T + j.
     Types, results, refused requests and rows behind the last request's are
-    tree_attention's.  workspace: an uint8 tensor of chunk_workspace_size bytes
-    for calls that must not allocate; calls that share one must not overlap."""
+    tree_attention's, and so are n_live and max_new.  workspace: an uint8 tensor of
+    chunk_workspace_size bytes for calls that must not allocate; calls that share
+    one must not overlap."""
     if stream is None and out is None and workspace is None:
-        r = (_fast or _load()).chunk(q, k_pool, v_pool, block_table, kv_lens, node_start, scale)
+        r = (_fast or _load()).chunk(q, k_pool, v_pool, block_table, kv_lens, node_start, scale, n_live, max_new)
         if r is not None:
             return r
     a_q = _data(q, "q", 3)
@@ -444,6 +446,8 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     rows, max_pages = block_table.shape
     if rows != n:
         raise ValueError(f"block_table must be [{n}, max_pages], got {tuple(block_table.shape)}")
+    if not (0 <= n_live <= 0x7fffffff and 0 <= max_new <= 0x7fffffff):
+        raise ValueError("n_live and max_new must not be negative")
     ctx = _enter(dev, stream)
     try:
         if out is None:
@@ -456,7 +460,7 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
             _ints(workspace, "workspace", dev, dtype=torch.uint8)
         _call("bml_attn_chunk", a_q, dtype_code(dtype), n_tokens, n_heads, n_kv, d, a_k, a_v, dtype_code(k_pool.dtype),
               n_pages, page_size, a_table, max_pages, a_len, a_start, n, scale, out.data_ptr(), workspace.data_ptr(),
-              workspace.shape[0], _raw_stream(dev.index))
+              workspace.shape[0], n_live, max_new, _raw_stream(dev.index))
     finally:
         if ctx is not None:
             ctx.__exit__(None, None, None)
@@ -847,7 +851,7 @@ class PagedBatcher:
                      theta=self.theta, stream=stream)
         if self._most > MAX_NODES:
             return chunk_attention(q, self.k[layer], self.v[layer], self.table, p.kv_lens, p.node_start, scale=self.scale,
-                                   out=out, stream=stream)
+                                   out=out, stream=stream, n_live=self._live, max_new=self._most)
         return tree_attention(q, self.k[layer], self.v[layer], self.table, p.kv_lens, p.node_start, mask=p.mask,
                               scale=self.scale, out=out, stream=stream, n_live=self._live, max_new=self._most)
 

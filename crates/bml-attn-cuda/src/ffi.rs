@@ -119,7 +119,7 @@ extern "C" {
                           head_dim: u32, k_pool: *const c_void, v_pool: *const c_void, kv: bml_dtype, n_pages: u32,
                           page_size: u32, block_table: *const i32, max_pages: u32, kv_lens: *const i32,
                           node_start: *const i32, n_seqs: u32, scale: f32, out: *mut c_void, ws: *mut c_void,
-                          ws_bytes: usize, stream: *mut c_void) -> bml_status;
+                          ws_bytes: usize, n_live: u32, max_new: u32, stream: *mut c_void) -> bml_status;
     pub fn bml_verify_drafts(target: *const c_void, draft: *const c_void, dtype: bml_dtype, vocab: u32,
                              tokens: *const i32, parents: *const i32, n_tokens: u32, node_start: *const i32, n: u32,
                              u: *const f32, u_next: *const f32, max_path: u32, path: *mut i32, n_accept: *mut i32,

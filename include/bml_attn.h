@@ -545,8 +545,10 @@ bml_status bml_attn_chunk_workspace_size(uint32_t head_dim, uint32_t n_tokens,
  * Types, layouts, refused requests, masked places, infinities, precision and the
  * limit of waits are bml_attn_tree's; workspace: bml_attn_chunk_workspace_size
  * bytes, 16-byte aligned, no contents needed, not shared by calls that overlap
- * in time.  Up to 256 tokens a request, where most have few, bml_attn_tree_sized
- * is the faster call.  head_dim 64 or 128.  Asynchronous. */
+ * in time.  n_live, max_new: as bml_attn_tree_sized's n_live and max_nodes, 0 where
+ * not known; the choice of a kernel goes by them.  Up to 256 tokens a request, where
+ * most have few, bml_attn_tree_sized is the faster call.  head_dim 64 or 128.
+ * Asynchronous. */
 bml_status bml_attn_chunk(const void *q_dev, bml_dtype q_dtype,
                           uint32_t n_tokens, uint32_t n_heads,
                           uint32_t n_kv_heads, uint32_t head_dim,
@@ -556,7 +558,8 @@ bml_status bml_attn_chunk(const void *q_dev, bml_dtype q_dtype,
                           uint32_t max_pages, const int32_t *kv_lens,
                           const int32_t *node_start, uint32_t n_seqs,
                           float scale, void *out_dev, void *workspace,
-                          size_t workspace_bytes, void *stream);
+                          size_t workspace_bytes, uint32_t n_live,
+                          uint32_t max_new, void *stream);
 
 /* Verification of drafted tokens: which path of each request's draft is kept,
  * and the token that follows it, so that tokens are distributed as the target

@@ -220,6 +220,19 @@ def test_between_the_forms_for_few_tokens(cuda, qt, ct, n, total):
 
 
 @pytest.mark.parametrize("qt,ct", TYPES)
+@pytest.mark.parametrize("nodes", [[0] * 40 + [400], [1] * 30 + [90], [0] * 60 + [70, 1]])
+def test_what_the_caller_says_of_the_batch(cuda, qt, ct, nodes):
+    """n_live and max_new, right or wrong, change the kernel and not the result."""
+    c = Paged([300] * (len(nodes) - 1) + [900], nodes, 8, 2, 128, 32, qt, ct, seed=71)
+    for live, most in ((0, 0), (sum(x > 0 for x in nodes), max(nodes)), (1, 1), (len(nodes) + 5, 0), (2, 1 << 30), (1, 0)):
+        for kw in ({}, {"out": torch.empty_like(c.q)}):
+            check(c, attend(c, n_live=live, max_new=most, **kw), sees_of(c), qt)
+    for bad in ({"n_live": -1}, {"max_new": 1 << 31}):
+        with pytest.raises(ValueError):
+            attend(c, **bad)
+
+
+@pytest.mark.parametrize("qt,ct", TYPES)
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("nodes", [[300, 5], [60, 40], [1, 3]])
 def test_keys_of_minus_infinite_scores(cuda, qt, ct, d, nodes):

@@ -28,8 +28,8 @@ def caller(fn, order, arrays, **rest):
 
 
 chunk = caller("bml_attn_chunk", "q qt n_tokens n_heads n_kv d k v kt n_pages page table max_pages kv_lens start n scale out ws "
-               "ws_bytes stream", ("q", "k", "v", "table", "kv_lens", "start", "out", "ws"), qt=2, n_tokens=4, n_heads=4, n_kv=2,
-               d=64, kt=2, n_pages=4, page=16, max_pages=8, n=2, scale=-1.0, ws_bytes=1 << 40)
+               "ws_bytes live most stream", ("q", "k", "v", "table", "kv_lens", "start", "out", "ws"), qt=2, n_tokens=4, n_heads=4, n_kv=2,
+               d=64, kt=2, n_pages=4, page=16, max_pages=8, n=2, scale=-1.0, ws_bytes=1 << 40, live=0, most=0)
 verify = caller("bml_verify_drafts", "p q dt vocab tok par n_tokens start n u un max_path path count next stream",
                 ("p", "q", "tok", "par", "start", "u", "un", "path", "count", "next"), dt=0, vocab=100, n_tokens=6, n=2, max_path=4)
 fork = caller("bml_page_fork", "k v layers n_pages page n_kv d dt src dst m lens owned n table max_pages shared free n_free used lens2 "
