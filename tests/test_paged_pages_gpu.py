@@ -458,3 +458,62 @@ def test_compact_at_the_edges_of_its_forms(cuda, n_pages, n, max_pages, held):
                                                       (2048, 9, 1024, 1100), (2047, 1, 8192, 700)])
 def test_compact_between_its_forms(cuda, n_pages, n, max_pages, held):
     test_compact_at_the_edges_of_its_forms(None, n_pages, n, max_pages, held)
+
+
+def test_long_forms_at_once_and_replayed(cuda, monkeypatch):
+    """page_free over all SMs and page_compact of a large pool: on two streams at once,
+    in a replayed graph and through ctypes, the same bits."""
+    import bml_b200.paged as P
+    rng = np.random.default_rng(9)
+    s = State([int(x) for x in rng.integers(100, 900, 700)], 16, spare=20000, seed=9)
+    keep = ints([int(rng.choice([-1, 0, a // 2 // 16 * 16])) for a in s.lens])
+    a = [keep, ints(s.lens), ints(s.owned), ints(s.table), 16, ints(s.shared), ints(s.free), ints([s.used])]
+    pools = [torch.randn(1, s.n_pages, 16, 1, 2, device="cuda") for _ in "kv"]
+
+    def both(k, v, **kw):
+        r = P.page_free(*a, **kw)
+        c = P.page_compact(k, v, r.owned, a[3], r.shared, **kw)
+        return [r.lens, r.owned, r.shared, r.free_pages, r.free_used, r.status, c.block_table, c.shared, c.free_pages, c.free_used, k, v]
+
+    def fresh():
+        return [p.clone() for p in pools]
+
+    want = both(*fresh())
+    assert int(want[4]) < s.used < s.n_pages and int(want[9]) == int(want[4])
+    xs, st = [fresh() for _ in range(8)], [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [both(*x, stream=st[i & 1]) for i, x in enumerate(xs)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, w) for g in got for x, w in zip(g, want))
+    x, start = fresh(), fresh()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = both(*x)
+    for _ in range(3):
+        for y, z in zip(x, start):
+            y.copy_(z)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, w) for y, w in zip(got, want))
+    monkeypatch.setattr(P, "_fast", P._Wrappers)
+    assert all(torch.equal(y, w) for y, w in zip(both(*fresh()), want))
+
+
+def test_pools_past_32_bits(cuda):
+    """Pages whose bytes lie 4 GiB and more behind the pools' start."""
+    import bml_b200
+    n_pages = 70001
+    k, v = (torch.empty(2, n_pages, 16, 8, 128, dtype=torch.bfloat16, device="cuda") for _ in "kv")   # 4.6 GB each
+    src = torch.randn(2, 2, 16, 8, 128, device="cuda").bfloat16()
+    for p, x in ((k, src), (v, -src)):
+        p[:, n_pages - 1], p[:, 40000] = x[0], x[1]
+    table = ints([[n_pages - 1, -1], [-1, -1]])
+    f = bml_b200.page_fork(k, v, ints([0]), ints([1]), ints([9, 0]), ints([1, 0]), table, ints([0] * n_pages),
+                           ints([n_pages - 1, n_pages - 2]), ints([1]))
+    assert f.status.tolist() == [0] and table.tolist() == [[n_pages - 1, -1], [n_pages - 2, -1]]
+    for p, x in ((k, src), (v, -src)):
+        assert torch.equal(p[:, n_pages - 2, :9], x[0][:, :9])
+    c = bml_b200.page_compact(k, v, ints([2, 1]), ints([[n_pages - 1, 40000], [n_pages - 2, 7]]), ints([0] * n_pages))
+    assert c.block_table.tolist() == [[2, 0], [1, 7]] and c.free_used.tolist() == [3]
+    for p, x in ((k, src), (v, -src)):
+        assert torch.equal(p[:, 2], x[0]) and torch.equal(p[:, 0], x[1]) and torch.equal(p[:, 1, :9], x[0][:, :9])
