@@ -402,6 +402,11 @@ def test_stalled_copies_leave_nan(cuda, qt, ct, heads, nodes, d):
     check(c, out, sees_of(c), qt, only=[0, 1, 33, 59])
 
 
+@pytest.mark.parametrize("ct,d", [("bf16", 128), ("f16", 64)])
+def test_stalled_copies_of_16_bit_pages_under_32_bit_queries(cuda, ct, d):
+    test_stalled_copies_leave_nan(None, "f32", ct, 16, [40, 300], d)
+
+
 @pytest.mark.parametrize("qt,ct", [("bf16", "bf16"), ("f32", "f16")])
 def test_batcher_takes_prompts_in_chunks(cuda, qt, ct):
     """A prompt that comes in chunks beside decoding requests: rows in the cache and
