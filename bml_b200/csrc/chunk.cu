@@ -35,7 +35,8 @@ struct PieceParams {
     uint32_t n, n_tokens, width, most;    // width: tokens of a piece; most: pieces
     uint64_t room;                        // positions of a row of the block table
     int32_t *first;                       // [n + 1]: a request's first piece
-    int32_t *start, *lens, *row_of;       // [most + 1], [most], [most]: the pieces
+    int32_t *start, *end, *lens, *row_of;  // [most] each: the pieces.  An end of its own: behind
+                                           // a request there may be rows that nobody computes
 };
 
 // One CTA: pieces of each request, their prefix sums, then a piece a thread.
@@ -69,9 +70,8 @@ __global__ void __launch_bounds__(kThreads) chunk_pieces_kernel(const PieceParam
     }
     if (threadIdx.x == 0) p.first[p.n] = (int32_t)base;
     __syncthreads();
-    const int32_t end = min(max(p.node_start[p.n], 0), (int32_t)p.n_tokens);
-    for (uint32_t v = threadIdx.x; v <= p.most; v += kThreads) {
-        int32_t start = end, len = 0;
+    for (uint32_t v = threadIdx.x; v < p.most; v += kThreads) {
+        int32_t start = 0, end = 0, len = 0;
         uint32_t row = 0;
         if (v < base) {
             uint32_t lo = 0, hi = p.n;  // the last request whose first piece is at most v
@@ -84,14 +84,14 @@ __global__ void __launch_bounds__(kThreads) chunk_pieces_kernel(const PieceParam
             const int32_t L = p.kv_lens[lo];
             row = lo;
             start = p.node_start[lo] + (int32_t)min(k, T);
+            end = p.node_start[lo] + (int32_t)min(k + p.width, T);
             // a refused request, or one whose positions its row does not hold: none
             if (L >= (int32_t)T && (uint64_t)L <= p.room) len = L - (int32_t)T + (int32_t)min(k + p.width, T);
         }
         p.start[v] = start;
-        if (v < p.most) {
-            p.lens[v] = len;
-            p.row_of[v] = (int32_t)row;
-        }
+        p.end[v] = end;
+        p.lens[v] = len;
+        p.row_of[v] = (int32_t)row;
     }
 }
 
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kThreads) chunk_pieces_kernel(const PieceParam
 
 size_t chunk_work_bytes(uint64_t n_tokens, uint64_t n_seqs, int num_sms) {
     // pieces of one token at the least (groups of more than 128 q heads)
-    const size_t pieces = (3 * (n_tokens + n_seqs) + n_seqs + 2) * sizeof(int32_t), cuts = chunk_umma_bytes(n_tokens, num_sms);
+    const size_t pieces = (4 * (n_tokens + n_seqs) + n_seqs + 1) * sizeof(int32_t), cuts = chunk_umma_bytes(n_tokens, num_sms);
     return pieces > cuts ? pieces : cuts;
 }
 
@@ -124,7 +124,8 @@ cudaError_t launch_chunk(const TreeArgs &args, int32_t *work, cudaStream_t st) {
     pp.room = (uint64_t)p.max_pages << p.page_shift;
     pp.first = work;
     pp.start = pp.first + p.n_seqs + 1;
-    pp.lens = pp.start + pp.most + 1;
+    pp.end = pp.start + pp.most;
+    pp.lens = pp.end + pp.most;
     pp.row_of = pp.lens + pp.most;
     cudaError_t e = launch_after(chunk_pieces_kernel, dim3(1), kThreads, 0, st, pp);
     // how many pieces have tokens, and the most of one, as far as the caller said it
@@ -133,6 +134,7 @@ cudaError_t launch_chunk(const TreeArgs &args, int32_t *work, cudaStream_t st) {
     for (uint32_t base = 0; base < pp.most && e == cudaSuccess; base += kTreeMaxSeqs) {
         p.n_seqs = pp.most - base < kTreeMaxSeqs ? pp.most - base : kTreeMaxSeqs;
         p.node_start = pp.start + base;
+        p.node_end = pp.end + base;
         p.kv_lens = pp.lens + base;
         p.row_of = pp.row_of + base;
         e = tf32 ? launch_tree_umma32(a, st) : launch_tree(a, st);

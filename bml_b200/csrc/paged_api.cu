@@ -181,6 +181,7 @@ bml_status attn_tree(const char *fn, bool chunk, const void *q_dev, bml_dtype q_
     p.k = k_pool;
     p.v = v_pool;
     p.node_start = node_start;
+    p.node_end = node_start + 1;
     p.mask = mask;
     p.n_tokens = n_tokens;
     p.n_heads = n_heads;
@@ -207,6 +208,7 @@ bml_status attn_tree(const char *fn, bool chunk, const void *q_dev, bml_dtype q_
         p.table = block_table + (size_t)base * max_pages;
         p.kv_lens = kv_lens + base;
         p.node_start = node_start + base;
+        p.node_end = p.node_start + 1;
         const cudaError_t e = bml::launch_tree(a, static_cast<cudaStream_t>(stream));
         if (e != cudaSuccess) return bml::api_cuda_fail(e, fn);
     }

@@ -19,7 +19,7 @@ struct TreeParams {
     void *out;      // same shape and type
     const void *k, *v;  // pools [n_pages][page][n_kv][D]
     const int32_t *table;  // [n_seqs][max_pages]
-    const int32_t *kv_lens, *node_start;
+    const int32_t *kv_lens, *node_start, *node_end;  // rows [node_start[i], node_end[i]): node_start + 1, or a piece's own end
     const int32_t *row_of;  // [n_seqs]: a request's row of table (pieces of a chunk share one); null: its own index
     const uint64_t *mask;  // [n_tokens][n_words] or null: node t sees nodes 0..t
     uint32_t n_seqs, n_tokens, n_heads, n_kv, group, max_pages, n_pages, page_shift, n_words;
@@ -162,8 +162,8 @@ struct TreeRaw {
 // kEarly: before griddepcontrol.wait (the merge, which reads past L1).
 template <bool kEarly>
 __device__ __forceinline__ TreeRaw tree_raw(const TreeParams &p, uint32_t i) {
-    if (kEarly) return {__ldcg(p.node_start + i), __ldcg(p.node_start + i + 1), __ldcg(p.kv_lens + i)};
-    return {p.node_start[i], p.node_start[i + 1], p.kv_lens[i]};
+    if (kEarly) return {__ldcg(p.node_start + i), __ldcg(p.node_end + i), __ldcg(p.kv_lens + i)};
+    return {p.node_start[i], p.node_end[i], p.kv_lens[i]};
 }
 template <bool kW>
 __device__ __forceinline__ TreeSeq tree_seq(const TreeParams &p, const TreeRaw &raw) {

@@ -136,6 +136,30 @@ def test_refused_requests_and_bad_pages(cuda, qt, ct, d):
 
 
 @pytest.mark.parametrize("qt,ct", TYPES)
+@pytest.mark.parametrize("heads,kv,d", [(8, 2, 64), (2, 2, 128), (3, 1, 64)])
+@pytest.mark.parametrize("start,rows", [([0, 300, 700], 600), ([0, 300, 310], 305), ([0, 300, 301], 300), ([0, 300, 200], 320),
+                                        ([0, 300, 1 << 30], 513), ([0, 300, -7], 500), ([0, 300, 900, 340], 600),
+                                        ([-3, 60, 360], 400), ([700, 100, 400], 700), ([0, 300, 650, 600, 900], 888)])
+def test_neighbours_of_requests_whose_rows_are_none(cuda, qt, ct, heads, kv, d, start, rows):
+    """A request whose rows leave the token rows, or that begins behind its end, is
+    not served; the requests beside it are, each to its own end, and rows that no
+    request holds stay as they were."""
+    n = len(start) - 1
+    good = [i for i in range(n) if 0 <= start[i] < start[i + 1] <= rows]
+    nodes = [start[i + 1] - start[i] if i in good else 5 for i in range(n)]
+    lens = [90, 20, 7, 500][:n]
+    c = Paged(lens, nodes, heads, kv, d, 32, qt, ct, seed=rows, spare_rows=rows - sum(nodes))
+    c.start = ints(start)
+    out = torch.full_like(c.q, 7.0)
+    got = attend(c, out=out)
+    check(c, got, sees_of(c), qt, only=good)
+    idle = torch.ones(rows, dtype=torch.bool)
+    for i in good:
+        idle[start[i]:start[i + 1]] = False
+    assert (got[idle.cuda()] == 7).all()
+
+
+@pytest.mark.parametrize("qt,ct", TYPES)
 @pytest.mark.parametrize("d", [64, 128])
 def test_later_tokens_do_not_reach_a_row(cuda, qt, ct, d):
     """NaN, infinities and the largest values in K and V of a chunk's later tokens,
