@@ -486,7 +486,8 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
     q(x)), r the target's probabilities at first and norm(max(r - q, 0)) after
     each rejection; if none is, the next token is drawn from r.  A path of
     max_path nodes ends there.  A request without nodes, or with more than 256,
-    has n_accept 0 and next -1.  include/bml_attn.h has the formulas."""
+    has n_accept 0 and next -1; one that page_plan refused is walked like any other
+    (look at its status).  include/bml_attn.h has the formulas."""
     if stream is None:
         r = (_fast or _load()).verify(target, draft, tokens, parents, node_start, u, u_next, max_path)
         if r is not None:
@@ -688,7 +689,8 @@ class PagedBatcher:
         self.free, self.used = torch.arange(n_pages, **i32), torch.zeros(1, **i32)
         self.shared = torch.zeros(n_pages, **i32)  # holders of a page beyond the first
         self._rows: dict = {}    # request -> its row of the tables
-        self._plan = None        # of the step that has begun
+        self._plan = None        # of the step that has begun,
+        self._checked = True     # and whether it refused nobody, as far as the host knows
         self._new = None         # new tokens of each row (host),
         self._live = self._most = 0  # how many rows have some, the most of one
         self._parents = []       # of the step's tokens (host)
@@ -833,7 +835,7 @@ class PagedBatcher:
         plan = self._planned(new)
         if check:
             plan.check()
-        self._plan = plan
+        self._plan, self._checked = plan, check
         return plan
 
     def step(self, layer: int, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
@@ -882,7 +884,8 @@ class PagedBatcher:
         request is its pending one, the others hang below it.  target, draft
         [n_tokens, vocab], tokens int32, u f32 [n_tokens]: by token row; u_next f32
         [max_requests]: by the requests' places.  Returns path, n_accept and the
-        next tokens, by place (place(rid)); idle places have n_accept 0, next -1."""
+        next tokens, by place (place(rid)); idle places, and requests that a plan
+        begun without check refused, have n_accept 0 and next -1."""
         if self._plan is None:
             raise RuntimeError("no step has begun")
         p, most = self._plan, max(1, self._most)
@@ -892,6 +895,11 @@ class PagedBatcher:
         path, count, token = verify_drafts(target, draft, tokens,
                                            torch.tensor(parents, dtype=torch.int32, device=self.device), p.node_start, u,
                                            u_next, max_path=most)
+        if not self._checked:  # a refused request has token rows, but attention left them zero
+            refused = p.status != 0
+            path.masked_fill_(refused[:, None], -1)
+            count.masked_fill_(refused, 0)
+            token.masked_fill_(refused, -1)
         self.lens = paged_commit(self.k, self.v, self.table, self.lens, p.kv_lens, p.node_start, path, count)
         self.owned, self.used = p.owned, p.free_used
         self._plan = None

@@ -587,8 +587,11 @@ bml_status bml_attn_chunk(const void *q_dev, bml_dtype q_dtype,
  * (no distribution), it is vocab - 1.  Sums are f64.  A path of max_path nodes ends there, its last
  * node's children untried.  Probabilities that are not positive finite numbers
  * count as 0; a child whose token is outside [0, vocab) is never tried.  A request
- * without nodes, or with more than 256, has n_accept 0 and next -1.  target and
- * draft are of one type, rows need no alignment beyond it.  Asynchronous. */
+ * without nodes, or with more than 256, has n_accept 0 and next -1.  A request
+ * that bml_paged_plan refused is walked like any other, though its attention was
+ * zero: bml_paged_commit keeps nothing of it, and its results here mean nothing.
+ * target and draft are of one type, rows need no alignment beyond it.
+ * Asynchronous. */
 bml_status bml_verify_drafts(const void *target, const void *draft,
                              bml_dtype dtype, uint32_t vocab,
                              const int32_t *tokens, const int32_t *parents,

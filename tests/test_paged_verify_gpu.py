@@ -383,3 +383,43 @@ def test_batcher_verifies(cuda, kind):
                     assert torch.equal(g, w)
     with pytest.raises(RuntimeError):
         made[0].verify(x["p"].cuda(), None, ints(x["tokens"]), x["u"].cuda(), un)
+
+
+@pytest.mark.parametrize("kind", ["tree", "chain"])
+def test_batcher_verifies_beside_a_refused_request(cuda, kind):
+    """A plan begun without check that refuses a request, for want of pages or of
+    places in its table: the request keeps nothing and gets no next token, the
+    others get the walk's, and a later step goes on from there."""
+    import bml_b200
+    b = bml_b200.PagedBatcher(1, 4, 2, 64, n_pages=5, page_size=16, max_positions=48, max_requests=6, rope=False)
+    row = lambda n, kv: torch.randn(n, kv, 64, device="cuda").bfloat16()  # noqa: E731
+    for r, t in zip("abcd", (30, 15, 2, 0)):             # 2 + 1 + 1 pages of 5
+        b.add(r, row(t, 2)[None], row(t, 2)[None])
+    nodes = {"a": 12, "b": 4, "c": 20, "d": 60}          # a third page for a, a second for b and c; d's table has 48 places
+    before = {r: b.length(r) for r in "abcd"}
+    n = sum(nodes.values())
+    x = batch(list(nodes.values()), 61, "f32", True, 3, sharp=0.5)
+    if kind == "chain":
+        x["parents"] = [a - 1 for t in nodes.values() for a in range(t)]
+    at, new = 0, {}
+    for r, t in nodes.items():
+        new[r] = t if kind == "chain" else x["parents"][at:at + t]
+        at += t
+    plan = b.begin(new, check=False)
+    status = plan.status.tolist()
+    assert status[:4] == [0, 1, 1, 2], status            # the page that is left is a's
+    b.step(0, row(n, 4), row(n, 2), row(n, 2))
+    un = torch.rand(6, device="cuda")
+    path, count, token = b.verify(x["p"].cuda(), x["q"].cuda(), ints(x["tokens"]), x["u"].cuda(), un)
+    want, nxt = walk(x["p"][:12].double().numpy(), x["q"][:12].double().numpy(), x["tokens"][:12], x["parents"][:12], x["u"][:12].numpy(),
+                     float(un[0]), 256)
+    assert count.tolist() == [len(want), 0, 0, 0, 0, 0] and token.tolist() == [nxt, -1, -1, -1, -1, -1]
+    assert path[0, :len(want)].tolist() == want and (path[0, len(want):] == -1).all() and (path[1:] == -1).all()
+    assert [b.length(r) for r in "abcd"] == [before["a"] + len(want), before["b"], before["c"], before["d"]]
+    # a checked step afterwards keeps everything
+    x = batch([1, 1], 61, "f32", True, 4)
+    b.begin({"b": 1, "c": 1})
+    b.step(0, row(2, 4), row(2, 2), row(2, 2))
+    path, count, token = b.verify(x["p"].cuda(), None, ints(x["tokens"]), x["u"].cuda(), un)
+    assert count.tolist() == [0, 1, 1, 0, 0, 0] and (token[1:3] >= 0).all()
+    assert [b.length(r) for r in "bc"] == [before["b"] + 1, before["c"] + 1]
