@@ -652,6 +652,16 @@ def page_compact(k_pools: torch.Tensor, v_pools: torch.Tensor, owned: torch.Tens
     return PageUpdate(None, None, out[0], out[1], out[2], table)
 
 
+def _on(device, values) -> torch.Tensor:
+    """int32 values of the host on the device, without waiting for the GPU as a copy
+    from pageable memory does.  Torch's allocator keeps the pinned block until the
+    copy has been made; only memory that it has to pin anew waits.  A graph would
+    replay the copy from a block that holds something else by then."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a PagedBatcher's host state cannot be captured: plan, commit and remove outside the graph")
+    return torch.tensor(values, dtype=torch.int32, pin_memory=True).to(device, non_blocking=True)
+
+
 class PagedBatcher:
     """DecodeBatcher over a paged cache, with drafts: requests join and leave
     between steps, a step brings each request any number of new tokens -- one
@@ -747,7 +757,7 @@ class PagedBatcher:
     def _keep(self, rows: dict, check: bool) -> None:
         """Releases what the given rows hold behind so many positions."""
         keep = [rows.get(r, -1) for r in range(self.max_requests)]
-        p = page_free(torch.tensor(keep, dtype=torch.int32, device=self.device), self.lens, self.owned, self.table,
+        p = page_free(_on(self.device, keep), self.lens, self.owned, self.table,
                       self.page_size, self.shared, self.free, self.used)
         if check:
             p.check()
@@ -755,9 +765,11 @@ class PagedBatcher:
         self.free, self.used = p.free_pages, p.free_used
 
     def remove(self, rid) -> None:
-        """Drops a request and returns the pages that no other one shares."""
+        """Drops a request and returns the pages that no other one shares, without
+        waiting for the GPU."""
         self._between_steps()
-        self._keep({self._rows.pop(rid): 0}, False)
+        self._keep({self._rows[rid]: 0}, False)
+        del self._rows[rid]
 
     def truncate(self, rid, n: int) -> None:
         """Rolls a request back to its first n positions.  PageRefused where that
@@ -782,8 +794,7 @@ class PagedBatcher:
         if not new:
             return
         free = sorted(set(range(self.max_requests)) - set(self._rows.values()))[:len(new)]
-        i32 = dict(dtype=torch.int32, device=self.device)
-        p = page_fork(self.k, self.v, torch.tensor([row] * len(new), **i32), torch.tensor(free, **i32), self.lens, self.owned,
+        p = page_fork(self.k, self.v, _on(self.device, [row] * len(new)), _on(self.device, free), self.lens, self.owned,
                       self.table, self.shared, self.free, self.used)
         p.check()
         self.lens, self.owned, self.shared, self.used = p.lens, p.owned, p.shared, p.free_used
@@ -812,9 +823,8 @@ class PagedBatcher:
             raise ValueError(f"{most} drafted tokens for a request (at most {MAX_NODES})")
         dev = self.device
         self._new, self._live, self._most, self._parents = counts, sum(x > 0 for x in counts), most, parents
-        return page_plan(self.lens, torch.tensor(counts, dtype=torch.int32, device=dev), self.owned, self.table,
-                         self.free, self.used, self.page_size, sum(counts),
-                         torch.tensor(parents, dtype=torch.int32, device=dev) if tree else None,
+        return page_plan(self.lens, _on(dev, counts), self.owned, self.table, self.free, self.used, self.page_size,
+                         sum(counts), _on(dev, parents) if tree else None,
                          n_words=max(1, -(-most // 64)) if tree else 1)
 
     def begin(self, new: dict, check: bool = True, chunks: bool = False) -> PagePlan:
@@ -871,8 +881,7 @@ class PagedBatcher:
         full = [want.get(r, list(range(t))) for r, t in enumerate(self._new)]
         wide = max(1, max(len(x) for x in full))
         dev = self.device
-        path = torch.tensor([x + [0] * (wide - len(x)) for x in full], dtype=torch.int32, device=dev)
-        count = torch.tensor([len(x) for x in full], dtype=torch.int32, device=dev)
+        path, count = _on(dev, [x + [0] * (wide - len(x)) for x in full]), _on(dev, [len(x) for x in full])
         self.lens = paged_commit(self.k, self.v, self.table, self.lens, p.kv_lens, p.node_start, path, count)
         self.owned, self.used = p.owned, p.free_used
         self._plan = None
@@ -892,9 +901,8 @@ class PagedBatcher:
         if most > MAX_NODES:
             raise ValueError(f"{most} tokens for a request (at most {MAX_NODES} can be verified)")
         parents = self._parents if p.mask is not None else [a - 1 for t in self._new for a in range(t)]
-        path, count, token = verify_drafts(target, draft, tokens,
-                                           torch.tensor(parents, dtype=torch.int32, device=self.device), p.node_start, u,
-                                           u_next, max_path=most)
+        path, count, token = verify_drafts(target, draft, tokens, _on(self.device, parents), p.node_start, u, u_next,
+                                           max_path=most)
         if not self._checked:  # a refused request has token rows, but attention left them zero
             refused = p.status != 0
             path.masked_fill_(refused[:, None], -1)

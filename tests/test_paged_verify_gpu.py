@@ -423,3 +423,82 @@ def test_batcher_verifies_beside_a_refused_request(cuda, kind):
     path, count, token = b.verify(x["p"].cuda(), None, ints(x["tokens"]), x["u"].cuda(), un)
     assert count.tolist() == [0, 1, 1, 0, 0, 0] and (token[1:3] >= 0).all()
     assert [b.length(r) for r in "bc"] == [before["b"] + 1, before["c"] + 1]
+
+
+def test_a_step_and_a_removal_do_not_wait(cuda):
+    """begin(check=False), step, verify, commit, remove and compact make no call that
+    waits for the GPU, and the lists that the host hands over may go at once.  A
+    round before loads the kernels, and more memory is pinned than the round takes,
+    since pinning waits."""
+    import bml_b200
+    b = bml_b200.PagedBatcher(1, 4, 2, 64, n_pages=40, page_size=16, max_positions=128, max_requests=4, rope=False)
+    for r in "abc":
+        b.add(r)
+    n = 14
+    x = batch([9, 5], 61, "f32", True, 5)
+    p, u, un, tokens = x["p"].cuda(), x["u"].cuda(), torch.rand(4, device="cuda"), ints(x["tokens"])
+    q, k = torch.randn(n, 4, 64, device="cuda").bfloat16(), torch.randn(n, 2, 64, device="cuda").bfloat16()
+    junk = []
+
+    def steps():
+        for kind in ("verify", "commit"):
+            b.begin({"a": x["parents"][:9], "b": x["parents"][9:]}, check=False)
+            b.step(0, q, k, k)
+            if kind == "verify":
+                got = b.verify(p, None, tokens, u, un)
+            else:
+                b.commit({"a": [0, 2, 5], "b": []})
+            junk.extend(torch.full((size,), -7, dtype=torch.int32, pin_memory=True) for size in (2, 4, 5, 9, 14, 16))
+        b.remove("c")
+        b.compact()
+        return got
+
+    steps()
+    junk.extend(torch.empty(size, dtype=torch.int32, pin_memory=True) for size in (2, 4, 8, 16, 32) for _ in range(40))
+    del junk[:]
+    b.add("c")
+    for r in "ab":
+        b.truncate(r, 0)
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        torch.cuda._sleep(1_000_000_000)                 # the copies lie behind half a second of work
+        path, count, token = steps()
+        busy = not torch.cuda.current_stream().query()
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert busy
+    want = [walk(x["p"][s].double().numpy(), None, x["tokens"][s], x["parents"][s], x["u"][s].numpy(), float(un[i]), 256)
+            for i, s in enumerate((slice(0, 9), slice(9, 14)))]
+    assert count.tolist() == [len(want[0][0]), len(want[1][0]), 0, 0] and token.tolist() == [want[0][1], want[1][1], -1, -1]
+    assert b.length("a") == len(want[0][0]) + 3 and b.length("b") == len(want[1][0])
+    assert b.active == ["a", "b"] and int(b.used) == int(b.owned.sum())
+
+
+def test_a_batchers_host_state_is_not_captured(cuda):
+    """The lists of a plan, a commit or a removal lie in host memory that is used again:
+    such a call in a graph is refused and changes nothing; the layers' calls may be captured."""
+    import bml_b200
+    b = bml_b200.PagedBatcher(1, 4, 2, 64, n_pages=8, page_size=16, max_positions=64, max_requests=2, rope=False)
+    b.add("a")
+    q, k = torch.randn(2, 4, 64, device="cuda").bfloat16(), torch.randn(2, 2, 64, device="cuda").bfloat16()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        for call in (lambda: b.begin({"a": 2}, check=False), lambda: b.remove("a"), lambda: b.fork("a", "b")):
+            with pytest.raises(RuntimeError, match="captured"):
+                call()
+        junk = q + 1                                     # a graph that holds something
+    assert b.active == ["a"]
+    b.begin({"a": 2})
+    b.step(0, q, k, k)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = b.step(0, q, k, k)
+        with pytest.raises(RuntimeError, match="captured"):
+            b.commit()
+    g.replay()
+    want = b.step(0, q, k, k)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    b.commit()
+    assert b.length("a") == 2
+    del g, junk
