@@ -785,7 +785,7 @@ class PagedBatcher:
         where the pool has no page for that; then none is admitted.  Waits for
         the GPU."""
         self._between_steps()
-        new = list(new) if isinstance(new, (list, tuple)) else [new]
+        new = list(new) if isinstance(new, list) else [new]  # (a tuple may be a request's name, as in add)
         row = self._rows[rid]
         if len(set(new)) < len(new) or any(r in self._rows for r in new):
             raise KeyError(f"requests {new!r}: one is already active, or named twice")

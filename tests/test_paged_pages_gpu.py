@@ -517,3 +517,19 @@ def test_pools_past_32_bits(cuda):
     assert c.block_table.tolist() == [[2, 0], [1, 7]] and c.free_used.tolist() == [3]
     for p, x in ((k, src), (v, -src)):
         assert torch.equal(p[:, 2], x[0]) and torch.equal(p[:, 0], x[1]) and torch.equal(p[:, 1, :9], x[0][:, :9])
+
+
+def test_a_tuple_names_one_request(cuda):
+    """A request's name may be anything that a dictionary takes, in fork as in add."""
+    import bml_b200
+    b = bml_b200.PagedBatcher(1, 4, 2, 64, n_pages=8, page_size=16, max_positions=64, max_requests=4, rope=False)
+    x = torch.randn(1, 20, 2, 64, device="cuda").bfloat16()
+    b.add(("user", 1), x, x)
+    b.fork(("user", 1), ("user", 2))
+    assert b.active == [("user", 1), ("user", 2)]
+    b.fork(("user", 2), [("user", 3), "c"])
+    assert b.active == [("user", 1), ("user", 2), ("user", 3), "c"]
+    for rid in b.active:
+        assert all(torch.equal(y, x[0]) for y in b.cache(rid, 0))
+    with pytest.raises(KeyError):
+        b.fork("c", ("user", 1))
