@@ -6,9 +6,10 @@
 // chunk is cut into pieces of W consecutive tokens: piece k is a request of its
 // own, W tokens behind P + k W positions on the same row of the block table, and
 // the kernels of drafted tokens (tree*.cu) compute it.  W * group is at most 256
-// rows, the largest row group, so no piece is read twice and the masked part of
-// one is at most W positions wide.  How many pieces a batch has is on the device;
-// n_seqs + n_tokens / W bound it, and those that are none have no tokens.
+// rows (W = 1 for larger groups), so the masked part of a piece is at most W
+// positions wide; its K and V are read once for each of its row groups, whose size
+// is the kernel's (128 rows at most with 32-bit queries).  How many pieces a batch has is on
+// the device; n_seqs + n_tokens / W bound it, and those that are none have no tokens.
 #include "tree.cuh"
 
 namespace bml {
@@ -24,10 +25,14 @@ constexpr uint32_t kPieceRows = 256;
 constexpr uint32_t kTf32Rows = 80;
 // Batches of so few tokens are a call of tree*.cu as they are, no request having more
 // than such a call takes: no pieces are made (32-bit queries: 3 us less), and with
-// 16-bit queries those kernels start sooner than chunk_umma.cu (bf16, d = 128, one
-// token behind 1000 positions 11.9 us, 15.3 there; 64 tokens 18.9 and 25.2; d = 64,
-// 8 of one token 9.6 and 16.0; one request of 128 tokens 24.7 and 28.2, d = 64 20.0 and 22.5; but 32 of one token 44.8 and 37.4, 3 of 80 tokens 31.7 and
-// 30.0, and 64 tokens of one among 64 idle requests 40.0 and 25.4).
+// 16-bit queries those kernels start sooner than chunk_umma.cu (behind 1000 positions,
+// bf16, d = 128: one token 11.9 us, 15.3 there; 64 tokens 18.9 and 25.2; one request of
+// 128 24.7 and 28.2; f16, d = 64: 8 of one token 9.6 and 16.0, one of 128 20.0 and 22.5).
+// The start that they save is the same behind any number of positions, and a tile of
+// 64 tokens costs more there: 8 of 64 tokens 48.2 and 34.7, 3 of 80 31.3 and 28.1, 64
+// tokens of one among 64 idle requests 37.3 and 26.0 (d = 64: 21.3 and 20.1).  For more than
+// 8 requests of a token each they would be the faster ones (32 of one: 28.2 and 38.4, d = 64
+// 16.0 and 22.6): tree_attention is the call for such a batch.
 constexpr uint32_t kFewTokens = 64, kFewSeqs = 8;
 
 struct PieceParams {

@@ -42,10 +42,15 @@
 //     only where that grew by more than 2^8 in either half (the result is exact for any
 //     fixed reference) takes them anew, from tensor memory, and rescales O.
 //
-// Measured on B200, d = 128, group 4: 2048 tokens behind 30,720 positions 870 us (1.22
-// PFLOP/s, at the power cap), 4 requests of 512 behind 4000 155 us (920 TFLOP/s; tensor
-// pipe 50% of active cycles, exponentials 51%: a chain's softmax and MMAs wait for each
-// other); d = 64, 300 tokens behind 700 21 us, most of it start and end.
+// Weights enter P.V rounded to the pages' 16-bit type, the only one that an MMA takes
+// beside such a V: half a step of each, at most eps / 2 of the sum of p |v|.  Their sum
+// stays f32 and takes them unrounded.
+//
+// Measured on B200, d = 128, group 4: 2048 tokens behind 30,720 positions 870 us alone
+// and 990 to 1010 in a loop, at the power cap (1.22 to 1.05 PFLOP/s); 4 requests of 512
+// behind 4000 155 us (920 TFLOP/s; tensor pipe 50% of active cycles, exponentials 51%: a
+// chain's softmax and MMAs wait for each other); d = 64, 300 tokens behind 700 21 us, most
+// of it start and end.
 #include <math.h>
 
 #include <type_traits>

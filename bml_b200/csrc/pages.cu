@@ -91,7 +91,8 @@ __device__ __forceinline__ void copy_cta(char *dst, const char *src, uint32_t by
 // Every CTA redoes the plan (a few loads a fork, one scan); cluster 0 keeps the
 // books, and all copy.  Memory-bound in the copies: 48 forks, 32 layers, rows of 2 KB
 // 81 us (6.2 TB/s; four CTAs an SM: 87 with one, 97 with two); 8 forks of one prompt 7 us,
-// launch and the plan's dependent loads.
+// launch and the plan's dependent loads; in a pool of 131,000 pages 12.8, whose counts one
+// cluster copies.
 // ---------------------------------------------------------------------------
 struct ForkOne {
     int32_t len;       // positions; -1: refused
@@ -393,7 +394,7 @@ __global__ void __launch_bounds__(kWideThreads) free_place_kernel(const __grid_c
 // moves need no order.  Tables and shared counts follow the pages, and the free
 // list becomes 0, 1, 2, ... with H taken.  The first kernel finds the moves, the
 // second makes them.  Memory-bound: 32 requests, 32 layers, pages of 131 KB 551 us (6.1
-// TB/s).
+// TB/s); 200 pages of 131,000 moved in one layer 76 us, the first kernel's five walks of the pool.
 // work: where[n_pages] (mark, then a page's new place), from[n_pages], to[n_pages],
 // the number of moves.
 // ---------------------------------------------------------------------------

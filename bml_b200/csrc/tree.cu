@@ -631,7 +631,7 @@ size_t tree_workspace_bytes(uint32_t D, int num_sms) {
 
 TreeForm tree_form(const TreeArgs &a) {
     // All but tree_f32_kernel scale masked scores after they were set to -inf, so a
-    // scale of 0 is its.  16-bit pages:  Up to 8 rows a kv head (on average): the
+    // scale of 0 is its.  16-bit pages: up to 8 rows a kv head (on average): the
     // form with positions as MMA rows (64 x 4000, d = 64, 8 rows: 49 us, 73 with
     // tree_warp.cu).  16-bit queries of more rows: tcgen05 where there is enough
     // work for its longer start (32 x 8000, d = 128: 24 rows 177 us against 217,
@@ -653,30 +653,6 @@ TreeForm tree_form(const TreeArgs &a) {
     // rows 13.8 us, 18.2 on tcgen05, 64 rows 19.0 and 19.4, 120 rows 25.8 and 21.2; of
     // 2000: 20 rows 18.8 and 24.8, 64 rows 29.7 and 26.1; d = 64, 700: 128 rows 12.3 and
     // 14.7, 240 rows 15.6 and 15.0; 2000: 64 rows 13.2 and 13.7, 128 rows 18.3 and 15.4.
-    // Rows count as TreeArgs::fits says: a caller that knows that most requests are
-    // idle, or one much wider than the others, does not get a form that reads the
-    // wide one's K and V for 8 rows at a time (1 of 131,008 positions and 64 nodes among
-    // 64 places, d = 128: 170 us, 1567 with tree_few.cu).  For 32-bit queries over 16-bit
-    // pages the forms differ little in a row's time and much in a request's, so the
-    // average decides (60 of one token and 4 of 64, 4000 positions: 618 us in row groups
-    // of 32, 917 of 64; the former one 1485 with groups of 64, 2204 with 8).
-    // 32-bit pages: row groups of 16 up to 16 rows (d = 128, 64 requests of 1000
-    // positions: 166 us, 247 on tcgen05; with 20 rows 391 against 247) and where they
-    // make little work for its longer start; one request of 700 positions, d = 128: 20
-    // rows 13.8 us, 18.2 on tcgen05, 64 rows 19.0 and 19.4, 120 rows 25.8 and 21.2; of
-    // 2000: 20 rows 18.8 and 24.8, 64 rows 29.7 and 26.1; d = 64, 700: 128 rows 12.3 and
-    // 14.7, 240 rows 15.6 and 15.0; 2000: 64 rows 13.2 and 13.7, 128 rows 18.3 and 15.4.
-    // Rows count as TreeArgs::fits says: a caller that knows that most requests are
-    // idle, or one much wider than the others, does not get a form that reads the
-    // wide one's K and V for 8 rows at a time (1 of 131,008 positions and 64 nodes among
-    // 64 places, d = 128: 170 us, 1567 with tree_few.cu).  For 32-bit queries over 16-bit
-    // pages the forms differ little in a row's time and much in a request's, so the
-    // average decides (60 of one token and 4 of 64, 4000 positions: 618 us in row groups
-    // of 32, 917 of 64; the former one 1485 with groups of 64, 2204 with 8).
-    // 32-bit pages, more than 16 rows: tcgen05, with d = 64 where there is work
-    // (d = 128: 64 requests of 1000 positions, 20 rows 247 us against 391, 1 of 700
-    // 19.5 against 17.4, 64 rows 20.7 against 22.1; with 16 rows 247 against 166.
-    // d = 64: 64 of 1000, 32 rows 180 against 212; 1 of 700 14.5 against 12.6).
     const bool little = a.most_tiles() <= 2ull * a.num_sms;
     if (a.p.scale_log2 > 0.f && a.kv_type != BML_F32) {
         if (a.fits(8)) return TreeForm::kFew;

@@ -24,8 +24,11 @@
 // its part of a row; the sums meet in distributed shared memory.  What bounds it:
 // latency for one request (launch, two dependent loads, a row pass: 8 picked nodes over
 // 32,001 tokens 7.3 us); for a batch over a large vocabulary its passes one after
-// another, 3 us each over 49 MB (48 requests, 2 to 32 drawn nodes, 128,000 f32 29 us; HBM
-// alone 7.5).
+// another.  48 requests, 2 to 32 drawn nodes, 128,000 f32, 29 us, by time stamps: lookups
+// 2.2, the first pass 8 (its 49 MB at 6.1 TB/s), one or two more of 5 to 7 out of L2, the
+// last one 4 to 6, the search in its piece 1.0 to 1.3, then the end.  bf16 rows 36 us: f64
+// sums of eight values a load do not fit 80 registers (376 bytes of spills), and the
+// search takes up to 6.5.
 #include <cooperative_groups.h>
 
 #include "pages.cuh"
@@ -160,8 +163,8 @@ __device__ __noinline__ double slow_pass(const Row<T, kDraft> &r, uint32_t k0, u
 }
 
 // Sum of vectors [k0, k1) by a warp; every lane gets it.  Instructions bound this (48
-// requests, 128,000 f32: 30 an element, with every value looked at, made a pass 8 us,
-// these 11 make it 3): the values are probabilities, so one OR of their bits says for
+// requests, 128,000 f32: 30 an element, with every value looked at, made the call 79 us,
+// these 11 make it 29): the values are probabilities, so one OR of their bits says for
 // many at once that none is negative, infinite or NaN; else all is summed again value
 // by value.  q is widened by integer operations beside the conversion unit, which
 // takes p.

@@ -426,8 +426,9 @@ def chunk_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     (row node_start[i] + j of q) attends over positions 0 to kv_lens[i] - T + j.
     Types, results, refused requests and rows behind the last request's are
     tree_attention's, and so are n_live and max_new.  workspace: an uint8 tensor of
-    chunk_workspace_size bytes for calls that must not allocate; calls that share
-    one must not overlap."""
+    chunk_workspace_size bytes (up to 158 MB from 1024 tokens on) for calls that must
+    not allocate; calls that share one must not overlap.  For batches of single
+    tokens tree_attention is the faster call (include/bml_attn.h has figures)."""
     if stream is None and out is None and workspace is None:
         r = (_fast or _load()).chunk(q, k_pool, v_pool, block_table, kv_lens, node_start, scale, n_live, max_new)
         if r is not None:
@@ -478,7 +479,9 @@ def verify_drafts(target: torch.Tensor, draft: torch.Tensor | None, tokens: torc
     probabilities behind each node; draft: those (of the same type) that each
     node's children were drawn from, independently, or None for tokens that were
     picked; tokens, parents int32 [n_tokens]; u [n_tokens] and u_next [n] f32:
-    random numbers in [0, 1).
+    random numbers in [0, 1).  Rows are distributions: where a draft row is none (it
+    sums to more than twice the target's) and nothing is left to draw from, the
+    next token is vocab - 1, which then means nothing.
 
     Returns path int32 [n, max_path] (-1 behind its end) and n_accept [n], as
     paged_commit takes them, and the next tokens int32 [n].  At a kept node its

@@ -543,11 +543,20 @@ bml_status bml_attn_chunk_workspace_size(uint32_t head_dim, uint32_t n_tokens,
  * requests that decode one token.  Token row t of request i (the j-th of its T,
  * j = t - node_start[i]) attends over the positions [0, kv_lens[i] - T + j].
  * Types, layouts, refused requests, masked places, infinities, precision and the
- * limit of waits are bml_attn_tree's; workspace: bml_attn_chunk_workspace_size
- * bytes, 16-byte aligned, no contents needed, not shared by calls that overlap
- * in time.  n_live, max_new: as bml_attn_tree_sized's n_live and max_nodes, 0 where
- * not known; the choice of a kernel goes by them.  Up to 256 tokens a request, where
- * most have few, bml_attn_tree_sized is the faster call.  head_dim 64 or 128.
+ * limit of waits are bml_attn_tree's (for values of normal distribution, results of
+ * 16-bit queries are off by 2.3e-3 of their norm with bf16 and 2.8e-4 with f16, where
+ * the rounding of the result alone makes 1.7e-3 and 2.1e-4: the weights' rounding
+ * makes the rest; of 32-bit queries by 6e-7).  workspace:
+ * bml_attn_chunk_workspace_size bytes, 16-byte aligned, no contents needed, not
+ * shared by calls that overlap in time; for batches of 1024 tokens and more four times
+ * bml_attn_tree's and a little (on a B200 158 MB with head_dim 128, 80 MB with 64),
+ * whatever the types, else once.  n_live, max_new: as bml_attn_tree_sized's n_live and
+ * max_nodes, 0 where not known; the choice of a kernel goes by them.
+ * bml_attn_tree_sized is the faster call for more than 8 requests of a token each
+ * (bf16, head_dim 128, 32 of them behind 1000 positions: 28 us and 38; behind 30,000:
+ * 582 and 612); from about 64 tokens a request on this one mostly is (8 of 64 behind
+ * 1000: 48 us and 35; 16 of 256: 176 and 126, but behind 8000 581 and 603; f32 queries
+ * over bf16 pages, 8 of 64 behind 8000: 758 and 417).  head_dim 64 or 128.
  * Asynchronous. */
 bml_status bml_attn_chunk(const void *q_dev, bml_dtype q_dtype,
                           uint32_t n_tokens, uint32_t n_heads,
@@ -584,8 +593,8 @@ bml_status bml_attn_chunk(const void *q_dev, bml_dtype q_dtype,
  * rejected x leaves p (S loses p(x), and it is neither kept nor drawn).  Where
  * nothing of positive weight is left, which rounding can do to 16-bit rows, next
  * is drawn from p itself; if p has nothing either, or q sums to more than twice p
- * (no distribution), it is vocab - 1.  Sums are f64.  A path of max_path nodes ends there, its last
- * node's children untried.  Probabilities that are not positive finite numbers
+ * (no distribution: nothing can be said of the token then), it is vocab - 1.  Sums are
+ * f64.  A path of max_path nodes ends there, its last node's children untried.  Probabilities that are not positive finite numbers
  * count as 0; a child whose token is outside [0, vocab) is never tried.  A request
  * without nodes, or with more than 256, has n_accept 0 and next -1.  A request
  * that bml_paged_plan refused is walked like any other, though its attention was
